@@ -32,6 +32,8 @@ from typing import Callable, Dict, List, Optional, Sequence
 
 import numpy as np
 
+from . import operators
+
 
 def size(shape: Sequence[int]) -> int:
     n = 1
@@ -184,6 +186,8 @@ def kernel(node, args: List[np.ndarray], graph) -> np.ndarray:
         body = node["attrs"]["body"]
         vals = evaluate(body, {f"a{k}": a for k, a in enumerate(args)})
         return vals[node["attrs"]["output"]]
+    if op in operators.KERNELS:
+        return operators.KERNELS[op](node, args, [nodes[i]["shape"] for i in node["inputs"]])
     raise ValueError(f"no kernel for '{op}'")
 
 

@@ -20,7 +20,7 @@
 //   forward-graph    (bundle) request {model, V?, B?, seed?, firstBatch?, params64?}: a model's forward pass, fused, with its inputs
 // GPU commands write a bundle (manifest.json + data.f32) under --out:
 //   gpu-direct       request {sabotage?}: every direct case, fused, canary-padded, on the GPU
-//   gpu-graphs       request {graphs: [{name, graph, inputs, keep, unfused?, perf?}]} fused (and unfused, and in the perf lowering) on the GPU
+//   gpu-graphs       request {graphs: [{name, graph, inputs, keep, unfused?, perf?, tuning?}]} fused (and unfused, and in the perf lowering) on the GPU
 //   gpu-fuzz         request {from, to, recompute?}: the reference's corpus programs, fused / perf / unfused, on the GPU
 //   gpu-configs      request {c3: [...], c4: [...], unfused} configs 3 and 4, kept outputs as oracle-computable slices
 //   gpu-workloads    request {ids?, families?, allNodes?}: the workload sweep's variants run once, outputs for the gate
@@ -263,6 +263,20 @@ function precompileGroup(group, arch, shard, shards) {
     }
     return precompile(lists, arch);
   }
+  if (group === 'operators') {
+    // The operators' GPU tests, in both lowerings, and the sizes they are measured at.
+    const { operatorGraph, CASES, MEASURED } = require('../src/testing/operator_cases');
+    let n = 0;
+    for (const [k, c] of CASES.concat(MEASURED).entries()) {
+      if (k % (shards || 1) !== (shard || 0)) continue;
+      const { graph, keep } = operatorGraph(c);
+      const f = fuse(graph, { keep });
+      const { tuning } = c;
+      const lists = [lowerMI355X(f.graph, { perf: true, keep: keep.map((id) => f.index.get(id)), tuning })];
+      n += precompile(MEASURED.includes(c) ? lists : lists.concat([lowerMI355X(f.graph, { tuning })]), arch);
+    }
+    return n;
+  }
   if (group === 'scratch') {
     // The no-allocation entry point's GPU test: split-K matmuls, one translation unit.
     return precompile(scratchLowerings(SCRATCH_SHAPES), arch);
@@ -374,7 +388,7 @@ async function gpuGraphs(req, dir) {
     const inputs = {};
     for (const n of g.inputs()) inputs[n.attrs.name] = Float32Array.from(c.inputs[n.attrs.name]);
     const f = fuse(g, { keep: c.keep || [], attention: !!c.attention });
-    const lf = lowerMI355X(f.graph);
+    const lf = lowerMI355X(f.graph, { tuning: c.tuning });
     const rf = await runner.run(f.graph, lf, inputs, { canary: true });
     const entry = { name: c.name, fused: f.graph.toJSON(), origin: f.origin, gpuFused: {}, canaryFused: rf.canaryIntact,
       kinds: lf.launches.map((l) => l.kind) };
@@ -382,7 +396,7 @@ async function gpuGraphs(req, dir) {
     if (c.perf) {
       // The perf lowering: transposes read in place by the matmuls, reshapes sharing buffers.
       const keepF = (c.keep || []).map((id) => f.index.get(id));
-      const lp = lowerMI355X(f.graph, { perf: true, keep: keepF });
+      const lp = lowerMI355X(f.graph, { perf: true, keep: keepF, tuning: c.tuning });
       const rp = await runner.run(f.graph, lp, inputs, { canary: true });
       entry.gpuPerf = {};
       for (const id of keepF) entry.gpuPerf[id] = bundle.put(rp.values[id]);
@@ -1243,6 +1257,67 @@ async function main() {
         return { workspace: l.workspace, params: Array.from(x.params),
           kernels: x.kernels.map((k) => ({ name: k.name, grid: k.grid, block: k.block, lds: k.lds })) };
       }) };
+      break;
+    }
+    case 'operator-graphs': {
+      // The operators' test graphs: the named cases, or one case given whole.
+      const { operatorGraph, CASES } = require('../src/testing/operator_cases');
+      const cases = req.cases || CASES.filter((c) => !req.family || c.family === req.family);
+      out = cases.map((c) => {
+        const { graph, keep, names } = operatorGraph(c);
+        const f = fuse(graph, { keep });
+        const at = keep.map((id) => f.index.get(id));
+        const lp = lowerMI355X(f.graph, { perf: true, keep: at, tuning: c.tuning });
+        return { name: c.name, case: c, graph: graph.toJSON(), keep, names, launches: lowerMI355X(f.graph).launches.map((l) => l.kind),
+          perf: lp.launches.map((l) => l.kind), batches: (lp.batches || []).map((b) => ({ count: b.count, joint: !!b.joint,
+            start: b.start, kernels: b.kernels.map((k) => k.name) })), workspace: lp.workspace };
+      });
+      break;
+    }
+    case 'operator-order': {
+      // Whether every launch of an operator's perf lowering, and of a joint launch as a whole, comes after its operands' writers.
+      const { operatorGraph } = require('../src/testing/operator_cases');
+      out = req.cases.map((c) => {
+        const { graph, keep } = operatorGraph(c);
+        const f = fuse(graph, { keep });
+        const lw = lowerMI355X(f.graph, { perf: true, keep: keep.map((id) => f.index.get(id)), tuning: c.tuning });
+        const alias = new Map(lw.aliases);
+        const owner = (id) => (alias.has(id) ? alias.get(id) : id);
+        const writers = new Set(lw.launches.map((l) => owner(l.node)));
+        const written = new Set();
+        const batchAt = new Map(lw.batches.map((b) => [b.start, b]));
+        let ok = true;
+        for (let i = 0; i < lw.launches.length;) {
+          const n = batchAt.has(i) ? batchAt.get(i).count : 1;
+          const members = lw.launches.slice(i, i + n);
+          for (const l of members) for (const id of l.inputs) if (writers.has(owner(id)) && !written.has(owner(id))) ok = false;
+          for (const l of members) written.add(owner(l.node));
+          i += n;
+        }
+        const all = lw.launches.reduce((q, l) => Math.max(q, l.workspace), 0);
+        return { name: c.name, ok: ok && written.size === writers.size && lw.workspace >= all };
+      });
+      break;
+    }
+    case 'operator-refusals': {
+      const { grad } = require('../src/autodiff');
+      const tries = {
+        targets: (g) => g.linearCrossEntropy(g.input('h', [4, 8]), g.input('W', [8, 5]), g.input('t', [5])),
+        inner: (g) => g.linearCrossEntropy(g.input('h', [4, 8]), g.input('W', [7, 5]), g.input('t', [4])),
+        rank: (g) => g.linearCrossEntropy(g.input('h', [2, 4, 8]), g.input('W', [8, 5]), g.input('t', [4])),
+        bias: (g) => g.linearCrossEntropy(g.input('h', [4, 8]), g.input('W', [8, 5]), g.input('t', [4]), g.input('b', [6])),
+        second: (g) => {
+          const h = g.input('h', [4, 8]);
+          const G = grad(g, [g.linearCrossEntropy(h, g.input('W', [8, 5]), g.input('t', [4]))], [h]);
+          return grad(G.graph, [G.grads[0]], [h], { prefix: 'e' });
+        },
+        orthogonalize: (g) => { const x = g.input('x', [4, 8]); return grad(g, [g.orthogonalize(x)], [x]); },
+        'unknown part': (g) => g.emit('linearCrossEntropyGrad', [g.input('h', [4, 8]), g.input('W', [8, 5]), g.input('t', [4]), g.input('d', [4])], { part: 'dt' }),
+      };
+      out = {};
+      for (const k of Object.keys(tries)) {
+        try { tries[k](new Graph()); } catch (e) { out[k] = e.message; }
+      }
       break;
     }
     case 'kernel-unit': {

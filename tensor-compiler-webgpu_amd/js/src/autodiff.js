@@ -97,6 +97,20 @@ const RULES = {
   broadcast: (B, n, g) => [unbroadcast(B, g, B.shape(n.inputs[0]), n.shape)],
   reshape: (B, n, g) => [B.reshape(g, B.shape(n.inputs[0]))],
   transpose: (B, n, g) => [B.transpose(g, inversePermutation(n.attrs.perm))],
+  // The operators of ir/operators.js: a gradient node for each operand that has one.
+  // Positions and targets have none.
+  rotary: (B, n, g) => {
+    const part = (p) => B.emit('rotaryGrad', n.inputs.concat([g]), Object.assign({}, n.attrs, { part: p }));
+    return n.inputs.length === 3 ? [part('dx'), null, part('dgain')] : [part('dx'), null];
+  },
+  linearCrossEntropy: (B, n, g) => {
+    const part = (p) => B.emit('linearCrossEntropyGrad', n.inputs.concat([g]), { part: p });
+    const shares = [part('dh'), part('dW'), null];
+    return n.inputs.length === 4 ? shares.concat([part('dbias')]) : shares;
+  },
+  orthogonalize: () => {
+    throw new GradientError('orthogonalize is not differentiable here: it is an optimizer\'s operator, applied to finished gradients');
+  },
   step: () => [null],
   stopGradient: () => [null],
   max: () => {

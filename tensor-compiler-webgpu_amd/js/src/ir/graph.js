@@ -9,6 +9,7 @@
 // as the reference's (pinned against its golden/cases.json), so the reference's
 // own graphs and this host's are interchangeable at the backend's boundary.
 
+const { rotaryPairs } = require('./operators');
 const { inferShape, broadcastShapes, normAxis, sameShape, size, fmt, ShapeError } = require('./shapes');
 
 /** Deep copy of plain attribute data (numbers, strings, booleans, arrays, objects). */
@@ -136,6 +137,38 @@ class Graph {
     perm[rank - 2] = rank - 1;
     perm[rank - 1] = rank - 2;
     return this.transpose(x, perm);
+  }
+
+  // ---- operators (operators.js) --------------------------------------------------
+
+  /**
+   * x [..., dh] rotated by its tokens' positions, its rows normalised first where `gain`
+   * [dh] is given (eps: 1e-5). Options: axis (the tokens' axis, default the third last),
+   * sections, base, restart or frequencies, axes (operators.js rotaryPairs), positionAxes
+   * (default: the sections', or 1 + the largest of axes), pairs ('halves' or 'adjacent').
+   * positions: [T] or [x's first axis, T], and a last axis of positionAxes where there are several.
+   */
+  rotary(x, positions, options) {
+    const o = options || {};
+    const shape = this.shape(x);
+    const { frequencies, axes, count } = rotaryPairs(shape[shape.length - 1], o);
+    const attrs = { axis: normAxis(o.axis !== undefined ? o.axis : shape.length < 3 ? 0 : -3, shape.length, 'rotary'), pairs: o.pairs || 'halves',
+      positionAxes: o.positionAxes || count || axes.reduce((m, a) => Math.max(m, a + 1), 1), frequencies, axes };
+    const gained = o.gain !== undefined && o.gain !== null;
+    if (gained) attrs.eps = o.eps === undefined ? 1e-5 : o.eps;
+    return this.emit('rotary', gained ? [x, positions, o.gain] : [x, positions], attrs);
+  }
+
+  /** Row losses [N] of softmax cross entropy: logits h [N, d] · W [d, V] (+ bias [V]), class indices targets [N]. */
+  linearCrossEntropy(h, W, targets, bias) {
+    return this.emit('linearCrossEntropy', bias === undefined || bias === null ? [h, W, targets] : [h, W, targets, bias], {});
+  }
+
+  /** Each matrix of x's last two axes with its singular values pushed towards 1 by Newton-Schulz steps. */
+  orthogonalize(x, options) {
+    const o = options || {};
+    return this.emit('orthogonalize', [x], { steps: o.steps === undefined ? 5 : o.steps,
+      coefficients: (o.coefficients || [3.4445, -4.7750, 2.0315]).slice(), eps: o.eps === undefined ? 1e-7 : o.eps });
   }
 
   // ---- composites ---------------------------------------------------------------

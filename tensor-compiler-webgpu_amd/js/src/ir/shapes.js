@@ -7,6 +7,8 @@
 // :29-39), since graphs must be interchangeable with its builder's; the reference's
 // module needs Node >= 24, so the host side of this backend carries its own.
 
+const { operatorRules } = require('./operators');
+
 class ShapeError extends Error {
   constructor(message) { super(message); this.name = 'ShapeError'; }
 }
@@ -161,11 +163,16 @@ for (const op of REDUCE) {
   };
 }
 
+Object.assign(SHAPE_RULES, operatorRules(ShapeError, fmt));
+
 /** The result shape of `op` on inputs of `shapes`, or a thrown ShapeError (the rules of shapes.js:55-116). */
 function inferShape(op, shapes, attrs) {
   const r = SHAPE_RULES[op];
   if (!r) throw new ShapeError(`'${op}' is not an op of this IR`);
-  if (shapes.length !== r.arity) throw new ShapeError(`${op} takes ${r.arity} operand(s), was given ${shapes.length}`);
+  const [least, most] = Array.isArray(r.arity) ? r.arity : [r.arity, r.arity];
+  if (shapes.length < least || shapes.length > most) {
+    throw new ShapeError(`${op} takes ${least === most ? least : `${least} to ${most}`} operand(s), was given ${shapes.length}`);
+  }
   return r.rule(shapes, attrs || {}, op);
 }
 

@@ -1592,7 +1592,7 @@ const MAX_BATCH = 32;
 // Kernel families generated here: each reads its launch only through A.in /
 // A.out / A.ws, and its z index only in its own text (the headers never read
 // blockIdx.z or gridDim.z). `_red`: a split-K matmul's second kernel.
-const BATCHABLE = /^(tcmi_(ew|row|mm|mmred|colred|colfin|attn)_[0-9a-f]+)(_red)?$/;
+const BATCHABLE = /^(tcmi_(ew|row|mm|mmred|colred|colfin|attn|rot|orth[a-z]+)_[0-9a-f]+)(_red)?$/;
 const MAX_GRID_Z = 65535;
 
 /** Whether kernel `k` may run as a member of a batched launch of `count` members. */
@@ -1889,7 +1889,7 @@ ${branches.join('\n')}
   return { name: b.name, source: b.source, grid: [at, 1, 1], block: [threads, 1, 1], lds: 0, members: ks.length, ragged: ks.map((k) => k.name) };
 }
 
-module.exports = { elementwiseKernel, rowwiseKernel, colreduceKernels, gemmKernel, gemmTiling, attentionKernel, attentionGradKernel,
+module.exports = { kernelText, elementwiseKernel, rowwiseKernel, colreduceKernels, gemmKernel, gemmTiling, attentionKernel, attentionGradKernel,
   gradPart, GRAD_PARTS, classifyGather, gatherStrides,
   literal, keyText, fnv, Emitter, ParamOverflow, WG, MAX_P, MAX_IN, MAX_BATCH, batchable, batchedKernel, batchFamily,
   mergedKernel, mergeFamily, wideRows, raggable, raggedFits, raggedKernel, textLds, RAGGED_MAX_BLOCKS, RAGGED_MAX_LDS, COLRED_ONE_PASS };

@@ -48,6 +48,7 @@ const { Graph } = require('../ir/graph');
 const { size } = require('../ir/shapes');
 const { bodyOf } = require('../fusion/fuse');
 const cg = require('./codegen');
+const { OPERATORS, lowerOperator } = require('./operators');
 
 const isReduce = (n) => n.op === 'sum' || n.op === 'max';
 const ELEMENTWISE_OPS = new Set(['add', 'sub', 'mul', 'div', 'neg', 'exp', 'log', 'relu', 'tanh', 'sqrt', 'step', 'stopGradient']);
@@ -302,6 +303,7 @@ function lowerNode(graph, node, opts, mmViews, folds, rowFold, lastReads, peers,
     const { body, output } = oneOpBody(graph, node);
     return Object.assign({ kind: 'matmul' }, single(cg.gemmKernel(body, output, Object.assign({ tuning: (opts.tuning || {}).gemm, peers }, mmViews))));
   }
+  if (OPERATORS.has(node.op)) return lowerOperator(graph, node, opts.tuning);
   throw new Error(`no MI355X lowering for '${node.op}'`);
 }
 
@@ -1249,7 +1251,7 @@ function lowerOnce(graph, opts, noAbsorb, noForm) {
     const b = batchPlan(launches, plan.aliases, (id) => 4 * size(graph.nodes[id].shape));
     out.launches = b.launches;
     out.batches = b.batches;
-    for (const x of b.batches) out.workspace = Math.max(out.workspace, x.count * x.wsStride);
+    for (const x of b.batches) out.workspace = Math.max(out.workspace, x.count * x.wsStride, x.workspace || 0);
   }
   return out;
 }
@@ -1286,6 +1288,7 @@ function lowerOnce(graph, opts, noAbsorb, noForm) {
  */
 function batchPlan(launches, aliases, bytesOf) {
   const owner = (id) => (aliases.has(id) ? aliases.get(id) : id);
+  launches = besideGradients(launches, owner);
   const n = launches.length;
   const writer = new Map();
   launches.forEach((l, i) => writer.set(owner(l.node), i));
@@ -1331,23 +1334,31 @@ function batchPlan(launches, aliases, bytesOf) {
   // An attention gradient's three parts (the same operands, none reading another) run as
   // one launch of their joint kernel, members in the order dQ, dK, dV, where the first
   // of them stood.
-  const jointOf = (l) => l.kernels.length === 1 && l.kernels[0].joint ? l.kernels[0].joint.name : null;
+  // So do the parts of one operator's gradient that the list holds, two or more (operators.js joint).
+  const jointOf = (l) => (l.kernels[0].joint ? l.kernels[0].joint.name : null);
   for (let i = 0; i < n; i++) {
     if (placed[i]) continue;
     const jn = jointOf(launches[i]);
     if (jn) {
+      const { operands } = launches[i].kernels[0].joint;
+      const same = (l) => l.inputs.slice(0, operands).join() === launches[i].inputs.slice(0, operands).join();
       const parts = new Map();
+      let rest = null;        // the operands that some of the parts read besides
       for (let j = i; j < n; j++) {
         const l = launches[j];
-        if (!placed[j] && jointOf(l) === jn && l.inputs.join() === launches[i].inputs.join() && !parts.has(l.kernels[0].part)) {
-          parts.set(l.kernels[0].part, j);
-        }
+        if (placed[j] || jointOf(l) !== jn || !same(l) || parts.has(l.kernels[0].part)) continue;
+        const more = operands === undefined ? '' : l.inputs.slice(operands).join();
+        if (!ready(l) || (more && rest && rest !== more)) continue;
+        if (more) rest = more;
+        parts.set(l.kernels[0].part, j);
       }
-      const order = launches[i].kernels[0].joint.parts;
-      if (order.every((p) => parts.has(p))) {
+      const { parts: all, order: any, build } = launches[i].kernels[0].joint;
+      const order = all || any.filter((p) => parts.has(p));
+      if (order.length > 1 && order.every((p) => parts.has(p))) {
         const group = order.map((p) => parts.get(p));
         const unit = group.map((j) => launches[j]);
-        unit.joint = launches[i].kernels[0].joint;
+        unit.joint = build ? build(order) : launches[i].kernels[0].joint;
+        if (build) for (const l of unit) l.joined = true;
         for (const j of group) placed[j] = 1;
         units.push(unit);
         continue;
@@ -1447,8 +1458,8 @@ function batchPlan(launches, aliases, bytesOf) {
   for (const u of units) {
     if (u.joint) {
       const j = u.joint;
-      batches.push({ start: order.length, count: u.length, kernels: [{ name: j.name, source: j.source, grid: j.grid, block: j.block, lds: j.lds }],
-        wsStride: 0, joint: true });
+      batches.push({ start: order.length, count: u.length, kernels: j.kernels || [{ name: j.name, source: j.source, grid: j.grid, block: j.block, lds: j.lds }],
+        wsStride: 0, joint: true, workspace: j.workspace || 0 });
       order.push(...u);
       continue;
     }
@@ -1468,6 +1479,37 @@ function batchPlan(launches, aliases, bytesOf) {
 }
 
 /**
+ * The launch list with each part that comes before the other parts of its joint launch (an operator's forward value:
+ * the losses of linearCrossEntropy, whose gradients read the cotangent that comes after them) moved
+ * to the first of those, and the launches that depend on it behind the last; as it was where a gradient
+ * depends on the value.
+ */
+function besideGradients(launches, owner) {
+  let list = launches;
+  for (const first of launches) {
+    const j = first.kernels[0].joint;
+    if (!j || j.operands === undefined || first.inputs.length !== j.operands) continue;
+    const at = list.indexOf(first);
+    const twin = (l) => l !== first && l.kernels[0].joint && l.kernels[0].joint.name === j.name && l.inputs.length > j.operands
+      && l.inputs.slice(0, j.operands).join() === first.inputs.join();
+    const twins = list.filter((l, i) => i > at && twin(l));
+    if (!twins.length) continue;
+    const last = list.indexOf(twins[twins.length - 1]);
+    const after = new Set([owner(first.node)]), moved = [], stay = [];
+    for (const l of list.slice(at + 1, last + 1)) {
+      if (l.inputs.some((id) => after.has(owner(id)))) {
+        after.add(owner(l.node));
+        moved.push(l);
+      } else stay.push(l);
+    }
+    if (moved.some((l) => twins.includes(l))) continue;
+    stay.splice(stay.indexOf(twins[0]), 0, first);
+    list = list.slice(0, at).concat(stay, moved, list.slice(last + 1));
+  }
+  return list;
+}
+
+/**
  * Algorithmic bytes of a lowering as it runs: every launch's unique operands and output once, and
  * an operand that several members of a merged batch read, which their kernel loads once, once.
  */
@@ -1479,10 +1521,13 @@ function movedBytes(lowered) {
   return bytes;
 }
 
-/** Every distinct kernel source of a launch list (its batched kernels included), in first-use order. */
-function kernelSources(lowered) {
+/**
+ * Every distinct kernel source of a launch list (its batched kernels included), in first-use
+ * order; with `apart`, those of an operator's parts that run as one launch too.
+ */
+function kernelSources(lowered, apart) {
   const seen = new Map();
-  for (const l of lowered.launches) for (const k of l.kernels) if (!seen.has(k.name)) seen.set(k.name, k.source);
+  for (const l of lowered.launches) if (apart || !l.joined) for (const k of l.kernels) if (!seen.has(k.name)) seen.set(k.name, k.source);
   for (const b of lowered.batches || []) for (const k of b.kernels) if (!seen.has(k.name)) seen.set(k.name, k.source);
   return seen;
 }

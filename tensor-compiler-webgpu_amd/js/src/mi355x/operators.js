@@ -1,0 +1,293 @@
+'use strict';
+// Launches of the operators that are one node each (ir/operators.js): the kernels of
+// tcmi_rotary.h, tcmi_loss.h and tcmi_orthogonalize.h, their sizes written as constants of
+// each text, and the workspace they share between the kernels of one launch.
+//
+// A gradient's parts (`dx`, `dgain`; `dh`, `dW`, `dbias`, and with them the losses) are nodes
+// of their own and lower to launches of their own. The perf lowering runs the parts that
+// it keeps as one launch (lower.js batchPlan): `joint` on a part's first kernel names the
+// node's parts and forms the kernels of any set of them. Every part is computed by the same code in either form.
+
+const { size } = require('../ir/shapes');
+const { singularBound } = require('../ir/operators');
+const { kernelText } = require('./codegen');
+
+const ceil = (a, b) => Math.ceil(a / b);
+const OPERATORS = new Set(['rotary', 'rotaryGrad', 'linearCrossEntropy', 'linearCrossEntropyGrad', 'orthogonalize']);
+
+/** A double as a C++ literal that reads back as itself. */
+function double(v) {
+  const t = String(v);
+  return /[.e]/.test(t) ? t : `${t}.0`;
+}
+
+/** One kernel record. */
+function kernel(kind, text, grid, threads, more) {
+  const k = kernelText(kind, text);
+  return Object.assign({ name: k.name, source: k.source, grid, block: [threads, 1, 1], lds: 0 }, more || {});
+}
+
+/**
+ * How a kernel's text reaches its launch: alone, `A` (TcmiArgs) with the part's output in
+ * A.out; as one of `parts` in a joint launch, member k of its argument block for the k-th part, the
+ * operands and the workspace in member 0's.
+ */
+function entry(parts) {
+  return parts ? { sig: `const TcmiBatch<${parts.length}> B`, open: '  const TcmiPtrs& A = B.m[0];\n', out: (part) => `B.m[${parts.indexOf(part)}].out` }
+    : { sig: 'const TcmiArgs A', open: '', out: () => 'A.out' };
+}
+
+// ---- rotary -------------------------------------------------------------------------------
+
+const ROTARY_THREADS = 256;
+const ROTARY_HEAD = 4096;       // floats of a head at most: 32 pairs a lane
+
+function rotarySizes(graph, node) {
+  const x = graph.nodes[node.inputs[0]].shape, pos = graph.nodes[node.inputs[1]].shape, a = node.attrs;
+  const DH = x[x.length - 1], R = a.frequencies.length, T = x[a.axis];
+  if (DH > ROTARY_HEAD) throw new Error(`rotary: heads of ${DH} floats (at most ${ROTARY_HEAD})`);
+  const B = a.axis > 0 ? x[0] : 1, M1 = size(x.slice(1, Math.max(1, a.axis))), M2 = size(x.slice(a.axis + 1, -1));
+  if (B * T >= 2 ** 32 || M1 * M2 >= 2 ** 32) throw new Error('rotary: tokens and heads are counted in 32 bits');
+  const axes = a.positionAxes;
+  const shared = size(pos) === T * axes && B > 1;
+  // 128-bit loads where a group of four pairs (and of four floats that are not rotated) is whole and aligned.
+  const E = DH % 4 === 0 && R % 4 === 0 ? 4 : 1;
+  const groups = Math.max(R, DH - 2 * R) / E;
+  let lanes = 1;
+  while (lanes < 64 && lanes < groups) lanes *= 2;
+  const slots = (() => { let s = 1; while (2 * s <= Math.min(M1 * M2, ROTARY_THREADS / lanes)) s *= 2; return s; })();
+  return { DH, R, B, M1, T, M2, axes, shared, E, lanes, units: ceil(R / E, lanes), tails: ceil((DH - 2 * R) / E, lanes), slots };
+}
+
+function rotaryText(z, attrs, gain, grads, parts) {
+  const e = entry(parts);
+  const dx = grads.includes('dx'), dgain = grads.includes('dgain');
+  const table = z.R ? `  static __device__ __forceinline__ double turns(int j) {
+    static constexpr double t[${z.R}] = {${attrs.frequencies.map((f) => double(f / (2 * Math.PI))).join(', ')}};
+    return t[j];
+  }
+  static __device__ __forceinline__ uint32_t axis(int j) {
+    static constexpr unsigned char t[${z.R}] = {${attrs.axes.join(', ')}};
+    return t[j];
+  }` : `  static __device__ __forceinline__ double turns(int) { return 0.0; }
+  static __device__ __forceinline__ uint32_t axis(int) { return 0u; }`;
+  const last = gain ? 3 : 2;
+  return `#include "tcmi_rotary.h"
+struct __KERNEL___s {
+  static constexpr int DH = ${z.DH}, R = ${z.R}, E = ${z.E}, LANES = ${z.lanes}, UNITS = ${z.units}, TAILS = ${z.tails}, THREADS = ${ROTARY_THREADS};
+  static constexpr bool ADJ = ${attrs.pairs === 'adjacent'}, GAIN = ${gain}, DX = ${dx}, DGAIN = ${dgain}, SHARED = ${z.shared};
+  static constexpr uint32_t B = ${z.B}u, M1 = ${z.M1}u, T = ${z.T}u, M2 = ${z.M2}u, AXES = ${z.axes}u, SLOTS = ${z.slots}u;
+  static __device__ __forceinline__ float eps() { return static_cast<float>(${double(gain ? attrs.eps : 0)}); }
+${table}
+};
+extern "C" __global__ void __launch_bounds__(${ROTARY_THREADS}) __KERNEL__(${e.sig}) {
+${e.open}${dgain ? `  __shared__ __attribute__((aligned(16))) float scratch[${ROTARY_THREADS / z.lanes * z.DH}];\n` : ''}  tcmi::rotary<__KERNEL___s>(A.in[0], A.in[1], ${gain ? 'A.in[2]' : 'nullptr'}, ${grads.length ? `A.in[${last}]` : 'nullptr'}, ${
+  dx || !grads.length ? e.out('dx') : 'nullptr'}, ${dgain ? 'A.ws, scratch' : 'nullptr, nullptr'}, blockIdx.x, gridDim.x);
+}
+`;
+}
+
+function rotaryKernels(z, attrs, gain, grads, parts) {
+  // A few tokens to a workgroup. The gradient of the gain walks them in at most 1024 workgroups, whose sums are then added.
+  const perBlock = ROTARY_THREADS / z.lanes / z.slots;
+  const want = ceil(z.B * z.T, perBlock);
+  const blocks = Math.min(want, grads.includes('dgain') ? 1024 : 65536);
+  const kernels = [kernel('rot', rotaryText(z, attrs, gain, grads, parts), [blocks, 1, 1], ROTARY_THREADS)];
+  let workspace = 0;
+  if (grads.includes('dgain')) {
+    const e = entry(parts);
+    workspace = blocks * z.DH * 4;
+    kernels.push(kernel('rotsum', `#include "tcmi_rotary.h"
+extern "C" __global__ void __launch_bounds__(256) __KERNEL__(${e.sig}) {
+${e.open}  __shared__ float scratch[256];
+  tcmi::rotary_gain_sum<${z.DH}>(A.ws, ${e.out('dgain')}, ${blocks}u, scratch, blockIdx.x);
+}
+`, [ceil(z.DH, 16), 1, 1], 256));
+  }
+  return { kernels, workspace };
+}
+
+function lowerRotary(graph, node) {
+  const grad = node.op === 'rotaryGrad';
+  const gain = node.inputs.length - (grad ? 1 : 0) === 3;
+  const z = rotarySizes(graph, node);
+  const k = rotaryKernels(z, node.attrs, gain, grad ? [node.attrs.part] : [], null);
+  if (grad && gain) {
+    const { part, ...rest } = node.attrs;
+    joint(k.kernels[0], part, ['dx', 'dgain'], ['rotary', rest, z], (parts) => rotaryKernels(z, node.attrs, gain, parts, parts));
+  }
+  return { kind: grad ? 'rotary-grad' : 'rotary', kernels: k.kernels, workspace: k.workspace };
+}
+
+// ---- linearCrossEntropy --------------------------------------------------------------------
+
+const LOSS_PIECE = 1 << 28;      // bytes of a piece's logits at most (a piece is 128 rows or more)
+const LOSS_PARTS = ['dh', 'dW', 'dbias', 'loss'];
+const CUS = 256;
+
+const align = (n, to) => ceil(n, to) * to;
+
+/** The sizes of a loss's launch forming `parts`, and its workspace's layout. */
+function lossSizes(N, D, V, bias, parts, piece) {
+  const grad = parts.some((p) => p !== 'loss');
+  const DP = align(D, 128), VP = align(V, 128);
+  // The rows of a piece: its logits, or without gradients a row's pair of statistics for each 64 columns.
+  const row = grad ? 4 * VP : VP / 8;
+  const most = Math.max(128, Math.floor((piece || LOSS_PIECE) / row / 128) * 128);
+  const PIECES = ceil(align(N, 128), most), NP = align(ceil(N, PIECES), 128);
+  const RB = NP * VP >= 2 ** 20 ? 32 : 16;
+  // K split over workgroups until two a CU have a tile; no chunk under 16 slices of 32.
+  const split = (tiles, slices) => {
+    const want = Math.max(1, Math.min(ceil(2 * CUS, tiles), Math.floor(slices / 16), 64));
+    const each = ceil(slices, want);
+    return { chunks: ceil(slices, each), each };
+  };
+  const hs = split(NP / 128 * (DP / 128), VP / 32), wsp = split(DP / 128 * (VP / 128), NP / 32);
+  const z = { N, D, V, DP, VP, NP, PIECES, RB, BIAS: bias, BLOCKS: 256, VECD: D % 4 === 0, VECV: V % 4 === 0,
+    HCHUNKS: hs.chunks, HK: hs.each, WCHUNKS: wsp.chunks, WK: wsp.each };
+  let at = 0;
+  const place = (name, bytes) => { z[name] = at; at = align(at + bytes, 256); };
+  place('STATE', 256);
+  place('MAXIMA', (2 * z.BLOCKS + 1) * 4);
+  place('HP', 4 * NP * PIECES * DP);
+  place('WP', 4 * DP * VP);
+  place('STATS', 8 * NP * (VP / 64));
+  place('PICKED', 4 * NP);
+  place('ROWS', 8 * NP);
+  if (grad) place('Z', 4 * NP * VP); else z.Z = 0;
+  if (parts.includes('dh') || parts.includes('dW')) place('GP', 4 * NP * VP); else z.GP = 0;
+  if (parts.includes('dbias')) place('SUMS', 4 * NP / RB * VP); else z.SUMS = 0;
+  if (parts.includes('dh') && hs.chunks > 1) place('HPART', 4 * hs.chunks * NP * DP); else z.HPART = 0;
+  if (parts.includes('dW') && wsp.chunks > 1) place('WPART', 4 * wsp.chunks * DP * VP); else z.WPART = 0;
+  return { z, workspace: at, grad };
+}
+
+function lossKernels(N, D, V, bias, parts, joined, bytes) {
+  const { z, workspace, grad } = lossSizes(N, D, V, bias, parts, bytes);
+  const e = entry(joined ? parts : null);
+  const has = (p) => parts.includes(p);
+  const sizes = Object.keys(z).map((k) => (typeof z[k] === 'boolean' ? `  static constexpr bool ${k} = ${z[k]};`
+    : `  static constexpr ${['N', 'D', 'V', 'DP', 'VP', 'NP', 'PIECES', 'RB', 'BLOCKS', 'HCHUNKS', 'HK', 'WCHUNKS', 'WK'].includes(k) ? 'uint32_t' : 'size_t'} ${k} = ${z[k]}${'u'};`)).join('\n');
+  const make = (kind, grid, threads, lds, call, least) => kernel(kind, `#include "tcmi_loss.h"
+struct __KERNEL___s {
+${sizes}
+};
+extern "C" __global__ void __launch_bounds__(${threads}${least ? `, ${least}` : ''}) __KERNEL__(${e.sig}) {
+${e.open}  const tcmi::Loss<__KERNEL___s> L{A.in[0], A.in[1], A.in[2], ${bias ? 'A.in[3]' : 'nullptr'}, ${grad ? `A.in[${bias ? 4 : 3}]` : 'nullptr'}, reinterpret_cast<char*>(A.ws)};
+${lds ? `  __shared__ __attribute__((aligned(1024))) ${lds};\n` : ''}  tcmi::${call};
+}
+`, grid, threads);
+  const pool = 'char lds[tcmi::f16x2_lds<128, 128>()]';
+  const S = '__KERNEL___s';
+  const HG = z.NP * z.PIECES * z.DP / 4, WG = z.DP * z.VP / 4;
+  const once = [make('lossmax', [2 * z.BLOCKS + (grad ? 1 : 0), 1, 1], 256, 'float scratch[4]', `loss_maxima<${S}, ${grad}>(L, scratch, blockIdx.x)`),
+    make('losssplit', [ceil(HG, 4096) + ceil(WG, 4096), 1, 1], 256, 'float scratch[4]', `loss_split<${S}, ${grad}>(L, scratch, blockIdx.x)`)];
+  const piece = [make('losslogits', [z.NP / 128 * (z.VP / 128), 1, 1], 256, pool, `loss_logits<${S}, ${grad}>(L, lds, blockIdx.x)`, 2),
+    make('lossjoin', [z.NP / 16, 1, 1], 256, 'float2 scratch[256]', `loss_join<${S}, ${has('loss')}, ${!grad}>(L, ${has('loss') ? e.out('loss') : 'nullptr'}, scratch, blockIdx.x)`)];
+  if (grad) {
+    piece.push(make('lossspread', [ceil(z.VP, 1024), z.NP / z.RB, 1], 256, `tcmi::f4 rows[${z.RB}]`,
+      `loss_spread<${S}, ${has('dh') || has('dW')}, ${has('dbias')}>(L, rows, blockIdx.x, blockIdx.y)`));
+    if (has('dh')) {
+      piece.push(make('lossdh', [z.NP / 128 * (z.DP / 128) * z.HCHUNKS, 1, 1], 256, pool, `loss_dh<${S}>(L, ${e.out('dh')}, lds, blockIdx.x)`, 2));
+      if (z.HCHUNKS > 1) piece.push(make('lossdhsum', [ceil(z.NP * z.DP / 4, 256), 1, 1], 256, null, `loss_dh_sum<${S}>(L, ${e.out('dh')}, blockIdx.x)`));
+    }
+    if (has('dW')) {
+      piece.push(make('lossdw', [z.DP / 128 * (z.VP / 128) * z.WCHUNKS, 1, 1], 256, pool, `loss_dw<${S}>(L, ${e.out('dW')}, lds, blockIdx.x)`, 2));
+      if (z.WCHUNKS > 1) piece.push(make('lossdwsum', [ceil(z.D * z.VP / 4, 256), 1, 1], 256, null, `loss_dw_sum<${S}>(L, ${e.out('dW')}, blockIdx.x)`));
+    }
+    piece.push(make('lossend', [has('dbias') ? z.VP / 16 : 1, 1, 1], 256, has('dbias') ? 'float scratch[256]' : null,
+      `loss_end<${S}, ${has('dbias')}>(L, ${has('dbias') ? `${e.out('dbias')}, scratch` : 'nullptr, nullptr'}, blockIdx.x)`));
+  }
+  const kernels = once.slice();
+  for (let p = 0; p < z.PIECES; p++) kernels.push(...piece);
+  return { kernels, workspace };
+}
+
+function lowerLoss(graph, node, tuning) {
+  const { piece } = (tuning || {}).loss || {};
+  const grad = node.op === 'linearCrossEntropyGrad';
+  const [N, D] = graph.nodes[node.inputs[0]].shape, V = graph.nodes[node.inputs[1]].shape[1];
+  const operands = node.inputs.length - (grad ? 1 : 0);
+  const bias = operands === 4;
+  const part = grad ? node.attrs.part : 'loss';
+  const k = lossKernels(N, D, V, bias, [part], false, piece);
+  joint(k.kernels[0], part, LOSS_PARTS, ['loss', N, D, V, bias], (parts) => lossKernels(N, D, V, bias, parts, true, piece), operands);
+  return { kind: grad ? 'linear-cross-entropy-grad' : 'linear-cross-entropy', kernels: k.kernels, workspace: k.workspace,
+    flops: part === 'dbias' ? 0 : 2 * N * D * V };
+}
+
+// ---- orthogonalize -------------------------------------------------------------------------
+
+/** The largest exponent that keeps values up to `top` within half's range. */
+const fits = (top) => Math.floor(Math.log2(60000 / top));
+
+function lowerOrthogonalize(graph, node) {
+  const x = node.shape, M = x[x.length - 2], N = x[x.length - 1], count = size(x.slice(0, -2));
+  const { steps, eps, coefficients: [a, b, c] } = node.attrs;
+  if (count > 65535) throw new Error(`orthogonalize: ${count} matrices (at most 65535)`);
+  const tall = M > N, s = Math.min(M, N), l = Math.max(M, N);
+  // Tiles of 128, or of 64 where those leave much of the chip idle.
+  const tiles = (t) => ceil(s, t) * ceil(l, t) * count;
+  const T = tiles(128) >= 2 * CUS ? 4 : 2;
+  const pad = 32 * T, MP = align(M, pad), NP = align(N, pad), SP = Math.min(MP, NP);
+  const top = singularBound(node.attrs);
+  const z = { M, N, MP, NP, SP, TALL: tall, VEC: N % 4 === 0, BLOCKS: Math.min(256, ceil(M * N, 4096)),
+    SX: fits(top), SA: fits(top ** 2), SB: Math.max(-60, Math.min(60, fits(Math.max(Math.abs(b) * top ** 2 + Math.abs(c) * top ** 4, 2 ** -40)))) };
+  let at = 0;
+  const place = (name, bytes) => { z[name] = at; at = align(at + bytes, 256); };
+  place('NORM', 8 * z.BLOCKS);
+  place('X0', steps > 0 ? 4 * MP * NP : 0);
+  place('X1', steps > 1 ? 4 * MP * NP : 0);
+  place('A', steps > 0 ? 4 * SP * SP : 0);
+  place('B', steps > 0 ? 4 * SP * SP : 0);
+  z.PER = at;
+  const sizes = Object.keys(z).map((k) => (typeof z[k] === 'boolean' ? `  static constexpr bool ${k} = ${z[k]};`
+    : ['SX', 'SA', 'SB'].includes(k) ? `  static constexpr int ${k} = ${z[k]};`
+      : `  static constexpr ${['M', 'N', 'MP', 'NP', 'SP', 'BLOCKS'].includes(k) ? 'uint32_t' : 'size_t'} ${k} = ${z[k]}u;`)).join('\n');
+  const S = '__KERNEL___s';
+  const make = (kind, blocks, lds, call) => kernel(kind, `#include "tcmi_orthogonalize.h"
+struct __KERNEL___s {
+${sizes}
+  static __device__ __forceinline__ float a() { return static_cast<float>(${double(a)}); }
+  static __device__ __forceinline__ float b() { return static_cast<float>(${double(b)}); }
+  static __device__ __forceinline__ float c() { return static_cast<float>(${double(c)}); }
+  static __device__ __forceinline__ double eps() { return ${double(eps)}; }
+};
+extern "C" __global__ void __launch_bounds__(256, 2) __KERNEL__(const TcmiArgs A) {
+  const tcmi::Orth<__KERNEL___s> o(A.in[0], A.out, A.ws, blockIdx.z);
+  __shared__ __attribute__((aligned(1024))) ${lds};
+  tcmi::${call};
+}
+`, [blocks, 1, count], 256);
+  const pool = `char lds[tcmi::f16x2_lds<${32 * T}, ${32 * T}>()]`;
+  const n = SP / pad, upper = n * (n + 1) / 2;
+  const kernels = [make('orthnorm', z.BLOCKS, 'double scratch[4]', `orth_norm<${S}>(o, scratch, blockIdx.x)`),
+    make('orthsplit', ceil(MP * NP, 4096), 'double scratch[4]', `orth_split<${S}, ${steps === 0}>(o, scratch, blockIdx.x)`)];
+  for (let k = 0; k < steps; k++) {
+    kernels.push(make('orthgram', upper, pool, `orth_gram<${S}, ${T}, ${k % 2}>(o, lds, blockIdx.x)`));
+    kernels.push(make('orthpoly', upper, pool, `orth_poly<${S}, ${T}>(o, lds, blockIdx.x)`));
+    kernels.push(make('orthapply', MP / pad * (NP / pad), pool, `orth_apply<${S}, ${T}, ${k % 2}, ${k === steps - 1}>(o, lds, blockIdx.x)`));
+  }
+  return { kind: 'orthogonalize', kernels, workspace: count * z.PER, flops: count * steps * (3 * s * s * l + s ** 3) };
+}
+
+/**
+ * Marks kernel `k` as the first of part `part` of a launch whose parts `build(parts)` forms
+ * together, in `order`. They read the same first `operands` operands (default: all).
+ */
+function joint(k, part, order, key, build, operands) {
+  Object.defineProperty(k, 'part', { value: part });
+  Object.defineProperty(k, 'joint', { value: { name: JSON.stringify(key), order, build, operands } });
+}
+
+/** The launch of an operator's node: { kind, kernels, params, workspace, flops }. tuning.loss.piece: bytes of a piece's logits. */
+function lowerOperator(graph, node, tuning) {
+  let k;
+  if (node.op === 'rotary' || node.op === 'rotaryGrad') k = lowerRotary(graph, node);
+  else if (node.op === 'linearCrossEntropy' || node.op === 'linearCrossEntropyGrad') k = lowerLoss(graph, node, tuning);
+  else if (node.op === 'orthogonalize') k = lowerOrthogonalize(graph, node);
+  else throw new Error(`no MI355X lowering for '${node.op}'`);
+  return Object.assign({ params: new Uint32Array(0), flops: 0 }, k);
+}
+
+module.exports = { OPERATORS, lowerOperator };

@@ -184,12 +184,12 @@ class HipRunner {
   /**
    * Function handles for every kernel of `lowered` (one launch list, or an
    * array of them): the kernels not loaded yet are compiled together as one
-   * module (one hiprtc call, cached on disk by its text).
+   * module (one hiprtc call, cached on disk by its text). `apart`: every launch by itself.
    */
-  functions(lowered) {
+  functions(lowered, apart) {
     const lists = Array.isArray(lowered) ? lowered : [lowered];
     const missing = new Map();
-    for (const l of lists) for (const [name, src] of kernelSources(l)) if (!this.loaded.has(name)) missing.set(name, src);
+    for (const l of lists) for (const [name, src] of kernelSources(l, apart)) if (!this.loaded.has(name)) missing.set(name, src);
     // Kernels compiled before in some unit: load that unit's module once per
     // process (a code-object cache hit) and take their functions from it.
     const index = loadIndex();
@@ -358,7 +358,7 @@ class Program {
     this.a = a;
     this.graph = graph;
     this.lowered = lowered;
-    const fns = runner.functions(lowered);
+    const fns = runner.functions(lowered, !!only || streams > 1);
     this.n = graph.nodes.map((node) => size(node.shape));
     const { alias, folded } = sharing(lowered);
     this.owned = [];

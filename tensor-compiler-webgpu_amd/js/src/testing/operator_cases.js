@@ -1,0 +1,108 @@
+'use strict';
+// Graphs of the operators that are one node each (ir/operators.js), from plain
+// descriptions: those of their GPU tests (CASES) and of their measurement (MEASURED).
+//   { family: 'rotary', x, positions, gain?, gradient?, options }   x twice over where `twin` gives a second shape
+//   { family: 'loss', N, d, V, bias?, gradient?, wrt?, after? }     wrt: 'h', 'W', 'b' (default all); `after`: the
+//       losses' cotangent depends on the losses, so their gradients cannot run beside them
+//   { family: 'orthogonalize', x, count, options }
+
+const { Graph } = require('../ir/graph');
+const { grad } = require('../autodiff');
+
+function operatorGraph(c) {
+  const g = new Graph();
+  let outs = [], names = [], wrt = [], grads = [];
+  if (c.family === 'rotary') {
+    const at = g.input('at', c.positions);
+    [c.x].concat(c.twin ? [c.twin] : []).forEach((shape, k) => {
+      const x = g.input(`x${k}`, shape);
+      const gain = c.gain ? g.input(`g${k}`, [shape[shape.length - 1]]) : null;
+      outs.push(g.rotary(x, at, Object.assign({ gain }, c.options || {})));
+      names.push(`y${k}`);
+      wrt.push(x);
+      grads.push(`dx${k}`);
+      if (c.gain) { wrt.push(gain); grads.push(`dg${k}`); }
+    });
+  } else if (c.family === 'loss') {
+    const h = g.input('h', [c.N, c.d]), W = g.input('W', [c.d, c.V]), t = g.input('t', [c.N]);
+    const b = c.bias ? g.input('b', [c.V]) : null;
+    const loss = g.linearCrossEntropy(h, W, t, b);
+    outs = [c.after ? g.mul(loss, loss) : loss];
+    names = ['loss'];
+    const all = { h, W, b };
+    for (const k of c.wrt || (c.bias ? ['h', 'W', 'b'] : ['h', 'W'])) { wrt.push(all[k]); grads.push(`d${k}`); }
+  } else if (c.family === 'orthogonalize') {
+    for (let k = 0; k < (c.count || 1); k++) {
+      outs.push(g.orthogonalize(g.input(`x${k}`, c.x), c.options));
+      names.push(`y${k}`);
+    }
+  } else throw new Error(`no operator '${c.family}'`);
+  if (!c.gradient) return { graph: g, keep: outs, names };
+  const G = grad(g, outs, wrt);
+  return { graph: G.graph, keep: outs.concat(G.grads), names: names.concat(grads) };
+}
+
+const rotary = (name, x, positions, more) => Object.assign({ name, family: 'rotary', x, positions }, more);
+const loss = (name, N, d, V, more) => Object.assign({ name, family: 'loss', N, d, V }, more);
+const orth = (name, x, more) => Object.assign({ name, family: 'orthogonalize', x }, more);
+
+const CASES = [
+  // One token and many; heads before and after the tokens; one position a token and one a sequence's token.
+  rotary('token', [3, 1, 5, 64], [3, 1], { gain: true, gradient: true }),
+  rotary('step', [4, 33, 4, 64], [33], { gain: true, gradient: true, twin: [4, 33, 2, 64] }),
+  rotary('heads-first', [2, 3, 17, 32], [2, 17], { gain: true, gradient: true, options: { axis: 2 } }),
+  rotary('one-head', [29, 48], [29], { gain: true, gradient: true }),
+  // Three axes, and frequencies that start over on each; adjacent pairs; a part of the head unrotated.
+  rotary('video', [1, 45, 3, 96], [1, 45, 3], { gain: true, gradient: true, options: { sections: [12, 18, 18] } }),
+  rotary('plane', [2, 16, 2, 40], [2, 16, 2], { gain: false, gradient: true, options: { sections: [8, 8], restart: true, pairs: 'adjacent' } }),
+  rotary('adjacent', [2, 9, 4, 128], [2, 9], { gain: true, gradient: true, options: { pairs: 'adjacent', sections: [32] } }),
+  rotary('partial', [2, 9, 4, 64], [9], { gain: true, gradient: true, options: { sections: [8] } }),
+  // No multiple of four anywhere, an odd head, no rotation at all, the longest head.
+  rotary('odd', [3, 7, 3, 15], [3, 7], { gain: true, gradient: true, options: { sections: [5] } }),
+  rotary('odd-adjacent', [7, 1, 7], [7], { gain: true, gradient: true, options: { pairs: 'adjacent', axis: 0 } }),
+  rotary('norm-only', [5, 2, 24], [5], { gain: true, gradient: true, options: { sections: [0], axis: 0 } }),
+  rotary('long-head', [3, 1, 4096], [3], { gain: true, gradient: true, options: { axis: 0 } }),
+  rotary('wide', [2, 700, 9, 32], [2, 700], { gain: true, gradient: true }),
+  // Rows from one to several pieces of tiles, classes from one to more than a tile, ragged and not; some gradients only.
+  loss('one', 1, 1, 1, { gradient: true }),
+  loss('few', 5, 16, 7, { bias: true, gradient: true }),
+  loss('square', 16, 8, 16, { gradient: true }),
+  loss('tile', 128, 64, 128, { bias: true, gradient: true }),
+  loss('step', 300, 96, 96, { bias: true, gradient: true }),
+  loss('ragged', 131, 37, 517, { bias: true, gradient: true }),
+  loss('deep', 40, 515, 260, { gradient: true }),
+  loss('wide', 70, 20, 5003, { bias: true, gradient: true }),
+  loss('rows', 3001, 20, 30, { bias: true, gradient: true }),
+  loss('values', 200, 24, 300, { bias: true }),
+  loss('only-h', 50, 24, 300, { bias: true, gradient: true, wrt: ['h'] }),
+  loss('only-W', 50, 24, 300, { bias: true, gradient: true, wrt: ['W'] }),
+  loss('only-b', 50, 24, 300, { bias: true, gradient: true, wrt: ['b'] }),
+  loss('pieces', 700, 24, 150, { bias: true, gradient: true, tuning: { loss: { piece: 1 } } }),
+  loss('piece-values', 400, 24, 150, { bias: true, tuning: { loss: { piece: 1 } } }),
+  loss('squared', 50, 24, 300, { bias: true, gradient: true, after: true }),
+  // Matrices from one element to several tiles, wide and tall, alone, stacked and side by side.
+  orth('one', [1, 1]),
+  orth('row', [1, 70]),
+  orth('column', [70, 1]),
+  orth('small', [8, 8]),
+  orth('square', [128, 128]),
+  orth('wide', [40, 300]),
+  orth('tall', [300, 130]),
+  orth('odd', [65, 67]),
+  orth('stack', [3, 2, 33, 20]),
+  orth('twins', [96, 64], { count: 3 }),
+  orth('steps', [50, 70], { options: { steps: 2, coefficients: [1.5, -0.5, 0], eps: 0 } }),
+  orth('none', [20, 30], { options: { steps: 0 } }),
+];
+
+const r = (B, T, H, dh, axes, gradient, twin) => rotary(null, [B, T, H, dh], axes === 1 ? [B, T] : [B, T, axes],
+  { gain: true, gradient, twin: [B, T, twin, dh], options: { axis: 1, base: 10000, eps: 1e-5,
+    sections: axes === 1 ? [dh / 2] : [dh / 2 - 2 * Math.floor(3 * dh / 16), Math.floor(3 * dh / 16), Math.floor(3 * dh / 16)] } });
+const MEASURED = [
+  r(32, 1, 8, 64, 1, false, 2), r(64, 128, 4, 64, 1, true, 4), r(1, 8191, 16, 128, 3, true, 4), r(2, 32768, 32, 128, 1, false, 8),
+  loss(null, 128, 64, 96, { bias: true }), loss(null, 8192, 256, 96, { bias: true, gradient: true }), loss(null, 4096, 512, 32768, {}),
+  loss(null, 1001, 515, 50021, { bias: true, gradient: true }), loss(null, 8192, 1024, 65536, { gradient: true }),
+  orth(null, [256, 256], { count: 16 }), orth(null, [1300, 777]), orth(null, [4096, 4096], { count: 2 }),
+];
+
+module.exports = { operatorGraph, CASES, MEASURED };
