@@ -10,18 +10,24 @@
 // in the root mean square by 2^-23.5: less than a float32 sum's own roundings from 16 terms on.
 // Half the matrix-core work of six products of bf16 parts (tcmi_gemm_bf16x3.h).
 //
-// Operands are planes in memory: element (line, k) of an operand (A: row of C, B: column
-// of C) at line·ld + k (KC: k contiguous) or k·ld + line, hi and lo planes of one layout.
-// They are padded with zeros to whole tiles (lines to the tile's, k to 32), so the loop has
-// no bounds. Loads go straight to LDS (16 bytes a lane). A slice of 32 k of L lines:
-//   KC       64 bytes a line, its four 16-byte chunks q rotated: chunk q of line l at
-//            slot q ^ (l / 2 % 4), so the 8 lanes of a 128-byte LDS cycle (8 lines, one q) meet
-//            all banks. A lane's fragment, 8 k of one line, is one ds_read_b128.
-//   not KC   2·L bytes a k, its 32-byte groups of 16 lines rotated: group g of row k at
-//            g ^ (k % 4). Fragments are read by ds_read_b64_tr_b16, which
-//            transposes: lanes of 16 each give the address of 4 lines of one of 4 rows of k, and
-//            each gets its own line's 4 k; two reads make a fragment.
-// Either way neither layout is materialised transposed.
+// Operands are read from memory as matrices of pairs: row r takes `ld` = 4·columns bytes, in blocks of 32
+// columns of 128 bytes, 32 hi halves and then their 32 lo halves, so a row's slice of 32 is one cache
+// line. An operand's lines (A: rows of C, B: columns of C) are the matrix's rows (KC: k runs along the
+// row) or its columns (k runs down): neither has to be transposed. The matrices are padded with zeros to
+// whole tiles (lines to the tile's, k to 32), so the loop has no bounds. Loads go straight to LDS (16
+// bytes a lane); a slice of 32 k of L lines there:
+//   KC       128 bytes a line, its eight 16-byte chunks c at slot c ^ (line % 8): the 16 lanes of a
+//            256-byte LDS cycle (16 lines, one chunk) meet all banks. A lane's fragment, 8 k of one line, is
+//            one ds_read_b128.
+//   not KC   4·L bytes a k row; its 32-byte groups g (16 lines of one half of the pairs) at g ^ (k % 4), its
+//            128-byte blocks at block ^ (k / 8 % 2). Fragments are read by ds_read_b64_tr_b16, which transposes: of
+//            16 lanes each gives the address of 4 lines of one of 4 rows, and gets its own line's 4 k; two reads
+//            make a fragment, and the 32 lanes of a cycle (4 rows k and 4 rows k + 8) meet all banks.
+//
+// Bound: power. 4096^3 by 128 x 128 tiles takes 314 us with pauses between launches and 370 us without
+// (438 and 371 TFLOP/s), the matrix cores busy for 67 % of the cycles at 1.86 GHz; reading the next
+// slice's fragments beside a column of products (one barrier a slice, as tcmi_gemm_bf16x3.h) is as fast, products of
+// 32 x 32 are slower (412 us). With planes of hi and of lo apart, a line's slice half a cache line: KC 417 us.
 
 #pragma once
 
@@ -57,120 +63,164 @@ __device__ __forceinline__ f4 join_pair(const h4& hi, const h4& lo) {
   return x;
 }
 
-// An operand: its hi plane, the lo plane `plane` bytes after it, and bytes a line (or k).
+// A matrix of pairs: its first byte, and bytes a row.
 struct Pairs {
-  const char* hi;
-  size_t plane;
+  const char* at;
   uint32_t ld;
 };
+
+// Where four floats of a row from column c on (a multiple of 4) keep their hi halves; the lo ones 64 bytes on.
+__device__ __forceinline__ char* pair_at(const Pairs& p, size_t row, uint32_t c) {
+  return const_cast<char*>(p.at) + row * p.ld + (c >> 5) * 128u + (c & 31u) * 2u;
+}
+__device__ __forceinline__ void put_pairs(const Pairs& p, size_t row, uint32_t c, const f4& v) {
+  h4 hi, lo;
+  split_pair(v, hi, lo);
+  char* at = pair_at(p, row, c);
+  *reinterpret_cast<h4*>(at) = hi;
+  *reinterpret_cast<h4*>(at + 64) = lo;
+}
+__device__ __forceinline__ f4 get_pairs(const Pairs& p, size_t row, uint32_t c) {
+  const char* at = pair_at(p, row, c);
+  return join_pair(*reinterpret_cast<const h4*>(at), *reinterpret_cast<const h4*>(at + 64));
+}
 
 // The tile of L lines x 32 k of one operand in LDS, filled by WAVES wavefronts.
 template <bool KC, int L, int WAVES>
 struct PairStage {
-  static constexpr int PLANE = L * 64, BYTES = 2 * PLANE;
-  static constexpr int UNITS = L / 16;                       // loads of 1 KiB a plane
-  static constexpr int LOADS = UNITS / WAVES;                // of each wavefront
-  static_assert(UNITS % WAVES == 0, "each wavefront fills as much of a plane");
-  static constexpr int CPR = L / 8;                          // 16-byte chunks of a k row
+  static constexpr int BYTES = L * 128;
+  static constexpr int LOADS = L / 8 / WAVES;                // of 1 KiB, of each wavefront
+  static_assert(L % (8 * WAVES) == 0 && L >= 64, "each wavefront fills as much of the tile");
+  static constexpr int CPR = L / 4;                          // 16-byte chunks of a k row
 
-  const char* base;        // of the tile at k = 0 (uniform)
-  size_t plane;
+  const char* base;        // of the tile at its k (uniform)
   size_t step;             // bytes of 32 k
   uint32_t off[LOADS];     // of this lane's 16 bytes
+  uint32_t at;             // of this lane in a fragment of the wavefront's first lines
 
-  __device__ __forceinline__ void begin(const Pairs& p, uint32_t line0, uint32_t k0, int wave, int lane) {
-    base = p.hi + (KC ? (size_t)line0 * p.ld + 2u * (size_t)k0 : (size_t)k0 * p.ld + 2u * (size_t)line0);
-    plane = p.plane;
-    step = KC ? 64u : (size_t)32u * p.ld;
+  // line0, k0: the tile's; first: the wavefront's own first line in it.
+  __device__ __forceinline__ void begin(const Pairs& p, uint32_t line0, uint32_t k0, int first, int wave, int lane) {
+    base = p.at + (KC ? (size_t)line0 * p.ld + 4u * (size_t)k0 : (size_t)k0 * p.ld + 4u * (size_t)line0);
+    step = KC ? 128u : (size_t)32u * p.ld;
 #pragma unroll
     for (int u = 0; u < LOADS; ++u) {
-      const int unit = u * WAVES + wave;
+      const int i = (u * WAVES + wave) * 64 + lane;
       if constexpr (KC) {
-        const int line = unit * 16 + (lane >> 2), q = (lane & 3) ^ ((line >> 1) & 3);
-        off[u] = line * p.ld + q * 16u;
+        const int line = i / 8, c = (i % 8) ^ (line % 8);
+        off[u] = line * p.ld + c * 16u;
       } else {
-        const int row = unit * (64 / CPR) + lane / CPR, c = (lane % CPR) ^ ((row & 3) << 1);
+        const int row = i / CPR, c = (i % CPR) ^ (row % 4 * 2) ^ (row / 8 % 2 * 8);
         off[u] = row * p.ld + c * 16u;
       }
+    }
+    const int t = lane & 15, q = lane >> 4;
+    if constexpr (KC) {
+      at = (first + t) * 128 + ((q ^ (t & 7)) << 4);
+    } else {
+      const int k = 8 * q + (t >> 2);
+      at = k * 4 * L + (((first >> 5) ^ (q & 1)) << 7) + ((((first >> 4) & 1) ^ (k & 3)) << 5) + (t & 3) * 8;
     }
   }
   // The next slice's loads, in flight until vmcnt reaches 0.
   __device__ __forceinline__ void load(char* tile, int wave) {
 #pragma unroll
-    for (int p = 0; p < 2; ++p)
-#pragma unroll
-      for (int u = 0; u < LOADS; ++u) {
-        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)(base + p * plane + off[u]),
-                                         (__attribute__((address_space(3))) uint32_t*)(tile + p * PLANE + (u * WAVES + wave) * 1024), 16, 0, 0);
-      }
+    for (int u = 0; u < LOADS; ++u) {
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)(base + off[u]),
+                                       (__attribute__((address_space(3))) uint32_t*)(tile + (u * WAVES + wave) * 1024), 16, 0, 0);
+    }
     base += step;
   }
-  // This lane's address in a plane: of fragment i of the lines from `line0` (a multiple of 32), at + i·FRAG (KC) or at ^ i·32.
-  static __device__ __forceinline__ uint32_t frag_at(int line0, int lane) {
-    const int t = lane & 15, q = lane >> 4;
-    if constexpr (KC) return (line0 + t) * 64 + ((q ^ ((t >> 1) & 3)) << 4);
-    const int k = 8 * q + (t >> 2);
-    return k * 2 * L + (((line0 >> 4) ^ (k & 3)) << 5) + (t & 3) * 8;
-  }
-  static __device__ __forceinline__ h8 frag(const char* plane, uint32_t at, int i) {
+  // The wavefront's fragment i (16 lines) of hi (p 0) or lo (1) halves. At most 4 fragments, the
+  // first line a multiple of 16 times as many (1, 2 or 4).
+  __device__ __forceinline__ h8 frag(const char* tile, int i, int p) const {
     if constexpr (KC) {
-      return *reinterpret_cast<const h8*>(plane + at + i * 1024);
+      return *reinterpret_cast<const h8*>(tile + (at ^ (p << 6)) + i * 2048);
     } else {
-      const char* p = plane + (at ^ (i << 5));
-      const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(p));
-      const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(p + 8 * L));
+      const char* x = tile + (at ^ (p << 6) ^ ((i & 1) << 5) ^ ((i >> 1) << 7));
+      const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(x));
+      const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(x + 16 * L));
       return __builtin_bit_cast(h8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
     }
   }
 };
 
-// LDS bytes of gemm_f16x2_sum: two buffers of both operands' slices.
-template <int BM, int BN>
-constexpr int f16x2_lds() { return 2 * 128 * (BM + BN); }
+// LDS bytes of a tile's product: STAGES slices of both operands.
+template <int BM, int BN, int STAGES = 2>
+constexpr int f16x2_lds() { return STAGES * 128 * (BM + BN); }
 
-// The BM x BN = (WM·TM·16) x (WN·TN·16) tile of A·B at (m0, n0), summed over `slices` slices of 32 k
+template <int N>
+struct Ahead { static constexpr int value = N; };
+
+// Waits until at most N of this wavefront's loads to LDS are in flight and all its reads of LDS are done.
+template <int N>
+__device__ __forceinline__ void arrived() {
+  static_assert(N < 64, "vmcnt");
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4 << 14) | 0x0070);   // vmcnt(N) lgkmcnt(0)
+  asm volatile("" ::: "memory");
+}
+// That of every wavefront (__syncthreads() would wait for every load).
+template <int N>
+__device__ __forceinline__ void barrier_ahead() {
+  arrived<N>();
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// The slices that nothing is loaded beside, A after the first of them and fewer after each.
+template <int A, class F>
+__device__ __forceinline__ void last_slices(uint32_t s, const uint32_t slices, F& slice) {
+  if (s + A < slices) {
+    slice(Ahead<A>(), false);
+    ++s;
+  }
+  if constexpr (A > 0) last_slices<A - 1>(s, slices, slice);
+}
+
+// The BM x BN = (WM·TM·16) x (WN·TN·16) tile of A·B at (m0, n0), summed over `slices` (1 or more) slices of 32 k
 // from k0: lane (t, q) = (lane % 16, lane / 16) of wavefront (wm, wn) holds in acc[i][j] row
-// m0 + (wm·TM + i)·16 + t, columns n0 + (wn·TN + j)·16 + 4q ... + 3. lds: f16x2_lds() bytes.
-template <int WM, int WN, int TM, int TN, bool AKC, bool BKC>
+// m0 + (wm·TM + i)·16 + t, columns n0 + (wn·TN + j)·16 + 4q ... + 3. STAGES - 1 slices are loaded ahead. With KW > 1, KW
+// wavefronts (WM = WN = 1) sum a part of the slices each, waiting for their own loads alone; their sums are added in
+// order, and wavefront g holds the fragments i = 0 .. TM/KW - 1 of rows from g·TM/KW on. lds: KW·f16x2_lds() bytes.
+template <int WM, int WN, int TM, int TN, bool AKC, bool BKC, int STAGES = 2, int KW = 1>
 __device__ __forceinline__ void gemm_f16x2_sum(const Pairs& a, const Pairs& b, const uint32_t m0, const uint32_t n0, const uint32_t k0,
-                                               const uint32_t slices, char* lds, f4 (&acc)[TM][TN]) {
+                                               const uint32_t slices, char* lds, f4 (&out)[TM / KW][TN]) {
   constexpr int WAVES = WM * WN, BM = WM * TM * 16, BN = WN * TN * 16;
   using SA = PairStage<AKC, BM, WAVES>;
   using SB = PairStage<BKC, BN, WAVES>;
-  constexpr int BUF = SA::BYTES + SB::BYTES;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wm = wave / WN, wn = wave % WN;
+  constexpr int BUF = SA::BYTES + SB::BYTES, LOADS = SA::LOADS + SB::LOADS;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % WAVES;
+  const uint32_t group = KW == 1 ? 0u : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / WAVES;
+  const uint32_t each = (slices + KW - 1) / KW, first = group * each;
+  if constexpr (KW > 1) lds += group * STAGES * BUF;
   SA sa;
   SB sb;
-  sa.begin(a, m0, k0, wave, lane);
-  sb.begin(b, n0, k0, wave, lane);
-  const uint32_t fa = SA::frag_at(wm * TM * 16, lane), fb = SB::frag_at(wn * TN * 16, lane);
-  f4 low[TM][TN];
+  sa.begin(a, m0, k0 + 32 * first, wave / WN * TM * 16, wave, lane);
+  sb.begin(b, n0, k0 + 32 * first, wave % WN * TN * 16, wave, lane);
+  f4 acc[TM][TN], low[TM][TN];
 #pragma unroll
   for (int i = 0; i < TM; ++i)
 #pragma unroll
     for (int j = 0; j < TN; ++j) acc[i][j] = low[i][j] = f4{0.f, 0.f, 0.f, 0.f};
 
-  sa.load(lds, wave);
-  sb.load(lds + SA::BYTES, wave);
-  for (uint32_t s = 0; s < slices; ++s) {
-    // This slice's loads have arrived, and every wavefront has read the other buffer's slice.
-    __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0)
-    __syncthreads();
-    const char* from = lds + (s & 1) * BUF;
+  uint32_t buf = 0, fill = 0;      // of the slice multiplied next, and of the slice loaded next
+  auto load = [&](char* to) {
+    sa.load(to, wave);
+    sb.load(to + SA::BYTES, wave);
+    fill = fill + 1 == STAGES ? 0 : fill + 1;
+  };
+  // The slice in `from` multiplied, and (more) the next one loaded into `to`. The pointers are restrict so that
+  // the compiler does not make the reads wait for every load to LDS: they wait at the barrier, for their own.
+  auto multiply = [&](const char* __restrict__ from, char* __restrict__ to, const bool more) __attribute__((always_inline)) {
     h8 x[TM][2], y[TN][2];
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
 #pragma unroll
-      for (int j = 0; j < TN; ++j) y[j][p] = SB::frag(from + SA::BYTES + p * SB::PLANE, fb, j);
+      for (int j = 0; j < TN; ++j) y[j][p] = sb.frag(from + SA::BYTES, j, p);
 #pragma unroll
-      for (int i = 0; i < TM; ++i) x[i][p] = SA::frag(from + p * SA::PLANE, fa, i);
+      for (int i = 0; i < TM; ++i) x[i][p] = sa.frag(from, i, p);
     }
-    if (s + 1 < slices) {
-      char* to = lds + ((s + 1) & 1) * BUF;
-      sa.load(to, wave);
-      sb.load(to + SA::BYTES, wave);
-    }
+    if (more) load(to);
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
@@ -183,11 +233,55 @@ __device__ __forceinline__ void gemm_f16x2_sum(const Pairs& a, const Pairs& b, c
     for (int i = 0; i < TM; ++i)
 #pragma unroll
       for (int j = 0; j < TN; ++j) low[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y[j][0], x[i][1], low[i][j], 0, 0, 0);
+  };
+  // One slice, once its loads (all but those of the `ahead` slices after it) have arrived and every wavefront has read
+  // the slice before, whose buffer is filled next.
+  auto slice = [&](auto ahead, const bool more) __attribute__((always_inline)) {
+    barrier_ahead<decltype(ahead)::value * LOADS>();
+    const char* from = lds + buf * BUF;
+    buf = buf + 1 == STAGES ? 0 : buf + 1;
+    multiply(from, lds + fill * BUF, more);
+  };
+  if constexpr (KW == 1) {
+    uint32_t s = 0;
+    for (uint32_t k = 0; k < STAGES - 1 && k < slices; ++k) load(lds + fill * BUF);
+    for (; s + STAGES - 1 < slices; ++s) slice(Ahead<STAGES - 2>(), true);
+    last_slices<STAGES - 2>(s, slices, slice);
+  } else {
+    static_assert(STAGES == 2 && WAVES == 1, "a slice ahead, and nobody else's");
+    const uint32_t mine = first < slices ? min(each, slices - first) : 0u;
+    if (mine > 0) load(lds);
+    for (uint32_t s = 0; s < mine; ++s) {
+      arrived<0>();
+      multiply(lds + (s & 1) * BUF, lds + ((s + 1) & 1) * BUF, s + 1 < mine);
+    }
   }
 #pragma unroll
   for (int i = 0; i < TM; ++i)
 #pragma unroll
-    for (int j = 0; j < TN; ++j) acc[i][j] += low[i][j] * (1.f / PAIR_LO);
+    for (int j = 0; j < TN; ++j) {
+      acc[i][j] += low[i][j] * (1.f / PAIR_LO);
+      if constexpr (KW == 1) out[i][j] = acc[i][j];
+    }
+  if constexpr (KW > 1) {
+    static_assert(TM % KW == 0 && TM * TN * 64 * 16 <= STAGES * BUF, "a wavefront's sums fit its slices' LDS");
+    f4* const sums = reinterpret_cast<f4*>(lds - group * STAGES * BUF);
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) reinterpret_cast<f4*>(lds)[(i * TN + j) * 64 + lane] = acc[i][j];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < TM / KW; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        const f4* at = sums + ((group * (TM / KW) + i) * TN + j) * 64 + lane;
+        f4 v = at[0];
+#pragma unroll
+        for (int g = 1; g < KW; ++g) v += at[g * (STAGES * BUF / 16)];
+        out[i][j] = v;
+      }
+  }
 }
 
 // The tile of workgroup `id` of rows x cols of them, so that the 8 XCDs (which take workgroups in
@@ -203,5 +297,41 @@ __device__ __forceinline__ TileAt tile_at(uint32_t id, uint32_t rows, uint32_t c
   const uint32_t band = t / (GROUP * cols), first = band * GROUP, tall = min(rows - first, GROUP), in = t - band * GROUP * cols;
   return {first + in % tall, in / tall};
 }
+
+// The tiles that kernels take: 64 x 64 by four wavefronts of 32 x 32 (SMALL), or by four that compute all of it over a
+// quarter of K each (FOUR); 128 x 128 by four of 64 x 64 (SQUARE); 128 x 256 (WIDE) and 256 x 128 (TALL) by eight. At 4096^3 SQUARE
+// takes 370 us, WIDE and TALL 352 - 365; 1024 x 1024 x 65536 448 and 417 - 425. The 64 x 64 ones are for products whose larger tiles
+// would leave CUs idle, FOUR where even those do and K is long: a wavefront of 32 x 32 reads 8 KiB of LDS for 192 cycles of
+// products, one of 64 x 64 16 KiB for 768 (91 tiles of K 1300: 20.5 us by SMALL, 16.1 by FOUR; 160 of K 256 6.3 and 9.3).
+enum { SMALL = 0, SQUARE = 1, WIDE = 2, TALL = 3, FOUR = 4 };
+template <int KIND>
+struct Tile {
+  static constexpr int T = KIND == SMALL ? 2 : 4, KW = KIND == FOUR ? 4 : 1;
+  static constexpr int WM = KIND == TALL ? 4 : KIND == FOUR ? 1 : 2, WN = KIND == WIDE ? 4 : KIND == FOUR ? 1 : 2;
+  static constexpr int ROWS = WM * T * 16, COLS = WN * T * 16, THREADS = KW * 64 * WM * WN;
+  static constexpr int STAGES = KIND == SQUARE || KW > 1 ? 2 : 3;
+  static constexpr int LDS = KW * f16x2_lds<ROWS, COLS, STAGES>();
+  // The fragments of 16 rows and of 16 columns that a wavefront holds.
+  static constexpr int TI = T / KW, TJ = T;
+  typedef f4 Sums[TI][TJ];
+
+  // The tile's sums over `slices` slices from k0.
+  template <bool AKC, bool BKC>
+  static __device__ __forceinline__ void sum(const Pairs& a, const Pairs& b, const TileAt& at, uint32_t k0, uint32_t slices, char* lds, Sums& acc) {
+    gemm_f16x2_sum<WM, WN, T, T, AKC, BKC, STAGES, KW>(a, b, at.row * ROWS, at.col * COLS, k0, slices, lds, acc);
+  }
+  // The row, and the first column, of this lane's first four sums: fragment (i, j)'s 16·i rows and 16·j columns on.
+  static __device__ __forceinline__ uint32_t row(const TileAt& at) { return at.row * ROWS + threadIdx.x / 64 / WN * TI * 16 + threadIdx.x % 16; }
+  static __device__ __forceinline__ uint32_t col(const TileAt& at) { return at.col * COLS + threadIdx.x / 64 % WN * TJ * 16 + threadIdx.x % 64 / 16 * 4; }
+  // f(row, col, v) of each four columns that this lane holds.
+  template <class F>
+  static __device__ __forceinline__ void each(const TileAt& at, Sums& acc, F f) {
+    const uint32_t row0 = row(at), col0 = col(at);
+#pragma unroll
+    for (int i = 0; i < TI; ++i)
+#pragma unroll
+      for (int j = 0; j < TJ; ++j) f(row0 + i * 16, col0 + j * 16, acc[i][j]);
+  }
+};
 
 }  // namespace tcmi

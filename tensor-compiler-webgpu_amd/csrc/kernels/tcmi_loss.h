@@ -14,13 +14,14 @@
 // |w|; every operand is read from the one layout it is written in.
 //
 //   maxima   partial maxima of |h|, |W| and |w|
-//   split    h's and W's planes, padded with zeros to tiles of 128 (k to 32)
+//   split    h and W as pairs, padded with zeros to tiles of 128 (k to 32)
 //   logits   z tile by tile; each wavefront's 64 columns of a row leave (maximum, sum of
 //            exponentials), and z itself where G will be formed
 //   join     a row's pairs joined in order; the losses; (M, 1/s) a row
-//   spread   G's planes, and the column sums of a few rows each
-//   dh, dW   products, their K split over workgroups where tiles are few; dW is added
-//            up over the pieces
+//   spread   G as pairs, and the column sums of a few rows each (with few pairs a row it joins them itself)
+//   grads    the tiles of dh and dW, and dbias, side by side in one launch; K split over
+//            workgroups where tiles are few; dW and dbias are added up over the pieces
+//   sums     the parts of a split K added in order
 // The piece that a kernel works on is counted in the workspace (two slots, so that no kernel
 // reads the one it writes), which keeps one kernel text and one argument block for all pieces.
 //
@@ -49,7 +50,9 @@ struct LossState {
 };
 
 // S: the sizes of one launch as constants of its text: N, D, V; NP rows a piece, PIECES of them; DP, VP: d and V padded to
-// 128; BIAS; BLOCKS partial maxima a tensor; RB rows a workgroup of `spread`; VECD, VECV: d, V multiples of 4.
+// 128 or 256; BIAS; HBLOCKS, WBLOCKS, GBLOCKS partial maxima of h, W and w; PER groups of four a thread of `split` takes; LKIND, HKIND and
+// WKIND of tiles for the logits, dh and dW; RB rows a workgroup of `spread`, CT threads across columns there;
+// JOINED: `join` runs; VECD, VECV: d, V multiples of 4; HCHUNKS, HK, WCHUNKS, WK: chunks of K of dh and dW, their slices.
 // WS: byte offsets in the workspace.
 template <class S>
 struct Loss {
@@ -57,9 +60,9 @@ struct Loss {
   char* ws;
   __device__ __forceinline__ LossState* state() const { return reinterpret_cast<LossState*>(ws); }
   __device__ __forceinline__ float* at(size_t off) const { return reinterpret_cast<float*>(ws + off); }
-  __device__ __forceinline__ Pairs h_planes() const { return {ws + S::HP, (size_t)S::NP * S::PIECES * S::DP * 2, S::DP * 2}; }
-  __device__ __forceinline__ Pairs w_planes() const { return {ws + S::WP, (size_t)S::DP * S::VP * 2, S::VP * 2}; }
-  __device__ __forceinline__ Pairs g_planes() const { return {ws + S::GP, (size_t)S::NP * S::VP * 2, S::VP * 2}; }
+  __device__ __forceinline__ Pairs h_pairs() const { return {ws + S::HP, S::DP * 4}; }
+  __device__ __forceinline__ Pairs w_pairs() const { return {ws + S::WP, S::VP * 4}; }
+  __device__ __forceinline__ Pairs g_pairs() const { return {ws + S::GP, S::VP * 4}; }
   // Whether row r counts, and its target.
   static __device__ __forceinline__ bool is_class(float c) { return c >= 0.f && c < static_cast<float>(S::V) && c == __builtin_floorf(c); }
   __device__ __forceinline__ bool kept(uint32_t r) const { return r < S::N && is_class(t[r]); }
@@ -75,33 +78,38 @@ __device__ __forceinline__ int scale_of(float top) {
   return 15 - e < 126 ? 15 - e : 126;
 }
 
+__device__ __forceinline__ float top_of(const f4& v, float top) {
+  return fmaxf(fmaxf(fmaxf(finite_abs(v[0]), finite_abs(v[1])), fmaxf(finite_abs(v[2]), finite_abs(v[3]))), top);
+}
+
 template <class S, bool GRAD>
 __device__ __forceinline__ void loss_maxima(const Loss<S>& L, float* scratch, uint32_t block) {
   float top = 0.f;
-  if (block < S::BLOCKS) {
-    for (uint32_t r = block * 4 + threadIdx.x / 64; r < S::N; r += S::BLOCKS * 4) {
-      if (!L.kept(r)) continue;
-      const float* x = L.h + (size_t)r * S::D;
-      if constexpr (S::VECD) {
-        for (uint32_t c = threadIdx.x % 64 * 4; c < S::D; c += 256) {
-          const f4 v = *reinterpret_cast<const f4*>(x + c);
-          top = fmaxf(fmaxf(fmaxf(finite_abs(v[0]), finite_abs(v[1])), fmaxf(finite_abs(v[2]), finite_abs(v[3]))), top);
-        }
-      } else {
-        for (uint32_t c = threadIdx.x % 64; c < S::D; c += 64) top = fmaxf(top, finite_abs(x[c]));
-      }
+  if (block < S::HBLOCKS) {
+    // Rows left out are loaded all the same, so that no load waits for a target.
+    constexpr uint32_t E = S::VECD ? 4 : 1;
+    constexpr size_t n = (size_t)S::N * S::D / E;
+#pragma unroll 4
+    for (size_t i = (size_t)block * 256 + threadIdx.x; i < n; i += (size_t)S::HBLOCKS * 256) {
+      float x;
+      if constexpr (S::VECD) x = top_of(reinterpret_cast<const f4*>(L.h)[i], 0.f);
+      else x = finite_abs(L.h[i]);
+      top = fmaxf(top, L.is_class(L.t[i * E / S::D]) ? x : 0.f);
     }
-  } else if (block < 2 * S::BLOCKS) {
-    constexpr size_t n = (size_t)S::D * S::V, n4 = n / 4;
-    const size_t i0 = (size_t)(block - S::BLOCKS) * 256 + threadIdx.x;
-    constexpr size_t step = (size_t)S::BLOCKS * 256;
-    for (size_t i = i0; i < n4; i += step) {
-      const f4 v = reinterpret_cast<const f4*>(L.W)[i];
-      top = fmaxf(fmaxf(fmaxf(finite_abs(v[0]), finite_abs(v[1])), fmaxf(finite_abs(v[2]), finite_abs(v[3]))), top);
+  } else if (block < S::HBLOCKS + S::WBLOCKS) {
+    // Four loads in flight a thread.
+    constexpr size_t n = (size_t)S::D * S::V, n4 = n / 4, step = (size_t)S::WBLOCKS * 256;
+    const size_t i0 = (size_t)(block - S::HBLOCKS) * 256 + threadIdx.x;
+    const f4* w = reinterpret_cast<const f4*>(L.W);
+    size_t i = i0;
+    for (; i + 3 * step < n4; i += 4 * step) {
+      const f4 a = w[i], b = w[i + step], c = w[i + 2 * step], d = w[i + 3 * step];
+      top = top_of(a, top_of(b, top_of(c, top_of(d, top))));
     }
+    for (; i < n4; i += step) top = top_of(w[i], top);
     if (i0 < n % 4) top = fmaxf(top, finite_abs(L.W[4 * n4 + i0]));
   } else if constexpr (GRAD) {
-    for (uint32_t r = threadIdx.x; r < S::N; r += 256)
+    for (uint32_t r = (block - S::HBLOCKS - S::WBLOCKS) * 256 + threadIdx.x; r < S::N; r += S::GBLOCKS * 256)
       if (L.kept(r)) top = fmaxf(top, finite_abs(L.w[r]));
   }
   top = block_reduce<true, 256>(top, scratch);
@@ -123,36 +131,37 @@ __device__ __forceinline__ f4 four(const float* x, size_t r, uint32_t rows, uint
   }
   return v;
 }
-__device__ __forceinline__ void put_pairs(const Pairs& p, size_t row, uint32_t col, const f4& v) {
-  h4 hi, lo;
-  split_pair(v, hi, lo);
-  char* at = const_cast<char*>(p.hi) + row * p.ld + 2u * col;
-  *reinterpret_cast<h4*>(at) = hi;
-  *reinterpret_cast<h4*>(at + p.plane) = lo;
+// The largest of maxima[0 .. count).
+__device__ __forceinline__ float top_of_blocks(const float* maxima, uint32_t count, float* scratch) {
+  float top = 0.f;
+  for (uint32_t i = threadIdx.x; i < count; i += 256) top = fmaxf(top, maxima[i]);
+  return block_reduce<true, 256>(top, scratch);
 }
-
-constexpr uint32_t SPLIT_PER = 16;      // groups of four that a thread of `split` takes
 
 template <class S, bool GRAD>
 __device__ __forceinline__ void loss_split(const Loss<S>& L, float* scratch, uint32_t block) {
   constexpr size_t HG = (size_t)S::NP * S::PIECES * S::DP / 4, WG = (size_t)S::DP * S::VP / 4;
-  constexpr uint32_t HB = (HG + 256 * SPLIT_PER - 1) / (256 * SPLIT_PER);
+  constexpr uint32_t HB = (HG + 256 * S::PER - 1) / (256 * S::PER);
   const bool of_w = block >= HB;
-  float top = 0.f;
-  for (uint32_t i = threadIdx.x; i < S::BLOCKS; i += 256) top = fmaxf(top, L.at(S::MAXIMA)[(of_w ? S::BLOCKS : 0u) + i]);
-  const int s = scale_of(block_reduce<true, 256>(top, scratch));
+  const float* maxima = L.at(S::MAXIMA);
+  const int s = scale_of(of_w ? top_of_blocks(maxima + S::HBLOCKS, S::WBLOCKS, scratch) : top_of_blocks(maxima, S::HBLOCKS, scratch));
+  if constexpr (GRAD) {
+    if (block == 0) {
+      const int g = scale_of(top_of_blocks(maxima + S::HBLOCKS + S::WBLOCKS, S::GBLOCKS, scratch));
+      if (threadIdx.x == 0) L.state()->g = g;
+    }
+  }
   if (threadIdx.x == 0) {
     LossState* st = L.state();
     if (block == 0) {
       st->piece = 0u;
       st->h = s;
-      if constexpr (GRAD) st->g = scale_of(L.at(S::MAXIMA)[2 * S::BLOCKS]);
     }
     if (block == HB) st->w = s;
   }
-  const Pairs p = of_w ? L.w_planes() : L.h_planes();
-  for (uint32_t u = 0; u < SPLIT_PER; ++u) {
-    const size_t i = ((size_t)(of_w ? block - HB : block) * SPLIT_PER + u) * 256 + threadIdx.x;
+  const Pairs p = of_w ? L.w_pairs() : L.h_pairs();
+  for (uint32_t u = 0; u < S::PER; ++u) {
+    const size_t i = ((size_t)(of_w ? block - HB : block) * S::PER + u) * 256 + threadIdx.x;
     f4 v;
     size_t row;
     uint32_t col;
@@ -177,75 +186,96 @@ __device__ __forceinline__ void loss_split(const Loss<S>& L, float* scratch, uin
 // One tile of the piece's logits.
 template <class S, bool KEEP>
 __device__ __forceinline__ void loss_logits(const Loss<S>& L, char* lds, uint32_t block) {
+  using P = Tile<S::LKIND>;
   LossState* st = L.state();
   const uint32_t piece = st->piece;
   if (block == 0 && threadIdx.x == 0) st->current = piece;
-  const TileAt tile = tile_at(block, S::NP / 128, S::VP / 128);
-  Pairs a = L.h_planes();
-  a.hi += (size_t)piece * S::NP * a.ld;
-  f4 acc[4][4];
-  gemm_f16x2_sum<2, 2, 4, 4, true, false>(a, L.w_planes(), tile.row * 128, tile.col * 128, 0, (S::D + 31) / 32, lds, acc);
+  const TileAt tile = tile_at(block, S::NP / P::ROWS, S::VP / P::COLS);
+  Pairs a = L.h_pairs();
+  a.at += (size_t)piece * S::NP * a.ld;
+  typename P::Sums acc;
+  P::template sum<true, false>(a, L.w_pairs(), tile, 0, (S::D + 31) / 32, lds, acc);
   const int back = -(st->h + st->w);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, t16 = lane & 15, q = lane >> 4;
-  const uint32_t col0 = tile.col * 128 + wave % 2 * 64 + 4 * q, row0 = tile.row * 128 + wave / 2 * 64 + t16;
-  f4 b[4];
+  const uint32_t col0 = P::col(tile), row0 = P::row(tile);
+  float m[P::TI];
+  uint32_t ahead[P::TI];       // the columns from col0 on to a row's target, where that is a class
 #pragma unroll
-  for (int j = 0; j < 4; ++j) b[j] = S::BIAS ? four<S::VECV>(L.bias, 0, 1, col0 + j * 16, S::V) : f4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t row = row0 + i * 16, r = piece * S::NP + row;
+  for (int i = 0; i < P::TI; ++i) {
+    const uint32_t r = piece * S::NP + row0 + i * 16;
     const float target = r < S::N ? L.t[r] : -1.f;
-    float m = -TCMI_INF;
+    ahead[i] = L.is_class(target) ? static_cast<uint32_t>(target) - col0 : ~0u;
+    m[i] = -TCMI_INF;
+  }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t col = col0 + j * 16;
+  for (int j = 0; j < P::TJ; ++j) {
+    const uint32_t col = col0 + j * 16;
+    const f4 b = S::BIAS ? four<S::VECV>(L.bias, 0, 1, col, S::V) : f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < P::TI; ++i) {
+      f4& z = acc[i][j];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float z = ldexpf(acc[i][j][e], back) + b[j][e];
-        acc[i][j][e] = z;
-        if (col + e < S::V) {
-          m = red_max(m, z);
-          if (static_cast<float>(col + e) == target) L.at(S::PICKED)[row] = z;
-        }
+        z[e] = ldexpf(z[e], back) + b[e];
+        if (S::V != S::VP && col + e >= S::V) z[e] = -TCMI_INF;
+        m[i] = fmaxf(m[i], z[e]);
       }
-      if constexpr (KEEP) *reinterpret_cast<f4*>(L.at(S::Z) + (size_t)row * S::VP + col) = acc[i][j];
+      const uint32_t e = ahead[i] - 16u * j;
+      if (e < 4u) L.at(S::PICKED)[row0 + i * 16] = e < 2u ? (e ? z[1] : z[0]) : e == 2u ? z[2] : z[3];
+      if constexpr (KEEP) *reinterpret_cast<f4*>(L.at(S::Z) + (size_t)(row0 + i * 16) * S::VP + col) = z;
     }
-    m = quad16_reduce<true>(m);
-    const float shift = m == -TCMI_INF ? 0.f : m;
+  }
+  // Sums of a wavefront's columns by op_exp: its error, |x|·2^-24 of an e^x, is least where e^x counts.
+#pragma unroll
+  for (int i = 0; i < P::TI; ++i) {
+    const float top = quad16_reduce<true>(m[i]), shift = top == -TCMI_INF ? 0.f : top;
     float s = 0.f;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < P::TJ; ++j)
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (col0 + j * 16 + e < S::V) s += exp_full(acc[i][j][e] - shift);
+      for (int e = 0; e < 4; ++e) s += op_exp(acc[i][j][e] - shift);
     s = quad16_reduce<false>(s);
-    if (q == 0) reinterpret_cast<float2*>(L.at(S::STATS))[(size_t)(tile.col * 2 + wave % 2) * S::NP + row] = make_float2(m, s);
+    if (threadIdx.x % 64 < 16) {
+      reinterpret_cast<float2*>(L.at(S::STATS))[(size_t)(tile.col * P::WN + threadIdx.x / 64 % P::WN) * S::NP + row0 + i * 16] = make_float2(top, s);
+    }
   }
 }
 
-// The statistics of 16 rows, 16 threads a row.
+// A row's statistics (maximum, sum of exponentials) joined with some columns' more.
+struct RowSum {
+  float m = -TCMI_INF, s = 0.f;
+  __device__ __forceinline__ void add(const float2 x) {
+    const float top = red_max(m, x.x), shift = top == -TCMI_INF ? 0.f : top;
+    s = s * exp_full(m - shift) + x.y * exp_full(x.x - shift);
+    m = top;
+  }
+};
+template <class S>
+constexpr uint32_t loss_parts() { return S::VP / (16 * Tile<S::LKIND>::T); }
+
+// The statistics of 16 rows, 64 threads a row.
 template <class S, bool LOSS, bool LAST>
 __device__ __forceinline__ void loss_join(const Loss<S>& L, float* out, float2* scratch, uint32_t block) {
   LossState* st = L.state();
   const uint32_t piece = st->current;
-  constexpr uint32_t PARTS = S::VP / 64;
   const uint32_t row = block * 16 + threadIdx.x % 16, k0 = threadIdx.x / 16;
   const float2* stats = reinterpret_cast<const float2*>(L.at(S::STATS)) + row;
-  float m = -TCMI_INF, s = 0.f;
-  auto add = [&](const float2 x) {
-    const float top = red_max(m, x.x), shift = top == -TCMI_INF ? 0.f : top;
-    s = s * exp_full(m - shift) + x.y * exp_full(x.x - shift);
-    m = top;
-  };
-  for (uint32_t k = k0; k < PARTS; k += 16) add(stats[(size_t)k * S::NP]);
-  scratch[threadIdx.x] = make_float2(m, s);
+  RowSum sum;
+#pragma unroll 4
+  for (uint32_t k = k0; k < loss_parts<S>(); k += 64) sum.add(stats[(size_t)k * S::NP]);
+  scratch[threadIdx.x] = make_float2(sum.m, sum.s);
+  __syncthreads();
+  if (k0 < 8) {
+    for (uint32_t k = k0 + 8; k < 64; k += 8) sum.add(scratch[k * 16 + threadIdx.x % 16]);
+  }
+  __syncthreads();
+  if (k0 < 8) scratch[threadIdx.x] = make_float2(sum.m, sum.s);
   __syncthreads();
   if (k0 == 0) {
-    for (uint32_t k = 1; k < 16; ++k) add(scratch[k * 16 + threadIdx.x]);
-    reinterpret_cast<float2*>(L.at(S::ROWS))[row] = make_float2(m, 1.f / s);
+    for (uint32_t k = 1; k < 8; ++k) sum.add(scratch[k * 16 + threadIdx.x]);
+    reinterpret_cast<float2*>(L.at(S::ROWS))[row] = make_float2(sum.m, 1.f / sum.s);
     const uint32_t r = piece * S::NP + row;
     if constexpr (LOSS) {
-      if (r < S::N) out[r] = L.kept(r) ? (m - L.at(S::PICKED)[row]) + op_log(s) : 0.f;
+      if (r < S::N) out[r] = L.kept(r) ? (sum.m - L.at(S::PICKED)[row]) + op_log(sum.s) : 0.f;
     }
   }
   if constexpr (LAST) {
@@ -253,9 +283,10 @@ __device__ __forceinline__ void loss_join(const Loss<S>& L, float* out, float2* 
   }
 }
 
-// RB rows of 1024 columns of G.
-template <class S, bool PLANES, bool SUMS>
-__device__ __forceinline__ void loss_spread(const Loss<S>& L, f4* rows, uint32_t bx, uint32_t by) {
+// RB rows of 8·CT columns of G: 256 / CT threads a column group, each its own rows in turn. rows: of LDS, and 512 more for
+// the sums. out: the losses, where this kernel joins the statistics (not JOINED).
+template <class S, bool PAIRS, bool SUMS, bool LOSS>
+__device__ __forceinline__ void loss_spread(const Loss<S>& L, float* out, f4* rows, uint32_t bx, uint32_t by) {
   const LossState* st = L.state();
   const uint32_t piece = st->current;
   const int sg = st->g;
@@ -263,36 +294,92 @@ __device__ __forceinline__ void loss_spread(const Loss<S>& L, f4* rows, uint32_t
   if (threadIdx.x < S::RB) {
     const uint32_t row = row0 + threadIdx.x, r = piece * S::NP + row;
     f4 c = {0.f, 0.f, 0.f, -1.f};       // M, w/s and w in G's scale, the target (-1: the row is left out)
-    if (L.kept(r)) {
-      const float2 x = reinterpret_cast<const float2*>(L.at(S::ROWS))[row];
+    const bool kept = L.kept(r);
+    if (kept) {
+      float2 x;
+      if constexpr (S::JOINED) {
+        x = reinterpret_cast<const float2*>(L.at(S::ROWS))[row];
+      } else {
+        RowSum sum;
+        for (uint32_t k = 0; k < loss_parts<S>(); ++k) sum.add(reinterpret_cast<const float2*>(L.at(S::STATS))[(size_t)k * S::NP + row]);
+        x = make_float2(sum.m, 1.f / sum.s);
+        if constexpr (LOSS) {
+          if (bx == 0) out[r] = (sum.m - L.at(S::PICKED)[row]) + op_log(sum.s);
+        }
+      }
       const float w = ldexpf(L.w[r], sg);
       c = f4{x.x, w * x.y, w, L.t[r]};
+    } else if constexpr (LOSS && !S::JOINED) {
+      if (bx == 0 && r < S::N) out[r] = 0.f;
     }
     rows[threadIdx.x] = c;
   }
   __syncthreads();
-  const uint32_t col = bx * 1024 + threadIdx.x * 4;
-  if (col >= S::VP) return;
-  const Pairs p = L.g_planes();
-  f4 sum = {0.f, 0.f, 0.f, 0.f};
-  for (uint32_t k = 0; k < S::RB; ++k) {
-    const f4 c = rows[k];
-    f4 g = {0.f, 0.f, 0.f, 0.f};
-    if (c[3] >= 0.f) {
-      const f4 z = *reinterpret_cast<const f4*>(L.at(S::Z) + (size_t)(row0 + k) * S::VP + col);
+  constexpr uint32_t RG = 256 / S::CT;
+  const uint32_t col = (bx * S::CT + threadIdx.x % S::CT) * 8, group = threadIdx.x / S::CT;
+  const Pairs p = L.g_pairs();
+  f4 sum[2] = {};
+  if (col < S::VP) {
+#pragma unroll 2
+    for (uint32_t k = group; k < S::RB; k += RG) {
+      const f4 c = rows[k];
+      const f4* z = reinterpret_cast<const f4*>(L.at(S::Z) + (size_t)(row0 + k) * S::VP + col);
+      const f4 y[2] = {z[0], z[1]};
+      f4 g[2] = {};
+      if (c[3] >= 0.f) {
+        const uint32_t ahead = static_cast<uint32_t>(c[3]) - col;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (col + e < S::V) g[e] = exp_full(z[e] - c[0]) * c[1] - (static_cast<float>(col + e) == c[3] ? c[2] : 0.f);
+        for (int e = 0; e < 8; ++e) {
+          // exp(-inf) of a column that is no class is 0.
+          g[e / 4][e % 4] = exp_full(y[e / 4][e % 4] - c[0]) * c[1] - (ahead == e ? c[2] : 0.f);
+        }
+        if (S::V % 8 != 0 && col + 8 > S::V) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (col + e >= S::V) g[e / 4][e % 4] = 0.f;      // also where M is not finite
+        }
+      }
+      if constexpr (SUMS) {
+        sum[0] += g[0];
+        sum[1] += g[1];
+      }
+      if constexpr (PAIRS) {
+        h8 hi, lo;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          _Float16 a, b;
+          split_pair(g[e / 4][e % 4], a, b);
+          hi[e] = a;
+          lo[e] = b;
+        }
+        char* at = pair_at(p, row0 + k, col);
+        *reinterpret_cast<h8*>(at) = hi;
+        *reinterpret_cast<h8*>(at + 64) = lo;
       }
     }
-    if constexpr (SUMS) sum += g;
-    if constexpr (PLANES) put_pairs(p, row0 + k, col, g);
   }
-  if constexpr (SUMS) *reinterpret_cast<f4*>(L.at(S::SUMS) + (size_t)by * S::VP + col) = sum;
+  if constexpr (SUMS) {
+    f4* const parts = rows + S::RB;
+    if constexpr (RG > 1) {
+      parts[2 * threadIdx.x] = sum[0];
+      parts[2 * threadIdx.x + 1] = sum[1];
+      __syncthreads();
+      if (group == 0) {
+        for (uint32_t k = 1; k < RG; ++k) {
+          sum[0] += parts[2 * (k * S::CT + threadIdx.x)];
+          sum[1] += parts[2 * (k * S::CT + threadIdx.x) + 1];
+        }
+      }
+    }
+    if (group == 0 && col < S::VP) {
+      f4* to = reinterpret_cast<f4*>(L.at(S::SUMS) + (size_t)by * S::VP + col);
+      to[0] = sum[0];
+      to[1] = sum[1];
+    }
+  }
 }
 
-// C rows x cols = the product's, scaled back by 2^back, added to what is there (ADD); chunk `z` of K to its own
-// partial [DPAD, cpad] where K is split.
+// Four columns of C [rows, cols] = v, or added to what is there.
 template <bool VEC>
 __device__ __forceinline__ void put_four(float* out, size_t row, uint32_t rows, uint32_t col, uint32_t cols, f4 v, bool add) {
   if (row >= rows) return;
@@ -308,114 +395,88 @@ __device__ __forceinline__ void put_four(float* out, size_t row, uint32_t rows, 
       if (col + e < cols) p[e] = add ? p[e] + v[e] : v[e];
   }
 }
+__device__ __forceinline__ f4 scaled(f4 v, int by) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = ldexpf(v[e], by);
+  return v;
+}
+// Workgroups of `grads`: dh's tiles by chunks of K, dW's, then dbias.
+template <class S>
+struct GradTiles {
+  using H = Tile<S::HKIND>;
+  using W = Tile<S::WKIND>;
+  static_assert(H::THREADS == W::THREADS, "one launch");
+  static constexpr uint32_t HR = S::NP / H::ROWS, HC = S::DP / H::COLS, WR = S::DP / W::ROWS, WC = S::VP / W::COLS;
+  static constexpr int LDS = H::LDS > W::LDS ? H::LDS : W::LDS;
+};
 
-// A tile of dh (rows of the piece): K = V in CHUNKS chunks of KC slices.
-template <class S>
-__device__ __forceinline__ void loss_dh(const Loss<S>& L, float* out, char* lds, uint32_t block) {
-  const LossState* st = L.state();
-  const uint32_t piece = st->current;
-  constexpr uint32_t TILES = S::NP / 128 * (S::DP / 128);
-  const uint32_t chunk = block / TILES;
-  const TileAt tile = tile_at(block % TILES, S::NP / 128, S::DP / 128);
-  f4 acc[4][4];
-  const uint32_t first = chunk * S::HK, left = S::VP / 32 - first;
-  gemm_f16x2_sum<2, 2, 4, 4, true, true>(L.g_planes(), L.w_planes(), tile.row * 128, tile.col * 128, first * 32, left < S::HK ? left : S::HK, lds, acc);
-  const int back = -(st->g + st->w);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const uint32_t col0 = tile.col * 128 + wave % 2 * 64 + 4 * (lane >> 4), row0 = tile.row * 128 + wave / 2 * 64 + (lane & 15);
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t row = row0 + i * 16, col = col0 + j * 16;
-      f4 v = acc[i][j];
-      if constexpr (S::HCHUNKS > 1) {
-        *reinterpret_cast<f4*>(L.at(S::HPART) + ((size_t)chunk * S::NP + row) * S::DP + col) = v;
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = ldexpf(v[e], back);
-        put_four<S::VECD>(out, (size_t)piece * S::NP + row, S::N, col, S::D, v, false);
-      }
-    }
-}
-// The chunks of dh added in order.
-template <class S>
-__device__ __forceinline__ void loss_dh_sum(const Loss<S>& L, float* out, uint32_t block) {
-  const LossState* st = L.state();
-  const uint32_t i = block * 256 + threadIdx.x, row = i / (S::DP / 4), col = i % (S::DP / 4) * 4;
-  if (row >= S::NP) return;
-  const int back = -(st->g + st->w);
-  f4 v = {0.f, 0.f, 0.f, 0.f};
-  for (uint32_t c = 0; c < S::HCHUNKS; ++c) v += *reinterpret_cast<const f4*>(L.at(S::HPART) + ((size_t)c * S::NP + row) * S::DP + col);
-#pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] = ldexpf(v[e], back);
-  put_four<S::VECD>(out, (size_t)st->current * S::NP + row, S::N, col, S::D, v, false);
-}
-
-// A tile of dW: K = the piece's rows in CHUNKS chunks of WK slices.
-template <class S>
-__device__ __forceinline__ void loss_dw(const Loss<S>& L, float* out, char* lds, uint32_t block) {
-  const LossState* st = L.state();
-  const uint32_t piece = st->current;
-  constexpr uint32_t TILES = S::DP / 128 * (S::VP / 128);
-  const uint32_t chunk = block / TILES;
-  const TileAt tile = tile_at(block % TILES, S::DP / 128, S::VP / 128);
-  Pairs a = L.h_planes();
-  a.hi += (size_t)piece * S::NP * a.ld;
-  f4 acc[4][4];
-  const uint32_t first = chunk * S::WK, left = S::NP / 32 - first;
-  gemm_f16x2_sum<2, 2, 4, 4, false, false>(a, L.g_planes(), tile.row * 128, tile.col * 128, first * 32, left < S::WK ? left : S::WK, lds, acc);
-  const int back = -(st->g + st->h);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const uint32_t col0 = tile.col * 128 + wave % 2 * 64 + 4 * (lane >> 4), row0 = tile.row * 128 + wave / 2 * 64 + (lane & 15);
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t row = row0 + i * 16, col = col0 + j * 16;
-      f4 v = acc[i][j];
-      if constexpr (S::WCHUNKS > 1) {
-        *reinterpret_cast<f4*>(L.at(S::WPART) + ((size_t)chunk * S::DP + row) * S::VP + col) = v;
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = ldexpf(v[e], back);
-        put_four<S::VECV>(out, row, S::D, col, S::V, v, piece > 0);
-      }
-    }
-}
-template <class S>
-__device__ __forceinline__ void loss_dw_sum(const Loss<S>& L, float* out, uint32_t block) {
-  const LossState* st = L.state();
-  const size_t i = (size_t)block * 256 + threadIdx.x;
-  const size_t row = i / (S::VP / 4);
-  const uint32_t col = i % (S::VP / 4) * 4;
-  if (row >= S::D) return;
-  const int back = -(st->g + st->h);
-  f4 v = {0.f, 0.f, 0.f, 0.f};
-  for (uint32_t c = 0; c < S::WCHUNKS; ++c) v += *reinterpret_cast<const f4*>(L.at(S::WPART) + ((size_t)c * S::DP + row) * S::VP + col);
-#pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] = ldexpf(v[e], back);
-  put_four<S::VECV>(out, row, S::D, col, S::V, v, st->current > 0);
-}
-
-// dbias from the column sums of each RB rows, added in order: 16 threads a column, then theirs. Counts the piece as done.
-template <class S, bool BIAS>
-__device__ __forceinline__ void loss_end(const Loss<S>& L, float* out, float* scratch, uint32_t block) {
+template <class S, bool DH, bool DW, bool DB>
+__device__ __forceinline__ void loss_grads(const Loss<S>& L, float* dh, float* dw, float* db, char* lds, uint32_t block) {
+  using G = GradTiles<S>;
+  constexpr uint32_t HB = DH ? G::HR * G::HC * S::HCHUNKS : 0, WB = DW ? G::WR * G::WC * S::WCHUNKS : 0;
   LossState* st = L.state();
   const uint32_t piece = st->current;
-  if constexpr (BIAS) {
-    const uint32_t col = block * 16 + threadIdx.x % 16, k0 = threadIdx.x / 16;
+  if (block == 0 && threadIdx.x == 0) st->piece = piece + 1;     // this piece is done with the next kernel
+  if (DH && block < HB) {
+    using P = typename G::H;
+    const uint32_t chunk = block / (G::HR * G::HC), first = chunk * S::HK, left = S::VP / 32 - first;
+    const TileAt tile = tile_at(block % (G::HR * G::HC), G::HR, G::HC);
+    typename P::Sums acc;
+    P::template sum<true, true>(L.g_pairs(), L.w_pairs(), tile, first * 32, left < S::HK ? left : S::HK, lds, acc);
+    const int back = -(st->g + st->w);
+    P::each(tile, acc, [&](uint32_t row, uint32_t col, const f4& v) {
+      if constexpr (S::HCHUNKS > 1) *reinterpret_cast<f4*>(L.at(S::HPART) + ((size_t)chunk * S::NP + row) * S::DP + col) = v;
+      else put_four<S::VECD>(dh, (size_t)piece * S::NP + row, S::N, col, S::D, scaled(v, back), false);
+    });
+  } else if (DW && block - HB < WB) {
+    using P = typename G::W;
+    const uint32_t id = block - HB, chunk = id / (G::WR * G::WC), first = chunk * S::WK, left = S::NP / 32 - first;
+    const TileAt tile = tile_at(id % (G::WR * G::WC), G::WR, G::WC);
+    Pairs a = L.h_pairs();
+    a.at += (size_t)piece * S::NP * a.ld;
+    typename P::Sums acc;
+    P::template sum<false, false>(a, L.g_pairs(), tile, first * 32, left < S::WK ? left : S::WK, lds, acc);
+    const int back = -(st->g + st->h);
+    P::each(tile, acc, [&](uint32_t row, uint32_t col, const f4& v) {
+      if constexpr (S::WCHUNKS > 1) *reinterpret_cast<f4*>(L.at(S::WPART) + ((size_t)chunk * S::DP + row) * S::VP + col) = v;
+      else put_four<S::VECV>(dw, row, S::D, col, S::V, scaled(v, back), piece > 0);
+    });
+  } else if constexpr (DB) {
+    // The column sums of each RB rows in order: PER threads a column, then theirs.
+    constexpr uint32_t PER = G::H::THREADS / 16;
+    float* const scratch = reinterpret_cast<float*>(lds);
+    const uint32_t col = (block - HB - WB) * 16 + threadIdx.x % 16, k0 = threadIdx.x / 16;
     float sum = 0.f;
-    for (uint32_t k = k0; k < S::NP / S::RB; k += 16) sum += L.at(S::SUMS)[(size_t)k * S::VP + col];
+    for (uint32_t k = k0; k < S::NP / S::RB; k += PER) sum += L.at(S::SUMS)[(size_t)k * S::VP + col];
     scratch[threadIdx.x] = sum;
     __syncthreads();
     if (k0 == 0 && col < S::V) {
-      for (uint32_t k = 1; k < 16; ++k) sum += scratch[k * 16 + threadIdx.x];
+      for (uint32_t k = 1; k < PER; ++k) sum += scratch[k * 16 + threadIdx.x];
       const float v = ldexpf(sum, -st->g);
-      out[col] = piece > 0 ? out[col] + v : v;
+      db[col] = piece > 0 ? db[col] + v : v;
     }
   }
-  if (block == 0 && threadIdx.x == 0) st->piece = piece + 1;
+}
+
+// The chunks of dh (HB workgroups) and of dW added in order, four columns a thread.
+template <class S, bool DH, bool DW>
+__device__ __forceinline__ void loss_sums(const Loss<S>& L, float* dh, float* dw, uint32_t block) {
+  constexpr uint32_t HB = DH ? (S::NP * (S::DP / 4) + 255) / 256 : 0;
+  const LossState* st = L.state();
+  if (DH && block < HB) {
+    const uint32_t i = block * 256 + threadIdx.x, row = i / (S::DP / 4), col = i % (S::DP / 4) * 4;
+    if (row >= S::NP) return;
+    f4 v = {0.f, 0.f, 0.f, 0.f};
+    for (uint32_t c = 0; c < S::HCHUNKS; ++c) v += *reinterpret_cast<const f4*>(L.at(S::HPART) + ((size_t)c * S::NP + row) * S::DP + col);
+    put_four<S::VECD>(dh, (size_t)st->current * S::NP + row, S::N, col, S::D, scaled(v, -(st->g + st->w)), false);
+  } else if constexpr (DW) {
+    const size_t i = (size_t)(block - HB) * 256 + threadIdx.x, row = i / (S::VP / 4);
+    const uint32_t col = i % (S::VP / 4) * 4;
+    if (row >= S::D) return;
+    f4 v = {0.f, 0.f, 0.f, 0.f};
+    for (uint32_t c = 0; c < S::WCHUNKS; ++c) v += *reinterpret_cast<const f4*>(L.at(S::WPART) + ((size_t)c * S::DP + row) * S::VP + col);
+    put_four<S::VECV>(dw, row, S::D, col, S::V, scaled(v, -(st->g + st->h)), st->current > 0);
+  }
 }
 
 }  // namespace tcmi

@@ -10,7 +10,8 @@
 // is as large as what the product that reads it leaves out. x keeps its layout:
 // a tall X is read transposed by its products, never written so.
 //
-// A and B are symmetric: only tiles on and above the diagonal are computed, and written twice.
+// A and B are symmetric: only tiles on and above the diagonal are computed, and written twice, where tiles are many; where
+// all of them fit the chip at once (HALF false), computing each takes no longer and spares the scattered mirrored writes.
 // The norm is summed in float64: no float's square overflows or vanishes.
 //
 // Bound: the matrix cores, s²·l + s³ + 2·s²·l flops a step (s, l: the smaller and larger of M, N).
@@ -21,7 +22,7 @@
 
 namespace tcmi {
 
-// S: the sizes of one launch as constants of its text: M, N; MP, NP padded to whole tiles of T·32 (SP: the
+// S: the sizes of one launch as constants of its text: M, N; GKIND, BKIND, AKIND of tiles for A, B and X; HALF; MP, NP padded to whole tiles (SP: the
 // smaller's); TALL; BLOCKS of the norm; SX, SA, SB exponents of the scales; VEC: N a multiple of 4; a(), b(), c(), eps().
 // WS: byte offsets in one matrix's workspace, PER bytes.
 template <class S>
@@ -31,20 +32,10 @@ struct Orth {
   char* ws;
   __device__ __forceinline__ Orth(const float* x_, float* out_, float* ws_, uint32_t z)
       : x(x_ + (size_t)z * S::M * S::N), out(out_ + (size_t)z * S::M * S::N), ws(reinterpret_cast<char*>(ws_) + (size_t)z * S::PER) {}
-  __device__ __forceinline__ Pairs xs(int which) const { return {ws + (which ? S::X1 : S::X0), (size_t)S::MP * S::NP * 2, S::NP * 2}; }
-  __device__ __forceinline__ Pairs as() const { return {ws + S::A, (size_t)S::SP * S::SP * 2, S::SP * 2}; }
-  __device__ __forceinline__ Pairs bs() const { return {ws + S::B, (size_t)S::SP * S::SP * 2, S::SP * 2}; }
+  __device__ __forceinline__ Pairs xs(int which) const { return {ws + (which ? S::X1 : S::X0), S::NP * 4}; }
+  __device__ __forceinline__ Pairs as() const { return {ws + S::A, S::SP * 4}; }
+  __device__ __forceinline__ Pairs bs() const { return {ws + S::B, S::SP * 4}; }
 };
-
-__device__ __forceinline__ void put_pair4(const Pairs& p, size_t row, uint32_t col, const h4& hi, const h4& lo) {
-  char* at = const_cast<char*>(p.hi) + row * p.ld + 2u * col;
-  *reinterpret_cast<h4*>(at) = hi;
-  *reinterpret_cast<h4*>(at + p.plane) = lo;
-}
-__device__ __forceinline__ f4 get_pair4(const Pairs& p, size_t row, uint32_t col) {
-  const char* at = p.hi + row * p.ld + 2u * col;
-  return join_pair(*reinterpret_cast<const h4*>(at), *reinterpret_cast<const h4*>(at + p.plane));
-}
 
 __device__ __forceinline__ double block_sum(double v, double* scratch) {
 #pragma unroll
@@ -109,9 +100,7 @@ __device__ __forceinline__ void orth_split(const Orth<S>& o, double* scratch, ui
       if (row >= S::M || col >= S::N) v = f4{0.f, 0.f, 0.f, 0.f};      // 0 / (0 + 0) is not padding
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] = col + e < S::N ? v[e] * static_cast<float>(1u << S::SX) : 0.f;
-      h4 hi, lo;
-      split_pair(v, hi, lo);
-      put_pair4(p, row, col, hi, lo);
+      put_pairs(p, row, col, v);
     }
   }
 }
@@ -126,65 +115,60 @@ __device__ __forceinline__ TileAt upper_tile(uint32_t id, uint32_t n) {
   return {t - col * (col + 1) / 2, col};
 }
 
-// f(row, col, v) of each four columns of a tile that a lane holds.
-template <int T, class F>
-__device__ __forceinline__ void each_four(const TileAt& tile, f4 (&acc)[T][T], F f) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const uint32_t row0 = tile.row * 32 * T + wave / 2 * 16 * T + (lane & 15), col0 = tile.col * 32 * T + wave % 2 * 16 * T + 4 * (lane >> 4);
-#pragma unroll
-  for (int i = 0; i < T; ++i)
-#pragma unroll
-    for (int j = 0; j < T; ++j) f(row0 + i * 16, col0 + j * 16, acc[i][j]);
-}
-
 // v at (row, col ... col + 3) of a symmetric matrix, and mirrored.
+template <bool HALF>
 __device__ __forceinline__ void put_symmetric(const Pairs& p, const TileAt& tile, uint32_t row, uint32_t col, const f4& v) {
   h4 hi, lo;
   split_pair(v, hi, lo);
-  put_pair4(p, row, col, hi, lo);
-  if (tile.row == tile.col) return;
+  char* at = pair_at(p, row, col);
+  *reinterpret_cast<h4*>(at) = hi;
+  *reinterpret_cast<h4*>(at + 64) = lo;
+  if (!HALF || tile.row == tile.col) return;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    char* at = const_cast<char*>(p.hi) + (size_t)(col + e) * p.ld + 2u * row;
+    at = pair_at(p, col + e, row);
     *reinterpret_cast<_Float16*>(at) = hi[e];
-    *reinterpret_cast<_Float16*>(at + p.plane) = lo[e];
+    *reinterpret_cast<_Float16*>(at + 64) = lo[e];
   }
 }
 
 constexpr float two_to(int e) { return e < 0 ? 1.f / static_cast<float>(1ull << -e) : static_cast<float>(1ull << e); }
 
 // A = X·Xᵀ (TALL: Xᵀ·X).
-template <class S, int T, int FROM>
+template <class S, int FROM>
 __device__ __forceinline__ void orth_gram(const Orth<S>& o, char* lds, uint32_t block) {
-  const TileAt tile = upper_tile(block, S::SP / (32 * T));
-  f4 acc[T][T];
-  gemm_f16x2_sum<2, 2, T, T, !S::TALL, !S::TALL>(o.xs(FROM), o.xs(FROM), tile.row * 32 * T, tile.col * 32 * T, 0, ((S::TALL ? S::M : S::N) + 31) / 32, lds, acc);
+  using P = Tile<S::GKIND>;
+  const TileAt tile = S::HALF ? upper_tile(block, S::SP / P::ROWS) : tile_at(block, S::SP / P::ROWS, S::SP / P::ROWS);
+  typename P::Sums acc;
+  P::template sum<!S::TALL, !S::TALL>(o.xs(FROM), o.xs(FROM), tile, 0, ((S::TALL ? S::M : S::N) + 31) / 32, lds, acc);
   const Pairs p = o.as();
-  each_four<T>(tile, acc, [&](uint32_t row, uint32_t col, const f4& v) { put_symmetric(p, tile, row, col, v * two_to(S::SA - 2 * S::SX)); });
+  P::each(tile, acc, [&](uint32_t row, uint32_t col, const f4& v) { put_symmetric<S::HALF>(p, tile, row, col, v * two_to(S::SA - 2 * S::SX)); });
 }
 
 // B = b·A + c·A·A.
-template <class S, int T>
+template <class S>
 __device__ __forceinline__ void orth_poly(const Orth<S>& o, char* lds, uint32_t block) {
-  const TileAt tile = upper_tile(block, S::SP / (32 * T));
-  f4 acc[T][T];
+  using P = Tile<S::BKIND>;
+  const TileAt tile = S::HALF ? upper_tile(block, S::SP / P::ROWS) : tile_at(block, S::SP / P::ROWS, S::SP / P::ROWS);
+  typename P::Sums acc;
   const Pairs a = o.as(), p = o.bs();
-  gemm_f16x2_sum<2, 2, T, T, true, true>(a, a, tile.row * 32 * T, tile.col * 32 * T, 0, ((S::TALL ? S::N : S::M) + 31) / 32, lds, acc);
-  each_four<T>(tile, acc, [&](uint32_t row, uint32_t col, const f4& v) {
-    put_symmetric(p, tile, row, col, get_pair4(a, row, col) * (S::b() * two_to(S::SB - S::SA)) + v * (S::c() * two_to(S::SB - 2 * S::SA)));
+  P::template sum<true, true>(a, a, tile, 0, ((S::TALL ? S::N : S::M) + 31) / 32, lds, acc);
+  P::each(tile, acc, [&](uint32_t row, uint32_t col, const f4& v) {
+    put_symmetric<S::HALF>(p, tile, row, col, get_pairs(a, row, col) * (S::b() * two_to(S::SB - S::SA)) + v * (S::c() * two_to(S::SB - 2 * S::SA)));
   });
 }
 
 // X <- a·X + B·X (TALL: X·B), into the other X, or as the result.
-template <class S, int T, int FROM, bool LAST>
+template <class S, int FROM, bool LAST>
 __device__ __forceinline__ void orth_apply(const Orth<S>& o, char* lds, uint32_t block) {
-  const TileAt tile = tile_at(block, S::MP / (32 * T), S::NP / (32 * T));
-  f4 acc[T][T];
+  using P = Tile<S::AKIND>;
+  const TileAt tile = tile_at(block, S::MP / P::ROWS, S::NP / P::COLS);
+  typename P::Sums acc;
   const Pairs x = o.xs(FROM), to = o.xs(1 - FROM);
-  if constexpr (S::TALL) gemm_f16x2_sum<2, 2, T, T, true, true>(x, o.bs(), tile.row * 32 * T, tile.col * 32 * T, 0, (S::N + 31) / 32, lds, acc);
-  else gemm_f16x2_sum<2, 2, T, T, true, false>(o.bs(), x, tile.row * 32 * T, tile.col * 32 * T, 0, (S::M + 31) / 32, lds, acc);
-  each_four<T>(tile, acc, [&](uint32_t row, uint32_t col, const f4& v) {
-    const f4 y = get_pair4(x, row, col) * (S::a() * (LAST ? two_to(-S::SX) : 1.f)) + v * (LAST ? two_to(-S::SB - S::SX) : two_to(-S::SB));
+  if constexpr (S::TALL) P::template sum<true, true>(x, o.bs(), tile, 0, (S::N + 31) / 32, lds, acc);
+  else P::template sum<true, false>(o.bs(), x, tile, 0, (S::M + 31) / 32, lds, acc);
+  P::each(tile, acc, [&](uint32_t row, uint32_t col, const f4& v) {
+    const f4 y = get_pairs(x, row, col) * (S::a() * (LAST ? two_to(-S::SX) : 1.f)) + v * (LAST ? two_to(-S::SB - S::SX) : two_to(-S::SB));
     if constexpr (LAST) {
       if (row >= S::M) return;
       float* q = o.out + (size_t)row * S::N + col;
@@ -196,9 +180,7 @@ __device__ __forceinline__ void orth_apply(const Orth<S>& o, char* lds, uint32_t
           if (col + e < S::N) q[e] = y[e];
       }
     } else {
-      h4 hi, lo;
-      split_pair(y, hi, lo);
-      put_pair4(to, row, col, hi, lo);
+      put_pairs(to, row, col, y);
     }
   });
 }

@@ -263,17 +263,26 @@ __device__ __forceinline__ void rotary(const float* __restrict__ x, const float*
   }
 }
 
-// out[e] = the sum of `blocks` partial rows, one workgroup of 256 a column chunk of 16: 16
-// threads a column, each its own rows in turn, their sums added in order.
+// out[e] = the sum of `blocks` partial rows: a workgroup of 1024 takes 16 columns, 64 threads a
+// column, each its own rows in turn, their sums added in order by eights.
 template <int DH>
 __device__ __forceinline__ void rotary_gain_sum(const float* __restrict__ partial, float* __restrict__ out, uint32_t blocks, float* scratch, uint32_t block) {
   const uint32_t e = block * 16u + threadIdx.x % 16u, part = threadIdx.x / 16u;
   float sum = 0.f;
-  if (e < DH) for (uint32_t k = part; k < blocks; k += 16u) sum += partial[(size_t)k * DH + e];
+  if (e < DH) {
+#pragma unroll 4
+    for (uint32_t k = part; k < blocks; k += 64u) sum += partial[(size_t)k * DH + e];
+  }
   scratch[threadIdx.x] = sum;
   __syncthreads();
-  if (part == 0 && e < DH) {
-    for (uint32_t p = 1; p < 16u; ++p) sum += scratch[p * 16u + threadIdx.x];
+  if (part < 8u) {
+    for (uint32_t p = part + 8u; p < 64u; p += 8u) sum += scratch[p * 16u + threadIdx.x % 16u];
+  }
+  __syncthreads();
+  if (part < 8u) scratch[threadIdx.x] = sum;
+  __syncthreads();
+  if (part == 0u && e < DH) {
+    for (uint32_t p = 1; p < 8u; ++p) sum += scratch[p * 16u + threadIdx.x];
     out[e] = sum;
   }
 }

@@ -98,11 +98,11 @@ function rotaryKernels(z, attrs, gain, grads, parts) {
     const e = entry(parts);
     workspace = blocks * z.DH * 4;
     kernels.push(kernel('rotsum', `#include "tcmi_rotary.h"
-extern "C" __global__ void __launch_bounds__(256) __KERNEL__(${e.sig}) {
-${e.open}  __shared__ float scratch[256];
+extern "C" __global__ void __launch_bounds__(1024) __KERNEL__(${e.sig}) {
+${e.open}  __shared__ float scratch[1024];
   tcmi::rotary_gain_sum<${z.DH}>(A.ws, ${e.out('dgain')}, ${blocks}u, scratch, blockIdx.x);
 }
-`, [ceil(z.DH, 16), 1, 1], 256));
+`, [ceil(z.DH, 16), 1, 1], 1024));
   }
   return { kernels, workspace };
 }
@@ -124,79 +124,120 @@ function lowerRotary(graph, node) {
 const LOSS_PIECE = 1 << 28;      // bytes of a piece's logits at most (a piece is 128 rows or more)
 const LOSS_PARTS = ['dh', 'dW', 'dbias', 'loss'];
 const CUS = 256;
+// tcmi_gemm_f16x2.h's tiles: rows, columns and threads of each kind.
+const SMALL = 0, SQUARE = 1, WIDE = 2, TALL = 3, FOUR = 4;
+const TILES = [[64, 64, 256], [128, 128, 256], [128, 256, 512], [256, 128, 512], [64, 64, 256]];
+/** The 64 x 64 tiles' kind for a product of so many workgroups and slices of K: 160 of 8 slices 6.3 us by SMALL, 9.3 by FOUR; 91 of 41 20.5 and 16.1. */
+const smallKind = (blocks, slices) => (blocks <= CUS && slices >= 32 ? FOUR : SMALL);
 
 const align = (n, to) => ceil(n, to) * to;
 
 /** The sizes of a loss's launch forming `parts`, and its workspace's layout. */
 function lossSizes(N, D, V, bias, parts, piece) {
   const grad = parts.some((p) => p !== 'loss');
-  const DP = align(D, 128), VP = align(V, 128);
+  // The large tiles are 128 x 256; padding of up to 256 columns and rows is little beside 2048 and 512.
+  const DP = align(D, 128), VP = align(V, V > 2048 ? 256 : 128), rows = N > 512 ? 256 : 128;
   // The rows of a piece: its logits, or without gradients a row's pair of statistics for each 64 columns.
   const row = grad ? 4 * VP : VP / 8;
-  const most = Math.max(128, Math.floor((piece || LOSS_PIECE) / row / 128) * 128);
-  const PIECES = ceil(align(N, 128), most), NP = align(ceil(N, PIECES), 128);
+  const most = Math.max(rows, Math.floor((piece || LOSS_PIECE) / row / rows) * rows);
+  const PIECES = ceil(align(N, rows), most), NP = align(ceil(N, PIECES), rows);
   const RB = NP * VP >= 2 ** 20 ? 32 : 16;
-  // K split over workgroups until two a CU have a tile; no chunk under 16 slices of 32.
-  const split = (tiles, slices) => {
-    const want = Math.max(1, Math.min(ceil(2 * CUS, tiles), Math.floor(slices / 16), 64));
-    const each = ceil(slices, want);
-    return { chunks: ceil(slices, each), each };
-  };
-  const hs = split(NP / 128 * (DP / 128), VP / 32), wsp = split(DP / 128 * (VP / 128), NP / 32);
-  const z = { N, D, V, DP, VP, NP, PIECES, RB, BIAS: bias, BLOCKS: 256, VECD: D % 4 === 0, VECV: V % 4 === 0,
-    HCHUNKS: hs.chunks, HK: hs.each, WCHUNKS: wsp.chunks, WK: wsp.each };
+  const clamp = (n, most) => Math.max(1, Math.min(Math.ceil(n), most));
+  // Large tiles unless they would leave much of the chip idle; the gradients' tiles and the chunks of K by time.
+  const large = VP % 256 === 0 && NP / 128 * (VP / 256) >= CUS / 2;
+  const LT = large ? 4 : 2;
+  const g = gradTiles(NP, DP, VP);
+  const CT = (() => { let t = 16; while (2 * t <= Math.min(256, VP / 8)) t *= 2; return t; })();
+  const z = { N, D, V, DP, VP, NP, PIECES, RB, CT, BIAS: bias, HBLOCKS: clamp(N * D / 4096, 256), WBLOCKS: clamp(D * V / 16384, 1024), GBLOCKS: clamp(N / 1024, 64),
+    PER: clamp((NP * PIECES * DP + DP * VP) / 4 / 256 / 1024, 16), LKIND: large ? WIDE : smallKind(NP / 64 * (VP / 64), DP / 32), HKIND: g.large ? TALL : SMALL, WKIND: g.large ? WIDE : SMALL, JOINED: !grad || VP / (16 * LT) > 32, VECD: D % 4 === 0, VECV: V % 4 === 0,
+    HCHUNKS: g.h.chunks, HK: g.h.each, WCHUNKS: g.w.chunks, WK: g.w.each };
   let at = 0;
   const place = (name, bytes) => { z[name] = at; at = align(at + bytes, 256); };
   place('STATE', 256);
-  place('MAXIMA', (2 * z.BLOCKS + 1) * 4);
+  place('MAXIMA', (z.HBLOCKS + z.WBLOCKS + z.GBLOCKS) * 4);
   place('HP', 4 * NP * PIECES * DP);
   place('WP', 4 * DP * VP);
-  place('STATS', 8 * NP * (VP / 64));
+  place('STATS', 8 * NP * (VP / (16 * LT)));
   place('PICKED', 4 * NP);
   place('ROWS', 8 * NP);
   if (grad) place('Z', 4 * NP * VP); else z.Z = 0;
   if (parts.includes('dh') || parts.includes('dW')) place('GP', 4 * NP * VP); else z.GP = 0;
   if (parts.includes('dbias')) place('SUMS', 4 * NP / RB * VP); else z.SUMS = 0;
-  if (parts.includes('dh') && hs.chunks > 1) place('HPART', 4 * hs.chunks * NP * DP); else z.HPART = 0;
-  if (parts.includes('dW') && wsp.chunks > 1) place('WPART', 4 * wsp.chunks * DP * VP); else z.WPART = 0;
+  if (parts.includes('dh') && g.h.chunks > 1) place('HPART', 4 * g.h.chunks * NP * DP); else z.HPART = 0;
+  if (parts.includes('dW') && g.w.chunks > 1) place('WPART', 4 * g.w.chunks * DP * VP); else z.WPART = 0;
   return { z, workspace: at, grad };
+}
+
+/**
+ * The tiles of dh [NP, d] over V and of dW [d, V] over NP, and the chunks their K is split
+ * into: those of the least estimated time, by how many rounds of workgroups the tiles of a product
+ * take (one of 256 x 128 a CU, two of 64 x 64). Measured (us): a slice of a large tile 1.2, of a small one
+ * 0.3; starting and ending a tile 6 and 4; a partial sum is written and read at 4 TB/s. Every
+ * choice depends on the sizes alone, not on which gradients a launch forms.
+ */
+function gradTiles(NP, DP, VP) {
+  const time = (large, tiles, slices, chunks, elements) => {
+    const each = ceil(slices, chunks), rounds = tiles * ceil(slices, each) / (large ? CUS : 2 * CUS);
+    return Math.max(1, rounds < 4 ? Math.ceil(rounds) : rounds) * (each * (large ? 1.2 : 0.3) + (large ? 6 : 4)) + (chunks > 1 ? 8 * chunks * elements / 4e6 + 3 : 0);
+  };
+  const best = (large, tiles, slices, elements) => {
+    let b = null;
+    for (let c = 1; c <= Math.min(64, Math.max(1, Math.floor(slices / 4))); c++) {
+      const t = time(large, tiles, slices, c, elements);
+      if (!b || t < b.t) b = { t, chunks: ceil(slices, ceil(slices, c)), each: ceil(slices, c) };
+    }
+    return b;
+  };
+  const of = (large) => {
+    const [hr, hc, wr, wc] = large ? [256, 128, 128, 256] : [64, 64, 64, 64];
+    const h = best(large, NP / hr * (DP / hc), VP / 32, NP * DP), w = best(large, DP / wr * (VP / wc), NP / 32, DP * VP);
+    return { large, h, w, t: h.t + w.t };
+  };
+  const small = of(false);
+  if (NP % 256 || VP % 256) return small;
+  const large = of(true);
+  return small.t < large.t ? small : large;
 }
 
 function lossKernels(N, D, V, bias, parts, joined, bytes) {
   const { z, workspace, grad } = lossSizes(N, D, V, bias, parts, bytes);
   const e = entry(joined ? parts : null);
   const has = (p) => parts.includes(p);
+  const counts = ['N', 'D', 'V', 'DP', 'VP', 'NP', 'PIECES', 'RB', 'CT', 'HBLOCKS', 'WBLOCKS', 'GBLOCKS', 'PER', 'HCHUNKS', 'HK', 'WCHUNKS', 'WK'];
   const sizes = Object.keys(z).map((k) => (typeof z[k] === 'boolean' ? `  static constexpr bool ${k} = ${z[k]};`
-    : `  static constexpr ${['N', 'D', 'V', 'DP', 'VP', 'NP', 'PIECES', 'RB', 'BLOCKS', 'HCHUNKS', 'HK', 'WCHUNKS', 'WK'].includes(k) ? 'uint32_t' : 'size_t'} ${k} = ${z[k]}${'u'};`)).join('\n');
-  const make = (kind, grid, threads, lds, call, least) => kernel(kind, `#include "tcmi_loss.h"
+    : k.endsWith('KIND') ? `  static constexpr int ${k} = ${z[k]};`
+      : `  static constexpr ${counts.includes(k) ? 'uint32_t' : 'size_t'} ${k} = ${z[k]}u;`)).join('\n');
+  const make = (kind, grid, threads, lds, call) => kernel(kind, `#include "tcmi_loss.h"
 struct __KERNEL___s {
 ${sizes}
 };
-extern "C" __global__ void __launch_bounds__(${threads}${least ? `, ${least}` : ''}) __KERNEL__(${e.sig}) {
+extern "C" __global__ void __launch_bounds__(${threads}) __KERNEL__(${e.sig}) {
 ${e.open}  const tcmi::Loss<__KERNEL___s> L{A.in[0], A.in[1], A.in[2], ${bias ? 'A.in[3]' : 'nullptr'}, ${grad ? `A.in[${bias ? 4 : 3}]` : 'nullptr'}, reinterpret_cast<char*>(A.ws)};
 ${lds ? `  __shared__ __attribute__((aligned(1024))) ${lds};\n` : ''}  tcmi::${call};
 }
 `, grid, threads);
-  const pool = 'char lds[tcmi::f16x2_lds<128, 128>()]';
   const S = '__KERNEL___s';
+  const [lr, lc, lt] = TILES[z.LKIND], [hr, hc, gt] = TILES[z.HKIND], [wr, wc] = TILES[z.WKIND];
+  const outs = (...names) => names.map((p) => (has(p) ? e.out(p) : 'nullptr')).join(', ');
   const HG = z.NP * z.PIECES * z.DP / 4, WG = z.DP * z.VP / 4;
-  const once = [make('lossmax', [2 * z.BLOCKS + (grad ? 1 : 0), 1, 1], 256, 'float scratch[4]', `loss_maxima<${S}, ${grad}>(L, scratch, blockIdx.x)`),
-    make('losssplit', [ceil(HG, 4096) + ceil(WG, 4096), 1, 1], 256, 'float scratch[4]', `loss_split<${S}, ${grad}>(L, scratch, blockIdx.x)`)];
-  const piece = [make('losslogits', [z.NP / 128 * (z.VP / 128), 1, 1], 256, pool, `loss_logits<${S}, ${grad}>(L, lds, blockIdx.x)`, 2),
-    make('lossjoin', [z.NP / 16, 1, 1], 256, 'float2 scratch[256]', `loss_join<${S}, ${has('loss')}, ${!grad}>(L, ${has('loss') ? e.out('loss') : 'nullptr'}, scratch, blockIdx.x)`)];
+  const once = [make('lossmax', [z.HBLOCKS + z.WBLOCKS + (grad ? z.GBLOCKS : 0), 1, 1], 256, 'float scratch[4]', `loss_maxima<${S}, ${grad}>(L, scratch, blockIdx.x)`),
+    make('losssplit', [ceil(HG, 256 * z.PER) + ceil(WG, 256 * z.PER), 1, 1], 256, 'float scratch[4]', `loss_split<${S}, ${grad}>(L, scratch, blockIdx.x)`)];
+  const piece = [make('losslogits', [z.NP / lr * (z.VP / lc), 1, 1], lt, `char lds[tcmi::Tile<${z.LKIND}>::LDS]`, `loss_logits<${S}, ${grad}>(L, lds, blockIdx.x)`)];
+  if (z.JOINED) {
+    piece.push(make('lossjoin', [z.NP / 16, 1, 1], 1024, 'float2 scratch[1024]',
+      `loss_join<${S}, ${has('loss')}, ${!grad}>(L, ${outs('loss')}, scratch, blockIdx.x)`));
+  }
   if (grad) {
-    piece.push(make('lossspread', [ceil(z.VP, 1024), z.NP / z.RB, 1], 256, `tcmi::f4 rows[${z.RB}]`,
-      `loss_spread<${S}, ${has('dh') || has('dW')}, ${has('dbias')}>(L, rows, blockIdx.x, blockIdx.y)`));
-    if (has('dh')) {
-      piece.push(make('lossdh', [z.NP / 128 * (z.DP / 128) * z.HCHUNKS, 1, 1], 256, pool, `loss_dh<${S}>(L, ${e.out('dh')}, lds, blockIdx.x)`, 2));
-      if (z.HCHUNKS > 1) piece.push(make('lossdhsum', [ceil(z.NP * z.DP / 4, 256), 1, 1], 256, null, `loss_dh_sum<${S}>(L, ${e.out('dh')}, blockIdx.x)`));
+    const [dh, dW, db] = ['dh', 'dW', 'dbias'].map(has);
+    piece.push(make('lossspread', [ceil(z.VP, 8 * z.CT), z.NP / z.RB, 1], 256, `tcmi::f4 rows[${z.RB + 512}]`,
+      `loss_spread<${S}, ${dh || dW}, ${db}, ${has('loss')}>(L, ${outs('loss')}, rows, blockIdx.x, blockIdx.y)`));
+    const blocks = (dh ? z.NP / hr * (z.DP / hc) * z.HCHUNKS : 0) + (dW ? z.DP / wr * (z.VP / wc) * z.WCHUNKS : 0) + (db ? z.VP / 16 : 0);
+    piece.push(make('lossgrads', [blocks, 1, 1], gt, `char lds[tcmi::GradTiles<${S}>::LDS]`, `loss_grads<${S}, ${dh}, ${dW}, ${db}>(L, ${outs('dh', 'dW', 'dbias')}, lds, blockIdx.x)`));
+    const sh = dh && z.HCHUNKS > 1, sw = dW && z.WCHUNKS > 1;
+    if (sh || sw) {
+      piece.push(make('losssums', [(sh ? ceil(z.NP * z.DP / 4, 256) : 0) + (sw ? ceil(z.D * z.VP / 4, 256) : 0), 1, 1], 256, null,
+        `loss_sums<${S}, ${sh}, ${sw}>(L, ${outs('dh', 'dW')}, blockIdx.x)`));
     }
-    if (has('dW')) {
-      piece.push(make('lossdw', [z.DP / 128 * (z.VP / 128) * z.WCHUNKS, 1, 1], 256, pool, `loss_dw<${S}>(L, ${e.out('dW')}, lds, blockIdx.x)`, 2));
-      if (z.WCHUNKS > 1) piece.push(make('lossdwsum', [ceil(z.D * z.VP / 4, 256), 1, 1], 256, null, `loss_dw_sum<${S}>(L, ${e.out('dW')}, blockIdx.x)`));
-    }
-    piece.push(make('lossend', [has('dbias') ? z.VP / 16 : 1, 1, 1], 256, has('dbias') ? 'float scratch[256]' : null,
-      `loss_end<${S}, ${has('dbias')}>(L, ${has('dbias') ? `${e.out('dbias')}, scratch` : 'nullptr, nullptr'}, blockIdx.x)`));
   }
   const kernels = once.slice();
   for (let p = 0; p < z.PIECES; p++) kernels.push(...piece);
@@ -228,10 +269,14 @@ function lowerOrthogonalize(graph, node) {
   const tall = M > N, s = Math.min(M, N), l = Math.max(M, N);
   // Tiles of 128, or of 64 where those leave much of the chip idle.
   const tiles = (t) => ceil(s, t) * ceil(l, t) * count;
-  const T = tiles(128) >= 2 * CUS ? 4 : 2;
-  const pad = 32 * T, MP = align(M, pad), NP = align(N, pad), SP = Math.min(MP, NP);
+  const square = tiles(128) >= 2 * CUS;
+  const pad = square ? 128 : 64, MP = align(M, pad), NP = align(N, pad), SP = Math.min(MP, NP);
+  const n = SP / pad, upper = n * (n + 1) / 2, all = MP / pad * (NP / pad);
+  const kind = (blocks, K) => (square ? SQUARE : smallKind(blocks * count, K / 32));
+  const half = square || n * n * count > CUS, tilesOf = half ? upper : n * n;
+  const GKIND = kind(tilesOf, l), BKIND = kind(tilesOf, s), AKIND = kind(all, s);
   const top = singularBound(node.attrs);
-  const z = { M, N, MP, NP, SP, TALL: tall, VEC: N % 4 === 0, BLOCKS: Math.min(256, ceil(M * N, 4096)),
+  const z = { M, N, MP, NP, SP, GKIND, BKIND, AKIND, HALF: half, TALL: tall, VEC: N % 4 === 0, BLOCKS: Math.min(256, ceil(M * N, 4096)),
     SX: fits(top), SA: fits(top ** 2), SB: Math.max(-60, Math.min(60, fits(Math.max(Math.abs(b) * top ** 2 + Math.abs(c) * top ** 4, 2 ** -40)))) };
   let at = 0;
   const place = (name, bytes) => { z[name] = at; at = align(at + bytes, 256); };
@@ -242,10 +287,10 @@ function lowerOrthogonalize(graph, node) {
   place('B', steps > 0 ? 4 * SP * SP : 0);
   z.PER = at;
   const sizes = Object.keys(z).map((k) => (typeof z[k] === 'boolean' ? `  static constexpr bool ${k} = ${z[k]};`
-    : ['SX', 'SA', 'SB'].includes(k) ? `  static constexpr int ${k} = ${z[k]};`
+    : ['GKIND', 'BKIND', 'AKIND', 'SX', 'SA', 'SB'].includes(k) ? `  static constexpr int ${k} = ${z[k]};`
       : `  static constexpr ${['M', 'N', 'MP', 'NP', 'SP', 'BLOCKS'].includes(k) ? 'uint32_t' : 'size_t'} ${k} = ${z[k]}u;`)).join('\n');
   const S = '__KERNEL___s';
-  const make = (kind, blocks, lds, call) => kernel(kind, `#include "tcmi_orthogonalize.h"
+  const make = (kind, blocks, threads, lds, call) => kernel(kind, `#include "tcmi_orthogonalize.h"
 struct __KERNEL___s {
 ${sizes}
   static __device__ __forceinline__ float a() { return static_cast<float>(${double(a)}); }
@@ -253,20 +298,19 @@ ${sizes}
   static __device__ __forceinline__ float c() { return static_cast<float>(${double(c)}); }
   static __device__ __forceinline__ double eps() { return ${double(eps)}; }
 };
-extern "C" __global__ void __launch_bounds__(256, 2) __KERNEL__(const TcmiArgs A) {
+extern "C" __global__ void __launch_bounds__(${threads}) __KERNEL__(const TcmiArgs A) {
   const tcmi::Orth<__KERNEL___s> o(A.in[0], A.out, A.ws, blockIdx.z);
   __shared__ __attribute__((aligned(1024))) ${lds};
   tcmi::${call};
 }
-`, [blocks, 1, count], 256);
-  const pool = `char lds[tcmi::f16x2_lds<${32 * T}, ${32 * T}>()]`;
-  const n = SP / pad, upper = n * (n + 1) / 2;
-  const kernels = [make('orthnorm', z.BLOCKS, 'double scratch[4]', `orth_norm<${S}>(o, scratch, blockIdx.x)`),
-    make('orthsplit', ceil(MP * NP, 4096), 'double scratch[4]', `orth_split<${S}, ${steps === 0}>(o, scratch, blockIdx.x)`)];
+`, [blocks, 1, count], threads);
+  const pool = (k) => `char lds[tcmi::Tile<${k}>::LDS]`;
+  const kernels = [make('orthnorm', z.BLOCKS, 256, 'double scratch[4]', `orth_norm<${S}>(o, scratch, blockIdx.x)`),
+    make('orthsplit', ceil(MP * NP, 4096), 256, 'double scratch[4]', `orth_split<${S}, ${steps === 0}>(o, scratch, blockIdx.x)`)];
   for (let k = 0; k < steps; k++) {
-    kernels.push(make('orthgram', upper, pool, `orth_gram<${S}, ${T}, ${k % 2}>(o, lds, blockIdx.x)`));
-    kernels.push(make('orthpoly', upper, pool, `orth_poly<${S}, ${T}>(o, lds, blockIdx.x)`));
-    kernels.push(make('orthapply', MP / pad * (NP / pad), pool, `orth_apply<${S}, ${T}, ${k % 2}, ${k === steps - 1}>(o, lds, blockIdx.x)`));
+    kernels.push(make('orthgram', tilesOf, TILES[GKIND][2], pool(GKIND), `orth_gram<${S}, ${k % 2}>(o, lds, blockIdx.x)`));
+    kernels.push(make('orthpoly', tilesOf, TILES[BKIND][2], pool(BKIND), `orth_poly<${S}>(o, lds, blockIdx.x)`));
+    kernels.push(make('orthapply', all, TILES[AKIND][2], pool(AKIND), `orth_apply<${S}, ${k % 2}, ${k === steps - 1}>(o, lds, blockIdx.x)`));
   }
   return { kind: 'orthogonalize', kernels, workspace: count * z.PER, flops: count * steps * (3 * s * s * l + s ** 3) };
 }
