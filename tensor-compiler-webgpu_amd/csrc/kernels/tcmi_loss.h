@@ -300,8 +300,13 @@ __device__ __forceinline__ void loss_spread(const Loss<S>& L, float* out, f4* ro
       if constexpr (S::JOINED) {
         x = reinterpret_cast<const float2*>(L.at(S::ROWS))[row];
       } else {
+        // As `join` adds them: every eighth in turn, then those eight.
         RowSum sum;
-        for (uint32_t k = 0; k < loss_parts<S>(); ++k) sum.add(reinterpret_cast<const float2*>(L.at(S::STATS))[(size_t)k * S::NP + row]);
+        for (uint32_t p = 0; p < 8 && p < loss_parts<S>(); ++p) {
+          RowSum part;
+          for (uint32_t k = p; k < loss_parts<S>(); k += 8) part.add(reinterpret_cast<const float2*>(L.at(S::STATS))[(size_t)k * S::NP + row]);
+          sum.add(make_float2(part.m, part.s));
+        }
         x = make_float2(sum.m, 1.f / sum.s);
         if constexpr (LOSS) {
           if (bx == 0) out[r] = (sum.m - L.at(S::PICKED)[row]) + op_log(sum.s);

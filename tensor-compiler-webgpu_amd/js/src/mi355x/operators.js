@@ -143,13 +143,14 @@ function lossSizes(N, D, V, bias, parts, piece) {
   const PIECES = ceil(align(N, rows), most), NP = align(ceil(N, PIECES), rows);
   const RB = NP * VP >= 2 ** 20 ? 32 : 16;
   const clamp = (n, most) => Math.max(1, Math.min(Math.ceil(n), most));
-  // Large tiles unless they would leave much of the chip idle; the gradients' tiles and the chunks of K by time.
-  const large = VP % 256 === 0 && NP / 128 * (VP / 256) >= CUS / 2;
+  // Large tiles unless they would leave much of the chip idle, by all rows: a loss has the same bits whatever its
+  // pieces. The gradients' tiles and the chunks of K by time.
+  const large = VP % 256 === 0 && rows === 256 && align(N, 256) / 128 * (VP / 256) >= CUS / 2;
   const LT = large ? 4 : 2;
   const g = gradTiles(NP, DP, VP);
   const CT = (() => { let t = 16; while (2 * t <= Math.min(256, VP / 8)) t *= 2; return t; })();
   const z = { N, D, V, DP, VP, NP, PIECES, RB, CT, BIAS: bias, HBLOCKS: clamp(N * D / 4096, 256), WBLOCKS: clamp(D * V / 16384, 1024), GBLOCKS: clamp(N / 1024, 64),
-    PER: clamp((NP * PIECES * DP + DP * VP) / 4 / 256 / 1024, 16), LKIND: large ? WIDE : smallKind(NP / 64 * (VP / 64), DP / 32), HKIND: g.large ? TALL : SMALL, WKIND: g.large ? WIDE : SMALL, JOINED: !grad || VP / (16 * LT) > 32, VECD: D % 4 === 0, VECV: V % 4 === 0,
+    PER: clamp((NP * PIECES * DP + DP * VP) / 4 / 256 / 1024, 16), LKIND: large ? WIDE : smallKind(align(N, 64) / 64 * (VP / 64), DP / 32), HKIND: g.large ? TALL : SMALL, WKIND: g.large ? WIDE : SMALL, JOINED: !grad || VP / (16 * LT) > 32, VECD: D % 4 === 0, VECV: V % 4 === 0,
     HCHUNKS: g.h.chunks, HK: g.h.each, WCHUNKS: g.w.chunks, WK: g.w.each };
   let at = 0;
   const place = (name, bytes) => { z[name] = at; at = align(at + bytes, 256); };

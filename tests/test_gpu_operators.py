@@ -64,7 +64,8 @@ def check(c, inputs, entry, b):
             print(f"{c['name']} {n['op']} {n['attrs'].get('part', '')}: {worst:.3f} of what is allowed")
     for k, h in entry["gpuPerf"].items():
         perf, plain = b.arr(h), b.arr(entry["gpuFused"][k])
-        assert np.array_equal(perf.view(np.uint32), plain.view(np.uint32)), (c["name"], k)
+        same = np.array_equal(perf.view(np.uint32), plain.view(np.uint32))
+        assert same, (c["name"], graph["nodes"][int(k)]["op"], np.flatnonzero(perf.view(np.uint32) != plain.view(np.uint32))[:5])
     del values
 
 
