@@ -275,6 +275,15 @@ function precompileGroup(group, arch, shard, shards) {
       const lists = [lowerMI355X(f.graph, { perf: true, keep: keep.map((id) => f.index.get(id)), tuning })];
       n += precompile(MEASURED.includes(c) ? lists : lists.concat([lowerMI355X(f.graph, { tuning })]), arch);
     }
+    // The training steps that run them together, as the trainer's tests do.
+    const { modelStep } = require('../src/builders/models');
+    const { fusedStep } = require('../src/mi355x/trainer');
+    const cfg = { T: 32, d: 64, H: 4, dh: 16, L: 2, ff: 160, positions: 'rotary', qkNorm: true, targets: 'classes' };
+    for (const attention of [false, true]) {
+      if ((shard || 0) !== (attention ? 1 : 0) % (shards || 1)) continue;
+      const fs = fusedStep(modelStep({ model: 'transformer', B: 5, V: 301, opt: 'muon', cfg }).step, { attention });
+      n += precompile([fs.lowered], arch) + precompile([fs.checked], arch);
+    }
     return n;
   }
   if (group === 'scratch') {

@@ -27,7 +27,8 @@ function randomTokens(B, T, V, seed) {
 
 /**
  * { step, params, state, batch(k) -> {x, y}, info } for a model request
- * { model, B?, V?, seed?, cfg? (overrides of the transformer config), firstBatch?, batches? }.
+ * { model, B?, V?, seed?, cfg? (overrides of the transformer config), opt? (the transformer's
+ * optimizer: 'sgd', 'adam', 'muon', or one given whole; default sgd), firstBatch?, batches? }.
  */
 function modelStep(req) {
   const model = req.model || 'mlp';
@@ -41,10 +42,13 @@ function modelStep(req) {
     const cfg = Object.assign({}, tf.C5_CONFIG, req.cfg || {});
     const V = req.V || 96, B = req.B || 64, seed = req.seed || 0;
     const lr = req.lr || C5_LR;
-    const step = tf.buildStep(V, B, cfg, { kind: 'sgd', lr });
+    const opt = typeof req.opt === 'object' ? req.opt : { sgd: { kind: 'sgd', lr }, adam: tf.ADAM_3B, muon: tf.MUON }[req.opt || 'sgd'];
+    if (!opt) throw new Error(`unknown optimizer '${req.opt}'`);
+    const step = tf.buildStep(V, B, cfg, opt);
     const params = tf.initNormal(V, seed, 0.02, cfg);
-    const batch = (k) => tf.encodeBatch(randomTokens(B, cfg.T, V, seed * 1000 + (k || 0)), V, cfg.T);
-    return { step, params, state: {}, batch, info: { config: 'C5', V, B, cfg, lr, init: 'N(0, 0.02) weights, LayerNorm gains 1 and biases 0' } };
+    const state = tf.initialState(step.names, step.shapes, opt);
+    const batch = (k) => tf.encodeBatch(randomTokens(B, cfg.T, V, seed * 1000 + (k || 0)), V, cfg.T, cfg.targets);
+    return { step, params, state, batch, info: { config: 'C5', V, B, cfg, lr, init: 'N(0, 0.02) weights, LayerNorm gains 1 and biases 0' } };
   }
   if (model === 'transformer-ref') {
     const cfg = Object.assign({}, tf.REFERENCE_CONFIG, req.cfg || {});
@@ -78,8 +82,8 @@ function modelForward(req) {
   const V = req.V || (ref ? 16 : 96), B = req.B || (ref ? 4 : 64), seed = req.seed || (ref ? 1 : 0);
   const fwd = tf.buildForward(V, B, cfg);
   const params = ref ? tf.initParams(V, seed, cfg) : tf.initNormal(V, seed, 0.02, cfg);
-  const batch = (k) => (req.firstBatch && !k ? tf.encodeBatch(req.firstBatch, V, cfg.T)
-    : tf.encodeBatch(randomTokens(B, cfg.T, V, seed * 1000 + (k || 0)), V, cfg.T));
+  const batch = (k) => (req.firstBatch && !k ? tf.encodeBatch(req.firstBatch, V, cfg.T, cfg.targets)
+    : tf.encodeBatch(randomTokens(B, cfg.T, V, seed * 1000 + (k || 0)), V, cfg.T, cfg.targets));
   return { fwd, params, batch, info: { config: ref ? 'reference transformer' : 'C5', V, B, cfg } };
 }
 

@@ -62,6 +62,9 @@ function formTransposedProducts(graph, keep, origin, index) {
   return count;
 }
 
+/** The nodes of a step that are read: the loss, the logits (null where the step keeps none) and every output. */
+const keptOf = (step) => (step.logits === null ? [step.loss] : [step.loss, step.logits]).concat(Object.values(step.outputs));
+
 /**
  * Fuse and lower a step from the builders ({ graph, loss, logits, inputs, outputs, cotangent, ... }).
  * `lowered` is the perf lowering the trainer runs (reshapes share buffers,
@@ -73,13 +76,13 @@ function formTransposedProducts(graph, keep, origin, index) {
  */
 function fusedStep(step, options) {
   const o = options || {};
-  const keep = [step.loss, step.logits].concat(Object.values(step.outputs));
+  const keep = keptOf(step);
   let f = fuse(step.graph, { keep, sabotage: o.passSabotage });
   formTransposedProducts(f.graph, new Set(keep.map((id) => f.index.get(id))), f.origin, f.index);
   // With `attention`, each attention and its gradient take the attention extension's
   // nodes (fusion/attention.js fuseAttentionTraining); off, the contract's partition.
   if (o.attention) f = fuseAttentionTraining(f, { keep });
-  const at = (id) => f.index.get(id);
+  const at = (id) => (id === null ? null : f.index.get(id));
   const remap = (m) => { const r = {}; for (const k of Object.keys(m)) r[k] = at(m[k]); return r; };
   const checked = lowerMI355X(f.graph, { sabotage: o.sabotage, tuning: o.tuning });
   const lowered = o.perf === false ? checked
@@ -103,9 +106,9 @@ function fusedStep(step, options) {
  */
 function fusedForward(fwd, options) {
   const o = options || {};
-  const keep = [fwd.logits, fwd.loss];
+  const keep = fwd.logits === null ? [fwd.loss] : [fwd.logits, fwd.loss];
   const f = fuse(fwd.graph, { keep, sabotage: o.passSabotage });
-  const at = (id) => f.index.get(id);
+  const at = (id) => (id === null ? null : f.index.get(id));
   const checked = lowerMI355X(f.graph, { sabotage: o.sabotage, tuning: o.tuning });
   const lowered = o.perf === false ? checked
     : lowerMI355X(f.graph, { sabotage: o.sabotage, tuning: o.tuning, perf: true, keep: keep.map(at), absorb: true });
@@ -126,7 +129,7 @@ class HipTrainer {
     this.step = step;
     this.graph = !!o.graph;
     if (this.graph && o.streams > 1) throw new Error('graph replay and several streams are not combined (multi-stream capture is switched off)');
-    const keep = [step.loss, step.logits].concat(Object.values(step.outputs));
+    const keep = keptOf(step);
     const first = runner.prepare(step.graph, step.lowered, Object.assign(o.arena ? { arena: { keep } } : {}, { streams: o.streams }));
     const cot = step.graph.inputId(step.cotangent);
     if (cot === undefined) throw new Error(`the step has no cotangent input '${step.cotangent}'`);
