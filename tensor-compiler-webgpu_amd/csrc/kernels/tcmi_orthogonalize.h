@@ -23,7 +23,7 @@
 namespace tcmi {
 
 // S: the sizes of one launch as constants of its text: M, N; GKIND, BKIND, AKIND of tiles for A, B and X; HALF; MP, NP padded to whole tiles (SP: the
-// smaller's); TALL; BLOCKS of the norm; SX, SA, SB exponents of the scales; VEC: N a multiple of 4; a(), b(), c(), eps().
+// smaller's); GSPLIT, GCHUNKS, GEACH and BSPLIT, BCHUNKS, BEACH: A's and B's split tiles; TALL; BLOCKS of the norm; SX, SA, SB exponents of the scales; VEC: N a multiple of 4; a(), b(), c(), eps().
 // WS: byte offsets in one matrix's workspace, PER bytes.
 template <class S>
 struct Orth {
@@ -134,28 +134,75 @@ __device__ __forceinline__ void put_symmetric(const Pairs& p, const TileAt& tile
 
 constexpr float two_to(int e) { return e < 0 ? 1.f / static_cast<float>(1ull << -e) : static_cast<float>(1ull << e); }
 
-// A = X·Xᵀ (TALL: Xᵀ·X).
-template <class S, int FROM>
-__device__ __forceinline__ void orth_gram(const Orth<S>& o, char* lds, uint32_t block) {
-  using P = Tile<S::GKIND>;
-  const TileAt tile = S::HALF ? upper_tile(block, S::SP / P::ROWS) : tile_at(block, S::SP / P::ROWS, S::SP / P::ROWS);
+// One of the two symmetric products: POLY B = b·A + c·A·A, else A = X·Xᵀ (TALL: Xᵀ·X) of X number FROM.
+template <class S, bool POLY, int FROM>
+struct Symmetric {
+  using P = Tile<POLY ? S::BKIND : S::GKIND>;
+  static constexpr bool KC = POLY || !S::TALL;
+  static constexpr uint32_t SLICES = ((POLY == S::TALL ? S::N : S::M) + 31) / 32;
+  static constexpr uint32_t LINES = S::SP / P::ROWS, TILES = S::HALF ? LINES * (LINES + 1) / 2 : LINES * LINES;
+  // The last SPLIT tiles are summed in CHUNKS chunks of EACH slices.
+  static constexpr uint32_t SPLIT = POLY ? S::BSPLIT : S::GSPLIT, CHUNKS = POLY ? S::BCHUNKS : S::GCHUNKS, EACH = POLY ? S::BEACH : S::GEACH;
+
+  static __device__ __forceinline__ TileAt tile(uint32_t id) { return S::HALF ? upper_tile(id, LINES) : tile_at(id, LINES, LINES); }
+  // A chunk's sums of fragment (i, 0) of this lane.
+  static __device__ __forceinline__ f4* part(const Orth<S>& o, uint32_t split, uint32_t chunk, int i) {
+    return reinterpret_cast<f4*>(o.ws + S::PART) + ((size_t)(chunk * SPLIT + split) * (P::TI * P::TJ) + i * P::TJ) * P::THREADS + threadIdx.x;
+  }
+  static __device__ __forceinline__ void put(const Orth<S>& o, const TileAt& at, uint32_t row, uint32_t col, const f4& v) {
+    if constexpr (POLY) {
+      put_symmetric<S::HALF>(o.bs(), at, row, col, get_pairs(o.as(), row, col) * (S::b() * two_to(S::SB - S::SA)) + v * (S::c() * two_to(S::SB - 2 * S::SA)));
+    } else {
+      put_symmetric<S::HALF>(o.as(), at, row, col, v * two_to(S::SA - 2 * S::SX));
+    }
+  }
+};
+
+template <class S, bool POLY, int FROM>
+__device__ __forceinline__ void orth_symmetric(const Orth<S>& o, char* lds, uint32_t block) {
+  using Y = Symmetric<S, POLY, FROM>;
+  using P = typename Y::P;
+  uint32_t id = block, k = 0, slices = Y::SLICES, chunk = 0;
+  const bool split = Y::SPLIT > 0 && block >= Y::TILES - Y::SPLIT;
+  if (split) {
+    constexpr uint32_t each = Y::SPLIT > 0 ? Y::SPLIT : 1u;
+    chunk = (block - (Y::TILES - Y::SPLIT)) / each;
+    id = block - chunk * each;
+    k = chunk * Y::EACH;
+    slices = min(Y::EACH, Y::SLICES - k);
+  }
+  const TileAt at = Y::tile(id);
   typename P::Sums acc;
-  P::template sum<!S::TALL, !S::TALL>(o.xs(FROM), o.xs(FROM), tile, 0, ((S::TALL ? S::M : S::N) + 31) / 32, lds, acc);
-  const Pairs p = o.as();
-  P::each(tile, acc, [&](uint32_t row, uint32_t col, const f4& v) { put_symmetric<S::HALF>(p, tile, row, col, v * two_to(S::SA - 2 * S::SX)); });
+  const Pairs x = POLY ? o.as() : o.xs(FROM);
+  P::template sum<Y::KC, Y::KC>(x, x, at, 32 * k, slices, lds, acc);
+  if (split) {
+#pragma unroll
+    for (int i = 0; i < P::TI; ++i)
+#pragma unroll
+      for (int j = 0; j < P::TJ; ++j) Y::part(o, id - (Y::TILES - Y::SPLIT), chunk, i)[j * P::THREADS] = acc[i][j];
+    return;
+  }
+  P::each(at, acc, [&](uint32_t row, uint32_t col, const f4& v) { Y::put(o, at, row, col, v); });
 }
 
-// B = b·A + c·A·A.
-template <class S>
-__device__ __forceinline__ void orth_poly(const Orth<S>& o, char* lds, uint32_t block) {
-  using P = Tile<S::BKIND>;
-  const TileAt tile = S::HALF ? upper_tile(block, S::SP / P::ROWS) : tile_at(block, S::SP / P::ROWS, S::SP / P::ROWS);
-  typename P::Sums acc;
-  const Pairs a = o.as(), p = o.bs();
-  P::template sum<true, true>(a, a, tile, 0, ((S::TALL ? S::N : S::M) + 31) / 32, lds, acc);
-  P::each(tile, acc, [&](uint32_t row, uint32_t col, const f4& v) {
-    put_symmetric<S::HALF>(p, tile, row, col, get_pairs(a, row, col) * (S::b() * two_to(S::SB - S::SA)) + v * (S::c() * two_to(S::SB - 2 * S::SA)));
-  });
+// The sums of the split tiles, chunk after chunk: 16 rows of each wavefront a workgroup.
+template <class S, bool POLY>
+__device__ __forceinline__ void orth_join(const Orth<S>& o, uint32_t block) {
+  using Y = Symmetric<S, POLY, 0>;
+  using P = typename Y::P;
+  const uint32_t split = block / P::TI;
+  const int i = block % P::TI;
+  const TileAt at = Y::tile(Y::TILES - Y::SPLIT + split);
+  f4 v[P::TJ];
+#pragma unroll
+  for (int j = 0; j < P::TJ; ++j) v[j] = Y::part(o, split, 0, i)[j * P::THREADS];
+#pragma unroll 2
+  for (uint32_t c = 1; c < Y::CHUNKS; ++c) {
+#pragma unroll
+    for (int j = 0; j < P::TJ; ++j) v[j] += Y::part(o, split, c, i)[j * P::THREADS];
+  }
+#pragma unroll
+  for (int j = 0; j < P::TJ; ++j) Y::put(o, at, P::row(at) + 16 * i, P::col(at) + 16 * j, v[j]);
 }
 
 // X <- a·X + B·X (TALL: X·B), into the other X, or as the result.

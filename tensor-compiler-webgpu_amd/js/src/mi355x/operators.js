@@ -130,6 +130,9 @@ const TILES = [[64, 64, 256], [128, 128, 256], [128, 256, 512], [256, 128, 512],
 /** The 64 x 64 tiles' kind for a product of so many workgroups and slices of K: 160 of 8 slices 6.3 us by SMALL, 9.3 by FOUR; 91 of 41 20.5 and 16.1. */
 const smallKind = (blocks, slices) => (blocks <= CUS && slices >= 32 ? FOUR : SMALL);
 
+/** A product's kernel keeps two wavefronts a SIMD, 256 registers each. */
+const bounds = (threads, lds) => (/Tile/.test(lds || '') ? ', 2' : '');
+
 const align = (n, to) => ceil(n, to) * to;
 
 /** The sizes of a loss's launch forming `parts`, and its workspace's layout. */
@@ -212,7 +215,7 @@ function lossKernels(N, D, V, bias, parts, joined, bytes) {
 struct __KERNEL___s {
 ${sizes}
 };
-extern "C" __global__ void __launch_bounds__(${threads}) __KERNEL__(${e.sig}) {
+extern "C" __global__ void __launch_bounds__(${threads}${bounds(threads, lds)}) __KERNEL__(${e.sig}) {
 ${e.open}  const tcmi::Loss<__KERNEL___s> L{A.in[0], A.in[1], A.in[2], ${bias ? 'A.in[3]' : 'nullptr'}, ${grad ? `A.in[${bias ? 4 : 3}]` : 'nullptr'}, reinterpret_cast<char*>(A.ws)};
 ${lds ? `  __shared__ __attribute__((aligned(1024))) ${lds};\n` : ''}  tcmi::${call};
 }
@@ -260,6 +263,17 @@ function lowerLoss(graph, node, tuning) {
 
 // ---- orthogonalize -------------------------------------------------------------------------
 
+/**
+ * Which of a symmetric product's tiles are split along K: those left over when the rest fill the chip (two workgroups a CU)
+ * a whole number of times, into as many chunks of 8 slices or more as fill it once more.
+ */
+function splitTiles(kind, tiles, slices) {
+  const split = tiles % (2 * CUS), chunks = kind === SQUARE && split ? Math.min(Math.floor(2 * CUS / split), Math.floor(slices / 8)) : 1;
+  if (chunks < 2) return { split: 0, chunks: 1, each: slices };
+  const each = ceil(slices, chunks);
+  return { split, chunks: ceil(slices, each), each };
+}
+
 /** The largest exponent that keeps values up to `top` within half's range. */
 const fits = (top) => Math.floor(Math.log2(60000 / top));
 
@@ -275,9 +289,13 @@ function lowerOrthogonalize(graph, node) {
   const n = SP / pad, upper = n * (n + 1) / 2, all = MP / pad * (NP / pad);
   const kind = (blocks, K) => (square ? SQUARE : smallKind(blocks * count, K / 32));
   const half = square || n * n * count > CUS, tilesOf = half ? upper : n * n;
-  const GKIND = kind(tilesOf, l), BKIND = kind(tilesOf, s), AKIND = kind(all, s);
+  const GKIND = kind(tilesOf, l), BKIND = kind(tilesOf, s);
+  const AKIND = square && NP % 256 === 0 ? WIDE : square && MP % 256 === 0 ? TALL : kind(all, s);
+  const ablocks = MP / TILES[AKIND][0] * (NP / TILES[AKIND][1]);
+  const G = splitTiles(GKIND, tilesOf, ceil(l, 32)), B = splitTiles(BKIND, tilesOf, ceil(s, 32));
   const top = singularBound(node.attrs);
   const z = { M, N, MP, NP, SP, GKIND, BKIND, AKIND, HALF: half, TALL: tall, VEC: N % 4 === 0, BLOCKS: Math.min(256, ceil(M * N, 4096)),
+    GSPLIT: G.split, GCHUNKS: G.chunks, GEACH: G.each, BSPLIT: B.split, BCHUNKS: B.chunks, BEACH: B.each,
     SX: fits(top), SA: fits(top ** 2), SB: Math.max(-60, Math.min(60, fits(Math.max(Math.abs(b) * top ** 2 + Math.abs(c) * top ** 4, 2 ** -40)))) };
   let at = 0;
   const place = (name, bytes) => { z[name] = at; at = align(at + bytes, 256); };
@@ -286,10 +304,12 @@ function lowerOrthogonalize(graph, node) {
   place('X1', steps > 1 ? 4 * MP * NP : 0);
   place('A', steps > 0 ? 4 * SP * SP : 0);
   place('B', steps > 0 ? 4 * SP * SP : 0);
+  const partial = (kind, t) => 4 * TILES[kind][0] * TILES[kind][1] * t.split * t.chunks;
+  place('PART', steps > 0 ? Math.max(partial(GKIND, G), partial(BKIND, B)) : 0);
   z.PER = at;
   const sizes = Object.keys(z).map((k) => (typeof z[k] === 'boolean' ? `  static constexpr bool ${k} = ${z[k]};`
     : ['GKIND', 'BKIND', 'AKIND', 'SX', 'SA', 'SB'].includes(k) ? `  static constexpr int ${k} = ${z[k]};`
-      : `  static constexpr ${['M', 'N', 'MP', 'NP', 'SP', 'BLOCKS'].includes(k) ? 'uint32_t' : 'size_t'} ${k} = ${z[k]}u;`)).join('\n');
+      : `  static constexpr ${/^([MNS]P?|BLOCKS|[GB](SPLIT|CHUNKS|EACH))$/.test(k) ? 'uint32_t' : 'size_t'} ${k} = ${z[k]}u;`)).join('\n');
   const S = '__KERNEL___s';
   const make = (kind, blocks, threads, lds, call) => kernel(kind, `#include "tcmi_orthogonalize.h"
 struct __KERNEL___s {
@@ -299,19 +319,21 @@ ${sizes}
   static __device__ __forceinline__ float c() { return static_cast<float>(${double(c)}); }
   static __device__ __forceinline__ double eps() { return ${double(eps)}; }
 };
-extern "C" __global__ void __launch_bounds__(${threads}) __KERNEL__(const TcmiArgs A) {
+extern "C" __global__ void __launch_bounds__(${threads}${bounds(threads, lds)}) __KERNEL__(const TcmiArgs A) {
   const tcmi::Orth<__KERNEL___s> o(A.in[0], A.out, A.ws, blockIdx.z);
-  __shared__ __attribute__((aligned(1024))) ${lds};
-  tcmi::${call};
+${lds ? `  __shared__ __attribute__((aligned(1024))) ${lds};\n` : ''}  tcmi::${call};
 }
 `, [blocks, 1, count], threads);
   const pool = (k) => `char lds[tcmi::Tile<${k}>::LDS]`;
   const kernels = [make('orthnorm', z.BLOCKS, 256, 'double scratch[4]', `orth_norm<${S}>(o, scratch, blockIdx.x)`),
     make('orthsplit', ceil(MP * NP, 4096), 256, 'double scratch[4]', `orth_split<${S}, ${steps === 0}>(o, scratch, blockIdx.x)`)];
   for (let k = 0; k < steps; k++) {
-    kernels.push(make('orthgram', tilesOf, TILES[GKIND][2], pool(GKIND), `orth_gram<${S}, ${k % 2}>(o, lds, blockIdx.x)`));
-    kernels.push(make('orthpoly', tilesOf, TILES[BKIND][2], pool(BKIND), `orth_poly<${S}>(o, lds, blockIdx.x)`));
-    kernels.push(make('orthapply', all, TILES[AKIND][2], pool(AKIND), `orth_apply<${S}, ${k % 2}, ${k === steps - 1}>(o, lds, blockIdx.x)`));
+    for (const [poly, kind, t] of [[false, GKIND, G], [true, BKIND, B]]) {
+      const from = poly ? 0 : k % 2, name = poly ? 'poly' : 'gram';
+      kernels.push(make(`orth${name}`, tilesOf + t.split * (t.chunks - 1), TILES[kind][2], pool(kind), `orth_symmetric<${S}, ${poly}, ${from}>(o, lds, blockIdx.x)`));
+      if (t.split) kernels.push(make(`orthjoin${name}`, t.split * (TILES[kind][0] === 128 ? 4 : kind === FOUR ? 1 : 2), TILES[kind][2], null, `orth_join<${S}, ${poly}>(o, blockIdx.x)`));
+    }
+    kernels.push(make('orthapply', ablocks, TILES[AKIND][2], pool(AKIND), `orth_apply<${S}, ${k % 2}, ${k === steps - 1}>(o, lds, blockIdx.x)`));
   }
   return { kind: 'orthogonalize', kernels, workspace: count * z.PER, flops: count * steps * (3 * s * s * l + s ** 3) };
 }
