@@ -178,4 +178,25 @@ __device__ __forceinline__ float block_reduce(float v, float* scratch) {
   return r;
 }
 
+// A workgroup's (x, y, z) place in its launch's grid.
+struct Wg {
+  uint32_t x, y, z;
+};
+
+// Workgroups grouped by XCD for split-K launches. The G = gridDim.x * gridDim.y tiles
+// of one z index (one K chunk of one product) read the same A and B panels; the
+// hardware hands a launch's workgroups to the 8 XCDs in turn by linear id L, so L
+// runs on XCD L % 8, and consecutive tiles would land on 8 different L2 caches.
+// Here z index q = L % 8 + 8 * (L / (8 * G)) and tile t = (L / 8) % G: every tile of
+// one z index runs on one XCD. A bijection of [0, G * gridDim.z) when gridDim.z is a
+// multiple of 8 (launch order kept otherwise), so every (tile, z) is computed once,
+// by the same code: only which workgroup computes it changes, not the result.
+__device__ __forceinline__ Wg xcd_grouped() {
+  const uint32_t gx = gridDim.x, gy = gridDim.y, nz = gridDim.z, G = gx * gy;
+  if (nz % 8u != 0u) return {blockIdx.x, blockIdx.y, blockIdx.z};
+  const uint32_t L = blockIdx.x + gx * (blockIdx.y + gy * blockIdx.z);
+  const uint32_t rest = L / 8u, t = rest % G;
+  return {t % gx, t / gx, L % 8u + 8u * (rest / G)};
+}
+
 }  // namespace tcmi

@@ -10,7 +10,7 @@
 
 const { size } = require('../ir/shapes');
 const { singularBound } = require('../ir/operators');
-const { kernelText } = require('./codegen');
+const { kernelText, XCD_GROUPED } = require('./codegen');
 
 const ceil = (a, b) => Math.ceil(a / b);
 const OPERATORS = new Set(['rotary', 'rotaryGrad', 'linearCrossEntropy', 'linearCrossEntropyGrad', 'orthogonalize']);
@@ -298,19 +298,19 @@ function lowerOrthogonalize(graph, node) {
     GSPLIT: G.split, GCHUNKS: G.chunks, GEACH: G.each, BSPLIT: B.split, BCHUNKS: B.chunks, BEACH: B.each,
     SX: fits(top), SA: fits(top ** 2), SB: Math.max(-60, Math.min(60, fits(Math.max(Math.abs(b) * top ** 2 + Math.abs(c) * top ** 4, 2 ** -40)))) };
   let at = 0;
-  const place = (name, bytes) => { z[name] = at; at = align(at + bytes, 256); };
-  place('NORM', 8 * z.BLOCKS);
-  place('X0', steps > 0 ? 4 * MP * NP : 0);
-  place('X1', steps > 1 ? 4 * MP * NP : 0);
-  place('A', steps > 0 ? 4 * SP * SP : 0);
-  place('B', steps > 0 ? 4 * SP * SP : 0);
+  const put = (name, bytes) => { z[name] = at; at = align(at + bytes, 256); };
+  put('NORM', 8 * z.BLOCKS);
+  put('X0', steps > 0 ? 4 * MP * NP : 0);
+  put('X1', steps > 1 ? 4 * MP * NP : 0);
+  put('A', steps > 0 ? 4 * SP * SP : 0);
+  put('B', steps > 0 ? 4 * SP * SP : 0);
   const partial = (kind, t) => 4 * TILES[kind][0] * TILES[kind][1] * t.split * t.chunks;
-  place('PART', steps > 0 ? Math.max(partial(GKIND, G), partial(BKIND, B)) : 0);
+  put('PART', steps > 0 ? Math.max(partial(GKIND, G), partial(BKIND, B)) : 0);
   z.PER = at;
   const sizes = Object.keys(z).map((k) => (typeof z[k] === 'boolean' ? `  static constexpr bool ${k} = ${z[k]};`
     : ['GKIND', 'BKIND', 'AKIND', 'SX', 'SA', 'SB'].includes(k) ? `  static constexpr int ${k} = ${z[k]};`
       : `  static constexpr ${/^([MNS]P?|BLOCKS|[GB](SPLIT|CHUNKS|EACH))$/.test(k) ? 'uint32_t' : 'size_t'} ${k} = ${z[k]}u;`)).join('\n');
-  const S = '__KERNEL___s';
+  const S = '__KERNEL___s', place = square ? 'blockIdx' : 'wg';
   const make = (kind, blocks, threads, lds, call) => kernel(kind, `#include "tcmi_orthogonalize.h"
 struct __KERNEL___s {
 ${sizes}
@@ -320,20 +320,20 @@ ${sizes}
   static __device__ __forceinline__ double eps() { return ${double(eps)}; }
 };
 extern "C" __global__ void __launch_bounds__(${threads}${bounds(threads, lds)}) __KERNEL__(const TcmiArgs A) {
-  const tcmi::Orth<__KERNEL___s> o(A.in[0], A.out, A.ws, blockIdx.z);
+${square ? '' : `  ${XCD_GROUPED}\n`}  const tcmi::Orth<__KERNEL___s> o(A.in[0], A.out, A.ws, ${place}.z);
 ${lds ? `  __shared__ __attribute__((aligned(1024))) ${lds};\n` : ''}  tcmi::${call};
 }
 `, [blocks, 1, count], threads);
   const pool = (k) => `char lds[tcmi::Tile<${k}>::LDS]`;
-  const kernels = [make('orthnorm', z.BLOCKS, 256, 'double scratch[4]', `orth_norm<${S}>(o, scratch, blockIdx.x)`),
-    make('orthsplit', ceil(MP * NP, 4096), 256, 'double scratch[4]', `orth_split<${S}, ${steps === 0}>(o, scratch, blockIdx.x)`)];
+  const kernels = [make('orthnorm', z.BLOCKS, 256, 'double scratch[4]', `orth_norm<${S}>(o, scratch, ${place}.x)`),
+    make('orthsplit', ceil(MP * NP, 4096), 256, 'double scratch[4]', `orth_split<${S}, ${steps === 0}>(o, scratch, ${place}.x)`)];
   for (let k = 0; k < steps; k++) {
     for (const [poly, kind, t] of [[false, GKIND, G], [true, BKIND, B]]) {
       const from = poly ? 0 : k % 2, name = poly ? 'poly' : 'gram';
-      kernels.push(make(`orth${name}`, tilesOf + t.split * (t.chunks - 1), TILES[kind][2], pool(kind), `orth_symmetric<${S}, ${poly}, ${from}>(o, lds, blockIdx.x)`));
-      if (t.split) kernels.push(make(`orthjoin${name}`, t.split * (TILES[kind][0] === 128 ? 4 : kind === FOUR ? 1 : 2), TILES[kind][2], null, `orth_join<${S}, ${poly}>(o, blockIdx.x)`));
+      kernels.push(make(`orth${name}`, tilesOf + t.split * (t.chunks - 1), TILES[kind][2], pool(kind), `orth_symmetric<${S}, ${poly}, ${from}>(o, lds, ${place}.x)`));
+      if (t.split) kernels.push(make(`orthjoin${name}`, t.split * (TILES[kind][0] === 128 ? 4 : kind === FOUR ? 1 : 2), TILES[kind][2], null, `orth_join<${S}, ${poly}>(o, ${place}.x)`));
     }
-    kernels.push(make('orthapply', ablocks, TILES[AKIND][2], pool(AKIND), `orth_apply<${S}, ${k % 2}, ${k === steps - 1}>(o, lds, blockIdx.x)`));
+    kernels.push(make('orthapply', ablocks, TILES[AKIND][2], pool(AKIND), `orth_apply<${S}, ${k % 2}, ${k === steps - 1}>(o, lds, ${place}.x)`));
   }
   return { kind: 'orthogonalize', kernels, workspace: count * z.PER, flops: count * steps * (3 * s * s * l + s ** 3) };
 }
