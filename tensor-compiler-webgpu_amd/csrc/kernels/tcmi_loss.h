@@ -256,7 +256,7 @@ constexpr uint32_t loss_parts() { return S::VP / (16 * Tile<S::LKIND>::T); }
 template <class S, bool LOSS, bool LAST>
 __device__ __forceinline__ void loss_join(const Loss<S>& L, float* out, float2* scratch, uint32_t block) {
   LossState* st = L.state();
-  const uint32_t piece = st->current;
+  const uint32_t piece = S::PIECES > 1 ? st->current : 0u;
   const uint32_t row = block * 16 + threadIdx.x % 16, k0 = threadIdx.x / 16;
   const float2* stats = reinterpret_cast<const float2*>(L.at(S::STATS)) + row;
   RowSum sum;

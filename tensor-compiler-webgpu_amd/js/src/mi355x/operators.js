@@ -124,6 +124,12 @@ function lowerRotary(graph, node) {
 const LOSS_PIECE = 1 << 28;      // bytes of a piece's logits at most (a piece is 128 rows or more)
 const LOSS_PARTS = ['dh', 'dW', 'dbias', 'loss'];
 const CUS = 256;
+/**
+ * Rows up to which W is read as it is (tcmi_loss_few.h), by time, without and with gradients (us): 64 rows of d 1024, V 131072
+ * 212 and 591, by products of pairs 504 and 1019; of d 64, V 96 10.0 and 18.8, by pairs 13.0 and 17.5. 16 rows: 115 and 394, 501
+ * and 1001; 7.3 and 11.8, 12.8 and 16.9. Its time grows with the rows from 16 on, the pairs' hardly before 128.
+ */
+const FEW_ROWS = 64;
 // tcmi_gemm_f16x2.h's tiles: rows, columns and threads of each kind.
 const SMALL = 0, SQUARE = 1, WIDE = 2, TALL = 3, FOUR = 4;
 const TILES = [[64, 64, 256], [128, 128, 256], [128, 256, 512], [256, 128, 512], [64, 64, 256]];
@@ -146,14 +152,15 @@ function lossSizes(N, D, V, bias, parts, piece) {
   const PIECES = ceil(align(N, rows), most), NP = align(ceil(N, PIECES), rows);
   const RB = NP * VP >= 2 ** 20 ? 32 : 16;
   const clamp = (n, most) => Math.max(1, Math.min(Math.ceil(n), most));
-  // Large tiles unless they would leave much of the chip idle, by all rows: a loss has the same bits whatever its
+  // Large tiles (1024 x 65536 of K 1024: 256 x 128 395 us, 128 x 256 426, 128 x 128 460) unless they would leave much of the chip
+  // idle, by all rows: a loss has the same bits whatever its
   // pieces. The gradients' tiles and the chunks of K by time.
   const large = VP % 256 === 0 && rows === 256 && align(N, 256) / 128 * (VP / 256) >= CUS / 2;
   const LT = large ? 4 : 2;
   const g = gradTiles(NP, DP, VP);
   const CT = (() => { let t = 16; while (2 * t <= Math.min(256, VP / 8)) t *= 2; return t; })();
   const z = { N, D, V, DP, VP, NP, PIECES, RB, CT, BIAS: bias, HBLOCKS: clamp(N * D / 4096, 256), WBLOCKS: clamp(D * V / 16384, 1024), GBLOCKS: clamp(N / 1024, 64),
-    PER: clamp((NP * PIECES * DP + DP * VP) / 4 / 256 / 1024, 16), LKIND: large ? WIDE : smallKind(align(N, 64) / 64 * (VP / 64), DP / 32), HKIND: g.large ? TALL : SMALL, WKIND: g.large ? WIDE : SMALL, JOINED: !grad || VP / (16 * LT) > 32, VECD: D % 4 === 0, VECV: V % 4 === 0,
+    PER: clamp((NP * PIECES * DP + DP * VP) / 4 / 256 / 1024, 16), LKIND: large ? TALL : smallKind(align(N, 64) / 64 * (VP / 64), DP / 32), HKIND: g.large ? TALL : SMALL, WKIND: g.large ? WIDE : SMALL, JOINED: !grad || VP / (16 * LT) > 32, VECD: D % 4 === 0, VECV: V % 4 === 0,
     HCHUNKS: g.h.chunks, HK: g.h.each, WCHUNKS: g.w.chunks, WK: g.w.each };
   let at = 0;
   const place = (name, bytes) => { z[name] = at; at = align(at + bytes, 256); };
@@ -203,15 +210,31 @@ function gradTiles(NP, DP, VP) {
   return small.t < large.t ? small : large;
 }
 
-function lossKernels(N, D, V, bias, parts, joined, bytes) {
-  const { z, workspace, grad } = lossSizes(N, D, V, bias, parts, bytes);
-  const e = entry(joined ? parts : null);
-  const has = (p) => parts.includes(p);
-  const counts = ['N', 'D', 'V', 'DP', 'VP', 'NP', 'PIECES', 'RB', 'CT', 'HBLOCKS', 'WBLOCKS', 'GBLOCKS', 'PER', 'HCHUNKS', 'HK', 'WCHUNKS', 'WK'];
+/** The sizes of a loss's launch over few rows (tcmi_loss_few.h), and its workspace's layout. */
+function fewSizes(N, D, V, bias, parts) {
+  const grad = parts.some((p) => p !== 'loss');
+  const NP = align(N, 16), DP = align(D, 16), VP = align(V, 64), RT = NP / 16;
+  // Enough workgroups for every CU: fewer columns of G, then fewer rows of W to each. LKIND: `join` finds a pair of
+  // statistics for each 64 columns, as of the large tiles.
+  const COLS = V >= 256 * CUS / 2 ? 256 : 64, CHUNKS = ceil(V, COLS), tiles = DP / 16;
+  const z = { N, D, V, DP, VP, NP, RT, PIECES: 1, BIAS: bias, LKIND: TALL, WAVES: RT > 2 ? 4 : 8, COLS, CHUNKS,
+    DTILES: Math.max(4, ceil(tiles, ceil(2 * CUS, CHUNKS))), VECD: D % 4 === 0, VECV: V % 4 === 0 };
+  let at = 0;
+  const place = (name, bytes) => { z[name] = at; at = align(at + bytes, 256); };
+  place('STATS', 8 * NP * (VP / 64));
+  place('PICKED', 4 * NP);
+  place('ROWS', 8 * NP);
+  if (grad) place('Z', 4 * NP * VP); else z.Z = 0;
+  if (parts.includes('dh') && CHUNKS > 1) place('HPART', 4 * CHUNKS * NP * DP); else z.HPART = 0;
+  return { z, workspace: at, grad };
+}
+
+function lossMaker(z, e, bias, grad) {
+  const counts = /^([NDV]P?|NP|RT|PIECES|RB|CT|[HWG]BLOCKS|PER|[HW]CHUNKS|[HW]K|WAVES|COLS|CHUNKS|DTILES)$/;
   const sizes = Object.keys(z).map((k) => (typeof z[k] === 'boolean' ? `  static constexpr bool ${k} = ${z[k]};`
     : k.endsWith('KIND') ? `  static constexpr int ${k} = ${z[k]};`
-      : `  static constexpr ${counts.includes(k) ? 'uint32_t' : 'size_t'} ${k} = ${z[k]}u;`)).join('\n');
-  const make = (kind, grid, threads, lds, call) => kernel(kind, `#include "tcmi_loss.h"
+      : `  static constexpr ${counts.test(k) ? 'uint32_t' : 'size_t'} ${k} = ${z[k]}u;`)).join('\n');
+  return (kind, grid, threads, lds, call) => kernel(kind, `#include "${/few_/.test(call) ? 'tcmi_loss_few.h' : 'tcmi_loss.h'}"
 struct __KERNEL___s {
 ${sizes}
 };
@@ -220,6 +243,34 @@ ${e.open}  const tcmi::Loss<__KERNEL___s> L{A.in[0], A.in[1], A.in[2], ${bias ? 
 ${lds ? `  __shared__ __attribute__((aligned(1024))) ${lds};\n` : ''}  tcmi::${call};
 }
 `, grid, threads);
+}
+
+function fewKernels(N, D, V, bias, parts, joined) {
+  const { z, workspace, grad } = fewSizes(N, D, V, bias, parts);
+  const e = entry(joined ? parts : null);
+  const has = (p) => parts.includes(p);
+  const make = lossMaker(z, e, bias, grad);
+  const S = '__KERNEL___s';
+  const outs = (...names) => names.map((p) => (has(p) ? e.out(p) : 'nullptr')).join(', ');
+  const kernels = [make('losslogits', [z.VP / 64, 1, 1], 64 * z.WAVES, `float lds[${z.WAVES * z.NP} * tcmi::FEW_LD]`, `few_logits<${S}, ${grad}>(L, lds, blockIdx.x)`),
+    make('lossjoin', [z.NP / 16, 1, 1], 1024, 'float2 scratch[1024]', `loss_join<${S}, ${has('loss')}, false>(L, ${outs('loss')}, scratch, blockIdx.x)`)];
+  const [dh, dW, db] = ['dh', 'dW', 'dbias'].map(has);
+  if (dh || dW || db) {
+    kernels.push(make('lossgrads', [z.CHUNKS, dh || dW ? ceil(z.DP / 16, z.DTILES) : 1, 1], 256, `float lds[${z.NP * (z.COLS + 4)}]`,
+      `few_grads<${S}, ${dh}, ${dW}, ${db}>(L, ${outs('dh', 'dW', 'dbias')}, lds, blockIdx.x, blockIdx.y)`));
+    if (dh && z.CHUNKS > 1) {
+      kernels.push(make('losssums', [ceil(z.NP * z.DP / 4, 32), 1, 1], 256, 'tcmi::f4 scratch[256]', `few_sums<${S}>(L, ${outs('dh')}, scratch, blockIdx.x)`));
+    }
+  }
+  return { kernels, workspace };
+}
+
+function lossKernels(N, D, V, bias, parts, joined, bytes) {
+  if (N <= FEW_ROWS) return fewKernels(N, D, V, bias, parts, joined);
+  const { z, workspace, grad } = lossSizes(N, D, V, bias, parts, bytes);
+  const e = entry(joined ? parts : null);
+  const has = (p) => parts.includes(p);
+  const make = lossMaker(z, e, bias, grad);
   const S = '__KERNEL___s';
   const [lr, lc, lt] = TILES[z.LKIND], [hr, hc, gt] = TILES[z.HKIND], [wr, wc] = TILES[z.WKIND];
   const outs = (...names) => names.map((p) => (has(p) ? e.out(p) : 'nullptr')).join(', ');
@@ -290,7 +341,7 @@ function lowerOrthogonalize(graph, node) {
   const kind = (blocks, K) => (square ? SQUARE : smallKind(blocks * count, K / 32));
   const half = square || n * n * count > CUS, tilesOf = half ? upper : n * n;
   const GKIND = kind(tilesOf, l), BKIND = kind(tilesOf, s);
-  const AKIND = square && NP % 256 === 0 ? WIDE : square && MP % 256 === 0 ? TALL : kind(all, s);
+  const AKIND = square && MP % 256 === 0 ? TALL : square && NP % 256 === 0 ? WIDE : kind(all, s);
   const ablocks = MP / TILES[AKIND][0] * (NP / TILES[AKIND][1]);
   const G = splitTiles(GKIND, tilesOf, ceil(l, 32)), B = splitTiles(BKIND, tilesOf, ceil(s, 32));
   const top = singularBound(node.attrs);

@@ -80,6 +80,20 @@ const CASES = [
   loss('pieces', 700, 24, 150, { bias: true, gradient: true, tuning: { loss: { piece: 1 } } }),
   loss('piece-values', 400, 24, 150, { bias: true, tuning: { loss: { piece: 1 } } }),
   loss('squared', 50, 24, 300, { bias: true, gradient: true, after: true }),
+  // Rows that are few, up to the most of them, by tiles of 64 and of 256 classes; one row more, and the same again.
+  loss('row', 1, 515, 1000, { bias: true, gradient: true }),
+  loss('few-odd', 33, 37, 517, { bias: true, gradient: true }),
+  loss('few-most', 64, 64, 128, { gradient: true }),
+  loss('few-classes', 17, 9, 3, { bias: true, gradient: true }),
+  loss('few-wide', 9, 20, 33001, { bias: true, gradient: true }),
+  loss('few-values', 49, 70, 132, {}),
+  loss('one-more', 65, 1, 1, { gradient: true }),
+  loss('more', 77, 17, 7, { bias: true, gradient: true }),
+  loss('more-deep', 100, 515, 260, { gradient: true }),
+  loss('more-h', 150, 24, 300, { bias: true, gradient: true, wrt: ['h'] }),
+  loss('more-W', 150, 24, 300, { bias: true, gradient: true, wrt: ['W'] }),
+  loss('more-b', 150, 24, 300, { bias: true, gradient: true, wrt: ['b'] }),
+  loss('more-squared', 150, 24, 300, { bias: true, gradient: true, after: true }),
   // Matrices from one element to several tiles, wide and tall, alone, stacked and side by side.
   orth('one', [1, 1]),
   orth('row', [1, 70]),
