@@ -1340,26 +1340,42 @@ function batchPlan(launches, aliases, bytesOf) {
     if (placed[i]) continue;
     const jn = jointOf(launches[i]);
     if (jn) {
-      const { operands } = launches[i].kernels[0].joint;
-      const same = (l) => l.inputs.slice(0, operands).join() === launches[i].inputs.slice(0, operands).join();
-      const parts = new Map();
-      let rest = null;        // the operands that some of the parts read besides
-      for (let j = i; j < n; j++) {
-        const l = launches[j];
-        if (placed[j] || jointOf(l) !== jn || !same(l) || parts.has(l.kernels[0].part)) continue;
-        const more = operands === undefined ? '' : l.inputs.slice(operands).join();
-        if (!ready(l) || (more && rest && rest !== more)) continue;
-        if (more) rest = more;
-        parts.set(l.kernels[0].part, j);
-      }
-      const { parts: all, order: any, build } = launches[i].kernels[0].joint;
+      const { operands, parts: all, order: any, build, groups } = launches[i].kernels[0].joint;
+      // The parts of launch i's node that may run now, by part: of the launches from i on, those of its operands.
+      const partsOf = (first) => {
+        const same = (l) => l.inputs.slice(0, operands).join() === launches[first].inputs.slice(0, operands).join();
+        const parts = new Map();
+        let rest = null;        // the operands that some of the parts read besides
+        for (let j = first; j < n; j++) {
+          const l = launches[j];
+          if (placed[j] || jointOf(l) !== jn || !same(l) || parts.has(l.kernels[0].part)) continue;
+          const more = operands === undefined ? '' : l.inputs.slice(operands).join();
+          if (!ready(l) || (more && rest && rest !== more)) continue;
+          if (more) rest = more;
+          parts.set(l.kernels[0].part, j);
+        }
+        return parts;
+      };
+      const parts = partsOf(i);
       const order = all || any.filter((p) => parts.has(p));
       if (order.length > 1 && order.every((p) => parts.has(p))) {
         const group = order.map((p) => parts.get(p));
-        const unit = group.map((j) => launches[j]);
-        unit.joint = build ? build(order) : launches[i].kernels[0].joint;
-        if (build) for (const l of unit) l.joined = true;
+        for (const j of group) placed[j] = 2;      // not yet a writer that a launch may wait for
+        // Equal nodes with the same parts (queries' and keys' of one head count): groups of one launch.
+        let count = 1;
+        for (let j = i + 1; groups && j < n && (count + 1) * order.length <= cg.MAX_BATCH; j++) {
+          if (placed[j] || jointOf(launches[j]) !== jn || !ready(launches[j])) continue;
+          const others = partsOf(j);
+          if (others.size !== order.length || !order.every((p) => others.has(p))) continue;
+          const twin = order.map((p) => others.get(p));
+          for (const x of twin) placed[x] = 2;
+          group.push(...twin);
+          count++;
+        }
         for (const j of group) placed[j] = 1;
+        const unit = group.map((j) => launches[j]);
+        unit.joint = build ? build(order, count) : launches[i].kernels[0].joint;
+        if (build) for (const l of unit) l.joined = true;
         units.push(unit);
         continue;
       }

@@ -30,11 +30,17 @@ function kernel(kind, text, grid, threads, more) {
 /**
  * How a kernel's text reaches its launch: alone, `A` (TcmiArgs) with the part's output in
  * A.out; as one of `parts` in a joint launch, member k of its argument block for the k-th part, the
- * operands and the workspace in member 0's.
+ * operands and the workspace in member 0's. With several `groups` of them (a joint launch of equal nodes), workgroups'
+ * z index is the group, its members one after another, its workspace `floats` long.
  */
-function entry(parts) {
-  return parts ? { sig: `const TcmiBatch<${parts.length}> B`, open: '  const TcmiPtrs& A = B.m[0];\n', out: (part) => `B.m[${parts.indexOf(part)}].out` }
-    : { sig: 'const TcmiArgs A', open: '', out: () => 'A.out' };
+function entry(parts, groups, floats) {
+  if (!parts) return { sig: 'const TcmiArgs A', open: '', out: () => 'A.out', ws: 'A.ws' };
+  const n = parts.length;
+  if (groups > 1) {
+    return { sig: `const TcmiBatch<${n * groups}> B`, open: `  const TcmiPtrs* const M = B.m + ${n}u * blockIdx.z;\n  const TcmiPtrs& A = M[0];\n`,
+      out: (part) => `M[${parts.indexOf(part)}].out`, ws: `A.ws + blockIdx.z * (size_t)${floats}u` };
+  }
+  return { sig: `const TcmiBatch<${n}> B`, open: '  const TcmiPtrs& A = B.m[0];\n', out: (part) => `B.m[${parts.indexOf(part)}].out`, ws: 'A.ws' };
 }
 
 // ---- rotary -------------------------------------------------------------------------------
@@ -59,8 +65,7 @@ function rotarySizes(graph, node) {
   return { DH, R, B, M1, T, M2, axes, shared, E, lanes, units: ceil(R / E, lanes), tails: ceil((DH - 2 * R) / E, lanes), slots };
 }
 
-function rotaryText(z, attrs, gain, grads, parts) {
-  const e = entry(parts);
+function rotaryText(z, attrs, gain, grads, e) {
   const dx = grads.includes('dx'), dgain = grads.includes('dgain');
   const table = z.R ? `  static __device__ __forceinline__ double turns(int j) {
     static constexpr double t[${z.R}] = {${attrs.frequencies.map((f) => double(f / (2 * Math.PI))).join(', ')}};
@@ -82,29 +87,27 @@ ${table}
 };
 extern "C" __global__ void __launch_bounds__(${ROTARY_THREADS}) __KERNEL__(${e.sig}) {
 ${e.open}${dgain ? `  __shared__ __attribute__((aligned(16))) float scratch[${ROTARY_THREADS / z.lanes * z.DH}];\n` : ''}  tcmi::rotary<__KERNEL___s>(A.in[0], A.in[1], ${gain ? 'A.in[2]' : 'nullptr'}, ${grads.length ? `A.in[${last}]` : 'nullptr'}, ${
-  dx || !grads.length ? e.out('dx') : 'nullptr'}, ${dgain ? 'A.ws, scratch' : 'nullptr, nullptr'}, blockIdx.x, gridDim.x);
+  dx || !grads.length ? e.out('dx') : 'nullptr'}, ${dgain ? `${e.ws}, scratch` : 'nullptr, nullptr'}, blockIdx.x, gridDim.x);
 }
 `;
 }
 
-function rotaryKernels(z, attrs, gain, grads, parts) {
+function rotaryKernels(z, attrs, gain, grads, parts, groups) {
   // A few tokens to a workgroup. The gradient of the gain walks them in at most 1024 workgroups, whose sums are then added.
   const perBlock = ROTARY_THREADS / z.lanes / z.slots;
-  const want = ceil(z.B * z.T, perBlock);
-  const blocks = Math.min(want, grads.includes('dgain') ? 1024 : 65536);
-  const kernels = [kernel('rot', rotaryText(z, attrs, gain, grads, parts), [blocks, 1, 1], ROTARY_THREADS)];
-  let workspace = 0;
-  if (grads.includes('dgain')) {
-    const e = entry(parts);
-    workspace = blocks * z.DH * 4;
+  const want = ceil(z.B * z.T, perBlock), dgain = grads.includes('dgain'), Z = groups || 1;
+  const blocks = Math.min(want, dgain ? 1024 : 65536), floats = dgain ? align(blocks * z.DH, 64) : 0;
+  const e = entry(parts, Z, floats);
+  const kernels = [kernel('rot', rotaryText(z, attrs, gain, grads, e), [blocks, 1, Z], ROTARY_THREADS)];
+  if (dgain) {
     kernels.push(kernel('rotsum', `#include "tcmi_rotary.h"
 extern "C" __global__ void __launch_bounds__(1024) __KERNEL__(${e.sig}) {
 ${e.open}  __shared__ float scratch[1024];
-  tcmi::rotary_gain_sum<${z.DH}>(A.ws, ${e.out('dgain')}, ${blocks}u, scratch, blockIdx.x);
+  tcmi::rotary_gain_sum<${z.DH}>(${e.ws}, ${e.out('dgain')}, ${blocks}u, scratch, blockIdx.x);
 }
-`, [ceil(z.DH, 16), 1, 1], 1024));
+`, [ceil(z.DH, 16), 1, Z], 1024));
   }
-  return { kernels, workspace };
+  return { kernels, workspace: 4 * floats * Z };
 }
 
 function lowerRotary(graph, node) {
@@ -114,7 +117,7 @@ function lowerRotary(graph, node) {
   const k = rotaryKernels(z, node.attrs, gain, grad ? [node.attrs.part] : [], null);
   if (grad && gain) {
     const { part, ...rest } = node.attrs;
-    joint(k.kernels[0], part, ['dx', 'dgain'], ['rotary', rest, z], (parts) => rotaryKernels(z, node.attrs, gain, parts, parts));
+    joint(k.kernels[0], part, ['dx', 'dgain'], ['rotary', rest, z], (parts, groups) => rotaryKernels(z, node.attrs, gain, parts, parts, groups), undefined, true);
   }
   return { kind: grad ? 'rotary-grad' : 'rotary', kernels: k.kernels, workspace: k.workspace };
 }
@@ -390,12 +393,13 @@ ${lds ? `  __shared__ __attribute__((aligned(1024))) ${lds};\n` : ''}  tcmi::${c
 }
 
 /**
- * Marks kernel `k` as the first of part `part` of a launch whose parts `build(parts)` forms
- * together, in `order`. They read the same first `operands` operands (default: all).
+ * Marks kernel `k` as the first of part `part` of a launch whose parts `build(parts, groups)` forms
+ * together, in `order`. They read the same first `operands` operands (default: all). `groups`: whether it forms those
+ * parts of several nodes of one key.
  */
-function joint(k, part, order, key, build, operands) {
+function joint(k, part, order, key, build, operands, groups) {
   Object.defineProperty(k, 'part', { value: part });
-  Object.defineProperty(k, 'joint', { value: { name: JSON.stringify(key), order, build, operands } });
+  Object.defineProperty(k, 'joint', { value: { name: JSON.stringify(key), order, build, operands, groups: !!groups } });
 }
 
 /** The launch of an operator's node: { kind, kernels, params, workspace, flops }. tuning.loss.piece: bytes of a piece's logits. */

@@ -1,7 +1,8 @@
 'use strict';
 // Graphs of the operators that are one node each (ir/operators.js), from plain
 // descriptions: those of their GPU tests (CASES) and of their measurement (MEASURED).
-//   { family: 'rotary', x, positions, gain?, gradient?, options }   x twice over where `twin` gives a second shape
+//   { family: 'rotary', x, positions, gain?, gradient?, options }   a second x where `twin`
+//       gives its shape; `twice`: rotated, and the result again
 //   { family: 'loss', N, d, V, bias?, gradient?, wrt?, after? }     wrt: 'h', 'W', 'b' (default all); `after`: the
 //       losses' cotangent depends on the losses, so their gradients cannot run beside them
 //   { family: 'orthogonalize', x, count, options }
@@ -17,7 +18,8 @@ function operatorGraph(c) {
     [c.x].concat(c.twin ? [c.twin] : []).forEach((shape, k) => {
       const x = g.input(`x${k}`, shape);
       const gain = c.gain ? g.input(`g${k}`, [shape[shape.length - 1]]) : null;
-      outs.push(g.rotary(x, at, Object.assign({ gain }, c.options || {})));
+      const y = g.rotary(x, at, Object.assign({ gain }, c.options || {}));
+      outs.push(c.twice ? g.rotary(y, at, Object.assign({ gain }, c.options || {})) : y);
       names.push(`y${k}`);
       wrt.push(x);
       grads.push(`dx${k}`);
@@ -50,6 +52,8 @@ const CASES = [
   // One token and many; heads before and after the tokens; one position a token and one a sequence's token.
   rotary('token', [3, 1, 5, 64], [3, 1], { gain: true, gradient: true }),
   rotary('step', [4, 33, 4, 64], [33], { gain: true, gradient: true, twin: [4, 33, 2, 64] }),
+  rotary('twins', [3, 40, 2, 64], [40], { gain: true, gradient: true, twin: [3, 40, 2, 64] }),
+  rotary('twice', [3, 40, 2, 64], [40], { gain: true, gradient: true, twice: true }),
   rotary('heads-first', [2, 3, 17, 32], [2, 17], { gain: true, gradient: true, options: { axis: 2 } }),
   rotary('one-head', [29, 48], [29], { gain: true, gradient: true }),
   // Three axes, and frequencies that start over on each; adjacent pairs; a part of the head unrotated.

@@ -72,6 +72,13 @@ def test_parts_that_are_kept_run_as_one_launch(graphs):
     assert g["perf"][0] == "linear-cross-entropy" and g["perf"].index("linear-cross-entropy-grad") > 1
 
 
+def test_equal_gradients_share_a_launch(graphs):
+    """Queries' and keys' parts in one launch; not those of a rotation of a rotation, of which one reads the other."""
+    assert [b["count"] for b in graphs["rotary-twins"]["batches"] if b["joint"]] == [4]
+    assert [b["count"] for b in graphs["rotary-twice"]["batches"] if b["joint"]] == [2, 2]
+    assert [b["count"] for b in graphs["rotary-step"]["batches"] if b["joint"]] == [2, 2]
+
+
 def test_every_launch_reads_what_is_written_before_it(tool, graphs):
     r = tool("operator-order", {"cases": [g["case"] for g in graphs.values()]}, timeout=120)
     assert len(r) == len(graphs)
