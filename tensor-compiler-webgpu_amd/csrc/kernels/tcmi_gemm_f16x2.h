@@ -323,14 +323,17 @@ struct Tile {
   // The row, and the first column, of this lane's first four sums: fragment (i, j)'s 16·i rows and 16·j columns on.
   static __device__ __forceinline__ uint32_t row(const TileAt& at) { return at.row * ROWS + threadIdx.x / 64 / WN * TI * 16 + threadIdx.x % 16; }
   static __device__ __forceinline__ uint32_t col(const TileAt& at) { return at.col * COLS + threadIdx.x / 64 % WN * TJ * 16 + threadIdx.x % 64 / 16 * 4; }
-  // f(row, col, v) of each four columns that this lane holds.
+  // f(row, col, v) of each four columns that this lane holds, 16 rows at a time: what f loads for all of them does not fit the
+  // registers beside the sums.
   template <class F>
   static __device__ __forceinline__ void each(const TileAt& at, Sums& acc, F f) {
     const uint32_t row0 = row(at), col0 = col(at);
 #pragma unroll
-    for (int i = 0; i < TI; ++i)
+    for (int i = 0; i < TI; ++i) {
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int j = 0; j < TJ; ++j) f(row0 + i * 16, col0 + j * 16, acc[i][j]);
+    }
   }
 };
 

@@ -1344,6 +1344,13 @@ async function main() {
         const f = fuse(v.graph, Object.assign({ keep: v.keep }, fuseOpts || {}));
         add(lowerMI355X(f.graph, { perf: true, keep: v.keep.map((id) => f.index.get(id)) }));
       };
+      if (req.operators) {
+        // Those of the operators' graphs instead (testing/operator_cases.js), from descriptions.
+        const { operatorGraph } = require('../src/testing/operator_cases');
+        for (const c of req.operators) perf(operatorGraph(c));
+        out = { kernels: Array.from(m.keys()), unit: translationUnit(m) };
+        break;
+      }
       const fs = fusedStep(modelStep({ model: 'transformer', B: 64 }).step);
       add(fs.lowered);
       add(fs.checked);

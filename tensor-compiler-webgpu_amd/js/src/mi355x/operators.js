@@ -53,7 +53,7 @@ function rotarySizes(graph, node) {
   const DH = x[x.length - 1], R = a.frequencies.length, T = x[a.axis];
   if (DH > ROTARY_HEAD) throw new Error(`rotary: heads of ${DH} floats (at most ${ROTARY_HEAD})`);
   const B = a.axis > 0 ? x[0] : 1, M1 = size(x.slice(1, Math.max(1, a.axis))), M2 = size(x.slice(a.axis + 1, -1));
-  if (B * T >= 2 ** 32 || M1 * M2 >= 2 ** 32) throw new Error('rotary: tokens and heads are counted in 32 bits');
+  if (B * T >= 2 ** 31 || M1 * M2 >= 2 ** 31) throw new Error('rotary: tokens and heads are counted in 32 bits (at most 2^31 - 1)');
   const axes = a.positionAxes;
   const shared = size(pos) === T * axes && B > 1;
   // 128-bit loads where a group of four pairs (and of four floats that are not rotated) is whole and aligned.
@@ -143,6 +143,8 @@ const smallKind = (blocks, slices) => (blocks <= CUS && slices >= 32 ? FOUR : SM
 const bounds = (threads, lds) => (/Tile/.test(lds || '') ? ', 2' : '');
 
 const align = (n, to) => ceil(n, to) * to;
+// Columns of a matrix of pairs at most: an offset among 256 of its rows has 32 bits.
+const PAIR_COLS = 2 ** 22;
 
 /** The sizes of a loss's launch forming `parts`, and its workspace's layout. */
 function lossSizes(N, D, V, bias, parts, piece) {
@@ -271,6 +273,7 @@ function fewKernels(N, D, V, bias, parts, joined) {
 function lossKernels(N, D, V, bias, parts, joined, bytes) {
   if (N <= FEW_ROWS) return fewKernels(N, D, V, bias, parts, joined);
   const { z, workspace, grad } = lossSizes(N, D, V, bias, parts, bytes);
+  if (Math.max(z.DP, z.VP) > PAIR_COLS) throw new Error(`linearCrossEntropy: ${Math.max(D, V)} columns (at most ${PAIR_COLS} for more than ${FEW_ROWS} rows)`);
   const e = entry(joined ? parts : null);
   const has = (p) => parts.includes(p);
   const make = lossMaker(z, e, bias, grad);
@@ -335,6 +338,7 @@ function lowerOrthogonalize(graph, node) {
   const x = node.shape, M = x[x.length - 2], N = x[x.length - 1], count = size(x.slice(0, -2));
   const { steps, eps, coefficients: [a, b, c] } = node.attrs;
   if (count > 65535) throw new Error(`orthogonalize: ${count} matrices (at most 65535)`);
+  if (Math.max(M, N) > PAIR_COLS) throw new Error(`orthogonalize: a matrix of ${M} x ${N} (at most ${PAIR_COLS} on a side)`);
   const tall = M > N, s = Math.min(M, N), l = Math.max(M, N);
   // Tiles of 128, or of 64 where those leave much of the chip idle.
   const tiles = (t) => ceil(s, t) * ceil(l, t) * count;

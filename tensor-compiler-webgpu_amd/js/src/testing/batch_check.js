@@ -154,6 +154,29 @@ function checkBatches(plain, batched) {
     if (b.start < next || b.count < 2 || b.start + b.count > L.length) return { ok: false, why: `batch at ${b.start} overlaps or is out of range` };
     next = b.start + b.count;
     const first = L[b.start];
+    if (b.joint && first.kernels[0].joint && first.kernels[0].joint.build) {
+      // An operator's parts in one launch of the kernels that form them together, or those of several equal nodes:
+      // members node after node, the parts in the operator's order, the parts of a node of the same operands.
+      const j = first.kernels[0].joint;
+      const ms = L.slice(b.start, b.start + b.count);
+      const again = ms.findIndex((l, k) => k > 0 && l.kernels[0].part === first.kernels[0].part);
+      const n = again < 0 ? b.count : again, groups = b.count / n;
+      const parts = ms.slice(0, n).map((l) => l.kernels[0].part);
+      const want = groups === 1 || (j.groups && Number.isInteger(groups)) ? j.build(parts, groups) : null;
+      const inOrder = parts.map((p) => j.order.indexOf(p));
+      const ok = want && b.wsStride === 0 && (b.workspace || 0) >= want.workspace && batched.workspace >= want.workspace
+        && inOrder.every((x, k) => x >= 0 && (k === 0 || x > inOrder[k - 1]))
+        && b.kernels.length === want.kernels.length && b.kernels.every((k, i) => k.name === want.kernels[i].name && k.source === want.kernels[i].source
+          && k.grid.join() === want.kernels[i].grid.join() && k.block.join() === want.kernels[i].block.join())
+        && ms.every((l, k) => {
+          const node = ms.slice(k - k % n, k - k % n + n), most = node.reduce((q, x) => (x.inputs.length > q.length ? x.inputs : q), []);
+          return l.kernels[0].joint && l.kernels[0].joint.name === j.name && l.kernels[0].part === parts[k % n]
+            && l.inputs.length >= (j.operands || most.length) && l.inputs.join() === most.slice(0, l.inputs.length).join();
+        });
+      if (!ok) return { ok: false, why: `batch at ${b.start}: not the parts of one operator, or of equal ones` };
+      for (let k = 0; k < b.count; k++) unitOf[b.start + k] = b.start;
+      continue;
+    }
     if (first.kernels.length === 1 && first.kernels[0].joint) {
       // An attention gradient's three parts in one launch of their joint kernel: members
       // dQ, dK, dV in that order, of one joint kernel, reading the same operands.

@@ -75,3 +75,20 @@ def test_an_unknown_optimizer_is_refused(tool, tmp_path):
     import tcmi_bridge
     with pytest.raises(tcmi_bridge.ToolError, match="unknown optimizer"):
         step(tool, tmp_path, "x", cfg=SMALL, opt="none")
+
+
+MODERN = {"positions": "rotary", "qkNorm": True, "targets": "classes"}
+STEPS = [{"model": "transformer", "B": 4, "opt": "muon", "cfg": MODERN}, {"model": "transformer", "B": 4, "opt": "muon", "cfg": MODERN, "attention": True},
+         {"model": "transformer", "B": 40, "V": 301, "cfg": dict(MODERN, **SMALL)}]
+
+
+def test_a_steps_joint_launches_hold_their_own_parts(tool):
+    for r in tool("batch-check", {"models": STEPS}):
+        assert r["check"]["ok"], r
+        assert r["check"]["saved"] > 50
+
+
+def test_an_arena_keeps_a_steps_values_until_their_last_use(tool):
+    for r in tool("arena-check", {"models": STEPS}):
+        assert r["check"]["ok"], r
+        assert r["peak"] <= r["bytes"] <= r["peak"] * 1.03 + 4096

@@ -1,11 +1,19 @@
 """The operators that are one node each (js/src/ir/operators.js) without a GPU: their shape rules and refusals, their
 gradients' formulas against differences of their values (float64, oracle/operators.py), and how they lower: an operator's
 parts as one launch where the perf lowering keeps several, alone otherwise."""
+import pathlib
+import re
+import shutil
+import subprocess
+
 import numpy as np
 import pytest
 
 from oracle import interp
 import operator_checks as checks
+
+KERNELS = pathlib.Path(__file__).resolve().parents[1] / "tensor-compiler-webgpu_amd" / "csrc" / "kernels"
+HIPCC = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
 
 
 @pytest.fixture(scope="module")
@@ -106,6 +114,10 @@ def refused(tool, case):
     ({"family": "rotary", "x": [2, 3, 4, 8], "positions": [2], "options": {"axis": 3}}, "no token axis 3"),
     ({"family": "rotary", "x": [3, 1, 4098], "positions": [3], "options": {"axis": 0}}, "at most 4096"),
     ({"family": "loss", "N": 4, "d": 8, "V": 2 ** 24 + 1}, "classes"),
+    ({"family": "loss", "N": 65, "d": 8, "V": 2 ** 22 + 1}, "at most 4194304"),
+    ({"family": "loss", "N": 65, "d": 2 ** 22 + 1, "V": 8}, "at most 4194304"),
+    ({"family": "orthogonalize", "x": [8, 2 ** 22 + 1]}, "at most 4194304"),
+    ({"family": "orthogonalize", "x": [65536, 8, 8]}, "at most 65535"),
     ({"family": "orthogonalize", "x": [8]}, "two axes"),
     ({"family": "orthogonalize", "x": [8, 8], "options": {"steps": -1}}, "steps"),
     ({"family": "orthogonalize", "x": [8, 8], "options": {"steps": 1.5}}, "steps"),
@@ -127,3 +139,37 @@ def test_operands_that_do_not_fit_and_gradients_that_are_none(tool):
     assert "no adjoint rule for op 'linearCrossEntropyGrad'" in r["second"]
     assert "orthogonalize is not differentiable" in r["orthogonalize"]
     assert "no part 'dt'" in r["unknown part"]
+
+
+# Every kind of tile and form: all parts of large and small losses of many rows and of few, wide, tall and square matrices, batched ones,
+# heads of both pairings.
+COMPILED = [
+    {"family": "loss", "N": 1001, "d": 515, "V": 50021, "bias": True, "gradient": True}, {"family": "loss", "N": 8192, "d": 256, "V": 96, "bias": True, "gradient": True},
+    {"family": "loss", "N": 4096, "d": 512, "V": 32768}, {"family": "loss", "N": 64, "d": 97, "V": 40001, "bias": True, "gradient": True},
+    {"family": "loss", "N": 9, "d": 64, "V": 1000, "gradient": True}, {"family": "loss", "N": 128, "d": 64, "V": 96},
+    {"family": "orthogonalize", "x": [256, 256], "count": 16}, {"family": "orthogonalize", "x": [1300, 777]}, {"family": "orthogonalize", "x": [4096, 4096], "count": 2},
+    {"family": "orthogonalize", "x": [2100, 9001]},
+    {"family": "rotary", "x": [2, 64, 4, 128], "positions": [2, 64], "gain": True, "gradient": True, "twin": [2, 64, 4, 128]},
+    {"family": "rotary", "x": [64, 4096], "positions": [64], "gain": True, "gradient": True, "options": {"axis": 0, "pairs": "adjacent"}},
+]
+
+
+@pytest.mark.skipif(not pathlib.Path(HIPCC).exists(), reason="hipcc is not installed")
+def test_kernels_use_no_scratch(tool, tmp_path):
+    """Compiled for gfx950 with the runner's options: no private array or spilled register in memory."""
+    r = tool("kernel-unit", {"operators": COMPILED}, timeout=120)
+    src = tmp_path / "unit.hip"
+    src.write_text(r["unit"])
+    opts = ["-O3", "-std=c++17", "-ffp-contract=off", "-fno-fast-math", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+    p = subprocess.run([HIPCC, "--offload-arch=gfx950", *opts, f"-I{KERNELS}", "--cuda-device-only", "-c", str(src), "-o", str(tmp_path / "unit.o"),
+                        "-Rpass-analysis=kernel-resource-usage"], capture_output=True, text=True, timeout=600)
+    assert p.returncode == 0, p.stderr[-2000:]
+    scratch, name = {}, None
+    for line in p.stderr.splitlines():
+        m = re.search(r"(Function Name|ScratchSize \[bytes/lane\]): (\S+)", line)
+        if m and m.group(1) == "Function Name":
+            name = m.group(2)
+        elif m:
+            scratch[name] = int(m.group(2))
+    assert set(scratch) == set(r["kernels"]) and len(scratch) > 40
+    assert not any(scratch.values()), {k: v for k, v in scratch.items() if v}
