@@ -133,6 +133,13 @@ const CUS = 256;
  * and 1001; 7.3 and 11.8, 12.8 and 16.9. Its time grows with the rows from 16 on, the pairs' hardly before 128.
  */
 const FEW_ROWS = 64;
+/**
+ * Whether losses over V classes take whole rows (tcmi_loss_narrow.h), by time, with gradients and by products of pairs (us): 8192 rows of d 256
+ * 29 and 42 (V 96), 35 and 42 (V 128); of d 1024 70 and 71, 85 and 72; 65 536 of d 512 226 and 287, 288 and 284. Without
+ * gradients: 8 and 22, 10 and 22; 23 and 37, 28 and 37; 75 and 135, 99 and 134. Of few rows (64 of d 64, V 96) 5 and 14, where
+ * few rows' own launches take 10 and 19. One workgroup walks a row's d.
+ */
+const fewClasses = (D, V) => D <= 65536 && (V <= 96 || (V <= 128 && D <= 512));
 // tcmi_gemm_f16x2.h's tiles: rows, columns and threads of each kind.
 const SMALL = 0, SQUARE = 1, WIDE = 2, TALL = 3, FOUR = 4;
 const TILES = [[64, 64, 256], [128, 128, 256], [128, 256, 512], [256, 128, 512], [64, 64, 256]];
@@ -235,11 +242,11 @@ function fewSizes(N, D, V, bias, parts) {
 }
 
 function lossMaker(z, e, bias, grad) {
-  const counts = /^([NDV]P?|NP|RT|PIECES|RB|CT|[HWG]BLOCKS|PER|[HW]CHUNKS|[HW]K|WAVES|COLS|CHUNKS|DTILES)$/;
+  const counts = /^([NDV]P?|NP|RT|PIECES|RB|CT|[HWG]BLOCKS|PER|[HW]CHUNKS|[HW]K|WAVES|COLS|CHUNKS|DTILES|CG|RC|DG)$/;
   const sizes = Object.keys(z).map((k) => (typeof z[k] === 'boolean' ? `  static constexpr bool ${k} = ${z[k]};`
     : k.endsWith('KIND') ? `  static constexpr int ${k} = ${z[k]};`
       : `  static constexpr ${counts.test(k) ? 'uint32_t' : 'size_t'} ${k} = ${z[k]}u;`)).join('\n');
-  return (kind, grid, threads, lds, call) => kernel(kind, `#include "${/few_/.test(call) ? 'tcmi_loss_few.h' : 'tcmi_loss.h'}"
+  return (kind, grid, threads, lds, call) => kernel(kind, `#include "${/narrow_/.test(call) ? 'tcmi_loss_narrow.h' : /few_/.test(call) ? 'tcmi_loss_few.h' : 'tcmi_loss.h'}"
 struct __KERNEL___s {
 ${sizes}
 };
@@ -270,7 +277,44 @@ function fewKernels(N, D, V, bias, parts, joined) {
   return { kernels, workspace };
 }
 
+/** The sizes of a loss's launch over few classes (tcmi_loss_narrow.h), and its workspace's layout. */
+function narrowSizes(N, D, V, bias, parts) {
+  const VP = align(V, 32), CG = VP / 32, DG = ceil(D, 64);
+  // 16 rows a workgroup, 32 where that leaves enough of them: 8192 rows 29.3 us by 32, 30.9 by 16; 1001 rows of d 515 33.6 and 27.7.
+  const RT = N >= 4096 ? 2 : 1;
+  // A workgroup of dw a CU.
+  const RC = align(ceil(N, Math.max(1, Math.min(ceil(N, 64), Math.floor(CUS / DG)))), 64), CHUNKS = ceil(N, RC);
+  const z = { N, D, V, VP, NP: align(N, 16 * RT), RT, CG, RC, CHUNKS, DG, BIAS: bias, VECD: D % 4 === 0, VECV: V % 4 === 0 };
+  const dw = parts.includes('dW'), db = parts.includes('dbias');
+  let at = 0;
+  const place = (name, bytes) => { z[name] = at; at = align(at + bytes, 256); };
+  place('GP', dw || db ? 4 * z.NP * VP : 0);
+  place('WPART', dw ? 4 * CHUNKS * D * VP : 0);
+  place('SUMS', db ? 4 * CHUNKS * VP : 0);
+  return { z, workspace: at };
+}
+
+function narrowKernels(N, D, V, bias, parts, joined) {
+  const { z, workspace } = narrowSizes(N, D, V, bias, parts);
+  const e = entry(joined ? parts : null);
+  const has = (p) => parts.includes(p);
+  const make = lossMaker(z, e, bias, parts.some((p) => p !== 'loss'));
+  const S = '__KERNEL___s';
+  const outs = (...names) => names.map((p) => (has(p) ? e.out(p) : 'nullptr')).join(', ');
+  const [dh, dW, db] = ['dh', 'dW', 'dbias'].map(has);
+  const kernels = [make('lossrows', [z.NP / (16 * z.RT), 1, 1], 256, `float lds[${64 * z.RT} * tcmi::narrow_ld<${S}>()]`,
+    `narrow_rows<${S}, ${has('loss')}, ${dh}, ${dW || db}>(L, ${outs('loss', 'dh')}, lds, blockIdx.x)`)];
+  if (dW || db) {
+    kernels.push(make('lossdw', [z.CHUNKS, dW ? z.DG : 1, 1], 256, `float lds[${dW ? 4 * 64 * (z.VP + 4) : 4 * z.VP}]`,
+      `narrow_dw<${S}, ${dW}, ${db}>(L, lds, blockIdx.x, blockIdx.y)`));
+    kernels.push(make('losssums', [ceil((dW ? D * z.VP / 4 : 0) + (db ? z.VP / 4 : 0), 32), 1, 1], 256, 'tcmi::f4 scratch[256]',
+      `narrow_sums<${S}, ${dW}, ${db}>(L, ${outs('dW', 'dbias')}, scratch, blockIdx.x)`));
+  }
+  return { kernels, workspace };
+}
+
 function lossKernels(N, D, V, bias, parts, joined, bytes) {
+  if (fewClasses(D, V)) return narrowKernels(N, D, V, bias, parts, joined);
   if (N <= FEW_ROWS) return fewKernels(N, D, V, bias, parts, joined);
   const { z, workspace, grad } = lossSizes(N, D, V, bias, parts, bytes);
   if (Math.max(z.DP, z.VP) > PAIR_COLS) throw new Error(`linearCrossEntropy: ${Math.max(D, V)} columns (at most ${PAIR_COLS} for more than ${FEW_ROWS} rows)`);

@@ -87,17 +87,30 @@ const CASES = [
   // Rows that are few, up to the most of them, by tiles of 64 and of 256 classes; one row more, and the same again.
   loss('row', 1, 515, 1000, { bias: true, gradient: true }),
   loss('few-odd', 33, 37, 517, { bias: true, gradient: true }),
-  loss('few-most', 64, 64, 128, { gradient: true }),
-  loss('few-classes', 17, 9, 3, { bias: true, gradient: true }),
+  loss('few-most', 64, 64, 132, { gradient: true }),
+  loss('few-classes', 17, 9, 129, { bias: true, gradient: true }),
   loss('few-wide', 9, 20, 33001, { bias: true, gradient: true }),
   loss('few-values', 49, 70, 132, {}),
-  loss('one-more', 65, 1, 1, { gradient: true }),
-  loss('more', 77, 17, 7, { bias: true, gradient: true }),
+  loss('one-more', 65, 1, 130, { gradient: true }),
+  loss('more', 77, 17, 131, { bias: true, gradient: true }),
   loss('more-deep', 100, 515, 260, { gradient: true }),
   loss('more-h', 150, 24, 300, { bias: true, gradient: true, wrt: ['h'] }),
   loss('more-W', 150, 24, 300, { bias: true, gradient: true, wrt: ['W'] }),
   loss('more-b', 150, 24, 300, { bias: true, gradient: true, wrt: ['b'] }),
   loss('more-squared', 150, 24, 300, { bias: true, gradient: true, after: true }),
+  // Classes that are few, in whole rows: one, an odd count, the most of them, one more; 16 and 32 rows a workgroup; deep and shallow.
+  loss('narrow-one', 6, 5, 1, { bias: true, gradient: true }),
+  loss('narrow-odd', 131, 37, 33, { bias: true, gradient: true }),
+  loss('narrow-most', 200, 512, 128, { gradient: true }),
+  loss('narrow-more', 200, 513, 128, { gradient: true }),
+  loss('narrow-rows', 4100, 70, 95, { bias: true, gradient: true }),
+  loss('narrow-deep', 70, 1030, 96, { bias: true, gradient: true }),
+  loss('narrow-h', 150, 24, 100, { bias: true, gradient: true, wrt: ['h'] }),
+  loss('narrow-b', 150, 24, 100, { bias: true, gradient: true, wrt: ['b'] }),
+  loss('narrow-values', 150, 24, 6, { bias: true }),
+  loss('narrow-squared', 150, 24, 100, { bias: true, gradient: true, after: true }),
+  loss('pairs-few', 77, 520, 117, { bias: true, gradient: true }),
+  loss('pairs-rows', 3001, 20, 130, { bias: true, gradient: true }),
   // Matrices from one element to several tiles, wide and tall, alone, stacked and side by side.
   orth('one', [1, 1]),
   orth('row', [1, 70]),
