@@ -378,12 +378,56 @@ function splitTiles(kind, tiles, slices) {
 /** The largest exponent that keeps values up to `top` within half's range. */
 const fits = (top) => Math.floor(Math.log2(60000 / top));
 
+/**
+ * The side up to which all steps are made on one small matrix in float64 (tcmi_orthogonalize_thin.h), what its LDS holds; by time, and by
+ * products of pairs (us, 5 steps): 8 x 8 10.9 and 51.5, 16 of 32 x 2416 24 and 144, 64 x 64 47 and 56, 64 x 4096 54 and 160, 16 of
+ * 64 x 1024 55 and 97.
+ */
+const THIN_SIDE = 64;
+
+/** Matrices with a side of at most THIN_SIDE. */
+function thinKernels(node, M, N, count) {
+  const { steps, eps, coefficients: [a, b, c] } = node.attrs;
+  const s = Math.min(M, N), l = Math.max(M, N), T = s <= 16 ? 1 : s <= 32 ? 2 : 4, SP = 16 * T, entries = T * (T + 1) / 2 * 256;
+  // A wavefront takes 16 of the long side at a time; 32 chunks are enough of them for any length that stays small beside a launch.
+  const KC = align(ceil(l, 32), 64), CHUNKS = ceil(l, KC), summed = CHUNKS > 4;
+  const z = { M, N, SIDE: s, LONG: l, T, KC, CHUNKS, STEPS: steps, TALL: M > N, VEC: N % 4 === 0, SUMMED: summed };
+  let at = 0;
+  const put = (name, bytes) => { z[name] = at; at = align(at + bytes, 256); };
+  put('PART', 8 * CHUNKS * entries);
+  put('SUM', 8 * entries);
+  put('Q', 8 * SP * SP);
+  z.PER = at;
+  const sizes = Object.keys(z).map((k) => (typeof z[k] === 'boolean' ? `  static constexpr bool ${k} = ${z[k]};`
+    : k === 'T' ? `  static constexpr int T = ${T};` : `  static constexpr ${/^(PART|SUM|Q|PER)$/.test(k) ? 'size_t' : 'uint32_t'} ${k} = ${z[k]}u;`)).join('\n');
+  const S = '__KERNEL___s';
+  const make = (kind, blocks, threads, lds, call) => kernel(kind, `#include "tcmi_orthogonalize_thin.h"
+struct __KERNEL___s {
+${sizes}
+  static __device__ __forceinline__ double a() { return ${double(a)}; }
+  static __device__ __forceinline__ double b() { return ${double(b)}; }
+  static __device__ __forceinline__ double c() { return ${double(c)}; }
+  static __device__ __forceinline__ double eps() { return ${double(eps)}; }
+};
+extern "C" __global__ void __launch_bounds__(${threads}) __KERNEL__(const TcmiArgs A) {
+  const tcmi::Thin<__KERNEL___s> o(A.in[0], A.out, A.ws, blockIdx.z);
+${lds ? `  __shared__ __attribute__((aligned(1024))) double lds[${lds}];\n` : ''}  tcmi::${call};
+}
+`, [blocks, 1, count], threads);
+  const kernels = [make('orththingram', CHUNKS, 256, 4 * entries, `thin_gram<${S}>(o, lds, blockIdx.x)`)];
+  if (summed) kernels.push(make('orththinsum', entries / 32, 256, 256, `thin_sum<${S}>(o, lds, blockIdx.x)`));
+  kernels.push(make('orththiniterate', 1, 512, 4 * SP * (SP + 2), `thin_iterate<${S}>(o, lds)`));
+  kernels.push(make('orththinapply', M > N ? ceil(M, 64) : ceil(ceil(N, 64) * T, 4), 256, null, `thin_apply<${S}>(o, blockIdx.x)`));
+  return { kind: 'orthogonalize', kernels, workspace: count * z.PER, flops: count * steps * (3 * s * s * l + s ** 3) };
+}
+
 function lowerOrthogonalize(graph, node) {
   const x = node.shape, M = x[x.length - 2], N = x[x.length - 1], count = size(x.slice(0, -2));
   const { steps, eps, coefficients: [a, b, c] } = node.attrs;
   if (count > 65535) throw new Error(`orthogonalize: ${count} matrices (at most 65535)`);
   if (Math.max(M, N) > PAIR_COLS) throw new Error(`orthogonalize: a matrix of ${M} x ${N} (at most ${PAIR_COLS} on a side)`);
   const tall = M > N, s = Math.min(M, N), l = Math.max(M, N);
+  if (s <= THIN_SIDE && steps > 0) return thinKernels(node, M, N, count);
   // Tiles of 128, or of 64 where those leave much of the chip idle.
   const tiles = (t) => ceil(s, t) * ceil(l, t) * count;
   const square = tiles(128) >= 2 * CUS;

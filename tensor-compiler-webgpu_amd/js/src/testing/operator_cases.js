@@ -123,6 +123,20 @@ const CASES = [
   orth('stack', [3, 2, 33, 20]),
   orth('twins', [96, 64], { count: 3 }),
   orth('steps', [50, 70], { options: { steps: 2, coefficients: [1.5, -0.5, 0], eps: 0 } }),
+  // Sides of 64 and one more, of each count of tiles, wide and tall, even rows of four and not; alone, stacked and side by side.
+  orth('thin-most', [64, 200]),
+  orth('thin-tall', [999, 64]),
+  orth('thin-odd', [31, 517]),
+  orth('thin-columns', [517, 31]),
+  orth('thin-47', [4099, 47]),
+  orth('thin-16', [2050, 16]),
+  orth('thin-row', [2, 9001]),
+  orth('thin-stack', [2, 3, 130, 12]),
+  orth('thin-twins', [48, 100], { count: 3 }),
+  orth('thin-steps', [70, 60], { options: { steps: 9, coefficients: [2, -1.5, 0.5], eps: 1e-3 } }),
+  orth('more-than-thin', [65, 500]),
+  orth('twins-large', [96, 70], { count: 3 }),
+  orth('stack-large', [3, 70, 90], { options: { steps: 2, coefficients: [1.5, -0.5, 0], eps: 0 } }),
   orth('none', [20, 30], { options: { steps: 0 } }),
 ];
 

@@ -149,7 +149,8 @@ COMPILED = [
     {"family": "loss", "N": 9, "d": 64, "V": 1000, "gradient": True}, {"family": "loss", "N": 128, "d": 64, "V": 96},
     {"family": "loss", "N": 8192, "d": 256, "V": 200, "bias": True, "gradient": True}, {"family": "loss", "N": 9000, "d": 63, "V": 127, "gradient": True},
     {"family": "orthogonalize", "x": [256, 256], "count": 16}, {"family": "orthogonalize", "x": [1300, 777]}, {"family": "orthogonalize", "x": [4096, 4096], "count": 2},
-    {"family": "orthogonalize", "x": [2100, 9001]},
+    {"family": "orthogonalize", "x": [2100, 9001]}, {"family": "orthogonalize", "x": [64, 4096], "count": 2}, {"family": "orthogonalize", "x": [999, 31]},
+    {"family": "orthogonalize", "x": [3000, 61]}, {"family": "orthogonalize", "x": [7, 51]},
     {"family": "rotary", "x": [2, 64, 4, 128], "positions": [2, 64], "gain": True, "gradient": True, "twin": [2, 64, 4, 128]},
     {"family": "rotary", "x": [64, 4096], "positions": [64], "gain": True, "gradient": True, "options": {"axis": 0, "pairs": "adjacent"}},
 ]
