@@ -73,3 +73,47 @@ def check(c, inputs, entry, b):
 def test_operators_match_float64(family, tmp_path, tool):
     for c, inputs, entry, b in run(tool, tmp_path, family):
         check(c, inputs, entry, b)
+
+
+# Few rows, few classes, and many of both.
+SHAPES = [(9, 16, 200), (70, 16, 40), (100, 16, 300)]
+
+
+@pytest.mark.parametrize("N, d, V", SHAPES)
+def test_targets_that_are_masked_and_rows_without_numbers(tool, tmp_path, N, d, V):
+    """A target whose class has a bias of -inf: an infinite loss, and gradients as the formula's. A row whose h is infinite or NaN: its own loss
+    and share of dh are no numbers, the other rows' are what they were. Products of at most 300 terms of magnitudes below 8, each off by
+    2^-21 + 300 / 2^24 at most: 1e-4 in all."""
+    import tcmi_bridge
+    case = {"name": "masked", "family": "loss", "N": N, "d": d, "V": V, "bias": True, "gradient": True}
+    c = tool("operator-graphs", {"cases": [case]})[0]
+    rng = np.random.default_rng(5)
+    v = {n["attrs"]["name"]: rng.standard_normal(n["shape"]).astype(np.float32) for n in c["graph"]["nodes"] if n["op"] == "input"}
+    v["W"] *= np.float32(0.3)
+    v["t"] = rng.integers(0, V, N).astype(np.float32)
+    v["t"][3] = 7
+    v["t"][v["t"] == 11] = 12
+    v["b"][[7, 11]] = -np.inf
+    v["t"][4:] = np.where(v["t"][4:] == 7, 8, v["t"][4:])
+    bad = dict(v, h=v["h"].copy())
+    bad["h"][5, 2], bad["h"][6] = np.inf, np.nan
+    print(f"gpu step: gpu-graphs, masked targets {N} x {d} x {V}", flush=True)
+    reqs = [{"name": name, "graph": c["graph"], "keep": c["keep"], "perf": True, "inputs": {k: checks.plain(x) for k, x in x.items()}}
+            for name, x in (("masked", v), ("bad", bad))]
+    tool("gpu-graphs", {"graphs": reqs}, out=str(tmp_path), timeout=300)
+    b = tcmi_bridge.Bundle(tmp_path)
+    with np.errstate(all="ignore"):
+        want = interp.evaluate(c["graph"], {k: x.astype(np.float64) for k, x in v.items()})
+    got = {}
+    for e in b.cases:
+        at = {o: i for i, o in enumerate(e["origin"])}
+        got[e["name"]] = {n: b.arr(e["gpuPerf"][str(at[k])]).astype(np.float64) for n, k in zip(c["names"], c["keep"])}
+    for n, k in zip(c["names"], c["keep"]):
+        np.testing.assert_allclose(got["masked"][n], want[k], rtol=1e-4, atol=1e-4, err_msg=n)
+    assert np.isinf(want[c["keep"][0]][3]) and np.isfinite(got["masked"]["dW"]).all()
+    rest = np.setdiff1d(np.arange(N), [5, 6])
+    assert not np.isfinite(got["bad"]["loss"][[5, 6]]).any()
+    # Up to the scale of h's pairs, which those rows' values no longer decide.
+    np.testing.assert_allclose(got["bad"]["loss"][rest], got["masked"]["loss"][rest], rtol=1e-5, atol=1e-5)
+    np.testing.assert_allclose(got["bad"]["dh"].reshape(N, d)[rest], got["masked"]["dh"].reshape(N, d)[rest], rtol=1e-5, atol=1e-5)
+    assert not np.isfinite(got["bad"]["dh"].reshape(N, d)[[5, 6]]).any()
