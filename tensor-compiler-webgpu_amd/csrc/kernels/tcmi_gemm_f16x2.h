@@ -284,16 +284,19 @@ __device__ __forceinline__ void gemm_f16x2_sum(const Pairs& a, const Pairs& b, c
   }
 }
 
-// The tile of workgroup `id` of rows x cols of them, so that the 8 XCDs (which take workgroups in
-// turn) each walk a run of tiles of their own, down `GROUP` tile rows before the next column:
-// neighbours in time share operand panels in one L2.
+// The place of workgroup `id` of n in an order whose runs stay on one XCD: the 8 XCDs take workgroups in turn, and each gets a run of
+// its own, so that neighbours in the order, which share operand panels, share an L2.
+__device__ __forceinline__ uint32_t xcd_run(uint32_t id, uint32_t n) {
+  const uint32_t per = n / 8u, left = n % 8u, x = id % 8u;
+  return x * per + min(x, left) + id / 8u;
+}
+// The tile of workgroup `id` of rows x cols of them: down GROUP tile rows before the next column.
 struct TileAt {
   uint32_t row, col;
 };
+template <uint32_t GROUP>
 __device__ __forceinline__ TileAt tile_at(uint32_t id, uint32_t rows, uint32_t cols) {
-  constexpr uint32_t GROUP = 8;
-  const uint32_t n = rows * cols, per = n / 8u, left = n % 8u, x = id % 8u;
-  const uint32_t t = x * per + min(x, left) + id / 8u;
+  const uint32_t t = xcd_run(id, rows * cols);
   const uint32_t band = t / (GROUP * cols), first = band * GROUP, tall = min(rows - first, GROUP), in = t - band * GROUP * cols;
   return {first + in % tall, in / tall};
 }
@@ -311,6 +314,8 @@ struct Tile {
   static constexpr int ROWS = WM * T * 16, COLS = WN * T * 16, THREADS = KW * 64 * WM * WN;
   static constexpr int STAGES = KIND == SQUARE || KW > 1 ? 2 : 3;
   static constexpr int LDS = KW * f16x2_lds<ROWS, COLS, STAGES>();
+  // Tile rows of a band: what the tiles that run at once on an XCD read is least where they form a square.
+  static constexpr uint32_t GROUP = KIND == TALL ? 4 : 8;
   // The fragments of 16 rows and of 16 columns that a wavefront holds.
   static constexpr int TI = T / KW, TJ = T;
   typedef f4 Sums[TI][TJ];

@@ -190,7 +190,7 @@ __device__ __forceinline__ void loss_logits(const Loss<S>& L, char* lds, uint32_
   LossState* st = L.state();
   const uint32_t piece = st->piece;
   if (block == 0 && threadIdx.x == 0) st->current = piece;
-  const TileAt tile = tile_at(block, S::NP / P::ROWS, S::VP / P::COLS);
+  const TileAt tile = tile_at<P::GROUP>(block, S::NP / P::ROWS, S::VP / P::COLS);
   Pairs a = L.h_pairs();
   a.at += (size_t)piece * S::NP * a.ld;
   typename P::Sums acc;
@@ -424,8 +424,9 @@ __device__ __forceinline__ void loss_grads(const Loss<S>& L, float* dh, float* d
   if (block == 0 && threadIdx.x == 0) st->piece = piece + 1;     // this piece is done with the next kernel
   if (DH && block < HB) {
     using P = typename G::H;
-    const uint32_t chunk = block / (G::HR * G::HC), first = chunk * S::HK, left = S::VP / 32 - first;
-    const TileAt tile = tile_at(block % (G::HR * G::HC), G::HR, G::HC);
+    // A chunk's tiles, which read the same columns of G and W, on one XCD.
+    const uint32_t at = xcd_run(block, HB), chunk = at / (G::HR * G::HC), in = at % (G::HR * G::HC), first = chunk * S::HK, left = S::VP / 32 - first;
+    const TileAt tile = {in % G::HR, in / G::HR};
     typename P::Sums acc;
     P::template sum<true, true>(L.g_pairs(), L.w_pairs(), tile, first * 32, left < S::HK ? left : S::HK, lds, acc);
     const int back = -(st->g + st->w);
@@ -436,7 +437,7 @@ __device__ __forceinline__ void loss_grads(const Loss<S>& L, float* dh, float* d
   } else if (DW && block - HB < WB) {
     using P = typename G::W;
     const uint32_t id = block - HB, chunk = id / (G::WR * G::WC), first = chunk * S::WK, left = S::NP / 32 - first;
-    const TileAt tile = tile_at(id % (G::WR * G::WC), G::WR, G::WC);
+    const TileAt tile = tile_at<P::GROUP>(id % (G::WR * G::WC), G::WR, G::WC);
     Pairs a = L.h_pairs();
     a.at += (size_t)piece * S::NP * a.ld;
     typename P::Sums acc;

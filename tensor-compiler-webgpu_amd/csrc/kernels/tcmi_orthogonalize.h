@@ -105,14 +105,24 @@ __device__ __forceinline__ void orth_split(const Orth<S>& o, double* scratch, ui
   }
 }
 
-// The tile on or above the diagonal that is workgroup `id`'s (of n·(n + 1) / 2, each XCD a run of them): column by column.
+// The tile on or above the diagonal that is workgroup `id`'s (of n·(n + 1) / 2): square after square of 8 x 8 tiles, column by
+// column of them.
 __device__ __forceinline__ TileAt upper_tile(uint32_t id, uint32_t n) {
-  const uint32_t all = n * (n + 1) / 2, per = all / 8u, left = all % 8u, x = id % 8u;
-  const uint32_t t = x * per + min(x, left) + id / 8u;
-  uint32_t col = static_cast<uint32_t>((__builtin_sqrtf(8.f * t + 1.f) - 1.f) * 0.5f);
-  while (col * (col + 1) / 2 > t) --col;
-  while ((col + 1) * (col + 2) / 2 <= t) ++col;
-  return {t - col * (col + 1) / 2, col};
+  constexpr uint32_t SIDE = 8;
+  uint32_t t = xcd_run(id, n * (n + 1) / 2);
+  for (uint32_t col = 0;; col += SIDE) {
+    const uint32_t wide = min(SIDE, n - col);
+    const uint32_t above = col * wide, all = above + wide * (wide + 1) / 2;
+    if (t >= all) {
+      t -= all;
+      continue;
+    }
+    if (t < above) return {t / (SIDE * wide) * SIDE + t % SIDE, col + t % (SIDE * wide) / SIDE};
+    t -= above;
+    uint32_t c = 0;
+    while (t > c) t -= ++c;
+    return {col + t, col + c};
+  }
 }
 
 // v at (row, col ... col + 3) of a symmetric matrix, and mirrored.
@@ -144,7 +154,7 @@ struct Symmetric {
   // The last SPLIT tiles are summed in CHUNKS chunks of EACH slices.
   static constexpr uint32_t SPLIT = POLY ? S::BSPLIT : S::GSPLIT, CHUNKS = POLY ? S::BCHUNKS : S::GCHUNKS, EACH = POLY ? S::BEACH : S::GEACH;
 
-  static __device__ __forceinline__ TileAt tile(uint32_t id) { return S::HALF ? upper_tile(id, LINES) : tile_at(id, LINES, LINES); }
+  static __device__ __forceinline__ TileAt tile(uint32_t id) { return S::HALF ? upper_tile(id, LINES) : tile_at<P::GROUP>(id, LINES, LINES); }
   // A chunk's sums of fragment (i, 0) of this lane.
   static __device__ __forceinline__ f4* part(const Orth<S>& o, uint32_t split, uint32_t chunk, int i) {
     return reinterpret_cast<f4*>(o.ws + S::PART) + ((size_t)(chunk * SPLIT + split) * (P::TI * P::TJ) + i * P::TJ) * P::THREADS + threadIdx.x;
@@ -209,7 +219,7 @@ __device__ __forceinline__ void orth_join(const Orth<S>& o, uint32_t block) {
 template <class S, int FROM, bool LAST>
 __device__ __forceinline__ void orth_apply(const Orth<S>& o, char* lds, uint32_t block) {
   using P = Tile<S::AKIND>;
-  const TileAt tile = tile_at(block, S::MP / P::ROWS, S::NP / P::COLS);
+  const TileAt tile = tile_at<P::GROUP>(block, S::MP / P::ROWS, S::NP / P::COLS);
   typename P::Sums acc;
   const Pairs x = o.xs(FROM), to = o.xs(1 - FROM);
   if constexpr (S::TALL) P::template sum<true, true>(x, o.bs(), tile, 0, (S::N + 31) / 32, lds, acc);
