@@ -124,7 +124,9 @@ function lowerRotary(graph, node) {
 
 // ---- linearCrossEntropy --------------------------------------------------------------------
 
-const LOSS_PIECE = 1 << 28;      // bytes of a piece's logits at most (a piece is 128 rows or more)
+// Bytes of a piece's logits at most (a piece is 128 rows or more): each piece reads W and adds to dW. 8192 rows of d 1024 against 65 536 classes
+// 10.08 ms by 2^28, 9.53 by 2^29, 9.52 by 2^30.
+const LOSS_PIECE = 2 ** 29;
 const LOSS_PARTS = ['dh', 'dW', 'dbias', 'loss'];
 const CUS = 256;
 /**
