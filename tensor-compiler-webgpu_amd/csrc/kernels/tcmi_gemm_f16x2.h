@@ -179,25 +179,20 @@ __device__ __forceinline__ void last_slices(uint32_t s, const uint32_t slices, F
 
 // The BM x BN = (WM·TM·16) x (WN·TN·16) tile of A·B at (m0, n0), summed over `slices` (1 or more) slices of 32 k
 // from k0: lane (t, q) = (lane % 16, lane / 16) of wavefront (wm, wn) holds in acc[i][j] row
-// m0 + (wm·TM + i)·16 + t, columns n0 + (wn·TN + j)·16 + 4q ... + 3. STAGES - 1 slices are loaded ahead. With KW > 1, KW
-// wavefronts (WM = WN = 1) sum a part of the slices each, waiting for their own loads alone; their sums are added in
-// order, and wavefront g holds the fragments i = 0 .. TM/KW - 1 of rows from g·TM/KW on. lds: KW·f16x2_lds() bytes.
-template <int WM, int WN, int TM, int TN, bool AKC, bool BKC, int STAGES = 2, int KW = 1>
+// m0 + (wm·TM + i)·16 + t, columns n0 + (wn·TN + j)·16 + 4q ... + 3. STAGES - 1 slices are loaded ahead. lds: f16x2_lds() bytes.
+template <int WM, int WN, int TM, int TN, bool AKC, bool BKC, int STAGES = 2>
 __device__ __forceinline__ void gemm_f16x2_sum(const Pairs& a, const Pairs& b, const uint32_t m0, const uint32_t n0, const uint32_t k0,
-                                               const uint32_t slices, char* lds, f4 (&out)[TM / KW][TN]) {
+                                               const uint32_t slices, char* lds, f4 (&acc)[TM][TN]) {
   constexpr int WAVES = WM * WN, BM = WM * TM * 16, BN = WN * TN * 16;
   using SA = PairStage<AKC, BM, WAVES>;
   using SB = PairStage<BKC, BN, WAVES>;
   constexpr int BUF = SA::BYTES + SB::BYTES, LOADS = SA::LOADS + SB::LOADS;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % WAVES;
-  const uint32_t group = KW == 1 ? 0u : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / WAVES;
-  const uint32_t each = (slices + KW - 1) / KW, first = group * each;
-  if constexpr (KW > 1) lds += group * STAGES * BUF;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   SA sa;
   SB sb;
-  sa.begin(a, m0, k0 + 32 * first, wave / WN * TM * 16, wave, lane);
-  sb.begin(b, n0, k0 + 32 * first, wave % WN * TN * 16, wave, lane);
-  f4 acc[TM][TN], low[TM][TN];
+  sa.begin(a, m0, k0, wave / WN * TM * 16, wave, lane);
+  sb.begin(b, n0, k0, wave % WN * TN * 16, wave, lane);
+  f4 low[TM][TN];
 #pragma unroll
   for (int i = 0; i < TM; ++i)
 #pragma unroll
@@ -242,46 +237,14 @@ __device__ __forceinline__ void gemm_f16x2_sum(const Pairs& a, const Pairs& b, c
     buf = buf + 1 == STAGES ? 0 : buf + 1;
     multiply(from, lds + fill * BUF, more);
   };
-  if constexpr (KW == 1) {
-    uint32_t s = 0;
-    for (uint32_t k = 0; k < STAGES - 1 && k < slices; ++k) load(lds + fill * BUF);
-    for (; s + STAGES - 1 < slices; ++s) slice(Ahead<STAGES - 2>(), true);
-    last_slices<STAGES - 2>(s, slices, slice);
-  } else {
-    static_assert(STAGES == 2 && WAVES == 1, "a slice ahead, and nobody else's");
-    const uint32_t mine = first < slices ? min(each, slices - first) : 0u;
-    if (mine > 0) load(lds);
-    for (uint32_t s = 0; s < mine; ++s) {
-      arrived<0>();
-      multiply(lds + (s & 1) * BUF, lds + ((s + 1) & 1) * BUF, s + 1 < mine);
-    }
-  }
+  uint32_t s = 0;
+  for (uint32_t k = 0; k < STAGES - 1 && k < slices; ++k) load(lds + fill * BUF);
+  for (; s + STAGES - 1 < slices; ++s) slice(Ahead<STAGES - 2>(), true);
+  last_slices<STAGES - 2>(s, slices, slice);
 #pragma unroll
   for (int i = 0; i < TM; ++i)
 #pragma unroll
-    for (int j = 0; j < TN; ++j) {
-      acc[i][j] += low[i][j] * (1.f / PAIR_LO);
-      if constexpr (KW == 1) out[i][j] = acc[i][j];
-    }
-  if constexpr (KW > 1) {
-    static_assert(TM % KW == 0 && TM * TN * 64 * 16 <= STAGES * BUF, "a wavefront's sums fit its slices' LDS");
-    f4* const sums = reinterpret_cast<f4*>(lds - group * STAGES * BUF);
-#pragma unroll
-    for (int i = 0; i < TM; ++i)
-#pragma unroll
-      for (int j = 0; j < TN; ++j) reinterpret_cast<f4*>(lds)[(i * TN + j) * 64 + lane] = acc[i][j];
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < TM / KW; ++i)
-#pragma unroll
-      for (int j = 0; j < TN; ++j) {
-        const f4* at = sums + ((group * (TM / KW) + i) * TN + j) * 64 + lane;
-        f4 v = at[0];
-#pragma unroll
-        for (int g = 1; g < KW; ++g) v += at[g * (STAGES * BUF / 16)];
-        out[i][j] = v;
-      }
-  }
+    for (int j = 0; j < TN; ++j) acc[i][j] += low[i][j] * (1.f / PAIR_LO);
 }
 
 // The place of workgroup `id` of n in an order whose runs stay on one XCD: the 8 XCDs take workgroups in turn, and each gets a run of
@@ -301,29 +264,29 @@ __device__ __forceinline__ TileAt tile_at(uint32_t id, uint32_t rows, uint32_t c
   return {first + in % tall, in / tall};
 }
 
-// The tiles that kernels take: 64 x 64 by four wavefronts of 32 x 32 (SMALL), or by four that compute all of it over a
-// quarter of K each (FOUR); 128 x 128 by four of 64 x 64 (SQUARE); 128 x 256 (WIDE) and 256 x 128 (TALL) by eight. At 4096^3 SQUARE
-// takes 370 us, WIDE and TALL 352 - 365; 1024 x 1024 x 65536 448 and 417 - 425. The 64 x 64 ones are for products whose larger tiles
-// would leave CUs idle, FOUR where even those do and K is long: a wavefront of 32 x 32 reads 8 KiB of LDS for 192 cycles of
-// products, one of 64 x 64 16 KiB for 768 (91 tiles of K 1300: 20.5 us by SMALL, 16.1 by FOUR; 160 of K 256 6.3 and 9.3).
-enum { SMALL = 0, SQUARE = 1, WIDE = 2, TALL = 3, FOUR = 4 };
+// The tiles that kernels take: 64 x 64 by four wavefronts of 32 x 32 (SMALL); 128 x 128 by four of 64 x 64 (SQUARE); 128 x 256 (WIDE)
+// and 256 x 128 (TALL) by eight. At 4096^3 SQUARE takes 370 us, WIDE and TALL 352 - 365; 1024 x 1024 x 65536 448 and 417 - 425. SMALL is
+// for products whose larger tiles would leave CUs idle: its wavefronts read 8 KiB of LDS for 192 cycles of products, the others' 16 KiB for 768, so
+// that a full chip of them runs at 245 TFLOP/s; one a CU takes 0.3 us a slice, whose 16 KiB come at that rate. Neither loads further
+// ahead nor a slice's fragments read while the one before is multiplied shorten that (25 slices 10.5 and 9.5 us, 8 slices 7.6 and 7.7).
+enum { SMALL = 0, SQUARE = 1, WIDE = 2, TALL = 3 };
 template <int KIND>
 struct Tile {
-  static constexpr int T = KIND == SMALL ? 2 : 4, KW = KIND == FOUR ? 4 : 1;
-  static constexpr int WM = KIND == TALL ? 4 : KIND == FOUR ? 1 : 2, WN = KIND == WIDE ? 4 : KIND == FOUR ? 1 : 2;
-  static constexpr int ROWS = WM * T * 16, COLS = WN * T * 16, THREADS = KW * 64 * WM * WN;
-  static constexpr int STAGES = KIND == SQUARE || KW > 1 ? 2 : 3;
-  static constexpr int LDS = KW * f16x2_lds<ROWS, COLS, STAGES>();
+  static constexpr int T = KIND == SMALL ? 2 : 4;
+  static constexpr int WM = KIND == TALL ? 4 : 2, WN = KIND == WIDE ? 4 : 2;
+  static constexpr int ROWS = WM * T * 16, COLS = WN * T * 16, THREADS = 64 * WM * WN;
+  static constexpr int STAGES = KIND == SQUARE ? 2 : 3;
+  static constexpr int LDS = f16x2_lds<ROWS, COLS, STAGES>();
   // Tile rows of a band: what the tiles that run at once on an XCD read is least where they form a square.
   static constexpr uint32_t GROUP = KIND == TALL ? 4 : 8;
   // The fragments of 16 rows and of 16 columns that a wavefront holds.
-  static constexpr int TI = T / KW, TJ = T;
+  static constexpr int TI = T, TJ = T;
   typedef f4 Sums[TI][TJ];
 
   // The tile's sums over `slices` slices from k0.
   template <bool AKC, bool BKC>
   static __device__ __forceinline__ void sum(const Pairs& a, const Pairs& b, const TileAt& at, uint32_t k0, uint32_t slices, char* lds, Sums& acc) {
-    gemm_f16x2_sum<WM, WN, T, T, AKC, BKC, STAGES, KW>(a, b, at.row * ROWS, at.col * COLS, k0, slices, lds, acc);
+    gemm_f16x2_sum<WM, WN, T, T, AKC, BKC, STAGES>(a, b, at.row * ROWS, at.col * COLS, k0, slices, lds, acc);
   }
   // The row, and the first column, of this lane's first four sums: fragment (i, j)'s 16·i rows and 16·j columns on.
   static __device__ __forceinline__ uint32_t row(const TileAt& at) { return at.row * ROWS + threadIdx.x / 64 / WN * TI * 16 + threadIdx.x % 16; }

@@ -22,7 +22,7 @@
 
 namespace tcmi {
 
-// S: the sizes of one launch as constants of its text: M, N; GKIND, BKIND, AKIND of tiles for A, B and X; HALF; MP, NP padded to whole tiles (SP: the
+// S: the sizes of one launch as constants of its text: M, N; KIND of tiles for A and B, AKIND for X; HALF; MP, NP padded to whole tiles (SP: the
 // smaller's); GSPLIT, GCHUNKS, GEACH and BSPLIT, BCHUNKS, BEACH: A's and B's split tiles; TALL; BLOCKS of the norm; SX, SA, SB exponents of the scales; VEC: N a multiple of 4; a(), b(), c(), eps().
 // WS: byte offsets in one matrix's workspace, PER bytes.
 template <class S>
@@ -147,7 +147,7 @@ constexpr float two_to(int e) { return e < 0 ? 1.f / static_cast<float>(1ull << 
 // One of the two symmetric products: POLY B = b·A + c·A·A, else A = X·Xᵀ (TALL: Xᵀ·X) of X number FROM.
 template <class S, bool POLY, int FROM>
 struct Symmetric {
-  using P = Tile<POLY ? S::BKIND : S::GKIND>;
+  using P = Tile<S::KIND>;
   static constexpr bool KC = POLY || !S::TALL;
   static constexpr uint32_t SLICES = ((POLY == S::TALL ? S::N : S::M) + 31) / 32;
   static constexpr uint32_t LINES = S::SP / P::ROWS, TILES = S::HALF ? LINES * (LINES + 1) / 2 : LINES * LINES;

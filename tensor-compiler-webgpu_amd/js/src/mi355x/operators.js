@@ -10,7 +10,7 @@
 
 const { size } = require('../ir/shapes');
 const { singularBound } = require('../ir/operators');
-const { kernelText, XCD_GROUPED } = require('./codegen');
+const { kernelText, XCD_GROUPED, MAX_BATCH } = require('./codegen');
 
 const ceil = (a, b) => Math.ceil(a / b);
 const OPERATORS = new Set(['rotary', 'rotaryGrad', 'linearCrossEntropy', 'linearCrossEntropyGrad', 'orthogonalize']);
@@ -143,10 +143,27 @@ const FEW_ROWS = 64;
  */
 const fewClasses = (D, V) => D <= 65536 && (V <= 96 || (V <= 128 && D <= 512));
 // tcmi_gemm_f16x2.h's tiles: rows, columns and threads of each kind.
-const SMALL = 0, SQUARE = 1, WIDE = 2, TALL = 3, FOUR = 4;
-const TILES = [[64, 64, 256], [128, 128, 256], [128, 256, 512], [256, 128, 512], [64, 64, 256]];
-/** The 64 x 64 tiles' kind for a product of so many workgroups and slices of K: 160 of 8 slices 6.3 us by SMALL, 9.3 by FOUR; 91 of 41 20.5 and 16.1. */
-const smallKind = (blocks, slices) => (blocks <= CUS && slices >= 32 ? FOUR : SMALL);
+const SMALL = 0, SQUARE = 1, WIDE = 2, TALL = 3;
+const TILES = [[64, 64, 256], [128, 128, 256], [128, 256, 512], [256, 128, 512]];
+/**
+ * The time (us) of a product of `tiles` tiles of `slices` slices of 32 k, K in chunks of `each` slices. 64 x 64 tiles: a slice of one a CU 0.3, of a
+ * full chip 0.275 a CU; larger ones (256 x 128, one a CU) 1.3. Starting and ending a tile: 3.4 and 6.
+ */
+function productTime(large, tiles, slices, each) {
+  const all = tiles * ceil(slices, each), rounds = all / CUS;
+  return large ? Math.max(1, rounds < 4 ? Math.ceil(rounds) : rounds) * (1.3 * each + 6) : 3.4 + each * Math.max(0.3, 0.275 * rounds);
+}
+/** How K is split for the least time: { chunks, each, time }. Partial sums (of tiles of so many elements) are written and read by one more launch, at 8 TB/s up to 32 MB, at 4 beyond. */
+function splitK(large, tiles, slices, elements, least) {
+  let best = null;
+  for (let c = 1; c <= Math.min(64, Math.max(1, Math.floor(slices / least))); c++) {
+    const each = ceil(slices, c), chunks = ceil(slices, each);
+    const bytes = 8 * chunks * tiles * elements;
+    const time = productTime(large, tiles, slices, each) + (chunks > 1 ? bytes / (bytes > 2 ** 25 ? 4e6 : 8e6) + 3.5 : 0);
+    if (!best || time < best.time) best = { chunks, each, time };
+  }
+  return best;
+}
 
 /** A product's kernel keeps two wavefronts a SIMD, 256 registers each. */
 const bounds = (threads, lds) => (/Tile/.test(lds || '') ? ', 2' : '');
@@ -159,7 +176,7 @@ const PAIR_COLS = 2 ** 22;
 function lossSizes(N, D, V, bias, parts, piece) {
   const grad = parts.some((p) => p !== 'loss');
   // The large tiles are 128 x 256; padding of up to 256 columns and rows is little beside 2048 and 512.
-  const DP = align(D, 128), VP = align(V, V > 2048 ? 256 : 128), rows = N > 512 ? 256 : 128;
+  const VP = align(V, V > 2048 ? 256 : 128), rows = N > 512 ? 256 : 128;
   // The rows of a piece: its logits, or without gradients a row's pair of statistics for each 64 columns.
   const row = grad ? 4 * VP : VP / 8;
   const most = Math.max(rows, Math.floor((piece || LOSS_PIECE) / row / rows) * rows);
@@ -171,10 +188,10 @@ function lossSizes(N, D, V, bias, parts, piece) {
   // pieces. The gradients' tiles and the chunks of K by time.
   const large = VP % 256 === 0 && rows === 256 && align(N, 256) / 128 * (VP / 256) >= CUS / 2;
   const LT = large ? 4 : 2;
-  const g = gradTiles(NP, DP, VP);
+  const g = gradTiles(NP, D, VP), DP = grad ? g.DP : align(D, 64);
   const CT = (() => { let t = 16; while (2 * t <= Math.min(256, VP / 8)) t *= 2; return t; })();
   const z = { N, D, V, DP, VP, NP, PIECES, RB, CT, BIAS: bias, HBLOCKS: clamp(N * D / 4096, 256), WBLOCKS: clamp(D * V / 16384, 1024), GBLOCKS: clamp(N / 1024, 64),
-    PER: clamp((NP * PIECES * DP + DP * VP) / 4 / 256 / 1024, 16), LKIND: large ? TALL : smallKind(align(N, 64) / 64 * (VP / 64), DP / 32), HKIND: g.large ? TALL : SMALL, WKIND: g.large ? WIDE : SMALL, JOINED: !grad || VP / (16 * LT) > 32, VECD: D % 4 === 0, VECV: V % 4 === 0,
+    PER: clamp((NP * PIECES * DP + DP * VP) / 4 / 256 / 1024, 16), LKIND: large ? TALL : SMALL, HKIND: g.large ? TALL : SMALL, WKIND: g.large ? WIDE : SMALL, JOINED: !grad || VP / (16 * LT) > 32, VECD: D % 4 === 0, VECV: V % 4 === 0,
     HCHUNKS: g.h.chunks, HK: g.h.each, WCHUNKS: g.w.chunks, WK: g.w.each };
   let at = 0;
   const place = (name, bytes) => { z[name] = at; at = align(at + bytes, 256); };
@@ -194,34 +211,19 @@ function lossSizes(N, D, V, bias, parts, piece) {
 }
 
 /**
- * The tiles of dh [NP, d] over V and of dW [d, V] over NP, and the chunks their K is split
- * into: those of the least estimated time, by how many rounds of workgroups the tiles of a product
- * take (one of 256 x 128 a CU, two of 64 x 64). Measured (us): a slice of a large tile 1.2, of a small one
- * 0.3; starting and ending a tile 6 and 4; a partial sum is written and read at 4 TB/s. Every
- * choice depends on the sizes alone, not on which gradients a launch forms.
+ * The tiles of dh [NP, d] over V and of dW [d, V] over NP, and the chunks their K is split into: those of the least estimated time, by
+ * the sizes alone, not by which gradients a launch forms. 1808 rows of d 907, 15 840 classes: 546 us by 64 x 64 tiles, 374 by 256 x 128.
  */
-function gradTiles(NP, DP, VP) {
-  const time = (large, tiles, slices, chunks, elements) => {
-    const each = ceil(slices, chunks), rounds = tiles * ceil(slices, each) / (large ? CUS : 2 * CUS);
-    return Math.max(1, rounds < 4 ? Math.ceil(rounds) : rounds) * (each * (large ? 1.2 : 0.3) + (large ? 6 : 4)) + (chunks > 1 ? 8 * chunks * elements / 4e6 + 3 : 0);
-  };
-  const best = (large, tiles, slices, elements) => {
-    let b = null;
-    for (let c = 1; c <= Math.min(64, Math.max(1, Math.floor(slices / 4))); c++) {
-      const t = time(large, tiles, slices, c, elements);
-      if (!b || t < b.t) b = { t, chunks: ceil(slices, ceil(slices, c)), each: ceil(slices, c) };
-    }
-    return b;
-  };
+function gradTiles(NP, D, VP) {
   const of = (large) => {
-    const [hr, hc, wr, wc] = large ? [256, 128, 128, 256] : [64, 64, 64, 64];
-    const h = best(large, NP / hr * (DP / hc), VP / 32, NP * DP), w = best(large, DP / wr * (VP / wc), NP / 32, DP * VP);
-    return { large, h, w, t: h.t + w.t };
+    const [hr, hc, wr, wc] = large ? [256, 128, 128, 256] : [64, 64, 64, 64], DP = align(D, large ? 128 : 64);
+    const h = splitK(large, NP / hr * (DP / hc), VP / 32, hr * hc, 4), w = splitK(large, DP / wr * (VP / wc), NP / 32, wr * wc, 4);
+    return { large, DP, h, w, time: h.time + w.time };
   };
   const small = of(false);
   if (NP % 256 || VP % 256) return small;
   const large = of(true);
-  return small.t < large.t ? small : large;
+  return small.time < large.time ? small : large;
 }
 
 /** The sizes of a loss's launch over few rows (tcmi_loss_few.h), and its workspace's layout. */
@@ -367,12 +369,18 @@ function lowerLoss(graph, node, tuning) {
 // ---- orthogonalize -------------------------------------------------------------------------
 
 /**
- * Which of a symmetric product's tiles are split along K: those left over when the rest fill the chip (two workgroups a CU)
- * a whole number of times, into as many chunks of 8 slices or more as fill it once more.
+ * Which of a symmetric product's tiles are split along K, of each of `count` matrices: by 128 x 128 tiles those left over when the rest fill the
+ * chip (two workgroups a CU) a whole number of times, into as many chunks of 8 slices or more as fill it once more; by 64 x 64 tiles all or none,
+ * by time (25 tiles of 114 slices: 38 us whole, 11 in chunks with their sums).
  */
-function splitTiles(kind, tiles, slices) {
-  const split = tiles % (2 * CUS), chunks = kind === SQUARE && split ? Math.min(Math.floor(2 * CUS / split), Math.floor(slices / 8)) : 1;
-  if (chunks < 2) return { split: 0, chunks: 1, each: slices };
+function splitTiles(kind, tiles, slices, count) {
+  const none = { split: 0, chunks: 1, each: slices };
+  if (kind === SMALL) {
+    const s = splitK(false, tiles * count, slices, 64 * 64, 4);
+    return s.chunks > 1 ? { split: tiles, chunks: s.chunks, each: s.each, time: s.time } : Object.assign(none, { time: s.time });
+  }
+  const split = Math.floor(tiles * count % (2 * CUS) / count), chunks = split ? Math.min(Math.floor(2 * CUS / (split * count)), Math.floor(slices / 8)) : 1;
+  if (chunks < 2) return none;
   const each = ceil(slices, chunks);
   return { split, chunks: ceil(slices, each), each };
 }
@@ -430,19 +438,21 @@ function lowerOrthogonalize(graph, node) {
   if (Math.max(M, N) > PAIR_COLS) throw new Error(`orthogonalize: a matrix of ${M} x ${N} (at most ${PAIR_COLS} on a side)`);
   const tall = M > N, s = Math.min(M, N), l = Math.max(M, N);
   if (s <= THIN_SIDE && steps > 0) return thinKernels(node, M, N, count);
-  // Tiles of 128, or of 64 where those leave much of the chip idle.
-  const tiles = (t) => ceil(s, t) * ceil(l, t) * count;
-  const square = tiles(128) >= 2 * CUS;
+  // Tiles of 128, or of 64 where those leave much of the chip idle, counting the graph's equal nodes: they run side by side.
+  const equal = graph.nodes.filter((n) => n.op === 'orthogonalize' && n.shape.join() === x.join() && JSON.stringify(n.attrs) === JSON.stringify(node.attrs)).length;
+  const alike = count * Math.min(equal, MAX_BATCH);
+  const square = ceil(s, 128) * ceil(l, 128) * alike >= 2 * CUS;
   const pad = square ? 128 : 64, MP = align(M, pad), NP = align(N, pad), SP = Math.min(MP, NP);
-  const n = SP / pad, upper = n * (n + 1) / 2, all = MP / pad * (NP / pad);
-  const kind = (blocks, K) => (square ? SQUARE : smallKind(blocks * count, K / 32));
-  const half = square || n * n * count > CUS, tilesOf = half ? upper : n * n;
-  const GKIND = kind(tilesOf, l), BKIND = kind(tilesOf, s);
-  const AKIND = square && MP % 256 === 0 ? TALL : square && NP % 256 === 0 ? WIDE : kind(all, s);
+  const n = SP / pad, kind = square ? SQUARE : SMALL, upper = n * (n + 1) / 2;
+  const AKIND = square && MP % 256 === 0 ? TALL : square && NP % 256 === 0 ? WIDE : kind;
   const ablocks = MP / TILES[AKIND][0] * (NP / TILES[AKIND][1]);
-  const G = splitTiles(GKIND, tilesOf, ceil(l, 32)), B = splitTiles(BKIND, tilesOf, ceil(s, 32));
+  const splits = (t) => [splitTiles(kind, t, ceil(l, 32), alike), splitTiles(kind, t, ceil(s, 32), alike)];
+  // All tiles where that costs no time (a mirrored tile's scattered writes take 1.5 us).
+  const time = (t) => splits(t).reduce((q, x) => q + x.time, 0);
+  const half = square || time(upper) + 3 < time(n * n), tilesOf = half ? upper : n * n;
+  const [G, B] = splits(tilesOf);
   const top = singularBound(node.attrs);
-  const z = { M, N, MP, NP, SP, GKIND, BKIND, AKIND, HALF: half, TALL: tall, VEC: N % 4 === 0, BLOCKS: Math.min(256, ceil(M * N, 4096)),
+  const z = { M, N, MP, NP, SP, KIND: kind, AKIND, HALF: half, TALL: tall, VEC: N % 4 === 0, BLOCKS: Math.min(256, ceil(M * N, 4096)),
     GSPLIT: G.split, GCHUNKS: G.chunks, GEACH: G.each, BSPLIT: B.split, BCHUNKS: B.chunks, BEACH: B.each,
     SX: fits(top), SA: fits(top ** 2), SB: Math.max(-60, Math.min(60, fits(Math.max(Math.abs(b) * top ** 2 + Math.abs(c) * top ** 4, 2 ** -40)))) };
   let at = 0;
@@ -452,11 +462,10 @@ function lowerOrthogonalize(graph, node) {
   put('X1', steps > 1 ? 4 * MP * NP : 0);
   put('A', steps > 0 ? 4 * SP * SP : 0);
   put('B', steps > 0 ? 4 * SP * SP : 0);
-  const partial = (kind, t) => 4 * TILES[kind][0] * TILES[kind][1] * t.split * t.chunks;
-  put('PART', steps > 0 ? Math.max(partial(GKIND, G), partial(BKIND, B)) : 0);
+  put('PART', steps > 0 ? 4 * pad * pad * Math.max(G.split * G.chunks, B.split * B.chunks) : 0);
   z.PER = at;
   const sizes = Object.keys(z).map((k) => (typeof z[k] === 'boolean' ? `  static constexpr bool ${k} = ${z[k]};`
-    : ['GKIND', 'BKIND', 'AKIND', 'SX', 'SA', 'SB'].includes(k) ? `  static constexpr int ${k} = ${z[k]};`
+    : ['KIND', 'AKIND', 'SX', 'SA', 'SB'].includes(k) ? `  static constexpr int ${k} = ${z[k]};`
       : `  static constexpr ${/^([MNS]P?|BLOCKS|[GB](SPLIT|CHUNKS|EACH))$/.test(k) ? 'uint32_t' : 'size_t'} ${k} = ${z[k]}u;`)).join('\n');
   const S = '__KERNEL___s', place = square ? 'blockIdx' : 'wg';
   const make = (kind, blocks, threads, lds, call) => kernel(kind, `#include "tcmi_orthogonalize.h"
@@ -476,10 +485,10 @@ ${lds ? `  __shared__ __attribute__((aligned(1024))) ${lds};\n` : ''}  tcmi::${c
   const kernels = [make('orthnorm', z.BLOCKS, 256, 'double scratch[4]', `orth_norm<${S}>(o, scratch, ${place}.x)`),
     make('orthsplit', ceil(MP * NP, 4096), 256, 'double scratch[4]', `orth_split<${S}, ${steps === 0}>(o, scratch, ${place}.x)`)];
   for (let k = 0; k < steps; k++) {
-    for (const [poly, kind, t] of [[false, GKIND, G], [true, BKIND, B]]) {
+    for (const [poly, t] of [[false, G], [true, B]]) {
       const from = poly ? 0 : k % 2, name = poly ? 'poly' : 'gram';
       kernels.push(make(`orth${name}`, tilesOf + t.split * (t.chunks - 1), TILES[kind][2], pool(kind), `orth_symmetric<${S}, ${poly}, ${from}>(o, lds, ${place}.x)`));
-      if (t.split) kernels.push(make(`orthjoin${name}`, t.split * (TILES[kind][0] === 128 ? 4 : kind === FOUR ? 1 : 2), TILES[kind][2], null, `orth_join<${S}, ${poly}>(o, ${place}.x)`));
+      if (t.split) kernels.push(make(`orthjoin${name}`, t.split * (square ? 4 : 2), TILES[kind][2], null, `orth_join<${S}, ${poly}>(o, ${place}.x)`));
     }
     kernels.push(make('orthapply', ablocks, TILES[AKIND][2], pool(AKIND), `orth_apply<${S}, ${k % 2}, ${k === steps - 1}>(o, lds, ${place}.x)`));
   }
