@@ -189,7 +189,8 @@ function lossSizes(N, D, V, bias, parts, piece) {
   const large = VP % 256 === 0 && rows === 256 && align(N, 256) / 128 * (VP / 256) >= CUS / 2;
   const LT = large ? 4 : 2;
   const g = gradTiles(NP, D, VP), DP = grad ? g.DP : align(D, 64);
-  const CT = (() => { let t = 16; while (2 * t <= Math.min(256, VP / 8)) t *= 2; return t; })();
+  // Threads across columns: fewer, and rows side by side, where workgroups would be fewer than two a CU.
+  const CT = (() => { let t = 16; while (2 * t <= Math.min(256, VP / 8) && ceil(VP, 16 * t) * NP / RB >= 2 * CUS) t *= 2; return t; })();
   const z = { N, D, V, DP, VP, NP, PIECES, RB, CT, BIAS: bias, HBLOCKS: clamp(N * D / 4096, 256), WBLOCKS: clamp(D * V / 16384, 1024), GBLOCKS: clamp(N / 1024, 64),
     PER: clamp((NP * PIECES * DP + DP * VP) / 4 / 256 / 1024, 16), LKIND: large ? TALL : SMALL, HKIND: g.large ? TALL : SMALL, WKIND: g.large ? WIDE : SMALL, JOINED: !grad || VP / (16 * LT) > 32, VECD: D % 4 === 0, VECV: V % 4 === 0,
     HCHUNKS: g.h.chunks, HK: g.h.each, WCHUNKS: g.w.chunks, WK: g.w.each };
