@@ -10,11 +10,14 @@
 // is as large as what the product that reads it leaves out. x keeps its layout:
 // a tall X is read transposed by its products, never written so.
 //
-// A and B are symmetric: only tiles on and above the diagonal are computed, and written twice, where tiles are many; where
-// all of them fit the chip at once (HALF false), computing each takes no longer and spares the scattered mirrored writes.
+// A and B are symmetric: only tiles on and above the diagonal are computed, and written twice; all of them (HALF false) where
+// that takes no longer, for few tiles, and spares the scattered mirrored writes. K is split over workgroups where tiles are few, or few are left
+// over, and `join` adds the parts.
 // The norm is summed in float64: no float's square overflows or vanishes.
 //
-// Bound: the matrix cores, s²·l + s³ + 2·s²·l flops a step (s, l: the smaller and larger of M, N).
+// Bound: the matrix cores, s²·l + s³ + 2·s²·l flops a step (s, l: the smaller and larger of M, N). Two of 4096 x 4096, us: norm 41,
+// split 45 (6.0 TB/s), and a step A 363 - 377 (380 TFLOP/s of the tiles computed), its join 16, B 370 - 387
+// and 16, X 690 - 718 (390 TFLOP/s).
 
 #pragma once
 

