@@ -179,7 +179,8 @@ function lossSizes(N, D, V, bias, parts, piece) {
   const VP = align(V, V > 2048 ? 256 : 128), rows = N > 512 ? 256 : 128;
   // The rows of a piece: its logits, or without gradients a row's pair of statistics for each 64 columns.
   const row = grad ? 4 * VP : VP / 8;
-  const most = Math.max(rows, Math.floor((piece || LOSS_PIECE) / row / rows) * rows);
+  // (At most 2^20 rows of logits: `spread` counts them by 32 in its grid's second extent.)
+  const most = Math.max(rows, Math.min(grad ? 2 ** 20 : Infinity, Math.floor((piece || LOSS_PIECE) / row / rows) * rows));
   const PIECES = ceil(align(N, rows), most), NP = align(ceil(N, PIECES), rows);
   const RB = NP * VP >= 2 ** 20 ? 32 : 16;
   const clamp = (n, most) => Math.max(1, Math.min(Math.ceil(n), most));

@@ -14,10 +14,11 @@ MODERN = {"positions": "rotary", "qkNorm": True, "targets": "classes"}
 SIZES = {"T": 32, "d": 64, "H": 4, "dh": 16, "L": 2, "ff": 160}
 
 
-@pytest.mark.parametrize("attention, graph, arena", [(False, False, False), (True, True, False), (True, True, True)])
-def test_trainer_is_the_checked_path_bit_for_bit(tool, attention, graph, arena):
+@pytest.mark.parametrize("attention, graph, arena, streams", [(False, False, False, 1), (True, True, False, 1), (True, True, True, 1), (True, False, False, 2)])
+def test_trainer_is_the_checked_path_bit_for_bit(tool, attention, graph, arena, streams):
+    """Over several streams every launch runs by itself, an operator's parts too."""
     req = {"model": "transformer", "B": 5, "V": 301, "opt": "muon", "cfg": dict(SIZES, **MODERN), "attention": attention, "graph": graph, "arena": arena,
-           "steps": 4, "consistency": True, "consistencySteps": 4}
+           "streams": streams, "steps": 4, "consistency": True, "consistencySteps": 4}
     print(f"gpu step: gpu-train {req}", flush=True)
     r = tool("gpu-train", req, timeout=300)
     assert r["identical"], r["losses"]
