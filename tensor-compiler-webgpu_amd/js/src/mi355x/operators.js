@@ -184,11 +184,12 @@ function lossSizes(N, D, V, bias, parts, piece) {
   const PIECES = ceil(align(N, rows), most), NP = align(ceil(N, PIECES), rows);
   const RB = NP * VP >= 2 ** 20 ? 32 : 16;
   const clamp = (n, most) => Math.max(1, Math.min(Math.ceil(n), most));
-  // Large tiles (1024 x 65536 of K 1024: 256 x 128 395 us, 128 x 256 426, 128 x 128 460) unless they would leave much of the chip
-  // idle, by all rows: a loss has the same bits whatever its
-  // pieces. The gradients' tiles and the chunks of K by time.
-  const large = VP % 256 === 0 && rows === 256 && align(N, 256) / 128 * (VP / 256) >= CUS / 2;
+  // Large tiles (1024 x 65536 of K 1024: 256 x 128 395 us, 128 x 256 426, 128 x 128 460) or 64 x 64, by time and by all rows: a
+  // loss has the same bits whatever its pieces.
+  const slices = ceil(D, 32), rowsAll = align(N, 256);
+  const large = VP % 256 === 0 && rows === 256 && productTime(true, rowsAll / 256 * (VP / 128), slices, slices) < productTime(false, rowsAll / 64 * (VP / 64), slices, slices);
   const LT = large ? 4 : 2;
+  // The gradients' tiles and the chunks of K by time.
   const g = gradTiles(NP, D, VP), DP = grad ? g.DP : align(D, 64);
   // Threads across columns: fewer, and rows side by side, where workgroups would be fewer than two a CU.
   const CT = (() => { let t = 16; while (2 * t <= Math.min(256, VP / 8) && ceil(VP, 16 * t) * NP / RB >= 2 * CUS) t *= 2; return t; })();
