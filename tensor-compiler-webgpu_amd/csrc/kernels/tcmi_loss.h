@@ -14,7 +14,7 @@
 // |w|; every operand is read from the one layout it is written in.
 //
 //   maxima   partial maxima of |h|, |W| and |w|
-//   split    h and W as pairs, padded with zeros to tiles of 128 (k to 32)
+//   split    h and W as pairs, padded with zeros to whole tiles
 //   logits   z tile by tile; each wavefront's 64 columns of a row leave (maximum, sum of
 //            exponentials), and z itself where G will be formed
 //   join     a row's pairs joined in order; the losses; (M, 1/s) a row
@@ -52,7 +52,7 @@ struct LossState {
 };
 
 // S: the sizes of one launch as constants of its text: N, D, V; NP rows a piece, PIECES of them; DP, VP: d and V padded to
-// 128 or 256; BIAS; HBLOCKS, WBLOCKS, GBLOCKS partial maxima of h, W and w; PER groups of four a thread of `split` takes; LKIND, HKIND and
+// whole tiles; BIAS; HBLOCKS, WBLOCKS, GBLOCKS partial maxima of h, W and w; PER groups of four a thread of `split` takes; LKIND, HKIND and
 // WKIND of tiles for the logits, dh and dW; RB rows a workgroup of `spread`, CT threads across columns there;
 // JOINED: `join` runs; VECD, VECV: d, V multiples of 4; HCHUNKS, HK, WCHUNKS, WK: chunks of K of dh and dW, their slices.
 // WS: byte offsets in the workspace.

@@ -11,7 +11,8 @@
 // one matrix instruction takes are 4 apart: sums take their terms in an order of their own, the result comes out in whole
 // groups of four columns.
 //
-// Bound: memory, 4·d·V bytes for the losses and 8·d·V more for the gradients.
+// Bound: memory, 4·d·V bytes for the losses and 8·d·V more for the gradients; past 32 rows the matrix cores. Of d 1024 and
+// 131 072 classes 109 us for one row, 115 for 16 (4.7 TB/s), 212 for 64 (81 TFLOP/s); with gradients 386, 394 and 591.
 
 #pragma once
 

@@ -25,8 +25,9 @@
 
 namespace tcmi {
 
-// S: the sizes of one launch as constants of its text: M, N; KIND of tiles for A and B, AKIND for X; HALF; MP, NP padded to whole tiles (SP: the
-// smaller's); GSPLIT, GCHUNKS, GEACH and BSPLIT, BCHUNKS, BEACH: A's and B's split tiles; TALL; BLOCKS of the norm; SX, SA, SB exponents of the scales; VEC: N a multiple of 4; a(), b(), c(), eps().
+// S: the sizes of one launch as constants of its text: M, N; KIND of tiles for A and B, AKIND for X; HALF; MP, NP padded to
+// whole tiles (SP: the smaller's); GSPLIT, GCHUNKS, GEACH and BSPLIT, BCHUNKS, BEACH: A's and B's split tiles; TALL; BLOCKS of
+// the norm; SX, SA, SB exponents of the scales; VEC: N a multiple of 4; a(), b(), c(), eps().
 // WS: byte offsets in one matrix's workspace, PER bytes.
 template <class S>
 struct Orth {

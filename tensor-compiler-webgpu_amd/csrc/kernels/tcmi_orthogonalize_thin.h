@@ -26,7 +26,7 @@ namespace tcmi {
 typedef double d2 __attribute__((ext_vector_type(2)));
 typedef double d4 __attribute__((ext_vector_type(4)));
 
-// S, beside M, N, TALL, VEC: SIDE (the smaller of M, N) and LONG; T (1, 2, 4) tiles of 16 in SIDE; KC of LONG a chunk, CHUNKS, SUMMED (by `sum`);
+// S, beside M, N, TALL, VEC: T (1, 2, 4) tiles of 16 in the short side; KC of the long side a chunk, CHUNKS, SUMMED (by `sum`);
 // STEPS; a(), b(), c(), eps() in float64. WS: PART, SUM, Q.
 template <class S>
 struct Thin {

@@ -153,7 +153,10 @@ function productTime(large, tiles, slices, each) {
   const all = tiles * ceil(slices, each), rounds = all / CUS;
   return large ? Math.max(1, rounds < 4 ? Math.ceil(rounds) : rounds) * (1.3 * each + 6) : 3.4 + each * Math.max(0.3, 0.275 * rounds);
 }
-/** How K is split for the least time: { chunks, each, time }. Partial sums (of tiles of so many elements) are written and read by one more launch, at 8 TB/s up to 32 MB, at 4 beyond. */
+/**
+ * How K is split for the least time: { chunks, each, time }. Partial sums (of tiles of so many elements) are written and read by one more
+ * launch, at 8 TB/s up to 32 MB, at 4 beyond.
+ */
 function splitK(large, tiles, slices, elements, least) {
   let best = null;
   for (let c = 1; c <= Math.min(64, Math.max(1, Math.floor(slices / least))); c++) {
@@ -404,7 +407,7 @@ function thinKernels(node, M, N, count) {
   const s = Math.min(M, N), l = Math.max(M, N), T = s <= 16 ? 1 : s <= 32 ? 2 : 4, SP = 16 * T, entries = T * (T + 1) / 2 * 256;
   // A wavefront takes 16 of the long side at a time; 32 chunks are enough of them for any length that stays small beside a launch.
   const KC = align(ceil(l, 32), 64), CHUNKS = ceil(l, KC), summed = CHUNKS > 4;
-  const z = { M, N, SIDE: s, LONG: l, T, KC, CHUNKS, STEPS: steps, TALL: M > N, VEC: N % 4 === 0, SUMMED: summed };
+  const z = { M, N, T, KC, CHUNKS, STEPS: steps, TALL: M > N, VEC: N % 4 === 0, SUMMED: summed };
   let at = 0;
   const put = (name, bytes) => { z[name] = at; at = align(at + bytes, 256); };
   put('PART', 8 * CHUNKS * entries);
