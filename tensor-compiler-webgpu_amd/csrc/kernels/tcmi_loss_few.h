@@ -27,13 +27,7 @@ typedef float run4 __attribute__((ext_vector_type(4), aligned(4)));
 // where it is used (placed).
 template <bool VEC>
 __device__ __forceinline__ f4 raw_four(const float* p, uint32_t c, uint32_t cols) {
-  if (cols < 4) {
-    f4 v = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int e = 0; e < 3; ++e)
-      if (c + e < cols) v[e] = p[c + e];
-    return v;
-  }
+  if (cols < 4) return f4{p[min(c, cols - 1)], p[min(c + 1, cols - 1)], p[min(c + 2, cols - 1)], 0.f};
   p += min(c, cols - 4);
   if (VEC) return *reinterpret_cast<const f4*>(p);
   const run4 x = *reinterpret_cast<const run4*>(p);
@@ -41,7 +35,11 @@ __device__ __forceinline__ f4 raw_four(const float* p, uint32_t c, uint32_t cols
 }
 template <bool VEC>
 __device__ __forceinline__ f4 placed(f4 v, uint32_t c, uint32_t cols) {
-  if (cols < 4) return v;
+  if (cols < 4) {
+#pragma unroll
+    for (int e = 0; e < 3; ++e) v[e] = c + e < cols ? v[e] : 0.f;
+    return v;
+  }
   const uint32_t over = c + 4 > cols ? c + 4 - cols : 0u;
   if (!VEC) {
     if (over & 1u) v = f4{v[1], v[2], v[3], 0.f};

@@ -24,12 +24,13 @@ typedef float run2 __attribute__((ext_vector_type(2), aligned(4)));
 
 // Two floats of a row from column c on, as raw_four and placed.
 __device__ __forceinline__ f2 raw_two(const float* p, uint32_t c, uint32_t cols) {
-  if (cols < 2) return f2{c == 0 ? p[0] : 0.f, 0.f};
+  if (cols < 2) return f2{p[0], 0.f};
   const run2 x = *reinterpret_cast<const run2*>(p + min(c, cols - 2));
   return f2{x[0], x[1]};
 }
 __device__ __forceinline__ f2 placed_two(f2 v, uint32_t c, uint32_t cols) {
-  if (cols < 2 || c + 2 <= cols) return v;
+  if (cols < 2) return f2{c == 0 ? v[0] : 0.f, 0.f};
+  if (c + 2 <= cols) return v;
   return f2{c + 1 == cols ? v[1] : 0.f, 0.f};
 }
 

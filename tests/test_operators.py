@@ -5,6 +5,7 @@ import pathlib
 import re
 import shutil
 import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -175,3 +176,20 @@ def test_kernels_use_no_scratch(tool, tmp_path):
             scratch[name] = int(m.group(2))
     assert set(scratch) == set(r["kernels"]) and len(scratch) > 40
     assert not any(scratch.values()), {k: v for k, v in scratch.items() if v}
+
+
+def test_the_smallest_losses_compile_beside_torch(tool, tmp_path):
+    """The C ABI's compiler, in a process that has torch's own copy of it loaded: rows of one to three floats, and as few classes, once ended that
+    process (rows read under a branch a float)."""
+    cases = [{"family": "loss", "N": N, "d": d, "V": V, "bias": True, "gradient": True} for N, d, V in ((63, 1, 3), (5, 2, 1), (70, 3, 2), (9, 1, 130))]
+    r = tool("kernel-unit", {"operators": cases}, timeout=120)
+    src = tmp_path / "unit.hip"
+    src.write_text(r["unit"])
+    lib = KERNELS.parents[1] / "lib" / "libtcmi.so"
+    code = f"""import ctypes, torch
+lib = ctypes.CDLL({str(lib)!r})
+lib.tcmi_set_include_dir({str(KERNELS)!r}.encode())
+lib.tcmi_set_cache_dir({str(tmp_path)!r}.encode())
+raise SystemExit(lib.tcmi_precompile(open({str(src)!r}, "rb").read(), b"", b"gfx950"))"""
+    p = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert p.returncode == 0, (p.returncode, p.stderr[-500:])
