@@ -31,6 +31,7 @@ namespace tcmi {
 // WS: byte offsets in one matrix's workspace, PER bytes.
 template <class S>
 struct Orth {
+  static_assert(S::SX >= 0 && S::SX <= 15 && S::SA >= 0 && S::SA <= 15 && S::SB >= -60 && S::SB <= 60, "two_to's exponents");
   const float* x;
   float* out;
   char* ws;
@@ -146,7 +147,8 @@ __device__ __forceinline__ void put_symmetric(const Pairs& p, const TileAt& tile
   }
 }
 
-constexpr float two_to(int e) { return e < 0 ? 1.f / static_cast<float>(1ull << -e) : static_cast<float>(1ull << e); }
+// 2^e of a normal float, -126 ... 127 (coefficients b and c near 0 take the scales' exponents past 64).
+constexpr float two_to(int e) { return __builtin_bit_cast(float, static_cast<uint32_t>(e + 127) << 23); }
 
 // One of the two symmetric products: POLY B = b·A + c·A·A, else A = X·Xᵀ (TALL: Xᵀ·X) of X number FROM.
 template <class S, bool POLY, int FROM>

@@ -265,9 +265,9 @@ function precompileGroup(group, arch, shard, shards) {
   }
   if (group === 'operators') {
     // The operators' GPU tests, in both lowerings, and the sizes they are measured at.
-    const { operatorGraph, CASES, MEASURED } = require('../src/testing/operator_cases');
+    const { operatorGraph, CASES, FORMS, MEASURED } = require('../src/testing/operator_cases');
     let n = 0;
-    for (const [k, c] of CASES.concat(MEASURED).entries()) {
+    for (const [k, c] of CASES.concat(FORMS, MEASURED).entries()) {
       if (k % (shards || 1) !== (shard || 0)) continue;
       const { graph, keep } = operatorGraph(c);
       const f = fuse(graph, { keep });
@@ -1269,9 +1269,9 @@ async function main() {
       break;
     }
     case 'operator-graphs': {
-      // The operators' test graphs: the named cases, or one case given whole.
-      const { operatorGraph, CASES } = require('../src/testing/operator_cases');
-      const cases = req.cases || CASES.filter((c) => !req.family || c.family === req.family);
+      // The operators' test graphs: the named cases, those of `forms` by name, or cases given whole.
+      const { operatorGraph, CASES, FORMS } = require('../src/testing/operator_cases');
+      const cases = req.cases || (req.forms ? FORMS.filter((c) => req.forms.includes(c.name)) : CASES.filter((c) => !req.family || c.family === req.family));
       out = cases.map((c) => {
         const { graph, keep, names } = operatorGraph(c);
         const f = fuse(graph, { keep });

@@ -1,6 +1,6 @@
 'use strict';
 // Graphs of the operators that are one node each (ir/operators.js), from plain
-// descriptions: those of their GPU tests (CASES) and of their measurement (MEASURED).
+// descriptions: those of their GPU tests (CASES; FORMS, whose tests name them) and of their measurement (MEASURED).
 //   { family: 'rotary', x, positions, gain?, gradient?, options }   a second x where `twin`
 //       gives its shape; `twice`: rotated, and the result again
 //   { family: 'loss', N, d, V, bias?, gradient?, wrt?, after? }     wrt: 'h', 'W', 'b' (default all); `after`: the
@@ -140,6 +140,12 @@ const CASES = [
   orth('none', [20, 30], { options: { steps: 0 } }),
 ];
 
+const FORMS = [
+  // Coefficients near 0 and at it, of a matrix that the products of pairs take: their scales' exponents are the largest.
+  orth('linear', [96, 100], { options: { steps: 1, coefficients: [1, 0, 0] } }),
+  orth('nearly-linear', [100, 70], { options: { steps: 2, coefficients: [0.5, -1e-12, 0] } }),
+];
+
 const r = (B, T, H, dh, axes, gradient, twin) => rotary(null, [B, T, H, dh], axes === 1 ? [B, T] : [B, T, axes],
   { gain: true, gradient, twin: [B, T, twin, dh], options: { axis: 1, base: 10000, eps: 1e-5,
     sections: axes === 1 ? [dh / 2] : [dh / 2 - 2 * Math.floor(3 * dh / 16), Math.floor(3 * dh / 16), Math.floor(3 * dh / 16)] } });
@@ -150,4 +156,4 @@ const MEASURED = [
   orth(null, [256, 256], { count: 16 }), orth(null, [1300, 777]), orth(null, [4096, 4096], { count: 2 }),
 ];
 
-module.exports = { operatorGraph, CASES, MEASURED };
+module.exports = { operatorGraph, CASES, FORMS, MEASURED };
