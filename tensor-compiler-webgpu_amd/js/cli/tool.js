@@ -1308,6 +1308,12 @@ async function main() {
       });
       break;
     }
+    case 'singular-bounds': {
+      // The largest singular value that one step of each set of coefficients can reach from [0, 1] (null: refused).
+      const { singularBound } = require('../src/ir/operators');
+      out = req.sets.map((coefficients) => singularBound({ steps: 1, coefficients })).map((x) => (Number.isFinite(x) ? x : null));
+      break;
+    }
     case 'operator-refusals': {
       const { grad } = require('../src/autodiff');
       const tries = {

@@ -132,9 +132,12 @@ function singularBound(attrs) {
   for (let k = 0; k < attrs.steps; k++) {
     const at = [top];
     const root = (s2) => { if (s2 > 0 && s2 < top * top) at.push(Math.sqrt(s2)); };
-    if (c === 0) { if (b !== 0) root(-a / (3 * b)); } else {
-      const d = 9 * b * b - 20 * a * c;
-      if (d >= 0) { root((-3 * b + Math.sqrt(d)) / (10 * c)); root((-3 * b - Math.sqrt(d)) / (10 * c)); }
+    // The roots of 5c·t² + 3b·t + a in t = s², q the sum of two terms of one sign: a root stays where c is next to 0.
+    const d = 9 * b * b - 20 * a * c;
+    if (d >= 0) {
+      const q = -0.5 * (3 * b + (b < 0 ? -1 : 1) * Math.sqrt(d));
+      root(q / (5 * c));
+      root(a / q);
     }
     top = Math.max(...at.map(p));
     most = Math.max(most, top);

@@ -4,6 +4,7 @@ import re
 import shutil
 import subprocess
 
+import numpy as np
 import pytest
 
 import operator_forms
@@ -34,3 +35,28 @@ def test_every_kernel_writes_its_result_whatever_the_coefficients(tool, tmp_path
         assert re.search(r"global_store|buffer_store", text), name
         if re.search("gram|poly|apply", name):
             assert "v_mfma" in text, name
+
+
+@pytest.mark.parametrize("c", [0, 1e-20, -1e-20, 1e-300, 1e-9])
+def test_how_far_singular_values_grow_does_not_hang_on_a_last_coefficient_near_zero(tool, c):
+    """45·(s - s³) reaches 17.3 between its zeros at 0 and 1: past what the pairs' scales hold."""
+    import tcmi_bridge
+    case = {"name": "grows", "family": "orthogonalize", "x": [96, 100], "options": {"steps": 1, "coefficients": [45, -45, c]}}
+    with pytest.raises(tcmi_bridge.ToolError, match="grow past 16"):
+        tool("operator-graphs", {"cases": [case]})
+    case["options"]["coefficients"] = [40, -40, c]       # 15.4
+    tool("operator-graphs", {"cases": [case]})
+
+
+def test_singular_values_stay_below_what_the_scales_are_made_for(tool):
+    """Against the polynomial's largest value over a grid, of coefficients of all magnitudes and signs."""
+    rng = np.random.default_rng(3)
+    sets = (rng.standard_normal((400, 3)) * 10.0 ** rng.integers(-14, 2, (400, 3))).tolist() + [[3, 0, 0], [0, 1, 0], [0, 0, 1], [0, 0, 0], [1, 0, -1]]
+    bounds = tool("singular-bounds", {"sets": sets})
+    s = np.linspace(0, 1, 4001)
+    for k, (a, b, c) in enumerate(sets):
+        top = max(1, np.abs(s * (a + s * s * (b + s * s * c))).max())
+        if bounds[k] is None:
+            assert top > 16 * (1 - 1e-6), (a, b, c)
+        else:
+            assert top * (1 - 1e-12) <= bounds[k] <= top * (1 + 1e-5), (a, b, c)
