@@ -9,12 +9,14 @@
 // its h counted as 0. With gradients that is three products: the logits are formed once, where
 // a pass over them that keeps only s would form them again for G.
 //
-// All products are of pairs of halves (tcmi_gemm_f16x2.h). h, W and G are split once each, W
-// and h times a power of two from their largest finite magnitude, G times one from the largest
-// |w|; every operand is read from the one layout it is written in.
+// All products are of pairs of halves (tcmi_gemm_f16x2.h), each operand split once, times a power of two that brings
+// its largest finite magnitude below 2^15: h's rows each their own, G's rows each its cotangent's, so that a row's
+// loss and dh hang on nothing that other rows hold; W one for all. dW sums over the rows: it takes a split of h of its own, each
+// row times what G's row lacks of one scale for all, that of the largest |w|·|h|. What a pair loses below 2^-36 is then at most
+// 2^-51 of |h row|·|W| a term of z, of |w|·|W| one of dh and of the largest |w|·|h| one of dW, these magnitudes the largest in each.
 //
-//   maxima   partial maxima of |h|, |W| and |w|
-//   split    h and W as pairs, padded with zeros to whole tiles
+//   maxima   h's row exponents, the least exponent of |w|·|h|, partial maxima of |W|
+//   split    h (for dW again, times w's scale) and W as pairs, padded with zeros to whole tiles
 //   logits   z tile by tile; each wavefront's 64 columns of a row leave (maximum, sum of
 //            exponentials), and z itself where G will be formed
 //   join     a row's pairs joined in order; the losses; (M, 1/s) a row
@@ -48,11 +50,11 @@ __device__ __forceinline__ float exp_full(float x) {
 // The counters at the workspace's start.
 struct LossState {
   uint32_t piece, current;         // the next piece; the one being worked on
-  int h, w, g;                     // exponents of the operands' scales
+  int w, g;                        // exponents of W's scale, and of dW's operands' (the row's of G and of its h together)
 };
 
 // S: the sizes of one launch as constants of its text: N, D, V; NP rows a piece, PIECES of them; DP, VP: d and V padded to
-// whole tiles; BIAS; HBLOCKS, WBLOCKS, GBLOCKS partial maxima of h, W and w; PER groups of four a thread of `split` takes; LKIND, HKIND and
+// whole tiles; BIAS; HBLOCKS, WBLOCKS workgroups of `maxima` over h's rows and W; PER groups of four a thread of `split` takes; LKIND, HKIND and
 // WKIND of tiles for the logits, dh and dW; RB rows a workgroup of `spread`, CT threads across columns there;
 // JOINED: `join` runs; VECD, VECV: d, V multiples of 4; HCHUNKS, HK, WCHUNKS, WK: chunks of K of dh and dW, their slices.
 // WS: byte offsets in the workspace.
@@ -63,6 +65,8 @@ struct Loss {
   __device__ __forceinline__ LossState* state() const { return reinterpret_cast<LossState*>(ws); }
   __device__ __forceinline__ float* at(size_t off) const { return reinterpret_cast<float*>(ws + off); }
   __device__ __forceinline__ Pairs h_pairs() const { return {ws + S::HP, S::DP * 4}; }
+  __device__ __forceinline__ Pairs x_pairs() const { return {ws + S::XP, S::DP * 4}; }       // h for dW
+  __device__ __forceinline__ int* exponents() const { return reinterpret_cast<int*>(ws + S::EXPS); }
   __device__ __forceinline__ Pairs w_pairs() const { return {ws + S::WP, S::VP * 4}; }
   __device__ __forceinline__ Pairs g_pairs() const { return {ws + S::GP, S::VP * 4}; }
   // Whether row r counts, and its target.
@@ -84,21 +88,47 @@ __device__ __forceinline__ float top_of(const f4& v, float top) {
   return fmaxf(fmaxf(fmaxf(finite_abs(v[0]), finite_abs(v[1])), fmaxf(finite_abs(v[2]), finite_abs(v[3]))), top);
 }
 
-template <class S, bool GRAD>
+// That of a row's cotangent.
+__device__ __forceinline__ int weight_scale(float w) { return scale_of(finite_abs(w)); }
+
+constexpr int NO_SCALE = 252;      // at most: two of scale_of's
+
+template <class S, bool DW>
 __device__ __forceinline__ void loss_maxima(const Loss<S>& L, float* scratch, uint32_t block) {
-  float top = 0.f;
   if (block < S::HBLOCKS) {
-    // Rows left out are loaded all the same, so that no load waits for a target.
-    constexpr uint32_t E = S::VECD ? 4 : 1;
-    constexpr size_t n = (size_t)S::N * S::D / E;
+    // A wavefront a row. Rows left out are loaded all the same, so that no load waits for a target.
+    const uint32_t lane = threadIdx.x % 64;
+    int least = NO_SCALE;
+    for (uint32_t r = block * 4 + threadIdx.x / 64; r < S::N; r += S::HBLOCKS * 4) {
+      const float* h = L.h + (size_t)r * S::D;
+      float top = 0.f;
+      if constexpr (S::VECD) {
 #pragma unroll 4
-    for (size_t i = (size_t)block * 256 + threadIdx.x; i < n; i += (size_t)S::HBLOCKS * 256) {
-      float x;
-      if constexpr (S::VECD) x = top_of(reinterpret_cast<const f4*>(L.h)[i], 0.f);
-      else x = finite_abs(L.h[i]);
-      top = fmaxf(top, L.is_class(L.t[i * E / S::D]) ? x : 0.f);
+        for (uint32_t i = lane; i < S::D / 4; i += 64) top = top_of(reinterpret_cast<const f4*>(h)[i], top);
+      } else {
+#pragma unroll 8
+        for (uint32_t i = lane; i < S::D; i += 64) top = fmaxf(top, finite_abs(h[i]));
+      }
+#pragma unroll
+      for (int off = 32; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+      const bool kept = L.kept(r);
+      const int e = scale_of(kept ? top : 0.f);
+      if (lane == 0) L.exponents()[r] = e;
+      if constexpr (DW) {
+        const float w = finite_abs(L.w[r]);
+        if (kept && top > 0.f && w > 0.f) least = min(least, e + weight_scale(w));
+      }
     }
-  } else if (block < S::HBLOCKS + S::WBLOCKS) {
+    if constexpr (DW) {
+      int* const leasts = reinterpret_cast<int*>(scratch);
+      if (lane == 0) leasts[threadIdx.x / 64] = least;
+      __syncthreads();
+      if (threadIdx.x == 0) reinterpret_cast<int*>(L.at(S::MAXIMA))[block] = min(min(leasts[0], leasts[1]), min(leasts[2], leasts[3]));
+    }
+    return;
+  }
+  float top = 0.f;
+  {
     // Four loads in flight a thread.
     constexpr size_t n = (size_t)S::D * S::V, n4 = n / 4, step = (size_t)S::WBLOCKS * 256;
     const size_t i0 = (size_t)(block - S::HBLOCKS) * 256 + threadIdx.x;
@@ -110,9 +140,6 @@ __device__ __forceinline__ void loss_maxima(const Loss<S>& L, float* scratch, ui
     }
     for (; i < n4; i += step) top = top_of(w[i], top);
     if (i0 < n % 4) top = fmaxf(top, finite_abs(L.W[4 * n4 + i0]));
-  } else if constexpr (GRAD) {
-    for (uint32_t r = (block - S::HBLOCKS - S::WBLOCKS) * 256 + threadIdx.x; r < S::N; r += S::GBLOCKS * 256)
-      if (L.kept(r)) top = fmaxf(top, finite_abs(L.w[r]));
   }
   top = block_reduce<true, 256>(top, scratch);
   if (threadIdx.x == 0) L.at(S::MAXIMA)[block] = top;
@@ -140,48 +167,59 @@ __device__ __forceinline__ float top_of_blocks(const float* maxima, uint32_t cou
   return block_reduce<true, 256>(top, scratch);
 }
 
-template <class S, bool GRAD>
+// The least of leasts[0 .. count).
+__device__ __forceinline__ int least_of_blocks(const int* leasts, uint32_t count, int* scratch) {
+  int least = NO_SCALE;
+  for (uint32_t i = threadIdx.x; i < count; i += 256) least = min(least, leasts[i]);
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) least = min(least, __shfl_xor(least, off, 64));
+  if (threadIdx.x % 64 == 0) scratch[threadIdx.x / 64] = least;
+  __syncthreads();
+  return min(min(scratch[0], scratch[1]), min(scratch[2], scratch[3]));
+}
+__device__ __forceinline__ f4 scaled(f4 v, int by) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = ldexpf(v[e], by);
+  return v;
+}
+
+template <class S, bool DW>
 __device__ __forceinline__ void loss_split(const Loss<S>& L, float* scratch, uint32_t block) {
   constexpr size_t HG = (size_t)S::NP * S::PIECES * S::DP / 4, WG = (size_t)S::DP * S::VP / 4;
   constexpr uint32_t HB = (HG + 256 * S::PER - 1) / (256 * S::PER);
-  const bool of_w = block >= HB;
   const float* maxima = L.at(S::MAXIMA);
-  const int s = scale_of(of_w ? top_of_blocks(maxima + S::HBLOCKS, S::WBLOCKS, scratch) : top_of_blocks(maxima, S::HBLOCKS, scratch));
-  if constexpr (GRAD) {
-    if (block == 0) {
-      const int g = scale_of(top_of_blocks(maxima + S::HBLOCKS + S::WBLOCKS, S::GBLOCKS, scratch));
-      if (threadIdx.x == 0) L.state()->g = g;
-    }
-  }
-  if (threadIdx.x == 0) {
-    LossState* st = L.state();
-    if (block == 0) {
-      st->piece = 0u;
-      st->h = s;
-    }
-    if (block == HB) st->w = s;
-  }
-  const Pairs p = of_w ? L.w_pairs() : L.h_pairs();
-  for (uint32_t u = 0; u < S::PER; ++u) {
-    const size_t i = ((size_t)(of_w ? block - HB : block) * S::PER + u) * 256 + threadIdx.x;
-    f4 v;
-    size_t row;
-    uint32_t col;
-    if (of_w) {
+  LossState* st = L.state();
+  if (block >= HB) {
+    const int s = scale_of(top_of_blocks(maxima + S::HBLOCKS, S::WBLOCKS, scratch));
+    if (block == HB && threadIdx.x == 0) st->w = s;
+    for (uint32_t u = 0; u < S::PER; ++u) {
+      const size_t i = ((size_t)(block - HB) * S::PER + u) * 256 + threadIdx.x;
       if (i >= WG) return;
-      row = i / (S::VP / 4);
-      col = i % (S::VP / 4) * 4;
-      v = four<S::VECV>(L.W, row, S::D, col, S::V);
-    } else {
-      if (i >= HG) return;
-      row = i / (S::DP / 4);
-      col = i % (S::DP / 4) * 4;
-      v = f4{0.f, 0.f, 0.f, 0.f};
-      if (L.kept(row)) v = four<S::VECD>(L.h, row, S::N, col, S::D);
+      const size_t row = i / (S::VP / 4);
+      const uint32_t col = i % (S::VP / 4) * 4;
+      put_pairs(L.w_pairs(), row, col, scaled(four<S::VECV>(L.W, row, S::D, col, S::V), s));
     }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = ldexpf(v[e], s);
-    put_pairs(p, row, col, v);
+    return;
+  }
+  const int least = DW ? least_of_blocks(reinterpret_cast<const int*>(maxima), S::HBLOCKS, reinterpret_cast<int*>(scratch)) : 0;
+  if (block == 0 && threadIdx.x == 0) {
+    st->piece = 0u;
+    st->g = least;
+  }
+  for (uint32_t u = 0; u < S::PER; ++u) {
+    const size_t i = ((size_t)block * S::PER + u) * 256 + threadIdx.x;
+    if (i >= HG) return;
+    const size_t row = i / (S::DP / 4);
+    const uint32_t col = i % (S::DP / 4) * 4;
+    f4 v = {0.f, 0.f, 0.f, 0.f};
+    const bool kept = L.kept(row);
+    if (kept) v = four<S::VECD>(L.h, row, S::N, col, S::D);
+    put_pairs(L.h_pairs(), row, col, scaled(v, kept ? L.exponents()[row] : 0));
+    if constexpr (DW) {
+      // A row of weight 0 (whose G is 0) has none of the least exponents.
+      const float w = kept ? finite_abs(L.w[row]) : 0.f;
+      put_pairs(L.x_pairs(), row, col, w > 0.f ? scaled(v, least - weight_scale(w)) : f4{0.f, 0.f, 0.f, 0.f});
+    }
   }
 }
 
@@ -197,14 +235,16 @@ __device__ __forceinline__ void loss_logits(const Loss<S>& L, char* lds, uint32_
   a.at += (size_t)piece * S::NP * a.ld;
   typename P::Sums acc;
   P::template sum<true, false>(a, L.w_pairs(), tile, 0, (S::D + 31) / 32, lds, acc);
-  const int back = -(st->h + st->w);
+  const int back_w = -st->w;
   const uint32_t col0 = P::col(tile), row0 = P::row(tile);
   float m[P::TI];
+  int back[P::TI];             // exponents of a row's sums
   uint32_t ahead[P::TI];       // the columns from col0 on to a row's target, where that is a class
 #pragma unroll
   for (int i = 0; i < P::TI; ++i) {
     const uint32_t r = piece * S::NP + row0 + i * 16;
     const float target = r < S::N ? L.t[r] : -1.f;
+    back[i] = r < S::N ? back_w - L.exponents()[r] : 0;
     ahead[i] = L.is_class(target) ? static_cast<uint32_t>(target) - col0 : ~0u;
     m[i] = -TCMI_INF;
   }
@@ -217,7 +257,7 @@ __device__ __forceinline__ void loss_logits(const Loss<S>& L, char* lds, uint32_
       f4& z = acc[i][j];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        z[e] = ldexpf(z[e], back) + b[e];
+        z[e] = ldexpf(z[e], back[i]) + b[e];
         if (S::V != S::VP && col + e >= S::V) z[e] = -TCMI_INF;
         m[i] = fmaxf(m[i], z[e]);
       }
@@ -286,16 +326,17 @@ __device__ __forceinline__ void loss_join(const Loss<S>& L, float* out, float2* 
 }
 
 // RB rows of 8·CT columns of G: 256 / CT threads a column group, each its own rows in turn. rows: of LDS, and 512 more for
-// the sums. out: the losses, where this kernel joins the statistics (not JOINED).
+// the sums, and RB / 4 for the rows' scales back. out: the losses, where this kernel joins the statistics (not JOINED).
 template <class S, bool PAIRS, bool SUMS, bool LOSS>
 __device__ __forceinline__ void loss_spread(const Loss<S>& L, float* out, f4* rows, uint32_t bx, uint32_t by) {
   const LossState* st = L.state();
   const uint32_t piece = st->current;
-  const int sg = st->g;
   const uint32_t row0 = by * S::RB;
+  float* const unscale = reinterpret_cast<float*>(rows + S::RB + 512);
   if (threadIdx.x < S::RB) {
     const uint32_t row = row0 + threadIdx.x, r = piece * S::NP + row;
-    f4 c = {0.f, 0.f, 0.f, -1.f};       // M, w/s and w in G's scale, the target (-1: the row is left out)
+    f4 c = {0.f, 0.f, 0.f, -1.f};       // M, w/s and w in the row's scale, the target (-1: the row is left out)
+    float one = 1.f;
     const bool kept = L.kept(r);
     if (kept) {
       float2 x;
@@ -314,12 +355,15 @@ __device__ __forceinline__ void loss_spread(const Loss<S>& L, float* out, f4* ro
           if (bx == 0) out[r] = (sum.m - L.at(S::PICKED)[row]) + op_log(sum.s);
         }
       }
-      const float w = ldexpf(L.w[r], sg);
+      const int scale = weight_scale(L.w[r]);
+      const float w = ldexpf(L.w[r], scale);
+      one = ldexpf(1.f, -scale);
       c = f4{x.x, w * x.y, w, L.t[r]};
     } else if constexpr (LOSS && !S::JOINED) {
       if (bx == 0 && r < S::N) out[r] = 0.f;
     }
     rows[threadIdx.x] = c;
+    if constexpr (SUMS) unscale[threadIdx.x] = one;
   }
   __syncthreads();
   constexpr uint32_t RG = 256 / S::CT;
@@ -347,8 +391,8 @@ __device__ __forceinline__ void loss_spread(const Loss<S>& L, float* out, f4* ro
         }
       }
       if constexpr (SUMS) {
-        sum[0] += g[0];
-        sum[1] += g[1];
+        sum[0] += g[0] * unscale[k];
+        sum[1] += g[1] * unscale[k];
       }
       if constexpr (PAIRS) {
         h8 hi, lo;
@@ -402,11 +446,6 @@ __device__ __forceinline__ void put_four(float* out, size_t row, uint32_t rows, 
       if (col + e < cols) p[e] = add ? p[e] + v[e] : v[e];
   }
 }
-__device__ __forceinline__ f4 scaled(f4 v, int by) {
-#pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] = ldexpf(v[e], by);
-  return v;
-}
 // Workgroups of `grads`: dh's tiles by chunks of K, dW's, then dbias.
 template <class S>
 struct GradTiles {
@@ -416,6 +455,12 @@ struct GradTiles {
   static constexpr uint32_t HR = S::NP / H::ROWS, HC = S::DP / H::COLS, WR = S::DP / W::ROWS, WC = S::VP / W::COLS;
   static constexpr int LDS = H::LDS > W::LDS ? H::LDS : W::LDS;
 };
+
+// The exponent that row r's sums of dh lack.
+template <class S>
+__device__ __forceinline__ int dh_back(const Loss<S>& L, uint32_t r) {
+  return r < S::N ? -(weight_scale(L.w[r]) + L.state()->w) : 0;
+}
 
 template <class S, bool DH, bool DW, bool DB>
 __device__ __forceinline__ void loss_grads(const Loss<S>& L, float* dh, float* dw, float* db, char* lds, uint32_t block) {
@@ -431,20 +476,25 @@ __device__ __forceinline__ void loss_grads(const Loss<S>& L, float* dh, float* d
     const TileAt tile = {in % G::HR, in / G::HR};
     typename P::Sums acc;
     P::template sum<true, true>(L.g_pairs(), L.w_pairs(), tile, first * 32, left < S::HK ? left : S::HK, lds, acc);
-    const int back = -(st->g + st->w);
+    const uint32_t row0 = P::row(tile);
+    int back[P::TI];
+    if constexpr (S::HCHUNKS == 1) {
+#pragma unroll
+      for (int i = 0; i < P::TI; ++i) back[i] = dh_back(L, piece * S::NP + row0 + i * 16);
+    }
     P::each(tile, acc, [&](uint32_t row, uint32_t col, const f4& v) {
       if constexpr (S::HCHUNKS > 1) *reinterpret_cast<f4*>(L.at(S::HPART) + ((size_t)chunk * S::NP + row) * S::DP + col) = v;
-      else put_four<S::VECD>(dh, (size_t)piece * S::NP + row, S::N, col, S::D, scaled(v, back), false);
+      else put_four<S::VECD>(dh, (size_t)piece * S::NP + row, S::N, col, S::D, scaled(v, back[(row - row0) / 16]), false);
     });
   } else if (DW && block - HB < WB) {
     using P = typename G::W;
     const uint32_t id = block - HB, chunk = id / (G::WR * G::WC), first = chunk * S::WK, left = S::NP / 32 - first;
     const TileAt tile = tile_at<P::GROUP>(id % (G::WR * G::WC), G::WR, G::WC);
-    Pairs a = L.h_pairs();
+    Pairs a = L.x_pairs();
     a.at += (size_t)piece * S::NP * a.ld;
     typename P::Sums acc;
     P::template sum<false, false>(a, L.g_pairs(), tile, first * 32, left < S::WK ? left : S::WK, lds, acc);
-    const int back = -(st->g + st->h);
+    const int back = -st->g;
     P::each(tile, acc, [&](uint32_t row, uint32_t col, const f4& v) {
       if constexpr (S::WCHUNKS > 1) *reinterpret_cast<f4*>(L.at(S::WPART) + ((size_t)chunk * S::DP + row) * S::VP + col) = v;
       else put_four<S::VECV>(dw, row, S::D, col, S::V, scaled(v, back), piece > 0);
@@ -460,8 +510,7 @@ __device__ __forceinline__ void loss_grads(const Loss<S>& L, float* dh, float* d
     __syncthreads();
     if (k0 == 0 && col < S::V) {
       for (uint32_t k = 1; k < PER; ++k) sum += scratch[k * 16 + threadIdx.x];
-      const float v = ldexpf(sum, -st->g);
-      db[col] = piece > 0 ? db[col] + v : v;
+      db[col] = piece > 0 ? db[col] + sum : sum;
     }
   }
 }
@@ -476,14 +525,14 @@ __device__ __forceinline__ void loss_sums(const Loss<S>& L, float* dh, float* dw
     if (row >= S::NP) return;
     f4 v = {0.f, 0.f, 0.f, 0.f};
     for (uint32_t c = 0; c < S::HCHUNKS; ++c) v += *reinterpret_cast<const f4*>(L.at(S::HPART) + ((size_t)c * S::NP + row) * S::DP + col);
-    put_four<S::VECD>(dh, (size_t)st->current * S::NP + row, S::N, col, S::D, scaled(v, -(st->g + st->w)), false);
+    put_four<S::VECD>(dh, (size_t)st->current * S::NP + row, S::N, col, S::D, scaled(v, dh_back(L, st->current * S::NP + row)), false);
   } else if constexpr (DW) {
     const size_t i = (size_t)(block - HB) * 256 + threadIdx.x, row = i / (S::VP / 4);
     const uint32_t col = i % (S::VP / 4) * 4;
     if (row >= S::D) return;
     f4 v = {0.f, 0.f, 0.f, 0.f};
     for (uint32_t c = 0; c < S::WCHUNKS; ++c) v += *reinterpret_cast<const f4*>(L.at(S::WPART) + ((size_t)c * S::DP + row) * S::VP + col);
-    put_four<S::VECV>(dw, row, S::D, col, S::V, scaled(v, -(st->g + st->h)), st->current > 0);
+    put_four<S::VECV>(dw, row, S::D, col, S::V, scaled(v, -st->g), st->current > 0);
   }
 }
 

@@ -196,14 +196,16 @@ function lossSizes(N, D, V, bias, parts, piece) {
   const g = gradTiles(NP, D, VP), DP = grad ? g.DP : align(D, 64);
   // Threads across columns: fewer, and rows side by side, where workgroups would be fewer than two a CU.
   const CT = (() => { let t = 16; while (2 * t <= Math.min(256, VP / 8) && ceil(VP, 16 * t) * NP / RB >= 2 * CUS) t *= 2; return t; })();
-  const z = { N, D, V, DP, VP, NP, PIECES, RB, CT, BIAS: bias, HBLOCKS: clamp(N * D / 4096, 256), WBLOCKS: clamp(D * V / 16384, 1024), GBLOCKS: clamp(N / 1024, 64),
+  const z = { N, D, V, DP, VP, NP, PIECES, RB, CT, BIAS: bias, HBLOCKS: clamp(N / 4, 1024), WBLOCKS: clamp(D * V / 16384, 1024),
     PER: clamp((NP * PIECES * DP + DP * VP) / 4 / 256 / 1024, 16), LKIND: large ? TALL : SMALL, HKIND: g.large ? TALL : SMALL, WKIND: g.large ? WIDE : SMALL, JOINED: !grad || VP / (16 * LT) > 32, VECD: D % 4 === 0, VECV: V % 4 === 0,
     HCHUNKS: g.h.chunks, HK: g.h.each, WCHUNKS: g.w.chunks, WK: g.w.each };
   let at = 0;
   const place = (name, bytes) => { z[name] = at; at = align(at + bytes, 256); };
   place('STATE', 256);
-  place('MAXIMA', (z.HBLOCKS + z.WBLOCKS + z.GBLOCKS) * 4);
+  place('MAXIMA', (z.HBLOCKS + z.WBLOCKS) * 4);
+  place('EXPS', 4 * N);
   place('HP', 4 * NP * PIECES * DP);
+  if (parts.includes('dW')) place('XP', 4 * NP * PIECES * DP); else z.XP = 0;
   place('WP', 4 * DP * VP);
   place('STATS', 8 * NP * (VP / (16 * LT)));
   place('PICKED', 4 * NP);
@@ -252,7 +254,7 @@ function fewSizes(N, D, V, bias, parts) {
 }
 
 function lossMaker(z, e, bias, grad) {
-  const counts = /^([NDV]P?|NP|RT|PIECES|RB|CT|[HWG]BLOCKS|PER|[HW]CHUNKS|[HW]K|WAVES|COLS|CHUNKS|DTILES|CG|RC|DG)$/;
+  const counts = /^([NDV]P?|NP|RT|PIECES|RB|CT|[HW]BLOCKS|PER|[HW]CHUNKS|[HW]K|WAVES|COLS|CHUNKS|DTILES|CG|RC|DG)$/;
   const sizes = Object.keys(z).map((k) => (typeof z[k] === 'boolean' ? `  static constexpr bool ${k} = ${z[k]};`
     : k.endsWith('KIND') ? `  static constexpr int ${k} = ${z[k]};`
       : `  static constexpr ${counts.test(k) ? 'uint32_t' : 'size_t'} ${k} = ${z[k]}u;`)).join('\n');
@@ -335,8 +337,8 @@ function lossKernels(N, D, V, bias, parts, joined, bytes) {
   const [lr, lc, lt] = TILES[z.LKIND], [hr, hc, gt] = TILES[z.HKIND], [wr, wc] = TILES[z.WKIND];
   const outs = (...names) => names.map((p) => (has(p) ? e.out(p) : 'nullptr')).join(', ');
   const HG = z.NP * z.PIECES * z.DP / 4, WG = z.DP * z.VP / 4;
-  const once = [make('lossmax', [z.HBLOCKS + z.WBLOCKS + (grad ? z.GBLOCKS : 0), 1, 1], 256, 'float scratch[4]', `loss_maxima<${S}, ${grad}>(L, scratch, blockIdx.x)`),
-    make('losssplit', [ceil(HG, 256 * z.PER) + ceil(WG, 256 * z.PER), 1, 1], 256, 'float scratch[4]', `loss_split<${S}, ${grad}>(L, scratch, blockIdx.x)`)];
+  const once = [make('lossmax', [z.HBLOCKS + z.WBLOCKS, 1, 1], 256, 'float scratch[4]', `loss_maxima<${S}, ${has('dW')}>(L, scratch, blockIdx.x)`),
+    make('losssplit', [ceil(HG, 256 * z.PER) + ceil(WG, 256 * z.PER), 1, 1], 256, 'float scratch[4]', `loss_split<${S}, ${has('dW')}>(L, scratch, blockIdx.x)`)];
   const piece = [make('losslogits', [z.NP / lr * (z.VP / lc), 1, 1], lt, `char lds[tcmi::Tile<${z.LKIND}>::LDS]`, `loss_logits<${S}, ${grad}>(L, lds, blockIdx.x)`)];
   if (z.JOINED) {
     piece.push(make('lossjoin', [z.NP / 16, 1, 1], 1024, 'float2 scratch[1024]',
@@ -344,7 +346,7 @@ function lossKernels(N, D, V, bias, parts, joined, bytes) {
   }
   if (grad) {
     const [dh, dW, db] = ['dh', 'dW', 'dbias'].map(has);
-    piece.push(make('lossspread', [ceil(z.VP, 8 * z.CT), z.NP / z.RB, 1], 256, `tcmi::f4 rows[${z.RB + 512}]`,
+    piece.push(make('lossspread', [ceil(z.VP, 8 * z.CT), z.NP / z.RB, 1], 256, `tcmi::f4 rows[${z.RB + 512 + z.RB / 4}]`,
       `loss_spread<${S}, ${dh || dW}, ${db}, ${has('loss')}>(L, ${outs('loss')}, rows, blockIdx.x, blockIdx.y)`));
     const blocks = (dh ? z.NP / hr * (z.DP / hc) * z.HCHUNKS : 0) + (dW ? z.DP / wr * (z.VP / wc) * z.WCHUNKS : 0) + (db ? z.VP / 16 : 0);
     piece.push(make('lossgrads', [blocks, 1, 1], gt, `char lds[tcmi::GradTiles<${S}>::LDS]`, `loss_grads<${S}, ${dh}, ${dW}, ${db}>(L, ${outs('dh', 'dW', 'dbias')}, lds, blockIdx.x)`));

@@ -144,6 +144,9 @@ const FORMS = [
   // Coefficients near 0 and at it, of a matrix that the products of pairs take: their scales' exponents are the largest.
   orth('linear', [96, 100], { options: { steps: 1, coefficients: [1, 0, 0] } }),
   orth('nearly-linear', [100, 70], { options: { steps: 2, coefficients: [0.5, -1e-12, 0] } }),
+  // Losses by products of pairs whose rows' magnitudes are far apart: whole, and in pieces with K split.
+  loss('far-rows', 128, 64, 512, { bias: true, gradient: true }),
+  loss('far-rows-pieces', 330, 40, 700, { bias: true, gradient: true, tuning: { loss: { piece: 1 } } }),
 ];
 
 const r = (B, T, H, dh, axes, gradient, twin) => rotary(null, [B, T, H, dh], axes === 1 ? [B, T] : [B, T, axes],
