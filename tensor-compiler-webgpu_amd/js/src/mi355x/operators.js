@@ -439,6 +439,16 @@ ${lds ? `  __shared__ __attribute__((aligned(1024))) double lds[${lds}];\n` : ''
   return { kind: 'orthogonalize', kernels, workspace: count * z.PER, flops: count * steps * (3 * s * s * l + s ** 3) };
 }
 
+/** How many other nodes are equal to `node` (op, shape, attributes) and neither depend on it nor it on them. */
+function equalBeside(graph, node) {
+  const same = (n) => n !== node && n.op === node.op && n.shape.join() === node.shape.join() && JSON.stringify(n.attrs) === JSON.stringify(node.attrs);
+  if (!graph.nodes.some(same)) return 0;
+  const before = new Set([node.id]), after = new Set([node.id]);
+  for (let id = node.id; id >= 0; id--) if (before.has(id)) for (const i of graph.nodes[id].inputs) before.add(i);
+  for (const n of graph.nodes) if (n.inputs.some((i) => after.has(i))) after.add(n.id);
+  return graph.nodes.filter((n) => same(n) && !before.has(n.id) && !after.has(n.id)).length;
+}
+
 function lowerOrthogonalize(graph, node) {
   const x = node.shape, M = x[x.length - 2], N = x[x.length - 1], count = size(x.slice(0, -2));
   const { steps, eps, coefficients: [a, b, c] } = node.attrs;
@@ -446,9 +456,8 @@ function lowerOrthogonalize(graph, node) {
   if (Math.max(M, N) > PAIR_COLS) throw new Error(`orthogonalize: a matrix of ${M} x ${N} (at most ${PAIR_COLS} on a side)`);
   const tall = M > N, s = Math.min(M, N), l = Math.max(M, N);
   if (s <= THIN_SIDE && steps > 0) return thinKernels(node, M, N, count);
-  // Tiles of 128, or of 64 where those leave much of the chip idle, counting the graph's equal nodes: they run side by side.
-  const equal = graph.nodes.filter((n) => n.op === 'orthogonalize' && n.shape.join() === x.join() && JSON.stringify(n.attrs) === JSON.stringify(node.attrs)).length;
-  const alike = count * Math.min(equal, MAX_BATCH);
+  // Tiles of 128, or of 64 where those leave much of the chip idle, counting the equal nodes that run side by side with it.
+  const alike = count * Math.min(1 + equalBeside(graph, node), MAX_BATCH);
   const square = ceil(s, 128) * ceil(l, 128) * alike >= 2 * CUS;
   const pad = square ? 128 : 64, MP = align(M, pad), NP = align(N, pad), SP = Math.min(MP, NP);
   const n = SP / pad, kind = square ? SQUARE : SMALL, upper = n * (n + 1) / 2;

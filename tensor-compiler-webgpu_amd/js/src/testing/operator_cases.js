@@ -5,7 +5,7 @@
 //       gives its shape; `twice`: rotated, and the result again
 //   { family: 'loss', N, d, V, bias?, gradient?, wrt?, after? }     wrt: 'h', 'W', 'b' (default all); `after`: the
 //       losses' cotangent depends on the losses, so their gradients cannot run beside them
-//   { family: 'orthogonalize', x, count, options }
+//   { family: 'orthogonalize', x, count, options, twice }
 
 const { Graph } = require('../ir/graph');
 const { grad } = require('../autodiff');
@@ -35,7 +35,8 @@ function operatorGraph(c) {
     for (const k of c.wrt || (c.bias ? ['h', 'W', 'b'] : ['h', 'W'])) { wrt.push(all[k]); grads.push(`d${k}`); }
   } else if (c.family === 'orthogonalize') {
     for (let k = 0; k < (c.count || 1); k++) {
-      outs.push(g.orthogonalize(g.input(`x${k}`, c.x), c.options));
+      const y = g.orthogonalize(g.input(`x${k}`, c.x), c.options);
+      outs.push(c.twice ? g.orthogonalize(y, c.options) : y);
       names.push(`y${k}`);
     }
   } else throw new Error(`no operator '${c.family}'`);

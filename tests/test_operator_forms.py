@@ -60,3 +60,13 @@ def test_singular_values_stay_below_what_the_scales_are_made_for(tool):
             assert top > 16 * (1 - 1e-6), (a, b, c)
         else:
             assert top * (1 - 1e-12) <= bounds[k] <= top * (1 + 1e-5), (a, b, c)
+
+
+@pytest.mark.parametrize("x", [[320, 3632], [1300, 777]])
+def test_matrices_that_depend_on_each_other_take_the_tiles_of_one(tool, x):
+    """Equal matrices side by side fill the chip together, and take other tiles; one of the other's result cannot."""
+    def kernels(**more):
+        return set(tool("kernel-unit", {"operators": [dict({"family": "orthogonalize", "x": x}, **more)]}, timeout=120)["kernels"])
+    one = kernels()
+    assert kernels(twice=True) == one
+    assert not kernels(count=2) & one
