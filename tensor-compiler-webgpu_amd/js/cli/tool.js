@@ -387,6 +387,13 @@ async function gpuDirect(dir, req) {
   bundle.close({ device: runner.info(), sabotage: sabotage || null });
 }
 
+/** A request's float32 values: an array, or the base64 text of their bytes. */
+function floatsOf(v) {
+  if (typeof v !== 'string') return Float32Array.from(v);
+  const b = Buffer.from(v, 'base64');
+  return new Float32Array(b.buffer.slice(b.byteOffset, b.byteOffset + b.length));
+}
+
 async function gpuGraphs(req, dir) {
   const { HipRunner } = require('../src/mi355x/runner');
   const runner = HipRunner.create();
@@ -395,7 +402,7 @@ async function gpuGraphs(req, dir) {
     process.stderr.write(`gpu-graphs: ${c.name}\n`);
     const g = Graph.fromJSON(c.graph);
     const inputs = {};
-    for (const n of g.inputs()) inputs[n.attrs.name] = Float32Array.from(c.inputs[n.attrs.name]);
+    for (const n of g.inputs()) inputs[n.attrs.name] = floatsOf(c.inputs[n.attrs.name]);
     const f = fuse(g, { keep: c.keep || [], attention: !!c.attention });
     const lf = lowerMI355X(f.graph, { tuning: c.tuning });
     const rf = await runner.run(f.graph, lf, inputs, { canary: true });
@@ -1346,14 +1353,14 @@ async function main() {
       const cfg = require('../src/builders/configs');
       const m = new Map();
       const add = (lw) => { for (const [name, src] of kernelSources(lw)) m.set(name, src); };
-      const perf = (v, fuseOpts) => {
+      const perf = (v, fuseOpts, tuning) => {
         const f = fuse(v.graph, Object.assign({ keep: v.keep }, fuseOpts || {}));
-        add(lowerMI355X(f.graph, { perf: true, keep: v.keep.map((id) => f.index.get(id)) }));
+        add(lowerMI355X(f.graph, { perf: true, keep: v.keep.map((id) => f.index.get(id)), tuning }));
       };
       if (req.operators) {
         // Those of the operators' graphs instead (testing/operator_cases.js), from descriptions.
         const { operatorGraph } = require('../src/testing/operator_cases');
-        for (const c of req.operators) perf(operatorGraph(c));
+        for (const c of req.operators) perf(operatorGraph(c), null, c.tuning);
         out = { kernels: Array.from(m.keys()), unit: translationUnit(m) };
         break;
       }

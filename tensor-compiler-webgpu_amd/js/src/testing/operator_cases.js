@@ -148,6 +148,30 @@ const FORMS = [
   // Losses by products of pairs whose rows' magnitudes are far apart: whole, and in pieces with K split.
   loss('far-rows', 128, 64, 512, { bias: true, gradient: true }),
   loss('far-rows-pieces', 330, 40, 700, { bias: true, gradient: true, tuning: { loss: { piece: 1 } } }),
+  // The loss by large tiles: of the logits alone, of the gradients with K split and whole, in pieces.
+  loss('tall-logits', 517, 131, 9001, { bias: true, gradient: true }),
+  loss('tall-logits-pieces', 517, 131, 9001, { bias: true, gradient: true, tuning: { loss: { piece: 2 ** 24 } } }),
+  loss('tall-values', 517, 131, 9001, { bias: true }),
+  loss('large-split', 1301, 201, 16001, { bias: true, gradient: true }),
+  loss('large-whole', 2499, 1999, 2401, { bias: true, gradient: true }),
+  loss('large-pieces', 513, 1001, 7001, { gradient: true, tuning: { loss: { piece: 2 ** 24 } } }),
+  loss('tall-after', 517, 131, 9001, { bias: true, gradient: true, after: true }),
+  // Matrices by 64 x 64 tiles whose upper half is computed, split along K, wide and tall.
+  orth('half', [771, 1301]),
+  orth('half-tall', [1301, 771]),
+  // By 128 x 128 tiles, X by each of the larger: stacks wide and tall, and one whose leftover tiles are split.
+  orth('square-tall-tiles', [128, 200, 250]),
+  orth('square-tall-tiles-tall', [128, 250, 200]),
+  orth('square-wide-tiles', [256, 100, 250]),
+  orth('square-wide-tiles-tall', [128, 300, 250]),
+  orth('square-tiles', [171, 100, 300]),
+  orth('square-tiles-tall', [171, 300, 100]),
+  orth('square-split', [60, 500, 520], { options: { steps: 2 } }),
+  // Equal stacks side by side, and matrices whose workgroups are dealt to the XCDs (eight of them, or a multiple).
+  orth('stack-twins', [8, 100, 90], { count: 3 }),
+  orth('stack-twins-odd', [3, 90, 100], { count: 2 }),
+  orth('eight', [90, 101], { count: 8 }),
+  orth('twice', [96, 100], { twice: true, count: 2, options: { steps: 2 } }),
 ];
 
 const r = (B, T, H, dh, axes, gradient, twin) => rotary(null, [B, T, H, dh], axes === 1 ? [B, T] : [B, T, axes],

@@ -70,3 +70,42 @@ def test_matrices_that_depend_on_each_other_take_the_tiles_of_one(tool, x):
     one = kernels()
     assert kernels(twice=True) == one
     assert not kernels(count=2) & one
+
+
+# What the named graphs run, that no graph of test_gpu_operators.py does.
+TAKEN = {
+    "far-rows": {"LKIND": 0, "HKIND": 0, "WKIND": 0, "JOINED": "false"},
+    "far-rows-pieces": {"LKIND": 0, "PIECES": 3, "HCHUNKS": None},
+    "tall-logits": {"LKIND": 3, "HKIND": 0, "WKIND": 0, "CT": 32, "JOINED": "true", "PIECES": 1, "HCHUNKS": None},
+    "tall-logits-pieces": {"LKIND": 3, "PIECES": 3, "HCHUNKS": None},
+    "tall-values": {"LKIND": 3, "PIECES": 1},
+    "tall-after": {"LKIND": 3},
+    "large-split": {"LKIND": 3, "HKIND": 3, "WKIND": 2, "HCHUNKS": None, "WCHUNKS": None, "CT": 128},
+    "large-whole": {"LKIND": 3, "HKIND": 3, "WKIND": 2, "HCHUNKS": 1, "WCHUNKS": 1},
+    "large-pieces": {"LKIND": 3, "HKIND": 3, "WKIND": 2, "PIECES": 2, "HCHUNKS": None},
+    "half": {"KIND": 0, "HALF": "true", "TALL": "false", "GSPLIT": None, "BSPLIT": None},
+    "half-tall": {"KIND": 0, "HALF": "true", "TALL": "true", "GSPLIT": None, "BSPLIT": None},
+    "square-tall-tiles": {"KIND": 1, "AKIND": 3, "HALF": "true", "TALL": "false"},
+    "square-tall-tiles-tall": {"KIND": 1, "AKIND": 3, "HALF": "true", "TALL": "true"},
+    "square-wide-tiles": {"KIND": 1, "AKIND": 2, "TALL": "false"},
+    "square-wide-tiles-tall": {"KIND": 1, "AKIND": 2, "TALL": "true"},
+    "square-tiles": {"KIND": 1, "AKIND": 1, "TALL": "false"},
+    "square-tiles-tall": {"KIND": 1, "AKIND": 1, "TALL": "true"},
+    "square-split": {"KIND": 1, "GSPLIT": 1, "GCHUNKS": 2, "BSPLIT": 1, "BCHUNKS": 2, "SP": 512},
+    "stack-twins": {"KIND": 0, "batch": 3},
+    "stack-twins-odd": {"KIND": 0, "batch": 2},
+    "eight": {"KIND": 0, "batch": 8},
+}
+
+
+def test_the_named_graphs_take_the_forms_that_they_are_named_for(tool):
+    """So that another choice of tiles does not leave a form untested (None: more than 1)."""
+    for g in operator_forms.forms(tool, list(TAKEN)):
+        sizes = operator_forms.constants(tool, g["case"])
+        for k, want in TAKEN[g["name"]].items():
+            if k == "batch":
+                assert [b["count"] for b in g["batches"]] == [want], g["name"]
+            elif want is None:
+                assert int(min(sizes[k])) > 1, (g["name"], k, sizes[k])
+            else:
+                assert sizes[k] == {str(want)}, (g["name"], k, sizes[k])
