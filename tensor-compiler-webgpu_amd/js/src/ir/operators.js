@@ -59,6 +59,7 @@ function operatorRules(ShapeError, fmt) {
     need(x.length >= 2, `${op} of ${fmt(x)}: tokens and a head take two axes or more`);
     const r = x.length, dh = x[r - 1], a = attrs.axis;
     need(Number.isInteger(a) && a >= 0 && a < r - 1, `${op} of ${fmt(x)}: no token axis ${a}`);
+    need(Number.isInteger(attrs.positionAxes) && attrs.positionAxes >= 1 && attrs.positionAxes <= 256, `${op}: ${attrs.positionAxes} position axes (1 to 256)`);
     const { frequencies: f, axes } = attrs;
     need(Array.isArray(f) && f.every(isNumber) && 2 * f.length <= dh, `${op}: at most ${Math.floor(dh / 2)} finite frequencies for heads of ${dh}`);
     need(Array.isArray(axes) && axes.length === f.length && axes.every((i) => Number.isInteger(i) && i >= 0 && i < attrs.positionAxes),

@@ -109,3 +109,21 @@ def test_the_named_graphs_take_the_forms_that_they_are_named_for(tool):
                 assert int(min(sizes[k])) > 1, (g["name"], k, sizes[k])
             else:
                 assert sizes[k] == {str(want)}, (g["name"], k, sizes[k])
+
+
+def refused(tool, case):
+    import tcmi_bridge
+    with pytest.raises(tcmi_bridge.ToolError) as e:
+        tool("operator-graphs", {"cases": [dict(case, name="refused")]})
+    return str(e.value)
+
+
+@pytest.mark.parametrize("count", [257, 0, -1])
+def test_position_axes_that_no_kernel_counts_are_refused(tool, count):
+    """A kernel's table names its pairs' axes in bytes."""
+    case = {"family": "rotary", "x": [4, 1, 600], "positions": [4] + [count] * (count > 1), "options": {"axis": 0, "frequencies": [], "positionAxes": count}}
+    if count == 0:
+        case["options"].update(frequencies=[1.0], axes=[-1])
+    assert "position axes" in refused(tool, case)
+    tool("operator-graphs", {"cases": [{"name": "most", "family": "rotary", "x": [4, 1, 600], "positions": [4, 256],
+                                        "options": {"axis": 0, "frequencies": [1.0], "axes": [255], "positionAxes": 256}}]})
