@@ -127,6 +127,8 @@ function lowerRotary(graph, node) {
 // Bytes of a piece's logits at most (a piece is 128 rows or more): each piece reads W and adds to dW. 8192 rows of d 1024 against 65 536 classes
 // 10.08 ms by 2^28, 9.53 by 2^29, 9.52 by 2^30.
 const LOSS_PIECE = 2 ** 29;
+// Rows at most: they are counted in 32 bits, and 16 of them take 256 threads of a grid of 2^32 at most.
+const LOSS_ROWS = 2 ** 28;
 const LOSS_PARTS = ['dh', 'dW', 'dbias', 'loss'];
 const CUS = 256;
 /**
@@ -365,6 +367,7 @@ function lowerLoss(graph, node, tuning) {
   const { piece } = (tuning || {}).loss || {};
   const grad = node.op === 'linearCrossEntropyGrad';
   const [N, D] = graph.nodes[node.inputs[0]].shape, V = graph.nodes[node.inputs[1]].shape[1];
+  if (N > LOSS_ROWS) throw new Error(`linearCrossEntropy: ${N} rows (at most ${LOSS_ROWS})`);
   const operands = node.inputs.length - (grad ? 1 : 0);
   const bias = operands === 4;
   const part = grad ? node.attrs.part : 'loss';

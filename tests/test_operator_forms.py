@@ -127,3 +127,10 @@ def test_position_axes_that_no_kernel_counts_are_refused(tool, count):
     assert "position axes" in refused(tool, case)
     tool("operator-graphs", {"cases": [{"name": "most", "family": "rotary", "x": [4, 1, 600], "positions": [4, 256],
                                         "options": {"axis": 0, "frequencies": [1.0], "axes": [255], "positionAxes": 256}}]})
+
+
+@pytest.mark.parametrize("V", [5, 200])
+def test_more_rows_than_a_kernel_counts_are_refused(tool, V):
+    """2^32 + 5 rows were 5 in a kernel's 32 bits."""
+    for N in (2 ** 28 + 1, 2 ** 32 + 5):
+        assert "rows (at most 268435456)" in refused(tool, {"family": "loss", "N": N, "d": 1, "V": V, "gradient": True})
