@@ -28,8 +28,8 @@
 // reads the one it writes), which keeps one kernel text and one argument block for all pieces.
 //
 // Bound: the matrix cores (6·N·d·V flops with gradients, 2·N·d·V without). 8192 rows of d 1024 against 65 536 classes, us: maxima
-// 57 (5.3 TB/s), split 114 (5.3 TB/s), and each of 4 pieces logits 763 - 788 (350 TFLOP/s), join 9, spread 212 (5.0 TB/s), grads 1323 -
-// 1399 (400), sums 9. Fewer passes would need W's scale before it is read, and a row's sum before its logits are left.
+// 59 (5.1 TB/s), split 114 (5.6 TB/s), and each of 4 pieces logits 747 (368 TFLOP/s), join 9, spread 214 (4.9 TB/s), grads 1311
+// (419), sums 9. Fewer passes would need W's scale before it is read, and a row's sum before its logits are left.
 
 #pragma once
 

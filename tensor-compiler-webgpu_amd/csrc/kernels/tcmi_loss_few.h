@@ -12,7 +12,7 @@
 // groups of four columns.
 //
 // Bound: memory, 4·d·V bytes for the losses and 8·d·V more for the gradients; past 32 rows the matrix cores. Of d 1024 and
-// 131 072 classes 109 us for one row, 115 for 16 (4.7 TB/s), 212 for 64 (81 TFLOP/s); with gradients 386, 394 and 591.
+// 131 072 classes 103 us for one row, 107 for 16 (5.0 TB/s), 178 for 64 (96 TFLOP/s); with gradients, which read W again, 384, 388 and 552.
 
 #pragma once
 

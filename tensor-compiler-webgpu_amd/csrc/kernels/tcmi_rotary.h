@@ -217,6 +217,7 @@ __device__ __forceinline__ void rotary(const float* __restrict__ x, const float*
       if constexpr (S::GAIN) {
         float ss = 0.f;
         L::zip([&](float& e) { ss = fmaf(e, e, ss); }, v);
+        // 1 ulp; a Newton step on it leaves every error as it is (outputs 6.5e-8, dx 7e-8, dgain 1.2e-7 - 2e-7 of their norms).
         r = __builtin_amdgcn_rsqf(lanes_sum<S::LANES>(ss) * (1.f / S::DH) + S::eps());
       }
       if constexpr (!GRAD) {

@@ -132,9 +132,10 @@ const LOSS_ROWS = 2 ** 28;
 const LOSS_PARTS = ['dh', 'dW', 'dbias', 'loss'];
 const CUS = 256;
 /**
- * Rows up to which W is read as it is (tcmi_loss_few.h), by time, without and with gradients (us): 64 rows of d 1024, V 131072
- * 212 and 591, by products of pairs 504 and 1019; of d 64, V 96 10.0 and 18.8, by pairs 13.0 and 17.5. 16 rows: 115 and 394, 501
- * and 1001; 7.3 and 11.8, 12.8 and 16.9. Its time grows with the rows from 16 on, the pairs' hardly before 128.
+ * Rows up to which W is read as it is (tcmi_loss_few.h): those its kernels are laid out for, four tiles of rows in registers, not where both
+ * forms take as long. Without and with gradients, of d 1024, V 131072 (us): 16 rows 107 and 388, 64 rows 178 and 552, by products of
+ * pairs 504 and 1019; the next row, by pairs, 484 and 962, and 128 rows 500 and 973: more tiles of rows would carry it to some 130 rows
+ * without gradients, 100 with them.
  */
 const FEW_ROWS = 64;
 /**
