@@ -54,7 +54,7 @@ struct LossState {
 };
 
 // S: the sizes of one launch as constants of its text: N, D, V; NP rows a piece, PIECES of them; DP, VP: d and V padded to
-// whole tiles; BIAS; HBLOCKS, WBLOCKS workgroups of `maxima` over h's rows and W; PER groups of four a thread of `split` takes; LKIND, HKIND and
+// whole tiles; BIAS; HBLOCKS, WBLOCKS workgroups of `maxima` over h's rows (HLANES lanes each) and W; PER groups of four a thread of `split` takes; LKIND, HKIND and
 // WKIND of tiles for the logits, dh and dW; RB rows a workgroup of `spread`, CT threads across columns there;
 // JOINED: `join` runs; VECD, VECV: d, V multiples of 4; HCHUNKS, HK, WCHUNKS, WK: chunks of K of dh and dW, their slices.
 // WS: byte offsets in the workspace.
@@ -96,21 +96,21 @@ constexpr int NO_SCALE = 252;      // at most: two of scale_of's
 template <class S, bool DW>
 __device__ __forceinline__ void loss_maxima(const Loss<S>& L, float* scratch, uint32_t block) {
   if (block < S::HBLOCKS) {
-    // A wavefront a row. Rows left out are loaded all the same, so that no load waits for a target.
-    const uint32_t lane = threadIdx.x % 64;
+    // HLANES lanes a row. Rows left out are loaded all the same, so that no load waits for a target.
+    const uint32_t lane = threadIdx.x % S::HLANES;
     int least = NO_SCALE;
-    for (uint32_t r = block * 4 + threadIdx.x / 64; r < S::N; r += S::HBLOCKS * 4) {
+    for (uint32_t r = block * (256 / S::HLANES) + threadIdx.x / S::HLANES; r < S::N; r += S::HBLOCKS * (256 / S::HLANES)) {
       const float* h = L.h + (size_t)r * S::D;
       float top = 0.f;
       if constexpr (S::VECD) {
 #pragma unroll 4
-        for (uint32_t i = lane; i < S::D / 4; i += 64) top = top_of(reinterpret_cast<const f4*>(h)[i], top);
+        for (uint32_t i = lane; i < S::D / 4; i += S::HLANES) top = top_of(reinterpret_cast<const f4*>(h)[i], top);
       } else {
 #pragma unroll 8
-        for (uint32_t i = lane; i < S::D; i += 64) top = fmaxf(top, finite_abs(h[i]));
+        for (uint32_t i = lane; i < S::D; i += S::HLANES) top = fmaxf(top, finite_abs(h[i]));
       }
 #pragma unroll
-      for (int off = 32; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+      for (int off = S::HLANES / 2; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
       const bool kept = L.kept(r);
       const int e = scale_of(kept ? top : 0.f);
       if (lane == 0) L.exponents()[r] = e;
@@ -121,7 +121,9 @@ __device__ __forceinline__ void loss_maxima(const Loss<S>& L, float* scratch, ui
     }
     if constexpr (DW) {
       int* const leasts = reinterpret_cast<int*>(scratch);
-      if (lane == 0) leasts[threadIdx.x / 64] = least;
+#pragma unroll
+      for (int off = 32; off >= S::HLANES; off >>= 1) least = min(least, __shfl_xor(least, off, 64));
+      if (threadIdx.x % 64 == 0) leasts[threadIdx.x / 64] = least;
       __syncthreads();
       if (threadIdx.x == 0) reinterpret_cast<int*>(L.at(S::MAXIMA))[block] = min(min(leasts[0], leasts[1]), min(leasts[2], leasts[3]));
     }

@@ -199,7 +199,8 @@ function lossSizes(N, D, V, bias, parts, piece) {
   const g = gradTiles(NP, D, VP), DP = grad ? g.DP : align(D, 64);
   // Threads across columns: fewer, and rows side by side, where workgroups would be fewer than two a CU.
   const CT = (() => { let t = 16; while (2 * t <= Math.min(256, VP / 8) && ceil(VP, 16 * t) * NP / RB >= 2 * CUS) t *= 2; return t; })();
-  const z = { N, D, V, DP, VP, NP, PIECES, RB, CT, BIAS: bias, HBLOCKS: clamp(N / 4, 1024), WBLOCKS: clamp(D * V / 16384, 1024),
+  const lanes = (() => { let n = 1; while (n < 64 && n < (D % 4 === 0 ? D / 4 : D)) n *= 2; return n; })();
+  const z = { N, D, V, DP, VP, NP, PIECES, RB, CT, BIAS: bias, HLANES: lanes, HBLOCKS: clamp(N * lanes / 256, 1024), WBLOCKS: clamp(D * V / 16384, 1024),
     PER: clamp((NP * PIECES * DP + DP * VP) / 4 / 256 / 1024, 16), LKIND: large ? TALL : SMALL, HKIND: g.large ? TALL : SMALL, WKIND: g.large ? WIDE : SMALL, JOINED: !grad || VP / (16 * LT) > 32, VECD: D % 4 === 0, VECV: V % 4 === 0,
     HCHUNKS: g.h.chunks, HK: g.h.each, WCHUNKS: g.w.chunks, WK: g.w.each };
   let at = 0;
@@ -257,7 +258,7 @@ function fewSizes(N, D, V, bias, parts) {
 }
 
 function lossMaker(z, e, bias, grad) {
-  const counts = /^([NDV]P?|NP|RT|PIECES|RB|CT|[HW]BLOCKS|PER|[HW]CHUNKS|[HW]K|WAVES|COLS|CHUNKS|DTILES|CG|RC|DG)$/;
+  const counts = /^([NDV]P?|NP|RT|PIECES|RB|CT|HLANES|[HW]BLOCKS|PER|[HW]CHUNKS|[HW]K|WAVES|COLS|CHUNKS|DTILES|CG|RC|DG)$/;
   const sizes = Object.keys(z).map((k) => (typeof z[k] === 'boolean' ? `  static constexpr bool ${k} = ${z[k]};`
     : k.endsWith('KIND') ? `  static constexpr int ${k} = ${z[k]};`
       : `  static constexpr ${counts.test(k) ? 'uint32_t' : 'size_t'} ${k} = ${z[k]}u;`)).join('\n');
