@@ -13,7 +13,7 @@
 // its largest finite magnitude below 2^15: h's rows each their own, G's rows each its cotangent's, so that a row's
 // loss and dh hang on nothing that other rows hold; W one for all. dW sums over the rows: it takes a split of h of its own, each
 // row times what G's row lacks of one scale for all, that of the largest |w|·|h|. What a pair loses below 2^-36 is then at most
-// 2^-51 of |h row|·|W| a term of z, of |w|·|W| one of dh and of the largest |w|·|h| one of dW, these magnitudes the largest in each.
+// 2^-50 of |h row|·|W| a term of z, of |w|·|W| one of dh and of the largest |w|·|h| one of dW, these magnitudes the largest in each.
 //
 //   maxima   h's row exponents, the least exponent of |w|·|h|, partial maxima of |W|
 //   split    h (for dW again, times w's scale) and W as pairs, padded with zeros to whole tiles

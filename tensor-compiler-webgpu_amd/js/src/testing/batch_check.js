@@ -177,7 +177,7 @@ function checkBatches(plain, batched) {
       for (let k = 0; k < b.count; k++) unitOf[b.start + k] = b.start;
       continue;
     }
-    if (first.kernels.length === 1 && first.kernels[0].joint) {
+    if (first.kernels.length === 1 && first.kernels[0].joint && !first.kernels[0].joint.build) {
       // An attention gradient's three parts in one launch of their joint kernel: members
       // dQ, dK, dV in that order, of one joint kernel, reading the same operands.
       const j = first.kernels[0].joint;

@@ -134,3 +134,12 @@ def test_more_rows_than_a_kernel_counts_are_refused(tool, V):
     """2^32 + 5 rows were 5 in a kernel's 32 bits."""
     for N in (2 ** 28 + 1, 2 ** 32 + 5):
         assert "rows (at most 268435456)" in refused(tool, {"family": "loss", "N": N, "d": 1, "V": V, "gradient": True})
+
+
+def test_equal_parts_that_run_side_by_side_pass_the_batch_check(tool):
+    """Two nodes of which the same one part is kept: a batch of their own kernels, no joint launch."""
+    case = {"name": "dx", "family": "rotary", "x": [3, 40, 2, 64], "positions": [40], "gain": True, "gradient": True, "twin": [3, 40, 2, 64]}
+    g = tool("operator-graphs", {"cases": [case]})[0]
+    keep = [k for n, k in zip(g["names"], g["keep"]) if n.startswith("dx")]
+    r = tool("batch-check", {"graphs": [{"name": "dx", "graph": g["graph"], "keep": keep}]})[0]
+    assert r["check"]["ok"] and len(keep) == 2
