@@ -1,0 +1,315 @@
+// A block's branch y joined to its stream x, with the norms on both sides of the block in the same pass:
+//
+//   h = residual·x + gate·N(y),   n = N(h),   N(v) = (v - mean)·r·gain + bias,  r = (mean((v - mean)²) + eps)^-1/2
+// (mean 0 and no bias for the root mean square; N(y) = y without a norm), and the gradient of both, with ^ for
+// (v - mean)·r:
+//   dH = dh + N'(dn·gain; h),   N'(g; v) = r·(g - mean(g) - v^·mean(g·v^)),
+//   dx = residual·dH,   dp = dH·gate,   dy = N'(dp·postGain; y),
+//   dgain = sum dn·h^, dbias = sum dn, dgate = sum dH·p (or each row's own), dpostGain = sum dp·y^, dpostBias = sum dp.
+//
+// LANES lanes share a row, at most 16 floats of it each, in registers: a row is read once and what the
+// gradient needs of the forward pass is formed again. Means are of the row itself, squares of what is left. A workgroup walks
+// its rows and keeps the vectors' sums in registers; its rows side by side are then added in LDS, and the
+// workgroups' sums by a second launch, always in the same order.
+//
+// Bound: HBM.
+
+#pragma once
+
+#include "tcmi_device.h"
+
+namespace tcmi {
+
+struct ResidualArgs {
+  const float *x, *y, *gain, *bias, *postGain, *postBias, *gate, *dh, *dn;
+};
+
+// A row's floats of one lane: UNITS groups of E, LANES groups apart; past the row's end 0.
+template <class S>
+struct ResidualLane {
+  static constexpr int F = S::UNITS * S::E;
+  typedef float Row[F];
+  uint32_t lane;
+  float* lds;
+
+  __device__ __forceinline__ uint32_t dim(int u) const { return (u * S::LANES + lane) * S::E; }
+  __device__ __forceinline__ bool in(int u) const { return S::D % (S::LANES * S::E) == 0u || dim(u) < S::D; }
+  __device__ __forceinline__ void load(const float* __restrict__ p, Row& v) const {
+#pragma unroll
+    for (int u = 0; u < S::UNITS; ++u) {
+      if constexpr (S::E == 4) {
+        f4 q = {0.f, 0.f, 0.f, 0.f};
+        if (in(u)) q = *reinterpret_cast<const f4*>(p + dim(u));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[u * 4 + e] = q[e];
+      } else {
+        v[u] = in(u) ? p[dim(u)] : 0.f;
+      }
+    }
+  }
+  __device__ __forceinline__ void store(float* __restrict__ p, const Row& v) const {
+#pragma unroll
+    for (int u = 0; u < S::UNITS; ++u) {
+      if (!in(u)) continue;
+      if constexpr (S::E == 4) *reinterpret_cast<f4*>(p + dim(u)) = f4{v[u * 4], v[u * 4 + 1], v[u * 4 + 2], v[u * 4 + 3]};
+      else p[dim(u)] = v[u];
+    }
+  }
+  // Sums over the row's lanes, every lane getting them; over several wavefronts through LDS.
+  template <int N>
+  __device__ __forceinline__ void total(float (&v)[N]) const {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+#pragma unroll
+      for (uint32_t off = min(S::LANES, 64u) / 2u; off >= 1u; off >>= 1) v[k] += __shfl_xor(v[k], off, 64);
+    }
+    if constexpr (S::LANES > 64u) {
+      // A row's wavefronts are the workgroup's (LANES = THREADS) or a part of them.
+      constexpr uint32_t WAVES = S::LANES / 64u;
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        __syncthreads();
+        if (threadIdx.x % 64u == 0u) lds[threadIdx.x / 64u] = v[k];
+        __syncthreads();
+        const uint32_t first = threadIdx.x / S::LANES * WAVES;
+        float sum = lds[first];
+#pragma unroll
+        for (uint32_t w = 1; w < WAVES; ++w) sum += lds[first + w];
+        v[k] = sum;
+      }
+    }
+  }
+  // v to its normalised row, without gain and bias; r.
+  __device__ __forceinline__ float normalise(Row& v) const {
+    if constexpr (S::LAYER) {
+      float m[1] = {0.f};
+#pragma unroll
+      for (int i = 0; i < F; ++i) m[0] += v[i];
+      total(m);
+      const float mean = m[0] * (1.f / S::D);
+#pragma unroll
+      for (int i = 0; i < F; ++i) v[i] = in(i / S::E) ? v[i] - mean : 0.f;
+    }
+    float s[1] = {0.f};
+#pragma unroll
+    for (int i = 0; i < F; ++i) s[0] = fmaf(v[i], v[i], s[0]);
+    total(s);
+    const float r = __builtin_amdgcn_rsqf(s[0] * (1.f / S::D) + S::eps());
+#pragma unroll
+    for (int i = 0; i < F; ++i) v[i] *= r;
+    return r;
+  }
+  // g, a gradient of a normalised row v, to that of the row: r·(g - mean(g) - v·mean(g·v)).
+  __device__ __forceinline__ void back(Row& g, const Row& v, float r) const {
+    float s[S::LAYER ? 2 : 1] = {};
+#pragma unroll
+    for (int i = 0; i < F; ++i) {
+      s[0] = fmaf(g[i], v[i], s[0]);
+      if constexpr (S::LAYER) s[1] += g[i];
+    }
+    total(s);
+    const float gv = s[0] * (1.f / S::D);
+    float m = 0.f;
+    if constexpr (S::LAYER) m = s[1] * (1.f / S::D);
+#pragma unroll
+    for (int i = 0; i < F; ++i) g[i] = r * (g[i] - m - v[i] * gv);
+  }
+};
+
+// A gate's floats of row `row`.
+template <class S>
+__device__ __forceinline__ void residual_gate(const ResidualLane<S>& l, const ResidualArgs& a, uint32_t row, typename ResidualLane<S>::Row& g) {
+  l.load(S::GATE == 2 ? a.gate + (size_t)row * S::D : a.gate, g);
+}
+
+// p = N(y) and h of one row; yh: y normalised (where it has a norm), with its r; gate.
+template <class S>
+__device__ __forceinline__ float residual_join(const ResidualLane<S>& l, const ResidualArgs& a, uint32_t row, typename ResidualLane<S>::Row& yh,
+                                               typename ResidualLane<S>::Row& p, typename ResidualLane<S>::Row& h) {
+  using L = ResidualLane<S>;
+  l.load(a.y + (size_t)row * S::D, yh);
+  l.load(a.x + (size_t)row * S::D, h);
+  float r = 1.f;
+  if constexpr (S::POST) {
+    r = l.normalise(yh);
+    typename L::Row g;
+    l.load(a.postGain, g);
+#pragma unroll
+    for (int i = 0; i < L::F; ++i) p[i] = yh[i] * g[i];
+    if (a.postBias != nullptr) {
+      l.load(a.postBias, g);
+#pragma unroll
+      for (int i = 0; i < L::F; ++i) p[i] += g[i];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < L::F; ++i) p[i] = yh[i];
+  }
+  if constexpr (S::GATE != 0) {
+    typename L::Row g;
+    residual_gate(l, a, row, g);
+#pragma unroll
+    for (int i = 0; i < L::F; ++i) h[i] = fmaf(S::residual(), h[i], g[i] * p[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < L::F; ++i) h[i] = fmaf(S::residual(), h[i], p[i]);
+  }
+  return r;
+}
+
+// H and NORM: which of h and n are written.
+template <class S>
+__device__ __forceinline__ void residual(const ResidualArgs& a, float* __restrict__ hout, float* __restrict__ nout, float* lds, uint32_t block, uint32_t blocks) {
+  using L = ResidualLane<S>;
+  constexpr uint32_t ROWS = S::THREADS / S::LANES;
+  const L l{threadIdx.x % S::LANES, lds};
+  for (uint32_t row0 = block * ROWS; row0 < S::N; row0 += blocks * ROWS) {
+    // (Every lane takes part in the sums: a row past the last is the last again, and not written.)
+    const uint32_t at = row0 + threadIdx.x / S::LANES, row = min(at, S::N - 1u);
+    typename L::Row yh, p, h;
+    residual_join<S>(l, a, row, yh, p, h);
+    if (S::H && at < S::N) l.store(hout + (size_t)row * S::D, h);
+    if constexpr (S::NORM) {
+      l.normalise(h);
+      typename L::Row g;
+      l.load(a.gain, g);
+#pragma unroll
+      for (int i = 0; i < L::F; ++i) h[i] *= g[i];
+      if (a.bias != nullptr) {
+        l.load(a.bias, g);
+#pragma unroll
+        for (int i = 0; i < L::F; ++i) h[i] += g[i];
+      }
+      if (at < S::N) l.store(nout + (size_t)row * S::D, h);
+    }
+  }
+}
+
+// DX ... DGATE: the gradients to form; DH, DN: which cotangents there are. partial: the SUMS vectors' sums of each
+// workgroup, [SUMS][blocks][D]; lds: ROWS·D floats where rows stand side by side.
+template <class S>
+__device__ __forceinline__ void residual_grad(const ResidualArgs& a, float* __restrict__ dx, float* __restrict__ dy, float* __restrict__ dgate,
+                                              float* __restrict__ partial, float* lds, uint32_t block, uint32_t blocks) {
+  using L = ResidualLane<S>;
+  constexpr uint32_t ROWS = S::THREADS / S::LANES;
+  constexpr bool BRANCH = S::DY || S::DPOSTGAIN || S::DPOSTBIAS || S::DGATE;
+  const L l{threadIdx.x % S::LANES, lds};
+  float sums[S::SUMS > 0 ? S::SUMS : 1][L::F];
+#pragma unroll
+  for (int k = 0; k < S::SUMS; ++k) {
+#pragma unroll
+    for (int i = 0; i < L::F; ++i) sums[k][i] = 0.f;
+  }
+  for (uint32_t row0 = block * ROWS; row0 < S::N; row0 += blocks * ROWS) {
+    const uint32_t at = row0 + threadIdx.x / S::LANES, row = min(at, S::N - 1u);
+    const bool on = at < S::N;
+    typename L::Row yh, p, h, d;
+    const float ry = residual_join<S>(l, a, row, yh, p, h);
+    int k = 0;
+    // What a sum adds of a row past the last: nothing.
+    auto add = [&](float (&sum)[L::F], auto f) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < L::F; ++i) sum[i] += on ? f(i) : 0.f;
+    };
+    if constexpr (S::DN) {
+      l.load(a.dn + (size_t)row * S::D, d);
+      const float rh = l.normalise(h);
+      if constexpr (S::DGAIN) add(sums[k++], [&](int i) { return d[i] * h[i]; });
+      if constexpr (S::DBIAS) add(sums[k++], [&](int i) { return d[i]; });
+      if constexpr (S::DX || BRANCH) {
+        typename L::Row g;
+        l.load(a.gain, g);
+#pragma unroll
+        for (int i = 0; i < L::F; ++i) d[i] *= g[i];
+        l.back(d, h, rh);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < L::F; ++i) d[i] = 0.f;
+    }
+    if constexpr (S::DH && (S::DX || BRANCH)) {
+      typename L::Row g;
+      l.load(a.dh + (size_t)row * S::D, g);
+#pragma unroll
+      for (int i = 0; i < L::F; ++i) d[i] += g[i];
+    }
+    if constexpr (S::DX) {
+      typename L::Row g;
+#pragma unroll
+      for (int i = 0; i < L::F; ++i) g[i] = S::residual() * d[i];
+      if (on) l.store(dx + (size_t)row * S::D, g);
+    }
+    if constexpr (BRANCH) {
+      if constexpr (S::GATE != 0) {
+        if constexpr (S::DGATE) {
+#pragma unroll
+          for (int i = 0; i < L::F; ++i) p[i] *= d[i];
+          if constexpr (S::GATE == 2) {
+            if (on) l.store(dgate + (size_t)row * S::D, p);
+          }
+        }
+        typename L::Row g;
+        residual_gate(l, a, row, g);
+#pragma unroll
+        for (int i = 0; i < L::F; ++i) d[i] *= g[i];
+      }
+      if constexpr (S::DPOSTGAIN) add(sums[k++], [&](int i) { return d[i] * yh[i]; });
+      if constexpr (S::DPOSTBIAS) add(sums[k++], [&](int i) { return d[i]; });
+      if constexpr (S::DGATE && S::GATE == 1) add(sums[k++], [&](int i) { return p[i]; });
+      if constexpr (S::DY) {
+        if constexpr (S::POST) {
+          typename L::Row g;
+          l.load(a.postGain, g);
+#pragma unroll
+          for (int i = 0; i < L::F; ++i) d[i] *= g[i];
+          l.back(d, yh, ry);
+        }
+        if (on) l.store(dy + (size_t)row * S::D, d);
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < S::SUMS; ++k) {
+    float* to = partial + ((size_t)k * blocks + block) * S::D;
+    if constexpr (ROWS == 1u) {
+      l.store(to, sums[k]);
+    } else {
+      __syncthreads();
+      l.store(lds + threadIdx.x / S::LANES * S::D, sums[k]);
+      __syncthreads();
+      for (uint32_t e = threadIdx.x; e < S::D; e += S::THREADS) {
+        float sum = lds[e];
+#pragma unroll
+        for (uint32_t g = 1; g < ROWS; ++g) sum += lds[g * S::D + e];
+        to[e] = sum;
+      }
+    }
+  }
+}
+
+// out[e] = the sum of vector `which`'s `blocks` partial rows: a workgroup of 1024 takes 16 columns, 64 threads a
+// column, each its own rows in turn, their sums added in order by eights.
+template <uint32_t D, int SUMS>
+__device__ __forceinline__ void residual_sum(const float* __restrict__ partial, float* __restrict__ out, uint32_t blocks, float* scratch, uint32_t block, uint32_t which) {
+  const uint32_t e = block * 16u + threadIdx.x % 16u, part = threadIdx.x / 16u;
+  const float* from = partial + (size_t)which * blocks * D;
+  float sum = 0.f;
+  if (e < D) {
+#pragma unroll 4
+    for (uint32_t k = part; k < blocks; k += 64u) sum += from[(size_t)k * D + e];
+  }
+  scratch[threadIdx.x] = sum;
+  __syncthreads();
+  if (part < 8u) {
+    for (uint32_t q = part + 8u; q < 64u; q += 8u) sum += scratch[q * 16u + threadIdx.x % 16u];
+  }
+  __syncthreads();
+  if (part < 8u) scratch[threadIdx.x] = sum;
+  __syncthreads();
+  if (part == 0u && e < D) {
+    for (uint32_t q = 1; q < 8u; ++q) sum += scratch[q * 16u + threadIdx.x];
+    out[e] = sum;
+  }
+}
+
+}  // namespace tcmi

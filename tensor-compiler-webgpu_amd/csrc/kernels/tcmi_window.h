@@ -1,0 +1,401 @@
+// Softmax attention over a sliding window with sinks, and its gradient, on the fp32 matrix cores.
+//
+// A query at position p of a sequence of L keys sees the keys j <= p with p - WINDOW < j or j < SINKS. With
+// s_j = scale·q·k_j over those:
+//   o = sum_j P_j v_j,  P_j = exp(s_j - lse),  lse = log(sum_j exp(s_j));
+//   dS_j = P_j·(dy·v_j - dy·o),  dq = scale·sum_j dS_j k_j,  dk_j = scale·sum dS_j q,  dv_j = sum P_j dy (over the queries that see j).
+// A query that sees nothing has o = 0, lse = -inf and no gradients.
+//
+// Rows: the queries of the R = H/HK heads that share a key head, query t's heads side by side, 16 rows a tile; keys 16 a
+// tile. With lane = 16·q + t (t in 0..15) of a 16x16x4 product:
+//   scores   mfma(key value, row value): lane (t, q) holds row t, keys 4q ... 4q + 3, which is
+//   output   mfma(V value, P value): the second product's operand for those keys; lane (t, q) gets row t, dims 16g + 4q ....
+// (The gradients of keys exchange the parts of rows and keys.) So scores never leave the registers, and keys and values are read
+// from memory as the products take them. The four wavefronts of a workgroup deal the tiles among them and join at the
+// end through LDS, always in the same order; of few rows, several workgroups do (SPLITS), whose sums are joined by a launch.
+
+#pragma once
+
+#include "tcmi_device.h"
+
+namespace tcmi {
+
+constexpr float LOG2E = 1.4426950408889634f;
+
+// What a sequence's queries see.
+template <class S>
+struct WindowSpan {
+  static constexpr uint32_t R = S::H / S::HK, ROWS = S::T * R;
+  int32_t length, first;       // keys, and the position of query 0
+
+  __device__ __forceinline__ WindowSpan(const float* lengths, uint32_t b) {
+    length = static_cast<int32_t>(S::KEYS);
+    if constexpr (S::LENGTHS) {
+      const float l = lengths[b];
+      // (Neither NaN nor what lies outside reaches the conversion.)
+      if (!(l < static_cast<float>(S::KEYS))) length = l >= static_cast<float>(S::KEYS) ? length : 0;
+      else length = l > 0.f ? static_cast<int32_t>(l) : 0;
+    }
+    first = S::LAST ? length - static_cast<int32_t>(S::T) : 0;
+  }
+  // The first key of the window of position p.
+  __device__ __forceinline__ int32_t from(int32_t p) const { return S::WINDOW == 0u || p < static_cast<int32_t>(S::WINDOW) ? 0 : p - static_cast<int32_t>(S::WINDOW) + 1; }
+  __device__ __forceinline__ bool stands(int32_t p) const { return p >= 0 && p < length; }
+  // Whether position p (in 0 .. length-1) sees key j.
+  __device__ __forceinline__ bool sees(int32_t p, int32_t j) const { return j <= p && (j >= from(p) || j < static_cast<int32_t>(S::SINKS)); }
+};
+
+// Tiles of 16 in order: `sinks` of them from 0, then from `main` up to `all` in number. Their keys that any of the rows sees: lo ... hi
+// and the sinks before.
+struct WindowTiles {
+  int32_t sinks, main, all, lo, hi;
+  __device__ __forceinline__ int32_t at(int32_t i) const { return i < sinks ? i : main + i - sinks; }
+};
+
+// The tiles of keys that rows row0 .. row1 see, of those that stand in their sequence.
+template <class S>
+__device__ __forceinline__ WindowTiles window_keys(const WindowSpan<S>& w, uint32_t row0, uint32_t row1) {
+  constexpr int32_t R = WindowSpan<S>::R;
+  int32_t p0 = w.first + static_cast<int32_t>(row0) / R, p1 = w.first + static_cast<int32_t>(row1) / R;
+  p0 = max(p0, 0);
+  p1 = min(p1, w.length - 1);
+  if (p0 > p1) return {0, 0, 0, 0, -1};
+  const int32_t lo = w.from(p0), sinks = (min(static_cast<int32_t>(S::SINKS), lo) + 15) / 16, main = max(lo / 16, sinks);
+  return {sinks, main, sinks + p1 / 16 + 1 - main, lo, p1};
+}
+
+// Floats at p, four of them where d is within the head.
+template <class S>
+__device__ __forceinline__ f4 window_load(const float* __restrict__ p, uint32_t d, bool on) {
+  f4 v = {0.f, 0.f, 0.f, 0.f};
+  if constexpr (S::VEC) {
+    if (on && d < S::DH) v = *reinterpret_cast<const f4*>(p + d);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (on && d + i < S::DH) v[i] = p[d + i];
+    }
+  }
+  return v;
+}
+template <class S>
+__device__ __forceinline__ void window_store(float* __restrict__ p, uint32_t d, const f4& v) {
+  if constexpr (S::VEC) {
+    if (d < S::DH) *reinterpret_cast<f4*>(p + d) = v;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (d + i < S::DH) p[d + i] = v[i];
+    }
+  }
+}
+
+// Lane (t, q)'s part of a 16 x DH tile along its rows: dims 16g + 4q ... of row t.
+template <class S, int G>
+__device__ __forceinline__ void window_along(f4 (&v)[G], const float* __restrict__ row, bool on) {
+#pragma unroll
+  for (int g = 0; g < G; ++g) v[g] = window_load<S>(row, 16 * g + 4 * ((threadIdx.x >> 4) & 3u), on);
+}
+// And across them: dim 16g + t of the tile's key 4q + s, of the keys from j0 on those that one of the rows sees (a value that
+// no query sees may be anything: it is 0 here, for 0 times it would be NaN).
+template <class S, int G>
+__device__ __forceinline__ void window_across(f4 (&v)[G], const float* __restrict__ base, size_t step, int32_t j0, const WindowTiles& tiles) {
+  const int t = threadIdx.x & 15, q = (threadIdx.x >> 4) & 3;
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+    const int32_t j = j0 + 4 * q + s;
+    const bool on = j <= tiles.hi && (j >= tiles.lo || j < static_cast<int32_t>(S::SINKS));
+#pragma unroll
+    for (int g = 0; g < G; ++g) v[g][s] = on && 16 * g + t < static_cast<int>(S::DH) ? base[(size_t)j * step + 16 * g + t] : 0.f;
+  }
+}
+// acc[k of a][t of b] += the products of two tiles along their rows.
+template <int G>
+__device__ __forceinline__ f4 window_scores(const f4 (&a)[G], const f4 (&b)[G]) {
+  f4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+#pragma unroll
+    for (int s = 0; s < 4; ++s) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[g][s], b[g][s], acc, 0, 0, 0);
+  }
+  return acc;
+}
+template <int G>
+__device__ __forceinline__ void window_sum(f4 (&acc)[G], const f4 (&across)[G], const f4& p) {
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+#pragma unroll
+    for (int s = 0; s < 4; ++s) acc[g] = __builtin_amdgcn_mfma_f32_16x16x4f32(across[g][s], p[s], acc[g], 0, 0, 0);
+  }
+}
+
+template <int DH>
+constexpr int window_lds() { return 4 * 64 * ((DH + 15) / 16) * 4 + 4 * 32; }
+
+// The four wavefronts' acc added into the first's, each times its factor f.
+template <int G>
+__device__ __forceinline__ void window_gather(f4 (&acc)[G], float f, float* lds) {
+  f4* at = reinterpret_cast<f4*>(lds);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  __syncthreads();
+#pragma unroll
+  for (int g = 0; g < G; ++g) at[(wave * G + g) * 64 + lane] = acc[g] * f;
+  __syncthreads();
+#pragma unroll
+  for (int g = 0; g < G; ++g) acc[g] = at[g * 64 + lane] + at[(G + g) * 64 + lane] + at[(2 * G + g) * 64 + lane] + at[(3 * G + g) * 64 + lane];
+}
+
+// Workgroup: a tile of rows, a split, a sequence's key head.
+template <class S>
+__device__ __forceinline__ void window_rows(const float* __restrict__ qp, const float* __restrict__ kp, const float* __restrict__ vp, const float* __restrict__ lengths,
+                                            float* __restrict__ out, float* __restrict__ lse, char* ws, float* lds, uint32_t wg) {
+  constexpr int G = (S::DH + 15) / 16;
+  using Span = WindowSpan<S>;
+  constexpr uint32_t R = Span::R, ROWS = Span::ROWS;
+  const uint32_t split = wg % S::SPLITS, tile = wg / S::SPLITS % S::TILES, head = wg / (S::SPLITS * S::TILES), b = head / S::HK, hk = head % S::HK;
+  const int lane = threadIdx.x & 63, t = lane & 15, q = lane >> 4, wave = threadIdx.x >> 6;
+  const Span w(lengths, b);
+  const uint32_t row0 = tile * 16u, row = row0 + t, at = min(row, ROWS - 1u);
+  const size_t line = ((size_t)b * S::T + at / R) * S::H + hk * R + at % R;
+  const int32_t p = w.first + static_cast<int32_t>(at / R);
+  const bool on = row < ROWS && w.stands(p);
+  f4 qf[G], acc[G];
+  window_along<S>(qf, qp + line * S::DH, on);
+  // Scores in powers of two.
+  const float scale = static_cast<float>(S::scale() * 1.4426950408889634);
+#pragma unroll
+  for (int g = 0; g < G; ++g) acc[g] = f4{0.f, 0.f, 0.f, 0.f};
+  const WindowTiles tiles = window_keys(w, row0, min(row0 + 15u, ROWS - 1u));
+  const int32_t each = (tiles.all + static_cast<int32_t>(S::SPLITS) - 1) / static_cast<int32_t>(S::SPLITS);
+  const int32_t begin = min(tiles.all, static_cast<int32_t>(split) * each), end = min(tiles.all, begin + each);
+  const size_t step = (size_t)S::HK * S::DH;
+  const float* kb = kp + ((size_t)b * S::KEYS * S::HK + hk) * S::DH;
+  const float* vb = vp + ((size_t)b * S::KEYS * S::HK + hk) * S::DH;
+  float m = -TCMI_INF, l = 0.f;
+  for (int32_t i = begin + wave; i < end; i += 4) {
+    const int32_t j0 = tiles.at(i) * 16;
+    f4 kf[G], vf[G];
+    window_along<S>(kf, kb + (size_t)min(j0 + t, w.length - 1) * step, j0 + t < w.length);
+    window_across<S>(vf, vb, step, j0, tiles);
+    f4 s = window_scores(kf, qf);
+    float top = -TCMI_INF;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      s[r] = on && w.sees(p, j0 + 4 * q + r) ? s[r] * scale : -TCMI_INF;
+      top = fmaxf(top, s[r]);
+    }
+    top = fmaxf(m, quad16_reduce<true>(top));
+    const float base = top == -TCMI_INF ? 0.f : top, alpha = __builtin_amdgcn_exp2f(m - base);
+    float sum = 0.f;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      s[r] = __builtin_amdgcn_exp2f(s[r] - base);
+      sum += s[r];
+    }
+    l = l * alpha + sum;
+    m = top;
+#pragma unroll
+    for (int g = 0; g < G; ++g) acc[g] *= alpha;
+    window_sum(acc, vf, s);
+  }
+  // (Each lane has added its own keys.)
+  l = quad16_reduce<false>(l);
+  float* stats = lds + 4 * 64 * G * 4;
+  if (q == 0) {
+    stats[wave * 32 + t] = m;
+    stats[wave * 32 + 16 + t] = l;
+  }
+  __syncthreads();
+  float top = -TCMI_INF, total = 0.f;
+#pragma unroll
+  for (int v = 0; v < 4; ++v) top = fmaxf(top, stats[v * 32 + t]);
+  const float base = top == -TCMI_INF ? 0.f : top;
+#pragma unroll
+  for (int v = 0; v < 4; ++v) total += stats[v * 32 + 16 + t] * __builtin_amdgcn_exp2f(stats[v * 32 + t] - base);
+  window_gather(acc, __builtin_amdgcn_exp2f(m - base), lds);
+  if (wave != 0 || row >= ROWS) return;
+  if constexpr (S::SPLITS == 1u) {
+    const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
+    if (out != nullptr) {
+#pragma unroll
+      for (int g = 0; g < G; ++g) window_store<S>(out + line * S::DH, 16 * g + 4 * q, acc[g] * inv);
+    }
+    if (lse != nullptr && q == 0) lse[line] = total > 0.f || total != total ? (base + __builtin_amdgcn_logf(total)) * 0.69314718055994531f : -TCMI_INF;
+  } else {
+    const size_t place = ((size_t)split * S::B * S::HK + head) * S::TILES * 16u + row;
+#pragma unroll
+    for (int g = 0; g < G; ++g) window_store<S>(reinterpret_cast<float*>(ws + S::OUT) + place * S::DH, 16 * g + 4 * q, acc[g]);
+    if (q == 0) reinterpret_cast<float2*>(ws + S::STATS)[place] = make_float2(top, total);
+  }
+}
+
+// Row `at` of all key heads' rows, a wavefront: its splits' sums.
+template <class S>
+__device__ __forceinline__ void window_join(float* __restrict__ out, float* __restrict__ lse, const char* __restrict__ ws, uint32_t at) {
+  using Span = WindowSpan<S>;
+  constexpr uint32_t R = Span::R, HEADS = S::B * S::HK;
+  const uint32_t head = at / (S::TILES * 16u), row = at % (S::TILES * 16u), lane = threadIdx.x & 63u;
+  if (head >= HEADS || row >= Span::ROWS) return;
+  const float2* stats = reinterpret_cast<const float2*>(ws + S::STATS);
+  const size_t step = (size_t)HEADS * S::TILES * 16u;
+  float top = -TCMI_INF, total = 0.f;
+  for (uint32_t k = lane; k < S::SPLITS; k += 64u) top = fmaxf(top, stats[k * step + at].x);
+  top = wave_reduce<true>(top);
+  const float base = top == -TCMI_INF ? 0.f : top;
+  for (uint32_t k = lane; k < S::SPLITS; k += 64u) total += stats[k * step + at].y * __builtin_amdgcn_exp2f(stats[k * step + at].x - base);
+  total = wave_reduce<false>(total);
+  const size_t line = ((size_t)(head / S::HK) * S::T + row / R) * S::H + head % S::HK * R + row % R;
+  if (lse != nullptr && lane == 0u) lse[line] = total > 0.f || total != total ? (base + __builtin_amdgcn_logf(total)) * 0.69314718055994531f : -TCMI_INF;
+  if (out == nullptr) return;
+  const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
+  for (uint32_t d = lane; d < S::DH; d += 64u) {
+    float sum = 0.f;
+#pragma unroll 4
+    for (uint32_t k = 0; k < S::SPLITS; ++k) sum += reinterpret_cast<const float*>(ws + S::OUT)[(k * step + at) * S::DH + d] * __builtin_amdgcn_exp2f(stats[k * step + at].x - base);
+    out[line * S::DH + d] = sum * inv;
+  }
+}
+
+struct WindowGradArgs {
+  const float *q, *k, *v, *lengths, *o, *lse, *dy, *mass;
+};
+
+// mass[line] = dy·o of one head of one query: 16 lanes a line.
+template <class S>
+__device__ __forceinline__ void window_mass(const float* __restrict__ o, const float* __restrict__ dy, float* __restrict__ mass, size_t line) {
+  constexpr size_t LINES = (size_t)S::B * S::T * S::H;
+  const uint32_t lane = threadIdx.x & 15u;
+  const size_t at = min(line, LINES - 1u);
+  float sum = 0.f;
+  for (uint32_t d = 4u * lane; d < S::DH; d += 64u) {
+    const f4 x = window_load<S>(o + at * S::DH, d, true), y = window_load<S>(dy + at * S::DH, d, true);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum = fmaf(x[i], y[i], sum);
+  }
+  sum = group_reduce<false, 16>(sum);
+  if (lane == 0u && line < LINES) mass[line] = sum;
+}
+
+// Workgroup: a tile of rows of a sequence's key head.
+template <class S>
+__device__ __forceinline__ void window_dq(const WindowGradArgs a, float* __restrict__ dq, float* lds, uint32_t wg) {
+  constexpr int G = (S::DH + 15) / 16;
+  using Span = WindowSpan<S>;
+  constexpr uint32_t R = Span::R, ROWS = Span::ROWS;
+  const uint32_t tile = wg % S::TILES, head = wg / S::TILES, b = head / S::HK, hk = head % S::HK;
+  const int lane = threadIdx.x & 63, t = lane & 15, q = lane >> 4, wave = threadIdx.x >> 6;
+  const Span w(a.lengths, b);
+  const uint32_t row0 = tile * 16u, row = row0 + t, at = min(row, ROWS - 1u);
+  const size_t line = ((size_t)b * S::T + at / R) * S::H + hk * R + at % R;
+  const int32_t p = w.first + static_cast<int32_t>(at / R);
+  const bool on = row < ROWS && w.stands(p);
+  const float scale = static_cast<float>(S::scale() * 1.4426950408889634);
+  f4 qf[G], df[G], acc[G];
+  window_along<S>(qf, a.q + line * S::DH, on);
+  window_along<S>(df, a.dy + line * S::DH, on);
+  const float lse = on ? a.lse[line] * LOG2E : 0.f, mass = on ? a.mass[line] : 0.f;
+#pragma unroll
+  for (int g = 0; g < G; ++g) acc[g] = f4{0.f, 0.f, 0.f, 0.f};
+  const WindowTiles tiles = window_keys(w, row0, min(row0 + 15u, ROWS - 1u));
+  const size_t step = (size_t)S::HK * S::DH, base = ((size_t)b * S::KEYS * S::HK + hk) * S::DH;
+  for (int32_t i = wave; i < tiles.all; i += 4) {
+    const int32_t j0 = tiles.at(i) * 16;
+    f4 f[G];
+    window_along<S>(f, a.k + base + (size_t)min(j0 + t, w.length - 1) * step, j0 + t < w.length);
+    f4 s = window_scores(f, qf);
+    window_along<S>(f, a.v + base + (size_t)min(j0 + t, w.length - 1) * step, j0 + t < w.length);
+    const f4 dp = window_scores(f, df);
+    window_across<S>(f, a.k + base, step, j0, tiles);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) s[r] = on && w.sees(p, j0 + 4 * q + r) ? __builtin_amdgcn_exp2f(fmaf(s[r], scale, -lse)) * (dp[r] - mass) : 0.f;
+    window_sum(acc, f, s);
+  }
+  window_gather(acc, 1.f, lds);
+  if (wave != 0 || row >= ROWS) return;
+#pragma unroll
+  for (int g = 0; g < G; ++g) window_store<S>(dq + line * S::DH, 16 * g + 4 * q, acc[g] * static_cast<float>(S::scale()));
+}
+
+// Workgroup: a tile of keys of a sequence's key head.
+template <class S, bool DK, bool DV>
+__device__ __forceinline__ void window_dkv(const WindowGradArgs a, float* __restrict__ dk, float* __restrict__ dv, float* lds, uint32_t wg) {
+  constexpr int G = (S::DH + 15) / 16;
+  using Span = WindowSpan<S>;
+  constexpr int32_t R = Span::R, ROWS = Span::ROWS;
+  const uint32_t tile = wg % S::KTILES, head = wg / S::KTILES, b = head / S::HK, hk = head % S::HK;
+  const int lane = threadIdx.x & 63, t = lane & 15, q = lane >> 4, wave = threadIdx.x >> 6;
+  const Span w(a.lengths, b);
+  const int32_t j0 = tile * 16, j = j0 + t, last = min(j0 + 15, w.length - 1);
+  const size_t key = ((size_t)b * S::KEYS + min(j, static_cast<int32_t>(S::KEYS) - 1)) * S::HK + hk;
+  const float scale = static_cast<float>(S::scale() * 1.4426950408889634);
+  f4 kf[G], vf[G], dka[G], dva[G];
+  window_along<S>(kf, a.k + key * S::DH, j < w.length);
+  window_along<S>(vf, a.v + key * S::DH, j < w.length);
+#pragma unroll
+  for (int g = 0; g < G; ++g) dka[g] = dva[g] = f4{0.f, 0.f, 0.f, 0.f};
+  // The positions that see one of the keys: from the first key on, up to the last one's window or the sequence's end.
+  int32_t p0 = max(j0, w.first), p1 = w.length - 1;
+  if (S::WINDOW != 0u && j0 >= static_cast<int32_t>(S::SINKS) && p1 - last >= static_cast<int32_t>(S::WINDOW)) p1 = last + static_cast<int32_t>(S::WINDOW) - 1;
+  p1 = min(p1, w.first + static_cast<int32_t>(S::T) - 1);
+  const int32_t begin = p0 <= p1 && j0 < w.length ? (p0 - w.first) * R / 16 : 0, end = p0 <= p1 && j0 < w.length ? ((p1 - w.first + 1) * R + 15) / 16 : 0;
+  const size_t top = ((size_t)b * S::T) * S::H + hk * R;
+  auto line = [&](int32_t r) { return top + (size_t)(r / R) * S::H + r % R; };
+  for (int32_t i = begin + wave; i < end; i += 4) {
+    const int32_t r0 = i * 16;
+    f4 x[G];
+    const bool on = r0 + t < ROWS && w.stands(w.first + (r0 + t) / R);
+    const size_t mine = line(min(r0 + t, ROWS - 1));
+    window_along<S>(x, a.q + mine * S::DH, on);
+    f4 s = window_scores(x, kf);
+    f4 dp;
+    if constexpr (DK) {
+      window_along<S>(x, a.dy + mine * S::DH, on);
+      dp = window_scores(x, vf);
+    }
+    // Rows 4q ... of this lane.
+    size_t at[4];
+    bool in[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int32_t row = r0 + 4 * q + r;
+      at[r] = line(min(row, ROWS - 1));
+      const int32_t p = w.first + row / R;
+      in[r] = row < ROWS && p >= p0 && p <= p1;
+      s[r] = in[r] && j < w.length && w.sees(p, j) ? __builtin_amdgcn_exp2f(fmaf(s[r], scale, -LOG2E * a.lse[at[r]])) : 0.f;
+    }
+    if constexpr (DV) {
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[g][r] = in[r] && 16 * g + t < static_cast<int>(S::DH) ? a.dy[at[r] * S::DH + 16 * g + t] : 0.f;
+      }
+      window_sum(dva, x, s);
+    }
+    if constexpr (DK) {
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[g][r] = in[r] && 16 * g + t < static_cast<int>(S::DH) ? a.q[at[r] * S::DH + 16 * g + t] : 0.f;
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s[r] = s[r] != 0.f ? s[r] * (dp[r] - a.mass[at[r]]) : 0.f;
+      window_sum(dka, x, s);
+    }
+  }
+  if constexpr (DK) {
+    window_gather(dka, static_cast<float>(S::scale()), lds);
+    if (wave == 0 && j < static_cast<int32_t>(S::KEYS)) {
+#pragma unroll
+      for (int g = 0; g < G; ++g) window_store<S>(dk + key * S::DH, 16 * g + 4 * q, dka[g]);
+    }
+  }
+  if constexpr (DV) {
+    window_gather(dva, 1.f, lds);
+    if (wave == 0 && j < static_cast<int32_t>(S::KEYS)) {
+#pragma unroll
+      for (int g = 0; g < G; ++g) window_store<S>(dv + key * S::DH, 16 * g + 4 * q, dva[g]);
+    }
+  }
+}
+
+}  // namespace tcmi

@@ -265,15 +265,16 @@ function precompileGroup(group, arch, shard, shards) {
   }
   if (group === 'operators') {
     // The operators' GPU tests, in both lowerings, and the sizes they are measured at.
-    const { operatorGraph, CASES, FORMS, MEASURED } = require('../src/testing/operator_cases');
+    const { operatorGraph, CASES, FORMS, MEASURED, CONTEXT, MEASURED_CONTEXT } = require('../src/testing/operator_cases');
+    const timed = MEASURED.concat(MEASURED_CONTEXT);
     let n = 0;
-    for (const [k, c] of CASES.concat(FORMS, MEASURED).entries()) {
+    for (const [k, c] of CASES.concat(FORMS, CONTEXT, timed).entries()) {
       if (k % (shards || 1) !== (shard || 0)) continue;
       const { graph, keep } = operatorGraph(c);
       const f = fuse(graph, { keep });
       const { tuning } = c;
       const lists = [lowerMI355X(f.graph, { perf: true, keep: keep.map((id) => f.index.get(id)), tuning })];
-      n += precompile(MEASURED.includes(c) ? lists : lists.concat([lowerMI355X(f.graph, { tuning })]), arch);
+      n += precompile(timed.includes(c) ? lists : lists.concat([lowerMI355X(f.graph, { tuning })]), arch);
     }
     // The training steps that run them together, as the trainer's tests do.
     const { modelStep } = require('../src/builders/models');
@@ -1276,9 +1277,10 @@ async function main() {
       break;
     }
     case 'operator-graphs': {
-      // The operators' test graphs: the named cases, those of `forms` by name, or cases given whole.
-      const { operatorGraph, CASES, FORMS } = require('../src/testing/operator_cases');
-      const cases = req.cases || (req.forms ? FORMS.filter((c) => req.forms.includes(c.name)) : CASES.filter((c) => !req.family || c.family === req.family));
+      // The operators' test graphs: the named cases (`context`: those of the operators for long contexts and large
+      // vocabularies), those of `forms` by name, or cases given whole.
+      const { operatorGraph, CASES, FORMS, CONTEXT } = require('../src/testing/operator_cases');
+      const cases = req.cases || (req.forms ? FORMS.filter((c) => req.forms.includes(c.name)) : (req.context ? CONTEXT : CASES).filter((c) => !req.family || c.family === req.family));
       out = cases.map((c) => {
         const { graph, keep, names } = operatorGraph(c);
         const f = fuse(graph, { keep });
@@ -1340,6 +1342,55 @@ async function main() {
       for (const k of Object.keys(tries)) {
         try { tries[k](new Graph()); } catch (e) { out[k] = e.message; }
       }
+      break;
+    }
+    case 'context-refusals': {
+      const { grad } = require('../src/autodiff');
+      const qkv = (g, more) => ['q', 'k', 'v'].map((n) => g.input(n, (more || {})[n] || [1, 4, 2, 8]));
+      const residual = (g, more) => g.residualNorm(g.input('x', [4, 8]), g.input('y', [4, 8]), more(g));
+      const twice = (g, out, x) => { const G = grad(g, [out], [x]); return grad(G.graph, [G.grads[0]], [x], { prefix: 'e' }); };
+      const tries = {
+        table: (g) => g.embedding(g.input('t', [3]), g.input('w', [4, 4, 4])),
+        branch: (g) => g.residualNorm(g.input('x', [4, 8]), g.input('y', [4, 9])),
+        gain: (g) => residual(g, () => ({ gain: g.input('g', [7]) })),
+        gate: (g) => residual(g, () => ({ gate: g.input('g', [4, 1]) })),
+        values: (g) => g.windowAttention(...qkv(g, { v: [1, 5, 2, 8] })),
+        lengths: (g) => g.windowAttention(...qkv(g), { lengths: g.input('l', [2]) }),
+        lse: (g) => { const [q, k, v] = qkv(g); return grad(g, [g.windowAttention(q, k, v) - 1], [q]); },
+        'embedding twice': (g) => {
+          const w = g.input('w', [4, 4]);
+          const G = grad(g, [g.embedding(g.input('t', [3]), w)], [w]);
+          return grad(G.graph, [G.grads[0]], [G.graph.inputId('d0')], { prefix: 'e' });
+        },
+        'residual twice': (g) => { const x = g.input('x', [4, 8]); return twice(g, g.residualNorm(x, g.input('y', [4, 8]), { gain: g.input('g', [8]) }).n, x); },
+        'window twice': (g) => { const [q, k, v] = qkv(g); return twice(g, g.windowAttention(q, k, v), q); },
+        'residual part': (g) => g.emit('residualNorm', [g.input('x', [4, 8]), g.input('y', [4, 8])], { norm: 'rms', eps: 0, residual: 1, part: 'n' }),
+        'residual grad part': (g) => g.emit('residualNormGrad', [g.input('x', [4, 8]), g.input('y', [4, 8]), g.input('d', [4, 8])],
+          { norm: 'rms', eps: 0, residual: 1, has: ['dh'], part: 'dgain' }),
+        'window part': (g) => g.emit('windowAttention', qkv(g), { window: 0, sinks: 0, scale: 1, queries: 'last', part: 'p' }),
+        'window grad part': (g) => { const a = qkv(g); return g.emit('windowAttentionGrad', a.concat([a[0], g.input('l', [1, 4, 2]), a[0]]), { window: 0, sinks: 0, scale: 1, queries: 'last', part: 'dp' }); },
+      };
+      out = {};
+      for (const k of Object.keys(tries)) {
+        try { tries[k](new Graph()); } catch (e) { out[k] = e.message; }
+      }
+      break;
+    }
+    case 'residual-adjoints': {
+      // Which cotangents a residualNorm's gradient reads: of h with other readers beside n, of n alone, of h alone.
+      const { grad } = require('../src/autodiff');
+      const build = (outs, wrt) => {
+        const g = new Graph(), x = g.input('x', [4, 8]), gain = g.input('gain', [8]);
+        const r = g.residualNorm(x, g.input('y', [4, 8]), { gain });
+        const other = g.mul(r.h, r.h), all = { h: r.h, n: r.n, other, x, gain };
+        const G = grad(g, outs.map((k) => all[k]), wrt.map((k) => all[k]));
+        const grads = G.graph.nodes.filter((n) => n.op === 'residualNormGrad');
+        return { G, r, has: grads[0] && grads[0].attrs.has, grads: grads.length };
+      };
+      const both = build(['n', 'other'], ['x', 'gain']), n = build(['n'], ['x']), h = build(['other'], ['x']), asked = build(['n', 'other'], ['h', 'x']);
+      const adjoint = asked.G.graph.nodes[asked.G.grads[0]];
+      out = { both: { has: both.has, grads: both.grads }, n: { has: n.has }, h: { has: h.has },
+        asked: { h: adjoint.op === 'add' ? 'the sum of its readers\' shares' : adjoint.op } };
       break;
     }
     case 'kernel-unit': {

@@ -44,9 +44,17 @@ function unbroadcast(B, g, from, to) {
   return B.reshape(acc, from);
 }
 
+/** Node `id` of B if it is part `part` of the operator that node `n` is a part of; else null. */
+function sibling(B, n, id, part) {
+  const m = B.nodes[id];
+  const rest = (x) => JSON.stringify(Object.assign({}, x.attrs, { part: '' }), Object.keys(n.attrs).sort());
+  return m && m.op === n.op && m.attrs.part === part && m.inputs.join() === n.inputs.join() && rest(m) === rest(n) ? id : null;
+}
+
 /**
- * Adjoint rules: rule(B, node, g) returns, per operand of the forward `node`, the id
- * of its share of the adjoint `g` (built into B), or null where there is none. The
+ * Adjoint rules: rule(B, node, g, adjoint, done) returns, per operand of the forward `node`, the id
+ * of its share of the adjoint `g` (built into B), or null where there is none; `adjoint` holds every node's so far,
+ * `done` the nodes that a rule pushed along with its own. The
  * order of the builder calls inside each rule is part of the contract (see above).
  */
 const RULES = {
@@ -111,6 +119,27 @@ const RULES = {
   orthogonalize: () => {
     throw new GradientError('orthogonalize is not differentiable here: it is an optimizer\'s operator, applied to finished gradients');
   },
+  embedding: (B, n, g) => [null, B.emit('embeddingGrad', [n.inputs[0], g], Object.assign({ rows: B.shape(n.inputs[1])[0] }, n.attrs))],
+  // h and n of one residualNorm stand side by side, so h's adjoint is whole when n is visited: one
+  // gradient for both.
+  residualNorm: (B, n, g, adjoint, done) => {
+    const a = n.attrs, both = a.part === 'n' ? sibling(B, n, n.id - 1, 'h') : null;
+    const dh = a.part === 'h' ? g : both === null ? null : adjoint[both], dn = a.part === 'n' ? g : null;
+    if (both !== null) done.add(both);
+    const named = ['gain', 'bias', 'postGain', 'postBias', 'gate'].filter((k) => (k === 'gain' ? a.pre : k === 'postGain' ? a.post : a[k]));
+    const at = (k) => n.inputs[2 + named.indexOf(k)];
+    const operands = n.inputs.slice(0, 2).concat(named.filter((k) => k !== 'bias').map(at));
+    const has = [dh !== null && 'dh', dn !== null && 'dn'].filter(Boolean);
+    const part = (p) => B.emit('residualNormGrad', operands.concat([dh, dn].filter((x) => x !== null)), Object.assign({}, a, { has, part: p }));
+    return [part('dx'), part('dy')].concat(named.map((k) => (dn === null && (k === 'gain' || k === 'bias') ? null : part(`d${k}`))));
+  },
+  windowAttention: (B, n, g) => {
+    if (n.attrs.part !== 'o') throw new GradientError('windowAttention: the logarithm of the sums is not differentiable here');
+    let lse = sibling(B, n, n.id - 1, 'lse');
+    if (lse === null) lse = B.emit('windowAttention', n.inputs, Object.assign({}, n.attrs, { part: 'lse' }));
+    const part = (p) => B.emit('windowAttentionGrad', n.inputs.concat([n.id, lse, g]), Object.assign({}, n.attrs, { part: p }));
+    return [part('dq'), part('dk'), part('dv'), null];
+  },
   step: () => [null],
   stopGradient: () => [null],
   max: () => {
@@ -150,6 +179,7 @@ function grad(graph, outputs, wrt, options) {
     }
     adjoint[id] = adjoint[id] === null ? share : B.add(adjoint[id], share);
   };
+  const done = new Set();
   const cotangents = outputs.map((id, k) => {
     const name = `${prefix}${k}`;
     addShare(id, B.input(name, graph.nodes[id].shape));
@@ -157,10 +187,10 @@ function grad(graph, outputs, wrt, options) {
   });
   for (let id = graph.nodes.length - 1; id >= 0; id--) {
     const node = graph.nodes[id];
-    if (adjoint[id] === null || !live[id] || !node.inputs.some((i) => live[i])) continue;
+    if (adjoint[id] === null || done.has(id) || !live[id] || !node.inputs.some((i) => live[i])) continue;
     const rule = rules[node.op];
     if (!rule) throw new GradientError(`no adjoint rule for op '${node.op}'`);
-    const shares = rule(B, node, adjoint[id]);
+    const shares = rule(B, node, adjoint[id], adjoint, done);
     node.inputs.forEach((operand, k) => {
       if (shares[k] !== null && live[operand]) addShare(operand, shares[k]);
     });

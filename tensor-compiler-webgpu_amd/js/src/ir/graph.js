@@ -171,6 +171,42 @@ class Graph {
       coefficients: (o.coefficients || [3.4445, -4.7750, 2.0315]).slice(), eps: o.eps === undefined ? 1e-7 : o.eps });
   }
 
+  /** Rows of `table` [rows, d] by token, times options.scale (1); zeros where a token is no row's index (padding: -1). */
+  embedding(tokens, table, options) {
+    const { scale } = options || {};
+    return this.emit('embedding', [tokens, table], { scale: scale === undefined ? 1 : scale });
+  }
+
+  /**
+   * { h, n }: h = residual·x + gate·N(y), and n = N(h) where there is a `gain` (operators.js residualNorm). Options: gain, bias (of
+   * n), postGain, postBias (of y's norm; none: y as it is), gate ([d] or x's shape), residual (1), norm ('rms' or 'layer';
+   * default 'layer' where there is a bias), eps (1e-5).
+   */
+  residualNorm(x, y, options) {
+    const o = options || {}, given = (k) => o[k] !== undefined && o[k] !== null;
+    const inputs = [x, y];
+    for (const k of ['gain', 'bias', 'postGain', 'postBias', 'gate']) if (given(k)) inputs.push(o[k]);
+    const attrs = { norm: o.norm || (given('bias') || given('postBias') ? 'layer' : 'rms'), eps: o.eps === undefined ? 1e-5 : o.eps,
+      residual: o.residual === undefined ? 1 : o.residual, pre: given('gain'), bias: given('bias'), post: given('postGain'), postBias: given('postBias'), gate: given('gate') };
+    const h = this.emit('residualNorm', inputs, Object.assign({ part: 'h' }, attrs));
+    return attrs.pre ? { h, n: this.emit('residualNorm', inputs, Object.assign({ part: 'n' }, attrs)) } : { h };
+  }
+
+  /**
+   * Softmax attention of q [B, T, H, dh] over k and v [B, S, Hk, dh], each query seeing the keys up to its own position, the last
+   * `window` of them (default: all) and the first `sinks` (0). Options: scale (1/sqrt(dh)), lengths [B] (each sequence's
+   * keys; the rest of k and v is not read), queries: their positions, 'last' (the default: the sequence's last T) or 'first' (0 ... T-1).
+   */
+  windowAttention(q, k, v, options) {
+    const o = options || {}, given = (x) => x !== undefined && x !== null;
+    const inputs = given(o.lengths) ? [q, k, v, o.lengths] : [q, k, v], dh = this.shape(q)[this.shape(q).length - 1];
+    if (given(o.window) && !(o.window >= 1)) throw new ShapeError(`windowAttention: a window of ${o.window}`);
+    const attrs = { window: given(o.window) ? o.window : 0, sinks: o.sinks === undefined ? 0 : o.sinks,
+      scale: o.scale === undefined ? 1 / Math.sqrt(dh) : o.scale, queries: o.queries || 'last' };
+    this.emit('windowAttention', inputs, Object.assign({ part: 'lse' }, attrs));      // for the gradient (autodiff.js)
+    return this.emit('windowAttention', inputs, Object.assign({ part: 'o' }, attrs));
+  }
+
   // ---- composites ---------------------------------------------------------------
 
   /** x minus its gradient-free maximum along `axis` (graph.js:133-136). */

@@ -18,6 +18,22 @@
 // orthogonalize     [x] -> x's shape: each matrix of the last two axes divided by its
 //   Frobenius norm plus eps, then `steps` times X <- a·X + (b·A + c·A·A)·X, A = X·Xᵀ (on the
 //   side of fewer rows). An optimizer's operator: it has no gradient.
+// embedding         [tokens, table] -> tokens' shape and the table's columns: scale · table[token],
+//   zeros where the token is not a whole number in 0..rows-1 (padding: -1).
+// embeddingGrad     [tokens, dy], attrs.rows the table's rows -> [rows, d]: each row scale times the
+//   sum of its tokens' rows of dy.
+// residualNorm      [x, y, (gain, (bias,)) (postGain, (postBias,)) (gate)], attrs.part 'h' | 'n'. Rows of the last
+//   axis: h = residual·x + gate·N(y), n = N(h). N(v) = (v - mean) / sqrt(mean of (v - mean)² + eps)·gain + bias for norm
+//   'layer', v / sqrt(mean of v² + eps)·gain for 'rms'; of y it is there with a postGain (else N(y) = y), of h with a gain.
+//   A gate of [d] or of x's shape. Which operands there are: attrs.pre, bias, post, postBias, gate.
+// residualNormGrad  [x, y, (gain,) (postGain, (postBias,)) (gate,) (dh,) (dn)], attrs.has names the last two; attrs.part
+//   'dx' | 'dy' | 'dgain' | 'dbias' | 'dpostGain' | 'dpostBias' | 'dgate'.
+// windowAttention   [q, k, v] or [q, k, v, lengths]: q [B, T, H, dh], k and v [B, S, Hk, dh] (query heads h·H/Hk ... share key
+//   head h), lengths [B]; attrs.part 'o' (q's shape) or 'lse' [B, T, H], the logarithm of the sums that o was divided by. Sequence
+//   b has its first L = lengths[b] keys (rounded down, within 0..S, NaN as 0; default S). Query t stands at position t
+//   (attrs.queries 'first') or L - T + t ('last') and sees the keys j <= position that are within attrs.window (position - window < j; 0:
+//   all) or among the first attrs.sinks. A query whose position is not in 0..L-1 sees nothing: zeros, and -Infinity in lse.
+// windowAttentionGrad  [q, k, v, (lengths,) o, lse, dy], attrs.part 'dq' | 'dk' | 'dv'.
 
 const isNumber = (v) => typeof v === 'number' && Number.isFinite(v);
 
@@ -83,7 +99,97 @@ function operatorRules(ShapeError, fmt) {
     return [h[0]];
   }
 
+  function embeddingShape([t, table], attrs, op) {
+    need(table.length === 2, `${op}: a table of ${fmt(table)}: [rows, d]`);
+    need(table[0] <= 2 ** 24, `${op}: ${table[0]} rows (a float32 names 2^24)`);
+    need(isNumber(attrs.scale), `${op}: scale ${attrs.scale}`);
+    return t.concat([table[1]]);
+  }
+
+  /** The operands of a residualNorm after x and y, by name; `grad`: those that its gradient reads. */
+  function residualOperands(s, attrs, op, grad) {
+    const names = [attrs.pre && 'gain', attrs.bias && !grad && 'bias', attrs.post && 'postGain', attrs.postBias && 'postBias', attrs.gate && 'gate'].filter(Boolean);
+    const more = grad ? attrs.has : [];
+    const [x, y] = s, d = x[x.length - 1];
+    need(x.length >= 1 && same(x, y), `${op} of ${fmt(x)} and ${fmt(y)}: a stream and a branch of one shape`);
+    need(s.length === 2 + names.length + more.length, `${op}: ${s.length} operands for ${['x', 'y'].concat(names, more).join(', ')}`);
+    need(attrs.norm === 'rms' || attrs.norm === 'layer', `${op}: norms are 'rms' or 'layer', not '${attrs.norm}'`);
+    need(attrs.norm === 'layer' || !(attrs.bias || attrs.postBias), `${op}: a norm by the root mean square has no bias`);
+    need((attrs.pre || !attrs.bias) && (attrs.post || !attrs.postBias), `${op}: a bias without its gain`);
+    need(isNumber(attrs.eps) && attrs.eps >= 0, `${op}: eps ${attrs.eps}`);
+    need(isNumber(attrs.residual), `${op}: a residual scale of ${attrs.residual}`);
+    const at = {};
+    names.forEach((n, k) => {
+      at[n] = s[2 + k];
+      need(same(at[n], [d]) || (n === 'gate' && same(at[n], x)), `${op}: a ${n} of ${fmt(at[n])} for rows of ${d}`);
+    });
+    more.forEach((n, k) => {
+      const g = s[2 + names.length + k];
+      need((n === 'dh' || (n === 'dn' && attrs.pre)) && same(g, x), `${op}: a gradient ${n} of ${fmt(g)} for ${fmt(x)}`);
+    });
+    return at;
+  }
+
+  function windowShape([q, k, v, lengths], attrs, op) {
+    need(q.length === 4 && k.length === 4, `${op} of ${fmt(q)} by ${fmt(k)}: [batch, tokens, heads, head size]`);
+    need(same(k, v), `${op}: keys of ${fmt(k)} and values of ${fmt(v)}`);
+    need(q[0] === k[0] && q[3] === k[3] && q[2] % k[2] === 0, `${op} of ${fmt(q)} by ${fmt(k)}: equal batches and head sizes, and a whole number of query heads to a key head`);
+    if (lengths) need(same(lengths, [q[0]]), `${op}: lengths of ${fmt(lengths)} for ${q[0]} sequences`);
+    const whole = (n) => Number.isInteger(n) && n >= 0 && n < 2 ** 31;
+    need(whole(attrs.window), `${op}: a window of ${attrs.window}`);
+    need(whole(attrs.sinks), `${op}: ${attrs.sinks} sinks`);
+    need(isNumber(attrs.scale), `${op}: scale ${attrs.scale}`);
+    need(attrs.queries === 'first' || attrs.queries === 'last', `${op}: queries are the 'first' or the 'last', not '${attrs.queries}'`);
+    return { o: q.slice(), lse: q.slice(0, 3) };
+  }
+
   return {
+    embedding: { arity: [2, 2], rule: embeddingShape },
+    embeddingGrad: {
+      arity: [2, 2],
+      rule([t, dy], attrs, op) {
+        const d = dy[dy.length - 1];
+        need(Number.isInteger(attrs.rows) && attrs.rows >= 1, `${op}: ${attrs.rows} rows`);
+        need(same(dy, embeddingShape([t, [attrs.rows, d]], attrs, op)), `${op}: a gradient of ${fmt(dy)} for tokens of ${fmt(t)}`);
+        return [attrs.rows, d];
+      },
+    },
+    residualNorm: {
+      arity: [2, 7],
+      rule(s, attrs, op) {
+        residualOperands(s, attrs, op, false);
+        need(attrs.part === 'h' || (attrs.part === 'n' && attrs.pre), `${op}: no part '${attrs.part}'`);
+        return s[0].slice();
+      },
+    },
+    residualNormGrad: {
+      arity: [3, 8],
+      rule(s, attrs, op) {
+        need(Array.isArray(attrs.has) && attrs.has.length >= 1 && attrs.has.length <= 2 && new Set(attrs.has).size === attrs.has.length, `${op}: gradients ${JSON.stringify(attrs.has)}`);
+        const at = residualOperands(s, attrs, op, true), dn = attrs.has.includes('dn');
+        const part = { dx: s[0], dy: s[1], dgain: dn ? at.gain : undefined, dbias: dn && attrs.bias ? at.gain : undefined, dpostGain: at.postGain, dpostBias: at.postBias, dgate: at.gate }[attrs.part];
+        need(part, `${op}: no part '${attrs.part}'`);
+        return part.slice();
+      },
+    },
+    windowAttention: {
+      arity: [3, 4],
+      rule(s, attrs, op) {
+        const part = windowShape(s, attrs, op)[attrs.part];
+        need(part, `${op}: no part '${attrs.part}'`);
+        return part;
+      },
+    },
+    windowAttentionGrad: {
+      arity: [6, 7],
+      rule(s, attrs, op) {
+        const to = windowShape(s.slice(0, -3), attrs, op), [o, lse, dy] = s.slice(-3);
+        need(same(o, to.o) && same(lse, to.lse) && same(dy, to.o), `${op}: ${fmt(o)}, ${fmt(lse)} and a gradient of ${fmt(dy)} for queries of ${fmt(s[0])}`);
+        const part = { dq: s[0], dk: s[1], dv: s[2] }[attrs.part];
+        need(part, `${op}: no part '${attrs.part}'`);
+        return part.slice();
+      },
+    },
     rotary: { arity: [2, 3], rule: rotaryShape },
     rotaryGrad: {
       arity: [3, 4],

@@ -1,0 +1,90 @@
+'use strict';
+// Launches of embedding and its gradient (tcmi_embedding.h).
+
+const { size } = require('../ir/shapes');
+const { ceil, align, double, constants, kernel } = require('./operator_parts');
+
+// Tokens at most: they are counted in 32 bits, and a column of 16 threads a token in a grid.
+const MOST_TOKENS = 2 ** 28;
+const S = '__KERNEL___s';
+
+function make(z, scale, types) {
+  return (kind, grid, threads, lds, call) => kernel(kind, `#include "tcmi_embedding.h"
+struct ${S} {
+${constants(z, types)}
+  static __device__ __forceinline__ float scale() { return static_cast<float>(${double(scale)}); }
+};
+extern "C" __global__ void __launch_bounds__(${threads}) __KERNEL__(const TcmiArgs A) {
+${lds ? `  __shared__ __attribute__((aligned(16))) ${lds};\n` : ''}  tcmi::${call};
+}
+`, grid, threads);
+}
+
+/** Lanes of a row of d floats, each with E of them, and blocks of columns that those lanes take at a time. */
+function rowLanes(d) {
+  const E = d % 4 === 0 ? 4 : 1, groups = d / E;
+  let lanes = 1;
+  while (lanes < 64 && lanes < groups) lanes *= 2;
+  return { E, lanes, columns: ceil(groups, lanes) };
+}
+
+function lowerEmbedding(graph, node) {
+  const [V, D] = graph.nodes[node.inputs[1]].shape, N = size(graph.nodes[node.inputs[0]].shape);
+  if (N > MOST_TOKENS) throw new Error(`embedding: ${N} tokens (at most ${MOST_TOKENS})`);
+  const { E, lanes, columns } = rowLanes(D);
+  // A lane takes up to four groups of a row; more of them are other workgroups'.
+  const z = { N, V, D, E, LANES: lanes, UNITS: Math.min(4, columns) };
+  const blocks = ceil(columns, z.UNITS);
+  if (N * lanes >= 2 ** 32) throw new Error(`embedding: ${N} tokens of ${D} floats (a grid has 2^32 threads, ${lanes} a token)`);
+  if (blocks > 65535) throw new Error(`embedding: rows of ${D} floats (at most ${65535 * 64 * 4 * E})`);
+  const k = make(z, node.attrs.scale)('emb', [ceil(N, 256 / lanes), blocks, 1], 256, null,
+    `embed<${S}>(A.in[0], A.in[1], A.out, blockIdx.x * (256u / ${S}::LANES) + threadIdx.x / ${S}::LANES, blockIdx.y)`);
+  return { kind: 'embedding', kernels: [k], workspace: 0 };
+}
+
+// Keys of a sort that its workgroups count for themselves; beyond, a launch before each pass counts each tile once.
+const COUNTED = 16384;
+
+function lowerEmbeddingGrad(graph, node) {
+  const N = size(graph.nodes[node.inputs[0]].shape), [V, D] = node.shape;
+  if (N > MOST_TOKENS) throw new Error(`embedding: ${N} tokens (at most ${MOST_TOKENS})`);
+  const { E, lanes, columns } = rowLanes(D);
+  if (columns > 65535) throw new Error(`embedding: rows of ${D} floats (at most ${65535 * 64 * E})`);
+  // Digits of at most nine bits of the token; a tile of keys a workgroup, at most 128 of them.
+  const bits = Math.max(1, Math.ceil(Math.log2(V))), passes = ceil(bits, 9), BITS = ceil(bits, passes);
+  const TILE = Math.max(1024, align(ceil(N, 128), 256)), TILES = ceil(N, TILE), self = N <= COUNTED;
+  // Keys of a sum: few enough that 4096 wavefronts walk them.
+  const waves = N * columns * lanes / 64;
+  let CH = 8;
+  while (CH < 64 && waves / CH > 4096) CH *= 2;
+  const CHUNKS = ceil(N, CH), split = CHUNKS > 1;
+  // Rows of the table that a workgroup looks for: a wavefront's worth where there are enough of them.
+  const ROWS = Math.max(4, Math.min(64, ceil(V, 2048)));
+  const z = { N, V, D, E, LANES: lanes, BITS, TILE, TILES, CH, CHUNKS, ROWS, SELF: self };
+  const types = { SELF: 'bool' };
+  let at = 0;
+  const place = (name, bytes) => { z[name] = at; types[name] = 'size_t'; at = align(at + bytes, 256); };
+  place('COUNT', 256);
+  place('HIST', self ? 0 : 4 * TILES * 2 ** BITS);
+  for (const i of [0, 1]) {
+    const used = i < passes;
+    place(`KEYS${i}`, used ? 4 * N : 0);
+    place(`PLACES${i}`, used ? 4 * N : 0);
+  }
+  place('PARTS', split ? 8 * CHUNKS * D : 0);
+  const m = make(z, node.attrs.scale, types);
+  const kernels = [];
+  for (let p = 0; p < passes; p++) {
+    const ws = 'reinterpret_cast<char*>(A.ws)';
+    if (!self) kernels.push(m('embcount', [TILES, 1, 1], 256, `uint32_t lds[${2 ** BITS}]`, `embed_count<${S}, ${p}>(A.in[0], ${ws}, lds, blockIdx.x)`));
+    kernels.push(m('embsort', [TILES, 1, 1], 256, `uint32_t lds[${6 * 2 ** BITS + 4}]`, `embed_sort<${S}, ${p}>(A.in[0], ${ws}, lds, blockIdx.x)`));
+  }
+  const last = (passes - 1) % 2, sums = ceil(CHUNKS, 256 / lanes) * columns, rows = ceil(V, ROWS);
+  kernels.push(m('embsums', [sums + rows, 1, 1], 256, `uint32_t lds[${ROWS}]`, `embed_sums<${S}, ${last}>(A.in[1], A.out, reinterpret_cast<char*>(A.ws), lds, blockIdx.x)`));
+  if (split) {
+    kernels.push(m('embjoin', [CHUNKS, ceil(D, 64 * E), 1], 512, `float lds[${8 * 64 * E}]`, `embed_join<${S}, ${last}>(A.out, reinterpret_cast<char*>(A.ws), lds, blockIdx.x, blockIdx.y)`));
+  }
+  return { kind: 'embedding-grad', kernels, workspace: at };
+}
+
+module.exports = { lowerEmbedding, lowerEmbeddingGrad };

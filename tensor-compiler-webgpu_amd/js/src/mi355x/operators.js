@@ -1,6 +1,7 @@
 'use strict';
 // Launches of the operators that are one node each (ir/operators.js): the kernels of
-// tcmi_rotary.h, tcmi_loss.h and tcmi_orthogonalize.h, their sizes written as constants of
+// tcmi_rotary.h, tcmi_loss.h and tcmi_orthogonalize.h (embedding.js, residual.js and window.js: of the
+// other operators'), their sizes written as constants of
 // each text, and the workspace they share between the kernels of one launch.
 //
 // A gradient's parts (`dx`, `dgain`; `dh`, `dW`, `dbias`, and with them the losses) are nodes
@@ -10,38 +11,14 @@
 
 const { size } = require('../ir/shapes');
 const { singularBound } = require('../ir/operators');
-const { kernelText, XCD_GROUPED, MAX_BATCH } = require('./codegen');
+const { XCD_GROUPED, MAX_BATCH } = require('./codegen');
+const { ceil, align, double, kernel, entry, joint } = require('./operator_parts');
+const { lowerEmbedding, lowerEmbeddingGrad } = require('./embedding');
+const { lowerResidual } = require('./residual');
+const { lowerWindow } = require('./window');
 
-const ceil = (a, b) => Math.ceil(a / b);
-const OPERATORS = new Set(['rotary', 'rotaryGrad', 'linearCrossEntropy', 'linearCrossEntropyGrad', 'orthogonalize']);
-
-/** A double as a C++ literal that reads back as itself. */
-function double(v) {
-  const t = String(v);
-  return /[.e]/.test(t) ? t : `${t}.0`;
-}
-
-/** One kernel record. */
-function kernel(kind, text, grid, threads, more) {
-  const k = kernelText(kind, text);
-  return Object.assign({ name: k.name, source: k.source, grid, block: [threads, 1, 1], lds: 0 }, more || {});
-}
-
-/**
- * How a kernel's text reaches its launch: alone, `A` (TcmiArgs) with the part's output in
- * A.out; as one of `parts` in a joint launch, member k of its argument block for the k-th part, the
- * operands and the workspace in member 0's. With several `groups` of them (a joint launch of equal nodes), workgroups'
- * z index is the group, its members one after another, its workspace `floats` long.
- */
-function entry(parts, groups, floats) {
-  if (!parts) return { sig: 'const TcmiArgs A', open: '', out: () => 'A.out', ws: 'A.ws' };
-  const n = parts.length;
-  if (groups > 1) {
-    return { sig: `const TcmiBatch<${n * groups}> B`, open: `  const TcmiPtrs* const M = B.m + ${n}u * blockIdx.z;\n  const TcmiPtrs& A = M[0];\n`,
-      out: (part) => `M[${parts.indexOf(part)}].out`, ws: `A.ws + blockIdx.z * (size_t)${floats}u` };
-  }
-  return { sig: `const TcmiBatch<${n}> B`, open: '  const TcmiPtrs& A = B.m[0];\n', out: (part) => `B.m[${parts.indexOf(part)}].out`, ws: 'A.ws' };
-}
+const OPERATORS = new Set(['rotary', 'rotaryGrad', 'linearCrossEntropy', 'linearCrossEntropyGrad', 'orthogonalize', 'embedding', 'embeddingGrad',
+  'residualNorm', 'residualNormGrad', 'windowAttention', 'windowAttentionGrad']);
 
 // ---- rotary -------------------------------------------------------------------------------
 
@@ -174,7 +151,6 @@ function splitK(large, tiles, slices, elements, least) {
 /** A product's kernel keeps two wavefronts a SIMD, 256 registers each. */
 const bounds = (threads, lds) => (/Tile/.test(lds || '') ? ', 2' : '');
 
-const align = (n, to) => ceil(n, to) * to;
 // Columns of a matrix of pairs at most: an offset among 256 of its rows has 32 bits.
 const PAIR_COLS = 2 ** 22;
 
@@ -517,22 +493,16 @@ ${lds ? `  __shared__ __attribute__((aligned(1024))) ${lds};\n` : ''}  tcmi::${c
   return { kind: 'orthogonalize', kernels, workspace: count * z.PER, flops: count * steps * (3 * s * s * l + s ** 3) };
 }
 
-/**
- * Marks kernel `k` as the first of part `part` of a launch whose parts `build(parts, groups)` forms
- * together, in `order`. They read the same first `operands` operands (default: all). `groups`: whether it forms those
- * parts of several nodes of one key.
- */
-function joint(k, part, order, key, build, operands, groups) {
-  Object.defineProperty(k, 'part', { value: part });
-  Object.defineProperty(k, 'joint', { value: { name: JSON.stringify(key), order, build, operands, groups: !!groups } });
-}
-
 /** The launch of an operator's node: { kind, kernels, params, workspace, flops }. tuning.loss.piece: bytes of a piece's logits. */
 function lowerOperator(graph, node, tuning) {
   let k;
   if (node.op === 'rotary' || node.op === 'rotaryGrad') k = lowerRotary(graph, node);
   else if (node.op === 'linearCrossEntropy' || node.op === 'linearCrossEntropyGrad') k = lowerLoss(graph, node, tuning);
   else if (node.op === 'orthogonalize') k = lowerOrthogonalize(graph, node);
+  else if (node.op === 'embedding') k = lowerEmbedding(graph, node);
+  else if (node.op === 'embeddingGrad') k = lowerEmbeddingGrad(graph, node);
+  else if (node.op === 'residualNorm' || node.op === 'residualNormGrad') k = lowerResidual(graph, node);
+  else if (node.op === 'windowAttention' || node.op === 'windowAttentionGrad') k = lowerWindow(graph, node);
   else throw new Error(`no MI355X lowering for '${node.op}'`);
   return Object.assign({ params: new Uint32Array(0), flops: 0 }, k);
 }

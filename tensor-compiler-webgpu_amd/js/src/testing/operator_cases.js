@@ -6,6 +6,10 @@
 //   { family: 'loss', N, d, V, bias?, gradient?, wrt?, after? }     wrt: 'h', 'W', 'b' (default all); `after`: the
 //       losses' cotangent depends on the losses, so their gradients cannot run beside them
 //   { family: 'orthogonalize', x, count, options, twice }
+//   { family: 'embedding', tokens, V, d, scale?, gradient? }
+//   { family: 'residual', x, options: { norm, residual, eps }, vectors: ['gain', 'bias', ...], gate: 'full'?, keep: 'h' | 'n'?,
+//       gradient?, wrt? }                                                     keep, wrt: default all
+//   { family: 'window', q, k, lengths?, options, gradient?, wrt? }          wrt: 'q', 'k', 'v' (default all)
 
 const { Graph } = require('../ir/graph');
 const { grad } = require('../autodiff');
@@ -39,6 +43,24 @@ function operatorGraph(c) {
       outs.push(c.twice ? g.orthogonalize(y, c.options) : y);
       names.push(`y${k}`);
     }
+  } else if (c.family === 'embedding') {
+    const t = g.input('tokens', c.tokens), table = g.input('table', [c.V, c.d]);
+    outs = [g.embedding(t, table, { scale: c.scale })];
+    names = ['e'];
+    wrt.push(table);
+    grads.push('dtable');
+  } else if (c.family === 'residual') {
+    const x = g.input('x', c.x), y = g.input('y', c.x), all = { x, y };
+    for (const k of c.vectors || []) all[k] = g.input(k, k === 'gate' && c.gate === 'full' ? c.x : c.x.slice(-1));
+    const r = g.residualNorm(x, y, Object.assign({}, all, c.options));
+    names = c.keep ? [c.keep] : Object.keys(r);
+    outs = names.map((k) => r[k]);
+    for (const k of c.wrt || Object.keys(all)) { wrt.push(all[k]); grads.push(`d${k}`); }
+  } else if (c.family === 'window') {
+    const all = { q: g.input('q', c.q), k: g.input('k', c.k), v: g.input('v', c.k) };
+    outs = [g.windowAttention(all.q, all.k, all.v, Object.assign({ lengths: c.lengths ? g.input('lengths', [c.q[0]]) : null }, c.options))];
+    names = ['o'];
+    for (const k of c.wrt || ['q', 'k', 'v']) { wrt.push(all[k]); grads.push(`d${k}`); }
   } else throw new Error(`no operator '${c.family}'`);
   if (!c.gradient) return { graph: g, keep: outs, names };
   const G = grad(g, outs, wrt);
@@ -48,6 +70,76 @@ function operatorGraph(c) {
 const rotary = (name, x, positions, more) => Object.assign({ name, family: 'rotary', x, positions }, more);
 const loss = (name, N, d, V, more) => Object.assign({ name, family: 'loss', N, d, V }, more);
 const orth = (name, x, more) => Object.assign({ name, family: 'orthogonalize', x }, more);
+
+const embedding = (name, tokens, V, d, more) => Object.assign({ name, family: 'embedding', tokens, V, d }, more);
+const residual = (name, x, vectors, options, more) => Object.assign({ name, family: 'residual', x, vectors, options }, more);
+const window = (name, q, k, options, more) => Object.assign({ name, family: 'window', q, k, options }, more);
+
+// Cases of the operators for long contexts and large vocabularies.
+const CONTEXT = [
+  // One row and one token; few; tables of one digit, of two and of three; tokens of several tiles and chunks.
+  embedding('one', [1], 1, 1, { gradient: true }),
+  embedding('token', [3], 50, 64, { scale: 8, gradient: true }),
+  embedding('scalar', [], 7, 12, { gradient: true }),
+  embedding('step', [4, 33], 96, 64, { scale: 0.5, gradient: true }),
+  embedding('odd', [131], 517, 37, { gradient: true }),
+  embedding('same', [700], 1, 20, { scale: -2, gradient: true }),
+  embedding('two', [3001], 2, 260, { gradient: true }),
+  embedding('wide', [65], 513, 1030, { gradient: true }),
+  embedding('narrow', [2000], 300, 3, { gradient: true }),
+  embedding('many', [2500], 70001, 4, { gradient: true }),
+  embedding('most', [300], 300000, 8, { gradient: true }),
+  embedding('counted', [17003], 300, 8, { gradient: true }),
+  embedding('counted-twice', [20480], 1000, 2, { gradient: true }),
+  embedding('values', [9, 5], 11, 24, { scale: 0 }),
+  // Norms of both kinds, with what may stand beside them; rows from one float to the longest; only some results.
+  residual('plain', [5, 64], ['gain'], {}, { gradient: true }),
+  residual('sum', [7, 24], [], { residual: 0.5 }, { gradient: true }),
+  residual('layer', [4, 33, 96], ['gain', 'bias'], {}, { gradient: true }),
+  residual('sandwich', [3, 7, 64], ['gain', 'postGain'], { residual: 0.7 }, { gradient: true }),
+  residual('all', [37, 260], ['gain', 'bias', 'postGain', 'postBias', 'gate'], { residual: 1.5, eps: 1e-3 }, { gradient: true }),
+  residual('full-gate', [19, 130], ['gain', 'bias', 'postGain', 'postBias', 'gate'], { residual: -1 }, { gradient: true, gate: 'full' }),
+  residual('gated', [33, 40], ['gain', 'gate'], {}, { gradient: true }),
+  residual('gate-alone', [33, 41], ['gate'], { residual: 0 }, { gradient: true }),
+  residual('post-alone', [21, 37], ['postGain', 'postBias'], {}, { gradient: true }),
+  residual('layer-gain', [9, 48], ['gain', 'postGain'], { norm: 'layer' }, { gradient: true }),
+  residual('one', [1], ['gain', 'postGain', 'gate'], {}, { gradient: true }),
+  residual('float', [5, 1], ['gain', 'bias'], {}, { gradient: true }),
+  residual('odd', [13, 515], ['gain', 'postGain', 'gate'], {}, { gradient: true }),
+  residual('wide', [70, 1028], ['gain', 'postGain'], {}, { gradient: true }),
+  residual('wider', [6, 4099], ['gain', 'bias', 'postGain', 'postBias', 'gate'], {}, { gradient: true }),
+  residual('longest', [3, 16384], ['gain', 'bias', 'postGain', 'postBias', 'gate'], {}, { gradient: true }),
+  residual('rows', [9001, 20], ['gain', 'postGain', 'gate'], {}, { gradient: true }),
+  residual('only-n', [40, 64], ['gain', 'postGain'], {}, { gradient: true, keep: 'n' }),
+  residual('only-h', [40, 64], ['gain', 'postGain'], {}, { gradient: true, keep: 'h' }),
+  residual('only-dy', [40, 64], ['gain', 'postGain', 'gate'], {}, { gradient: true, wrt: ['y'] }),
+  residual('only-vectors', [40, 64], ['gain', 'postGain', 'gate'], {}, { gradient: true, wrt: ['gate', 'gain'] }),
+  residual('values', [11, 100], ['gain', 'bias', 'postGain', 'gate'], { norm: 'layer' }, {}),
+  // One token and many, over its own keys or a cache; windows and sinks of one key, of a tile's, of all; heads alone and shared;
+  // sequences of their own lengths, some of no key.
+  window('one', [1, 1, 1, 1], [1, 1, 1, 1], {}, { gradient: true }),
+  window('token', [3, 1, 8, 64], [3, 50, 2, 64], { window: 20, sinks: 4 }, { lengths: true, gradient: true }),
+  window('token-all', [5, 1, 4, 32], [5, 700, 4, 32], {}, { lengths: true }),
+  window('token-far', [2, 1, 6, 80], [2, 5003, 2, 80], { window: 4000, sinks: 3 }, { lengths: true }),
+  window('tokens', [3, 5, 6, 24], [3, 90, 2, 24], { window: 7 }, { lengths: true, gradient: true }),
+  window('tokens-beyond', [6, 9, 3, 16], [6, 11, 1, 16], { window: 3, sinks: 1 }, { lengths: true, gradient: true }),
+  window('step', [2, 64, 4, 64], [2, 64, 4, 64], {}, { gradient: true }),
+  window('first', [6, 33, 4, 16], [6, 33, 2, 16], { queries: 'first', window: 9, sinks: 2 }, { lengths: true, gradient: true }),
+  window('self', [2, 40, 2, 32], [2, 40, 1, 32], { window: 1 }, { gradient: true }),
+  window('self-sink', [2, 40, 2, 32], [2, 40, 1, 32], { window: 1, sinks: 1, scale: 0.3 }, { gradient: true }),
+  window('sinks-all', [1, 50, 2, 48], [1, 50, 2, 48], { window: 2, sinks: 50 }, { gradient: true }),
+  window('sinks-tile', [1, 90, 2, 16], [1, 90, 2, 16], { window: 17, sinks: 17 }, { gradient: true }),
+  window('odd', [2, 37, 3, 15], [2, 37, 3, 15], { window: 11, sinks: 2 }, { gradient: true }),
+  window('odd-heads', [1, 21, 15, 9], [1, 21, 3, 9], { window: 30 }, { gradient: true }),
+  window('long', [1, 530, 2, 64], [1, 530, 1, 64], { window: 100, sinks: 5 }, { gradient: true }),
+  window('longer', [1, 700, 3, 128], [1, 700, 1, 128], {}, { gradient: true }),
+  window('wide', [1, 150, 2, 256], [1, 150, 1, 256], { window: 70 }, { gradient: true }),
+  window('late', [2, 70, 4, 96], [2, 300, 2, 96], { window: 120, sinks: 4 }, { gradient: true }),
+  window('more-queries', [2, 20, 2, 32], [2, 7, 2, 32], { queries: 'first' }, { gradient: true }),
+  window('only-q', [2, 64, 4, 32], [2, 64, 2, 32], { window: 20 }, { gradient: true, wrt: ['q'] }),
+  window('only-k', [2, 64, 4, 32], [2, 64, 2, 32], { window: 20 }, { gradient: true, wrt: ['k'] }),
+  window('only-v', [2, 64, 4, 32], [2, 64, 2, 32], { window: 20 }, { gradient: true, wrt: ['v'] }),
+];
 
 const CASES = [
   // One token and many; heads before and after the tokens; one position a token and one a sequence's token.
@@ -184,4 +276,17 @@ const MEASURED = [
   orth(null, [256, 256], { count: 16 }), orth(null, [1300, 777]), orth(null, [4096, 4096], { count: 2 }),
 ];
 
-module.exports = { operatorGraph, CASES, FORMS, MEASURED };
+// The sizes of perf/more_operators.py.
+const e = (N, V, d, gradient) => embedding(null, [N], V, d, { scale: Math.sqrt(d), gradient });
+const n = (N, d, vectors, options, gradient) => residual(null, [N, d], vectors, Object.assign({ eps: 1e-5 }, options), { gradient });
+const w = (B, T, S, H, Hk, dh, options, more) => window(null, [B, T, H, dh], [B, S, Hk, dh], Object.assign({ sinks: 0, queries: T === S ? 'first' : 'last' }, options), more);
+const MEASURED_CONTEXT = [
+  e(32, 32768, 1024, false), e(8192, 96, 256, true), e(32768, 65536, 1024, true),
+  n(32, 1024, ['gain', 'postGain'], { residual: 0.75, norm: 'rms' }, false), n(8192, 256, ['gain', 'bias'], { norm: 'layer' }, true),
+  n(8189, 4095, ['gain', 'postGain', 'gate'], { residual: 0.75, norm: 'rms' }, true),
+  w(32, 1, 4096, 8, 2, 64, { window: 1024, sinks: 4 }, { lengths: true }), w(4, 1, 131072, 8, 2, 64, {}, { lengths: true }),
+  w(64, 128, 128, 4, 4, 64, {}, { gradient: true }), w(3, 1001, 1001, 6, 3, 80, { window: 257, sinks: 3 }, { lengths: true, gradient: true }),
+  w(2, 16384, 16384, 16, 4, 128, { window: 1024, sinks: 4 }, {}), w(1, 8192, 8192, 8, 2, 64, {}, { gradient: true }),
+];
+
+module.exports = { operatorGraph, CASES, FORMS, MEASURED, CONTEXT, MEASURED_CONTEXT };
