@@ -1,0 +1,644 @@
+// Attention over a sliding window (tcmi_window.h's formulas) for many rows, on the bf16 matrix cores: every operand as three
+// bf16 parts, x = x0 + x1 + x2, and every product as the six of a_i·b_j with i + j <= 2, in float32 (what is left
+// out: 2^-24 of a product at most). No operand needs a scale, so a key or value of any size is what it is to the queries that see it and
+// nothing to the others; parts below bf16's least normal number, of values below 2^-102, are lost.
+//
+// A workgroup's four wavefronts take 32 rows each (tcmi_window.h's rows: the queries of the heads that share a key head) and walk
+// the tiles of NB keys that one of the 128 sees. A tile is loaded one ahead into registers, split by the thread that loaded it and
+// kept in LDS as three planes, lines `ld` bytes apart. With lane = 16·q + t of a 16 x 16 x 32 product, whose operands are lines of 32 along the
+// sum (8q ... of line t) and whose result is (lines 4q ... of the first, line t of the second):
+//   scores   first operand K (lines: keys; the sum: dims), second Q: lane (t, q) holds row t, keys 4q ... of each 16;
+//   output   first V transposed (lines: dims; the sum: 32 keys), second P: lane (t, q) gives row t, keys 4q ... of the first 16
+//            and of the second 16 as its eight, as it holds them; V's lines are read in the same order of keys by
+//            ds_read_b64_tr_b16, 4 keys of each lane's dim at a time.
+// K's lines are 16 bytes longer than a row, V's 32: the lanes that meet in a cycle then read all banks.
+// A tile's output is summed from 0 and joined to the rows' by one multiplication and addition with their change of maximum, so an
+// accumulator is rounded once a tile.
+
+#pragma once
+
+#include "tcmi_window.h"
+#include "tcmi_gemm_bf16x3.h"
+
+namespace tcmi {
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+// Eight floats as three parts each.
+struct Parts {
+  bf16x8 p[3];
+};
+__device__ __forceinline__ void window_parts(const f4& a, const f4& b, const Minus& minus, Parts& out) {
+  u4 w[3];
+  float x[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float u = x[2 * i], v = x[2 * i + 1];
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+      const bf16x2 h = bf16_pair(u, v);
+      w[p][i] = __builtin_bit_cast(uint32_t, h);
+      if (p < 2) {
+        u = minus.less_lo(u, h);
+        v = minus.less_hi(v, h);
+      }
+    }
+  }
+#pragma unroll
+  for (int p = 0; p < 3; ++p) out.p[p] = __builtin_bit_cast(bf16x8, w[p]);
+}
+
+// acc += a·b.
+__device__ __forceinline__ void window_mfma(f4& acc, const Parts& a, const Parts& b) {
+  acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[0], b.p[2], acc, 0, 0, 0);
+  acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[2], b.p[0], acc, 0, 0, 0);
+  acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[1], b.p[1], acc, 0, 0, 0);
+  acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[0], b.p[1], acc, 0, 0, 0);
+  acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[1], b.p[0], acc, 0, 0, 0);
+  acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[0], b.p[0], acc, 0, 0, 0);
+}
+
+// A tile of NB lines of DP floats in LDS, `pad` bytes after each line of a plane; 256 threads load and split it.
+template <class S, int NB, int PAD>
+struct WindowTile {
+  static constexpr int DP = (S::DH + 31) / 32 * 32, LD = 2 * DP + PAD, PLANE = NB * LD, BYTES = 3 * PLANE;
+  static constexpr int CHUNKS = NB * DP / 4 / 256;             // of four floats, a thread's
+  static_assert(NB * DP / 4 % 256 == 0, "whole chunks a thread");
+  f4 x[CHUNKS];
+
+  static __device__ __forceinline__ int line(int i) { return (threadIdx.x + i * 256) / (DP / 4); }
+  static __device__ __forceinline__ int dim(int i) { return (threadIdx.x + i * 256) % (DP / 4) * 4; }
+  // f(i, line): where line `line`'s floats are, or nullptr for zeros.
+  template <class F>
+  __device__ __forceinline__ void load(F at) {
+#pragma unroll
+    for (int i = 0; i < CHUNKS; ++i) {
+      const float* p = at(line(i));
+      x[i] = window_load<S>(p, dim(i), p != nullptr);
+    }
+  }
+  __device__ __forceinline__ void store(char* tile, const Minus& minus) const {
+#pragma unroll
+    for (int i = 0; i < CHUNKS; ++i) {
+      float u[4] = {x[i][0], x[i][1], x[i][2], x[i][3]};
+      char* to = tile + line(i) * LD + dim(i) * 2;
+#pragma unroll
+      for (int p = 0; p < 3; ++p) {
+        const bf16x2 a = bf16_pair(u[0], u[1]), b = bf16_pair(u[2], u[3]);
+        *reinterpret_cast<uint2*>(to + p * PLANE) = make_uint2(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b));
+        if (p < 2) {
+          u[0] = minus.less_lo(u[0], a);
+          u[1] = minus.less_hi(u[1], a);
+          u[2] = minus.less_lo(u[2], b);
+          u[3] = minus.less_hi(u[3], b);
+        }
+      }
+    }
+  }
+  // This lane's part of a first operand: lines line0 + t, floats 32·slice + 8q ....
+  static __device__ __forceinline__ void lines(const char* tile, int line0, int slice, Parts& f) {
+    const int t = threadIdx.x & 15, q = (threadIdx.x >> 4) & 3;
+#pragma unroll
+    for (int p = 0; p < 3; ++p) f.p[p] = *reinterpret_cast<const bf16x8*>(tile + p * PLANE + (line0 + t) * LD + slice * 64 + q * 16);
+  }
+  // Transposed: line dim0 + t, the sum over tile lines line0 + 4q ... and line0 + 16 + 4q ....
+  static __device__ __forceinline__ void across(const char* tile, int line0, int dim0, Parts& f) {
+    const int t = threadIdx.x & 15, q = (threadIdx.x >> 4) & 3;
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+      const char* at = tile + p * PLANE + (line0 + 4 * q + (t >> 2)) * LD + dim0 * 2 + (t & 3) * 8;
+      const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at));
+      const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at + 16 * LD));
+      f.p[p] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+  }
+};
+
+// Tiles of `size` keys that rows row0 .. row1 see, as window_keys gives those of 16.
+template <int NB>
+__device__ __forceinline__ WindowTiles window_wider(const WindowTiles& k) {
+  if (k.hi < k.lo) return {0, 0, 0, 0, -1};
+  const int32_t sinks = (k.sinks * 16 + NB - 1) / NB, main = max(k.lo / NB, sinks);
+  return {sinks, main, sinks + k.hi / NB + 1 - main, k.lo, k.hi};
+}
+
+template <class S>
+struct WindowWide {
+  static constexpr int DP = (S::DH + 31) / 32 * 32, SLICES = DP / 32, G = DP / 16;
+  static constexpr int NB = DP <= 64 ? 64 : 32;        // keys of a tile: as many floats whatever the head
+  static constexpr int BLOCKS = NB / 16;
+  static constexpr int HB = DP <= 128 ? 2 : 1;         // blocks of 16 rows of a wavefront: what its registers hold
+  static constexpr uint32_t ROWS = 64 * HB;            // of a workgroup
+  using K = WindowTile<S, NB, 16>;
+  using V = WindowTile<S, NB, 32>;
+  static constexpr int LDS = K::BYTES + V::BYTES;
+};
+
+// The `split`-th of SPLITS runs of n.
+template <class S>
+__device__ __forceinline__ void window_run(int32_t n, uint32_t split, int32_t& begin, int32_t& end) {
+  const int32_t each = (n + static_cast<int32_t>(S::SPLITS) - 1) / static_cast<int32_t>(S::SPLITS);
+  begin = min(n, static_cast<int32_t>(split) * each);
+  end = min(n, begin + each);
+}
+
+// Workgroup: W::ROWS rows of a sequence's key head, a split of the keys they see.
+template <class S>
+__device__ __forceinline__ void window_wide(const float* __restrict__ qp, const float* __restrict__ kp, const float* __restrict__ vp, const float* __restrict__ lengths,
+                                            float* __restrict__ out, float* __restrict__ lse, char* ws, char* lds, uint32_t head, uint32_t tile, uint32_t split) {
+  using W = WindowWide<S>;
+  using Span = WindowSpan<S>;
+  constexpr uint32_t R = Span::R, ROWS = Span::ROWS;
+  constexpr int NB = W::NB, HB = W::HB, BLOCKS = W::BLOCKS, SLICES = W::SLICES, G = W::G;
+  const uint32_t b = head / S::HK, hk = head % S::HK;
+  const int lane = threadIdx.x & 63, t = lane & 15, q = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Span w(lengths, b);
+  const Minus minus;
+  const uint32_t row0 = tile * W::ROWS;
+  const WindowTiles keys = window_keys(w, min(row0, ROWS - 1u), min(row0 + W::ROWS - 1u, ROWS - 1u)), tiles = window_wider<NB>(keys);
+  // The wavefront's rows, scores in powers of two.
+  const uint32_t mine = row0 + 16u * HB * wave;
+  const float scale = static_cast<float>(S::scale() * 1.4426950408889634);
+  size_t line[HB];
+  int32_t pos[HB];
+  bool on[HB];
+  Parts qf[HB][SLICES];
+#pragma unroll
+  for (int i = 0; i < HB; ++i) {
+    const uint32_t row = mine + 16u * i + t, at = min(row, ROWS - 1u);
+    line[i] = ((size_t)b * S::T + at / R) * S::H + hk * R + at % R;
+    pos[i] = w.first + static_cast<int32_t>(at / R);
+    on[i] = row < ROWS && w.stands(pos[i]);
+#pragma unroll
+    for (int s = 0; s < SLICES; ++s) {
+      const f4 x = window_load<S>(qp + line[i] * S::DH, 32 * s + 8 * q, on[i]), y = window_load<S>(qp + line[i] * S::DH, 32 * s + 8 * q + 4, on[i]);
+      window_parts(x * scale, y * scale, minus, qf[i][s]);
+    }
+  }
+  // Positions of the wavefront's first and last row: tiles between them need no look at each pair.
+  const bool full = mine + 16u * HB <= ROWS && w.stands(w.first + static_cast<int32_t>(mine / R)) && w.stands(w.first + static_cast<int32_t>((mine + 16u * HB - 1u) / R));
+  const int32_t p0 = w.first + static_cast<int32_t>(min(mine, ROWS - 1u) / R), p1 = w.first + static_cast<int32_t>(min(mine + 16u * HB - 1u, ROWS - 1u) / R);
+  f4 o[HB][G];
+  float m[HB], l[HB];
+#pragma unroll
+  for (int i = 0; i < HB; ++i) {
+    m[i] = -TCMI_INF;
+    l[i] = 0.f;
+#pragma unroll
+    for (int g = 0; g < G; ++g) o[i][g] = f4{0.f, 0.f, 0.f, 0.f};
+  }
+  const size_t step = (size_t)S::HK * S::DH, base = ((size_t)b * S::KEYS * S::HK + hk) * S::DH;
+  typename W::K kt;
+  typename W::V vt;
+  char *klds = lds, *vlds = lds + W::K::BYTES;
+  auto load = [&](int32_t i) __attribute__((always_inline)) {
+    const int32_t j0 = tiles.at(i) * NB;
+    auto at = [&](const float* p) {
+      return [=, &keys](int line) -> const float* {
+        const int32_t j = j0 + line;
+        return j <= keys.hi && (j >= keys.lo || j < static_cast<int32_t>(S::SINKS)) ? p + base + (size_t)j * step : nullptr;
+      };
+    };
+    kt.load(at(kp));
+    vt.load(at(vp));
+  };
+  int32_t begin, end;
+  window_run<S>(tiles.all, split, begin, end);
+  if (begin < end) load(begin);
+  for (int32_t i = begin; i < end; ++i) {
+    const int32_t j0 = tiles.at(i) * NB;
+    __syncthreads();
+    kt.store(klds, minus);
+    vt.store(vlds, minus);
+    __syncthreads();
+    if (i + 1 < end) load(i + 1);
+    // (What none of the wavefront's rows sees: past its last position, or between its sinks and its windows.)
+    if (j0 > p1 || (j0 + NB <= w.from(p0) && j0 >= static_cast<int32_t>(S::SINKS))) continue;
+    const bool whole = full && j0 + NB - 1 <= p0 && (j0 >= w.from(p1) || j0 + NB <= static_cast<int32_t>(S::SINKS));
+    f4 s[HB][BLOCKS];
+#pragma unroll
+    for (int k = 0; k < BLOCKS; ++k) {
+#pragma unroll
+      for (int h = 0; h < HB; ++h) s[h][k] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int d = 0; d < SLICES; ++d) {
+        Parts f;
+        W::K::lines(klds, 16 * k, d, f);
+#pragma unroll
+        for (int h = 0; h < HB; ++h) window_mfma(s[h][k], f, qf[h][d]);
+      }
+    }
+    if (!whole) {
+#pragma unroll
+      for (int h = 0; h < HB; ++h) {
+#pragma unroll
+        for (int k = 0; k < BLOCKS; ++k) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[h][k][r] = on[h] && w.sees(pos[h], j0 + 16 * k + 4 * q + r) ? s[h][k][r] : -TCMI_INF;
+        }
+      }
+    }
+    float alpha[HB];
+    Parts pf[HB][BLOCKS / 2];
+#pragma unroll
+    for (int h = 0; h < HB; ++h) {
+      float top = -TCMI_INF;
+#pragma unroll
+      for (int k = 0; k < BLOCKS; ++k) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) top = fmaxf(top, s[h][k][r]);
+      }
+      top = fmaxf(m[h], quad16_reduce<true>(top));
+      const float zero = top == -TCMI_INF ? 0.f : top;
+      alpha[h] = __builtin_amdgcn_exp2f(m[h] - zero);
+      m[h] = top;
+      float sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < BLOCKS; ++k) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          s[h][k][r] = __builtin_amdgcn_exp2f(s[h][k][r] - zero);
+          sum += s[h][k][r];
+        }
+      }
+      l[h] = fmaf(l[h], alpha[h], sum);
+#pragma unroll
+      for (int k = 0; k < BLOCKS; k += 2) window_parts(s[h][k], s[h][k + 1], minus, pf[h][k / 2]);
+    }
+#pragma unroll
+    for (int g = 0; g < G; g += 2) {
+      f4 sum[HB][2];
+#pragma unroll
+      for (int h = 0; h < HB; ++h) sum[h][0] = sum[h][1] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < BLOCKS / 2; ++k) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          Parts f;
+          W::V::across(vlds, 32 * k, 16 * (g + e), f);
+#pragma unroll
+          for (int h = 0; h < HB; ++h) window_mfma(sum[h][e], f, pf[h][k]);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int h = 0; h < HB; ++h) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) o[h][g + e][r] = fmaf(o[h][g + e][r], alpha[h], sum[h][e][r]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int h = 0; h < HB; ++h) {
+    const float total = quad16_reduce<false>(l[h]);
+    const bool some = total > 0.f || total != total;
+    const float inv = some ? 1.f / total : 0.f;
+    const uint32_t row = mine + 16u * h + t;
+    if (row >= ROWS) continue;
+    if constexpr (S::SPLITS > 1u) {
+      const size_t place = ((size_t)split * S::B * S::HK + head) * S::TILES * 16u + row;
+#pragma unroll
+      for (int g = 0; g < G; ++g) window_store<S>(reinterpret_cast<float*>(ws + S::OUT) + place * S::DH, 16 * g + 4 * q, o[h][g]);
+      if (q == 0) reinterpret_cast<float2*>(ws + S::STATS)[place] = make_float2(m[h], total);
+      continue;
+    }
+    if (out != nullptr) {
+#pragma unroll
+      for (int g = 0; g < G; ++g) window_store<S>(out + line[h] * S::DH, 16 * g + 4 * q, o[h][g] * inv);
+    }
+    if (lse != nullptr && q == 0) lse[line[h]] = some ? (m[h] + __builtin_amdgcn_logf(total)) * 0.69314718055994531f : -TCMI_INF;
+  }
+}
+
+// Dot products of this lane's rows with a tile's lines: acc[h][k] += lines 16k ... of `tile` by f[h].
+template <class T, int HB, int BLOCKS, int SLICES>
+__device__ __forceinline__ void window_dots(f4 (&acc)[HB][BLOCKS], const char* tile, const Parts (&f)[HB][SLICES]) {
+#pragma unroll
+  for (int k = 0; k < BLOCKS; ++k) {
+#pragma unroll
+    for (int h = 0; h < HB; ++h) acc[h][k] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int d = 0; d < SLICES; ++d) {
+      Parts x;
+      T::lines(tile, 16 * k, d, x);
+#pragma unroll
+      for (int h = 0; h < HB; ++h) window_mfma(acc[h][k], x, f[h][d]);
+    }
+  }
+}
+// acc[h][g] += the sums over a tile's lines of its floats 16g ... times f[h].
+template <class T, int HB, int G, int PAIRS>
+__device__ __forceinline__ void window_sums(f4 (&acc)[HB][G], const char* tile, const Parts (&f)[HB][PAIRS]) {
+#pragma unroll
+  for (int g = 0; g < G; g += 2) {
+    f4 sum[HB][2];
+#pragma unroll
+    for (int h = 0; h < HB; ++h) sum[h][0] = sum[h][1] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < PAIRS; ++k) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        Parts x;
+        T::across(tile, 32 * k, 16 * (g + e), x);
+#pragma unroll
+        for (int h = 0; h < HB; ++h) window_mfma(sum[h][e], x, f[h][k]);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+#pragma unroll
+      for (int h = 0; h < HB; ++h) acc[h][g + e] += sum[h][e];
+    }
+  }
+}
+// A line's parts, as a second operand.
+template <class S, int SLICES>
+__device__ __forceinline__ void window_line(Parts (&f)[SLICES], const float* __restrict__ p, bool on, float scale, const Minus& minus) {
+  const int q = (threadIdx.x >> 4) & 3;
+#pragma unroll
+  for (int s = 0; s < SLICES; ++s) {
+    const f4 x = window_load<S>(p, 32 * s + 8 * q, on), y = window_load<S>(p, 32 * s + 8 * q + 4, on);
+    window_parts(x * scale, y * scale, minus, f[s]);
+  }
+}
+
+// The gradients: tiles of 32 lines, and 32 lines a wavefront's own where its registers hold both of their operands.
+template <class S>
+struct WindowBack {
+  static constexpr int DP = (S::DH + 31) / 32 * 32, SLICES = DP / 32, G = DP / 16, NB = 32, BLOCKS = 2;
+  static constexpr int HB = DP <= 64 ? 2 : 1;
+  static constexpr uint32_t ROWS = 64 * HB;
+  using T = WindowTile<S, NB, 16>;
+  static constexpr int LDS = 2 * T::BYTES + 3 * NB * 4;
+};
+
+// Workgroup: W::ROWS rows of a sequence's key head, a split of the keys they see. parts: the splits' sums, [SPLITS][lines][DH].
+template <class S>
+__device__ __forceinline__ void window_wide_dq(const WindowGradArgs a, float* __restrict__ dq, float* __restrict__ parts, char* lds, uint32_t head, uint32_t tile, uint32_t split) {
+  using W = WindowBack<S>;
+  using T = typename W::T;
+  using Span = WindowSpan<S>;
+  constexpr uint32_t R = Span::R, ROWS = Span::ROWS;
+  constexpr int NB = W::NB, HB = W::HB, BLOCKS = W::BLOCKS, SLICES = W::SLICES, G = W::G;
+  const uint32_t b = head / S::HK, hk = head % S::HK;
+  const int lane = threadIdx.x & 63, t = lane & 15, q = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Span w(a.lengths, b);
+  const Minus minus;
+  const uint32_t row0 = tile * W::ROWS, mine = row0 + 16u * HB * wave;
+  const WindowTiles keys = window_keys(w, min(row0, ROWS - 1u), min(row0 + W::ROWS - 1u, ROWS - 1u)), tiles = window_wider<NB>(keys);
+  const float scale = static_cast<float>(S::scale() * 1.4426950408889634);
+  size_t line[HB];
+  int32_t pos[HB];
+  bool on[HB];
+  float lse[HB], mass[HB];
+  Parts qf[HB][SLICES], df[HB][SLICES];
+  f4 acc[HB][G];
+#pragma unroll
+  for (int h = 0; h < HB; ++h) {
+    const uint32_t row = mine + 16u * h + t, at = min(row, ROWS - 1u);
+    line[h] = ((size_t)b * S::T + at / R) * S::H + hk * R + at % R;
+    pos[h] = w.first + static_cast<int32_t>(at / R);
+    on[h] = row < ROWS && w.stands(pos[h]);
+    window_line<S>(qf[h], a.q + line[h] * S::DH, on[h], scale, minus);
+    window_line<S>(df[h], a.dy + line[h] * S::DH, on[h], 1.f, minus);
+    lse[h] = on[h] ? a.lse[line[h]] * LOG2E : 0.f;
+    mass[h] = on[h] ? a.mass[line[h]] : 0.f;
+#pragma unroll
+    for (int g = 0; g < G; ++g) acc[h][g] = f4{0.f, 0.f, 0.f, 0.f};
+  }
+  const bool full = mine + 16u * HB <= ROWS && w.stands(w.first + static_cast<int32_t>(mine / R)) && w.stands(w.first + static_cast<int32_t>((mine + 16u * HB - 1u) / R));
+  const int32_t p0 = w.first + static_cast<int32_t>(min(mine, ROWS - 1u) / R), p1 = w.first + static_cast<int32_t>(min(mine + 16u * HB - 1u, ROWS - 1u) / R);
+  const size_t step = (size_t)S::HK * S::DH, base = ((size_t)b * S::KEYS * S::HK + hk) * S::DH;
+  T kt, vt;
+  char *klds = lds, *vlds = lds + T::BYTES;
+  auto load = [&](int32_t i) __attribute__((always_inline)) {
+    const int32_t j0 = tiles.at(i) * NB;
+    auto at = [&](const float* p) {
+      return [=, &keys](int line) -> const float* {
+        const int32_t j = j0 + line;
+        return j <= keys.hi && (j >= keys.lo || j < static_cast<int32_t>(S::SINKS)) ? p + base + (size_t)j * step : nullptr;
+      };
+    };
+    kt.load(at(a.k));
+    vt.load(at(a.v));
+  };
+  int32_t begin, end;
+  window_run<S>(tiles.all, split, begin, end);
+  if (begin < end) load(begin);
+  for (int32_t i = begin; i < end; ++i) {
+    const int32_t j0 = tiles.at(i) * NB;
+    __syncthreads();
+    kt.store(klds, minus);
+    vt.store(vlds, minus);
+    __syncthreads();
+    if (i + 1 < end) load(i + 1);
+    if (j0 > p1 || (j0 + NB <= w.from(p0) && j0 >= static_cast<int32_t>(S::SINKS))) continue;
+    const bool whole = full && j0 + NB - 1 <= p0 && (j0 >= w.from(p1) || j0 + NB <= static_cast<int32_t>(S::SINKS));
+    f4 s[HB][BLOCKS], dp[HB][BLOCKS];
+    window_dots<T>(s, klds, qf);
+    window_dots<T>(dp, vlds, df);
+    Parts ds[HB][1];
+#pragma unroll
+    for (int h = 0; h < HB; ++h) {
+#pragma unroll
+      for (int k = 0; k < BLOCKS; ++k) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float d = __builtin_amdgcn_exp2f(s[h][k][r] - lse[h]) * (dp[h][k][r] - mass[h]);
+          s[h][k][r] = whole || (on[h] && w.sees(pos[h], j0 + 16 * k + 4 * q + r)) ? d : 0.f;
+        }
+      }
+      window_parts(s[h][0], s[h][1], minus, ds[h][0]);
+    }
+    window_sums<T>(acc, klds, ds);
+  }
+#pragma unroll
+  for (int h = 0; h < HB; ++h) {
+    if (mine + 16u * h + t >= ROWS) continue;
+    float* to = S::SPLITS > 1u ? parts + ((size_t)split * S::B * S::T * S::H + line[h]) * S::DH : dq + line[h] * S::DH;
+    const float by = S::SPLITS > 1u ? 1.f : static_cast<float>(S::scale());
+#pragma unroll
+    for (int g = 0; g < G; ++g) window_store<S>(to, 16 * g + 4 * q, acc[h][g] * by);
+  }
+}
+
+// Workgroup: W::ROWS keys of a sequence's key head, the `chunk`-th CHUNK tiles of 32 rows of those that see one of them. parts of chunk c: of
+// dk, then of dv, [c][keys][DH] for c < CHUNKS, and for more (keys below SINKS alone have them) the FEW first keys' [c - CHUNKS][B][FEW][HK][DH].
+template <class S, bool DK, bool DV>
+__device__ __forceinline__ void window_wide_dkv(const WindowGradArgs a, float* __restrict__ dk, float* __restrict__ dv, char* ws, char* lds, uint32_t head, uint32_t tile, uint32_t chunk) {
+  using W = WindowBack<S>;
+  using T = typename W::T;
+  using Span = WindowSpan<S>;
+  constexpr int32_t R = Span::R, ROWS = Span::ROWS;
+  constexpr int NB = W::NB, HB = W::HB, BLOCKS = W::BLOCKS, SLICES = W::SLICES, G = W::G;
+  const uint32_t b = head / S::HK, hk = head % S::HK;
+  const int lane = threadIdx.x & 63, t = lane & 15, q = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Span w(a.lengths, b);
+  const Minus minus;
+  const int32_t j0 = tile * W::ROWS, mine = j0 + 16 * HB * wave;
+  const float scale = static_cast<float>(S::scale() * 1.4426950408889634);
+  int32_t key[HB];
+  size_t line[HB];
+  Parts kf[HB][SLICES], vf[HB][SLICES];
+  f4 dka[HB][G], dva[HB][G];
+  // The positions that see one of the keys: from the first key on, up to the last one's window or the sequence's end.
+  auto seen = [&](int32_t first, int32_t keys, int32_t& p0, int32_t& p1) __attribute__((always_inline)) {
+    const int32_t last = min(first + keys, w.length) - 1;
+    p0 = max(first, w.first);
+    p1 = w.length - 1;
+    if (S::WINDOW != 0u && first >= static_cast<int32_t>(S::SINKS) && p1 - last >= static_cast<int32_t>(S::WINDOW)) p1 = last + static_cast<int32_t>(S::WINDOW) - 1;
+    p1 = min(p1, w.first + static_cast<int32_t>(S::T) - 1);
+    if (first >= w.length) p1 = p0 - 1;
+  };
+  int32_t p0, p1, m0, m1;
+  seen(j0, W::ROWS, p0, p1);
+  seen(mine, 16 * HB, m0, m1);
+  int32_t begin = 0, end = 0;
+  if (p0 <= p1) {
+    begin = (p0 - w.first) * R / NB + static_cast<int32_t>(chunk * S::CHUNK);
+    end = min(((p1 - w.first + 1) * R + NB - 1) / NB, begin + static_cast<int32_t>(S::CHUNK));
+  }
+#pragma unroll
+  for (int h = 0; h < HB; ++h) {
+    key[h] = mine + 16 * h + t;
+    line[h] = ((size_t)b * S::KEYS + min(key[h], static_cast<int32_t>(S::KEYS) - 1)) * S::HK + hk;
+    const bool on = begin < end && key[h] < w.length;
+    window_line<S>(kf[h], a.k + line[h] * S::DH, on, scale, minus);
+    if constexpr (DK) window_line<S>(vf[h], a.v + line[h] * S::DH, on, 1.f, minus);
+#pragma unroll
+    for (int g = 0; g < G; ++g) dka[h][g] = dva[h][g] = f4{0.f, 0.f, 0.f, 0.f};
+  }
+  const size_t top = ((size_t)b * S::T) * S::H + hk * R;
+  auto place = [&](int32_t r) { return top + (size_t)(r / R) * S::H + r % R; };
+  T qt, dt;
+  float stats[2];
+  char *qlds = lds, *dlds = lds + T::BYTES;
+  float* const row_lse = reinterpret_cast<float*>(lds + 2 * T::BYTES);
+  float* const row_mass = row_lse + NB;
+  int32_t* const row_pos = reinterpret_cast<int32_t*>(row_mass + NB);
+  int32_t row_at = 0;
+  auto load = [&](int32_t i) __attribute__((always_inline)) {
+    const int32_t r0 = i * NB;
+    auto at = [&](const float* p) {
+      return [=, &place, &w](int l) -> const float* {
+        const int32_t r = r0 + l, pos = w.first + r / R;
+        return r < ROWS && pos >= p0 && pos <= p1 ? p + place(r) * S::DH : nullptr;
+      };
+    };
+    qt.load(at(a.q));
+    dt.load(at(a.dy));
+    if (threadIdx.x < NB) {
+      const int32_t r = r0 + threadIdx.x;
+      row_at = w.first + r / R;
+      const bool on = r < ROWS && row_at >= p0 && row_at <= p1;
+      if (!on) row_at = -1;
+      stats[0] = on ? a.lse[place(r)] * LOG2E : 0.f;
+      stats[1] = on && DK ? a.mass[place(r)] : 0.f;
+    }
+  };
+  if (begin < end) load(begin);
+  for (int32_t i = begin; i < end; ++i) {
+    __syncthreads();
+    qt.store(qlds, minus);
+    dt.store(dlds, minus);
+    if (threadIdx.x < NB) {
+      row_lse[threadIdx.x] = stats[0];
+      row_mass[threadIdx.x] = stats[1];
+      row_pos[threadIdx.x] = row_at;
+    }
+    __syncthreads();
+    if (i + 1 < end) load(i + 1);
+    const int32_t r0 = i * NB, a0 = w.first + r0 / R, a1 = w.first + min(r0 + NB - 1, ROWS - 1) / R;
+    if (m0 > m1 || a1 < m0 || a0 > m1) continue;
+    const bool whole = r0 + NB <= ROWS && a0 >= max(p0, mine + 16 * HB - 1) && a1 <= p1 && (w.from(a1) <= mine || mine + 16 * HB <= static_cast<int32_t>(S::SINKS));
+    f4 s[HB][BLOCKS], dp[HB][BLOCKS];
+    window_dots<T>(s, qlds, kf);
+    if constexpr (DK) window_dots<T>(dp, dlds, vf);
+    Parts pf[HB][1], ds[HB][1];
+#pragma unroll
+    for (int k = 0; k < BLOCKS; ++k) {
+      const f4 ls = *reinterpret_cast<const f4*>(row_lse + 16 * k + 4 * q);
+      const f4 ms = *reinterpret_cast<const f4*>(row_mass + 16 * k + 4 * q);
+      const int4 ps = *reinterpret_cast<const int4*>(row_pos + 16 * k + 4 * q);
+      const int32_t pos[4] = {ps.x, ps.y, ps.z, ps.w};
+#pragma unroll
+      for (int h = 0; h < HB; ++h) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const bool sees = whole || (pos[r] >= 0 && w.sees(pos[r], key[h]));
+          s[h][k][r] = sees ? __builtin_amdgcn_exp2f(s[h][k][r] - ls[r]) : 0.f;
+          if constexpr (DK) dp[h][k][r] = sees ? s[h][k][r] * (dp[h][k][r] - ms[r]) : 0.f;
+        }
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < HB; ++h) {
+      if constexpr (DV) window_parts(s[h][0], s[h][1], minus, pf[h][0]);
+      if constexpr (DK) window_parts(dp[h][0], dp[h][1], minus, ds[h][0]);
+    }
+    if constexpr (DV) window_sums<T>(dva, dlds, pf);
+    if constexpr (DK) window_sums<T>(dka, qlds, ds);
+  }
+#pragma unroll
+  for (int h = 0; h < HB; ++h) {
+    if (key[h] >= static_cast<int32_t>(S::KEYS)) continue;
+    float *tk = dk + line[h] * S::DH, *tv = dv + line[h] * S::DH;
+    float by = static_cast<float>(S::scale());
+    if constexpr (S::CHUNKS_MOST > 1u) {
+      // (Their first CHUNKS as all keys', further ones of the first keys apart.)
+      const size_t few = ((size_t)b * S::FEW + min(key[h], static_cast<int32_t>(S::FEW) - 1)) * S::HK + hk;
+      const size_t at = chunk < S::CHUNKS ? ((size_t)chunk * S::B * S::KEYS * S::HK + line[h]) * S::DH : (size_t)S::CHUNKS * S::B * S::KEYS * S::HK * S::DH + ((size_t)(chunk - S::CHUNKS) * S::B * S::FEW * S::HK + few) * S::DH;
+      if (chunk >= S::CHUNKS && key[h] >= static_cast<int32_t>(S::FEW)) continue;
+      tk = reinterpret_cast<float*>(ws + S::DKPARTS) + at;
+      tv = reinterpret_cast<float*>(ws + S::DVPARTS) + at;
+      by = 1.f;
+    }
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      if constexpr (DK) window_store<S>(tk, 16 * g + 4 * q, dka[h][g] * by);
+      if constexpr (DV) window_store<S>(tv, 16 * g + 4 * q, dva[h][g]);
+    }
+  }
+}
+
+// dq from its splits' sums: thread `at`, four floats.
+template <class S>
+__device__ __forceinline__ void window_wide_add(float* __restrict__ dq, const float* __restrict__ parts, size_t at) {
+  constexpr size_t N = (size_t)S::B * S::T * S::H * S::DH, E = S::VEC ? 4 : 1;
+  if (at * E >= N) return;
+  f4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (uint32_t k = 0; k < S::SPLITS; ++k) {
+    if constexpr (S::VEC) sum += *reinterpret_cast<const f4*>(parts + k * N + at * E);
+    else sum[0] += parts[k * N + at];
+  }
+  sum *= static_cast<float>(S::scale());
+  if constexpr (S::VEC) *reinterpret_cast<f4*>(dq + at * E) = sum;
+  else dq[at] = sum[0];
+}
+// dk (scaled) or dv from their chunks' sums.
+template <class S>
+__device__ __forceinline__ void window_wide_join(float* __restrict__ out, const float* __restrict__ parts, float by, size_t at) {
+  constexpr size_t ROW = (size_t)S::HK * S::DH, N = (size_t)S::B * S::KEYS * ROW, E = S::VEC ? 4 : 1;
+  if (at * E >= N) return;
+  f4 sum = {0.f, 0.f, 0.f, 0.f};
+  auto add = [&](const float* p) __attribute__((always_inline)) {
+    if constexpr (S::VEC) sum += *reinterpret_cast<const f4*>(p);
+    else sum[0] += *p;
+  };
+#pragma unroll 4
+  for (uint32_t k = 0; k < S::CHUNKS; ++k) add(parts + k * N + at * E);
+  const size_t b = at * E / (S::KEYS * ROW), key = at * E / ROW % S::KEYS;
+  if (key < S::FEW) {
+    const float* more = parts + S::CHUNKS * N + ((size_t)b * S::FEW + key) * ROW + at * E % ROW;
+#pragma unroll 4
+    for (uint32_t k = S::CHUNKS; k < S::CHUNKS_MOST; ++k) add(more + (size_t)(k - S::CHUNKS) * S::B * S::FEW * ROW);
+  }
+  sum *= by;
+  if constexpr (S::VEC) *reinterpret_cast<f4*>(out + at * E) = sum;
+  else out[at] = sum[0];
+}
+
+}  // namespace tcmi
