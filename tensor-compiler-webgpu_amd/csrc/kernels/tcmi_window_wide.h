@@ -5,13 +5,12 @@
 //
 // A workgroup's four wavefronts take 32 rows each (tcmi_window.h's rows: the queries of the heads that share a key head) and walk
 // the tiles of NB keys that one of the 128 sees. A tile is loaded one ahead into registers, split by the thread that loaded it and
-// kept in LDS as three planes, lines `ld` bytes apart. With lane = 16·q + t of a 16 x 16 x 32 product, whose operands are lines of 32 along the
+// kept in LDS as three planes. With lane = 16·q + t of a 16 x 16 x 32 product, whose operands are lines of 32 along the
 // sum (8q ... of line t) and whose result is (lines 4q ... of the first, line t of the second):
 //   scores   first operand K (lines: keys; the sum: dims), second Q: lane (t, q) holds row t, keys 4q ... of each 16;
 //   output   first V transposed (lines: dims; the sum: 32 keys), second P: lane (t, q) gives row t, keys 4q ... of the first 16
 //            and of the second 16 as its eight, as it holds them; V's lines are read in the same order of keys by
 //            ds_read_b64_tr_b16, 4 keys of each lane's dim at a time.
-// K's lines are 16 bytes longer than a row, V's 32: the lanes that meet in a cycle then read all banks.
 // A tile's output is summed from 0 and joined to the rows' by one multiplication and addition with their change of maximum, so an
 // accumulator is rounded once a tile.
 
@@ -58,17 +57,23 @@ __device__ __forceinline__ void window_mfma(f4& acc, const Parts& a, const Parts
   acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[0], b.p[0], acc, 0, 0, 0);
 }
 
-// A tile of NB lines of DP floats in LDS, `pad` bytes after each line of a plane; 256 threads load and split it.
-template <class S, int NB, int PAD>
+// A tile of NB lines of DP floats in LDS, three planes of LD bytes a line; 256 threads load and split it. A line's 16-byte chunk c is at
+// place c ^ swap(line), so that the lanes that meet in a cycle of 256 bytes read all banks both ways: 16 lines of one chunk each, and 8
+// lines of two chunks each.
+template <class S, int NB>
 struct WindowTile {
-  static constexpr int DP = (S::DH + 31) / 32 * 32, LD = 2 * DP + PAD, PLANE = NB * LD, BYTES = 3 * PLANE;
+  static constexpr int DP = (S::DH + 31) / 32 * 32, LD = DP <= 32 ? 64 : DP <= 64 ? 128 : DP <= 128 ? 256 : 512, PLANE = NB * LD, BYTES = 3 * PLANE;
   static constexpr int CHUNKS = NB * DP / 4 / 256;             // of four floats, a thread's
   static_assert(NB * DP / 4 % 256 == 0, "whole chunks a thread");
   f4 x[CHUNKS];
 
+  static __device__ __forceinline__ int swap(int line) {
+    const int low = LD == 64 ? (line >> 2) & 1 : LD == 128 ? (line >> 1) & 3 : line & 7;
+    return 2 * low + ((line >> 3) & 1);
+  }
   static __device__ __forceinline__ int line(int i) { return (threadIdx.x + i * 256) / (DP / 4); }
   static __device__ __forceinline__ int dim(int i) { return (threadIdx.x + i * 256) % (DP / 4) * 4; }
-  // f(i, line): where line `line`'s floats are, or nullptr for zeros.
+  // f(line): where line `line`'s floats are, or nullptr for zeros.
   template <class F>
   __device__ __forceinline__ void load(F at) {
 #pragma unroll
@@ -81,7 +86,7 @@ struct WindowTile {
 #pragma unroll
     for (int i = 0; i < CHUNKS; ++i) {
       float u[4] = {x[i][0], x[i][1], x[i][2], x[i][3]};
-      char* to = tile + line(i) * LD + dim(i) * 2;
+      char* to = tile + line(i) * LD + (((dim(i) >> 3) ^ swap(line(i))) << 4) + (dim(i) & 4) * 2;
 #pragma unroll
       for (int p = 0; p < 3; ++p) {
         const bf16x2 a = bf16_pair(u[0], u[1]), b = bf16_pair(u[2], u[3]);
@@ -95,20 +100,21 @@ struct WindowTile {
       }
     }
   }
-  // This lane's part of a first operand: lines line0 + t, floats 32·slice + 8q ....
+  // This lane's part of a first operand: lines line0 + t, floats 32·slice + 8q .... (line0: a multiple of 16)
   static __device__ __forceinline__ void lines(const char* tile, int line0, int slice, Parts& f) {
-    const int t = threadIdx.x & 15, q = (threadIdx.x >> 4) & 3;
+    const int t = threadIdx.x & 15, q = (threadIdx.x >> 4) & 3, at = t * LD + ((q ^ swap(t)) << 4);
 #pragma unroll
-    for (int p = 0; p < 3; ++p) f.p[p] = *reinterpret_cast<const bf16x8*>(tile + p * PLANE + (line0 + t) * LD + slice * 64 + q * 16);
+    for (int p = 0; p < 3; ++p) f.p[p] = *reinterpret_cast<const bf16x8*>(tile + p * PLANE + line0 * LD + (at ^ (slice << 6)));
   }
   // Transposed: line dim0 + t, the sum over tile lines line0 + 4q ... and line0 + 16 + 4q ....
   static __device__ __forceinline__ void across(const char* tile, int line0, int dim0, Parts& f) {
-    const int t = threadIdx.x & 15, q = (threadIdx.x >> 4) & 3;
+    const int t = threadIdx.x & 15, q = (threadIdx.x >> 4) & 3, line = 4 * q + (t >> 2);
+    const int at = (line * LD + ((((t >> 1) & 1) ^ swap(line)) << 4) + (t & 1) * 8) ^ (dim0 << 1);
 #pragma unroll
     for (int p = 0; p < 3; ++p) {
-      const char* at = tile + p * PLANE + (line0 + 4 * q + (t >> 2)) * LD + dim0 * 2 + (t & 3) * 8;
-      const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at));
-      const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at + 16 * LD));
+      const char* from = tile + p * PLANE + line0 * LD + at;
+      const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(from));
+      const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(from + 16 * LD));
       f.p[p] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
     }
   }
@@ -127,11 +133,10 @@ struct WindowWide {
   static constexpr int DP = (S::DH + 31) / 32 * 32, SLICES = DP / 32, G = DP / 16;
   static constexpr int NB = DP <= 64 ? 64 : 32;        // keys of a tile: as many floats whatever the head
   static constexpr int BLOCKS = NB / 16;
-  static constexpr int HB = DP <= 128 ? 2 : 1;         // blocks of 16 rows of a wavefront: what its registers hold
+  static constexpr int HB = S::HB;                     // blocks of 16 rows of a wavefront
   static constexpr uint32_t ROWS = 64 * HB;            // of a workgroup
-  using K = WindowTile<S, NB, 16>;
-  using V = WindowTile<S, NB, 32>;
-  static constexpr int LDS = K::BYTES + V::BYTES;
+  using T = WindowTile<S, NB>;
+  static constexpr int LDS = 2 * T::BYTES;
 };
 
 // The `split`-th of SPLITS runs of n.
@@ -188,33 +193,19 @@ __device__ __forceinline__ void window_wide(const float* __restrict__ qp, const 
     for (int g = 0; g < G; ++g) o[i][g] = f4{0.f, 0.f, 0.f, 0.f};
   }
   const size_t step = (size_t)S::HK * S::DH, base = ((size_t)b * S::KEYS * S::HK + hk) * S::DH;
-  typename W::K kt;
-  typename W::V vt;
-  char *klds = lds, *vlds = lds + W::K::BYTES;
-  auto load = [&](int32_t i) __attribute__((always_inline)) {
+  using T = typename W::T;
+  T x;                                   // K's next tile, or V's: never both at once
+  char *klds = lds, *vlds = lds + T::BYTES;
+  auto load = [&](const float* p, int32_t i) __attribute__((always_inline)) {
     const int32_t j0 = tiles.at(i) * NB;
-    auto at = [&](const float* p) {
-      return [=, &keys](int line) -> const float* {
-        const int32_t j = j0 + line;
-        return j <= keys.hi && (j >= keys.lo || j < static_cast<int32_t>(S::SINKS)) ? p + base + (size_t)j * step : nullptr;
-      };
-    };
-    kt.load(at(kp));
-    vt.load(at(vp));
+    x.load([&](int line) -> const float* {
+      const int32_t j = j0 + line;
+      return j <= keys.hi && (j >= keys.lo || j < static_cast<int32_t>(S::SINKS)) ? p + base + (size_t)j * step : nullptr;
+    });
   };
   int32_t begin, end;
   window_run<S>(tiles.all, split, begin, end);
-  if (begin < end) load(begin);
-  for (int32_t i = begin; i < end; ++i) {
-    const int32_t j0 = tiles.at(i) * NB;
-    __syncthreads();
-    kt.store(klds, minus);
-    vt.store(vlds, minus);
-    __syncthreads();
-    if (i + 1 < end) load(i + 1);
-    // (What none of the wavefront's rows sees: past its last position, or between its sinks and its windows.)
-    if (j0 > p1 || (j0 + NB <= w.from(p0) && j0 >= static_cast<int32_t>(S::SINKS))) continue;
-    const bool whole = full && j0 + NB - 1 <= p0 && (j0 >= w.from(p1) || j0 + NB <= static_cast<int32_t>(S::SINKS));
+  auto scores = [&](int32_t j0, bool whole, float (&alpha)[HB], Parts (&pf)[HB][BLOCKS / 2]) __attribute__((always_inline)) {
     f4 s[HB][BLOCKS];
 #pragma unroll
     for (int k = 0; k < BLOCKS; ++k) {
@@ -223,7 +214,7 @@ __device__ __forceinline__ void window_wide(const float* __restrict__ qp, const 
 #pragma unroll
       for (int d = 0; d < SLICES; ++d) {
         Parts f;
-        W::K::lines(klds, 16 * k, d, f);
+        T::lines(klds, 16 * k, d, f);
 #pragma unroll
         for (int h = 0; h < HB; ++h) window_mfma(s[h][k], f, qf[h][d]);
       }
@@ -238,8 +229,6 @@ __device__ __forceinline__ void window_wide(const float* __restrict__ qp, const 
         }
       }
     }
-    float alpha[HB];
-    Parts pf[HB][BLOCKS / 2];
 #pragma unroll
     for (int h = 0; h < HB; ++h) {
       float top = -TCMI_INF;
@@ -265,6 +254,24 @@ __device__ __forceinline__ void window_wide(const float* __restrict__ qp, const 
 #pragma unroll
       for (int k = 0; k < BLOCKS; k += 2) window_parts(s[h][k], s[h][k + 1], minus, pf[h][k / 2]);
     }
+  };
+  if (begin < end) load(kp, begin);
+  for (int32_t i = begin; i < end; ++i) {
+    const int32_t j0 = tiles.at(i) * NB;
+    __syncthreads();
+    x.store(klds, minus);
+    load(vp, i);
+    __syncthreads();
+    // (What none of the wavefront's rows sees: past its last position, or between its sinks and its windows.)
+    const bool some = j0 <= p1 && (j0 + NB > w.from(p0) || j0 < static_cast<int32_t>(S::SINKS));
+    const bool whole = full && j0 + NB - 1 <= p0 && (j0 >= w.from(p1) || j0 + NB <= static_cast<int32_t>(S::SINKS));
+    float alpha[HB];
+    Parts pf[HB][BLOCKS / 2];
+    if (some) scores(j0, whole, alpha, pf);
+    x.store(vlds, minus);
+    __syncthreads();
+    if (i + 1 < end) load(kp, i + 1);
+    if (!some) continue;
 #pragma unroll
     for (int g = 0; g < G; g += 2) {
       f4 sum[HB][2];
@@ -275,7 +282,7 @@ __device__ __forceinline__ void window_wide(const float* __restrict__ qp, const 
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           Parts f;
-          W::V::across(vlds, 32 * k, 16 * (g + e), f);
+          T::across(vlds, 32 * k, 16 * (g + e), f);
 #pragma unroll
           for (int h = 0; h < HB; ++h) window_mfma(sum[h][e], f, pf[h][k]);
         }
@@ -364,13 +371,13 @@ __device__ __forceinline__ void window_line(Parts (&f)[SLICES], const float* __r
   }
 }
 
-// The gradients: tiles of 32 lines, and 32 lines a wavefront's own where its registers hold both of their operands.
+// The gradients: tiles of 32 lines, 16·HB lines a wavefront's own.
 template <class S>
 struct WindowBack {
   static constexpr int DP = (S::DH + 31) / 32 * 32, SLICES = DP / 32, G = DP / 16, NB = 32, BLOCKS = 2;
-  static constexpr int HB = DP <= 64 ? 2 : 1;
+  static constexpr int HB = S::HB;
   static constexpr uint32_t ROWS = 64 * HB;
-  using T = WindowTile<S, NB, 16>;
+  using T = WindowTile<S, NB>;
   static constexpr int LDS = 2 * T::BYTES + 3 * NB * 4;
 };
 
@@ -464,8 +471,57 @@ __device__ __forceinline__ void window_wide_dq(const WindowGradArgs a, float* __
   }
 }
 
-// Workgroup: W::ROWS keys of a sequence's key head, the `chunk`-th CHUNK tiles of 32 rows of those that see one of them. parts of chunk c: of
-// dk, then of dv, [c][keys][DH] for c < CHUNKS, and for more (keys below SINKS alone have them) the FEW first keys' [c - CHUNKS][B][FEW][HK][DH].
+// The positions that see one of `keys` keys from `first` on: from the first key on, up to the last one's window or the sequence's
+// end; and their tiles of 32 rows.
+template <class S>
+struct WindowSeen {
+  int32_t p0, p1, begin, end;
+  __device__ __forceinline__ WindowSeen(const WindowSpan<S>& w, int32_t first, int32_t keys) {
+    constexpr int32_t R = WindowSpan<S>::R;
+    const int32_t last = min(first + keys, w.length) - 1;
+    p0 = max(first, w.first);
+    p1 = w.length - 1;
+    if (S::WINDOW != 0u && first >= static_cast<int32_t>(S::SINKS) && p1 - last >= static_cast<int32_t>(S::WINDOW)) p1 = last + static_cast<int32_t>(S::WINDOW) - 1;
+    p1 = min(p1, w.first + static_cast<int32_t>(S::T) - 1);
+    if (first >= w.length) p1 = p0 - 1;
+    begin = end = 0;
+    if (p0 <= p1) {
+      begin = (p0 - w.first) * R / 32;
+      end = ((p1 - w.first + 1) * R + 31) / 32;
+    }
+  }
+  __device__ __forceinline__ uint32_t chunks() const { return (end - begin + S::CHUNK - 1u) / S::CHUNK; }
+};
+
+// The sums of a lane's keys to dk and dv, or to chunk `chunk` of their parts: [c][keys][DH] for c < CHUNKS, and for more (keys below
+// SINKS alone have them) the FEW first keys' [c - CHUNKS][B][FEW][HK][DH].
+template <class S, bool DK, bool DV, int HB, int G>
+__device__ __forceinline__ void window_key_sums(float* __restrict__ dk, float* __restrict__ dv, char* ws, uint32_t b, uint32_t hk, uint32_t chunk, const int32_t (&key)[HB],
+                                                const f4 (&dka)[HB][G], const f4 (&dva)[HB][G]) {
+  const int q = (threadIdx.x >> 4) & 3;
+#pragma unroll
+  for (int h = 0; h < HB; ++h) {
+    if (key[h] >= static_cast<int32_t>(S::KEYS)) continue;
+    const size_t line = ((size_t)b * S::KEYS + key[h]) * S::HK + hk;
+    float *tk = dk + line * S::DH, *tv = dv + line * S::DH;
+    float by = static_cast<float>(S::scale());
+    if constexpr (S::CHUNKS_MOST > 1u) {
+      if (chunk >= S::CHUNKS && key[h] >= static_cast<int32_t>(S::FEW)) continue;
+      constexpr size_t ALL = (size_t)S::B * S::KEYS * S::HK, SOME = (size_t)S::B * S::FEW * S::HK;
+      const size_t at = (chunk < S::CHUNKS ? chunk * ALL + line : S::CHUNKS * ALL + (chunk - S::CHUNKS) * SOME + ((size_t)b * S::FEW + key[h]) * S::HK + hk) * S::DH;
+      tk = reinterpret_cast<float*>(ws + S::DKPARTS) + at;
+      tv = reinterpret_cast<float*>(ws + S::DVPARTS) + at;
+      by = 1.f;
+    }
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      if constexpr (DK) window_store<S>(tk, 16 * g + 4 * q, dka[h][g] * by);
+      if constexpr (DV) window_store<S>(tv, 16 * g + 4 * q, dva[h][g]);
+    }
+  }
+}
+
+// Workgroup: W::ROWS keys of a sequence's key head, the `chunk`-th CHUNK tiles of 32 rows of those that see one of them.
 template <class S, bool DK, bool DV>
 __device__ __forceinline__ void window_wide_dkv(const WindowGradArgs a, float* __restrict__ dk, float* __restrict__ dv, char* ws, char* lds, uint32_t head, uint32_t tile, uint32_t chunk) {
   using W = WindowBack<S>;
@@ -483,23 +539,10 @@ __device__ __forceinline__ void window_wide_dkv(const WindowGradArgs a, float* _
   size_t line[HB];
   Parts kf[HB][SLICES], vf[HB][SLICES];
   f4 dka[HB][G], dva[HB][G];
-  // The positions that see one of the keys: from the first key on, up to the last one's window or the sequence's end.
-  auto seen = [&](int32_t first, int32_t keys, int32_t& p0, int32_t& p1) __attribute__((always_inline)) {
-    const int32_t last = min(first + keys, w.length) - 1;
-    p0 = max(first, w.first);
-    p1 = w.length - 1;
-    if (S::WINDOW != 0u && first >= static_cast<int32_t>(S::SINKS) && p1 - last >= static_cast<int32_t>(S::WINDOW)) p1 = last + static_cast<int32_t>(S::WINDOW) - 1;
-    p1 = min(p1, w.first + static_cast<int32_t>(S::T) - 1);
-    if (first >= w.length) p1 = p0 - 1;
-  };
-  int32_t p0, p1, m0, m1;
-  seen(j0, W::ROWS, p0, p1);
-  seen(mine, 16 * HB, m0, m1);
-  int32_t begin = 0, end = 0;
-  if (p0 <= p1) {
-    begin = (p0 - w.first) * R / NB + static_cast<int32_t>(chunk * S::CHUNK);
-    end = min(((p1 - w.first + 1) * R + NB - 1) / NB, begin + static_cast<int32_t>(S::CHUNK));
-  }
+  const WindowSeen<S> all(w, j0, W::ROWS), own(w, mine, 16 * HB);
+  if (chunk > 0u && chunk >= all.chunks()) return;
+  const int32_t p0 = all.p0, p1 = all.p1, m0 = own.p0, m1 = own.p1;
+  const int32_t begin = all.begin + static_cast<int32_t>(chunk * S::CHUNK), end = min(all.end, begin + static_cast<int32_t>(S::CHUNK));
 #pragma unroll
   for (int h = 0; h < HB; ++h) {
     key[h] = mine + 16 * h + t;
@@ -552,55 +595,44 @@ __device__ __forceinline__ void window_wide_dkv(const WindowGradArgs a, float* _
     if (i + 1 < end) load(i + 1);
     const int32_t r0 = i * NB, a0 = w.first + r0 / R, a1 = w.first + min(r0 + NB - 1, ROWS - 1) / R;
     if (m0 > m1 || a1 < m0 || a0 > m1) continue;
-    const bool whole = r0 + NB <= ROWS && a0 >= max(p0, mine + 16 * HB - 1) && a1 <= p1 && (w.from(a1) <= mine || mine + 16 * HB <= static_cast<int32_t>(S::SINKS));
-    f4 s[HB][BLOCKS], dp[HB][BLOCKS];
+    const bool whole = r0 + NB <= ROWS && a0 >= max(p0, mine + 16 * HB - 1) && a1 <= p1 && mine + 16 * HB <= w.length && (w.from(a1) <= mine || mine + 16 * HB <= static_cast<int32_t>(S::SINKS));
+    f4 s[HB][BLOCKS];
     window_dots<T>(s, qlds, kf);
-    if constexpr (DK) window_dots<T>(dp, dlds, vf);
-    Parts pf[HB][1], ds[HB][1];
+    Parts f[HB][1];
 #pragma unroll
     for (int k = 0; k < BLOCKS; ++k) {
       const f4 ls = *reinterpret_cast<const f4*>(row_lse + 16 * k + 4 * q);
-      const f4 ms = *reinterpret_cast<const f4*>(row_mass + 16 * k + 4 * q);
       const int4 ps = *reinterpret_cast<const int4*>(row_pos + 16 * k + 4 * q);
       const int32_t pos[4] = {ps.x, ps.y, ps.z, ps.w};
 #pragma unroll
       for (int h = 0; h < HB; ++h) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const bool sees = whole || (pos[r] >= 0 && w.sees(pos[r], key[h]));
-          s[h][k][r] = sees ? __builtin_amdgcn_exp2f(s[h][k][r] - ls[r]) : 0.f;
-          if constexpr (DK) dp[h][k][r] = sees ? s[h][k][r] * (dp[h][k][r] - ms[r]) : 0.f;
-        }
+        for (int r = 0; r < 4; ++r) s[h][k][r] = whole || (pos[r] >= 0 && w.sees(pos[r], key[h])) ? __builtin_amdgcn_exp2f(s[h][k][r] - ls[r]) : 0.f;
       }
     }
+    if constexpr (DV) {
 #pragma unroll
-    for (int h = 0; h < HB; ++h) {
-      if constexpr (DV) window_parts(s[h][0], s[h][1], minus, pf[h][0]);
-      if constexpr (DK) window_parts(dp[h][0], dp[h][1], minus, ds[h][0]);
+      for (int h = 0; h < HB; ++h) window_parts(s[h][0], s[h][1], minus, f[h][0]);
+      window_sums<T>(dva, dlds, f);
     }
-    if constexpr (DV) window_sums<T>(dva, dlds, pf);
-    if constexpr (DK) window_sums<T>(dka, qlds, ds);
-  }
+    if constexpr (DK) {
+      f4 dp[HB][BLOCKS];
+      window_dots<T>(dp, dlds, vf);
 #pragma unroll
-  for (int h = 0; h < HB; ++h) {
-    if (key[h] >= static_cast<int32_t>(S::KEYS)) continue;
-    float *tk = dk + line[h] * S::DH, *tv = dv + line[h] * S::DH;
-    float by = static_cast<float>(S::scale());
-    if constexpr (S::CHUNKS_MOST > 1u) {
-      // (Their first CHUNKS as all keys', further ones of the first keys apart.)
-      const size_t few = ((size_t)b * S::FEW + min(key[h], static_cast<int32_t>(S::FEW) - 1)) * S::HK + hk;
-      const size_t at = chunk < S::CHUNKS ? ((size_t)chunk * S::B * S::KEYS * S::HK + line[h]) * S::DH : (size_t)S::CHUNKS * S::B * S::KEYS * S::HK * S::DH + ((size_t)(chunk - S::CHUNKS) * S::B * S::FEW * S::HK + few) * S::DH;
-      if (chunk >= S::CHUNKS && key[h] >= static_cast<int32_t>(S::FEW)) continue;
-      tk = reinterpret_cast<float*>(ws + S::DKPARTS) + at;
-      tv = reinterpret_cast<float*>(ws + S::DVPARTS) + at;
-      by = 1.f;
-    }
+      for (int k = 0; k < BLOCKS; ++k) {
+        const f4 ms = *reinterpret_cast<const f4*>(row_mass + 16 * k + 4 * q);
 #pragma unroll
-    for (int g = 0; g < G; ++g) {
-      if constexpr (DK) window_store<S>(tk, 16 * g + 4 * q, dka[h][g] * by);
-      if constexpr (DV) window_store<S>(tv, 16 * g + 4 * q, dva[h][g]);
+        for (int h = 0; h < HB; ++h) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[h][k][r] = s[h][k][r] != 0.f ? s[h][k][r] * (dp[h][k][r] - ms[r]) : 0.f;
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < HB; ++h) window_parts(s[h][0], s[h][1], minus, f[h][0]);
+      window_sums<T>(dka, qlds, f);
     }
   }
+  window_key_sums<S, DK, DV>(dk, dv, ws, b, hk, chunk, key, dka, dva);
 }
 
 // dq from its splits' sums: thread `at`, four floats.
@@ -620,21 +652,24 @@ __device__ __forceinline__ void window_wide_add(float* __restrict__ dq, const fl
 }
 // dk (scaled) or dv from their chunks' sums.
 template <class S>
-__device__ __forceinline__ void window_wide_join(float* __restrict__ out, const float* __restrict__ parts, float by, size_t at) {
+__device__ __forceinline__ void window_wide_join(float* __restrict__ out, const float* __restrict__ parts, const float* __restrict__ lengths, float by, size_t at) {
   constexpr size_t ROW = (size_t)S::HK * S::DH, N = (size_t)S::B * S::KEYS * ROW, E = S::VEC ? 4 : 1;
   if (at * E >= N) return;
+  const uint32_t b = at * E / (S::KEYS * ROW), key = at * E / ROW % S::KEYS;
+  const WindowSpan<S> w(lengths, b);
+  // (A chunk without rows was not written, but the first.)
+  const uint32_t chunks = max(1u, WindowSeen<S>(w, key / S::ROWS_EACH * S::ROWS_EACH, S::ROWS_EACH).chunks());
   f4 sum = {0.f, 0.f, 0.f, 0.f};
   auto add = [&](const float* p) __attribute__((always_inline)) {
     if constexpr (S::VEC) sum += *reinterpret_cast<const f4*>(p);
     else sum[0] += *p;
   };
 #pragma unroll 4
-  for (uint32_t k = 0; k < S::CHUNKS; ++k) add(parts + k * N + at * E);
-  const size_t b = at * E / (S::KEYS * ROW), key = at * E / ROW % S::KEYS;
+  for (uint32_t k = 0; k < min(chunks, S::CHUNKS + 0u); ++k) add(parts + k * N + at * E);
   if (key < S::FEW) {
     const float* more = parts + S::CHUNKS * N + ((size_t)b * S::FEW + key) * ROW + at * E % ROW;
 #pragma unroll 4
-    for (uint32_t k = S::CHUNKS; k < S::CHUNKS_MOST; ++k) add(more + (size_t)(k - S::CHUNKS) * S::B * S::FEW * ROW);
+    for (uint32_t k = S::CHUNKS; k < chunks; ++k) add(more + (size_t)(k - S::CHUNKS) * S::B * S::FEW * ROW);
   }
   sum *= by;
   if constexpr (S::VEC) *reinterpret_cast<f4*>(out + at * E) = sum;

@@ -17,12 +17,12 @@ function windowSizes(graph, node) {
 }
 
 function maker(s, e, types) {
-  return (kind, grid, threads, lds, call, more) => kernel(kind, `#include "${/_wide/.test(call) ? 'tcmi_window_wide.h' : 'tcmi_window.h'}"
+  return (kind, grid, threads, lds, call, more) => kernel(kind, `#include "${/_pack/.test(call) ? 'tcmi_window_packed.h' : /_wide/.test(call) ? 'tcmi_window_wide.h' : 'tcmi_window.h'}"
 struct ${S} {
 ${constants(Object.assign({}, s.z, more || {}), types)}
   static __device__ __forceinline__ double scale() { return ${double(s.scale)}; }
 };
-extern "C" __global__ void __launch_bounds__(${threads}${/_wide(_dq|_dkv)?</.test(call) && s.z.DH <= 128 ? ', 2' : ''}) __KERNEL__(${e.sig}) {
+extern "C" __global__ void __launch_bounds__(${threads}${/_(wide|packed)(_dq|_dkv)?</.test(call) && s.z.DH <= 128 ? ', 2' : ''}) __KERNEL__(${e.sig}) {
 ${e.open}${lds ? `  __shared__ __attribute__((aligned(16))) ${lds};\n` : ''}  tcmi::${call};
 }
 `, grid, threads);
@@ -43,6 +43,21 @@ const WIDE_ROWS = 64;
  */
 const FILL = 4 * CUS;
 
+/** Blocks of 16 lines of a wavefront's own, of `lines` of a head: two where its registers `hold` them and two workgroups a CU are left. */
+function blocksOf(hold, lines, heads) { return hold && ceil(lines, 128) * heads >= 2 * CUS ? 2 : 1; }
+
+/**
+ * Whether operands are split by a launch of their own (tcmi_window_packed.h), not by each workgroup that reads them (tcmi_window_wide.h): where
+ * four workgroups or more read a key, by its registers for heads up to 128.
+ */
+const packs = (z) => z.DH <= 128 && ceil(Math.min(z.T, z.WINDOW || z.T) * (z.H / z.HK), 128) >= 4;
+
+/** Floats of a line, eight a lane, as they stand in LDS (WindowTile::LD). */
+const lanesOf = (DH) => (DH <= 32 ? 4 : DH <= 64 ? 8 : DH <= 128 ? 16 : 32);
+
+/** Workspace of `planes` planes of `lines` lines a head of two bytes a float. */
+const formBytes = (z, lines, planes) => z.B * z.HK * lines * lanesOf(z.DH) * 16 * planes;
+
 /** Splits of the tiles of NB keys that `rows` rows of one head see, of `blocks` workgroups otherwise: eight tiles each or more. */
 function keySplits(z, rows, NB, blocks) {
   const R = z.H / z.HK;
@@ -52,19 +67,63 @@ function keySplits(z, rows, NB, blocks) {
 
 function wideForward(s, parts, joined) {
   const { z } = s, e = entry(joined ? parts : null), heads = z.B * z.HK, R = z.H / z.HK;
-  const rows = z.DH <= 128 ? 128 : 64, tiles = ceil(z.T * R, rows), SPLITS = keySplits(z, rows, z.DH <= 64 ? 64 : 32, tiles * heads);
-  const more = { TILES: ceil(z.T * R, 16), SPLITS }, types = {};
+  const HB = blocksOf(z.DH <= 128, z.T * R, heads), rows = 64 * HB, tiles = ceil(z.T * R, rows), SPLITS = keySplits(z, rows, z.DH <= 64 ? 64 : 32, tiles * heads);
+  const more = { TILES: ceil(z.T * R, 16), SPLITS, HB }, types = { HB: 'int' };
   let at = 0;
   const place = (name, bytes) => { more[name] = at; types[name] = 'size_t'; at = align(at + bytes, 256); };
   place('OUT', SPLITS > 1 ? 4 * SPLITS * heads * more.TILES * 16 * z.DH : 0);
   place('STATS', SPLITS > 1 ? 8 * SPLITS * heads * more.TILES * 16 : 0);
+  const KP = align(z.KEYS, 64), packed = packs(z);
+  if (packed) {
+    more.WAVES = 4;
+    types.WAVES = 'int';
+    place('KSCALE', 4 * heads * KP);
+    place('KDOTS', formBytes(z, KP, 2));
+    place('VSUMS', formBytes(z, KP, 3));
+  }
   const out = (p) => (parts.includes(p) ? e.out(p) : 'nullptr');
   const L = s.lengths ? 'A.in[3]' : 'nullptr', ws = `reinterpret_cast<char*>(${e.ws})`, m = maker(s, e, types);
   // The last rows, which see most, first; a head's on one XCD, whose L2 its keys share, where heads are a multiple of eight.
-  const kernels = [m('winwide', grid(tiles * heads * SPLITS), 256, `char lds[tcmi::WindowWide<${S}>::LDS]`,
-    `window_wide<${S}>(A.in[0], A.in[1], A.in[2], ${L}, ${out('o')}, ${out('lse')}, ${ws}, lds, blockIdx.x % ${heads}u, ${tiles - 1}u - blockIdx.x / ${heads * SPLITS}u, blockIdx.x / ${heads}u % ${SPLITS}u)`, more)];
+  const kernels = [], where = `blockIdx.x % ${heads}u, ${tiles - 1}u - blockIdx.x / ${heads * SPLITS}u, blockIdx.x / ${heads}u % ${SPLITS}u`;
+  if (packed) {
+    kernels.push(packKeys(m, z, L, ws, more, heads, KP, false));
+    kernels.push(m('winpacked', grid(tiles * heads * SPLITS), 256, `char lds[tcmi::WindowPacked<${S}>::FORWARD]`,
+      `window_packed<${S}>(A.in[0], ${L}, ${out('o')}, ${out('lse')}, ${ws}, lds, ${where})`, more));
+  } else {
+    kernels.push(m('winwide', grid(tiles * heads * SPLITS), 256, `char lds[tcmi::WindowWide<${S}>::LDS]`,
+      `window_wide<${S}>(A.in[0], A.in[1], A.in[2], ${L}, ${out('o')}, ${out('lse')}, ${ws}, lds, ${where})`, more));
+  }
   if (SPLITS > 1) kernels.push(joinKernel(m, z, out, ws, more, heads));
   return { kernels, workspace: at };
+}
+
+/** The launch that splits keys and values. */
+function packKeys(m, z, L, ws, more, heads, KP, back) {
+  const each = 256 / lanesOf(z.DH);
+  return m('winpack', grid(ceil(heads * KP, each)), 256, null,
+    `window_pack_keys<${S}, ${back}>(A.in[1], A.in[2], ${L}, ${ws}, blockIdx.x * ${each}u + threadIdx.x / ${lanesOf(z.DH)}u)`, more);
+}
+
+/**
+ * Tiles of 32 rows a chunk of a gradient of keys, `rows` of them a workgroup's: the fewest rounds of chunks over the `slots` workgroups that run at
+ * once, each chunk with what four more tiles cost, and its sums' bytes.
+ */
+function rowChunk(z, rows, heads, slots) {
+  const R = z.H / z.HK, first = z.LAST ? z.KEYS - z.T : 0, counts = [];
+  for (let j = 0; j < z.KEYS; j += rows) {
+    const p0 = Math.max(j, first), last = Math.min(j + rows, z.KEYS) - 1;
+    const p1 = Math.min(z.WINDOW && j >= z.SINKS ? Math.min(z.KEYS - 1, last + z.WINDOW - 1) : z.KEYS - 1, first + z.T - 1);
+    counts.push(p0 <= p1 ? ceil((p1 - first + 1) * R, 32) - Math.floor((p0 - first) * R / 32) : 0);
+  }
+  const most = Math.max(1, ...counts);
+  let best = null;
+  for (let chunk = Math.min(most, 8); ; chunk = Math.min(most, Math.ceil(chunk * 1.1))) {
+    const n = heads * counts.reduce((q, c) => q + Math.max(1, ceil(c, chunk)), 0), rounds = ceil(n, slots);
+    // (A tile takes about 3 us, of four products; a byte of sums is written and read at 5 TB/s in all.)
+    const time = (rounds < 3 ? rounds : Math.max(2, n / slots + 0.5)) * (chunk + 4) * 3 * z.DH / 64 + (n > heads * counts.length ? n * rows * z.DH * 16 / 5e6 : 0);
+    if (!best || time < best.time) best = { chunk, time };
+    if (chunk >= most) return best.chunk;
+  }
 }
 
 /** The launch that joins the splits of rows. */
@@ -101,7 +160,7 @@ function backwardKernels(s, parts, joined) {
   const L = s.lengths ? 'A.in[3]' : 'nullptr', first = s.lengths ? 4 : 3;
   const args = `{A.in[0], A.in[1], A.in[2], ${L}, A.in[${first}], A.in[${first + 1}], A.in[${first + 2}], ${e.ws}}`;
   const dq = parts.includes('dq'), dk = parts.includes('dk'), dv = parts.includes('dv');
-  const types = {}, more = {};
+  const types = { HB: 'int' }, more = {};
   let at = align(4 * z.B * z.T * z.H, 256);
   const place = (name, bytes) => { more[name] = at; types[name] = 'size_t'; at = align(at + bytes, 256); };
   const m = maker(s, e, types), ws = `reinterpret_cast<char*>(${e.ws})`;
@@ -113,35 +172,59 @@ function backwardKernels(s, parts, joined) {
     if (dk || dv) kernels.push(m('windkv', grid(KTILES * heads), 256, lds, `window_dkv<${S}, ${dk}, ${dv}>(${args}, ${out('dk')}, ${out('dv')}, lds, blockIdx.x)`, { KTILES }));
     return { kernels, workspace: at };
   }
-  const rows = z.DH <= 64 ? 128 : 64, lds = `char lds[tcmi::WindowBack<${S}>::LDS]`, add = (n) => grid(ceil(z.DH % 4 ? n : n / 4, 256));
+  const add = (n) => grid(ceil(z.DH % 4 ? n : n / 4, 256)), KP = align(z.KEYS, 64), RP = align(z.T * R, 64), packed = packs(z), lanes = lanesOf(z.DH);
+  const hold = z.DH <= 64;
+  if (packed) {
+    types.WAVES = 'int';
+    Object.assign(more, { WAVES: 4, HB: 1, SPLITS: 1 });
+    place('KSCALE', 4 * heads * KP);
+    place('VSCALE', 4 * heads * KP);
+    place('KDOTS', formBytes(z, KP, 2));
+    place('VDOTS', formBytes(z, KP, 2));
+    place('KSUMS', dq ? formBytes(z, KP, 3) : 0);
+    place('ROWSTATS', 16 * heads * RP);
+    for (const [name, planes] of [['QDOTS', 2], ['DDOTS', 2], ['QSUMS', 3], ['DSUMS', 3]]) place(name, dk || dv ? formBytes(z, RP, planes) : 0);
+    kernels.length = 0;
+    kernels.push(packKeys(m, z, L, ws, Object.assign({ VSUMS: 0 }, more), heads, KP, true));
+    kernels.push(m('winpack', grid(ceil(heads * RP, 256 / lanes)), 256, null, `window_pack_rows<${S}, ${dk || dv}>(${args}, ${ws}, blockIdx.x * ${256 / lanes}u + threadIdx.x / ${lanes}u)`, more));
+  }
   if (dq) {
-    const tiles = ceil(z.T * R, rows), SPLITS = keySplits(z, rows, 32, tiles * heads), lines = z.B * z.T * z.H;
-    more.SPLITS = SPLITS;
+    more.HB = blocksOf(hold, z.T * R, heads);
+    const rows = 64 * more.HB, tiles = ceil(z.T * R, rows), lines = z.B * z.T * z.H;
+    const SPLITS = more.SPLITS = keySplits(z, rows, packed && hold ? 64 : 32, tiles * heads);
     place('DQPARTS', SPLITS > 1 ? 4 * SPLITS * lines * z.DH : 0);
     const sums = `reinterpret_cast<float*>(${ws} + ${S}::DQPARTS)`;
-    kernels.push(m('winwidedq', grid(tiles * heads * SPLITS), 256, lds,
-      `window_wide_dq<${S}>(${args}, ${out('dq')}, ${sums}, lds, blockIdx.x % ${heads}u, ${tiles - 1}u - blockIdx.x / ${heads * SPLITS}u, blockIdx.x / ${heads}u % ${SPLITS}u)`, more));
+    const where = `blockIdx.x % ${heads}u, ${tiles - 1}u - blockIdx.x / ${heads * SPLITS}u, blockIdx.x / ${heads}u % ${SPLITS}u`;
+    if (packed) kernels.push(m('winpackeddq', grid(tiles * heads * SPLITS), 256, `char lds[tcmi::WindowPacked<${S}>::DQ]`, `window_packed_dq<${S}>(${args}, ${out('dq')}, ${sums}, ${ws}, lds, ${where})`, more));
+    else kernels.push(m('winwidedq', grid(tiles * heads * SPLITS), 256, `char lds[tcmi::WindowBack<${S}>::LDS]`, `window_wide_dq<${S}>(${args}, ${out('dq')}, ${sums}, lds, ${where})`, more));
     if (SPLITS > 1) kernels.push(m('winadd', add(lines * z.DH), 256, null, `window_wide_add<${S}>(${out('dq')}, ${sums}, blockIdx.x * 256u + threadIdx.x)`, more));
   }
   if (dk || dv) {
-    // Tiles of 32 rows that see a key of one workgroup's at most: of any key by the window, of a sink all.
-    const tiles = ceil(z.KEYS, rows), all = ceil(z.T * R, 32), most = z.WINDOW ? Math.min(all, ceil((z.WINDOW + rows) * R, 32) + 1) : all;
+    // Eight wavefronts where a packed tile takes most of LDS.
+    const waves = packed && z.DH > 64 ? 8 : 4;
+    more.HB = blocksOf(hold, z.KEYS, heads);
+    if (packed) more.WAVES = waves;
+    const rows = 16 * waves * more.HB, tiles = ceil(z.KEYS, rows), all = ceil(z.T * R, 32), most = z.WINDOW ? Math.min(all, ceil((z.WINDOW + rows) * R, 32) + 1) : all;
     const sinks = z.WINDOW ? Math.min(tiles, ceil(Math.min(z.SINKS, z.KEYS), rows)) : 0;
-    const CHUNK = Math.max(8, ceil(most, Math.max(1, ceil(FILL, tiles * heads))));
+    const CHUNK = rowChunk(z, rows, heads, waves === 8 ? CUS : 2 * CUS);
     const CHUNKS = ceil(most, CHUNK), CHUNKS_MOST = sinks ? Math.max(CHUNKS, ceil(all, CHUNK)) : CHUNKS, FEW = Math.min(z.KEYS, sinks * rows);
-    Object.assign(more, { CHUNK, CHUNKS, CHUNKS_MOST, FEW });
+    Object.assign(more, { CHUNK, CHUNKS, CHUNKS_MOST, FEW, ROWS_EACH: rows });
     const floats = CHUNKS_MOST > 1 ? (CHUNKS * z.KEYS + (CHUNKS_MOST - CHUNKS) * FEW) * z.B * z.HK * z.DH : 0;
     place('DKPARTS', dk ? 4 * floats : 0);
     place('DVPARTS', dv ? 4 * floats : 0);
     // The sinks' chunks, then the other tiles', the keys that most queries see first.
     const few = sinks * CHUNKS_MOST, id = `(blockIdx.x / ${heads}u)`;
     const where = `blockIdx.x % ${heads}u, ${id} < ${few}u ? ${id} / ${CHUNKS_MOST}u : ${sinks}u + (${id} - ${few}u) / ${CHUNKS}u, ${id} < ${few}u ? ${id} % ${CHUNKS_MOST}u : (${id} - ${few}u) % ${CHUNKS}u`;
-    kernels.push(m('winwidedkv', grid((few + (tiles - sinks) * CHUNKS) * heads), 256, lds,
-      `window_wide_dkv<${S}, ${dk}, ${dv}>(${args}, ${out('dk')}, ${out('dv')}, ${ws}, lds, ${where})`, more));
+    const blocks = grid((few + (tiles - sinks) * CHUNKS) * heads);
+    // Both at once, or of the largest heads, which its registers do not hold both of, one after the other.
+    for (const [k, v] of dk && dv && z.DH > 128 ? [[false, true], [true, false]] : [[dk, dv]]) {
+      if (packed) kernels.push(m('winpackeddkv', blocks, 64 * waves, `char lds[tcmi::WindowPackedRows<${S}>::LDS]`, `window_packed_dkv<${S}, ${k}, ${v}>(${args}, ${out('dk')}, ${out('dv')}, ${ws}, lds, ${where})`, more));
+      else kernels.push(m('winwidedkv', blocks, 256, `char lds[tcmi::WindowBack<${S}>::LDS]`, `window_wide_dkv<${S}, ${k}, ${v}>(${args}, ${out('dk')}, ${out('dv')}, ${ws}, lds, ${where})`, more));
+    }
     if (CHUNKS_MOST > 1) {
       const n = z.B * z.KEYS * z.HK * z.DH;
       for (const [p, name, by] of [['dk', 'DKPARTS', `static_cast<float>(${S}::scale())`], ['dv', 'DVPARTS', '1.f']]) {
-        if (parts.includes(p)) kernels.push(m('winadd', add(n), 256, null, `window_wide_join<${S}>(${out(p)}, reinterpret_cast<const float*>(${ws} + ${S}::${name}), ${by}, blockIdx.x * 256u + threadIdx.x)`, more));
+        if (parts.includes(p)) kernels.push(m('winadd', add(n), 256, null, `window_wide_join<${S}>(${out(p)}, reinterpret_cast<const float*>(${ws} + ${S}::${name}), ${L}, ${by}, blockIdx.x * 256u + threadIdx.x)`, more));
       }
     }
   }

@@ -136,6 +136,17 @@ const CONTEXT = [
   window('wide', [1, 150, 2, 256], [1, 150, 1, 256], { window: 70 }, { gradient: true }),
   window('late', [2, 70, 4, 96], [2, 300, 2, 96], { window: 120, sinks: 4 }, { gradient: true }),
   window('more-queries', [2, 20, 2, 32], [2, 7, 2, 32], { queries: 'first' }, { gradient: true }),
+  // By operands split once (several workgroups read each key).
+  window('packed', [2, 300, 8, 64], [2, 300, 1, 64], { window: 70, sinks: 5 }, { lengths: true, gradient: true }),
+  window('packed-odd', [1, 517, 6, 15], [1, 517, 2, 15], { window: 200, sinks: 20 }, { gradient: true }),
+  window('packed-late', [4, 200, 8, 80], [4, 700, 2, 80], { window: 150, sinks: 3 }, { lengths: true, gradient: true }),
+  window('packed-first', [3, 333, 6, 96], [3, 333, 2, 96], { queries: 'first', window: 190 }, { lengths: true, gradient: true }),
+  window('packed-heads', [1, 601, 2, 128], [1, 601, 2, 128], { scale: -0.05 }, { gradient: true }),
+  window('packed-small', [1, 1100, 1, 24], [1, 1100, 1, 24], {}, { gradient: true }),
+  window('packed-sinks', [1, 520, 4, 32], [1, 520, 2, 32], { window: 258, sinks: 300 }, { gradient: true }),
+  window('packed-k', [1, 140, 4, 64], [1, 140, 1, 64], {}, { gradient: true, wrt: ['k'] }),
+  window('packed-v', [1, 140, 4, 64], [1, 140, 1, 64], {}, { gradient: true, wrt: ['v'] }),
+  window('packed-q', [1, 140, 4, 64], [1, 140, 1, 64], {}, { gradient: true, wrt: ['q'] }),
   window('only-q', [2, 64, 4, 32], [2, 64, 2, 32], { window: 20 }, { gradient: true, wrt: ['q'] }),
   window('only-k', [2, 64, 4, 32], [2, 64, 2, 32], { window: 20 }, { gradient: true, wrt: ['k'] }),
   window('only-v', [2, 64, 4, 32], [2, 64, 2, 32], { window: 20 }, { gradient: true, wrt: ['v'] }),

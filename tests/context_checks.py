@@ -11,6 +11,8 @@ import numpy as np
 from oracle import operators
 from operator_checks import FLOOR, U, pair_sum
 
+ROW_FLOOR = 2.0 ** -39
+
 
 def inputs_of(case, graph, seed):
     """float32 inputs by name, with what the operators meet in earnest: tokens that are no row over rows that hold no numbers, rows of
@@ -174,8 +176,9 @@ def window_allowed(node, args, shapes):
     T, R = shapes[0][1], shapes[0][2] // shapes[1][2]
     mt = lambda x: np.abs(x).transpose(0, 1, 3, 2)
     top = lambda x: np.abs(x).max(initial=0.0)
+    rows = lambda x, y: 2 * dh * ROW_FLOOR * np.abs(x).max(3, keepdims=True) * np.abs(y).max(3)[:, :, None]
     seen = np.where(sees, np.abs(s), 0.0)
-    es = scale * (pair_sum(dh) * (np.abs(q) @ mt(k)) + 2 * dh * FLOOR * top(q) * top(k)) + 6 * U * seen
+    es = scale * (pair_sum(dh) * (np.abs(q) @ mt(k)) + rows(q, k)) + 6 * U * seen
     some = sees.any(3)[..., None]
     with np.errstate(all="ignore"):
         if node["op"] == "windowAttention":
@@ -201,7 +204,7 @@ def window_allowed(node, args, shapes):
             a, K = dy, T * R
         else:
             dp, D = dy @ v.transpose(0, 1, 3, 2), (dy * o).sum(3, keepdims=True)
-            edp = pair_sum(dh) * (np.abs(dy) @ mt(v)) + 2 * dh * FLOOR * top(dy) * top(v) + (dh + 16) * U * (np.abs(dy) * np.abs(o)).sum(3, keepdims=True)
+            edp = pair_sum(dh) * (np.abs(dy) @ mt(v)) + rows(dy, v) + (dh + 16) * U * (np.abs(dy) * np.abs(o)).sum(3, keepdims=True)
             mass = p * np.abs(dp - D)
             off = mass * (rel + 4 * U) + p * (edp + 2 * U * (np.abs(dp) + np.abs(D)))
             a, K = (k, S) if part == "dq" else (q, T * R)
