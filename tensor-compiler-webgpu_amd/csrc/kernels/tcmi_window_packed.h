@@ -172,26 +172,34 @@ __device__ __forceinline__ void window_pack_rows(const WindowGradArgs a, char* w
   P::sums(ws + S::DSUMS, P::RP, head, r, c, d0, d1, minus);
 }
 
-// The copy of PLANES planes of NB lines of a form to LDS, by THREADS threads: in flight until vmcnt reaches 0.
+// Copies of 16 bytes (4: one word) a lane from `from` on to LDS from `to` on (both uniform), in flight until vmcnt reaches 0. Written as
+// instructions: of the compiler's own it takes every later read of LDS to depend on them, and waits for them there (of a gradient of keys
+// twice a tile: 950 us, 757 so). They have no register results, and a wait that the compiler counts without them is only
+// longer for them; barrier_ahead() is what the tiles' readers wait at.
+__device__ __forceinline__ void window_copy16(uint32_t to, const char* from) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"((threadIdx.x & 63u) * 16u), "s"(from) : "memory", "m0");
+}
+__device__ __forceinline__ void window_copy4(uint32_t to, const char* from) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(to), "v"((threadIdx.x & 63u) * 4u), "s"(from) : "memory", "m0");
+}
+__device__ __forceinline__ uint32_t window_lds(char* p) { return static_cast<uint32_t>(reinterpret_cast<size_t>((__attribute__((address_space(3))) char*)p)); }
+
+// The copy of PLANES planes of NB lines of a form to LDS, by THREADS threads.
 template <int NB, int LD, int PLANES, int THREADS>
 __device__ __forceinline__ void window_fetch(char* to, const char* from, size_t plane) {
   constexpr int BYTES = NB * LD, ALL = PLANES * BYTES;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   static_assert(BYTES % 1024 == 0, "a wavefront's 1 KiB is of one plane");
 #pragma unroll
   for (int u = 0; u < (ALL + THREADS * 16 - 1) / (THREADS * 16); ++u) {
     const int byte = (u * (THREADS / 64) + wave) * 1024;
     if (ALL % (THREADS * 16) != 0 && byte >= ALL) break;
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)(from + byte / BYTES * plane + byte % BYTES + lane * 16),
-                                     (__attribute__((address_space(3))) uint32_t*)(to + byte), 16, 0, 0);
+    window_copy16(window_lds(to) + byte, from + byte / BYTES * plane + byte % BYTES);
   }
 }
-// And of `lanes` words (a wavefront's, 64 at most) by wavefront `by`.
+// And of 64 words by wavefront `by`.
 __device__ __forceinline__ void window_fetch_words(char* to, const void* from, int by) {
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (wave != by) return;
-  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)(static_cast<const uint32_t*>(from) + lane),
-                                   (__attribute__((address_space(3))) uint32_t*)to, 4, 0, 0);
+  if (__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) == by) window_copy4(window_lds(to), static_cast<const char*>(from));
 }
 
 // This lane's part of a first operand of dots: lines line0 + t, floats 32·slice + 8q ....
@@ -591,13 +599,13 @@ __device__ __forceinline__ void window_packed_dkv(const WindowGradArgs a, float*
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int row = 16 * k + 4 * q + r;
-          const float4 st = *reinterpret_cast<const float4*>(stats + row * 16);
+          const f4 st = *reinterpret_cast<const f4*>(stats + row * 16);
           const int32_t at = r0 + row, pos = at < ROWS ? w.first + at / R : -1;
 #pragma unroll
           for (int h = 0; h < HB; ++h) {
             const bool sees = whole || (w.stands(pos) && key[h] < w.length && w.sees(pos, key[h]));
-            s[h][k][r] = sees ? __builtin_amdgcn_exp2f(fmaf(s[h][k][r] * ks[h], st.x, -st.z)) : 0.f;
-            if constexpr (DK) dp[h][k][r] = sees ? s[h][k][r] * fmaf(dp[h][k][r] * vs[h], st.y, -st.w) : 0.f;
+            s[h][k][r] = sees ? __builtin_amdgcn_exp2f(fmaf(s[h][k][r] * ks[h], st[0], -st[2])) : 0.f;
+            if constexpr (DK) dp[h][k][r] = sees ? s[h][k][r] * fmaf(dp[h][k][r] * vs[h], st[1], -st[3]) : 0.f;
           }
         }
       }

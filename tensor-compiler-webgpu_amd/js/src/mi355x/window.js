@@ -43,8 +43,11 @@ const WIDE_ROWS = 64;
  */
 const FILL = 4 * CUS;
 
-/** Blocks of 16 lines of a wavefront's own, of `lines` of a head: two where its registers `hold` them and two workgroups a CU are left. */
-function blocksOf(hold, lines, heads) { return hold && ceil(lines, 128) * heads >= 2 * CUS ? 2 : 1; }
+/**
+ * Blocks of 16 lines of a wavefront's own, of `lines` of a head over `tiles` tiles of the other side: two where its registers `hold` them and two
+ * workgroups a CU are left, of which several may deal the tiles among them, eight each or more.
+ */
+function blocksOf(hold, lines, heads, tiles) { return hold && ceil(lines, 128) * heads * Math.max(1, Math.min(8, Math.floor(tiles / 8))) >= 2 * CUS ? 2 : 1; }
 
 /**
  * Whether operands are split by a launch of their own (tcmi_window_packed.h), not by each workgroup that reads them (tcmi_window_wide.h): where
@@ -67,7 +70,7 @@ function keySplits(z, rows, NB, blocks) {
 
 function wideForward(s, parts, joined) {
   const { z } = s, e = entry(joined ? parts : null), heads = z.B * z.HK, R = z.H / z.HK;
-  const HB = blocksOf(z.DH <= 128, z.T * R, heads), rows = 64 * HB, tiles = ceil(z.T * R, rows), SPLITS = keySplits(z, rows, z.DH <= 64 ? 64 : 32, tiles * heads);
+  const HB = blocksOf(z.DH <= 128, z.T * R, heads, ceil(z.WINDOW ? Math.min(z.KEYS, z.WINDOW) : z.KEYS, 64)), rows = 64 * HB, tiles = ceil(z.T * R, rows), SPLITS = keySplits(z, rows, z.DH <= 64 ? 64 : 32, tiles * heads);
   const more = { TILES: ceil(z.T * R, 16), SPLITS, HB }, types = { HB: 'int' };
   let at = 0;
   const place = (name, bytes) => { more[name] = at; types[name] = 'size_t'; at = align(at + bytes, 256); };
@@ -189,7 +192,7 @@ function backwardKernels(s, parts, joined) {
     kernels.push(m('winpack', grid(ceil(heads * RP, 256 / lanes)), 256, null, `window_pack_rows<${S}, ${dk || dv}>(${args}, ${ws}, blockIdx.x * ${256 / lanes}u + threadIdx.x / ${lanes}u)`, more));
   }
   if (dq) {
-    more.HB = blocksOf(hold, z.T * R, heads);
+    more.HB = blocksOf(hold, z.T * R, heads, ceil(z.WINDOW ? Math.min(z.KEYS, z.WINDOW) : z.KEYS, 64));
     const rows = 64 * more.HB, tiles = ceil(z.T * R, rows), lines = z.B * z.T * z.H;
     const SPLITS = more.SPLITS = keySplits(z, rows, packed && hold ? 64 : 32, tiles * heads);
     place('DQPARTS', SPLITS > 1 ? 4 * SPLITS * lines * z.DH : 0);
@@ -202,7 +205,7 @@ function backwardKernels(s, parts, joined) {
   if (dk || dv) {
     // Eight wavefronts where a packed tile takes most of LDS.
     const waves = packed && z.DH > 64 ? 8 : 4;
-    more.HB = blocksOf(hold, z.KEYS, heads);
+    more.HB = blocksOf(hold, z.KEYS, heads, ceil(Math.min(z.T, z.WINDOW || z.T) * R, 32));
     if (packed) more.WAVES = waves;
     const rows = 16 * waves * more.HB, tiles = ceil(z.KEYS, rows), all = ceil(z.T * R, 32), most = z.WINDOW ? Math.min(all, ceil((z.WINDOW + rows) * R, 32) + 1) : all;
     const sinks = z.WINDOW ? Math.min(tiles, ceil(Math.min(z.SINKS, z.KEYS), rows)) : 0;
