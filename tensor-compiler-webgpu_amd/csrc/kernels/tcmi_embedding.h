@@ -12,7 +12,7 @@
 //
 // A pass of the sort, a tile of keys a workgroup: a key's place is the count of smaller digits, of
 // its digit in the tiles before, in the wavefronts before and among the lanes before it (found by comparing digits bit by bit
-// over the wavefront). The counts over all tiles are each workgroup's own (SELF: few keys) or a launch's before.
+// over the wavefront). The tiles are counted by a launch before each pass; a few keys are one tile, and one launch makes all passes.
 //
 // Bound: HBM (dy read, the table's gradient written).
 
@@ -82,7 +82,7 @@ struct EmbedPairs {
   static __device__ __forceinline__ uint32_t digit(int32_t key) { return (static_cast<uint32_t>(key) >> (PASS * S::BITS)) & ((1u << S::BITS) - 1u); }
 };
 
-// The lanes that have a key of this lane's digit. (Its first counts for all of them: a frequent token's lanes would queue at its bin.)
+// The lanes that have a key of this lane's digit.
 template <int BITS>
 __device__ __forceinline__ uint64_t embed_same(bool has, uint32_t digit) {
   uint64_t same = __ballot(has);
@@ -100,82 +100,87 @@ __device__ __forceinline__ void embed_step() {
   __builtin_amdgcn_wave_barrier();
 }
 
+// Keys that a wavefront of the sort holds at a time, 64 each: their loads are in flight together.
+constexpr uint32_t EMBED_HELD = 8;
+
 // Counts tile `tile`'s digits.
 template <class S, int PASS>
 __device__ __forceinline__ void embed_count(const float* __restrict__ tokens, char* ws, uint32_t* bins, uint32_t tile) {
   const EmbedPairs<S, PASS> in{tokens, ws};
   constexpr uint32_t BINS = 1u << S::BITS;
   const uint32_t n = in.count(), begin = tile * S::TILE, end = min(n, begin + S::TILE), lane = threadIdx.x % 64u;
-  for (uint32_t b = threadIdx.x; b < BINS; b += 256u) bins[b] = 0u;
+  for (uint32_t b = threadIdx.x; b < BINS; b += S::SORT) bins[b] = 0u;
   __syncthreads();
-  for (uint32_t base = begin + threadIdx.x - lane; base < end; base += 256u) {
-    const uint32_t i = base + lane;
-    const int32_t key = i < end ? in.key(i) : -1;
-    const uint32_t d = in.digit(key);
-    const uint64_t same = embed_same<S::BITS>(key >= 0, d);
-    if (key >= 0 && __builtin_ctzll(same) == static_cast<int>(lane)) atomicAdd(bins + d, static_cast<uint32_t>(__popcll(same)));
+  for (uint32_t base = begin + threadIdx.x - lane; base < end; base += S::SORT * EMBED_HELD) {
+    int32_t key[EMBED_HELD];
+#pragma unroll
+    for (uint32_t u = 0; u < EMBED_HELD; ++u) {
+      const uint32_t i = base + u * S::SORT + lane;
+      key[u] = i < end ? in.key(i) : -1;
+    }
+#pragma unroll
+    for (uint32_t u = 0; u < EMBED_HELD; ++u) {
+      if (key[u] >= 0) atomicAdd(bins + in.digit(key[u]), 1u);
+    }
   }
   __syncthreads();
   uint32_t* hist = reinterpret_cast<uint32_t*>(ws + S::HIST) + (size_t)tile * BINS;
-  for (uint32_t b = threadIdx.x; b < BINS; b += 256u) hist[b] = bins[b];
+  for (uint32_t b = threadIdx.x; b < BINS; b += S::SORT) hist[b] = bins[b];
 }
 
-// Tile `tile`'s pairs to their places. lds: 6·BINS + 4 words.
+// Tile `tile`'s pairs to their places, by SORT threads. lds: (1 + SORT / 64)·BINS + SORT / 64 words.
 template <class S, int PASS>
 __device__ __forceinline__ void embed_sort(const float* __restrict__ tokens, char* ws, uint32_t* lds, uint32_t tile) {
   const EmbedPairs<S, PASS> in{tokens, ws};
-  constexpr uint32_t BINS = 1u << S::BITS;
+  constexpr uint32_t BINS = 1u << S::BITS, WAVES = S::SORT / 64u;
   const uint32_t n = in.count(), begin = tile * S::TILE, end = min(n, begin + S::TILE);
   const uint32_t lane = threadIdx.x % 64u, wave = threadIdx.x / 64u;
-  uint32_t *all = lds, *before = lds + BINS, *own = lds + 2u * BINS, *part = lds + 6u * BINS;    // own: of each wavefront
-  for (uint32_t b = threadIdx.x; b < 6u * BINS; b += 256u) lds[b] = 0u;
-  __syncthreads();
+  uint32_t *own = lds, *before = lds + WAVES * BINS, *part = before + BINS;    // own: of each wavefront; before: of smaller digits, and of the tiles before
+  for (uint32_t b = threadIdx.x; b < WAVES * BINS; b += S::SORT) own[b] = 0u;
   // Each wavefront's keys of the tile are a run of their own.
-  constexpr uint32_t RUN = S::TILE / 4u;
-  const uint32_t mine = begin + wave * RUN, mine_end = min(end, mine + RUN);
-  if constexpr (S::SELF) {
-    for (uint32_t base = wave * 64u; base < n; base += 256u) {
-      const uint32_t i = base + lane;
-      const int32_t key = i < n ? in.key(i) : -1;
-      const uint32_t d = in.digit(key);
-      const uint64_t same = embed_same<S::BITS>(key >= 0, d);
-      if (key >= 0 && __builtin_ctzll(same) == static_cast<int>(lane)) {
-        const uint32_t c = static_cast<uint32_t>(__popcll(same));
-        atomicAdd(all + d, c);
-        // (A tile is a multiple of 64 keys: the wavefront's are all before it or none.)
-        if (base < begin) atomicAdd(before + d, c);
-      }
+  constexpr uint32_t RUN = S::TILE / WAVES;
+  static_assert(RUN % 64u == 0u, "runs of whole wavefronts");
+  const uint32_t mine = min(end, begin + wave * RUN), mine_end = min(end, mine + RUN);
+  __syncthreads();
+  for (uint32_t base = mine; base < mine_end; base += 64u * EMBED_HELD) {
+    int32_t key[EMBED_HELD];
+#pragma unroll
+    for (uint32_t u = 0; u < EMBED_HELD; ++u) {
+      const uint32_t i = base + u * 64u + lane;
+      key[u] = i < mine_end ? in.key(i) : -1;
     }
-  } else {
-    const uint32_t* hist = reinterpret_cast<const uint32_t*>(ws + S::HIST);
-    for (uint32_t b = threadIdx.x; b < BINS; b += 256u) {
-      uint32_t sum = 0u, prior = 0u;
-      for (uint32_t t = 0; t < S::TILES; ++t) {
-        if (t == tile) prior = sum;
-        sum += hist[(size_t)t * BINS + b];
-      }
-      all[b] = sum;
-      before[b] = prior;
+#pragma unroll
+    for (uint32_t u = 0; u < EMBED_HELD; ++u) {
+      if (key[u] >= 0) atomicAdd(own + wave * BINS + in.digit(key[u]), 1u);
     }
-  }
-  for (uint32_t base = mine; base < mine_end; base += 64u) {
-    const uint32_t i = base + lane;
-    const int32_t key = i < mine_end ? in.key(i) : -1;
-    const uint32_t d = in.digit(key);
-    const uint64_t same = embed_same<S::BITS>(key >= 0, d);
-    if (key >= 0 && __builtin_ctzll(same) == static_cast<int>(lane)) own[wave * BINS + d] += static_cast<uint32_t>(__popcll(same));
-    embed_step();
   }
   __syncthreads();
-  // The first place of each digit: thread t sums its PER digits, and the sums of the threads before it come by wavefront.
-  constexpr uint32_t PER = (BINS + 255u) / 256u;
-  uint32_t sum = 0u, mineof[PER];
+  // Thread t's PER digits: how many there are of each, and of them in the tiles before.
+  constexpr uint32_t PER = (BINS + S::SORT - 1u) / S::SORT;
+  uint32_t sum = 0u, smaller[PER], prior[PER];
 #pragma unroll
   for (uint32_t k = 0; k < PER; ++k) {
     const uint32_t b = threadIdx.x * PER + k;
-    mineof[k] = sum;
-    sum += b < BINS ? all[b] : 0u;
+    smaller[k] = sum;
+    prior[k] = 0u;
+    if (b < BINS) {
+      uint32_t all = 0u;
+      if constexpr (S::TILES == 1u) {
+#pragma unroll
+        for (uint32_t w = 0; w < WAVES; ++w) all += own[w * BINS + b];
+      } else {
+        const uint32_t* hist = reinterpret_cast<const uint32_t*>(ws + S::HIST) + b;
+#pragma unroll 8
+        for (uint32_t t = 0; t < S::TILES; ++t) {
+          const uint32_t c = hist[(size_t)t * BINS];
+          all += c;
+          prior[k] += t < tile ? c : 0u;
+        }
+      }
+      sum += all;
+    }
   }
+  // The sums of the threads before it come by wavefront.
   uint32_t scan = sum;
 #pragma unroll
   for (int off = 1; off < 64; off *= 2) {
@@ -190,29 +195,49 @@ __device__ __forceinline__ void embed_sort(const float* __restrict__ tokens, cha
   for (uint32_t k = 0; k < PER; ++k) {
     const uint32_t b = threadIdx.x * PER + k;
     if (b < BINS) {
-      uint32_t at = first + mineof[k] + before[b];
+      uint32_t at = first + smaller[k] + prior[k];
 #pragma unroll
-      for (uint32_t w = 0; w < 4u; ++w) {
+      for (uint32_t w = 0; w < WAVES; ++w) {
         const uint32_t c = own[w * BINS + b];
         own[w * BINS + b] = at;
         at += c;
       }
     }
   }
-  if (PASS == 0 && tile == 0 && threadIdx.x == 255u) *reinterpret_cast<uint32_t*>(ws + S::COUNT) = first + sum;
+  if (PASS == 0 && tile == 0 && threadIdx.x == S::SORT - 1u) *reinterpret_cast<uint32_t*>(ws + S::COUNT) = first + sum;
   __syncthreads();
-  for (uint32_t base = mine; base < mine_end; base += 64u) {
-    const uint32_t i = base + lane;
-    const int32_t key = i < mine_end ? in.key(i) : -1;
-    const uint32_t d = in.digit(key);
-    const uint64_t same = embed_same<S::BITS>(key >= 0, d);
-    if (key >= 0) {
-      const uint32_t at = own[wave * BINS + d];
-      embed_step();
-      in.put(at + static_cast<uint32_t>(__popcll(same & ((1ull << lane) - 1ull))), key, in.place(i));
-      if (__builtin_ctzll(same) == static_cast<int>(lane)) own[wave * BINS + d] = at + static_cast<uint32_t>(__popcll(same));
+  for (uint32_t base = mine; base < mine_end; base += 64u * EMBED_HELD) {
+    int32_t key[EMBED_HELD];
+    uint32_t from[EMBED_HELD];
+#pragma unroll
+    for (uint32_t u = 0; u < EMBED_HELD; ++u) {
+      const uint32_t i = base + u * 64u + lane;
+      key[u] = i < mine_end ? in.key(i) : -1;
+      from[u] = i < mine_end ? in.place(i) : 0u;
     }
-    embed_step();
+#pragma unroll
+    for (uint32_t u = 0; u < EMBED_HELD; ++u) {
+      const uint32_t d = in.digit(key[u]);
+      const uint64_t same = embed_same<S::BITS>(key[u] >= 0, d);
+      if (key[u] >= 0) {
+        const uint32_t at = own[wave * BINS + d];
+        embed_step();
+        in.put(at + static_cast<uint32_t>(__popcll(same & ((1ull << lane) - 1ull))), key[u], from[u]);
+        if (__builtin_ctzll(same) == static_cast<int>(lane)) own[wave * BINS + d] = at + static_cast<uint32_t>(__popcll(same));
+      }
+      embed_step();
+    }
+  }
+}
+
+// All passes by one workgroup, whose tile all keys are: a pass reads what the one before wrote.
+template <class S, int PASS = 0>
+__device__ __forceinline__ void embed_sort_all(const float* __restrict__ tokens, char* ws, uint32_t* lds) {
+  embed_sort<S, PASS>(tokens, ws, lds, 0u);
+  if constexpr (PASS + 1 < S::PASSES) {
+    __threadfence();
+    __syncthreads();
+    embed_sort_all<S, PASS + 1>(tokens, ws, lds);
   }
 }
 

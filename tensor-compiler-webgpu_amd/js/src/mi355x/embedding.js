@@ -42,8 +42,8 @@ function lowerEmbedding(graph, node) {
   return { kind: 'embedding', kernels: [k], workspace: 0 };
 }
 
-// Keys of a sort that its workgroups count for themselves; beyond, a launch before each pass counts each tile once.
-const COUNTED = 16384;
+// Keys that one workgroup sorts, of 1024 threads; beyond, tiles of them are sorted by 256.
+const ONE_TILE = 16384;
 
 function lowerEmbeddingGrad(graph, node) {
   const N = size(graph.nodes[node.inputs[0]].shape), [V, D] = node.shape;
@@ -51,8 +51,9 @@ function lowerEmbeddingGrad(graph, node) {
   const { E, lanes, columns } = rowLanes(D);
   if (columns > 65535) throw new Error(`embedding: rows of ${D} floats (at most ${65535 * 64 * E})`);
   // Digits of at most nine bits of the token; a tile of keys a workgroup, at most 128 of them.
-  const bits = Math.max(1, Math.ceil(Math.log2(V))), passes = ceil(bits, 9), BITS = ceil(bits, passes);
-  const TILE = Math.max(1024, align(ceil(N, 128), 256)), TILES = ceil(N, TILE), self = N <= COUNTED;
+  const bits = Math.max(1, Math.ceil(Math.log2(V))), PASSES = ceil(bits, 9), BITS = ceil(bits, PASSES);
+  const one = N <= ONE_TILE, SORT = one ? Math.min(1024, align(N, 64)) : 256;
+  const TILE = one ? align(N, SORT) : Math.max(1024, align(ceil(N, 128), 256)), TILES = ceil(N, TILE);
   // Keys of a sum: few enough that 4096 wavefronts walk them.
   const waves = N * columns * lanes / 64;
   let CH = 8;
@@ -60,26 +61,27 @@ function lowerEmbeddingGrad(graph, node) {
   const CHUNKS = ceil(N, CH), split = CHUNKS > 1;
   // Rows of the table that a workgroup looks for: a wavefront's worth where there are enough of them.
   const ROWS = Math.max(4, Math.min(64, ceil(V, 2048)));
-  const z = { N, V, D, E, LANES: lanes, BITS, TILE, TILES, CH, CHUNKS, ROWS, SELF: self };
-  const types = { SELF: 'bool' };
+  const z = { N, V, D, E, LANES: lanes, BITS, PASSES, TILE, TILES, SORT, CH, CHUNKS, ROWS };
+  const types = {};
   let at = 0;
   const place = (name, bytes) => { z[name] = at; types[name] = 'size_t'; at = align(at + bytes, 256); };
   place('COUNT', 256);
-  place('HIST', self ? 0 : 4 * TILES * 2 ** BITS);
+  place('HIST', one ? 0 : 4 * TILES * 2 ** BITS);
   for (const i of [0, 1]) {
-    const used = i < passes;
+    const used = i < PASSES;
     place(`KEYS${i}`, used ? 4 * N : 0);
     place(`PLACES${i}`, used ? 4 * N : 0);
   }
   place('PARTS', split ? 8 * CHUNKS * D : 0);
   const m = make(z, node.attrs.scale, types);
   const kernels = [];
-  for (let p = 0; p < passes; p++) {
-    const ws = 'reinterpret_cast<char*>(A.ws)';
-    if (!self) kernels.push(m('embcount', [TILES, 1, 1], 256, `uint32_t lds[${2 ** BITS}]`, `embed_count<${S}, ${p}>(A.in[0], ${ws}, lds, blockIdx.x)`));
-    kernels.push(m('embsort', [TILES, 1, 1], 256, `uint32_t lds[${6 * 2 ** BITS + 4}]`, `embed_sort<${S}, ${p}>(A.in[0], ${ws}, lds, blockIdx.x)`));
+  const ws = 'reinterpret_cast<char*>(A.ws)', lds = `uint32_t lds[${(1 + SORT / 64) * 2 ** BITS + SORT / 64}]`;
+  if (one) kernels.push(m('embsort', [1, 1, 1], SORT, lds, `embed_sort_all<${S}>(A.in[0], ${ws}, lds)`));
+  for (let p = 0; p < PASSES && !one; p++) {
+    kernels.push(m('embcount', [TILES, 1, 1], SORT, `uint32_t lds[${2 ** BITS}]`, `embed_count<${S}, ${p}>(A.in[0], ${ws}, lds, blockIdx.x)`));
+    kernels.push(m('embsort', [TILES, 1, 1], SORT, lds, `embed_sort<${S}, ${p}>(A.in[0], ${ws}, lds, blockIdx.x)`));
   }
-  const last = (passes - 1) % 2, sums = ceil(CHUNKS, 256 / lanes) * columns, rows = ceil(V, ROWS);
+  const last = (PASSES - 1) % 2, sums = ceil(CHUNKS, 256 / lanes) * columns, rows = ceil(V, ROWS);
   kernels.push(m('embsums', [sums + rows, 1, 1], 256, `uint32_t lds[${ROWS}]`, `embed_sums<${S}, ${last}>(A.in[1], A.out, reinterpret_cast<char*>(A.ws), lds, blockIdx.x)`));
   if (split) {
     kernels.push(m('embjoin', [CHUNKS, ceil(D, 64 * E), 1], 512, `float lds[${8 * 64 * E}]`, `embed_join<${S}, ${last}>(A.out, reinterpret_cast<char*>(A.ws), lds, blockIdx.x, blockIdx.y)`));
