@@ -97,7 +97,7 @@ __device__ __forceinline__ void window_along(f4 (&v)[G], const float* __restrict
   for (int g = 0; g < G; ++g) v[g] = window_load<S>(row, 16 * g + 4 * ((threadIdx.x >> 4) & 3u), on);
 }
 // And across them: dim 16g + t of the tile's key 4q + s, of the keys from j0 on those that one of the rows sees (a value that
-// no query sees may be anything: it is 0 here, for 0 times it would be NaN).
+// no query sees may be anything: it is 0 here, for 0 times it would be NaN). Every load is made, of the last such key where its own is past it.
 template <class S, int G>
 __device__ __forceinline__ void window_across(f4 (&v)[G], const float* __restrict__ base, size_t step, int32_t j0, const WindowTiles& tiles) {
   const int t = threadIdx.x & 15, q = (threadIdx.x >> 4) & 3;
@@ -105,8 +105,13 @@ __device__ __forceinline__ void window_across(f4 (&v)[G], const float* __restric
   for (int s = 0; s < 4; ++s) {
     const int32_t j = j0 + 4 * q + s;
     const bool on = j <= tiles.hi && (j >= tiles.lo || j < static_cast<int32_t>(S::SINKS));
+    const float* at = base + (size_t)min(j, tiles.hi) * step + t;
 #pragma unroll
-    for (int g = 0; g < G; ++g) v[g][s] = on && 16 * g + t < static_cast<int>(S::DH) ? base[(size_t)j * step + 16 * g + t] : 0.f;
+    for (int g = 0; g < G; ++g) {
+      const bool in = 16 * g + 16 <= static_cast<int>(S::DH) || 16 * g + t < static_cast<int>(S::DH);
+      const float x = at[in ? 16 * g : 0 - t];
+      v[g][s] = on && in ? x : 0.f;
+    }
   }
 }
 // acc[k of a][t of b] += the products of two tiles along their rows.
@@ -172,11 +177,23 @@ __device__ __forceinline__ void window_rows(const float* __restrict__ qp, const 
   const float* kb = kp + ((size_t)b * S::KEYS * S::HK + hk) * S::DH;
   const float* vb = vp + ((size_t)b * S::KEYS * S::HK + hk) * S::DH;
   float m = -TCMI_INF, l = 0.f;
+  // (Of a key past the last, the last again: its scores are not taken.) All loads of a tile are made before the tile before it is used.
+  auto load = [&](int32_t i, f4 (&kf)[G], f4 (&vf)[G]) __attribute__((always_inline)) {
+    const int32_t j0 = tiles.at(i) * 16;
+    window_along<S>(kf, kb + (size_t)min(j0 + t, tiles.hi) * step, true);
+    window_across<S>(vf, vb, step, j0, tiles);
+  };
+  f4 kf[G], vf[G], kn[G], vn[G];
+  if (begin + wave < end) load(begin + wave, kn, vn);
   for (int32_t i = begin + wave; i < end; i += 4) {
     const int32_t j0 = tiles.at(i) * 16;
-    f4 kf[G], vf[G];
-    window_along<S>(kf, kb + (size_t)min(j0 + t, w.length - 1) * step, j0 + t < w.length);
-    window_across<S>(vf, vb, step, j0, tiles);
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      kf[g] = kn[g];
+      vf[g] = vn[g];
+    }
+    if (G <= 8 && i + 4 < end) load(i + 4, kn, vn);
+    __builtin_amdgcn_sched_barrier(0);
     f4 s = window_scores(kf, qf);
     float top = -TCMI_INF;
 #pragma unroll
@@ -197,6 +214,7 @@ __device__ __forceinline__ void window_rows(const float* __restrict__ qp, const 
 #pragma unroll
     for (int g = 0; g < G; ++g) acc[g] *= alpha;
     window_sum(acc, vf, s);
+    if (G > 8 && i + 4 < end) load(i + 4, kn, vn);
   }
   // (Each lane has added its own keys.)
   l = quad16_reduce<false>(l);
@@ -229,12 +247,12 @@ __device__ __forceinline__ void window_rows(const float* __restrict__ qp, const 
   }
 }
 
-// Row `at` of all key heads' rows, a wavefront: its splits' sums.
-template <class S>
-__device__ __forceinline__ void window_join(float* __restrict__ out, float* __restrict__ lse, const char* __restrict__ ws, uint32_t at) {
+// Row `at` of all key heads' rows: its splits' sums, by WAVES wavefronts (more than one: a workgroup; lds: WAVES·DH floats).
+template <class S, uint32_t WAVES>
+__device__ __forceinline__ void window_join(float* __restrict__ out, float* __restrict__ lse, const char* __restrict__ ws, float* lds, uint32_t at) {
   using Span = WindowSpan<S>;
   constexpr uint32_t R = Span::R, HEADS = S::B * S::HK;
-  const uint32_t head = at / (S::TILES * 16u), row = at % (S::TILES * 16u), lane = threadIdx.x & 63u;
+  const uint32_t head = at / (S::TILES * 16u), row = at % (S::TILES * 16u), lane = threadIdx.x & 63u, wave = WAVES > 1u ? threadIdx.x / 64u : 0u;
   if (head >= HEADS || row >= Span::ROWS) return;
   const float2* stats = reinterpret_cast<const float2*>(ws + S::STATS);
   const size_t step = (size_t)HEADS * S::TILES * 16u;
@@ -244,15 +262,26 @@ __device__ __forceinline__ void window_join(float* __restrict__ out, float* __re
   const float base = top == -TCMI_INF ? 0.f : top;
   for (uint32_t k = lane; k < S::SPLITS; k += 64u) total += stats[k * step + at].y * __builtin_amdgcn_exp2f(stats[k * step + at].x - base);
   total = wave_reduce<false>(total);
+  const bool some = total > 0.f || total != total;
   const size_t line = ((size_t)(head / S::HK) * S::T + row / R) * S::H + head % S::HK * R + row % R;
-  if (lse != nullptr && lane == 0u) lse[line] = total > 0.f || total != total ? (base + __builtin_amdgcn_logf(total)) * 0.69314718055994531f : -TCMI_INF;
+  if (lse != nullptr && lane == 0u && wave == 0u) lse[line] = some ? (base + __builtin_amdgcn_logf(total)) * 0.69314718055994531f : -TCMI_INF;
   if (out == nullptr) return;
-  const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
+  const float inv = some ? 1.f / total : 0.f;
   for (uint32_t d = lane; d < S::DH; d += 64u) {
     float sum = 0.f;
-#pragma unroll 4
-    for (uint32_t k = 0; k < S::SPLITS; ++k) sum += reinterpret_cast<const float*>(ws + S::OUT)[(k * step + at) * S::DH + d] * __builtin_amdgcn_exp2f(stats[k * step + at].x - base);
-    out[line * S::DH + d] = sum * inv;
+#pragma unroll 8
+    for (uint32_t k = wave; k < S::SPLITS; k += WAVES) sum = fmaf(reinterpret_cast<const float*>(ws + S::OUT)[(k * step + at) * S::DH + d], __builtin_amdgcn_exp2f(stats[k * step + at].x - base), sum);
+    if constexpr (WAVES > 1u) lds[wave * S::DH + d] = sum;
+    else out[line * S::DH + d] = sum * inv;
+  }
+  if constexpr (WAVES > 1u) {
+    __syncthreads();
+    for (uint32_t d = threadIdx.x; d < S::DH; d += 64u * WAVES) {
+      float sum = lds[d];
+#pragma unroll
+      for (uint32_t w = 1; w < WAVES; ++w) sum += lds[w * S::DH + d];
+      out[line * S::DH + d] = sum * inv;
+    }
   }
 }
 

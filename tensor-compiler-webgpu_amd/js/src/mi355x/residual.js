@@ -16,12 +16,11 @@ function residualSizes(graph, node) {
   const names = ['x', 'y', a.pre && 'gain', a.bias && !grad && 'bias', a.post && 'postGain', a.postBias && 'postBias', a.gate && 'gate'].filter(Boolean).concat(grad ? a.has : []);
   const gated = names.indexOf('gate');
   const full = gated >= 0 && size(graph.nodes[node.inputs[gated]].shape) !== D;
-  const E = D % 4 === 0 ? 4 : 1;
   // Lanes of a row, a power of two, with at most 16 floats each.
   let lanes = 16;
   while (lanes * 16 < D) lanes *= 2;
-  const threads = Math.max(256, lanes), units = ceil(D, lanes * E);
-  return { z: { N, D, E, LANES: lanes, UNITS: units, THREADS: threads, LAYER: a.norm === 'layer', PRE: a.pre, POST: a.post, GATE: gated < 0 ? GATE.none : full ? GATE.full : GATE.vector },
+  const threads = Math.max(256, lanes), units = ceil(D, lanes * 4);
+  return { z: { N, D, LANES: lanes, UNITS: units, THREADS: threads, LAYER: a.norm === 'layer', PRE: a.pre, POST: a.post, GATE: gated < 0 ? GATE.none : full ? GATE.full : GATE.vector },
     names, grad };
 }
 
@@ -37,7 +36,7 @@ function residualKernels(node, sizes, parts, joined) {
   const out = (p) => (parts.includes(p) ? e.out(p) : 'nullptr');
   const text = (includes, call, threads, lds) => `#include "tcmi_residual.h"
 struct __KERNEL___s {
-${constants(Object.assign({}, z, includes), { GATE: 'int', E: 'int', UNITS: 'int', SUMS: 'int' })}
+${constants(Object.assign({}, z, includes), { GATE: 'int', UNITS: 'int', SUMS: 'int' })}
   static __device__ __forceinline__ float eps() { return static_cast<float>(${double(a.eps)}); }
   static __device__ __forceinline__ float residual() { return static_cast<float>(${double(a.residual)}); }
 };

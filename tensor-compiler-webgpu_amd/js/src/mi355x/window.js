@@ -131,7 +131,11 @@ function rowChunk(z, rows, heads, slots) {
 
 /** The launch that joins the splits of rows. */
 function joinKernel(m, z, out, ws, more, heads) {
-  return m('winjoin', grid(ceil(heads * more.TILES * 16, 4)), 256, null, `window_join<${S}>(${out('o')}, ${out('lse')}, ${ws}, blockIdx.x * 4u + threadIdx.x / 64u)`, more);
+  const rows = heads * more.TILES * 16;
+  // A wavefront a row, or a workgroup where the splits are many (32 rows of 128 splits 14.3 us by one, 6 by four).
+  const waves = more.SPLITS >= 16 && rows < 2 ** 20 ? 4 : 1;
+  return m('winjoin', grid(ceil(rows, 4 / waves)), 256, waves > 1 ? `float lds[${4 * z.DH}]` : null,
+    `window_join<${S}, ${waves}>(${out('o')}, ${out('lse')}, ${ws}, ${waves > 1 ? 'lds, blockIdx.x' : 'nullptr, blockIdx.x * 4u + threadIdx.x / 64u'})`, more);
 }
 
 function forwardKernels(s, parts, joined) {
@@ -139,6 +143,7 @@ function forwardKernels(s, parts, joined) {
   if (z.T * (z.H / z.HK) >= WIDE_ROWS) return wideForward(s, parts, joined);
   const R = z.H / z.HK, TILES = ceil(z.T * R, 16), heads = z.B * z.HK;
   // The keys that one tile sees at most, in tiles of 16, dealt to as many workgroups as fill the chip four times, eight tiles each or more.
+  // (32 tokens of 8 heads over 1028 keys: 16.8 us by nine tiles, 21.6 by five.)
   const most = ceil(z.WINDOW ? Math.min(z.KEYS, z.WINDOW + ceil(16, R) + 32 + z.SINKS) : z.KEYS, 16);
   const SPLITS = Math.max(1, Math.min(256, Math.floor(most / 8), ceil(4 * CUS, TILES * heads)));
   const types = { SUMS: 'size_t' };
