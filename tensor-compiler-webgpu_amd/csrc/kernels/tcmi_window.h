@@ -247,42 +247,54 @@ __device__ __forceinline__ void window_rows(const float* __restrict__ qp, const 
   }
 }
 
-// Row `at` of all key heads' rows: its splits' sums, by WAVES wavefronts (more than one: a workgroup; lds: WAVES·DH floats).
-template <class S, uint32_t WAVES>
+// Row `at` of all key heads' rows: its splits' sums. LANES lanes hold its floats; of many splits a
+// workgroup's PARTS groups of them take some each (lds: PARTS·4·LANES floats).
+template <class S, uint32_t LANES, uint32_t PARTS>
 __device__ __forceinline__ void window_join(float* __restrict__ out, float* __restrict__ lse, const char* __restrict__ ws, float* lds, uint32_t at) {
   using Span = WindowSpan<S>;
   constexpr uint32_t R = Span::R, HEADS = S::B * S::HK;
-  const uint32_t head = at / (S::TILES * 16u), row = at % (S::TILES * 16u), lane = threadIdx.x & 63u, wave = WAVES > 1u ? threadIdx.x / 64u : 0u;
+  const uint32_t head = at / (S::TILES * 16u), row = at % (S::TILES * 16u), lane = threadIdx.x % LANES, part = PARTS > 1u ? threadIdx.x / LANES : 0u;
   if (head >= HEADS || row >= Span::ROWS) return;
-  const float2* stats = reinterpret_cast<const float2*>(ws + S::STATS);
+  const float2* stats = reinterpret_cast<const float2*>(ws + S::STATS) + at;
+  const float* sums = reinterpret_cast<const float*>(ws + S::OUT) + (size_t)at * S::DH;
   const size_t step = (size_t)HEADS * S::TILES * 16u;
-  float top = -TCMI_INF, total = 0.f;
-  for (uint32_t k = lane; k < S::SPLITS; k += 64u) top = fmaxf(top, stats[k * step + at].x);
-  top = wave_reduce<true>(top);
-  const float base = top == -TCMI_INF ? 0.f : top;
-  for (uint32_t k = lane; k < S::SPLITS; k += 64u) total += stats[k * step + at].y * __builtin_amdgcn_exp2f(stats[k * step + at].x - base);
-  total = wave_reduce<false>(total);
+  float top = -TCMI_INF, total = 0.f, base;
+  if constexpr (PARTS > 1u) {
+    // (A wavefront's lanes look at a split each.)
+    for (uint32_t k = threadIdx.x & 63u; k < S::SPLITS; k += 64u) top = fmaxf(top, stats[k * step].x);
+    top = wave_reduce<true>(top);
+    base = top == -TCMI_INF ? 0.f : top;
+    for (uint32_t k = threadIdx.x & 63u; k < S::SPLITS; k += 64u) total = fmaf(stats[k * step].y, __builtin_amdgcn_exp2f(stats[k * step].x - base), total);
+    total = wave_reduce<false>(total);
+  } else {
+#pragma unroll 8
+    for (uint32_t k = 0; k < S::SPLITS; ++k) top = fmaxf(top, stats[k * step].x);
+    base = top == -TCMI_INF ? 0.f : top;
+#pragma unroll 8
+    for (uint32_t k = 0; k < S::SPLITS; ++k) total = fmaf(stats[k * step].y, __builtin_amdgcn_exp2f(stats[k * step].x - base), total);
+  }
   const bool some = total > 0.f || total != total;
   const size_t line = ((size_t)(head / S::HK) * S::T + row / R) * S::H + head % S::HK * R + row % R;
-  if (lse != nullptr && lane == 0u && wave == 0u) lse[line] = some ? (base + __builtin_amdgcn_logf(total)) * 0.69314718055994531f : -TCMI_INF;
+  if (lse != nullptr && lane == 0u && part == 0u) lse[line] = some ? (base + __builtin_amdgcn_logf(total)) * 0.69314718055994531f : -TCMI_INF;
   if (out == nullptr) return;
   const float inv = some ? 1.f / total : 0.f;
-  for (uint32_t d = lane; d < S::DH; d += 64u) {
-    float sum = 0.f;
+  f4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
-    for (uint32_t k = wave; k < S::SPLITS; k += WAVES) sum = fmaf(reinterpret_cast<const float*>(ws + S::OUT)[(k * step + at) * S::DH + d], __builtin_amdgcn_exp2f(stats[k * step + at].x - base), sum);
-    if constexpr (WAVES > 1u) lds[wave * S::DH + d] = sum;
-    else out[line * S::DH + d] = sum * inv;
-  }
-  if constexpr (WAVES > 1u) {
-    __syncthreads();
-    for (uint32_t d = threadIdx.x; d < S::DH; d += 64u * WAVES) {
-      float sum = lds[d];
+  for (uint32_t k = part; k < S::SPLITS; k += PARTS) {
+    const f4 x = window_load<S>(sums + k * step * S::DH, 4u * lane, true);
+    const float f = __builtin_amdgcn_exp2f(stats[k * step].x - base);
 #pragma unroll
-      for (uint32_t w = 1; w < WAVES; ++w) sum += lds[w * S::DH + d];
-      out[line * S::DH + d] = sum * inv;
-    }
+    for (int i = 0; i < 4; ++i) sum[i] = fmaf(x[i], f, sum[i]);
   }
+  if constexpr (PARTS > 1u) {
+    f4* all = reinterpret_cast<f4*>(lds);
+    all[threadIdx.x] = sum;
+    __syncthreads();
+    if (part != 0u) return;
+#pragma unroll
+    for (uint32_t p = 1; p < PARTS; ++p) sum += all[p * LANES + lane];
+  }
+  window_store<S>(out + line * S::DH, 4u * lane, sum * inv);
 }
 
 struct WindowGradArgs {

@@ -94,8 +94,8 @@ struct Packed {
   }
 };
 
-// Line `id` of the heads' keys: K's dots, V's sums and (BACK) V's dots and K's sums, K's and V's scales.
-template <class S, bool BACK>
+// Line `id` of the heads' keys: K's dots and V's sums, or of the gradients (BACK) K's and V's dots and (DQ) K's sums; their scales.
+template <class S, bool BACK, bool DQ>
 __device__ __forceinline__ void window_pack_keys(const float* __restrict__ kp, const float* __restrict__ vp, const float* __restrict__ lengths, char* ws, uint32_t id) {
   using P = Packed<S>;
   const uint32_t head = id / P::KP, j = id % P::KP;
@@ -125,7 +125,7 @@ __device__ __forceinline__ void window_pack_keys(const float* __restrict__ kp, c
   const Minus minus;
   P::dots(ws + S::KDOTS, P::KP, head, j, c, k0, k1, ks.up);
   if constexpr (BACK) {
-    P::sums(ws + S::KSUMS, P::KP, head, j, c, k0, k1, minus);
+    if constexpr (DQ) P::sums(ws + S::KSUMS, P::KP, head, j, c, k0, k1, minus);
     P::dots(ws + S::VDOTS, P::KP, head, j, c, v0, v1, vs.up);
   } else {
     P::sums(ws + S::VSUMS, P::KP, head, j, c, v0, v1, minus);
@@ -170,6 +170,13 @@ __device__ __forceinline__ void window_pack_rows(const WindowGradArgs a, char* w
   P::dots(ws + S::DDOTS, P::RP, head, r, c, d0, d1, ds.up);
   P::sums(ws + S::QSUMS, P::RP, head, r, c, q0, q1, minus);
   P::sums(ws + S::DSUMS, P::RP, head, r, c, d0, d1, minus);
+}
+
+// The first KEYBLOCKS workgroups: keys, the rest: rows.
+template <class S, bool DQ, bool DKV, uint32_t KEYBLOCKS>
+__device__ __forceinline__ void window_pack_both(const WindowGradArgs a, char* ws, uint32_t block, uint32_t key, uint32_t row) {
+  if (block < KEYBLOCKS) window_pack_keys<S, true, DQ>(a.k, a.v, a.lengths, ws, key);
+  else window_pack_rows<S, DKV>(a, ws, row);
 }
 
 // Copies of 16 bytes (4: one word) a lane from `from` on to LDS from `to` on (both uniform), in flight until vmcnt reaches 0. Written as

@@ -371,6 +371,31 @@ __device__ __forceinline__ void window_line(Parts (&f)[SLICES], const float* __r
   }
 }
 
+// dy·o of a row, whose floats 32·s + 8q ... lane (t, q) adds up; every lane of the row gets it.
+template <class S>
+__device__ __forceinline__ float window_row_mass(const float* __restrict__ o, const float* __restrict__ dy, bool on) {
+  const int q = (threadIdx.x >> 4) & 3;
+  float sum = 0.f;
+#pragma unroll
+  for (int s = 0; s < (static_cast<int>(S::DH) + 31) / 32; ++s) {
+#pragma unroll
+    for (int h = 0; h < 8; h += 4) {
+      const f4 x = window_load<S>(o, 32 * s + 8 * q + h, on), y = window_load<S>(dy, 32 * s + 8 * q + h, on);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum = fmaf(x[i], y[i], sum);
+    }
+  }
+  return quad16_reduce<false>(sum);
+}
+// Of 16 lines a wavefront from `line` on (where no gradient of queries forms them beside its own).
+template <class S>
+__device__ __forceinline__ void window_wide_mass(const float* __restrict__ o, const float* __restrict__ dy, float* __restrict__ mass, size_t line) {
+  constexpr size_t LINES = (size_t)S::B * S::T * S::H;
+  const size_t at = line + (threadIdx.x & 15u), row = min(at, LINES - 1u) * S::DH;
+  const float sum = window_row_mass<S>(o + row, dy + row, true);
+  if ((threadIdx.x & 48u) == 0u && at < LINES) mass[at] = sum;
+}
+
 // The gradients: tiles of 32 lines, 16·HB lines a wavefront's own.
 template <class S>
 struct WindowBack {
@@ -381,9 +406,10 @@ struct WindowBack {
   static constexpr int LDS = 2 * T::BYTES + 3 * NB * 4;
 };
 
-// Workgroup: W::ROWS rows of a sequence's key head, a split of the keys they see. parts: the splits' sums, [SPLITS][lines][DH].
+// Workgroup: W::ROWS rows of a sequence's key head, a split of the keys they see. parts: the splits' sums, [SPLITS][lines][DH]. Writes
+// dy·o of its rows for the gradients of keys.
 template <class S>
-__device__ __forceinline__ void window_wide_dq(const WindowGradArgs a, float* __restrict__ dq, float* __restrict__ parts, char* lds, uint32_t head, uint32_t tile, uint32_t split) {
+__device__ __forceinline__ void window_wide_dq(const WindowGradArgs a, float* __restrict__ dq, float* __restrict__ parts, float* __restrict__ masses, char* lds, uint32_t head, uint32_t tile, uint32_t split) {
   using W = WindowBack<S>;
   using T = typename W::T;
   using Span = WindowSpan<S>;
@@ -411,7 +437,8 @@ __device__ __forceinline__ void window_wide_dq(const WindowGradArgs a, float* __
     window_line<S>(qf[h], a.q + line[h] * S::DH, on[h], scale, minus);
     window_line<S>(df[h], a.dy + line[h] * S::DH, on[h], 1.f, minus);
     lse[h] = on[h] ? a.lse[line[h]] * LOG2E : 0.f;
-    mass[h] = on[h] ? a.mass[line[h]] : 0.f;
+    mass[h] = window_row_mass<S>(a.o + line[h] * S::DH, a.dy + line[h] * S::DH, on[h]);
+    if (split == 0u && q == 0 && row < ROWS) masses[line[h]] = mass[h];
 #pragma unroll
     for (int g = 0; g < G; ++g) acc[h][g] = f4{0.f, 0.f, 0.f, 0.f};
   }
@@ -649,6 +676,12 @@ __device__ __forceinline__ void window_wide_add(float* __restrict__ dq, const fl
   sum *= static_cast<float>(S::scale());
   if constexpr (S::VEC) *reinterpret_cast<f4*>(dq + at * E) = sum;
   else dq[at] = sum[0];
+}
+// The first of two calls, or the second.
+template <class S, class F, class G>
+__device__ __forceinline__ void window_either(uint32_t which, F first, G second) {
+  if (which == 0u) first();
+  else second();
 }
 // dk (scaled) or dv from their chunks' sums.
 template <class S>

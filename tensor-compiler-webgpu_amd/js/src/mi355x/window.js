@@ -61,11 +61,14 @@ const lanesOf = (DH) => (DH <= 32 ? 4 : DH <= 64 ? 8 : DH <= 128 ? 16 : 32);
 /** Workspace of `planes` planes of `lines` lines a head of two bytes a float. */
 const formBytes = (z, lines, planes) => z.B * z.HK * lines * lanesOf(z.DH) * 16 * planes;
 
-/** Splits of the tiles of NB keys that `rows` rows of one head see, of `blocks` workgroups otherwise: eight tiles each or more. */
+/**
+ * Splits of the tiles of NB keys that `rows` rows of one head see, of `blocks` workgroups otherwise: eight tiles each or more, four where there would be
+ * fewer than two workgroups a CU (288 workgroups of ten tiles, each with its loads' time: 22 us, by halves 14 and 4 to join them).
+ */
 function keySplits(z, rows, NB, blocks) {
   const R = z.H / z.HK;
   const most = ceil(z.WINDOW ? Math.min(z.KEYS, z.WINDOW + ceil(rows, R) + z.SINKS) : z.KEYS, NB);
-  return Math.max(1, Math.min(64, Math.floor(most / 8), ceil(FILL, blocks)));
+  return Math.max(1, Math.min(64, Math.floor(most / (blocks < 2 * CUS ? 4 : 8)), ceil(FILL, blocks)));
 }
 
 function wideForward(s, parts, joined) {
@@ -89,7 +92,7 @@ function wideForward(s, parts, joined) {
   // The last rows, which see most, first; a head's on one XCD, whose L2 its keys share, where heads are a multiple of eight.
   const kernels = [], where = `blockIdx.x % ${heads}u, ${tiles - 1}u - blockIdx.x / ${heads * SPLITS}u, blockIdx.x / ${heads}u % ${SPLITS}u`;
   if (packed) {
-    kernels.push(packKeys(m, z, L, ws, more, heads, KP, false));
+    kernels.push(packKeys(m, z, L, ws, more, heads, KP));
     kernels.push(m('winpacked', grid(tiles * heads * SPLITS), 256, `char lds[tcmi::WindowPacked<${S}>::FORWARD]`,
       `window_packed<${S}>(A.in[0], ${L}, ${out('o')}, ${out('lse')}, ${ws}, lds, ${where})`, more));
   } else {
@@ -101,10 +104,10 @@ function wideForward(s, parts, joined) {
 }
 
 /** The launch that splits keys and values. */
-function packKeys(m, z, L, ws, more, heads, KP, back) {
+function packKeys(m, z, L, ws, more, heads, KP) {
   const each = 256 / lanesOf(z.DH);
   return m('winpack', grid(ceil(heads * KP, each)), 256, null,
-    `window_pack_keys<${S}, ${back}>(A.in[1], A.in[2], ${L}, ${ws}, blockIdx.x * ${each}u + threadIdx.x / ${lanesOf(z.DH)}u)`, more);
+    `window_pack_keys<${S}, false, false>(A.in[1], A.in[2], ${L}, ${ws}, blockIdx.x * ${each}u + threadIdx.x / ${lanesOf(z.DH)}u)`, more);
 }
 
 /**
@@ -131,11 +134,11 @@ function rowChunk(z, rows, heads, slots) {
 
 /** The launch that joins the splits of rows. */
 function joinKernel(m, z, out, ws, more, heads) {
-  const rows = heads * more.TILES * 16;
-  // A wavefront a row, or a workgroup where the splits are many (32 rows of 128 splits 14.3 us by one, 6 by four).
-  const waves = more.SPLITS >= 16 && rows < 2 ** 20 ? 4 : 1;
-  return m('winjoin', grid(ceil(rows, 4 / waves)), 256, waves > 1 ? `float lds[${4 * z.DH}]` : null,
-    `window_join<${S}, ${waves}>(${out('o')}, ${out('lse')}, ${ws}, ${waves > 1 ? 'lds, blockIdx.x' : 'nullptr, blockIdx.x * 4u + threadIdx.x / 64u'})`, more);
+  const rows = heads * more.TILES * 16, lanes = z.DH <= 64 ? 16 : z.DH <= 128 ? 32 : 64;
+  // Of many splits a workgroup a row (32 rows of 128 splits 14.3 us by a wavefront each, 5 so).
+  const parts = more.SPLITS >= 16 && rows < 2 ** 20 ? 256 / lanes : 1;
+  return m('winjoin', grid(parts > 1 ? rows : ceil(rows, 256 / lanes)), 256, parts > 1 ? 'float lds[1024]' : null,
+    `window_join<${S}, ${lanes}, ${parts}>(${out('o')}, ${out('lse')}, ${ws}, ${parts > 1 ? 'lds, blockIdx.x' : `nullptr, blockIdx.x * ${256 / lanes}u + threadIdx.x / ${lanes}u`})`, more);
 }
 
 function forwardKernels(s, parts, joined) {
@@ -173,7 +176,7 @@ function backwardKernels(s, parts, joined) {
   const place = (name, bytes) => { more[name] = at; types[name] = 'size_t'; at = align(at + bytes, 256); };
   const m = maker(s, e, types), ws = `reinterpret_cast<char*>(${e.ws})`;
   const kernels = [];
-  if (dk || dq) kernels.push(m('winmass', grid(ceil(z.B * z.T * z.H, 16)), 256, null, `window_mass<${S}>(A.in[${first}], A.in[${first + 2}], ${e.ws}, blockIdx.x * 16u + threadIdx.x / 16u)`));
+  if (!wide && (dk || dq)) kernels.push(m('winmass', grid(ceil(z.B * z.T * z.H, 16)), 256, null, `window_mass<${S}>(A.in[${first}], A.in[${first + 2}], ${e.ws}, blockIdx.x * 16u + threadIdx.x / 16u)`));
   if (!wide) {
     const TILES = ceil(z.T * R, 16), KTILES = ceil(z.KEYS, 16), lds = `float lds[tcmi::window_lds<${z.DH}>()]`;
     if (dq) kernels.push(m('windq', grid(TILES * heads), 256, lds, `window_dq<${S}>(${args}, ${out('dq')}, lds, blockIdx.x)`, { TILES }));
@@ -192,9 +195,12 @@ function backwardKernels(s, parts, joined) {
     place('KSUMS', dq ? formBytes(z, KP, 3) : 0);
     place('ROWSTATS', 16 * heads * RP);
     for (const [name, planes] of [['QDOTS', 2], ['DDOTS', 2], ['QSUMS', 3], ['DSUMS', 3]]) place(name, dk || dv ? formBytes(z, RP, planes) : 0);
-    kernels.length = 0;
-    kernels.push(packKeys(m, z, L, ws, Object.assign({ VSUMS: 0 }, more), heads, KP, true));
-    kernels.push(m('winpack', grid(ceil(heads * RP, 256 / lanes)), 256, null, `window_pack_rows<${S}, ${dk || dv}>(${args}, ${ws}, blockIdx.x * ${256 / lanes}u + threadIdx.x / ${lanes}u)`, more));
+    const keys = ceil(heads * KP, 256 / lanes), place256 = (first) => `(blockIdx.x - ${first}u) * ${256 / lanes}u + threadIdx.x / ${lanes}u`;
+    kernels.push(m('winpack', grid(keys + ceil(heads * RP, 256 / lanes)), 256, null,
+      `window_pack_both<${S}, ${dq}, ${dk || dv}, ${keys}u>(${args}, ${ws}, blockIdx.x, ${place256(0)}, ${place256(keys)})`, Object.assign({ VSUMS: 0 }, more)));
+  }
+  if (!packed && dk && !dq) {
+    kernels.push(m('winmass', grid(ceil(z.B * z.T * z.H, 64)), 256, null, `window_wide_mass<${S}>(A.in[${first}], A.in[${first + 2}], ${e.ws}, blockIdx.x * 64u + threadIdx.x / 64u * 16u)`));
   }
   if (dq) {
     more.HB = blocksOf(hold, z.T * R, heads, ceil(z.WINDOW ? Math.min(z.KEYS, z.WINDOW) : z.KEYS, 64));
@@ -204,7 +210,7 @@ function backwardKernels(s, parts, joined) {
     const sums = `reinterpret_cast<float*>(${ws} + ${S}::DQPARTS)`;
     const where = `blockIdx.x % ${heads}u, ${tiles - 1}u - blockIdx.x / ${heads * SPLITS}u, blockIdx.x / ${heads}u % ${SPLITS}u`;
     if (packed) kernels.push(m('winpackeddq', grid(tiles * heads * SPLITS), 256, `char lds[tcmi::WindowPacked<${S}>::DQ]`, `window_packed_dq<${S}>(${args}, ${out('dq')}, ${sums}, ${ws}, lds, ${where})`, more));
-    else kernels.push(m('winwidedq', grid(tiles * heads * SPLITS), 256, `char lds[tcmi::WindowBack<${S}>::LDS]`, `window_wide_dq<${S}>(${args}, ${out('dq')}, ${sums}, lds, ${where})`, more));
+    else kernels.push(m('winwidedq', grid(tiles * heads * SPLITS), 256, `char lds[tcmi::WindowBack<${S}>::LDS]`, `window_wide_dq<${S}>(${args}, ${out('dq')}, ${sums}, ${e.ws}, lds, ${where})`, more));
     if (SPLITS > 1) kernels.push(m('winadd', add(lines * z.DH), 256, null, `window_wide_add<${S}>(${out('dq')}, ${sums}, blockIdx.x * 256u + threadIdx.x)`, more));
   }
   if (dk || dv) {
@@ -230,10 +236,10 @@ function backwardKernels(s, parts, joined) {
       else kernels.push(m('winwidedkv', blocks, 256, `char lds[tcmi::WindowBack<${S}>::LDS]`, `window_wide_dkv<${S}, ${k}, ${v}>(${args}, ${out('dk')}, ${out('dv')}, ${ws}, lds, ${where})`, more));
     }
     if (CHUNKS_MOST > 1) {
-      const n = z.B * z.KEYS * z.HK * z.DH;
-      for (const [p, name, by] of [['dk', 'DKPARTS', `static_cast<float>(${S}::scale())`], ['dv', 'DVPARTS', '1.f']]) {
-        if (parts.includes(p)) kernels.push(m('winadd', add(n), 256, null, `window_wide_join<${S}>(${out(p)}, reinterpret_cast<const float*>(${ws} + ${S}::${name}), ${L}, ${by}, blockIdx.x * 256u + threadIdx.x)`, more));
-      }
+      const n = z.B * z.KEYS * z.HK * z.DH, [blocks1] = add(n);
+      const call = (p, name, by) => `window_wide_join<${S}>(${out(p)}, reinterpret_cast<const float*>(${ws} + ${S}::${name}), ${L}, ${by}, blockIdx.x * 256u + threadIdx.x)`;
+      const calls = [[dk, 'dk', 'DKPARTS', `static_cast<float>(${S}::scale())`], [dv, 'dv', 'DVPARTS', '1.f']].filter((c) => c[0]).map(([, ...c]) => call(...c));
+      kernels.push(m('winadd', [blocks1, calls.length, 1], 256, null, calls.length > 1 ? `window_either<${S}>(blockIdx.y, [&] { tcmi::${calls[0]}; }, [&] { tcmi::${calls[1]}; })` : calls[0], more));
     }
   }
   return { kernels, workspace: at };
