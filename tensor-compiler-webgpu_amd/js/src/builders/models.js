@@ -47,7 +47,7 @@ function modelStep(req) {
     const step = tf.buildStep(V, B, cfg, opt);
     const params = tf.initNormal(V, seed, 0.02, cfg);
     const state = tf.initialState(step.names, step.shapes, opt);
-    const batch = (k) => tf.encodeBatch(randomTokens(B, cfg.T, V, seed * 1000 + (k || 0)), V, cfg.T, cfg.targets);
+    const batch = (k) => tf.encodeBatch(randomTokens(B, cfg.T, V, seed * 1000 + (k || 0)), V, cfg.T, cfg.targets, cfg.tokens);
     return { step, params, state, batch, info: { config: 'C5', V, B, cfg, lr, init: 'N(0, 0.02) weights, LayerNorm gains 1 and biases 0' } };
   }
   if (model === 'transformer-ref') {
@@ -82,8 +82,8 @@ function modelForward(req) {
   const V = req.V || (ref ? 16 : 96), B = req.B || (ref ? 4 : 64), seed = req.seed || (ref ? 1 : 0);
   const fwd = tf.buildForward(V, B, cfg);
   const params = ref ? tf.initParams(V, seed, cfg) : tf.initNormal(V, seed, 0.02, cfg);
-  const batch = (k) => (req.firstBatch && !k ? tf.encodeBatch(req.firstBatch, V, cfg.T, cfg.targets)
-    : tf.encodeBatch(randomTokens(B, cfg.T, V, seed * 1000 + (k || 0)), V, cfg.T, cfg.targets));
+  const batch = (k) => (req.firstBatch && !k ? tf.encodeBatch(req.firstBatch, V, cfg.T, cfg.targets, cfg.tokens)
+    : tf.encodeBatch(randomTokens(B, cfg.T, V, seed * 1000 + (k || 0)), V, cfg.T, cfg.targets, cfg.tokens));
   return { fwd, params, batch, info: { config: ref ? 'reference transformer' : 'C5', V, B, cfg } };
 }
 

@@ -19,6 +19,14 @@
 //   qkNorm: true          and normalised for each head, with gains b{l}.qg and b{l}.kg
 //   targets: 'classes'    y [B·T] holds class indices (-1: the row counts for nothing, the loss is still the
 //                         sum over B·T) and the loss is linearCrossEntropy: no logits are kept
+//   tokens: 'indices'     x [B·T] holds token indices (-1: padding, a row of zeros) and the embedding is Graph.embedding of
+//                         the same table, times embedScale (1): no one-hot rows
+//   attention: 'window'   Graph.windowAttention in place of scores, mask and softmax: no [T, T] values are kept, and each token sees
+//                         the last `window` tokens (default all) and the first `sinks` (0); kvHeads (H): key heads,
+//                         each shared by H / kvHeads query heads
+//   norms: 'joined'       Graph.residualNorm: each residual sum with the LayerNorm that follows it; postNorm: true also
+//                         normalises each branch (gains b{l}.pn1, b{l}.pn2), gates: true gates it for each channel (b{l}.g1, b{l}.g2, 1
+//                         at first), residual (1) scales the stream
 // and an optimizer { kind: 'muon', lr, momentum, adam }: momentum and orthogonalised updates for
 // the blocks' matrices, Adam for everything else.
 
@@ -42,10 +50,13 @@ function paramSpec(V, cfg) {
   if (cfg.positions !== 'rotary') spec.push(['pos', [T, d], ['uniform', 1]]);
   for (let l = 0; l < L; l++) {
     const p = `b${l}.`;
+    const keys = (cfg.kvHeads || cfg.H) * cfg.dh;
     if (cfg.qkNorm) spec.push([`${p}qg`, [cfg.dh], ['ones']], [`${p}kg`, [cfg.dh], ['ones']]);
+    if (cfg.postNorm) spec.push([`${p}pn1`, [d], ['ones']], [`${p}pn2`, [d], ['ones']]);
+    if (cfg.gates) spec.push([`${p}g1`, [d], ['ones']], [`${p}g2`, [d], ['ones']]);
     spec.push(
       [`${p}ln1.g`, [d], ['ones']], [`${p}ln1.b`, [d], ['zeros']],
-      [`${p}wq`, [d, d], linear(d)], [`${p}wk`, [d, d], linear(d)], [`${p}wv`, [d, d], linear(d)],
+      [`${p}wq`, [d, d], linear(d)], [`${p}wk`, [d, keys], linear(d)], [`${p}wv`, [d, keys], linear(d)],
       [`${p}wo`, [d, d], linear(d)], [`${p}bo`, [d], linear(d)],
       [`${p}ln2.g`, [d], ['ones']], [`${p}ln2.b`, [d], ['zeros']],
       [`${p}w1`, [d, ff], linear(d)], [`${p}b1`, [ff], linear(d)],
@@ -85,18 +96,35 @@ function causalMask(T, mask) {
   return m;
 }
 
+/** Options that only go with another. */
+function checkOptions(cfg) {
+  const windowed = cfg.attention === 'window', joined = cfg.norms === 'joined';
+  for (const k of ['window', 'sinks', 'kvHeads']) if (cfg[k] && !windowed) throw new Error(`the transformer's '${k}' takes attention: 'window'`);
+  for (const k of ['postNorm', 'gates', 'residual']) if (cfg[k] !== undefined && cfg[k] !== false && !joined) throw new Error(`the transformer's '${k}' takes norms: 'joined'`);
+  if (cfg.embedScale !== undefined && cfg.tokens !== 'indices') throw new Error("the transformer's 'embedScale' takes tokens: 'indices'");
+  for (const [k, v] of [['attention', 'window'], ['norms', 'joined'], ['tokens', 'indices']]) {
+    if (cfg[k] !== undefined && cfg[k] !== v) throw new Error(`the transformer's '${k}' is '${v}' or not given, not '${cfg[k]}'`);
+  }
+  if (cfg.kvHeads && cfg.H % cfg.kvHeads) throw new Error(`${cfg.kvHeads} key heads for ${cfg.H} query heads`);
+}
+
 function attention(g, a, p, B, cfg) {
-  const { T, d, H, dh } = cfg;
+  const { T, d, H, dh } = cfg, windowed = cfg.attention === 'window';
   // A head split, its rows normalised and rotated by the tokens' positions where the config says so.
   const rotated = cfg.positions === 'rotary' || cfg.qkNorm;
   const at = rotated ? g.const(Array.from({ length: T }, (_, t) => t), [T]) : null;
   const turn = (x, gain) => g.rotary(x, at, Object.assign({ eps: cfg.eps }, cfg.rotary || {}, cfg.positions === 'rotary' ? {} : { sections: [0] },
     { axis: 1, gain }));
   const heads = (w, gain) => {
-    const x = g.reshape(g.matmul(a, p[w]), [B, T, H, dh]);
-    return g.transpose(rotated && w !== 'wv' ? turn(x, gain) : x, [0, 2, 1, 3]);
+    const x = g.reshape(g.matmul(a, p[w]), [B, T, w === 'wq' ? H : cfg.kvHeads || H, dh]);
+    const y = rotated && w !== 'wv' ? turn(x, gain) : x;
+    return windowed ? y : g.transpose(y, [0, 2, 1, 3]);
   };
   const q = heads('wq', p.qg), k = heads('wk', p.kg), v = heads('wv');
+  if (windowed) {
+    const o = g.windowAttention(q, k, v, { queries: 'first', window: cfg.window, sinks: cfg.sinks });
+    return g.add(g.matmul(g.reshape(o, [B * T, d]), p.wo), p.bo);
+  }
   let s = g.matmul(q, g.transpose(k, [0, 1, 3, 2]));
   s = g.mul(s, g.const(1 / Math.sqrt(dh)));
   s = g.add(s, g.const(causalMask(T, cfg.mask), [T, T]));
@@ -112,14 +140,33 @@ const BLOCK_KEYS = ['ln1.g', 'ln1.b', 'wq', 'wk', 'wv', 'wo', 'bo', 'ln2.g', 'ln
 function hiddenOf(g, ids, B, cfg) {
   const { T, d, L } = cfg;
   const act = (x) => (cfg.act === 'relu' ? g.relu(x) : geluGraph(g, x));
-  let h = g.matmul(ids.x, ids.tok);
-  if (cfg.positions !== 'rotary') h = g.reshape(g.add(g.reshape(h, [B, T, d]), ids.pos), [B * T, d]);
-  for (let l = 0; l < L; l++) {
+  const keys = BLOCK_KEYS.concat(cfg.qkNorm ? ['qg', 'kg'] : [], cfg.postNorm ? ['pn1', 'pn2'] : [], cfg.gates ? ['g1', 'g2'] : []);
+  const block = (l) => {
     const p = {};
-    for (const k of cfg.qkNorm ? BLOCK_KEYS.concat(['qg', 'kg']) : BLOCK_KEYS) p[k] = ids[`b${l}.${k}`];
+    for (const k of keys) p[k] = ids[`b${l}.${k}`];
+    return p;
+  };
+  const mlp = (m, p) => g.add(g.matmul(act(g.add(g.matmul(m, p.w1), p.b1)), p.w2), p.b2);
+  let h = cfg.tokens === 'indices' ? g.embedding(ids.x, ids.tok, { scale: cfg.embedScale }) : g.matmul(ids.x, ids.tok);
+  if (cfg.positions !== 'rotary') h = g.reshape(g.add(g.reshape(h, [B, T, d]), ids.pos), [B * T, d]);
+  if (cfg.norms === 'joined') {
+    // A branch, and the norm of the stream that the next one reads.
+    const join = (x, branch, gain, bias, postGain, gate) => g.residualNorm(x, branch, { gain, bias, postGain, gate, residual: cfg.residual, norm: 'layer', eps: cfg.eps });
+    let n = L ? layerNormGraph(g, h, ids['b0.ln1.g'], ids['b0.ln1.b'], cfg.eps) : layerNormGraph(g, h, ids['lnf.g'], ids['lnf.b'], cfg.eps);
+    for (let l = 0; l < L; l++) {
+      const p = block(l), next = l + 1 < L ? `b${l + 1}.ln1` : 'lnf';
+      const a = join(h, attention(g, n, p, B, cfg), p['ln2.g'], p['ln2.b'], p.pn1, p.g1);
+      const m = join(a.h, mlp(a.n, p), ids[`${next}.g`], ids[`${next}.b`], p.pn2, p.g2);
+      h = m.h;
+      n = m.n;
+    }
+    return n;
+  }
+  for (let l = 0; l < L; l++) {
+    const p = block(l);
     h = g.add(h, attention(g, layerNormGraph(g, h, p['ln1.g'], p['ln1.b'], cfg.eps), p, B, cfg));
     const m = layerNormGraph(g, h, p['ln2.g'], p['ln2.b'], cfg.eps);
-    h = g.add(h, g.add(g.matmul(act(g.add(g.matmul(m, p.w1), p.b1)), p.w2), p.b2));
+    h = g.add(h, mlp(m, p));
   }
   return layerNormGraph(g, h, ids['lnf.g'], ids['lnf.b'], cfg.eps);
 }
@@ -136,10 +183,11 @@ function lossOf(g, logits, y, rows) {
 }
 
 function buildForward(V, B, cfg) {
+  checkOptions(cfg);
   const g = new Graph();
   const ids = {};
   for (const [name, shape] of paramSpec(V, cfg)) ids[name] = g.input(name, shape);
-  ids.x = g.input('x', [B * cfg.T, V]);
+  ids.x = g.input('x', cfg.tokens === 'indices' ? [B * cfg.T] : [B * cfg.T, V]);
   if (cfg.targets === 'classes') {
     const rows = B * cfg.T;
     ids.y = g.input('y', [rows]);
@@ -267,14 +315,15 @@ function buildStep(V, B, cfg, opt) {
 
 /**
  * One-hot x and y [B·T, V] for sequences of T + 1 tokens (m3b/data.js:62-72): targets are x[t+1].
- * With targets 'classes', y [B·T] holds the targets themselves.
+ * With targets 'classes', y [B·T] holds the targets themselves, and with tokens 'indices' x [B·T] the tokens.
  */
-function encodeBatch(seqs, V, T, targets) {
-  const classes = targets === 'classes';
-  const x = new Float32Array(seqs.length * T * V), y = new Float32Array(seqs.length * T * (classes ? 1 : V));
+function encodeBatch(seqs, V, T, targets, tokens) {
+  const classes = targets === 'classes', indices = tokens === 'indices';
+  const x = new Float32Array(seqs.length * T * (indices ? 1 : V)), y = new Float32Array(seqs.length * T * (classes ? 1 : V));
   seqs.forEach((s, b) => {
     for (let t = 0; t < T; t++) {
-      x[(b * T + t) * V + s[t]] = 1;
+      if (indices) x[b * T + t] = s[t];
+      else x[(b * T + t) * V + s[t]] = 1;
       if (classes) y[b * T + t] = s[t + 1];
       else y[(b * T + t) * V + s[t + 1]] = 1;
     }
