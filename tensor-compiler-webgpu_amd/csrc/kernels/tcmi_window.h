@@ -4,7 +4,9 @@
 // s_j = scale·q·k_j over those:
 //   o = sum_j P_j v_j,  P_j = exp(s_j - lse),  lse = log(sum_j exp(s_j));
 //   dS_j = P_j·(dy·v_j - dy·o),  dq = scale·sum_j dS_j k_j,  dk_j = scale·sum dS_j q,  dv_j = sum P_j dy (over the queries that see j).
-// A query that sees nothing has o = 0, lse = -inf and no gradients.
+// A query that sees nothing has o = 0, lse = -inf and no gradients. A key whose key or value holds a number that is not finite makes
+// NaN of o and lse of the queries that see it, and a query's row with one (dy's too) of the gradients of the keys it sees; what does not
+// see them, or is not seen, is as without them: 0 times them is taken as 0 (they are read as 0 where a sum runs over them).
 //
 // Rows: the queries of the R = H/HK heads that share a key head, query t's heads side by side, 16 rows a tile; keys 16 a
 // tile. With lane = 16·q + t (t in 0..15) of a 16x16x4 product:
@@ -90,29 +92,46 @@ __device__ __forceinline__ void window_store(float* __restrict__ p, uint32_t d, 
   }
 }
 
+// x, or 0 where it is not finite.
+__device__ __forceinline__ float window_finite(float x) { return __builtin_isfinite(x) ? x : 0.f; }
+
 // Lane (t, q)'s part of a 16 x DH tile along its rows: dims 16g + 4q ... of row t.
 template <class S, int G>
 __device__ __forceinline__ void window_along(f4 (&v)[G], const float* __restrict__ row, bool on) {
 #pragma unroll
   for (int g = 0; g < G; ++g) v[g] = window_load<S>(row, 16 * g + 4 * ((threadIdx.x >> 4) & 3u), on);
 }
-// And across them: dim 16g + t of the tile's key 4q + s, of the keys from j0 on those that one of the rows sees (a value that
-// no query sees may be anything: it is 0 here, for 0 times it would be NaN). Every load is made, of the last such key where its own is past it.
+// And across them: dim 16g + t of the tile's key 4q + s, of the keys from j0 on. Every load is made, of the last key that one of the rows
+// sees where its own is past it.
 template <class S, int G>
-__device__ __forceinline__ void window_across(f4 (&v)[G], const float* __restrict__ base, size_t step, int32_t j0, const WindowTiles& tiles) {
+__device__ __forceinline__ void window_read(f4 (&v)[G], const float* __restrict__ base, size_t step, int32_t j0, const WindowTiles& tiles) {
   const int t = threadIdx.x & 15, q = (threadIdx.x >> 4) & 3;
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+    const float* at = base + (size_t)min(j0 + 4 * q + s, tiles.hi) * step + t;
+#pragma unroll
+    for (int g = 0; g < G; ++g) v[g][s] = at[16 * g + 16 <= static_cast<int>(S::DH) || 16 * g + t < static_cast<int>(S::DH) ? 16 * g : 0 - t];
+  }
+}
+// What was read, 0 where it is not finite or of a key that none of the rows sees. Bit s: key 4q + s held a number that is not finite.
+template <class S, int G>
+__device__ __forceinline__ uint32_t window_clean(f4 (&v)[G], int32_t j0, const WindowTiles& tiles) {
+  const int t = threadIdx.x & 15, q = (threadIdx.x >> 4) & 3;
+  uint32_t bad = 0u;
 #pragma unroll
   for (int s = 0; s < 4; ++s) {
     const int32_t j = j0 + 4 * q + s;
     const bool on = j <= tiles.hi && (j >= tiles.lo || j < static_cast<int32_t>(S::SINKS));
-    const float* at = base + (size_t)min(j, tiles.hi) * step + t;
+    bool all = true;
 #pragma unroll
     for (int g = 0; g < G; ++g) {
-      const bool in = 16 * g + 16 <= static_cast<int>(S::DH) || 16 * g + t < static_cast<int>(S::DH);
-      const float x = at[in ? 16 * g : 0 - t];
-      v[g][s] = on && in ? x : 0.f;
+      const bool in = on && (16 * g + 16 <= static_cast<int>(S::DH) || 16 * g + t < static_cast<int>(S::DH)), finite = __builtin_isfinite(v[g][s]);
+      all = all && (finite || !in);
+      v[g][s] = in && finite ? v[g][s] : 0.f;
     }
+    if ((__ballot(!all) >> (threadIdx.x & 48u)) & 0xffffu) bad |= 1u << s;
   }
+  return bad;
 }
 // acc[k of a][t of b] += the products of two tiles along their rows.
 template <int G>
@@ -181,7 +200,7 @@ __device__ __forceinline__ void window_rows(const float* __restrict__ qp, const 
   auto load = [&](int32_t i, f4 (&kf)[G], f4 (&vf)[G]) __attribute__((always_inline)) {
     const int32_t j0 = tiles.at(i) * 16;
     window_along<S>(kf, kb + (size_t)min(j0 + t, tiles.hi) * step, true);
-    window_across<S>(vf, vb, step, j0, tiles);
+    window_read<S>(vf, vb, step, j0, tiles);
   };
   f4 kf[G], vf[G], kn[G], vn[G];
   if (begin + wave < end) load(begin + wave, kn, vn);
@@ -194,11 +213,12 @@ __device__ __forceinline__ void window_rows(const float* __restrict__ qp, const 
     }
     if (G <= 8 && i + 4 < end) load(i + 4, kn, vn);
     __builtin_amdgcn_sched_barrier(0);
+    const uint32_t bad = window_clean<S>(vf, j0, tiles);
     f4 s = window_scores(kf, qf);
     float top = -TCMI_INF;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      s[r] = on && w.sees(p, j0 + 4 * q + r) ? s[r] * scale : -TCMI_INF;
+      s[r] = on && w.sees(p, j0 + 4 * q + r) ? (bad >> r & 1u ? __builtin_nanf("") : s[r] * scale) : -TCMI_INF;
       top = fmaxf(top, s[r]);
     }
     top = fmaxf(m, quad16_reduce<true>(top));
@@ -346,7 +366,8 @@ __device__ __forceinline__ void window_dq(const WindowGradArgs a, float* __restr
     f4 s = window_scores(f, qf);
     window_along<S>(f, a.v + base + (size_t)min(j0 + t, w.length - 1) * step, j0 + t < w.length);
     const f4 dp = window_scores(f, df);
-    window_across<S>(f, a.k + base, step, j0, tiles);
+    window_read<S>(f, a.k + base, step, j0, tiles);
+    window_clean<S>(f, j0, tiles);
 #pragma unroll
     for (int r = 0; r < 4; ++r) s[r] = on && w.sees(p, j0 + 4 * q + r) ? __builtin_amdgcn_exp2f(fmaf(s[r], scale, -lse)) * (dp[r] - mass) : 0.f;
     window_sum(acc, f, s);
@@ -396,19 +417,23 @@ __device__ __forceinline__ void window_dkv(const WindowGradArgs a, float* __rest
     // Rows 4q ... of this lane.
     size_t at[4];
     bool in[4];
+    float mass[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int32_t row = r0 + 4 * q + r;
       at[r] = line(min(row, ROWS - 1));
       const int32_t p = w.first + row / R;
       in[r] = row < ROWS && p >= p0 && p <= p1;
-      s[r] = in[r] && j < w.length && w.sees(p, j) ? __builtin_amdgcn_exp2f(fmaf(s[r], scale, -LOG2E * a.lse[at[r]])) : 0.f;
+      mass[r] = in[r] ? a.mass[at[r]] : 0.f;
+      // (NaN where q or dy hold a number that is not finite.)
+      const float lse = in[r] ? LOG2E * a.lse[at[r]] + 0.f * mass[r] : 0.f;
+      s[r] = in[r] && j < w.length && w.sees(p, j) ? __builtin_amdgcn_exp2f(fmaf(s[r], scale, -lse)) : 0.f;
     }
     if constexpr (DV) {
 #pragma unroll
       for (int g = 0; g < G; ++g) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) x[g][r] = in[r] && 16 * g + t < static_cast<int>(S::DH) ? a.dy[at[r] * S::DH + 16 * g + t] : 0.f;
+        for (int r = 0; r < 4; ++r) x[g][r] = window_finite(in[r] && 16 * g + t < static_cast<int>(S::DH) ? a.dy[at[r] * S::DH + 16 * g + t] : 0.f);
       }
       window_sum(dva, x, s);
     }
@@ -416,10 +441,10 @@ __device__ __forceinline__ void window_dkv(const WindowGradArgs a, float* __rest
 #pragma unroll
       for (int g = 0; g < G; ++g) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) x[g][r] = in[r] && 16 * g + t < static_cast<int>(S::DH) ? a.q[at[r] * S::DH + 16 * g + t] : 0.f;
+        for (int r = 0; r < 4; ++r) x[g][r] = window_finite(in[r] && 16 * g + t < static_cast<int>(S::DH) ? a.q[at[r] * S::DH + 16 * g + t] : 0.f);
       }
 #pragma unroll
-      for (int r = 0; r < 4; ++r) s[r] = s[r] != 0.f ? s[r] * (dp[r] - a.mass[at[r]]) : 0.f;
+      for (int r = 0; r < 4; ++r) s[r] = s[r] != 0.f ? s[r] * (dp[r] - mass[r]) : 0.f;
       window_sum(dka, x, s);
     }
   }

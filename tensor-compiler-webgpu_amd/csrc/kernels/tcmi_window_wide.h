@@ -1,7 +1,8 @@
 // Attention over a sliding window (tcmi_window.h's formulas) for many rows, on the bf16 matrix cores: every operand as three
 // bf16 parts, x = x0 + x1 + x2, and every product as the six of a_i·b_j with i + j <= 2, in float32 (what is left
 // out: 2^-24 of a product at most). No operand needs a scale, so a key or value of any size is what it is to the queries that see it and
-// nothing to the others; parts below bf16's least normal number, of values below 2^-102, are lost.
+// nothing to the others; parts below bf16's least normal number, of values below 2^-102, are lost, and values from 2^128 - 2^119 on, which
+// bf16 rounds to infinity, count as infinite.
 //
 // A workgroup's four wavefronts take 32 rows each (tcmi_window.h's rows: the queries of the heads that share a key head) and walk
 // the tiles of NB keys that one of the 128 sees. A tile is loaded one ahead into registers, split by the thread that loaded it and
@@ -82,10 +83,25 @@ struct WindowTile {
       x[i] = window_load<S>(p, dim(i), p != nullptr);
     }
   }
-  __device__ __forceinline__ void store(char* tile, const Minus& minus) const {
+  // CLEAN: what is not finite as 0, with bad[line] (if there is one) and *some set for its line.
+  template <bool CLEAN>
+  __device__ __forceinline__ void store(char* tile, const Minus& minus, uint32_t* bad = nullptr, uint32_t* some = nullptr) const {
 #pragma unroll
     for (int i = 0; i < CHUNKS; ++i) {
       float u[4] = {x[i][0], x[i][1], x[i][2], x[i][3]};
+      if constexpr (CLEAN) {
+        bool all = true;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const bool finite = fabsf(u[e]) < 0x1.ffp127f;
+          all = all && finite;
+          u[e] = finite ? u[e] : 0.f;
+        }
+        if (bad != nullptr && !all) {
+          bad[line(i)] = 1u;
+          *some = 1u;
+        }
+      }
       char* to = tile + line(i) * LD + (((dim(i) >> 3) ^ swap(line(i))) << 4) + (dim(i) & 4) * 2;
 #pragma unroll
       for (int p = 0; p < 3; ++p) {
@@ -136,7 +152,7 @@ struct WindowWide {
   static constexpr int HB = S::HB;                     // blocks of 16 rows of a wavefront
   static constexpr uint32_t ROWS = 64 * HB;            // of a workgroup
   using T = WindowTile<S, NB>;
-  static constexpr int LDS = 2 * T::BYTES;
+  static constexpr int LDS = 2 * T::BYTES + (NB + 4) * 4;
 };
 
 // The `split`-th of SPLITS runs of n.
@@ -196,6 +212,7 @@ __device__ __forceinline__ void window_wide(const float* __restrict__ qp, const 
   using T = typename W::T;
   T x;                                   // K's next tile, or V's: never both at once
   char *klds = lds, *vlds = lds + T::BYTES;
+  uint32_t *bad = reinterpret_cast<uint32_t*>(lds + 2 * T::BYTES), *some_bad = bad + NB;      // values of the tile that are not finite
   auto load = [&](const float* p, int32_t i) __attribute__((always_inline)) {
     const int32_t j0 = tiles.at(i) * NB;
     x.load([&](int line) -> const float* {
@@ -259,7 +276,8 @@ __device__ __forceinline__ void window_wide(const float* __restrict__ qp, const 
   for (int32_t i = begin; i < end; ++i) {
     const int32_t j0 = tiles.at(i) * NB;
     __syncthreads();
-    x.store(klds, minus);
+    x.template store<false>(klds, minus);
+    if (threadIdx.x <= NB) bad[threadIdx.x] = 0u;
     load(vp, i);
     __syncthreads();
     // (What none of the wavefront's rows sees: past its last position, or between its sinks and its windows.)
@@ -268,10 +286,19 @@ __device__ __forceinline__ void window_wide(const float* __restrict__ qp, const 
     float alpha[HB];
     Parts pf[HB][BLOCKS / 2];
     if (some) scores(j0, whole, alpha, pf);
-    x.store(vlds, minus);
+    x.template store<true>(vlds, minus, bad, some_bad);
     __syncthreads();
     if (i + 1 < end) load(kp, i + 1);
     if (!some) continue;
+    if (*some_bad) {
+#pragma unroll
+      for (int h = 0; h < HB; ++h) {
+        for (int k = 0; k < BLOCKS * 4; ++k) {
+          const int at = k / 4 * 16 + 4 * q + k % 4;
+          if (bad[at] && on[h] && w.sees(pos[h], j0 + at)) l[h] = __builtin_nanf("");
+        }
+      }
+    }
 #pragma unroll
     for (int g = 0; g < G; g += 2) {
       f4 sum[HB][2];
@@ -464,8 +491,8 @@ __device__ __forceinline__ void window_wide_dq(const WindowGradArgs a, float* __
   for (int32_t i = begin; i < end; ++i) {
     const int32_t j0 = tiles.at(i) * NB;
     __syncthreads();
-    kt.store(klds, minus);
-    vt.store(vlds, minus);
+    kt.template store<true>(klds, minus);
+    vt.template store<false>(vlds, minus);
     __syncthreads();
     if (i + 1 < end) load(i + 1);
     if (j0 > p1 || (j0 + NB <= w.from(p0) && j0 >= static_cast<int32_t>(S::SINKS))) continue;
@@ -604,15 +631,16 @@ __device__ __forceinline__ void window_wide_dkv(const WindowGradArgs a, float* _
       row_at = w.first + r / R;
       const bool on = r < ROWS && row_at >= p0 && row_at <= p1;
       if (!on) row_at = -1;
-      stats[0] = on ? a.lse[place(r)] * LOG2E : 0.f;
-      stats[1] = on && DK ? a.mass[place(r)] : 0.f;
+      // (NaN where q or dy hold a number that is not finite.)
+      stats[1] = on ? a.mass[place(r)] : 0.f;
+      stats[0] = on ? a.lse[place(r)] * LOG2E + 0.f * stats[1] : 0.f;
     }
   };
   if (begin < end) load(begin);
   for (int32_t i = begin; i < end; ++i) {
     __syncthreads();
-    qt.store(qlds, minus);
-    dt.store(dlds, minus);
+    qt.template store<true>(qlds, minus);
+    dt.template store<true>(dlds, minus);
     if (threadIdx.x < NB) {
       row_lse[threadIdx.x] = stats[0];
       row_mass[threadIdx.x] = stats[1];
@@ -651,7 +679,7 @@ __device__ __forceinline__ void window_wide_dkv(const WindowGradArgs a, float* _
 #pragma unroll
         for (int h = 0; h < HB; ++h) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r) s[h][k][r] = s[h][k][r] != 0.f ? s[h][k][r] * (dp[h][k][r] - ms[r]) : 0.f;
+          for (int r = 0; r < 4; ++r) s[h][k][r] = whole || s[h][k][r] != 0.f ? s[h][k][r] * (dp[h][k][r] - ms[r]) : 0.f;
         }
       }
 #pragma unroll

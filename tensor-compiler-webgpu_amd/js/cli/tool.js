@@ -285,6 +285,20 @@ function precompileGroup(group, arch, shard, shards) {
       const fs = fusedStep(modelStep({ model: 'transformer', B: 5, V: 301, opt: 'muon', cfg }).step, { attention });
       n += precompile([fs.lowered], arch) + precompile([fs.checked], arch);
     }
+    const context = { d: 64, H: 4, dh: 16, L: 2, ff: 160, tokens: 'indices', targets: 'classes', positions: 'rotary', qkNorm: true, attention: 'window', sinks: 2, kvHeads: 2,
+      norms: 'joined', postNorm: true, gates: true, residual: 0.9, embedScale: 8 };
+    const steps = [{ T: 32, window: 9 }, { T: 300, window: 270 }].map((c) => Object.assign(c, context));
+    [{ B: 3, V: 301, opt: 'muon', cfg: steps[0] }, { B: 3, V: 301, opt: 'muon', cfg: steps[1] }, { B: 2, V: 150, opt: 'adam', cfg: steps[0] }, { B: 2, V: 150, opt: 'adam', cfg: steps[1] }].forEach((r, k) => {
+      if ((shard || 0) !== (k + 2) % (shards || 1)) return;
+      const { step } = modelStep(Object.assign({ model: 'transformer' }, r));
+      if (r.opt === 'muon') {
+        const fs = fusedStep(step);
+        n += precompile([fs.lowered], arch) + precompile([fs.checked], arch);
+      } else {
+        const keep = [step.loss].concat(Object.values(step.outputs)), f = fuse(step.graph, { keep });
+        n += precompile([lowerMI355X(f.graph)], arch) + precompile([lowerMI355X(f.graph, { perf: true, keep: keep.map((id) => f.index.get(id)) })], arch);
+      }
+    });
     return n;
   }
   if (group === 'scratch') {

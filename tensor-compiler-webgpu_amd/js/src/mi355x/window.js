@@ -22,7 +22,7 @@ struct ${S} {
 ${constants(Object.assign({}, s.z, more || {}), types)}
   static __device__ __forceinline__ double scale() { return ${double(s.scale)}; }
 };
-extern "C" __global__ void __launch_bounds__(${threads}${/_(wide|packed)(_dq|_dkv)?</.test(call) && s.z.DH <= 128 ? ', 2' : ''}) __KERNEL__(${e.sig}) {
+extern "C" __global__ void __launch_bounds__(${threads}${/_packed(_dq|_dkv)?</.test(call) || (/_wide(_dq|_dkv)?</.test(call) && s.z.DH <= 64) ? ', 2' : ''}) __KERNEL__(${e.sig}) {
 ${e.open}${lds ? `  __shared__ __attribute__((aligned(16))) ${lds};\n` : ''}  tcmi::${call};
 }
 `, grid, threads);
@@ -176,7 +176,7 @@ function backwardKernels(s, parts, joined) {
   const place = (name, bytes) => { more[name] = at; types[name] = 'size_t'; at = align(at + bytes, 256); };
   const m = maker(s, e, types), ws = `reinterpret_cast<char*>(${e.ws})`;
   const kernels = [];
-  if (!wide && (dk || dq)) kernels.push(m('winmass', grid(ceil(z.B * z.T * z.H, 16)), 256, null, `window_mass<${S}>(A.in[${first}], A.in[${first + 2}], ${e.ws}, blockIdx.x * 16u + threadIdx.x / 16u)`));
+  if (!wide) kernels.push(m('winmass', grid(ceil(z.B * z.T * z.H, 16)), 256, null, `window_mass<${S}>(A.in[${first}], A.in[${first + 2}], ${e.ws}, blockIdx.x * 16u + threadIdx.x / 16u)`));
   if (!wide) {
     const TILES = ceil(z.T * R, 16), KTILES = ceil(z.KEYS, 16), lds = `float lds[tcmi::window_lds<${z.DH}>()]`;
     if (dq) kernels.push(m('windq', grid(TILES * heads), 256, lds, `window_dq<${S}>(${args}, ${out('dq')}, lds, blockIdx.x)`, { TILES }));
@@ -199,7 +199,7 @@ function backwardKernels(s, parts, joined) {
     kernels.push(m('winpack', grid(keys + ceil(heads * RP, 256 / lanes)), 256, null,
       `window_pack_both<${S}, ${dq}, ${dk || dv}, ${keys}u>(${args}, ${ws}, blockIdx.x, ${place256(0)}, ${place256(keys)})`, Object.assign({ VSUMS: 0 }, more)));
   }
-  if (!packed && dk && !dq) {
+  if (!packed && !dq) {
     kernels.push(m('winmass', grid(ceil(z.B * z.T * z.H, 64)), 256, null, `window_wide_mass<${S}>(A.in[${first}], A.in[${first + 2}], ${e.ws}, blockIdx.x * 64u + threadIdx.x / 64u * 16u)`));
   }
   if (dq) {
