@@ -10,6 +10,9 @@
 // chunk that it starts in. So the order of a sum is given by the tokens alone. Rows without a token are found by a
 // search for each and written as zeros.
 //
+// A table of few rows takes no sort: a wavefront adds its rows of dy in their order into a table of its own in LDS, a lane a column, and the
+// wavefronts' and then the workgroups' tables are added in order.
+//
 // A pass of the sort, a tile of keys a workgroup: a key's place is the count of smaller digits, of
 // its digit in the tiles before, in the wavefronts before and among the lanes before it (found by comparing digits bit by bit
 // over the wavefront). The tiles are counted by a launch before each pass; a few keys are one tile, and one launch makes all passes.
@@ -351,6 +354,74 @@ __device__ __forceinline__ void embed_join(float* __restrict__ out, char* ws, fl
     for (uint32_t e = 0; e < S::E; ++e) sum[e] += lds[(w * S::E + e) * 64u + lane];
   }
   embed_store<S::E>(out + (size_t)key * S::D + c, sum * S::scale());
+}
+
+// A table of few rows: workgroup `chunk` of CHUNKS adds CH rows of dy, a quarter a wavefront, 64 columns from 64·`block` on. lds: 4·V·64 floats.
+template <class S>
+__device__ __forceinline__ void embed_few(const float* __restrict__ tokens, const float* __restrict__ dy, float* __restrict__ out, float* __restrict__ parts, float* lds, uint32_t chunk, uint32_t block) {
+  const uint32_t lane = threadIdx.x % 64u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64u), c = block * 64u + lane;
+  float* const own = lds + wave * S::V * 64u;
+  constexpr uint32_t RUN = S::CH / 4u, HELD = 32u;
+  const uint32_t begin = min(static_cast<uint32_t>(S::N), chunk * S::CH + wave * RUN), end = min(static_cast<uint32_t>(S::N), begin + RUN);
+  for (uint32_t i = begin; i < end; i += HELD) {
+    // (Every load is made, of the run's last row and the table's last column where its own is past them.)
+    float x[HELD];
+    const float token = tokens[min(i + lane % HELD, end - 1u)];
+#pragma unroll
+    for (uint32_t u = 0; u < HELD; ++u) x[u] = dy[(size_t)min(i + u, end - 1u) * S::D + min(c, S::D - 1u)];
+    const int32_t mine = i + lane % HELD < end ? embed_key(token, S::V) : -1;
+    if (i == begin) {
+      // (While the first rows are on their way.)
+      for (uint32_t v = lane; v < S::V * 16u; v += 64u) reinterpret_cast<f4*>(own)[v] = f4{0.f, 0.f, 0.f, 0.f};
+      embed_step();
+    }
+#pragma unroll
+    for (uint32_t u = 0; u < HELD; ++u) {
+      const int32_t key = __builtin_amdgcn_readlane(mine, u);
+      if (key >= 0) own[key * 64 + lane] += x[u];
+    }
+  }
+  if (begin >= end) {
+    for (uint32_t v = lane; v < S::V * 16u; v += 64u) reinterpret_cast<f4*>(own)[v] = f4{0.f, 0.f, 0.f, 0.f};
+  }
+  __syncthreads();
+  float* const to = S::CHUNKS > 1u ? parts + (size_t)chunk * S::V * S::D : out;
+#pragma unroll 8
+  for (uint32_t v = wave; v < S::V; v += 4u) {
+    float sum = lds[v * 64u + lane];
+#pragma unroll
+    for (uint32_t w = 1; w < 4u; ++w) sum += lds[(w * S::V + v) * 64u + lane];
+    if (c < S::D) to[(size_t)v * S::D + c] = S::CHUNKS > 1u ? sum : sum * S::scale();
+  }
+}
+
+// Its chunks' tables: a workgroup takes 16 groups of four floats, 16 threads a group, each its own chunks in turn. lds: 1024 floats.
+template <class S>
+__device__ __forceinline__ void embed_fold(float* __restrict__ out, const float* __restrict__ parts, float* lds, uint32_t block) {
+  constexpr size_t ALL = (size_t)S::V * S::D;
+  const uint32_t part = threadIdx.x / 16u;
+  const size_t at = ((size_t)block * 16u + threadIdx.x % 16u) * 4u;
+  f4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+  for (uint32_t k = part; k < S::CHUNKS; k += 16u) {
+    if constexpr (ALL % 4u == 0u) {
+      if (at < ALL) sum += *reinterpret_cast<const f4*>(parts + k * ALL + at);
+    } else {
+#pragma unroll
+      for (uint32_t e = 0; e < 4u; ++e) sum[e] += at + e < ALL ? parts[k * ALL + at + e] : 0.f;
+    }
+  }
+  f4* all = reinterpret_cast<f4*>(lds);
+  all[threadIdx.x] = sum;
+  __syncthreads();
+  if (part != 0u) return;
+#pragma unroll
+  for (uint32_t p = 1; p < 16u; ++p) sum += all[p * 16u + threadIdx.x];
+  sum *= S::scale();
+#pragma unroll
+  for (uint32_t e = 0; e < 4u; ++e) {
+    if (at + e < ALL) out[at + e] = sum[e];
+  }
 }
 
 }  // namespace tcmi

@@ -67,6 +67,26 @@ struct ResidualLane {
       }
     }
   }
+  // A vector of a row's floats, kept in LDS as the lanes hold it (STAGED), or read from memory.
+  static constexpr uint32_t PAD = S::UNITS * 4 * S::LANES;
+  __device__ __forceinline__ void keep(const float* __restrict__ p, float* to) const {
+    Row v;
+    load(p, v);
+#pragma unroll
+    for (int u = 0; u < F; u += 4) *reinterpret_cast<f4*>(to + dim(u)) = f4{v[u], v[u + 1], v[u + 2], v[u + 3]};
+  }
+  __device__ __forceinline__ void kept(const float* __restrict__ p, const float* from, Row& v) const {
+    if constexpr (S::STAGED) {
+#pragma unroll
+      for (int u = 0; u < F; u += 4) {
+        const f4 q = *reinterpret_cast<const f4*>(from + dim(u));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[u + e] = q[e];
+      }
+    } else {
+      load(p, v);
+    }
+  }
   // Sums over the row's lanes, every lane getting them; over several wavefronts through LDS.
   template <int N>
   __device__ __forceinline__ void total(float (&v)[N]) const {
@@ -130,26 +150,25 @@ struct ResidualLane {
 
 // A gate's floats of row `row`.
 template <class S>
-__device__ __forceinline__ void residual_gate(const ResidualLane<S>& l, const ResidualArgs& a, uint32_t row, typename ResidualLane<S>::Row& g) {
-  l.load(S::GATE == 2 ? a.gate + (size_t)row * S::D : a.gate, g);
+__device__ __forceinline__ void residual_gate(const ResidualLane<S>& l, const ResidualArgs& a, uint32_t row, const float* vectors, typename ResidualLane<S>::Row& g) {
+  if constexpr (S::GATE == 2) l.load(a.gate + (size_t)row * S::D, g);
+  else l.kept(a.gate, vectors + 3 * ResidualLane<S>::PAD, g);
 }
 
-// p = N(y) and h of one row; yh: y normalised (where it has a norm), with its r; gate.
+// p = N(y) and h of one row; yh: y, then y normalised (where it has a norm), whose r is returned; h: x, then h.
 template <class S>
 __device__ __forceinline__ float residual_join(const ResidualLane<S>& l, const ResidualArgs& a, uint32_t row, typename ResidualLane<S>::Row& yh,
-                                               typename ResidualLane<S>::Row& p, typename ResidualLane<S>::Row& h) {
+                                               typename ResidualLane<S>::Row& p, typename ResidualLane<S>::Row& h, const float* vectors) {
   using L = ResidualLane<S>;
-  l.load(a.y + (size_t)row * S::D, yh);
-  l.load(a.x + (size_t)row * S::D, h);
   float r = 1.f;
   if constexpr (S::POST) {
     r = l.normalise(yh);
     typename L::Row g;
-    l.load(a.postGain, g);
+    l.kept(a.postGain, vectors + L::PAD, g);
 #pragma unroll
     for (int i = 0; i < L::F; ++i) p[i] = yh[i] * g[i];
     if (a.postBias != nullptr) {
-      l.load(a.postBias, g);
+      l.kept(a.postBias, vectors + 2 * L::PAD, g);
 #pragma unroll
       for (int i = 0; i < L::F; ++i) p[i] += g[i];
     }
@@ -159,7 +178,7 @@ __device__ __forceinline__ float residual_join(const ResidualLane<S>& l, const R
   }
   if constexpr (S::GATE != 0) {
     typename L::Row g;
-    residual_gate(l, a, row, g);
+    residual_gate(l, a, row, vectors, g);
 #pragma unroll
     for (int i = 0; i < L::F; ++i) h[i] = fmaf(S::residual(), h[i], g[i] * p[i]);
   } else {
@@ -179,7 +198,9 @@ __device__ __forceinline__ void residual(const ResidualArgs& a, float* __restric
     // (Every lane takes part in the sums: a row past the last is the last again, and not written.)
     const uint32_t at = row0 + threadIdx.x / S::LANES, row = min(at, S::N - 1u);
     typename L::Row yh, p, h;
-    residual_join<S>(l, a, row, yh, p, h);
+    l.load(a.y + (size_t)row * S::D, yh);
+    l.load(a.x + (size_t)row * S::D, h);
+    residual_join<S>(l, a, row, yh, p, h, nullptr);
     if (S::H && at < S::N) l.store(hout + (size_t)row * S::D, h);
     if constexpr (S::NORM) {
       l.normalise(h);
@@ -197,7 +218,8 @@ __device__ __forceinline__ void residual(const ResidualArgs& a, float* __restric
   }
 }
 
-// DX ... DGATE: the gradients to form; DH, DN: which cotangents there are. partial: the SUMS vectors' sums of each
+// DX ... DGATE: the gradients to form; DH, DN: which cotangents there are; STAGED: gain, postGain, postBias and a gate of one
+// vector are kept in LDS, from lds + SCRATCH on. partial: the SUMS vectors' sums of each
 // workgroup, [SUMS][blocks][D]; lds: ROWS·D floats where rows stand side by side.
 template <class S>
 __device__ __forceinline__ void residual_grad(const ResidualArgs& a, float* __restrict__ dx, float* __restrict__ dy, float* __restrict__ dgate,
@@ -206,6 +228,16 @@ __device__ __forceinline__ void residual_grad(const ResidualArgs& a, float* __re
   constexpr uint32_t ROWS = S::THREADS / S::LANES;
   constexpr bool BRANCH = S::DY || S::DPOSTGAIN || S::DPOSTBIAS || S::DGATE;
   const L l{threadIdx.x % S::LANES, lds};
+  // The vectors, which every row waits for (8189 rows of 4095 floats 180 us where they come from memory for each).
+  float* const vectors = lds + S::SCRATCH;
+  if constexpr (S::STAGED) {
+    const float* from[4] = {a.gain, a.postGain, a.postBias, S::GATE == 1 ? a.gate : nullptr};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (from[k] != nullptr && threadIdx.x < S::LANES) l.keep(from[k], vectors + k * L::PAD);
+    }
+    __syncthreads();
+  }
   float sums[S::SUMS > 0 ? S::SUMS : 1][L::F];
 #pragma unroll
   for (int k = 0; k < S::SUMS; ++k) {
@@ -215,8 +247,14 @@ __device__ __forceinline__ void residual_grad(const ResidualArgs& a, float* __re
   for (uint32_t row0 = block * ROWS; row0 < S::N; row0 += blocks * ROWS) {
     const uint32_t at = row0 + threadIdx.x / S::LANES, row = min(at, S::N - 1u);
     const bool on = at < S::N;
-    typename L::Row yh, p, h, d;
-    const float ry = residual_join<S>(l, a, row, yh, p, h);
+    // All that is read of the row, before any of it is used.
+    typename L::Row yh, p, h, d, dh;
+    l.load(a.y + (size_t)row * S::D, yh);
+    l.load(a.x + (size_t)row * S::D, h);
+    if constexpr (S::DN) l.load(a.dn + (size_t)row * S::D, d);
+    if constexpr (S::DH && (S::DX || BRANCH)) l.load(a.dh + (size_t)row * S::D, dh);
+    __builtin_amdgcn_sched_barrier(0);
+    const float ry = residual_join<S>(l, a, row, yh, p, h, vectors);
     int k = 0;
     // What a sum adds of a row past the last: nothing.
     auto add = [&](float (&sum)[L::F], auto f) __attribute__((always_inline)) {
@@ -224,13 +262,12 @@ __device__ __forceinline__ void residual_grad(const ResidualArgs& a, float* __re
       for (int i = 0; i < L::F; ++i) sum[i] += on ? f(i) : 0.f;
     };
     if constexpr (S::DN) {
-      l.load(a.dn + (size_t)row * S::D, d);
       const float rh = l.normalise(h);
       if constexpr (S::DGAIN) add(sums[k++], [&](int i) { return d[i] * h[i]; });
       if constexpr (S::DBIAS) add(sums[k++], [&](int i) { return d[i]; });
       if constexpr (S::DX || BRANCH) {
         typename L::Row g;
-        l.load(a.gain, g);
+        l.kept(a.gain, vectors, g);
 #pragma unroll
         for (int i = 0; i < L::F; ++i) d[i] *= g[i];
         l.back(d, h, rh);
@@ -240,10 +277,8 @@ __device__ __forceinline__ void residual_grad(const ResidualArgs& a, float* __re
       for (int i = 0; i < L::F; ++i) d[i] = 0.f;
     }
     if constexpr (S::DH && (S::DX || BRANCH)) {
-      typename L::Row g;
-      l.load(a.dh + (size_t)row * S::D, g);
 #pragma unroll
-      for (int i = 0; i < L::F; ++i) d[i] += g[i];
+      for (int i = 0; i < L::F; ++i) d[i] += dh[i];
     }
     if constexpr (S::DX) {
       typename L::Row g;
@@ -261,7 +296,7 @@ __device__ __forceinline__ void residual_grad(const ResidualArgs& a, float* __re
           }
         }
         typename L::Row g;
-        residual_gate(l, a, row, g);
+        residual_gate(l, a, row, vectors, g);
 #pragma unroll
         for (int i = 0; i < L::F; ++i) d[i] *= g[i];
       }
@@ -271,7 +306,7 @@ __device__ __forceinline__ void residual_grad(const ResidualArgs& a, float* __re
       if constexpr (S::DY) {
         if constexpr (S::POST) {
           typename L::Row g;
-          l.load(a.postGain, g);
+          l.kept(a.postGain, vectors + L::PAD, g);
 #pragma unroll
           for (int i = 0; i < L::F; ++i) d[i] *= g[i];
           l.back(d, yh, ry);
@@ -299,27 +334,29 @@ __device__ __forceinline__ void residual_grad(const ResidualArgs& a, float* __re
   }
 }
 
-// out[e] = the sum of vector `which`'s `blocks` partial rows: a workgroup of 1024 takes 16 columns, 64 threads a
-// column, each its own rows in turn, their sums added in order by eights.
-template <uint32_t D, int SUMS>
+// out[e] = the sum of vector `which`'s `blocks` partial rows: a workgroup of 1024 takes 32 columns, 32 threads a
+// column, each its own rows in turn, their sums added in order by fours.
+template <uint32_t D>
 __device__ __forceinline__ void residual_sum(const float* __restrict__ partial, float* __restrict__ out, uint32_t blocks, float* scratch, uint32_t block, uint32_t which) {
-  const uint32_t e = block * 16u + threadIdx.x % 16u, part = threadIdx.x / 16u;
+  const uint32_t e = block * 32u + threadIdx.x % 32u, part = threadIdx.x / 32u;
   const float* from = partial + (size_t)which * blocks * D;
   float sum = 0.f;
   if (e < D) {
-#pragma unroll 4
-    for (uint32_t k = part; k < blocks; k += 64u) sum += from[(size_t)k * D + e];
+#pragma unroll 8
+    for (uint32_t k = part; k < blocks; k += 32u) sum += from[(size_t)k * D + e];
   }
   scratch[threadIdx.x] = sum;
   __syncthreads();
-  if (part < 8u) {
-    for (uint32_t q = part + 8u; q < 64u; q += 8u) sum += scratch[q * 16u + threadIdx.x % 16u];
+  if (part < 4u) {
+#pragma unroll
+    for (uint32_t q = part + 4u; q < 32u; q += 4u) sum += scratch[q * 32u + threadIdx.x % 32u];
   }
   __syncthreads();
-  if (part < 8u) scratch[threadIdx.x] = sum;
+  if (part < 4u) scratch[threadIdx.x] = sum;
   __syncthreads();
   if (part == 0u && e < D) {
-    for (uint32_t q = 1; q < 8u; ++q) sum += scratch[q * 16u + threadIdx.x];
+#pragma unroll
+    for (uint32_t q = 1; q < 4u; ++q) sum += scratch[q * 32u + threadIdx.x];
     out[e] = sum;
   }
 }

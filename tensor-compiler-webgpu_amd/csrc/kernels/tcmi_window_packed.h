@@ -218,6 +218,7 @@ __device__ __forceinline__ void window_pair_lines(const char* tile, int line0, i
 }
 template <class T, int HB, int BLOCKS, int SLICES>
 __device__ __forceinline__ void window_pair_dots(f4 (&acc)[HB][BLOCKS], const char* tile, const Pair8 (&f)[HB][SLICES]) {
+  __builtin_amdgcn_s_setprio(1);
 #pragma unroll
   for (int k = 0; k < BLOCKS; ++k) {
 #pragma unroll
@@ -230,6 +231,7 @@ __device__ __forceinline__ void window_pair_dots(f4 (&acc)[HB][BLOCKS], const ch
       for (int h = 0; h < HB; ++h) window_mfma(acc[h][k], x, f[h][d]);
     }
   }
+  __builtin_amdgcn_s_setprio(0);
 }
 // A row's dots as a second operand, from memory: `up` times it. Its scale comes back in `down`.
 template <class S, int SLICES>
@@ -404,6 +406,7 @@ __device__ __forceinline__ void window_packed(const float* __restrict__ qp, cons
 #pragma unroll
         for (int k = 0; k < BLOCKS; k += 2) window_parts(s[h][k], s[h][k + 1], minus, pf[h][k / 2]);
       }
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int g = 0; g < G; g += 2) {
         f4 sum[HB][2];
@@ -429,6 +432,7 @@ __device__ __forceinline__ void window_packed(const float* __restrict__ qp, cons
         }
       }
     }
+    __builtin_amdgcn_s_setprio(0);
     barrier_ahead<0>();
   }
 #pragma unroll

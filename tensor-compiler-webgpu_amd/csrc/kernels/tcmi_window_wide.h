@@ -365,6 +365,7 @@ __device__ __forceinline__ void window_dots(f4 (&acc)[HB][BLOCKS], const char* t
 // acc[h][g] += the sums over a tile's lines of its floats 16g ... times f[h].
 template <class T, int HB, int G, int PAIRS>
 __device__ __forceinline__ void window_sums(f4 (&acc)[HB][G], const char* tile, const Parts (&f)[HB][PAIRS]) {
+  __builtin_amdgcn_s_setprio(1);
 #pragma unroll
   for (int g = 0; g < G; g += 2) {
     f4 sum[HB][2];
@@ -386,6 +387,7 @@ __device__ __forceinline__ void window_sums(f4 (&acc)[HB][G], const char* tile, 
       for (int h = 0; h < HB; ++h) acc[h][g + e] += sum[h][e];
     }
   }
+  __builtin_amdgcn_s_setprio(0);
 }
 // A line's parts, as a second operand.
 template <class S, int SLICES>

@@ -47,22 +47,25 @@ ${e.open}  __shared__ __attribute__((aligned(16))) float lds[${lds}];
 }
 `;
   if (!grad) {
-    const k = kernel('res', text({ H: parts.includes('h'), NORM: parts.includes('n') }, `residual<__KERNEL___s>(R, ${out('h')}, ${out('n')}, lds, blockIdx.x, gridDim.x)`, z.THREADS, z.THREADS / 64), [blocks, 1, 1], z.THREADS);
+    const k = kernel('res', text({ H: parts.includes('h'), NORM: parts.includes('n'), STAGED: false }, `residual<__KERNEL___s>(R, ${out('h')}, ${out('n')}, lds, blockIdx.x, gridDim.x)`, z.THREADS, z.THREADS / 64), [blocks, 1, 1], z.THREADS);
     return { kernels: [k], workspace: 0 };
   }
   const has = (p) => parts.includes(p);
   const flags = { DX: has('dx'), DY: has('dy'), DGAIN: has('dgain'), DBIAS: has('dbias'), DPOSTGAIN: has('dpostGain'), DPOSTBIAS: has('dpostBias'), DGATE: has('dgate'),
     DH: a.has.includes('dh'), DN: a.has.includes('dn'), SUMS: sums.length };
-  const lds = Math.max(z.THREADS / 64, sums.length && rows > 1 ? z.THREADS / z.LANES * z.D : 0);
+  // Vectors in LDS where four of them, for two workgroups a CU, fit.
+  const pad = z.UNITS * 4 * z.LANES, STAGED = pad <= 4096, SCRATCH = align(Math.max(z.THREADS / 64, sums.length && rows > 1 ? z.THREADS / z.LANES * z.D : 0), 4);
+  Object.assign(flags, { STAGED, SCRATCH });
+  const lds = SCRATCH + (STAGED ? 4 * pad : 0);
   const kernels = [kernel('resgrad', text(flags, `residual_grad<__KERNEL___s>(R, ${out('dx')}, ${out('dy')}, ${out('dgate')}, ${e.ws}, lds, blockIdx.x, gridDim.x)`, z.THREADS, lds), [blocks, 1, 1], z.THREADS)];
   if (sums.length) {
     kernels.push(kernel('ressum', `#include "tcmi_residual.h"
 extern "C" __global__ void __launch_bounds__(1024) __KERNEL__(${e.sig}) {
 ${e.open}  __shared__ float scratch[1024];
   float* const out[] = {${sums.map(e.out).join(', ')}};
-  tcmi::residual_sum<${z.D}, ${sums.length}>(${e.ws}, out[blockIdx.y], ${blocks}u, scratch, blockIdx.x, blockIdx.y);
+  tcmi::residual_sum<${z.D}>(${e.ws}, out[blockIdx.y], ${blocks}u, scratch, blockIdx.x, blockIdx.y);
 }
-`, [ceil(z.D, 16), sums.length, 1], 1024));
+`, [ceil(z.D, 32), sums.length, 1], 1024));
   }
   return { kernels, workspace: align(4 * floats, 256) };
 }

@@ -6,7 +6,7 @@
 //   { family: 'loss', N, d, V, bias?, gradient?, wrt?, after? }     wrt: 'h', 'W', 'b' (default all); `after`: the
 //       losses' cotangent depends on the losses, so their gradients cannot run beside them
 //   { family: 'orthogonalize', x, count, options, twice }
-//   { family: 'embedding', tokens, V, d, scale?, gradient? }
+//   { family: 'embedding', tokens, V, d, scale?, gradient?, one? }          one: the token of nine rows of ten
 //   { family: 'residual', x, options: { norm, residual, eps }, vectors: ['gain', 'bias', ...], gate: 'full'?, keep: 'h' | 'n'?,
 //       gradient?, wrt? }                                                     keep, wrt: default all
 //   { family: 'window', q, k, lengths?, options, gradient?, wrt? }          wrt: 'q', 'k', 'v' (default all)
@@ -91,6 +91,12 @@ const CONTEXT = [
   embedding('most', [300], 300000, 8, { gradient: true }),
   embedding('counted', [17003], 300, 8, { gradient: true }),
   embedding('counted-twice', [20480], 1000, 2, { gradient: true }),
+  // Of a table of few rows, the most of them, and one more; sorted tokens that are all one.
+  embedding('few-most', [3001], 128, 70, { scale: 2, gradient: true }),
+  embedding('few-more', [3001], 129, 70, { scale: 2, gradient: true }),
+  embedding('few-long', [40000], 5, 7, { gradient: true }),
+  embedding('same-sorted', [1500], 130, 20, { scale: -2, gradient: true, one: 77 }),
+  embedding('two-sorted', [3001], 200, 260, { gradient: true, one: 3 }),
   embedding('values', [9, 5], 11, 24, { scale: 0 }),
   // Norms of both kinds, with what may stand beside them; rows from one float to the longest; only some results.
   residual('plain', [5, 64], ['gain'], {}, { gradient: true }),

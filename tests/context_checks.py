@@ -26,6 +26,8 @@ def inputs_of(case, graph, seed):
         t[: N // 3] = rng.integers(0, V, N // 3)
         if N > 2:
             t[-1] = V - 1
+        if case.get("one") is not None:
+            t[rng.random(N) < 0.9] = case["one"]
         left = rng.random(N) < 0.1
         t[left] = rng.choice([-1.0, V, 0.5, np.nan, 1e30, -np.inf], size=left.sum())
         v["tokens"] = t.astype(np.float32).reshape(shapes["tokens"])
@@ -142,9 +144,10 @@ def residual_off(node, args, shapes):
         n = normalised(h)[1] * v["gain"]
         return n + v["bias"] if "bias" in v else n
     part = a["part"]
-    # A column's sum: a workgroup's rows (their count over its share of them, 512 workgroups), its lane groups, then the partial sums.
+    # A column's sum: a workgroup's rows (their count over its share of them, 512 workgroups), its 16 lane groups, then the partial sums: a 32nd of
+    # them a thread, eights and fours of threads.
     N = len(v["x"])
-    deep = N / 512 + 16 + min(512, N) / 64 + 8 + 8
+    deep = N / 512 + 16 + min(512, N) / 32 + 8 + 4
     dh = Off(v["dh"]) if "dh" in v else None
     if "dn" in v:
         r, hat = normalised(h)
