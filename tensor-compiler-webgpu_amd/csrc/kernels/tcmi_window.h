@@ -66,16 +66,23 @@ __device__ __forceinline__ WindowTiles window_keys(const WindowSpan<S>& w, uint3
   return {sinks, main, sinks + p1 / 16 + 1 - main, lo, p1};
 }
 
-// Floats at p, four of them where d is within the head.
-template <class S>
+// Floats d ... d + 3 of the head at p, 0 where not `on` or past its end. The load is made in any case, of the head's last floats where d is
+// past them (so p is a head that may be read): a branch around it would make the next one wait for it. INSIDE: of a head of whole 32 floats,
+// d is within it.
+template <class S, bool INSIDE = false>
 __device__ __forceinline__ f4 window_load(const float* __restrict__ p, uint32_t d, bool on) {
-  f4 v = {0.f, 0.f, 0.f, 0.f};
+  f4 v;
   if constexpr (S::VEC) {
-    if (on && d < S::DH) v = *reinterpret_cast<const f4*>(p + d);
+    constexpr bool WHOLE = INSIDE && S::DH % 32u == 0u;
+    v = *reinterpret_cast<const f4*>(p + (WHOLE ? d : min(d, S::DH - 4u)));
+    const bool in = on && (WHOLE || d < S::DH);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = in ? v[i] : 0.f;
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      if (on && d + i < S::DH) v[i] = p[d + i];
+      const float x = p[min(d + i, S::DH - 1u)];
+      v[i] = on && d + i < S::DH ? x : 0.f;
     }
   }
   return v;
@@ -99,7 +106,7 @@ __device__ __forceinline__ float window_finite(float x) { return __builtin_isfin
 template <class S, int G>
 __device__ __forceinline__ void window_along(f4 (&v)[G], const float* __restrict__ row, bool on) {
 #pragma unroll
-  for (int g = 0; g < G; ++g) v[g] = window_load<S>(row, 16 * g + 4 * ((threadIdx.x >> 4) & 3u), on);
+  for (int g = 0; g < G; ++g) v[g] = window_load<S, true>(row, 16 * g + 4 * ((threadIdx.x >> 4) & 3u), on);
 }
 // And across them: dim 16g + t of the tile's key 4q + s, of the keys from j0 on. Every load is made, of the last key that one of the rows
 // sees where its own is past it.

@@ -241,8 +241,8 @@ __device__ __forceinline__ void window_pair_row(Pair8 (&f)[SLICES], const float*
   float top = 0.f;
 #pragma unroll
   for (int s = 0; s < SLICES; ++s) {
-    x[s] = window_load<S>(p, 32 * s + 8 * q, on) * by;
-    y[s] = window_load<S>(p, 32 * s + 8 * q + 4, on) * by;
+    x[s] = window_load<S, true>(p, 32 * s + 8 * q, on) * by;
+    y[s] = window_load<S, true>(p, 32 * s + 8 * q + 4, on) * by;
     top = window_larger(top, window_top(x[s], y[s], 0.f));
   }
   top = window_larger(top, __shfl_xor(top, 16, 64));

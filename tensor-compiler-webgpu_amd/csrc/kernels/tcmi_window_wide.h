@@ -74,13 +74,14 @@ struct WindowTile {
   }
   static __device__ __forceinline__ int line(int i) { return (threadIdx.x + i * 256) / (DP / 4); }
   static __device__ __forceinline__ int dim(int i) { return (threadIdx.x + i * 256) % (DP / 4) * 4; }
-  // f(line): where line `line`'s floats are, or nullptr for zeros.
+  // at(line, on): where line `line`'s floats are (in any case somewhere that may be read); on = false for zeros.
   template <class F>
   __device__ __forceinline__ void load(F at) {
 #pragma unroll
     for (int i = 0; i < CHUNKS; ++i) {
-      const float* p = at(line(i));
-      x[i] = window_load<S>(p, dim(i), p != nullptr);
+      bool on = true;
+      const float* p = at(line(i), on);
+      x[i] = window_load<S, true>(p, dim(i), on);
     }
   }
   // CLEAN: what is not finite as 0, with bad[line] (if there is one) and *some set for its line.
@@ -192,7 +193,7 @@ __device__ __forceinline__ void window_wide(const float* __restrict__ qp, const 
     on[i] = row < ROWS && w.stands(pos[i]);
 #pragma unroll
     for (int s = 0; s < SLICES; ++s) {
-      const f4 x = window_load<S>(qp + line[i] * S::DH, 32 * s + 8 * q, on[i]), y = window_load<S>(qp + line[i] * S::DH, 32 * s + 8 * q + 4, on[i]);
+      const f4 x = window_load<S, true>(qp + line[i] * S::DH, 32 * s + 8 * q, on[i]), y = window_load<S, true>(qp + line[i] * S::DH, 32 * s + 8 * q + 4, on[i]);
       window_parts(x * scale, y * scale, minus, qf[i][s]);
     }
   }
@@ -215,9 +216,10 @@ __device__ __forceinline__ void window_wide(const float* __restrict__ qp, const 
   uint32_t *bad = reinterpret_cast<uint32_t*>(lds + 2 * T::BYTES), *some_bad = bad + NB;      // values of the tile that are not finite
   auto load = [&](const float* p, int32_t i) __attribute__((always_inline)) {
     const int32_t j0 = tiles.at(i) * NB;
-    x.load([&](int line) -> const float* {
+    x.load([&](int line, bool& on) {
       const int32_t j = j0 + line;
-      return j <= keys.hi && (j >= keys.lo || j < static_cast<int32_t>(S::SINKS)) ? p + base + (size_t)j * step : nullptr;
+      on = j <= keys.hi && (j >= keys.lo || j < static_cast<int32_t>(S::SINKS));
+      return p + base + (size_t)min(j, keys.hi) * step;
     });
   };
   int32_t begin, end;
@@ -395,7 +397,7 @@ __device__ __forceinline__ void window_line(Parts (&f)[SLICES], const float* __r
   const int q = (threadIdx.x >> 4) & 3;
 #pragma unroll
   for (int s = 0; s < SLICES; ++s) {
-    const f4 x = window_load<S>(p, 32 * s + 8 * q, on), y = window_load<S>(p, 32 * s + 8 * q + 4, on);
+    const f4 x = window_load<S, true>(p, 32 * s + 8 * q, on), y = window_load<S, true>(p, 32 * s + 8 * q + 4, on);
     window_parts(x * scale, y * scale, minus, f[s]);
   }
 }
@@ -409,7 +411,7 @@ __device__ __forceinline__ float window_row_mass(const float* __restrict__ o, co
   for (int s = 0; s < (static_cast<int>(S::DH) + 31) / 32; ++s) {
 #pragma unroll
     for (int h = 0; h < 8; h += 4) {
-      const f4 x = window_load<S>(o, 32 * s + 8 * q + h, on), y = window_load<S>(dy, 32 * s + 8 * q + h, on);
+      const f4 x = window_load<S, true>(o, 32 * s + 8 * q + h, on), y = window_load<S, true>(dy, 32 * s + 8 * q + h, on);
 #pragma unroll
       for (int i = 0; i < 4; ++i) sum = fmaf(x[i], y[i], sum);
     }
@@ -479,9 +481,10 @@ __device__ __forceinline__ void window_wide_dq(const WindowGradArgs a, float* __
   auto load = [&](int32_t i) __attribute__((always_inline)) {
     const int32_t j0 = tiles.at(i) * NB;
     auto at = [&](const float* p) {
-      return [=, &keys](int line) -> const float* {
+      return [=, &keys](int line, bool& on) {
         const int32_t j = j0 + line;
-        return j <= keys.hi && (j >= keys.lo || j < static_cast<int32_t>(S::SINKS)) ? p + base + (size_t)j * step : nullptr;
+        on = j <= keys.hi && (j >= keys.lo || j < static_cast<int32_t>(S::SINKS));
+        return p + base + (size_t)min(j, keys.hi) * step;
       };
     };
     kt.load(at(a.k));
@@ -621,9 +624,10 @@ __device__ __forceinline__ void window_wide_dkv(const WindowGradArgs a, float* _
   auto load = [&](int32_t i) __attribute__((always_inline)) {
     const int32_t r0 = i * NB;
     auto at = [&](const float* p) {
-      return [=, &place, &w](int l) -> const float* {
+      return [=, &place, &w](int l, bool& on) {
         const int32_t r = r0 + l, pos = w.first + r / R;
-        return r < ROWS && pos >= p0 && pos <= p1 ? p + place(r) * S::DH : nullptr;
+        on = r < ROWS && pos >= p0 && pos <= p1;
+        return p + place(min(r, ROWS - 1)) * S::DH;
       };
     };
     qt.load(at(a.q));
