@@ -406,6 +406,9 @@ __device__ __forceinline__ void window_packed(const float* __restrict__ qp, cons
 #pragma unroll
         for (int k = 0; k < BLOCKS; k += 2) window_parts(s[h][k], s[h][k + 1], minus, pf[h][k / 2]);
       }
+      // (The places of heads above 64 are found again for each tile: kept, they spill other registers, whose reloads wait for the copies.)
+      int own = lane;
+      if constexpr (G > 4) asm volatile("" : "+v"(own));
       __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int g = 0; g < G; g += 2) {
@@ -417,7 +420,7 @@ __device__ __forceinline__ void window_packed(const float* __restrict__ qp, cons
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             Parts f;
-            T::across(vs, 32 * k, 16 * (g + e), f);
+            T::across(vs, 32 * k, 16 * (g + e), f, own);
 #pragma unroll
             for (int h = 0; h < HB; ++h) window_mfma(sum[h][e], f, pf[h][k]);
           }
@@ -439,8 +442,11 @@ __device__ __forceinline__ void window_packed(const float* __restrict__ qp, cons
   for (int h = 0; h < HB; ++h) {
     const float total = quad16_reduce<false>(l[h]);
     const bool some = total > 0.f || total != total;
-    const uint32_t row = mine + 16u * h + t;
+    uint32_t row = mine + 16u * h + t;
     if (row >= ROWS) continue;
+    // (Its line is found again too.)
+    asm("" : "+v"(row));
+    const size_t line = ((size_t)b * S::T + row / Span::R) * S::H + hk * Span::R + row % Span::R;
     if constexpr (S::SPLITS > 1u) {
       const size_t place = ((size_t)split * S::B * S::HK + head) * S::TILES * 16u + row;
 #pragma unroll
@@ -451,9 +457,9 @@ __device__ __forceinline__ void window_packed(const float* __restrict__ qp, cons
     const float inv = some ? 1.f / total : 0.f;
     if (out != nullptr) {
 #pragma unroll
-      for (int g = 0; g < G; ++g) window_store<S>(out + rows.line[h] * S::DH, 16 * g + 4 * q, o[h][g] * inv);
+      for (int g = 0; g < G; ++g) window_store<S>(out + line * S::DH, 16 * g + 4 * q, o[h][g] * inv);
     }
-    if (lse != nullptr && q == 0) lse[rows.line[h]] = some ? (m[h] + __builtin_amdgcn_logf(total)) * 0.69314718055994531f : -TCMI_INF;
+    if (lse != nullptr && q == 0) lse[line] = some ? (m[h] + __builtin_amdgcn_logf(total)) * 0.69314718055994531f : -TCMI_INF;
   }
 }
 

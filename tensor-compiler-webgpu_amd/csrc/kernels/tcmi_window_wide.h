@@ -124,8 +124,8 @@ struct WindowTile {
     for (int p = 0; p < 3; ++p) f.p[p] = *reinterpret_cast<const bf16x8*>(tile + p * PLANE + line0 * LD + (at ^ (slice << 6)));
   }
   // Transposed: line dim0 + t, the sum over tile lines line0 + 4q ... and line0 + 16 + 4q ....
-  static __device__ __forceinline__ void across(const char* tile, int line0, int dim0, Parts& f) {
-    const int t = threadIdx.x & 15, q = (threadIdx.x >> 4) & 3, line = 4 * q + (t >> 2);
+  static __device__ __forceinline__ void across(const char* tile, int line0, int dim0, Parts& f, int lane = threadIdx.x) {
+    const int t = lane & 15, q = (lane >> 4) & 3, line = 4 * q + (t >> 2);
     const int at = (line * LD + ((((t >> 1) & 1) ^ swap(line)) << 4) + (t & 1) * 8) ^ (dim0 << 1);
 #pragma unroll
     for (int p = 0; p < 3; ++p) {
