@@ -134,7 +134,10 @@ function operatorRules(ShapeError, fmt) {
     need(q.length === 4 && k.length === 4, `${op} of ${fmt(q)} by ${fmt(k)}: [batch, tokens, heads, head size]`);
     need(same(k, v), `${op}: keys of ${fmt(k)} and values of ${fmt(v)}`);
     need(q[0] === k[0] && q[3] === k[3] && q[2] % k[2] === 0, `${op} of ${fmt(q)} by ${fmt(k)}: equal batches and head sizes, and a whole number of query heads to a key head`);
-    if (lengths) need(same(lengths, [q[0]]), `${op}: lengths of ${fmt(lengths)} for ${q[0]} sequences`);
+    if (lengths) {
+      need(same(lengths, [q[0]]), `${op}: lengths of ${fmt(lengths)} for ${q[0]} sequences`);
+      need(k[1] <= 2 ** 24, `${op}: lengths up to ${k[1]} keys (a float32 names 2^24)`);
+    }
     const whole = (n) => Number.isInteger(n) && n >= 0 && n < 2 ** 31;
     need(whole(attrs.window), `${op}: a window of ${attrs.window}`);
     need(whole(attrs.sinks), `${op}: ${attrs.sinks} sinks`);

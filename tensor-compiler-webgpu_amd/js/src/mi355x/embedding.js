@@ -35,7 +35,7 @@ function lowerEmbedding(graph, node) {
   // A lane takes up to four groups of a row; more of them are other workgroups'.
   const z = { N, V, D, E, LANES: lanes, UNITS: Math.min(4, columns) };
   const blocks = ceil(columns, z.UNITS);
-  if (N * lanes >= 2 ** 32) throw new Error(`embedding: ${N} tokens of ${D} floats (a grid has 2^32 threads, ${lanes} a token)`);
+  if (ceil(N, 256 / lanes) * 256 >= 2 ** 32) throw new Error(`embedding: ${N} tokens of ${D} floats (a grid has 2^32 threads, ${lanes} a token)`);
   if (blocks > 65535) throw new Error(`embedding: rows of ${D} floats (at most ${65535 * 64 * 4 * E})`);
   const k = make(z, node.attrs.scale)('emb', [ceil(N, 256 / lanes), blocks, 1], 256, null,
     `embed<${S}>(A.in[0], A.in[1], A.out, blockIdx.x * (256u / ${S}::LANES) + threadIdx.x / ${S}::LANES, blockIdx.y)`);

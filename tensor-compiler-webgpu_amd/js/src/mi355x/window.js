@@ -11,7 +11,8 @@ function windowSizes(graph, node) {
   const [B, T, H, DH] = graph.nodes[node.inputs[0]].shape, [, KEYS, HK] = graph.nodes[node.inputs[1]].shape, a = node.attrs;
   const grad = node.op === 'windowAttentionGrad';
   if (DH > MOST_HEAD) throw new Error(`windowAttention: heads of ${DH} floats (at most ${MOST_HEAD})`);
-  if (T * H >= 2 ** 31 || KEYS * HK >= 2 ** 31) throw new Error('windowAttention: a sequence\'s rows are counted in 32 bits (at most 2^31 - 1)');
+  // (Positions of a tile or a window past the last stay below 2^31.)
+  if (T * H > 2 ** 30 || KEYS * HK > 2 ** 30) throw new Error('windowAttention: a sequence\'s rows are counted in 32 bits (at most 2^30)');
   const lengths = node.inputs.length - (grad ? 3 : 0) === 4;
   return { z: { B, T, H, DH, KEYS, HK, WINDOW: a.window, SINKS: a.sinks, LAST: a.queries === 'last', LENGTHS: lengths, VEC: DH % 4 === 0 }, scale: a.scale, lengths, grad };
 }
@@ -28,9 +29,9 @@ ${e.open}${lds ? `  __shared__ __attribute__((aligned(16))) ${lds};\n` : ''}  tc
 `, grid, threads);
 }
 
-/** Workgroups of `rows` x `heads`, along the first axis of a grid. */
+/** n workgroups along the first axis of a grid, whose threads are counted in 32 bits: up to 512 each. */
 function grid(n) {
-  if (n >= 2 ** 24) throw new Error(`windowAttention: ${n} workgroups (at most 2^24)`);
+  if (n >= 2 ** 23) throw new Error(`windowAttention: ${n} workgroups (at most 2^23)`);
   return [n, 1, 1];
 }
 
@@ -121,7 +122,7 @@ function rowChunk(z, rows, heads, slots) {
     const p1 = Math.min(z.WINDOW && j >= z.SINKS ? Math.min(z.KEYS - 1, last + z.WINDOW - 1) : z.KEYS - 1, first + z.T - 1);
     counts.push(p0 <= p1 ? ceil((p1 - first + 1) * R, 32) - Math.floor((p0 - first) * R / 32) : 0);
   }
-  const most = Math.max(1, ...counts);
+  const most = counts.reduce((a, c) => Math.max(a, c), 1);
   let best = null;
   for (let chunk = Math.min(most, 8); ; chunk = Math.min(most, Math.ceil(chunk * 1.1))) {
     const n = heads * counts.reduce((q, c) => q + Math.max(1, ceil(c, chunk)), 0), rounds = ceil(n, slots);
@@ -245,17 +246,15 @@ function backwardKernels(s, parts, joined) {
   return { kernels, workspace: at };
 }
 
-/** Products of one head's pairs of a query and a key that it sees, were its sequence full: the flops of one product. */
+/** The flops of one product over the pairs of a query and a key that it sees, were every sequence full. */
 function seen(z) {
-  const first = z.LAST ? z.KEYS - z.T : 0;
-  let pairs = 0;
-  for (let t = 0; t < z.T; t++) {
-    const at = first + t;
-    if (at < 0 || at >= z.KEYS) continue;
-    const from = z.WINDOW ? Math.max(0, at - z.WINDOW + 1) : 0;
-    pairs += at + 1 - from + Math.min(from, z.SINKS);
-  }
-  return 2 * z.B * z.H * z.DH * pairs;
+  const first = z.LAST ? z.KEYS - z.T : 0, p0 = Math.max(0, first), p1 = Math.min(z.KEYS, first + z.T) - 1;
+  // Of the positions below p: the keys up to each, less those before the window, and the sinks among those.
+  const to = (p) => {
+    const n = Math.max(0, p - (z.WINDOW || p)), few = Math.min(n, z.SINKS);
+    return p * (p + 1) / 2 - n * (n + 1) / 2 + few * (few + 1) / 2 + (n - few) * z.SINKS;
+  };
+  return p0 <= p1 ? 2 * z.B * z.H * z.DH * (to(p1 + 1) - to(p0)) : 0;
 }
 
 function lowerWindow(graph, node) {

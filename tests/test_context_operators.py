@@ -94,6 +94,7 @@ def test_every_launch_reads_what_is_written_before_it(tool, graphs):
     ({"family": "embedding", "tokens": [4], "V": 2 ** 24 + 1, "d": 1}, "a float32 names 2^24"),
     ({"family": "embedding", "tokens": [2 ** 28 + 1], "V": 3, "d": 1}, "at most 268435456"),
     ({"family": "embedding", "tokens": [2 ** 27], "V": 3, "d": 256}, "2^32 threads"),
+    ({"family": "embedding", "tokens": [2 ** 28 - 1], "V": 3, "d": 64}, "2^32 threads"),
     ({"family": "embedding", "tokens": [1], "V": 1, "d": 2 ** 26}, "at most 67107840"),
     ({"family": "embedding", "tokens": [4], "V": 8, "d": 4, "scale": "NaN"}, "scale NaN"),
     ({"family": "residual", "x": [4, 16385], "vectors": ["gain"]}, "at most 16384"),
@@ -115,6 +116,9 @@ def test_every_launch_reads_what_is_written_before_it(tool, graphs):
     ({"family": "window", "q": [1, 4, 2, 8], "k": [1, 4, 2, 8], "options": {"queries": "middle"}}, "queries are"),
     ({"family": "window", "q": [1, 4, 2, 8], "k": [1, 4, 2, 8], "options": {"scale": "x"}}, "scale x"),
     ({"family": "window", "q": [1, 2 ** 25, 64, 1], "k": [1, 1, 64, 1]}, "counted in 32 bits"),
+    ({"family": "window", "q": [1, 1, 1, 4], "k": [1, 2 ** 30 + 1, 1, 4]}, "counted in 32 bits"),
+    ({"family": "window", "q": [1, 1, 1, 4], "k": [1, 2 ** 24 + 1, 1, 4], "lengths": True}, "a float32 names 2^24"),
+    ({"family": "window", "q": [4, 2 ** 27, 1, 1], "k": [4, 2 ** 27, 1, 1]}, "workgroups (at most 2^23)"),
 ])
 def test_calls_that_are_refused(tool, case, why):
     import tcmi_bridge
