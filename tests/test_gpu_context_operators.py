@@ -121,6 +121,18 @@ def test_numbers_of_any_size_where_a_query_does_not_see_them(tool, tmp_path, for
     np.testing.assert_array_equal(x, y)
 
 
+@pytest.mark.parametrize("form", FORMS)
+def test_powers_of_two_pass_through(tool, tmp_path, form):
+    """Queries 2^-40 and keys 2^40 times themselves have the scores that they had, and every result is its power of two times what it was,
+    bit for bit: the scales of rows and the parts of operands lose nothing. (What is split into parts stays above 2^-102: the smallest, dS
+    here, is 2^10 times what it was.)"""
+    _, _, v = window_inputs(tool, f"window-{form}", 4)
+    by = {"q": -40, "k": 40, "v": 30, "d0": -20}
+    _, (plain, got) = run_form(tool, tmp_path, f"window-{form}", [v, {n: np.ldexp(x, by[n]).astype(np.float32) for n, x in v.items()}])
+    for n, e in {"o": 30, "dq": 40 + 30 - 20, "dk": -40 + 30 - 20, "dv": -20}.items():
+        np.testing.assert_array_equal(got[n], np.ldexp(plain[n], e), err_msg=n)
+
+
 def test_a_padded_batch_of_the_embedding_and_its_order(tool, tmp_path):
     """Tokens in another order: the same rows, and gradients that differ by no more than their sums' roundings; all padding: zeros."""
     N, V, d = 900, 40, 36
