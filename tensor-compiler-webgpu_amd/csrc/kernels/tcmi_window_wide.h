@@ -418,7 +418,7 @@ __device__ __forceinline__ float window_row_mass(const float* __restrict__ o, co
   }
   return quad16_reduce<false>(sum);
 }
-// Of 16 lines a wavefront from `line` on (where no gradient of queries forms them beside its own).
+// Of 16 lines a wavefront from `line` on, for heads above 128.
 template <class S>
 __device__ __forceinline__ void window_wide_mass(const float* __restrict__ o, const float* __restrict__ dy, float* __restrict__ mass, size_t line) {
   constexpr size_t LINES = (size_t)S::B * S::T * S::H;
@@ -434,13 +434,12 @@ struct WindowBack {
   static constexpr int HB = S::HB;
   static constexpr uint32_t ROWS = 64 * HB;
   using T = WindowTile<S, NB>;
-  static constexpr int LDS = 2 * T::BYTES + 3 * NB * 4;
+  static constexpr int LDS = 2 * T::BYTES + (2 + SLICES) * NB * 4;
 };
 
-// Workgroup: W::ROWS rows of a sequence's key head, a split of the keys they see. parts: the splits' sums, [SPLITS][lines][DH]. Writes
-// dy·o of its rows for the gradients of keys.
+// Workgroup: W::ROWS rows of a sequence's key head, a split of the keys they see. parts: the splits' sums, [SPLITS][lines][DH].
 template <class S>
-__device__ __forceinline__ void window_wide_dq(const WindowGradArgs a, float* __restrict__ dq, float* __restrict__ parts, float* __restrict__ masses, char* lds, uint32_t head, uint32_t tile, uint32_t split) {
+__device__ __forceinline__ void window_wide_dq(const WindowGradArgs a, float* __restrict__ dq, float* __restrict__ parts, char* lds, uint32_t head, uint32_t tile, uint32_t split) {
   using W = WindowBack<S>;
   using T = typename W::T;
   using Span = WindowSpan<S>;
@@ -469,7 +468,6 @@ __device__ __forceinline__ void window_wide_dq(const WindowGradArgs a, float* __
     window_line<S>(df[h], a.dy + line[h] * S::DH, on[h], 1.f, minus);
     lse[h] = on[h] ? a.lse[line[h]] * LOG2E : 0.f;
     mass[h] = window_row_mass<S>(a.o + line[h] * S::DH, a.dy + line[h] * S::DH, on[h]);
-    if (split == 0u && q == 0 && row < ROWS) masses[line[h]] = mass[h];
 #pragma unroll
     for (int g = 0; g < G; ++g) acc[h][g] = f4{0.f, 0.f, 0.f, 0.f};
   }
@@ -614,42 +612,63 @@ __device__ __forceinline__ void window_wide_dkv(const WindowGradArgs a, float* _
   }
   const size_t top = ((size_t)b * S::T) * S::H + hk * R;
   auto place = [&](int32_t r) { return top + (size_t)(r / R) * S::H + r % R; };
-  T qt, dt;
-  float stats[2];
+  T qt, dt, ot;
+  float lse = 0.f, before = 0.f;
   char *qlds = lds, *dlds = lds + T::BYTES;
   float* const row_lse = reinterpret_cast<float*>(lds + 2 * T::BYTES);
   float* const row_mass = row_lse + NB;
-  int32_t* const row_pos = reinterpret_cast<int32_t*>(row_mass + NB);
+  int32_t* const row_pos = reinterpret_cast<int32_t*>(row_mass + SLICES * NB);
   int32_t row_at = 0;
+  auto at = [&](const float* p, int32_t r0) {
+    return [=, &place, &w](int l, bool& on) {
+      const int32_t r = r0 + l, pos = w.first + r / R;
+      on = r < ROWS && pos >= p0 && pos <= p1;
+      return p + place(min(r, ROWS - 1)) * S::DH;
+    };
+  };
+  // dy·o is formed of the tiles here; of heads above 128, whose products leave no registers for o, by a launch before.
+  constexpr bool OWN = SLICES <= 4;
   auto load = [&](int32_t i) __attribute__((always_inline)) {
     const int32_t r0 = i * NB;
-    auto at = [&](const float* p) {
-      return [=, &place, &w](int l, bool& on) {
-        const int32_t r = r0 + l, pos = w.first + r / R;
-        on = r < ROWS && pos >= p0 && pos <= p1;
-        return p + place(min(r, ROWS - 1)) * S::DH;
-      };
-    };
-    qt.load(at(a.q));
-    dt.load(at(a.dy));
+    qt.load(at(a.q, r0));
+    dt.load(at(a.dy, r0));
+    if constexpr (DK && OWN) ot.load(at(a.o, r0));
     if (threadIdx.x < NB) {
       const int32_t r = r0 + threadIdx.x;
       row_at = w.first + r / R;
       const bool on = r < ROWS && row_at >= p0 && row_at <= p1;
       if (!on) row_at = -1;
-      // (NaN where q or dy hold a number that is not finite.)
-      stats[1] = on ? a.mass[place(r)] : 0.f;
-      stats[0] = on ? a.lse[place(r)] * LOG2E + 0.f * stats[1] : 0.f;
+      lse = on ? a.lse[place(r)] * LOG2E : 0.f;
+      if constexpr (!OWN) before = on ? a.mass[place(r)] : 0.f;
     }
+  };
+  auto mass = [&](int k) __attribute__((always_inline)) {
+    f4 sum = *reinterpret_cast<const f4*>(row_mass + 16 * k + 4 * q);
+#pragma unroll
+    for (int s = 1; OWN && s < SLICES; ++s) sum += *reinterpret_cast<const f4*>(row_mass + s * NB + 16 * k + 4 * q);
+    return sum;
   };
   if (begin < end) load(begin);
   for (int32_t i = begin; i < end; ++i) {
     __syncthreads();
     qt.template store<true>(qlds, minus);
     dt.template store<true>(dlds, minus);
+    // dy·o of 32 floats of a row by its eight threads; NaN where q or dy hold a number that is not finite, as 0 times it is.
+    if constexpr (OWN) {
+#pragma unroll
+      for (int c = 0; c < T::CHUNKS; ++c) {
+        float sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum = fmaf(0.f, qt.x[c][e], fmaf(dt.x[c][e], DK ? ot.x[c][e] : 0.f, sum));
+#pragma unroll
+        for (int off = 1; off < 8; off *= 2) sum += __shfl_xor(sum, off, 64);
+        if (threadIdx.x % 8u == 0u) row_mass[T::dim(c) / 32 * NB + T::line(c)] = sum;
+      }
+    } else if (threadIdx.x < NB) {
+      row_mass[threadIdx.x] = before;
+    }
     if (threadIdx.x < NB) {
-      row_lse[threadIdx.x] = stats[0];
-      row_mass[threadIdx.x] = stats[1];
+      row_lse[threadIdx.x] = lse;
       row_pos[threadIdx.x] = row_at;
     }
     __syncthreads();
@@ -662,7 +681,8 @@ __device__ __forceinline__ void window_wide_dkv(const WindowGradArgs a, float* _
     Parts f[HB][1];
 #pragma unroll
     for (int k = 0; k < BLOCKS; ++k) {
-      const f4 ls = *reinterpret_cast<const f4*>(row_lse + 16 * k + 4 * q);
+      // (NaN where the row's numbers are not finite.)
+      const f4 ls = *reinterpret_cast<const f4*>(row_lse + 16 * k + 4 * q) + mass(k) * 0.f;
       const int4 ps = *reinterpret_cast<const int4*>(row_pos + 16 * k + 4 * q);
       const int32_t pos[4] = {ps.x, ps.y, ps.z, ps.w};
 #pragma unroll
@@ -681,7 +701,7 @@ __device__ __forceinline__ void window_wide_dkv(const WindowGradArgs a, float* _
       window_dots<T>(dp, dlds, vf);
 #pragma unroll
       for (int k = 0; k < BLOCKS; ++k) {
-        const f4 ms = *reinterpret_cast<const f4*>(row_mass + 16 * k + 4 * q);
+        const f4 ms = mass(k);
 #pragma unroll
         for (int h = 0; h < HB; ++h) {
 #pragma unroll

@@ -18,15 +18,39 @@ function windowSizes(graph, node) {
 }
 
 function maker(s, e, types) {
-  return (kind, grid, threads, lds, call, more) => kernel(kind, `#include "${/_pack/.test(call) ? 'tcmi_window_packed.h' : /_wide/.test(call) ? 'tcmi_window_wide.h' : 'tcmi_window.h'}"
-struct ${S} {
+  const text = (kind, blocks, threads, structs, calls, lds, body) => {
+    const header = calls.some((c) => /_pack/.test(c)) ? 'tcmi_window_packed.h' : calls.some((c) => /_wide/.test(c)) ? 'tcmi_window_wide.h' : 'tcmi_window.h';
+    // Two workgroups of four wavefronts a CU, or one of eight: 256 registers each.
+    const two = calls.some((c) => /_packed(_dq|_dkv)?</.test(c) || (/_wide(_dq|_dkv)?</.test(c) && s.z.DH <= 64));
+    return kernel(kind, `#include "${header}"
+${structs.map(([name, more]) => `struct ${name} {
 ${constants(Object.assign({}, s.z, more || {}), types)}
   static __device__ __forceinline__ double scale() { return ${double(s.scale)}; }
-};
-extern "C" __global__ void __launch_bounds__(${threads}${/_packed(_dq|_dkv)?</.test(call) || (/_wide(_dq|_dkv)?</.test(call) && s.z.DH <= 64) ? ', 2' : ''}) __KERNEL__(${e.sig}) {
-${e.open}${lds ? `  __shared__ __attribute__((aligned(16))) ${lds};\n` : ''}  tcmi::${call};
-}
-`, grid, threads);
+};`).join('\n')}
+extern "C" __global__ void __launch_bounds__(${threads}${two ? ', 2' : ''}) __KERNEL__(${e.sig}) {
+${e.open}${lds ? `  __shared__ __attribute__((aligned(16))) ${lds};\n` : ''}${body}}
+`, blocks, threads);
+  };
+  const m = (kind, blocks, threads, lds, call, more) => text(kind, blocks, threads, [[S, more]], [call], lds, `  tcmi::${call};\n`);
+  /**
+   * Several jobs in one launch, a run of workgroups each. A job: { blocks, more, lds, call }, its LDS in bytes and its call given its struct of
+   * sizes' name, the call also its workgroup's number.
+   */
+  m.jobs = (kind, threads, jobs) => {
+    if (jobs.length === 1) {
+      const [j] = jobs;
+      return m(kind, grid(j.blocks), threads, j.lds && `char lds[${j.lds(S)}]`, j.call(S, 'blockIdx.x'), j.more);
+    }
+    const structs = jobs.map((j, k) => [k ? `${S}${k}` : S, j.more]), calls = jobs.map((j, k) => j.call(structs[k][0], 'block'));
+    const bytes = jobs.map((j, k) => j.lds && j.lds(structs[k][0])).filter(Boolean);
+    let first = 0, body = '';
+    jobs.forEach((j, k) => {
+      body += `  ${k ? '} else ' : ''}${k < jobs.length - 1 ? `if (blockIdx.x < ${first + j.blocks}u) ` : ''}{\n    const uint32_t block = blockIdx.x - ${first}u;\n    tcmi::${calls[k]};\n`;
+      first += j.blocks;
+    });
+    return text(kind, grid(first), threads, structs, calls, bytes.length ? `char lds[${bytes.reduce((x, y) => `(${x} > ${y} ? ${x} : ${y})`)}]` : null, `${body}  }\n`);
+  };
+  return m;
 }
 
 /** n workgroups along the first axis of a grid, whose threads are counted in 32 bits: up to 512 each. */
@@ -173,7 +197,9 @@ function backwardKernels(s, parts, joined) {
   const args = `{A.in[0], A.in[1], A.in[2], ${L}, A.in[${first}], A.in[${first + 1}], A.in[${first + 2}], ${e.ws}}`;
   const dq = parts.includes('dq'), dk = parts.includes('dk'), dv = parts.includes('dv');
   const types = { HB: 'int' }, more = {};
-  let at = align(4 * z.B * z.T * z.H, 256);
+  // dy·o of every row, where the gradients of keys do not form it.
+  const masses = !wide || (z.DH > 128 && (dk || dv));
+  let at = masses ? align(4 * z.B * z.T * z.H, 256) : 0;
   const place = (name, bytes) => { more[name] = at; types[name] = 'size_t'; at = align(at + bytes, 256); };
   const m = maker(s, e, types), ws = `reinterpret_cast<char*>(${e.ws})`;
   const kernels = [];
@@ -184,7 +210,7 @@ function backwardKernels(s, parts, joined) {
     if (dk || dv) kernels.push(m('windkv', grid(KTILES * heads), 256, lds, `window_dkv<${S}, ${dk}, ${dv}>(${args}, ${out('dk')}, ${out('dv')}, lds, blockIdx.x)`, { KTILES }));
     return { kernels, workspace: at };
   }
-  const add = (n) => grid(ceil(z.DH % 4 ? n : n / 4, 256)), KP = align(z.KEYS, 64), RP = align(z.T * R, 64), packed = packs(z), lanes = lanesOf(z.DH);
+  const add = (n) => ceil(z.DH % 4 ? n : n / 4, 256), KP = align(z.KEYS, 64), RP = align(z.T * R, 64), packed = packs(z), lanes = lanesOf(z.DH);
   const hold = z.DH <= 64;
   if (packed) {
     types.WAVES = 'int';
@@ -200,49 +226,51 @@ function backwardKernels(s, parts, joined) {
     kernels.push(m('winpack', grid(keys + ceil(heads * RP, 256 / lanes)), 256, null,
       `window_pack_both<${S}, ${dq}, ${dk || dv}, ${keys}u>(${args}, ${ws}, blockIdx.x, ${place256(0)}, ${place256(keys)})`, Object.assign({ VSUMS: 0 }, more)));
   }
-  if (!packed && !dq) {
+  if (masses) {
     kernels.push(m('winmass', grid(ceil(z.B * z.T * z.H, 64)), 256, null, `window_wide_mass<${S}>(A.in[${first}], A.in[${first + 2}], ${e.ws}, blockIdx.x * 64u + threadIdx.x / 64u * 16u)`));
   }
-  if (dq) {
-    more.HB = blocksOf(hold, z.T * R, heads, ceil(z.WINDOW ? Math.min(z.KEYS, z.WINDOW) : z.KEYS, 64));
-    const rows = 64 * more.HB, tiles = ceil(z.T * R, rows), lines = z.B * z.T * z.H;
-    const SPLITS = more.SPLITS = keySplits(z, rows, packed && hold ? 64 : 32, tiles * heads);
-    place('DQPARTS', SPLITS > 1 ? 4 * SPLITS * lines * z.DH : 0);
-    const sums = `reinterpret_cast<float*>(${ws} + ${S}::DQPARTS)`;
-    const where = `blockIdx.x % ${heads}u, ${tiles - 1}u - blockIdx.x / ${heads * SPLITS}u, blockIdx.x / ${heads}u % ${SPLITS}u`;
-    if (packed) kernels.push(m('winpackeddq', grid(tiles * heads * SPLITS), 256, `char lds[tcmi::WindowPacked<${S}>::DQ]`, `window_packed_dq<${S}>(${args}, ${out('dq')}, ${sums}, ${ws}, lds, ${where})`, more));
-    else kernels.push(m('winwidedq', grid(tiles * heads * SPLITS), 256, `char lds[tcmi::WindowBack<${S}>::LDS]`, `window_wide_dq<${S}>(${args}, ${out('dq')}, ${sums}, ${e.ws}, lds, ${where})`, more));
-    if (SPLITS > 1) kernels.push(m('winadd', add(lines * z.DH), 256, null, `window_wide_add<${S}>(${out('dq')}, ${sums}, blockIdx.x * 256u + threadIdx.x)`, more));
-  }
+  // The gradients of queries and of keys run side by side, and what joins their parts.
+  const jobs = [], joins = [], waves = packed && z.DH > 64 ? 8 : 4;
+  if (packed) more.WAVES = waves;
+  const place4 = (name, floats) => place(name, 4 * floats);
   if (dk || dv) {
     // Eight wavefronts where a packed tile takes most of LDS.
-    const waves = packed && z.DH > 64 ? 8 : 4;
-    more.HB = blocksOf(hold, z.KEYS, heads, ceil(Math.min(z.T, z.WINDOW || z.T) * R, 32));
-    if (packed) more.WAVES = waves;
-    const rows = 16 * waves * more.HB, tiles = ceil(z.KEYS, rows), all = ceil(z.T * R, 32), most = z.WINDOW ? Math.min(all, ceil((z.WINDOW + rows) * R, 32) + 1) : all;
+    const HB = blocksOf(hold, z.KEYS, heads, ceil(Math.min(z.T, z.WINDOW || z.T) * R, 32));
+    const rows = 16 * waves * HB, tiles = ceil(z.KEYS, rows), all = ceil(z.T * R, 32), most = z.WINDOW ? Math.min(all, ceil((z.WINDOW + rows) * R, 32) + 1) : all;
     const sinks = z.WINDOW ? Math.min(tiles, ceil(Math.min(z.SINKS, z.KEYS), rows)) : 0;
     const CHUNK = rowChunk(z, rows, heads, waves === 8 ? CUS : 2 * CUS);
     const CHUNKS = ceil(most, CHUNK), CHUNKS_MOST = sinks ? Math.max(CHUNKS, ceil(all, CHUNK)) : CHUNKS, FEW = Math.min(z.KEYS, sinks * rows);
     Object.assign(more, { CHUNK, CHUNKS, CHUNKS_MOST, FEW, ROWS_EACH: rows });
     const floats = CHUNKS_MOST > 1 ? (CHUNKS * z.KEYS + (CHUNKS_MOST - CHUNKS) * FEW) * z.B * z.HK * z.DH : 0;
-    place('DKPARTS', dk ? 4 * floats : 0);
-    place('DVPARTS', dv ? 4 * floats : 0);
+    place4('DKPARTS', dk ? floats : 0);
+    place4('DVPARTS', dv ? floats : 0);
     // The sinks' chunks, then the other tiles', the keys that most queries see first.
-    const few = sinks * CHUNKS_MOST, id = `(blockIdx.x / ${heads}u)`;
-    const where = `blockIdx.x % ${heads}u, ${id} < ${few}u ? ${id} / ${CHUNKS_MOST}u : ${sinks}u + (${id} - ${few}u) / ${CHUNKS}u, ${id} < ${few}u ? ${id} % ${CHUNKS_MOST}u : (${id} - ${few}u) % ${CHUNKS}u`;
-    const blocks = grid((few + (tiles - sinks) * CHUNKS) * heads);
+    const few = sinks * CHUNKS_MOST;
+    const where = (block) => [`(${block} / ${heads}u)`].map((id) => `${block} % ${heads}u, ${id} < ${few}u ? ${id} / ${CHUNKS_MOST}u : ${sinks}u + (${id} - ${few}u) / ${CHUNKS}u, ${id} < ${few}u ? ${id} % ${CHUNKS_MOST}u : (${id} - ${few}u) % ${CHUNKS}u`)[0];
     // Both at once, or of the largest heads, which its registers do not hold both of, one after the other.
     for (const [k, v] of dk && dv && z.DH > 128 ? [[false, true], [true, false]] : [[dk, dv]]) {
-      if (packed) kernels.push(m('winpackeddkv', blocks, 64 * waves, `char lds[tcmi::WindowPackedRows<${S}>::LDS]`, `window_packed_dkv<${S}, ${k}, ${v}>(${args}, ${out('dk')}, ${out('dv')}, ${ws}, lds, ${where})`, more));
-      else kernels.push(m('winwidedkv', blocks, 256, `char lds[tcmi::WindowBack<${S}>::LDS]`, `window_wide_dkv<${S}, ${k}, ${v}>(${args}, ${out('dk')}, ${out('dv')}, ${ws}, lds, ${where})`, more));
+      jobs.push({ HB, blocks: (few + (tiles - sinks) * CHUNKS) * heads, lds: (sizes) => (packed ? `tcmi::WindowPackedRows<${sizes}>::LDS` : `tcmi::WindowBack<${sizes}>::LDS`),
+        call: (sizes, block) => `${packed ? 'window_packed_dkv' : 'window_wide_dkv'}<${sizes}, ${k}, ${v}>(${args}, ${out('dk')}, ${out('dv')}, ${ws}, lds, ${where(block)})` });
     }
-    if (CHUNKS_MOST > 1) {
-      const n = z.B * z.KEYS * z.HK * z.DH, [blocks1] = add(n);
-      const call = (p, name, by) => `window_wide_join<${S}>(${out(p)}, reinterpret_cast<const float*>(${ws} + ${S}::${name}), ${L}, ${by}, blockIdx.x * 256u + threadIdx.x)`;
-      const calls = [[dk, 'dk', 'DKPARTS', `static_cast<float>(${S}::scale())`], [dv, 'dv', 'DVPARTS', '1.f']].filter((c) => c[0]).map(([, ...c]) => call(...c));
-      kernels.push(m('winadd', [blocks1, calls.length, 1], 256, null, calls.length > 1 ? `window_either<${S}>(blockIdx.y, [&] { tcmi::${calls[0]}; }, [&] { tcmi::${calls[1]}; })` : calls[0], more));
+    for (const [is, p, by] of [[dk, 'dk', `static_cast<float>(${S}::scale())`], [dv, 'dv', '1.f']]) {
+      if (is && CHUNKS_MOST > 1) joins.push({ blocks: add(z.B * z.KEYS * z.HK * z.DH), call: (sizes, block) => `window_wide_join<${sizes}>(${out(p)}, reinterpret_cast<const float*>(${ws} + ${sizes}::${p.toUpperCase()}PARTS), ${L}, ${by}, ${block} * 256u + threadIdx.x)` });
     }
   }
+  if (dq) {
+    const HB = blocksOf(hold, z.T * R, heads, ceil(z.WINDOW ? Math.min(z.KEYS, z.WINDOW) : z.KEYS, 64));
+    const rows = 16 * waves * HB, tiles = ceil(z.T * R, rows), lines = z.B * z.T * z.H;
+    const SPLITS = more.SPLITS = keySplits(z, rows, packed && hold ? 64 : 32, tiles * heads);
+    place4('DQPARTS', SPLITS > 1 ? SPLITS * lines * z.DH : 0);
+    const sums = (sizes) => `reinterpret_cast<float*>(${ws} + ${sizes}::DQPARTS)`;
+    const where = (block) => `${block} % ${heads}u, ${tiles - 1}u - ${block} / ${heads * SPLITS}u, ${block} / ${heads}u % ${SPLITS}u`;
+    jobs.push({ HB, blocks: tiles * heads * SPLITS, lds: (sizes) => (packed ? `tcmi::WindowPacked<${sizes}>::DQ` : `tcmi::WindowBack<${sizes}>::LDS`),
+      call: (sizes, block) => (packed ? `window_packed_dq<${sizes}>(${args}, ${out('dq')}, ${sums(sizes)}, ${ws}, lds, ${where(block)})`
+        : `window_wide_dq<${sizes}>(${args}, ${out('dq')}, ${sums(sizes)}, lds, ${where(block)})`) });
+    if (SPLITS > 1) joins.push({ blocks: add(lines * z.DH), call: (sizes, block) => `window_wide_add<${sizes}>(${out('dq')}, ${sums(sizes)}, ${block} * 256u + threadIdx.x)` });
+  }
+  for (const j of jobs.concat(joins)) j.more = Object.assign({}, more, { HB: j.HB || 1 });
+  kernels.push(m.jobs('winback', 64 * waves, jobs));
+  if (joins.length) kernels.push(m.jobs('winadd', 256, joins));
   return { kernels, workspace: at };
 }
 
