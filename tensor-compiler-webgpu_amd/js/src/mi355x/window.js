@@ -136,25 +136,36 @@ function packKeys(m, z, L, ws, more, heads, KP) {
 }
 
 /**
- * Tiles of 32 rows a chunk of a gradient of keys, `rows` of them a workgroup's: the fewest rounds of chunks over the `slots` workgroups that run at
- * once, each chunk with what four more tiles cost, and its sums' bytes.
+ * How the gradients are dealt out: CHUNK tiles of 32 rows of those that see one of `keyRows` keys a workgroup's, and SPLITS of the tiles of 32 keys
+ * that `rows` rows see, the gradients of keys before those of queries on the `slots` workgroups that run at once. A tile of the
+ * first is four products and about 3 us of heads of 64, one of the second three; a workgroup starts in the time of four tiles; the last ones end a
+ * quarter of one apart; a byte of sums is written and read at 5 TB/s in all. (9 heads of 1001 tokens in a window of 257: chunks of 8 tiles 105 us, of 12, which
+ * this takes, 92, of 16 102; 8192 tokens without a window: chunks from 70 to 200 within 1 %, by no splits 1360, by two 1245, by four 1256; two sequences of
+ * 1024 tokens, 16 heads of 128: by no splits, which this takes, 298, by two 300, by four 317.)
  */
-function rowChunk(z, rows, heads, slots) {
-  const R = z.H / z.HK, first = z.LAST ? z.KEYS - z.T : 0, counts = [];
-  for (let j = 0; j < z.KEYS; j += rows) {
-    const p0 = Math.max(j, first), last = Math.min(j + rows, z.KEYS) - 1;
+function deal(z, heads, slots, keyRows, rows) {
+  const R = z.H / z.HK, first = z.LAST ? z.KEYS - z.T : 0, counts = [], us = 3 * z.DH / 64;
+  for (let j = 0; j < z.KEYS; j += keyRows) {
+    const p0 = Math.max(j, first), last = Math.min(j + keyRows, z.KEYS) - 1;
     const p1 = Math.min(z.WINDOW && j >= z.SINKS ? Math.min(z.KEYS - 1, last + z.WINDOW - 1) : z.KEYS - 1, first + z.T - 1);
     counts.push(p0 <= p1 ? ceil((p1 - first + 1) * R, 32) - Math.floor((p0 - first) * R / 32) : 0);
   }
-  const most = counts.reduce((a, c) => Math.max(a, c), 1);
-  let best = null;
-  for (let chunk = Math.min(most, 8); ; chunk = Math.min(most, Math.ceil(chunk * 1.1))) {
-    const n = heads * counts.reduce((q, c) => q + Math.max(1, ceil(c, chunk)), 0), rounds = ceil(n, slots);
-    // (A tile takes about 3 us, of four products; a byte of sums is written and read at 5 TB/s in all.)
-    const time = (rounds < 3 ? rounds : Math.max(2, n / slots + 0.5)) * (chunk + 4) * 3 * z.DH / 64 + (n > heads * counts.length ? n * rows * z.DH * 16 / 5e6 : 0);
-    if (!best || time < best.time) best = { chunk, time };
-    if (chunk >= most) return best.chunk;
+  const most = counts.reduce((a, c) => Math.max(a, c), 1), work = 1.75 * heads * counts.reduce((a, c) => a + c, 0);
+  const time = (block, starts) => us * Math.max(block, (work + starts) / slots + block / 4);
+  let best = { time: Infinity };
+  for (let CHUNK = Math.min(most, 8); ; CHUNK = Math.min(most, Math.floor(CHUNK * 1.05) + 1)) {
+    const n = heads * counts.reduce((q, c) => q + Math.max(1, ceil(c, CHUNK)), 0);
+    const t = time(CHUNK + 4, 4 * n) + (n > heads * counts.length ? n * keyRows * z.DH * 16 / 5e6 : 0);
+    if (t < best.time) best = { CHUNK, time: t };
+    if (CHUNK >= most) break;
   }
+  const { CHUNK } = best, keys = ceil(z.WINDOW ? Math.min(z.KEYS, z.WINDOW + ceil(rows, R) + z.SINKS) : z.KEYS, 32), blocks = ceil(z.T * R, rows) * heads;
+  best = { time: Infinity };
+  for (let SPLITS = 1; SPLITS <= Math.max(1, Math.min(64, keys / 4)); SPLITS++) {
+    const t = time(0.75 * (keys / SPLITS + 4), 3 * blocks * SPLITS) + (SPLITS > 1 ? 5 + SPLITS * z.B * z.T * z.H * z.DH * 8 / 5e6 : 0);
+    if (t < best.time) best = { SPLITS, time: t };
+  }
+  return { CHUNK, SPLITS: best.SPLITS };
 }
 
 /** The launch that joins the splits of rows. */
@@ -232,21 +243,23 @@ function backwardKernels(s, parts, joined) {
   // The gradients of queries and of keys run side by side, and what joins their parts.
   const jobs = [], joins = [], waves = packed && z.DH > 64 ? 8 : 4;
   if (packed) more.WAVES = waves;
+  const keyBlocks = blocksOf(hold, z.KEYS, heads, ceil(Math.min(z.T, z.WINDOW || z.T) * R, 32)), rowBlocks = blocksOf(hold, z.T * R, heads, ceil(z.WINDOW ? Math.min(z.KEYS, z.WINDOW) : z.KEYS, 64));
+  const keyRows = 16 * waves * keyBlocks, rows = 16 * waves * rowBlocks;
+  // (Of heads above 64 a workgroup a CU, by its registers.)
+  const { CHUNK, SPLITS } = deal(z, heads, hold ? 2 * CUS : CUS, keyRows, rows);
   const place4 = (name, floats) => place(name, 4 * floats);
   if (dk || dv) {
     // Eight wavefronts where a packed tile takes most of LDS.
-    const HB = blocksOf(hold, z.KEYS, heads, ceil(Math.min(z.T, z.WINDOW || z.T) * R, 32));
-    const rows = 16 * waves * HB, tiles = ceil(z.KEYS, rows), all = ceil(z.T * R, 32), most = z.WINDOW ? Math.min(all, ceil((z.WINDOW + rows) * R, 32) + 1) : all;
-    const sinks = z.WINDOW ? Math.min(tiles, ceil(Math.min(z.SINKS, z.KEYS), rows)) : 0;
-    const CHUNK = rowChunk(z, rows, heads, waves === 8 ? CUS : 2 * CUS);
-    const CHUNKS = ceil(most, CHUNK), CHUNKS_MOST = sinks ? Math.max(CHUNKS, ceil(all, CHUNK)) : CHUNKS, FEW = Math.min(z.KEYS, sinks * rows);
-    Object.assign(more, { CHUNK, CHUNKS, CHUNKS_MOST, FEW, ROWS_EACH: rows });
+    const HB = keyBlocks, tiles = ceil(z.KEYS, keyRows), all = ceil(z.T * R, 32), most = z.WINDOW ? Math.min(all, ceil((z.WINDOW + keyRows) * R, 32) + 1) : all;
+    const sinks = z.WINDOW ? Math.min(tiles, ceil(Math.min(z.SINKS, z.KEYS), keyRows)) : 0;
+    const CHUNKS = ceil(most, CHUNK), CHUNKS_MOST = sinks ? Math.max(CHUNKS, ceil(all, CHUNK)) : CHUNKS, FEW = Math.min(z.KEYS, sinks * keyRows);
+    Object.assign(more, { CHUNK, CHUNKS, CHUNKS_MOST, FEW, ROWS_EACH: keyRows });
     const floats = CHUNKS_MOST > 1 ? (CHUNKS * z.KEYS + (CHUNKS_MOST - CHUNKS) * FEW) * z.B * z.HK * z.DH : 0;
     place4('DKPARTS', dk ? floats : 0);
     place4('DVPARTS', dv ? floats : 0);
     // The sinks' chunks, then the other tiles', the keys that most queries see first.
     const few = sinks * CHUNKS_MOST;
-    const where = (block) => [`(${block} / ${heads}u)`].map((id) => `${block} % ${heads}u, ${id} < ${few}u ? ${id} / ${CHUNKS_MOST}u : ${sinks}u + (${id} - ${few}u) / ${CHUNKS}u, ${id} < ${few}u ? ${id} % ${CHUNKS_MOST}u : (${id} - ${few}u) % ${CHUNKS}u`)[0];
+    const where = (block) => [`(${block} / ${heads}u)`].map((id) => `${block} % ${heads}u, ${id} < ${few}u ? ${id} / ${CHUNKS_MOST}u : ${sinks}u + (${id} - ${few}u) % ${Math.max(1, tiles - sinks)}u, ${id} < ${few}u ? ${id} % ${CHUNKS_MOST}u : (${id} - ${few}u) / ${Math.max(1, tiles - sinks)}u`)[0];
     // Both at once, or of the largest heads, which its registers do not hold both of, one after the other.
     for (const [k, v] of dk && dv && z.DH > 128 ? [[false, true], [true, false]] : [[dk, dv]]) {
       jobs.push({ HB, blocks: (few + (tiles - sinks) * CHUNKS) * heads, lds: (sizes) => (packed ? `tcmi::WindowPackedRows<${sizes}>::LDS` : `tcmi::WindowBack<${sizes}>::LDS`),
@@ -257,9 +270,8 @@ function backwardKernels(s, parts, joined) {
     }
   }
   if (dq) {
-    const HB = blocksOf(hold, z.T * R, heads, ceil(z.WINDOW ? Math.min(z.KEYS, z.WINDOW) : z.KEYS, 64));
-    const rows = 16 * waves * HB, tiles = ceil(z.T * R, rows), lines = z.B * z.T * z.H;
-    const SPLITS = more.SPLITS = keySplits(z, rows, packed && hold ? 64 : 32, tiles * heads);
+    const HB = rowBlocks, tiles = ceil(z.T * R, rows), lines = z.B * z.T * z.H;
+    more.SPLITS = SPLITS;
     place4('DQPARTS', SPLITS > 1 ? SPLITS * lines * z.DH : 0);
     const sums = (sizes) => `reinterpret_cast<float*>(${ws} + ${sizes}::DQPARTS)`;
     const where = (block) => `${block} % ${heads}u, ${tiles - 1}u - ${block} / ${heads * SPLITS}u, ${block} / ${heads}u % ${SPLITS}u`;
