@@ -566,8 +566,10 @@ __device__ __forceinline__ void window_packed_dkv(const WindowGradArgs a, float*
   const Minus minus;
   const int32_t mine = tile * W::ROWS + 16 * HB * wave;
   const WindowSeen<S> all(w, tile * W::ROWS, W::ROWS), own(w, mine, 16 * HB);
+  if (chunk < all.start()) return;
+  chunk -= all.start();
   if (chunk > 0u && chunk >= all.chunks()) return;
-  const int32_t begin = all.begin + static_cast<int32_t>(chunk * S::CHUNK), end = min(all.end, begin + static_cast<int32_t>(S::CHUNK));
+  const int32_t begin = all.from(chunk), end = all.to(chunk);
   char *qd = lds, *dd = qd + X::DOTS, *qs = dd + X::DOTS, *ds = qs + X::SUMS, *stats = ds + X::SUMS;
   auto dots = [&](int32_t i) __attribute__((always_inline)) {
     const size_t r0 = (size_t)i * NB;

@@ -547,7 +547,12 @@ struct WindowSeen {
       end = ((p1 - w.first + 1) * R + 31) / 32;
     }
   }
-  __device__ __forceinline__ uint32_t chunks() const { return (end - begin + S::CHUNK - 1u) / S::CHUNK; }
+  // Their chunks of CHUNK tiles: of a window's counted from the first tile, or of all rows', which the chunks of other keys share.
+  static constexpr bool SHARED = S::WINDOW == 0u;
+  __device__ __forceinline__ uint32_t start() const { return SHARED ? begin / S::CHUNK : 0u; }
+  __device__ __forceinline__ uint32_t chunks() const { return (end - (SHARED ? begin / S::CHUNK * S::CHUNK : begin) + S::CHUNK - 1u) / S::CHUNK; }
+  __device__ __forceinline__ int32_t from(uint32_t chunk) const { return SHARED ? max(begin, static_cast<int32_t>((start() + chunk) * S::CHUNK)) : begin + static_cast<int32_t>(chunk * S::CHUNK); }
+  __device__ __forceinline__ int32_t to(uint32_t chunk) const { return min(end, static_cast<int32_t>(SHARED ? (start() + chunk + 1u) * S::CHUNK : begin + (chunk + 1u) * S::CHUNK)); }
 };
 
 // The sums of a lane's keys to dk and dv, or to chunk `chunk` of their parts: [c][keys][DH] for c < CHUNKS, and for more (keys below
@@ -597,9 +602,11 @@ __device__ __forceinline__ void window_wide_dkv(const WindowGradArgs a, float* _
   Parts kf[HB][SLICES], vf[HB][SLICES];
   f4 dka[HB][G], dva[HB][G];
   const WindowSeen<S> all(w, j0, W::ROWS), own(w, mine, 16 * HB);
+  if (chunk < all.start()) return;
+  chunk -= all.start();
   if (chunk > 0u && chunk >= all.chunks()) return;
   const int32_t p0 = all.p0, p1 = all.p1, m0 = own.p0, m1 = own.p1;
-  const int32_t begin = all.begin + static_cast<int32_t>(chunk * S::CHUNK), end = min(all.end, begin + static_cast<int32_t>(S::CHUNK));
+  const int32_t begin = all.from(chunk), end = all.to(chunk);
 #pragma unroll
   for (int h = 0; h < HB; ++h) {
     key[h] = mine + 16 * h + t;

@@ -139,9 +139,9 @@ function packKeys(m, z, L, ws, more, heads, KP) {
  * How the gradients are dealt out: CHUNK tiles of 32 rows of those that see one of `keyRows` keys a workgroup's, and SPLITS of the tiles of 32 keys
  * that `rows` rows see, the gradients of keys before those of queries on the `slots` workgroups that run at once. A tile of the
  * first is four products and about 3 us of heads of 64, one of the second three; a workgroup starts in the time of four tiles; the last ones end a
- * quarter of one apart; a byte of sums is written and read at 5 TB/s in all. (9 heads of 1001 tokens in a window of 257: chunks of 8 tiles 105 us, of 12, which
- * this takes, 92, of 16 102; 8192 tokens without a window: chunks from 70 to 200 within 1 %, by no splits 1360, by two 1245, by four 1256; two sequences of
- * 1024 tokens, 16 heads of 128: by no splits, which this takes, 298, by two 300, by four 317.)
+ * sixth of one apart; a byte of sums is written and read at 5 TB/s in all. (9 heads of 1001 tokens in a window of 257: chunks of 8 tiles 105 us, of 12 (this takes
+ * 13) 92, of 16 102; 8192 tokens of 8 heads: chunks of 50 tiles 1271, of 94 1220, of 128 1208, by no splits 1360, by two 1245, by four 1256; two
+ * sequences of 1024 tokens, 16 heads of 128: by no splits 298, by two 300, by four 317.)
  */
 function deal(z, heads, slots, keyRows, rows) {
   const R = z.H / z.HK, first = z.LAST ? z.KEYS - z.T : 0, counts = [], us = 3 * z.DH / 64;
@@ -151,7 +151,7 @@ function deal(z, heads, slots, keyRows, rows) {
     counts.push(p0 <= p1 ? ceil((p1 - first + 1) * R, 32) - Math.floor((p0 - first) * R / 32) : 0);
   }
   const most = counts.reduce((a, c) => Math.max(a, c), 1), work = 1.75 * heads * counts.reduce((a, c) => a + c, 0);
-  const time = (block, starts) => us * Math.max(block, (work + starts) / slots + block / 4);
+  const time = (block, starts) => us * Math.max(block, (work + starts) / slots + block / 6);
   let best = { time: Infinity };
   for (let CHUNK = Math.min(most, 8); ; CHUNK = Math.min(most, Math.floor(CHUNK * 1.05) + 1)) {
     const n = heads * counts.reduce((q, c) => q + Math.max(1, ceil(c, CHUNK)), 0);
@@ -246,7 +246,7 @@ function backwardKernels(s, parts, joined) {
   const keyBlocks = blocksOf(hold, z.KEYS, heads, ceil(Math.min(z.T, z.WINDOW || z.T) * R, 32)), rowBlocks = blocksOf(hold, z.T * R, heads, ceil(z.WINDOW ? Math.min(z.KEYS, z.WINDOW) : z.KEYS, 64));
   const keyRows = 16 * waves * keyBlocks, rows = 16 * waves * rowBlocks;
   // (Of heads above 64 a workgroup a CU, by its registers.)
-  const { CHUNK, SPLITS } = deal(z, heads, hold ? 2 * CUS : CUS, keyRows, rows);
+  const { CHUNK, SPLITS } = deal(z, heads, (hold ? 2 : 1) * CUS, keyRows, rows);
   const place4 = (name, floats) => place(name, 4 * floats);
   if (dk || dv) {
     // Eight wavefronts where a packed tile takes most of LDS.
@@ -257,12 +257,16 @@ function backwardKernels(s, parts, joined) {
     const floats = CHUNKS_MOST > 1 ? (CHUNKS * z.KEYS + (CHUNKS_MOST - CHUNKS) * FEW) * z.B * z.HK * z.DH : 0;
     place4('DKPARTS', dk ? floats : 0);
     place4('DVPARTS', dv ? floats : 0);
-    // The sinks' chunks, then the other tiles', the keys that most queries see first.
-    const few = sinks * CHUNKS_MOST;
-    const where = (block) => [`(${block} / ${heads}u)`].map((id) => `${block} % ${heads}u, ${id} < ${few}u ? ${id} / ${CHUNKS_MOST}u : ${sinks}u + (${id} - ${few}u) % ${Math.max(1, tiles - sinks)}u, ${id} < ${few}u ? ${id} % ${CHUNKS_MOST}u : (${id} - ${few}u) / ${Math.max(1, tiles - sinks)}u`)[0];
+    // The sinks' chunks, then the other tiles', the keys that most queries see first. (Workgroups go to the XCDs in turn: an odd number of chunks a
+    // tile, one more than there are where that is even, gives each of them first and last ones alike. 512 tokens of 8 heads 93.6 us, 89.4 so.)
+    const few = sinks * CHUNKS_MOST, ODD = CHUNKS | 1;
+    const where = (block) => {
+      const id = `(${block} / ${heads}u)`, at = `(${id} - ${few}u)`;
+      return `${block} % ${heads}u, ${id} < ${few}u ? ${id} / ${CHUNKS_MOST}u : ${sinks}u + ${at} / ${ODD}u, ${id} < ${few}u ? ${id} % ${CHUNKS_MOST}u : ${at} % ${ODD}u`;
+    };
     // Both at once, or of the largest heads, which its registers do not hold both of, one after the other.
     for (const [k, v] of dk && dv && z.DH > 128 ? [[false, true], [true, false]] : [[dk, dv]]) {
-      jobs.push({ HB, blocks: (few + (tiles - sinks) * CHUNKS) * heads, lds: (sizes) => (packed ? `tcmi::WindowPackedRows<${sizes}>::LDS` : `tcmi::WindowBack<${sizes}>::LDS`),
+      jobs.push({ HB, blocks: (few + (tiles - sinks) * ODD) * heads, lds: (sizes) => (packed ? `tcmi::WindowPackedRows<${sizes}>::LDS` : `tcmi::WindowBack<${sizes}>::LDS`),
         call: (sizes, block) => `${packed ? 'window_packed_dkv' : 'window_wide_dkv'}<${sizes}, ${k}, ${v}>(${args}, ${out('dk')}, ${out('dv')}, ${ws}, lds, ${where(block)})` });
     }
     for (const [is, p, by] of [[dk, 'dk', `static_cast<float>(${S}::scale())`], [dv, 'dv', '1.f']]) {
