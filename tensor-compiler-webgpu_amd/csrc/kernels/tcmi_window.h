@@ -8,13 +8,17 @@
 // NaN of o and lse of the queries that see it, and a query's row with one (dy's too) of the gradients of the keys it sees; what does not
 // see them, or is not seen, is as without them: 0 times them is taken as 0 (they are read as 0 where a sum runs over them).
 //
-// Rows: the queries of the R = H/HK heads that share a key head, query t's heads side by side, 16 rows a tile; keys 16 a
+// Rows: the queries of the R = H/HK heads that share a key head, query t's heads side by side. Here up to 16 of them, single tokens over a cache,
+// on the fp32 matrix cores; more are tcmi_window_wide.h's, and all gradients. Keys 16 a
 // tile. With lane = 16·q + t (t in 0..15) of a 16x16x4 product:
 //   scores   mfma(key value, row value): lane (t, q) holds row t, keys 4q ... 4q + 3, which is
 //   output   mfma(V value, P value): the second product's operand for those keys; lane (t, q) gets row t, dims 16g + 4q ....
-// (The gradients of keys exchange the parts of rows and keys.) So scores never leave the registers, and keys and values are read
+// So scores never leave the registers, and keys and values are read
 // from memory as the products take them. The four wavefronts of a workgroup deal the tiles among them and join at the
-// end through LDS, always in the same order; of few rows, several workgroups do (SPLITS), whose sums are joined by a launch.
+// end through LDS, always in the same order; several workgroups do (SPLITS), whose sums are joined by a launch.
+//
+// Bound: HBM (the keys and values that are seen, read once). 8 heads of 64 by 2 over caches of 131072 keys, 4 sequences: 101 us (5.3 TB/s) with 5 of them to
+// join 128 splits; over 1024 keys and 4 of 32 sequences (34 MB) 12 and 4: the loads' time of a few tiles a wavefront, and the second launch's.
 
 #pragma once
 
@@ -98,9 +102,6 @@ __device__ __forceinline__ void window_store(float* __restrict__ p, uint32_t d, 
     }
   }
 }
-
-// x, or 0 where it is not finite.
-__device__ __forceinline__ float window_finite(float x) { return __builtin_isfinite(x) ? x : 0.f; }
 
 // Lane (t, q)'s part of a 16 x DH tile along its rows: dims 16g + 4q ... of row t.
 template <class S, int G>
@@ -322,153 +323,6 @@ __device__ __forceinline__ void window_join(float* __restrict__ out, float* __re
     for (uint32_t p = 1; p < PARTS; ++p) sum += all[p * LANES + lane];
   }
   window_store<S>(out + line * S::DH, 4u * lane, sum * inv);
-}
-
-struct WindowGradArgs {
-  const float *q, *k, *v, *lengths, *o, *lse, *dy, *mass;
-};
-
-// mass[line] = dy·o of one head of one query: 16 lanes a line.
-template <class S>
-__device__ __forceinline__ void window_mass(const float* __restrict__ o, const float* __restrict__ dy, float* __restrict__ mass, size_t line) {
-  constexpr size_t LINES = (size_t)S::B * S::T * S::H;
-  const uint32_t lane = threadIdx.x & 15u;
-  const size_t at = min(line, LINES - 1u);
-  float sum = 0.f;
-  for (uint32_t d = 4u * lane; d < S::DH; d += 64u) {
-    const f4 x = window_load<S>(o + at * S::DH, d, true), y = window_load<S>(dy + at * S::DH, d, true);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) sum = fmaf(x[i], y[i], sum);
-  }
-  sum = group_reduce<false, 16>(sum);
-  if (lane == 0u && line < LINES) mass[line] = sum;
-}
-
-// Workgroup: a tile of rows of a sequence's key head.
-template <class S>
-__device__ __forceinline__ void window_dq(const WindowGradArgs a, float* __restrict__ dq, float* lds, uint32_t wg) {
-  constexpr int G = (S::DH + 15) / 16;
-  using Span = WindowSpan<S>;
-  constexpr uint32_t R = Span::R, ROWS = Span::ROWS;
-  const uint32_t tile = wg % S::TILES, head = wg / S::TILES, b = head / S::HK, hk = head % S::HK;
-  const int lane = threadIdx.x & 63, t = lane & 15, q = lane >> 4, wave = threadIdx.x >> 6;
-  const Span w(a.lengths, b);
-  const uint32_t row0 = tile * 16u, row = row0 + t, at = min(row, ROWS - 1u);
-  const size_t line = ((size_t)b * S::T + at / R) * S::H + hk * R + at % R;
-  const int32_t p = w.first + static_cast<int32_t>(at / R);
-  const bool on = row < ROWS && w.stands(p);
-  const float scale = static_cast<float>(S::scale() * 1.4426950408889634);
-  f4 qf[G], df[G], acc[G];
-  window_along<S>(qf, a.q + line * S::DH, on);
-  window_along<S>(df, a.dy + line * S::DH, on);
-  const float lse = on ? a.lse[line] * LOG2E : 0.f, mass = on ? a.mass[line] : 0.f;
-#pragma unroll
-  for (int g = 0; g < G; ++g) acc[g] = f4{0.f, 0.f, 0.f, 0.f};
-  const WindowTiles tiles = window_keys(w, row0, min(row0 + 15u, ROWS - 1u));
-  const size_t step = (size_t)S::HK * S::DH, base = ((size_t)b * S::KEYS * S::HK + hk) * S::DH;
-  for (int32_t i = wave; i < tiles.all; i += 4) {
-    const int32_t j0 = tiles.at(i) * 16;
-    f4 f[G];
-    window_along<S>(f, a.k + base + (size_t)min(j0 + t, w.length - 1) * step, j0 + t < w.length);
-    f4 s = window_scores(f, qf);
-    window_along<S>(f, a.v + base + (size_t)min(j0 + t, w.length - 1) * step, j0 + t < w.length);
-    const f4 dp = window_scores(f, df);
-    window_read<S>(f, a.k + base, step, j0, tiles);
-    window_clean<S>(f, j0, tiles);
-#pragma unroll
-    for (int r = 0; r < 4; ++r) s[r] = on && w.sees(p, j0 + 4 * q + r) ? __builtin_amdgcn_exp2f(fmaf(s[r], scale, -lse)) * (dp[r] - mass) : 0.f;
-    window_sum(acc, f, s);
-  }
-  window_gather(acc, 1.f, lds);
-  if (wave != 0 || row >= ROWS) return;
-#pragma unroll
-  for (int g = 0; g < G; ++g) window_store<S>(dq + line * S::DH, 16 * g + 4 * q, acc[g] * static_cast<float>(S::scale()));
-}
-
-// Workgroup: a tile of keys of a sequence's key head.
-template <class S, bool DK, bool DV>
-__device__ __forceinline__ void window_dkv(const WindowGradArgs a, float* __restrict__ dk, float* __restrict__ dv, float* lds, uint32_t wg) {
-  constexpr int G = (S::DH + 15) / 16;
-  using Span = WindowSpan<S>;
-  constexpr int32_t R = Span::R, ROWS = Span::ROWS;
-  const uint32_t tile = wg % S::KTILES, head = wg / S::KTILES, b = head / S::HK, hk = head % S::HK;
-  const int lane = threadIdx.x & 63, t = lane & 15, q = lane >> 4, wave = threadIdx.x >> 6;
-  const Span w(a.lengths, b);
-  const int32_t j0 = tile * 16, j = j0 + t, last = min(j0 + 15, w.length - 1);
-  const size_t key = ((size_t)b * S::KEYS + min(j, static_cast<int32_t>(S::KEYS) - 1)) * S::HK + hk;
-  const float scale = static_cast<float>(S::scale() * 1.4426950408889634);
-  f4 kf[G], vf[G], dka[G], dva[G];
-  window_along<S>(kf, a.k + key * S::DH, j < w.length);
-  window_along<S>(vf, a.v + key * S::DH, j < w.length);
-#pragma unroll
-  for (int g = 0; g < G; ++g) dka[g] = dva[g] = f4{0.f, 0.f, 0.f, 0.f};
-  // The positions that see one of the keys: from the first key on, up to the last one's window or the sequence's end.
-  int32_t p0 = max(j0, w.first), p1 = w.length - 1;
-  if (S::WINDOW != 0u && j0 >= static_cast<int32_t>(S::SINKS) && p1 - last >= static_cast<int32_t>(S::WINDOW)) p1 = last + static_cast<int32_t>(S::WINDOW) - 1;
-  p1 = min(p1, w.first + static_cast<int32_t>(S::T) - 1);
-  const int32_t begin = p0 <= p1 && j0 < w.length ? (p0 - w.first) * R / 16 : 0, end = p0 <= p1 && j0 < w.length ? ((p1 - w.first + 1) * R + 15) / 16 : 0;
-  const size_t top = ((size_t)b * S::T) * S::H + hk * R;
-  auto line = [&](int32_t r) { return top + (size_t)(r / R) * S::H + r % R; };
-  for (int32_t i = begin + wave; i < end; i += 4) {
-    const int32_t r0 = i * 16;
-    f4 x[G];
-    const bool on = r0 + t < ROWS && w.stands(w.first + (r0 + t) / R);
-    const size_t mine = line(min(r0 + t, ROWS - 1));
-    window_along<S>(x, a.q + mine * S::DH, on);
-    f4 s = window_scores(x, kf);
-    f4 dp;
-    if constexpr (DK) {
-      window_along<S>(x, a.dy + mine * S::DH, on);
-      dp = window_scores(x, vf);
-    }
-    // Rows 4q ... of this lane.
-    size_t at[4];
-    bool in[4];
-    float mass[4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int32_t row = r0 + 4 * q + r;
-      at[r] = line(min(row, ROWS - 1));
-      const int32_t p = w.first + row / R;
-      in[r] = row < ROWS && p >= p0 && p <= p1;
-      mass[r] = in[r] ? a.mass[at[r]] : 0.f;
-      // (NaN where q or dy hold a number that is not finite.)
-      const float lse = in[r] ? LOG2E * a.lse[at[r]] + 0.f * mass[r] : 0.f;
-      s[r] = in[r] && j < w.length && w.sees(p, j) ? __builtin_amdgcn_exp2f(fmaf(s[r], scale, -lse)) : 0.f;
-    }
-    if constexpr (DV) {
-#pragma unroll
-      for (int g = 0; g < G; ++g) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) x[g][r] = window_finite(in[r] && 16 * g + t < static_cast<int>(S::DH) ? a.dy[at[r] * S::DH + 16 * g + t] : 0.f);
-      }
-      window_sum(dva, x, s);
-    }
-    if constexpr (DK) {
-#pragma unroll
-      for (int g = 0; g < G; ++g) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) x[g][r] = window_finite(in[r] && 16 * g + t < static_cast<int>(S::DH) ? a.q[at[r] * S::DH + 16 * g + t] : 0.f);
-      }
-#pragma unroll
-      for (int r = 0; r < 4; ++r) s[r] = s[r] != 0.f ? s[r] * (dp[r] - mass[r]) : 0.f;
-      window_sum(dka, x, s);
-    }
-  }
-  if constexpr (DK) {
-    window_gather(dka, static_cast<float>(S::scale()), lds);
-    if (wave == 0 && j < static_cast<int32_t>(S::KEYS)) {
-#pragma unroll
-      for (int g = 0; g < G; ++g) window_store<S>(dk + key * S::DH, 16 * g + 4 * q, dka[g]);
-    }
-  }
-  if constexpr (DV) {
-    window_gather(dva, 1.f, lds);
-    if (wave == 0 && j < static_cast<int32_t>(S::KEYS)) {
-#pragma unroll
-      for (int g = 0; g < G; ++g) window_store<S>(dv + key * S::DH, 16 * g + 4 * q, dva[g]);
-    }
-  }
 }
 
 }  // namespace tcmi

@@ -14,6 +14,13 @@
 //
 // The kernels' layout is tcmi_window_wide.h's. A tile's dots are copied while the sums before them are multiplied, and its sums while the
 // dots are: each form has one place in LDS, and a barrier after each of the two halves of a tile.
+//
+// Bound: the matrix cores. A library's bf16 product of 8192 x 8192 x 8192 reaches 1310 TFLOP/s here, which is 291 of these forward products (three of halves and
+// six of bf16 for two), and 218 of the gradients' (30 for five, as scores and dy·v are formed for queries and for keys).
+//   two sequences of 16384 tokens, 16 heads of 128 by 4, a window of 1024    1090 us (253 TFLOP/s), 48 to split keys and values
+//   8192 tokens, 8 heads of 64 by 2: 310 us (221 TFLOP/s) and 9 to join two splits; its gradients 830 (207) and 28 to split, 21 to join
+// Of the cycles the matrix cores are busy in 53 %: the rest are the softmax, the split of P and dS into parts and the barriers, which two wavefronts a
+// SIMD do not hide whole. Taking the next tile's scores beside this one's softmax needs their registers twice: 313 us of 320 at heads of 64, and spilled at 128.
 
 #pragma once
 
@@ -181,7 +188,7 @@ __device__ __forceinline__ void window_pack_both(const WindowGradArgs a, char* w
 
 // Copies of 16 bytes (4: one word) a lane from `from` on to LDS from `to` on (both uniform), in flight until vmcnt reaches 0. Written as
 // instructions: of the compiler's own it takes every later read of LDS to depend on them, and waits for them there (of a gradient of keys
-// twice a tile: 950 us, 757 so). They have no register results, and a wait that the compiler counts without them is only
+// twice a tile: 950 us, 908 so). They have no register results, and a wait that the compiler counts without them is only
 // longer for them; barrier_ahead() is what the tiles' readers wait at.
 __device__ __forceinline__ void window_copy16(uint32_t to, const char* from) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"((threadIdx.x & 63u) * 16u), "s"(from) : "memory", "m0");
@@ -218,6 +225,7 @@ __device__ __forceinline__ void window_pair_lines(const char* tile, int line0, i
 }
 template <class T, int HB, int BLOCKS, int SLICES>
 __device__ __forceinline__ void window_pair_dots(f4 (&acc)[HB][BLOCKS], const char* tile, const Pair8 (&f)[HB][SLICES]) {
+  // (The wavefront that multiplies goes before the one beside it: forward 349 -> 320 us of 8192 tokens.)
   __builtin_amdgcn_s_setprio(1);
 #pragma unroll
   for (int k = 0; k < BLOCKS; ++k) {

@@ -14,6 +14,13 @@
 //            ds_read_b64_tr_b16, 4 keys of each lane's dim at a time.
 // A tile's output is summed from 0 and joined to the rows' by one multiplication and addition with their change of maximum, so an
 // accumulator is rounded once a tile.
+//
+// The gradients: tiles of 32 rows or keys; a gradient of queries walks the keys that its rows see, one of keys the rows that see its keys, in chunks, and
+// each forms the scores again (seven products in all where five would do, but no sum is left to be joined over workgroups that
+// do not share its lines). Both run side by side in one launch.
+//
+// Bound: few tiles a workgroup, with each its loads' time, its split into parts and two barriers; of longer sequences the matrix cores (tcmi_window_packed.h).
+// 64 sequences of 128 tokens, 4 heads of 64: 11.5 us, with the gradients' 27; six bf16 products at the rate of a large one would take 2 and 5, the bytes 3 and 9.
 
 #pragma once
 
@@ -367,6 +374,7 @@ __device__ __forceinline__ void window_dots(f4 (&acc)[HB][BLOCKS], const char* t
 // acc[h][g] += the sums over a tile's lines of its floats 16g ... times f[h].
 template <class T, int HB, int G, int PAIRS>
 __device__ __forceinline__ void window_sums(f4 (&acc)[HB][G], const char* tile, const Parts (&f)[HB][PAIRS]) {
+  // (The wavefront that multiplies goes before one that loads or forms parts.)
   __builtin_amdgcn_s_setprio(1);
 #pragma unroll
   for (int g = 0; g < G; g += 2) {
@@ -401,6 +409,10 @@ __device__ __forceinline__ void window_line(Parts (&f)[SLICES], const float* __r
     window_parts(x * scale, y * scale, minus, f[s]);
   }
 }
+
+struct WindowGradArgs {
+  const float *q, *k, *v, *lengths, *o, *lse, *dy, *mass;
+};
 
 // dy·o of a row, whose floats 32·s + 8q ... lane (t, q) adds up; every lane of the row gets it.
 template <class S>

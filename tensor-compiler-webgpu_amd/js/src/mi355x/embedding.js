@@ -42,11 +42,13 @@ function lowerEmbedding(graph, node) {
   return { kind: 'embedding', kernels: [k], workspace: 0 };
 }
 
-// Keys that one workgroup sorts, of 1024 threads; beyond, tiles of them are sorted by 256.
-const ONE_TILE = 16384;
+// Keys that one workgroup sorts, of 1024 threads; beyond, tiles of them are sorted by 256. (Gradients of 2000 tokens over 1000 rows 22.7 us by one, 26.7 by
+// tiles; of 4096 27.0 and 25.2; of 16384 57.7 and 32.9.)
+const ONE_TILE = 2048;
 
 /**
- * Rows of a table that a wavefront keeps for itself, four wavefronts' in LDS: 8192 tokens of 256 floats over 96 rows 20.5 us by sorted tokens, 12 so.
+ * Rows of a table that a wavefront keeps for itself, four wavefronts' in LDS, which holds no more: with rows and gradients, 8192 tokens of 256 floats over 96 rows
+ * 23.8 us by sorted tokens, 14.0 so, over 128 23.6 and 15.3; 65536 tokens of 1024 over 128 149 and 153.
  */
 const FEW_ROWS = 128;
 

@@ -59,8 +59,12 @@ function grid(n) {
   return [n, 1, 1];
 }
 
-/** Rows of a key head from which 128 of them are a workgroup's (tcmi_window_wide.h). */
-const WIDE_ROWS = 64;
+/**
+ * Rows of a key head that tcmi_window.h takes, a tile of it: more of them are a workgroup's of tcmi_window_wide.h, which reads the keys once for all. (16
+ * rows over 4096 keys, heads of 64: 32.6 us by the first, 43.6 by the second; 20 rows, heads of 128: 71 and 45. The gradients are the second's for any
+ * rows: 8 tokens of 64 sequences, heads of 64, 16.4 us by the first's way, 9.1 by the second's; 1 over 8000 keys 460 and 64.)
+ */
+const FEW_ROWS = 16;
 
 /**
  * Workgroups that a chip's worth is: two a CU run at once, and as many wait, so that those that see many keys leave no CU idle
@@ -76,7 +80,8 @@ function blocksOf(hold, lines, heads, tiles) { return hold && ceil(lines, 128) *
 
 /**
  * Whether operands are split by a launch of their own (tcmi_window_packed.h), not by each workgroup that reads them (tcmi_window_wide.h): where
- * four workgroups or more read a key, by its registers for heads up to 128.
+ * four workgroups or more read a key, by its registers for heads up to 128. (With gradients, heads of 64: windows of 512 266 us packed, 298 otherwise, 4
+ * sequences of 512 tokens without one 67 and 64, of 768 111 and 119; heads of 128, 2 of 896 tokens: 153 and 190.)
  */
 const packs = (z) => z.DH <= 128 && ceil(Math.min(z.T, z.WINDOW || z.T) * (z.H / z.HK), 128) >= 4;
 
@@ -88,12 +93,13 @@ const formBytes = (z, lines, planes) => z.B * z.HK * lines * lanesOf(z.DH) * 16 
 
 /**
  * Splits of the tiles of NB keys that `rows` rows of one head see, of `blocks` workgroups otherwise: eight tiles each or more, four where there would be
- * fewer than two workgroups a CU (288 workgroups of ten tiles, each with its loads' time: 22 us, by halves 14 and 4 to join them).
+ * fewer than two workgroups a CU (288 workgroups of ten tiles, each with its loads' time: 22 us, by halves 15 and 5 to join them; by fifths 30 in all), two
+ * where there would be fewer than one (80 workgroups of ten tiles: by halves 20 us in all, by fifths 15, by tenths 18).
  */
 function keySplits(z, rows, NB, blocks) {
   const R = z.H / z.HK;
   const most = ceil(z.WINDOW ? Math.min(z.KEYS, z.WINDOW + ceil(rows, R) + z.SINKS) : z.KEYS, NB);
-  return Math.max(1, Math.min(64, Math.floor(most / (blocks < 2 * CUS ? 4 : 8)), ceil(FILL, blocks)));
+  return Math.max(1, Math.min(64, Math.floor(most / (blocks < CUS ? 2 : blocks < 2 * CUS ? 4 : 8)), ceil(FILL, blocks)));
 }
 
 function wideForward(s, parts, joined) {
@@ -179,7 +185,7 @@ function joinKernel(m, z, out, ws, more, heads) {
 
 function forwardKernels(s, parts, joined) {
   const { z } = s, e = entry(joined ? parts : null);
-  if (z.T * (z.H / z.HK) >= WIDE_ROWS) return wideForward(s, parts, joined);
+  if (z.T * (z.H / z.HK) > FEW_ROWS) return wideForward(s, parts, joined);
   const R = z.H / z.HK, TILES = ceil(z.T * R, 16), heads = z.B * z.HK;
   // The keys that one tile sees at most, in tiles of 16, dealt to as many workgroups as fill the chip four times, eight tiles each or more.
   // (32 tokens of 8 heads over 1028 keys: 16.8 us by nine tiles, 21.6 by five.)
@@ -202,25 +208,18 @@ function forwardKernels(s, parts, joined) {
 
 function backwardKernels(s, parts, joined) {
   const { z } = s, e = entry(joined ? parts : null);
-  const R = z.H / z.HK, heads = z.B * z.HK, wide = z.T * R >= WIDE_ROWS;
+  const R = z.H / z.HK, heads = z.B * z.HK;
   const out = (p) => (parts.includes(p) ? e.out(p) : 'nullptr');
   const L = s.lengths ? 'A.in[3]' : 'nullptr', first = s.lengths ? 4 : 3;
   const args = `{A.in[0], A.in[1], A.in[2], ${L}, A.in[${first}], A.in[${first + 1}], A.in[${first + 2}], ${e.ws}}`;
   const dq = parts.includes('dq'), dk = parts.includes('dk'), dv = parts.includes('dv');
   const types = { HB: 'int' }, more = {};
   // dy·o of every row, where the gradients of keys do not form it.
-  const masses = !wide || (z.DH > 128 && (dk || dv));
+  const masses = z.DH > 128 && (dk || dv);
   let at = masses ? align(4 * z.B * z.T * z.H, 256) : 0;
   const place = (name, bytes) => { more[name] = at; types[name] = 'size_t'; at = align(at + bytes, 256); };
   const m = maker(s, e, types), ws = `reinterpret_cast<char*>(${e.ws})`;
   const kernels = [];
-  if (!wide) kernels.push(m('winmass', grid(ceil(z.B * z.T * z.H, 16)), 256, null, `window_mass<${S}>(A.in[${first}], A.in[${first + 2}], ${e.ws}, blockIdx.x * 16u + threadIdx.x / 16u)`));
-  if (!wide) {
-    const TILES = ceil(z.T * R, 16), KTILES = ceil(z.KEYS, 16), lds = `float lds[tcmi::window_lds<${z.DH}>()]`;
-    if (dq) kernels.push(m('windq', grid(TILES * heads), 256, lds, `window_dq<${S}>(${args}, ${out('dq')}, lds, blockIdx.x)`, { TILES }));
-    if (dk || dv) kernels.push(m('windkv', grid(KTILES * heads), 256, lds, `window_dkv<${S}, ${dk}, ${dv}>(${args}, ${out('dk')}, ${out('dv')}, lds, blockIdx.x)`, { KTILES }));
-    return { kernels, workspace: at };
-  }
   const add = (n) => ceil(z.DH % 4 ? n : n / 4, 256), KP = align(z.KEYS, 64), RP = align(z.T * R, 64), packed = packs(z), lanes = lanesOf(z.DH);
   const hold = z.DH <= 64;
   if (packed) {

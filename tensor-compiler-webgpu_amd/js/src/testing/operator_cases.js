@@ -283,7 +283,7 @@ const FORMS = [
   orth('twice', [96, 100], { twice: true, count: 2, options: { steps: 2 } }),
   // Attention of few rows, of many, of many that share their split operands; heads of whole tiles and not. With gradients, and without.
   ...[false, true].reduce((all, gradient) => all.concat([
-    ['few', [2, 9, 4, 24], [2, 30, 2, 24], { window: 11, sinks: 2 }], ['few-whole', [1, 13, 2, 64], [1, 13, 2, 64], {}],
+    ['few', [2, 5, 6, 24], [2, 30, 2, 24], { window: 11, sinks: 2 }], ['more', [2, 9, 4, 24], [2, 30, 2, 24], { window: 11, sinks: 2 }], ['few-whole', [1, 13, 2, 64], [1, 13, 2, 64], {}],
     ['wide', [2, 80, 2, 64], [2, 80, 2, 64], { window: 37, sinks: 3 }], ['wide-large', [1, 70, 2, 160], [1, 70, 2, 160], {}],
     ['packed', [1, 300, 4, 64], [1, 300, 2, 64], { window: 260, sinks: 5 }], ['packed-odd', [1, 280, 4, 40], [1, 280, 2, 40], {}],
   ].map(([name, q, k, options]) => window(`window-${name}${gradient ? '' : '-forward'}`, q, k, options, { gradient }))), []),

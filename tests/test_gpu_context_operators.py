@@ -73,8 +73,8 @@ def window_inputs(tool, form, seed):
     return q, k, {n: rng.standard_normal(s).astype(np.float32) for n, s in (("q", q), ("k", k), ("v", k), ("d0", q))}
 
 
-# Of few rows, of many, of many that share their split operands; heads of whole tiles and not.
-FORMS = ["few", "few-whole", "wide", "wide-large", "packed", "packed-odd"]
+# Of a tile of rows or less, of more, of many that share their split operands; heads of whole tiles and not.
+FORMS = ["few", "few-whole", "more", "wide", "wide-large", "packed", "packed-odd"]
 
 
 @pytest.mark.parametrize("form", FORMS)
