@@ -4,8 +4,8 @@
 // nothing to the others; parts below bf16's least normal number, of values below 2^-102, are lost, and values from 2^128 - 2^119 on, which
 // bf16 rounds to infinity, count as infinite.
 //
-// A workgroup's four wavefronts take 32 rows each (tcmi_window.h's rows: the queries of the heads that share a key head) and walk
-// the tiles of NB keys that one of the 128 sees. A tile is loaded one ahead into registers, split by the thread that loaded it and
+// A workgroup's four wavefronts take 16 rows each (tcmi_window.h's rows: the queries of the heads that share a key head; HB = 1 here) and walk
+// the tiles of NB keys that one of the 64 sees. A tile is loaded one ahead into registers, split by the thread that loaded it and
 // kept in LDS as three planes. With lane = 16·q + t of a 16 x 16 x 32 product, whose operands are lines of 32 along the
 // sum (8q ... of line t) and whose result is (lines 4q ... of the first, line t of the second):
 //   scores   first operand K (lines: keys; the sum: dims), second Q: lane (t, q) holds row t, keys 4q ... of each 16;

@@ -74,7 +74,8 @@ const FILL = 4 * CUS;
 
 /**
  * Blocks of 16 lines of a wavefront's own, of `lines` of a head over `tiles` tiles of the other side: two where its registers `hold` them and two
- * workgroups a CU are left, of which several may deal the tiles among them, eight each or more.
+ * workgroups a CU are left, of which several may deal the tiles among them, eight each or more. Of packed operands alone: where a workgroup splits
+ * what it reads, one is faster (4 sequences of 4000 tokens, 8 heads of 64, a window of 100 62 us by two, 53 by one; gradients of 2000 tokens 152 and 134).
  */
 function blocksOf(hold, lines, heads, tiles) { return hold && ceil(lines, 128) * heads * Math.max(1, Math.min(8, Math.floor(tiles / 8))) >= 2 * CUS ? 2 : 1; }
 
@@ -104,7 +105,7 @@ function keySplits(z, rows, NB, blocks) {
 
 function wideForward(s, parts, joined) {
   const { z } = s, e = entry(joined ? parts : null), heads = z.B * z.HK, R = z.H / z.HK;
-  const HB = blocksOf(z.DH <= 128, z.T * R, heads, ceil(z.WINDOW ? Math.min(z.KEYS, z.WINDOW) : z.KEYS, 64)), rows = 64 * HB, tiles = ceil(z.T * R, rows), SPLITS = keySplits(z, rows, z.DH <= 64 ? 64 : 32, tiles * heads);
+  const HB = blocksOf(packs(z), z.T * R, heads, ceil(z.WINDOW ? Math.min(z.KEYS, z.WINDOW) : z.KEYS, 64)), rows = 64 * HB, tiles = ceil(z.T * R, rows), SPLITS = keySplits(z, rows, z.DH <= 64 ? 64 : 32, tiles * heads);
   const more = { TILES: ceil(z.T * R, 16), SPLITS, HB }, types = { HB: 'int' };
   let at = 0;
   const place = (name, bytes) => { more[name] = at; types[name] = 'size_t'; at = align(at + bytes, 256); };
@@ -242,7 +243,7 @@ function backwardKernels(s, parts, joined) {
   // The gradients of queries and of keys run side by side, and what joins their parts.
   const jobs = [], joins = [], waves = packed && z.DH > 64 ? 8 : 4;
   if (packed) more.WAVES = waves;
-  const keyBlocks = blocksOf(hold, z.KEYS, heads, ceil(Math.min(z.T, z.WINDOW || z.T) * R, 32)), rowBlocks = blocksOf(hold, z.T * R, heads, ceil(z.WINDOW ? Math.min(z.KEYS, z.WINDOW) : z.KEYS, 64));
+  const keyBlocks = blocksOf(hold && packed, z.KEYS, heads, ceil(Math.min(z.T, z.WINDOW || z.T) * R, 32)), rowBlocks = blocksOf(hold && packed, z.T * R, heads, ceil(z.WINDOW ? Math.min(z.KEYS, z.WINDOW) : z.KEYS, 64));
   const keyRows = 16 * waves * keyBlocks, rows = 16 * waves * rowBlocks;
   // (Of heads above 64 a workgroup a CU, by its registers.)
   const { CHUNK, SPLITS } = deal(z, heads, (hold ? 2 : 1) * CUS, keyRows, rows);

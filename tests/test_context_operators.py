@@ -155,6 +155,8 @@ COMPILED = [
     {"family": "window", "q": [2, 4096, 16, 128], "k": [2, 4096, 4, 128], "options": {"window": 1024, "sinks": 4}, "gradient": True},
     {"family": "window", "q": [1, 300, 4, 256], "k": [1, 300, 2, 256], "gradient": True},
     {"family": "window", "q": [2, 37, 3, 15], "k": [2, 37, 3, 15], "gradient": True},
+    {"family": "window", "q": [4, 2000, 8, 64], "k": [4, 2000, 8, 64], "options": {"window": 100}, "gradient": True},
+    {"family": "window", "q": [1, 8192, 8, 64], "k": [1, 8192, 2, 64], "gradient": True}, {"family": "window", "q": [8, 1024, 8, 96], "k": [8, 1024, 2, 96], "lengths": True, "gradient": True},
 ]
 
 
