@@ -19,7 +19,7 @@
 // six of bf16 for two), and 218 of the gradients' (30 for five, as scores and dy·v are formed for queries and for keys).
 //   two sequences of 16384 tokens, 16 heads of 128 by 4, a window of 1024    1090 us (253 TFLOP/s), 48 to split keys and values
 //   8192 tokens, 8 heads of 64 by 2: 310 us (221 TFLOP/s) and 9 to join two splits; its gradients 830 (207) and 28 to split, 21 to join
-// Of the cycles the matrix cores are busy in 53 %: the rest are the softmax, the split of P and dS into parts and the barriers, which two wavefronts a
+// Of the cycles the matrix cores are busy in 49 %: the rest are the softmax, the split of P and dS into parts and the barriers, which two wavefronts a
 // SIMD do not hide whole. Taking the next tile's scores beside this one's softmax needs their registers twice: 313 us of 320 at heads of 64, and spilled at 128.
 
 #pragma once

@@ -750,12 +750,6 @@ __device__ __forceinline__ void window_wide_add(float* __restrict__ dq, const fl
   if constexpr (S::VEC) *reinterpret_cast<f4*>(dq + at * E) = sum;
   else dq[at] = sum[0];
 }
-// The first of two calls, or the second.
-template <class S, class F, class G>
-__device__ __forceinline__ void window_either(uint32_t which, F first, G second) {
-  if (which == 0u) first();
-  else second();
-}
 // dk (scaled) or dv from their chunks' sums.
 template <class S>
 __device__ __forceinline__ void window_wide_join(float* __restrict__ out, const float* __restrict__ parts, const float* __restrict__ lengths, float by, size_t at) {

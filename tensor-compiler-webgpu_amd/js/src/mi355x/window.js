@@ -192,7 +192,7 @@ function forwardKernels(s, parts, joined) {
   // (32 tokens of 8 heads over 1028 keys: 16.8 us by nine tiles, 21.6 by five.)
   const most = ceil(z.WINDOW ? Math.min(z.KEYS, z.WINDOW + ceil(16, R) + 32 + z.SINKS) : z.KEYS, 16);
   const SPLITS = Math.max(1, Math.min(256, Math.floor(most / 8), ceil(4 * CUS, TILES * heads)));
-  const types = { SUMS: 'size_t' };
+  const types = {};
   let at = 0;
   const more = { TILES, SPLITS };
   const place = (name, bytes) => { more[name] = at; types[name] = 'size_t'; at = align(at + bytes, 256); };
