@@ -153,6 +153,10 @@ const CONTEXT = [
   window('packed-k', [1, 140, 4, 64], [1, 140, 1, 64], {}, { gradient: true, wrt: ['k'] }),
   window('packed-v', [1, 140, 4, 64], [1, 140, 1, 64], {}, { gradient: true, wrt: ['v'] }),
   window('packed-q', [1, 140, 4, 64], [1, 140, 1, 64], {}, { gradient: true, wrt: ['q'] }),
+  // Gradients of few rows and large heads.
+  window('token-large', [2, 1, 3, 200], [2, 40, 1, 200], { window: 9, sinks: 2 }, { lengths: true, gradient: true }),
+  window('few-large', [3, 7, 2, 130], [3, 7, 2, 130], {}, { gradient: true }),
+  window('few-long', [1, 2, 4, 128], [1, 1500, 2, 128], {}, { gradient: true }),
   window('only-q', [2, 64, 4, 32], [2, 64, 2, 32], { window: 20 }, { gradient: true, wrt: ['q'] }),
   window('only-k', [2, 64, 4, 32], [2, 64, 2, 32], { window: 20 }, { gradient: true, wrt: ['k'] }),
   window('only-v', [2, 64, 4, 32], [2, 64, 2, 32], { window: 20 }, { gradient: true, wrt: ['v'] }),
