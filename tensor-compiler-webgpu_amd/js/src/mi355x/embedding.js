@@ -73,7 +73,8 @@ function lowerEmbeddingGrad(graph, node) {
   const bits = Math.max(1, Math.ceil(Math.log2(V))), PASSES = ceil(bits, 9), BITS = ceil(bits, PASSES);
   const one = N <= ONE_TILE, SORT = one ? Math.min(1024, align(N, 64)) : 256;
   const TILE = one ? align(N, SORT) : Math.max(1024, align(ceil(N, 128), 256)), TILES = ceil(N, TILE);
-  // Keys of a sum: few enough that 4096 wavefronts walk them.
+  // Keys of a sum: few enough that 4096 wavefronts walk them. (32768 tokens of 1024 floats, in all: by 8 169 us, 16 161, 32, which this takes, 154, 64 160; 8192 of 256
+  // by 8, which this takes, 27.1, 16 28.4, 64 43.)
   const waves = N * columns * lanes / 64;
   let CH = 8;
   while (CH < 64 && waves / CH > 4096) CH *= 2;

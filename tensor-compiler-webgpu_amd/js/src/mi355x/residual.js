@@ -30,6 +30,7 @@ function residualKernels(node, sizes, parts, joined) {
   const rows = z.THREADS / z.LANES;
   // The gradients of vectors: sums of each workgroup's rows, added by a second launch.
   const sums = ['dgain', 'dbias', 'dpostGain', 'dpostBias'].concat(z.GATE === GATE.vector ? ['dgate'] : []).filter((p) => parts.includes(p));
+  // (8189 rows of 4095, forward and back: by 256 workgroups 300 us, 512 268, 1024 283; 8192 of 256 19.2, 17.9 and 17.9; 4096 of 1024 35.8, 36.8 and 39.2.)
   const blocks = Math.min(ceil(z.N, rows), sums.length ? 512 : 65536);
   const floats = blocks * sums.length * z.D;
   const at = (name) => (names.includes(name) ? `A.in[${names.indexOf(name)}]` : 'nullptr');
