@@ -5,7 +5,8 @@
 // Two forms of an operand:
 //   dots   for sums over a head (q·k, dy·v): pairs of halves, hi = half(x·2^e), lo = half(x·2^e - hi), e a row's own so that its
 //          largest |x|·2^e is in 2^14 ... 2^15: 22 bits of every entry from 2^-17 of the row's largest on, an absolute 2^-39 of it below. The product is
-//          hi·hi + hi·lo + lo·hi (2^-22 of it left out) times 2^-e of both rows.
+//          hi·hi + hi·lo + lo·hi (2^-22 of it left out) times 2^-e of both rows. Neither of the two steps leaves float32 where the
+//          result does not (WindowFactor).
 //   sums   for sums over keys or queries: three bf16 parts and the six products of tcmi_window_wide.h, since such a sum has no
 //          scale of its own: a key may be any size where another query sees it alone.
 // A row that holds a number that is not finite is zeros in both forms, and its 2^-e is NaN (a key's where its value
@@ -47,13 +48,45 @@ __device__ __forceinline__ void window_mfma(f4& acc, const Pair8& a, const Pair8
   acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.p[1], b.p[0], acc, 0, 0, 0);
   acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.p[0], b.p[0], acc, 0, 0, 0);
 }
-// 2^e for a row whose largest magnitude is `top`, and 2^-e. (e at most 126: both are normal numbers.)
+// 2^e for a row whose largest magnitude is `top`, and 2^-e. (e at most 126: both are normal numbers.) Packed is `word`, 2^-23 of the second: a dot
+// of 128 products below 2^30 times it stays in float32 whatever e is, and a dot of that size keeps 30 bits where the word is
+// below the normal numbers, all of which the multiplication takes.
 struct RowScale {
   float up, down;
   __device__ __forceinline__ RowScale(float top) {
     const int e = top > 0.f ? min(126, 14 - static_cast<int>((__float_as_uint(top) >> 23) - 127u)) : 0;
     up = __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
     down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+  }
+  __device__ __forceinline__ float word() const { return down * 0x1p-23f; }
+};
+// What a lane's rows multiply dots by that were multiplied by the other operand's words: 2^23 of their own 2^-e. Of the rows for which that
+// leaves float32 (their largest entry is 2^118 or more) 2^14 of it, and `far` has the dots multiplied by the other 2^9 before: 2^9 times
+// dots that leave float32 leave it once more by such a row's scale.
+template <int HB>
+struct WindowFactor {
+  float by[HB];
+  bool far[HB];
+  __device__ __forceinline__ void set(int h, float down) {
+    far[h] = !(down <= 0x1p104f);
+    by[h] = down * (far[h] ? 0x1p14f : 0x1p23f);
+  }
+  __device__ __forceinline__ float more(int h) const { return far[h] ? 0x1p9f : 1.f; }
+  // Whether a row of the wavefront's is.
+  __device__ __forceinline__ bool some() const {
+    bool any = false;
+#pragma unroll
+    for (int h = 0; h < HB; ++h) any = any || far[h];
+    return __ballot(any) != 0ull;
+  }
+  template <int BLOCKS>
+  __device__ __forceinline__ void reach(f4 (&s)[HB][BLOCKS]) const {
+    if (!some()) return;
+#pragma unroll
+    for (int h = 0; h < HB; ++h) {
+#pragma unroll
+      for (int k = 0; k < BLOCKS; ++k) s[h][k] *= more(h);
+    }
   }
 };
 // The largest magnitude; NaN where one of the eight is not finite (a sum of zeros and what is not).
@@ -125,8 +158,8 @@ __device__ __forceinline__ void window_pack_keys(const float* __restrict__ kp, c
   if (bad) k0 = k1 = v0 = v1 = f4{0.f, 0.f, 0.f, 0.f};
   const RowScale ks(bad ? 0.f : kt), vs(bad ? 0.f : vt);
   if (c == 0) {
-    reinterpret_cast<float*>(ws + S::KSCALE)[id] = bad ? __builtin_nanf("") : ks.down;
-    if constexpr (BACK) reinterpret_cast<float*>(ws + S::VSCALE)[id] = bad ? __builtin_nanf("") : vs.down;
+    reinterpret_cast<float*>(ws + S::KSCALE)[id] = bad ? __builtin_nanf("") : ks.word();
+    if constexpr (BACK) reinterpret_cast<float*>(ws + S::VSCALE)[id] = bad ? __builtin_nanf("") : vs.word();
   }
   if (c >= P::DP / 8) return;
   const Minus minus;
@@ -169,7 +202,7 @@ __device__ __forceinline__ void window_pack_rows(const WindowGradArgs a, char* w
   if (bad) q0 = q1 = d0 = d1 = zero;
   const RowScale qs(bad ? 0.f : qt), ds(bad ? 0.f : dt);
   if (c == 0) {
-    reinterpret_cast<float4*>(ws + S::ROWSTATS)[id] = make_float4(bad ? __builtin_nanf("") : qs.down, ds.down, on ? a.lse[line] * LOG2E : 0.f, mass);
+    reinterpret_cast<float4*>(ws + S::ROWSTATS)[id] = make_float4(bad ? __builtin_nanf("") : qs.word(), ds.word(), on ? a.lse[line] * LOG2E : 0.f, mass);
   }
   if (!DOTS || c >= P::DP / 8) return;
   const Minus minus;
@@ -348,10 +381,13 @@ __device__ __forceinline__ void window_packed(const float* __restrict__ qp, cons
   const float scale = static_cast<float>(S::scale() * 1.4426950408889634);
   Pair8 qf[HB][SLICES];
   f4 o[HB][G];
-  float m[HB], l[HB], qs[HB];
+  float m[HB], l[HB];
+  WindowFactor<HB> qs;
 #pragma unroll
   for (int h = 0; h < HB; ++h) {
-    window_pair_row<S>(qf[h], qp + rows.line[h] * S::DH, rows.on[h], scale, qs[h]);
+    float down;
+    window_pair_row<S>(qf[h], qp + rows.line[h] * S::DH, rows.on[h], scale, down);
+    qs.set(h, down);
     m[h] = -TCMI_INF;
     l[h] = 0.f;
 #pragma unroll
@@ -376,13 +412,19 @@ __device__ __forceinline__ void window_packed(const float* __restrict__ qp, cons
     barrier_ahead<0>();
     if (i + 1 < end) keys(i + 1);
     if (some) {
-      if (!rows.whole(w, j0, NB)) {
+      if (!rows.whole(w, j0, NB) || qs.some()) {
+        // (The rows' positions are found again here: kept, they spill other registers.)
+        int own = lane;
+        asm volatile("" : "+v"(own));
 #pragma unroll
         for (int h = 0; h < HB; ++h) {
+          const uint32_t row = mine + 16u * h + (own & 15);
+          const int32_t pos = w.first + static_cast<int32_t>(min(row, ROWS - 1u) / Span::R);
+          const bool on = row < ROWS && w.stands(pos);
 #pragma unroll
           for (int k = 0; k < BLOCKS; ++k) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) s[h][k][r] = rows.on[h] && w.sees(rows.pos[h], j0 + 16 * k + 4 * q + r) ? s[h][k][r] : -TCMI_INF;
+            for (int r = 0; r < 4; ++r) s[h][k][r] = on && w.sees(pos, j0 + 16 * k + 4 * (own >> 4) + r) ? s[h][k][r] * qs.more(h) : -TCMI_INF;
           }
         }
       }
@@ -397,7 +439,7 @@ __device__ __forceinline__ void window_packed(const float* __restrict__ qp, cons
           for (int r = 0; r < 4; ++r) top = fmaxf(top, s[h][k][r]);
         }
         // (A row's scale is positive, or NaN: its scores' order is theirs before it.)
-        top = fmaxf(m[h], quad16_reduce<true>(top) * qs[h]);
+        top = fmaxf(m[h], quad16_reduce<true>(top) * qs.by[h]);
         const float zero = top == -TCMI_INF ? 0.f : top;
         alpha[h] = __builtin_amdgcn_exp2f(m[h] - zero);
         m[h] = top;
@@ -406,7 +448,7 @@ __device__ __forceinline__ void window_packed(const float* __restrict__ qp, cons
         for (int k = 0; k < BLOCKS; ++k) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            s[h][k][r] = __builtin_amdgcn_exp2f(fmaf(s[h][k][r], qs[h], -zero));
+            s[h][k][r] = __builtin_amdgcn_exp2f(fmaf(s[h][k][r], qs.by[h], -zero));
             sum += s[h][k][r];
           }
         }
@@ -500,12 +542,17 @@ __device__ __forceinline__ void window_packed_dq(const WindowGradArgs a, float* 
   const WindowLines<S, HB> rows(w, b, hk, mine);
   Pair8 qf[HB][SLICES], df[HB][SLICES];
   f4 acc[HB][G];
-  float4 stats[HB];
+  WindowFactor<HB> qby, dby;
+  float lse[HB], mass[HB];
   const float scale = static_cast<float>(S::scale() * 1.4426950408889634);
 #pragma unroll
   for (int h = 0; h < HB; ++h) {
     const uint32_t at = min(mine + 16u * h + t, ROWS - 1u);
-    stats[h] = reinterpret_cast<const float4*>(ws + S::ROWSTATS)[head * P::RP + at];
+    const float4 stats = reinterpret_cast<const float4*>(ws + S::ROWSTATS)[head * P::RP + at];
+    qby.set(h, stats.x * 0x1p23f);
+    dby.set(h, stats.y * 0x1p23f);
+    lse[h] = stats.z;
+    mass[h] = stats.w;
     float down;
     window_pair_row<S>(qf[h], a.q + rows.line[h] * S::DH, rows.on[h], scale, down);
     window_pair_row<S>(df[h], a.dy + rows.line[h] * S::DH, rows.on[h], 1.f, down);
@@ -523,6 +570,8 @@ __device__ __forceinline__ void window_packed_dq(const WindowGradArgs a, float* 
       f4 s[HB][BLOCKS], dp[HB][BLOCKS];
       window_pair_dots<T>(s, kd, qf);
       window_pair_dots<T>(dp, vd, df);
+      qby.reach(s);
+      dby.reach(dp);
       const float* by = reinterpret_cast<const float*>(words) + (NB == 64 ? 0 : j0 & 63);
 #pragma unroll
       for (int k = 0; k < BLOCKS; ++k) {
@@ -531,8 +580,8 @@ __device__ __forceinline__ void window_packed_dq(const WindowGradArgs a, float* 
         for (int h = 0; h < HB; ++h) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const float p = __builtin_amdgcn_exp2f(fmaf(s[h][k][r] * ks[r], stats[h].x, -stats[h].z));
-            const float d = p * fmaf(dp[h][k][r] * vs[r], stats[h].y, -stats[h].w);
+            const float p = __builtin_amdgcn_exp2f(fmaf(s[h][k][r] * ks[r], qby.by[h], -lse[h]));
+            const float d = p * fmaf(dp[h][k][r] * vs[r], dby.by[h], -mass[h]);
             s[h][k][r] = whole || (rows.on[h] && w.sees(rows.pos[h], j0 + 16 * k + 4 * q + r)) ? d : 0.f;
           }
         }
@@ -595,7 +644,7 @@ __device__ __forceinline__ void window_packed_dkv(const WindowGradArgs a, float*
   };
   if (begin < end) dots(begin);
   int32_t key[HB];
-  float ks[HB], vs[HB];
+  WindowFactor<HB> kby, vby;
   Pair8 kf[HB][SLICES], vf[HB][SLICES];
   f4 dka[HB][G], dva[HB][G];
 #pragma unroll
@@ -605,8 +654,8 @@ __device__ __forceinline__ void window_packed_dkv(const WindowGradArgs a, float*
     const uint32_t at = min(key[h], static_cast<int32_t>(P::KP) - 1);
     window_packed_row<S>(kf[h], ws + S::KDOTS, P::KP, head, at);
     if constexpr (DK) window_packed_row<S>(vf[h], ws + S::VDOTS, P::KP, head, at);
-    ks[h] = reinterpret_cast<const float*>(ws + S::KSCALE)[head * P::KP + at];
-    vs[h] = reinterpret_cast<const float*>(ws + S::VSCALE)[head * P::KP + at];
+    kby.set(h, reinterpret_cast<const float*>(ws + S::KSCALE)[head * P::KP + at] * 0x1p23f);
+    vby.set(h, reinterpret_cast<const float*>(ws + S::VSCALE)[head * P::KP + at] * 0x1p23f);
 #pragma unroll
     for (int g = 0; g < G; ++g) dka[h][g] = dva[h][g] = f4{0.f, 0.f, 0.f, 0.f};
   }
@@ -620,7 +669,11 @@ __device__ __forceinline__ void window_packed_dkv(const WindowGradArgs a, float*
       const bool whole = r0 + NB <= ROWS && a0 >= max(own.p0, mine + 16 * HB - 1) && a1 <= own.p1 && mine + 16 * HB <= w.length && (w.from(a1) <= mine || mine + 16 * HB <= static_cast<int32_t>(S::SINKS));
       f4 s[HB][BLOCKS], dp[HB][BLOCKS];
       window_pair_dots<T>(s, qd, kf);
-      if constexpr (DK) window_pair_dots<T>(dp, dd, vf);
+      kby.reach(s);
+      if constexpr (DK) {
+        window_pair_dots<T>(dp, dd, vf);
+        vby.reach(dp);
+      }
 #pragma unroll
       for (int k = 0; k < BLOCKS; ++k) {
 #pragma unroll
@@ -631,8 +684,8 @@ __device__ __forceinline__ void window_packed_dkv(const WindowGradArgs a, float*
 #pragma unroll
           for (int h = 0; h < HB; ++h) {
             const bool sees = whole || (w.stands(pos) && key[h] < w.length && w.sees(pos, key[h]));
-            s[h][k][r] = sees ? __builtin_amdgcn_exp2f(fmaf(s[h][k][r] * ks[h], st[0], -st[2])) : 0.f;
-            if constexpr (DK) dp[h][k][r] = sees ? s[h][k][r] * fmaf(dp[h][k][r] * vs[h], st[1], -st[3]) : 0.f;
+            s[h][k][r] = sees ? __builtin_amdgcn_exp2f(fmaf(s[h][k][r] * st[0], kby.by[h], -st[2])) : 0.f;
+            if constexpr (DK) dp[h][k][r] = sees ? s[h][k][r] * fmaf(dp[h][k][r] * st[1], vby.by[h], -st[3]) : 0.f;
           }
         }
       }

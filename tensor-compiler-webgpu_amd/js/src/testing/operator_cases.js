@@ -292,6 +292,12 @@ const FORMS = [
     ['packed', [1, 300, 4, 64], [1, 300, 2, 64], { window: 260, sinks: 5 }], ['packed-odd', [1, 280, 4, 40], [1, 280, 2, 40], {}],
   ].map(([name, q, k, options]) => window(`window-${name}${gradient ? '' : '-forward'}`, q, k, options, { gradient }))), []),
   embedding('embedding-order', [900], 40, 36, { scale: 3, gradient: true }),
+  // Of each form, with a scale that leaves scores in powers of two exact where the operands are few bits.
+  ...[
+    ['few', [2, 5, 6, 24], [2, 30, 2, 24], { window: 11, sinks: 2 }], ['wide', [2, 80, 2, 64], [2, 80, 2, 64], { window: 37, sinks: 3 }], ['wide-large', [1, 70, 2, 160], [1, 70, 2, 160], {}],
+    ['packed', [1, 300, 4, 64], [1, 300, 2, 64], { window: 260, sinks: 5 }], ['packed-odd', [1, 280, 4, 40], [1, 280, 2, 40], {}], ['packed-large', [1, 300, 4, 128], [1, 300, 2, 128], {}],
+    ['packed-blocks', [32, 150, 16, 24], [32, 150, 4, 24], { window: 130, sinks: 3 }],
+  ].map(([name, q, k, options]) => window(`window-exact-${name}`, q, k, Object.assign({ scale: Math.LN2 / 4 }, options), { gradient: true })),
 ];
 
 const r = (B, T, H, dh, axes, gradient, twin) => rotary(null, [B, T, H, dh], axes === 1 ? [B, T] : [B, T, axes],
