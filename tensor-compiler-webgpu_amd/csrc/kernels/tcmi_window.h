@@ -141,6 +141,20 @@ __device__ __forceinline__ uint32_t window_clean(f4 (&v)[G], int32_t j0, const W
   }
   return bad;
 }
+// Bit t: row t of a tile read along its rows holds a number that is not finite.
+template <int G>
+__device__ __forceinline__ uint32_t window_infinite(const f4 (&v)[G]) {
+  bool all = true;
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) all = all && __builtin_isfinite(v[g][i]);
+  }
+  uint64_t bad = __ballot(!all);
+  bad |= bad >> 32;
+  bad |= bad >> 16;
+  return static_cast<uint32_t>(bad) & 0xffffu;
+}
 // acc[k of a][t of b] += the products of two tiles along their rows.
 template <int G>
 __device__ __forceinline__ f4 window_scores(const f4 (&a)[G], const f4 (&b)[G]) {
@@ -203,7 +217,7 @@ __device__ __forceinline__ void window_rows(const float* __restrict__ qp, const 
   const size_t step = (size_t)S::HK * S::DH;
   const float* kb = kp + ((size_t)b * S::KEYS * S::HK + hk) * S::DH;
   const float* vb = vp + ((size_t)b * S::KEYS * S::HK + hk) * S::DH;
-  float m = -TCMI_INF, l = 0.f;
+  float m = -TCMI_INF, l = 0.f, lowest = 0.f;
   // (Of a key past the last, the last again: its scores are not taken.) All loads of a tile are made before the tile before it is used.
   auto load = [&](int32_t i, f4 (&kf)[G], f4 (&vf)[G]) __attribute__((always_inline)) {
     const int32_t j0 = tiles.at(i) * 16;
@@ -226,6 +240,7 @@ __device__ __forceinline__ void window_rows(const float* __restrict__ qp, const 
     float top = -TCMI_INF;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
+      lowest = fminf(lowest, s[r]);
       s[r] = on && w.sees(p, j0 + 4 * q + r) ? (bad >> r & 1u ? __builtin_nanf("") : s[r] * scale) : -TCMI_INF;
       top = fmaxf(top, s[r]);
     }
@@ -243,6 +258,24 @@ __device__ __forceinline__ void window_rows(const float* __restrict__ qp, const 
     for (int g = 0; g < G; ++g) acc[g] *= alpha;
     window_sum(acc, vf, s);
     if (G > 8 && i + 4 < end) load(i + 4, kn, vn);
+  }
+  // A key or a query that is infinite gives scores of NaN or of infinities, and of -infinity, which has no weight, makes NaN like the
+  // others: where there was one, keys and queries are looked at again. (Read again, not kept,
+  // for the registers.)
+  if (__ballot(lowest == -TCMI_INF) != 0ull) {
+    const float* again = qp;
+    asm volatile("" : "+s"(again));
+    window_along<S>(kf, again + line * S::DH, on);
+    if (window_infinite(kf) >> t & 1u) l = __builtin_nanf("");
+    for (int32_t i = begin + wave; i < end; i += 4) {
+      const int32_t j0 = tiles.at(i) * 16;
+      window_along<S>(kf, kb + (size_t)min(j0 + t, tiles.hi) * step, true);
+      const uint32_t bad = window_infinite(kf) >> 4 * q;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        if (bad >> r & 1u && on && w.sees(p, j0 + 4 * q + r)) l = __builtin_nanf("");
+      }
+    }
   }
   // (Each lane has added its own keys.)
   l = quad16_reduce<false>(l);

@@ -20,8 +20,8 @@ function windowSizes(graph, node) {
 function maker(s, e, types) {
   const text = (kind, blocks, threads, structs, calls, lds, body) => {
     const header = calls.some((c) => /_pack/.test(c)) ? 'tcmi_window_packed.h' : calls.some((c) => /_wide/.test(c)) ? 'tcmi_window_wide.h' : 'tcmi_window.h';
-    // Two workgroups of four wavefronts a CU, or one of eight: 256 registers each.
-    const two = calls.some((c) => /_packed(_dq|_dkv)?</.test(c) || (/_wide(_dq|_dkv)?</.test(c) && s.z.DH <= 64));
+    // Two workgroups of four wavefronts a CU, or one of eight: 256 registers each. (Few rows, heads of 128 over 50000 keys: 106 us by one, 86 by two.)
+    const two = calls.some((c) => /_packed(_dq|_dkv)?</.test(c) || (/_wide(_dq|_dkv)?</.test(c) && s.z.DH <= 64) || (/window_rows</.test(c) && s.z.DH > 64 && s.z.DH <= 128));
     return kernel(kind, `#include "${header}"
 ${structs.map(([name, more]) => `struct ${name} {
 ${constants(Object.assign({}, s.z, more || {}), types)}

@@ -40,3 +40,65 @@ def test_far_operands_of_near_results(tool, tmp_path, form):
             want = np.ldexp(plain[n].astype(np.float64), power[n]).astype(np.float32)
             assert np.isfinite(want).all() and want.any()
             np.testing.assert_array_equal(r[n], want, err_msg=f"{name} {n}")
+
+
+def touched(c, v, keys, queries, cotangents):
+    """Where results are NaN, by name: keys (sequence, key, key head) and rows (sequence, token, head) of q, or of dy alone, that hold no number."""
+    from oracle import operators
+    node = next(n for n in c["graph"]["nodes"] if n["op"] == "windowAttention")
+    (B, T, H, _), (_, S, HK, _) = v["q"].shape, v["k"].shape
+    R = H // HK
+    sees = np.repeat(operators.window_sees(node, [None] * 3, [v["q"].shape, v["k"].shape, v["k"].shape])[:, None], H, 1)
+    key = np.zeros((B, H, S), bool)
+    for b, j, hk in keys:
+        key[b, hk * R:(hk + 1) * R, j] = True
+    row = (sees & key[:, :, None]).any(3)
+    for b, t, h in queries:
+        row[b, h, t] |= sees[b, h, t].any()
+    back = row.copy()
+    for b, t, h in cotangents:
+        back[b, h, t] |= sees[b, h, t].any()
+    at = (sees & back[..., None]).any(2).reshape(B, HK, R, S).any(2)
+    return {"o": row.transpose(0, 2, 1), "dq": back.transpose(0, 2, 1), "dk": at.transpose(0, 2, 1), "dv": at.transpose(0, 2, 1)}
+
+
+NUMBERS = ["few", "few-whole", "more", "wide", "wide-large", "packed", "packed-odd", "exact-packed-blocks"]
+
+
+def check_touched(tool, directory, form, v, bad, keys=(), queries=(), cotangents=()):
+    c, (plain, got) = run_form(tool, directory, f"window-{form}", [v, bad])
+    for n, at in touched(c, v, keys, queries, cotangents).items():
+        x, y = (r[n].reshape(at.shape + (v["q"].shape[3],)) for r in (got, plain))
+        assert np.isfinite(y).all() and at.any() == (n != "o" or bool(keys or queries)), n
+        assert np.isnan(x[at]).all(), (n, np.argwhere(~np.isnan(x).all(-1) & at)[:5])
+        np.testing.assert_array_equal(x[~at], y[~at], err_msg=n)
+
+
+def normal_inputs(tool, form, seed):
+    case = tool("operator-graphs", {"forms": [f"window-{form}"]})[0]["case"]
+    rng = np.random.default_rng(seed)
+    return {n: rng.standard_normal(s).astype(np.float32) for n, s in (("q", case["q"]), ("k", case["k"]), ("v", case["k"]), ("d0", case["q"]))}
+
+
+@pytest.mark.parametrize("sign", [-1, 1])
+@pytest.mark.parametrize("form", NUMBERS)
+def test_an_infinite_key(tool, tmp_path, form, sign):
+    """Its scores are all infinities of one sign: -infinity is no weight of 0."""
+    v = normal_inputs(tool, form, 6)
+    S = v["k"].shape[1]
+    v["q"][..., 1] = np.abs(v["q"][..., 1]) + np.float32(0.1)
+    bad = dict(v, k=v["k"].copy())
+    bad["k"][0, S - 3, 0, 1] = sign * np.inf
+    check_touched(tool, tmp_path, form, v, bad, keys=[(0, S - 3, 0)])
+
+
+@pytest.mark.parametrize("sign", [-1, 1])
+@pytest.mark.parametrize("form", NUMBERS)
+def test_an_infinite_query(tool, tmp_path, form, sign):
+    """Where every score of it is -infinity it is not a query that sees nothing."""
+    v = normal_inputs(tool, form, 7)
+    (_, T, H, _) = v["q"].shape
+    v["k"][..., 2] = np.abs(v["k"][..., 2]) + np.float32(0.1)
+    bad = dict(v, q=v["q"].copy())
+    bad["q"][0, T - 1, 0, 2] = bad["q"][0, 0, H - 1, 2] = sign * np.inf
+    check_touched(tool, tmp_path, form, v, bad, queries=[(0, T - 1, 0), (0, 0, H - 1)])
