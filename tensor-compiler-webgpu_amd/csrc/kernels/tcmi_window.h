@@ -32,6 +32,7 @@ constexpr float LOG2E = 1.4426950408889634f;
 template <class S>
 struct WindowSpan {
   static constexpr uint32_t R = S::H / S::HK, ROWS = S::T * R;
+  static constexpr bool FEW = ROWS <= 16u;      // whose forward pass is window_rows
   int32_t length, first;       // keys, and the position of query 0
 
   __device__ __forceinline__ WindowSpan(const float* lengths, uint32_t b) {

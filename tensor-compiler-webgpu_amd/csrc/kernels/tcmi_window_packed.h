@@ -151,8 +151,8 @@ __device__ __forceinline__ void window_pack_keys(const float* __restrict__ kp, c
   if (first > keys.hi || (first + 63 < keys.lo && first >= static_cast<int32_t>(S::SINKS))) return;
   const bool on = seen(key);
   const size_t row = (((size_t)b * S::KEYS + (on ? j : 0u)) * S::HK + hk) * S::DH;
-  f4 k0 = window_load<S>(kp + row, 8 * c, on), k1 = window_load<S>(kp + row, 8 * c + 4, on);
-  f4 v0 = window_load<S>(vp + row, 8 * c, on), v1 = window_load<S>(vp + row, 8 * c + 4, on);
+  const auto load = [&](const float* p, int d) { return window_number(window_load<S>(p + row, 8 * c + d, on)); };
+  f4 k0 = load(kp, 0), k1 = load(kp, 4), v0 = load(vp, 0), v1 = load(vp, 4);
   const float kt = P::row_top(window_top(k0, k1, 0.f)), vt = P::row_top(window_top(v0, v1, 0.f));
   const bool bad = kt != kt || vt != vt;
   if (bad) k0 = k1 = v0 = v1 = f4{0.f, 0.f, 0.f, 0.f};
@@ -186,8 +186,8 @@ __device__ __forceinline__ void window_pack_rows(const WindowGradArgs a, char* w
   const bool on = r < Span::ROWS && w.stands(w.first + static_cast<int32_t>(r / R));
   const uint32_t at = on ? r : 0u;
   const size_t line = ((size_t)b * S::T + at / R) * S::H + hk * R + at % R;
-  f4 q0 = window_load<S>(a.q + line * S::DH, 8 * c, on), q1 = window_load<S>(a.q + line * S::DH, 8 * c + 4, on);
-  f4 d0 = window_load<S>(a.dy + line * S::DH, 8 * c, on), d1 = window_load<S>(a.dy + line * S::DH, 8 * c + 4, on);
+  const auto load = [&](const float* p, int d) { return window_number(window_load<S>(p + line * S::DH, 8 * c + d, on)); };
+  f4 q0 = load(a.q, 0), q1 = load(a.q, 4), d0 = load(a.dy, 0), d1 = load(a.dy, 4);
   const f4 o0 = window_load<S>(a.o + line * S::DH, 8 * c, on), o1 = window_load<S>(a.o + line * S::DH, 8 * c + 4, on);
   float mass = 0.f;
 #pragma unroll
@@ -282,8 +282,8 @@ __device__ __forceinline__ void window_pair_row(Pair8 (&f)[SLICES], const float*
   float top = 0.f;
 #pragma unroll
   for (int s = 0; s < SLICES; ++s) {
-    x[s] = window_load<S, true>(p, 32 * s + 8 * q, on) * by;
-    y[s] = window_load<S, true>(p, 32 * s + 8 * q + 4, on) * by;
+    x[s] = window_number(window_load<S, true>(p, 32 * s + 8 * q, on)) * by;
+    y[s] = window_number(window_load<S, true>(p, 32 * s + 8 * q + 4, on)) * by;
     top = window_larger(top, window_top(x[s], y[s], 0.f));
   }
   top = window_larger(top, __shfl_xor(top, 16, 64));

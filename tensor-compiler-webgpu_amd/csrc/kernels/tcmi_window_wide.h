@@ -31,6 +31,22 @@ namespace tcmi {
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
+// What counts as a number here: what is below 2^128 - 2^119. The rest as NaN.
+__device__ __forceinline__ bool window_finite(float x) { return fabsf(x) < 0x1.ffp127f; }
+__device__ __forceinline__ f4 window_number(f4 v) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = window_finite(v[i]) ? v[i] : __builtin_nanf("");
+  return v;
+}
+// Of eight floats the first four, the first NaN where one of them is no number.
+__device__ __forceinline__ f4 window_row(f4 a, const f4& b) {
+  float most = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) most = fmaxf(fmaxf(most, fabsf(a[i])), fabsf(b[i]));
+  a[0] = window_finite(most) ? a[0] : __builtin_nanf("");
+  return a;
+}
+
 // Eight floats as three parts each.
 struct Parts {
   bf16x8 p[3];
@@ -101,7 +117,7 @@ struct WindowTile {
         bool all = true;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const bool finite = fabsf(u[e]) < 0x1.ffp127f;
+          const bool finite = window_finite(u[e]);
           all = all && finite;
           u[e] = finite ? u[e] : 0.f;
         }
@@ -201,7 +217,7 @@ __device__ __forceinline__ void window_wide(const float* __restrict__ qp, const 
 #pragma unroll
     for (int s = 0; s < SLICES; ++s) {
       const f4 x = window_load<S, true>(qp + line[i] * S::DH, 32 * s + 8 * q, on[i]), y = window_load<S, true>(qp + line[i] * S::DH, 32 * s + 8 * q + 4, on[i]);
-      window_parts(x * scale, y * scale, minus, qf[i][s]);
+      window_parts(window_row(x, y) * scale, y * scale, minus, qf[i][s]);
     }
   }
   // Positions of the wavefront's first and last row: tiles between them need no look at each pair.
@@ -414,28 +430,37 @@ struct WindowGradArgs {
   const float *q, *k, *v, *lengths, *o, *lse, *dy, *mass;
 };
 
-// dy·o of a row, whose floats 32·s + 8q ... lane (t, q) adds up; every lane of the row gets it.
+// dy·o of a row, whose floats 32·s + 8q ... lane (t, q) adds up; every lane of the row gets it. NaN where dy holds what is no number.
 template <class S>
 __device__ __forceinline__ float window_row_mass(const float* __restrict__ o, const float* __restrict__ dy, bool on) {
   const int q = (threadIdx.x >> 4) & 3;
-  float sum = 0.f;
+  float sum = 0.f, most = 0.f;
 #pragma unroll
   for (int s = 0; s < (static_cast<int>(S::DH) + 31) / 32; ++s) {
 #pragma unroll
     for (int h = 0; h < 8; h += 4) {
       const f4 x = window_load<S, true>(o, 32 * s + 8 * q + h, on), y = window_load<S, true>(dy, 32 * s + 8 * q + h, on);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sum = fmaf(x[i], y[i], sum);
+      for (int i = 0; i < 4; ++i) {
+        sum = fmaf(x[i], y[i], sum);
+        most = fmaxf(most, fabsf(y[i]));
+      }
     }
   }
-  return quad16_reduce<false>(sum);
+  return quad16_reduce<false>(window_finite(most) ? sum : __builtin_nanf(""));
 }
-// Of 16 lines a wavefront from `line` on, for heads above 128.
+// Of 16 lines a wavefront from `line` on, for heads above 128. (NaN also of a query that is no number here and was one to tcmi_window.h.)
 template <class S>
-__device__ __forceinline__ void window_wide_mass(const float* __restrict__ o, const float* __restrict__ dy, float* __restrict__ mass, size_t line) {
+__device__ __forceinline__ void window_wide_mass(const float* __restrict__ qp, const float* __restrict__ o, const float* __restrict__ dy, float* __restrict__ mass, size_t line) {
   constexpr size_t LINES = (size_t)S::B * S::T * S::H;
   const size_t at = line + (threadIdx.x & 15u), row = min(at, LINES - 1u) * S::DH;
-  const float sum = window_row_mass<S>(o + row, dy + row, true);
+  float sum = window_row_mass<S>(o + row, dy + row, true);
+  if constexpr (WindowSpan<S>::FEW) {
+    bool all = true;
+    for (uint32_t d = threadIdx.x >> 4 & 3u; d < S::DH; d += 4u) all = all && window_finite(qp[row + d]);
+    const uint64_t bad = __ballot(!all);
+    if ((bad | bad >> 16 | bad >> 32 | bad >> 48) >> (threadIdx.x & 15u) & 1u) sum = __builtin_nanf("");
+  }
   if ((threadIdx.x & 48u) == 0u && at < LINES) mass[at] = sum;
 }
 
@@ -506,6 +531,12 @@ __device__ __forceinline__ void window_wide_dq(const WindowGradArgs a, float* __
   for (int32_t i = begin; i < end; ++i) {
     const int32_t j0 = tiles.at(i) * NB;
     __syncthreads();
+    // (Of a key that is no number the scores here are of zeros, whose row's lse is NaN. Where tcmi_window.h took it for a number its value's line is.)
+#pragma unroll
+    for (int c = 0; c < T::CHUNKS && Span::FEW; ++c) {
+      const f4 x = kt.x[c];
+      if (!window_finite(fmaxf(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fabsf(x[2])), fabsf(x[3])))) vt.x[c][0] = __builtin_nanf("");
+    }
     kt.template store<true>(klds, minus);
     vt.template store<false>(vlds, minus);
     __syncthreads();
@@ -672,13 +703,17 @@ __device__ __forceinline__ void window_wide_dkv(const WindowGradArgs a, float* _
     __syncthreads();
     qt.template store<true>(qlds, minus);
     dt.template store<true>(dlds, minus);
-    // dy·o of 32 floats of a row by its eight threads; NaN where q or dy hold a number that is not finite, as 0 times it is.
+    // dy·o of 32 floats of a row by its eight threads; NaN where q or dy hold what is no number.
     if constexpr (OWN) {
 #pragma unroll
       for (int c = 0; c < T::CHUNKS; ++c) {
-        float sum = 0.f;
+        float sum = 0.f, most = 0.f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sum = fmaf(0.f, qt.x[c][e], fmaf(dt.x[c][e], DK ? ot.x[c][e] : 0.f, sum));
+        for (int e = 0; e < 4; ++e) {
+          sum = fmaf(0.f, qt.x[c][e], fmaf(dt.x[c][e], DK ? ot.x[c][e] : 0.f, sum));
+          most = fmaxf(fmaxf(most, Span::FEW ? fabsf(qt.x[c][e]) : 0.f), fabsf(dt.x[c][e]));
+        }
+        sum = window_finite(most) ? sum : __builtin_nanf("");
 #pragma unroll
         for (int off = 1; off < 8; off *= 2) sum += __shfl_xor(sum, off, 64);
         if (threadIdx.x % 8u == 0u) row_mass[T::dim(c) / 32 * NB + T::line(c)] = sum;

@@ -238,7 +238,7 @@ function backwardKernels(s, parts, joined) {
       `window_pack_both<${S}, ${dq}, ${dk || dv}, ${keys}u>(${args}, ${ws}, blockIdx.x, ${place256(0)}, ${place256(keys)})`, Object.assign({ VSUMS: 0 }, more)));
   }
   if (masses) {
-    kernels.push(m('winmass', grid(ceil(z.B * z.T * z.H, 64)), 256, null, `window_wide_mass<${S}>(A.in[${first}], A.in[${first + 2}], ${e.ws}, blockIdx.x * 64u + threadIdx.x / 64u * 16u)`));
+    kernels.push(m('winmass', grid(ceil(z.B * z.T * z.H, 64)), 256, null, `window_wide_mass<${S}>(A.in[0], A.in[${first}], A.in[${first + 2}], ${e.ws}, blockIdx.x * 64u + threadIdx.x / 64u * 16u)`));
   }
   // The gradients of queries and of keys run side by side, and what joins their parts.
   const jobs = [], joins = [], waves = packed && z.DH > 64 ? 8 : 4;

@@ -292,6 +292,7 @@ const FORMS = [
     ['packed', [1, 300, 4, 64], [1, 300, 2, 64], { window: 260, sinks: 5 }], ['packed-odd', [1, 280, 4, 40], [1, 280, 2, 40], {}],
   ].map(([name, q, k, options]) => window(`window-${name}${gradient ? '' : '-forward'}`, q, k, options, { gradient }))), []),
   embedding('embedding-order', [900], 40, 36, { scale: 3, gradient: true }),
+  window('window-few-large', [2, 4, 6, 160], [2, 21, 2, 160], { window: 11, sinks: 2 }, { gradient: true }),
   // Of each form, with a scale that leaves scores in powers of two exact where the operands are few bits.
   ...[
     ['few', [2, 5, 6, 24], [2, 30, 2, 24], { window: 11, sinks: 2 }], ['wide', [2, 80, 2, 64], [2, 80, 2, 64], { window: 37, sinks: 3 }], ['wide-large', [1, 70, 2, 160], [1, 70, 2, 160], {}],

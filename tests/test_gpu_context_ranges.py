@@ -62,7 +62,7 @@ def touched(c, v, keys, queries, cotangents):
     return {"o": row.transpose(0, 2, 1), "dq": back.transpose(0, 2, 1), "dk": at.transpose(0, 2, 1), "dv": at.transpose(0, 2, 1)}
 
 
-NUMBERS = ["few", "few-whole", "more", "wide", "wide-large", "packed", "packed-odd", "exact-packed-blocks"]
+NUMBERS = ["few", "few-whole", "few-large", "more", "wide", "wide-large", "packed", "packed-odd", "exact-packed-blocks"]
 
 
 def check_touched(tool, directory, form, v, bad, keys=(), queries=(), cotangents=()):
@@ -102,3 +102,44 @@ def test_an_infinite_query(tool, tmp_path, form, sign):
     bad = dict(v, q=v["q"].copy())
     bad["q"][0, T - 1, 0, 2] = bad["q"][0, 0, H - 1, 2] = sign * np.inf
     check_touched(tool, tmp_path, form, v, bad, queries=[(0, T - 1, 0), (0, 0, H - 1)])
+
+
+@pytest.mark.parametrize("operand", ["q", "k", "v", "d0"])
+@pytest.mark.parametrize("form", NUMBERS)
+def test_the_largest_numbers(tool, tmp_path, form, operand):
+    """From 2^128 - 2^119 on, which the split into bf16 rounds to infinity: as infinite as infinity, and nothing to what does not see them. The operands
+    of up to 16 rows of a key head are not split in the forward pass: there they are numbers, and in the gradients NaN wherever they are split."""
+    v = normal_inputs(tool, form, 8)
+    (_, T, H, dh), (_, S, _, _) = v["q"].shape, v["k"].shape
+    bad = dict(v, **{operand: v[operand].copy()})
+    at = {"q": (0, T - 1, 0), "k": (0, S - 3, 0), "v": (0, S - 2, 1), "d0": (0, T // 2, H - 1)}[operand]
+    bad[operand][at + (dh // 2,)] = {"q": -1, "d0": -1}.get(operand, 1) * np.finfo(np.float32).max
+    planted = {"queries": [at]} if operand == "q" else {"cotangents": [at]} if operand == "d0" else {"keys": [at]}
+    if not form.startswith("few") or operand == "d0":
+        return check_touched(tool, tmp_path, form, v, bad, **planted)
+    c, (plain, got) = run_form(tool, tmp_path, f"window-{form}", [v, bad])
+    for n, where in touched(c, v, **dict({"keys": (), "queries": (), "cotangents": ()}, **planted)).items():
+        x, y = (r[n].reshape(where.shape + (dh,)) for r in (got, plain))
+        np.testing.assert_array_equal(x[~where], y[~where], err_msg=n)
+        if n == "dq" and operand != "q" or n != "dq" and n != "o" and operand == "q":
+            assert np.isnan(x[where]).all(), n
+
+
+@pytest.mark.parametrize("operand", ["q", "k", "v", "d0"])
+@pytest.mark.parametrize("form", NUMBERS)
+def test_numbers_below_the_largest(tool, tmp_path, form, operand):
+    """2^128 - 2^120 is a number: in a padded batch's last sequences nothing of the first changes, and o is what a value of that size makes of it."""
+    v = normal_inputs(tool, form, 9)
+    (_, T, H, dh), (_, S, HK, _) = v["q"].shape, v["k"].shape
+    bad = dict(v, **{operand: v[operand].copy()})
+    at = {"q": (0, T - 1, 0), "k": (0, S - 1, 0), "v": (0, S - 1, 0), "d0": (0, T - 1, 0)}[operand]
+    bad[operand][at + (dh // 2,)] = np.float32(2.0 ** 128 - 2.0 ** 120)
+    c, (plain, got) = run_form(tool, tmp_path, f"window-{form}", [v, bad])
+    where = touched(c, v, **{k: [at] if k == {"q": "queries", "d0": "cotangents"}.get(operand, "keys") else () for k in ("keys", "queries", "cotangents")})
+    for n, w in where.items():
+        x, y = (r[n].reshape(w.shape + (dh,)) for r in (got, plain))
+        np.testing.assert_array_equal(x[~w], y[~w], err_msg=n)
+        if operand == "v" and n == "o":
+            # The other values' sum is below half a step of the product.
+            seen = x[w][:, dh // 2]
+            assert np.isfinite(x).all() and (seen > 2.0 ** 90).all()
