@@ -430,11 +430,21 @@ struct WindowGradArgs {
   const float *q, *k, *v, *lengths, *o, *lse, *dy, *mass;
 };
 
+// The bits of the largest magnitude so far (of NaN above all others), and whether all are numbers.
+__device__ __forceinline__ uint32_t window_most(uint32_t most, float x) { return max(most, __float_as_uint(x) & 0x7fffffffu); }
+__device__ __forceinline__ bool window_numbers(uint32_t most) { return most < __float_as_uint(0x1.ffp127f); }
+// A lane's share of dy·o, to be added to others': 2^-8 of it, so that up to 128 of them stay in float32, infinity where it has left that itself, and NaN
+// only where an operand is no number: P, which dv is made of, does not hang on dy·o.
+__device__ __forceinline__ float window_share(float sum, uint32_t most) {
+  sum = fabsf(sum) < TCMI_INF ? sum * 0x1p-8f : TCMI_INF;
+  return window_numbers(most) ? sum : __builtin_nanf("");
+}
 // dy·o of a row, whose floats 32·s + 8q ... lane (t, q) adds up; every lane of the row gets it. NaN where dy holds what is no number.
 template <class S>
 __device__ __forceinline__ float window_row_mass(const float* __restrict__ o, const float* __restrict__ dy, bool on) {
   const int q = (threadIdx.x >> 4) & 3;
-  float sum = 0.f, most = 0.f;
+  float sum = 0.f;
+  uint32_t most = 0u;
 #pragma unroll
   for (int s = 0; s < (static_cast<int>(S::DH) + 31) / 32; ++s) {
 #pragma unroll
@@ -443,11 +453,11 @@ __device__ __forceinline__ float window_row_mass(const float* __restrict__ o, co
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         sum = fmaf(x[i], y[i], sum);
-        most = fmaxf(most, fabsf(y[i]));
+        most = window_most(most, y[i]);
       }
     }
   }
-  return quad16_reduce<false>(window_finite(most) ? sum : __builtin_nanf(""));
+  return quad16_reduce<false>(window_share(sum, most)) * 0x1p8f;
 }
 // Of 16 lines a wavefront from `line` on, for heads above 128. (NaN also of a query that is no number here and was one to tcmi_window.h.)
 template <class S>
@@ -703,17 +713,19 @@ __device__ __forceinline__ void window_wide_dkv(const WindowGradArgs a, float* _
     __syncthreads();
     qt.template store<true>(qlds, minus);
     dt.template store<true>(dlds, minus);
-    // dy·o of 32 floats of a row by its eight threads; NaN where q or dy hold what is no number.
+    // dy·o of 32 floats of a row by its eight threads; NaN where dy holds what is no number, or q does that tcmi_window.h took for one (of the
+    // others' lse is NaN).
     if constexpr (OWN) {
 #pragma unroll
       for (int c = 0; c < T::CHUNKS; ++c) {
-        float sum = 0.f, most = 0.f;
+        float sum = 0.f;
+        uint32_t most = 0u;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          sum = fmaf(0.f, qt.x[c][e], fmaf(dt.x[c][e], DK ? ot.x[c][e] : 0.f, sum));
-          most = fmaxf(fmaxf(most, Span::FEW ? fabsf(qt.x[c][e]) : 0.f), fabsf(dt.x[c][e]));
+          sum = fmaf(dt.x[c][e], DK ? ot.x[c][e] : 0.f, sum);
+          most = window_most(Span::FEW ? window_most(most, qt.x[c][e]) : most, dt.x[c][e]);
         }
-        sum = window_finite(most) ? sum : __builtin_nanf("");
+        sum = window_share(sum, most);
 #pragma unroll
         for (int off = 1; off < 8; off *= 2) sum += __shfl_xor(sum, off, 64);
         if (threadIdx.x % 8u == 0u) row_mass[T::dim(c) / 32 * NB + T::line(c)] = sum;
@@ -736,7 +748,10 @@ __device__ __forceinline__ void window_wide_dkv(const WindowGradArgs a, float* _
 #pragma unroll
     for (int k = 0; k < BLOCKS; ++k) {
       // (NaN where the row's numbers are not finite.)
-      const f4 ls = *reinterpret_cast<const f4*>(row_lse + 16 * k + 4 * q) + mass(k) * 0.f;
+      f4 ls = *reinterpret_cast<const f4*>(row_lse + 16 * k + 4 * q);
+      const f4 marks = mass(k);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) ls[r] = marks[r] == marks[r] ? ls[r] : marks[r];
       const int4 ps = *reinterpret_cast<const int4*>(row_pos + 16 * k + 4 * q);
       const int32_t pos[4] = {ps.x, ps.y, ps.z, ps.w};
 #pragma unroll
@@ -759,7 +774,7 @@ __device__ __forceinline__ void window_wide_dkv(const WindowGradArgs a, float* _
 #pragma unroll
         for (int h = 0; h < HB; ++h) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r) s[h][k][r] = whole || s[h][k][r] != 0.f ? s[h][k][r] * (dp[h][k][r] - ms[r]) : 0.f;
+          for (int r = 0; r < 4; ++r) s[h][k][r] = whole || s[h][k][r] != 0.f ? s[h][k][r] * fmaf(ms[r], OWN ? -0x1p8f : -1.f, dp[h][k][r]) : 0.f;
         }
       }
 #pragma unroll

@@ -17,6 +17,8 @@ FAR = {
     "queries-back": ((120, -120, 40, 40), ("o", "dq", "dv")),
     "values": ((0, 0, 118, -60), ("o", "dq", "dk", "dv")),
     "cotangents": ((0, 0, -60, 120), ("o", "dq", "dk", "dv")),
+    # (dy.o leaves float32, which dv does not hang on.)
+    "both": ((0, 0, 100, 100), ("o", "dv")),
 }
 
 
