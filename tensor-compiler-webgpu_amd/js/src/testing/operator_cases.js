@@ -293,6 +293,12 @@ const FORMS = [
   ].map(([name, q, k, options]) => window(`window-${name}${gradient ? '' : '-forward'}`, q, k, options, { gradient }))), []),
   embedding('embedding-order', [900], 40, 36, { scale: 3, gradient: true }),
   window('window-few-large', [2, 4, 6, 160], [2, 21, 2, 160], { window: 11, sinks: 2 }, { gradient: true }),
+  // Two blocks of rows, and in the gradients of keys, a wavefront (window.js blocksOf): sizes that end inside their tiles, heads of whole tiles and not.
+  window('window-blocks', [32, 151, 16, 20], [32, 151, 4, 20], { window: 130, sinks: 3 }, { lengths: true, gradient: true }),
+  window('window-blocks-odd', [32, 69, 32, 37], [32, 139, 4, 37], {}, { lengths: true, gradient: true }),
+  window('window-blocks-first', [32, 150, 16, 64], [32, 150, 4, 64], { queries: 'first', window: 125, sinks: 70 }, { lengths: true, gradient: true }),
+  window('window-blocks-large', [32, 141, 16, 112], [32, 141, 4, 112], { window: 130, sinks: 5 }, { lengths: true, gradient: true }),
+  window('window-blocks-largest', [16, 139, 32, 128], [16, 201, 4, 128], {}, { lengths: true }),
   // Of each form, with a scale that leaves scores in powers of two exact where the operands are few bits.
   ...[
     ['few', [2, 5, 6, 24], [2, 30, 2, 24], { window: 11, sinks: 2 }], ['wide', [2, 80, 2, 64], [2, 80, 2, 64], { window: 37, sinks: 3 }], ['wide-large', [1, 70, 2, 160], [1, 70, 2, 160], {}],
