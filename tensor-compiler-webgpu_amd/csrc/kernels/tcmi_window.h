@@ -192,17 +192,17 @@ __device__ __forceinline__ void window_gather(f4 (&acc)[G], float f, float* lds)
   for (int g = 0; g < G; ++g) acc[g] = at[g * 64 + lane] + at[(G + g) * 64 + lane] + at[(2 * G + g) * 64 + lane] + at[(3 * G + g) * 64 + lane];
 }
 
-// Workgroup: a tile of rows, a split, a sequence's key head.
+// Workgroup: a sequence's key head, a split of the keys that its rows see.
 template <class S>
 __device__ __forceinline__ void window_rows(const float* __restrict__ qp, const float* __restrict__ kp, const float* __restrict__ vp, const float* __restrict__ lengths,
                                             float* __restrict__ out, float* __restrict__ lse, char* ws, float* lds, uint32_t wg) {
   constexpr int G = (S::DH + 15) / 16;
   using Span = WindowSpan<S>;
   constexpr uint32_t R = Span::R, ROWS = Span::ROWS;
-  const uint32_t split = wg % S::SPLITS, tile = wg / S::SPLITS % S::TILES, head = wg / (S::SPLITS * S::TILES), b = head / S::HK, hk = head % S::HK;
+  const uint32_t split = wg % S::SPLITS, head = wg / S::SPLITS, b = head / S::HK, hk = head % S::HK;
   const int lane = threadIdx.x & 63, t = lane & 15, q = lane >> 4, wave = threadIdx.x >> 6;
   const Span w(lengths, b);
-  const uint32_t row0 = tile * 16u, row = row0 + t, at = min(row, ROWS - 1u);
+  const uint32_t row = t, at = min(row, ROWS - 1u);
   const size_t line = ((size_t)b * S::T + at / R) * S::H + hk * R + at % R;
   const int32_t p = w.first + static_cast<int32_t>(at / R);
   const bool on = row < ROWS && w.stands(p);
@@ -212,7 +212,7 @@ __device__ __forceinline__ void window_rows(const float* __restrict__ qp, const 
   const float scale = static_cast<float>(S::scale() * 1.4426950408889634);
 #pragma unroll
   for (int g = 0; g < G; ++g) acc[g] = f4{0.f, 0.f, 0.f, 0.f};
-  const WindowTiles tiles = window_keys(w, row0, min(row0 + 15u, ROWS - 1u));
+  const WindowTiles tiles = window_keys(w, 0u, ROWS - 1u);
   const int32_t each = (tiles.all + static_cast<int32_t>(S::SPLITS) - 1) / static_cast<int32_t>(S::SPLITS);
   const int32_t begin = min(tiles.all, static_cast<int32_t>(split) * each), end = min(tiles.all, begin + each);
   const size_t step = (size_t)S::HK * S::DH;
@@ -302,7 +302,7 @@ __device__ __forceinline__ void window_rows(const float* __restrict__ qp, const 
     }
     if (lse != nullptr && q == 0) lse[line] = total > 0.f || total != total ? (base + __builtin_amdgcn_logf(total)) * 0.69314718055994531f : -TCMI_INF;
   } else {
-    const size_t place = ((size_t)split * S::B * S::HK + head) * S::TILES * 16u + row;
+    const size_t place = ((size_t)split * S::B * S::HK + head) * 16u + row;
 #pragma unroll
     for (int g = 0; g < G; ++g) window_store<S>(reinterpret_cast<float*>(ws + S::OUT) + place * S::DH, 16 * g + 4 * q, acc[g]);
     if (q == 0) reinterpret_cast<float2*>(ws + S::STATS)[place] = make_float2(top, total);

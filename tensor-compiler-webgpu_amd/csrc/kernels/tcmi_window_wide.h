@@ -4,7 +4,7 @@
 // nothing to the others; parts below bf16's least normal number, of values below 2^-102, are lost, and values from 2^128 - 2^119 on, which
 // bf16 rounds to infinity, count as infinite.
 //
-// A workgroup's four wavefronts take 16 rows each (tcmi_window.h's rows: the queries of the heads that share a key head; HB = 1 here) and walk
+// A workgroup's four wavefronts take 16 rows each (tcmi_window.h's rows: the queries of the heads that share a key head) and walk
 // the tiles of NB keys that one of the 64 sees. A tile is loaded one ahead into registers, split by the thread that loaded it and
 // kept in LDS as three planes. With lane = 16·q + t of a 16 x 16 x 32 product, whose operands are lines of 32 along the
 // sum (8q ... of line t) and whose result is (lines 4q ... of the first, line t of the second):
@@ -173,8 +173,7 @@ struct WindowWide {
   static constexpr int DP = (S::DH + 31) / 32 * 32, SLICES = DP / 32, G = DP / 16;
   static constexpr int NB = DP <= 64 ? 64 : 32;        // keys of a tile: as many floats whatever the head
   static constexpr int BLOCKS = NB / 16;
-  static constexpr int HB = S::HB;                     // blocks of 16 rows of a wavefront
-  static constexpr uint32_t ROWS = 64 * HB;            // of a workgroup
+  static constexpr uint32_t ROWS = 64;                 // of a workgroup
   using T = WindowTile<S, NB>;
   static constexpr int LDS = 2 * T::BYTES + (NB + 4) * 4;
 };
@@ -187,6 +186,21 @@ __device__ __forceinline__ void window_run(int32_t n, uint32_t split, int32_t& b
   end = min(n, begin + each);
 }
 
+// Dot products of this lane's row with a tile's lines: acc[k] = lines 16k ... of `tile` by f.
+template <class T, int BLOCKS, int SLICES>
+__device__ __forceinline__ void window_dots(f4 (&acc)[BLOCKS], const char* tile, const Parts (&f)[SLICES]) {
+#pragma unroll
+  for (int k = 0; k < BLOCKS; ++k) {
+    acc[k] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int d = 0; d < SLICES; ++d) {
+      Parts x;
+      T::lines(tile, 16 * k, d, x);
+      window_mfma(acc[k], x, f[d]);
+    }
+  }
+}
+
 // Workgroup: W::ROWS rows of a sequence's key head, a split of the keys they see.
 template <class S>
 __device__ __forceinline__ void window_wide(const float* __restrict__ qp, const float* __restrict__ kp, const float* __restrict__ vp, const float* __restrict__ lengths,
@@ -194,7 +208,7 @@ __device__ __forceinline__ void window_wide(const float* __restrict__ qp, const 
   using W = WindowWide<S>;
   using Span = WindowSpan<S>;
   constexpr uint32_t R = Span::R, ROWS = Span::ROWS;
-  constexpr int NB = W::NB, HB = W::HB, BLOCKS = W::BLOCKS, SLICES = W::SLICES, G = W::G;
+  constexpr int NB = W::NB, BLOCKS = W::BLOCKS, SLICES = W::SLICES, G = W::G;
   const uint32_t b = head / S::HK, hk = head % S::HK;
   const int lane = threadIdx.x & 63, t = lane & 15, q = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Span w(lengths, b);
@@ -202,36 +216,24 @@ __device__ __forceinline__ void window_wide(const float* __restrict__ qp, const 
   const uint32_t row0 = tile * W::ROWS;
   const WindowTiles keys = window_keys(w, min(row0, ROWS - 1u), min(row0 + W::ROWS - 1u, ROWS - 1u)), tiles = window_wider<NB>(keys);
   // The wavefront's rows, scores in powers of two.
-  const uint32_t mine = row0 + 16u * HB * wave;
+  const uint32_t mine = row0 + 16u * wave, row = mine + t, at = min(row, ROWS - 1u);
   const float scale = static_cast<float>(S::scale() * 1.4426950408889634);
-  size_t line[HB];
-  int32_t pos[HB];
-  bool on[HB];
-  Parts qf[HB][SLICES];
+  const size_t line = ((size_t)b * S::T + at / R) * S::H + hk * R + at % R;
+  const int32_t pos = w.first + static_cast<int32_t>(at / R);
+  const bool on = row < ROWS && w.stands(pos);
+  Parts qf[SLICES];
 #pragma unroll
-  for (int i = 0; i < HB; ++i) {
-    const uint32_t row = mine + 16u * i + t, at = min(row, ROWS - 1u);
-    line[i] = ((size_t)b * S::T + at / R) * S::H + hk * R + at % R;
-    pos[i] = w.first + static_cast<int32_t>(at / R);
-    on[i] = row < ROWS && w.stands(pos[i]);
-#pragma unroll
-    for (int s = 0; s < SLICES; ++s) {
-      const f4 x = window_load<S, true>(qp + line[i] * S::DH, 32 * s + 8 * q, on[i]), y = window_load<S, true>(qp + line[i] * S::DH, 32 * s + 8 * q + 4, on[i]);
-      window_parts(window_row(x, y) * scale, y * scale, minus, qf[i][s]);
-    }
+  for (int s = 0; s < SLICES; ++s) {
+    const f4 x = window_load<S, true>(qp + line * S::DH, 32 * s + 8 * q, on), y = window_load<S, true>(qp + line * S::DH, 32 * s + 8 * q + 4, on);
+    window_parts(window_row(x, y) * scale, y * scale, minus, qf[s]);
   }
   // Positions of the wavefront's first and last row: tiles between them need no look at each pair.
-  const bool full = mine + 16u * HB <= ROWS && w.stands(w.first + static_cast<int32_t>(mine / R)) && w.stands(w.first + static_cast<int32_t>((mine + 16u * HB - 1u) / R));
-  const int32_t p0 = w.first + static_cast<int32_t>(min(mine, ROWS - 1u) / R), p1 = w.first + static_cast<int32_t>(min(mine + 16u * HB - 1u, ROWS - 1u) / R);
-  f4 o[HB][G];
-  float m[HB], l[HB];
+  const bool full = mine + 16u <= ROWS && w.stands(w.first + static_cast<int32_t>(mine / R)) && w.stands(w.first + static_cast<int32_t>((mine + 15u) / R));
+  const int32_t p0 = w.first + static_cast<int32_t>(min(mine, ROWS - 1u) / R), p1 = w.first + static_cast<int32_t>(min(mine + 15u, ROWS - 1u) / R);
+  f4 o[G];
+  float m = -TCMI_INF, l = 0.f;
 #pragma unroll
-  for (int i = 0; i < HB; ++i) {
-    m[i] = -TCMI_INF;
-    l[i] = 0.f;
-#pragma unroll
-    for (int g = 0; g < G; ++g) o[i][g] = f4{0.f, 0.f, 0.f, 0.f};
-  }
+  for (int g = 0; g < G; ++g) o[g] = f4{0.f, 0.f, 0.f, 0.f};
   const size_t step = (size_t)S::HK * S::DH, base = ((size_t)b * S::KEYS * S::HK + hk) * S::DH;
   using T = typename W::T;
   T x;                                   // K's next tile, or V's: never both at once
@@ -247,55 +249,38 @@ __device__ __forceinline__ void window_wide(const float* __restrict__ qp, const 
   };
   int32_t begin, end;
   window_run<S>(tiles.all, split, begin, end);
-  auto scores = [&](int32_t j0, bool whole, float (&alpha)[HB], Parts (&pf)[HB][BLOCKS / 2]) __attribute__((always_inline)) {
-    f4 s[HB][BLOCKS];
+  auto scores = [&](int32_t j0, bool whole, float& alpha, Parts (&pf)[BLOCKS / 2]) __attribute__((always_inline)) {
+    f4 s[BLOCKS];
+    window_dots<T>(s, klds, qf);
+    if (!whole) {
+#pragma unroll
+      for (int k = 0; k < BLOCKS; ++k) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[k][r] = on && w.sees(pos, j0 + 16 * k + 4 * q + r) ? s[k][r] : -TCMI_INF;
+      }
+    }
+    float top = -TCMI_INF;
 #pragma unroll
     for (int k = 0; k < BLOCKS; ++k) {
 #pragma unroll
-      for (int h = 0; h < HB; ++h) s[h][k] = f4{0.f, 0.f, 0.f, 0.f};
+      for (int r = 0; r < 4; ++r) top = fmaxf(top, s[k][r]);
+    }
+    top = fmaxf(m, quad16_reduce<true>(top));
+    const float zero = top == -TCMI_INF ? 0.f : top;
+    alpha = __builtin_amdgcn_exp2f(m - zero);
+    m = top;
+    float sum = 0.f;
 #pragma unroll
-      for (int d = 0; d < SLICES; ++d) {
-        Parts f;
-        T::lines(klds, 16 * k, d, f);
+    for (int k = 0; k < BLOCKS; ++k) {
 #pragma unroll
-        for (int h = 0; h < HB; ++h) window_mfma(s[h][k], f, qf[h][d]);
+      for (int r = 0; r < 4; ++r) {
+        s[k][r] = __builtin_amdgcn_exp2f(s[k][r] - zero);
+        sum += s[k][r];
       }
     }
-    if (!whole) {
+    l = fmaf(l, alpha, sum);
 #pragma unroll
-      for (int h = 0; h < HB; ++h) {
-#pragma unroll
-        for (int k = 0; k < BLOCKS; ++k) {
-#pragma unroll
-          for (int r = 0; r < 4; ++r) s[h][k][r] = on[h] && w.sees(pos[h], j0 + 16 * k + 4 * q + r) ? s[h][k][r] : -TCMI_INF;
-        }
-      }
-    }
-#pragma unroll
-    for (int h = 0; h < HB; ++h) {
-      float top = -TCMI_INF;
-#pragma unroll
-      for (int k = 0; k < BLOCKS; ++k) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) top = fmaxf(top, s[h][k][r]);
-      }
-      top = fmaxf(m[h], quad16_reduce<true>(top));
-      const float zero = top == -TCMI_INF ? 0.f : top;
-      alpha[h] = __builtin_amdgcn_exp2f(m[h] - zero);
-      m[h] = top;
-      float sum = 0.f;
-#pragma unroll
-      for (int k = 0; k < BLOCKS; ++k) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          s[h][k][r] = __builtin_amdgcn_exp2f(s[h][k][r] - zero);
-          sum += s[h][k][r];
-        }
-      }
-      l[h] = fmaf(l[h], alpha[h], sum);
-#pragma unroll
-      for (int k = 0; k < BLOCKS; k += 2) window_parts(s[h][k], s[h][k + 1], minus, pf[h][k / 2]);
-    }
+    for (int k = 0; k < BLOCKS; k += 2) window_parts(s[k], s[k + 1], minus, pf[k / 2]);
   };
   if (begin < end) load(kp, begin);
   for (int32_t i = begin; i < end; ++i) {
@@ -308,85 +293,56 @@ __device__ __forceinline__ void window_wide(const float* __restrict__ qp, const 
     // (What none of the wavefront's rows sees: past its last position, or between its sinks and its windows.)
     const bool some = j0 <= p1 && (j0 + NB > w.from(p0) || j0 < static_cast<int32_t>(S::SINKS));
     const bool whole = full && j0 + NB - 1 <= p0 && (j0 >= w.from(p1) || j0 + NB <= static_cast<int32_t>(S::SINKS));
-    float alpha[HB];
-    Parts pf[HB][BLOCKS / 2];
+    float alpha;
+    Parts pf[BLOCKS / 2];
     if (some) scores(j0, whole, alpha, pf);
     x.template store<true>(vlds, minus, bad, some_bad);
     __syncthreads();
     if (i + 1 < end) load(kp, i + 1);
     if (!some) continue;
     if (*some_bad) {
-#pragma unroll
-      for (int h = 0; h < HB; ++h) {
-        for (int k = 0; k < BLOCKS * 4; ++k) {
-          const int at = k / 4 * 16 + 4 * q + k % 4;
-          if (bad[at] && on[h] && w.sees(pos[h], j0 + at)) l[h] = __builtin_nanf("");
-        }
+      for (int k = 0; k < BLOCKS * 4; ++k) {
+        const int at = k / 4 * 16 + 4 * q + k % 4;
+        if (bad[at] && on && w.sees(pos, j0 + at)) l = __builtin_nanf("");
       }
     }
 #pragma unroll
     for (int g = 0; g < G; g += 2) {
-      f4 sum[HB][2];
-#pragma unroll
-      for (int h = 0; h < HB; ++h) sum[h][0] = sum[h][1] = f4{0.f, 0.f, 0.f, 0.f};
+      f4 sum[2] = {f4{0.f, 0.f, 0.f, 0.f}, f4{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
       for (int k = 0; k < BLOCKS / 2; ++k) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           Parts f;
           T::across(vlds, 32 * k, 16 * (g + e), f);
-#pragma unroll
-          for (int h = 0; h < HB; ++h) window_mfma(sum[h][e], f, pf[h][k]);
+          window_mfma(sum[e], f, pf[k]);
         }
       }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
 #pragma unroll
-        for (int h = 0; h < HB; ++h) {
-#pragma unroll
-          for (int r = 0; r < 4; ++r) o[h][g + e][r] = fmaf(o[h][g + e][r], alpha[h], sum[h][e][r]);
-        }
+        for (int r = 0; r < 4; ++r) o[g + e][r] = fmaf(o[g + e][r], alpha, sum[e][r]);
       }
     }
   }
+  const float total = quad16_reduce<false>(l);
+  const bool some = total > 0.f || total != total;
+  if (row >= ROWS) return;
+  if constexpr (S::SPLITS > 1u) {
+    const size_t place = ((size_t)split * S::B * S::HK + head) * S::TILES * 16u + row;
 #pragma unroll
-  for (int h = 0; h < HB; ++h) {
-    const float total = quad16_reduce<false>(l[h]);
-    const bool some = total > 0.f || total != total;
-    const float inv = some ? 1.f / total : 0.f;
-    const uint32_t row = mine + 16u * h + t;
-    if (row >= ROWS) continue;
-    if constexpr (S::SPLITS > 1u) {
-      const size_t place = ((size_t)split * S::B * S::HK + head) * S::TILES * 16u + row;
-#pragma unroll
-      for (int g = 0; g < G; ++g) window_store<S>(reinterpret_cast<float*>(ws + S::OUT) + place * S::DH, 16 * g + 4 * q, o[h][g]);
-      if (q == 0) reinterpret_cast<float2*>(ws + S::STATS)[place] = make_float2(m[h], total);
-      continue;
-    }
-    if (out != nullptr) {
-#pragma unroll
-      for (int g = 0; g < G; ++g) window_store<S>(out + line[h] * S::DH, 16 * g + 4 * q, o[h][g] * inv);
-    }
-    if (lse != nullptr && q == 0) lse[line[h]] = some ? (m[h] + __builtin_amdgcn_logf(total)) * 0.69314718055994531f : -TCMI_INF;
+    for (int g = 0; g < G; ++g) window_store<S>(reinterpret_cast<float*>(ws + S::OUT) + place * S::DH, 16 * g + 4 * q, o[g]);
+    if (q == 0) reinterpret_cast<float2*>(ws + S::STATS)[place] = make_float2(m, total);
+    return;
   }
+  const float inv = some ? 1.f / total : 0.f;
+  if (out != nullptr) {
+#pragma unroll
+    for (int g = 0; g < G; ++g) window_store<S>(out + line * S::DH, 16 * g + 4 * q, o[g] * inv);
+  }
+  if (lse != nullptr && q == 0) lse[line] = some ? (m + __builtin_amdgcn_logf(total)) * 0.69314718055994531f : -TCMI_INF;
 }
 
-// Dot products of this lane's rows with a tile's lines: acc[h][k] += lines 16k ... of `tile` by f[h].
-template <class T, int HB, int BLOCKS, int SLICES>
-__device__ __forceinline__ void window_dots(f4 (&acc)[HB][BLOCKS], const char* tile, const Parts (&f)[HB][SLICES]) {
-#pragma unroll
-  for (int k = 0; k < BLOCKS; ++k) {
-#pragma unroll
-    for (int h = 0; h < HB; ++h) acc[h][k] = f4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int d = 0; d < SLICES; ++d) {
-      Parts x;
-      T::lines(tile, 16 * k, d, x);
-#pragma unroll
-      for (int h = 0; h < HB; ++h) window_mfma(acc[h][k], x, f[h][d]);
-    }
-  }
-}
 // acc[h][g] += the sums over a tile's lines of its floats 16g ... times f[h].
 template <class T, int HB, int G, int PAIRS>
 __device__ __forceinline__ void window_sums(f4 (&acc)[HB][G], const char* tile, const Parts (&f)[HB][PAIRS]) {
@@ -474,12 +430,11 @@ __device__ __forceinline__ void window_wide_mass(const float* __restrict__ qp, c
   if ((threadIdx.x & 48u) == 0u && at < LINES) mass[at] = sum;
 }
 
-// The gradients: tiles of 32 lines, 16·HB lines a wavefront's own.
+// The gradients: tiles of 32 lines, 16 lines a wavefront's own.
 template <class S>
 struct WindowBack {
-  static constexpr int DP = (S::DH + 31) / 32 * 32, SLICES = DP / 32, G = DP / 16, NB = 32, BLOCKS = 2;
-  static constexpr int HB = S::HB;
-  static constexpr uint32_t ROWS = 64 * HB;
+  static constexpr int DP = (S::DH + 31) / 32 * 32, SLICES = DP / 32, G = DP / 16, NB = 32;
+  static constexpr uint32_t ROWS = 64;
   using T = WindowTile<S, NB>;
   static constexpr int LDS = 2 * T::BYTES + (2 + SLICES) * NB * 4;
 };
@@ -491,35 +446,26 @@ __device__ __forceinline__ void window_wide_dq(const WindowGradArgs a, float* __
   using T = typename W::T;
   using Span = WindowSpan<S>;
   constexpr uint32_t R = Span::R, ROWS = Span::ROWS;
-  constexpr int NB = W::NB, HB = W::HB, BLOCKS = W::BLOCKS, SLICES = W::SLICES, G = W::G;
+  constexpr int NB = W::NB, SLICES = W::SLICES, G = W::G;
   const uint32_t b = head / S::HK, hk = head % S::HK;
   const int lane = threadIdx.x & 63, t = lane & 15, q = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Span w(a.lengths, b);
   const Minus minus;
-  const uint32_t row0 = tile * W::ROWS, mine = row0 + 16u * HB * wave;
+  const uint32_t row0 = tile * W::ROWS, mine = row0 + 16u * wave, row = mine + t, own = min(row, ROWS - 1u);
   const WindowTiles keys = window_keys(w, min(row0, ROWS - 1u), min(row0 + W::ROWS - 1u, ROWS - 1u)), tiles = window_wider<NB>(keys);
   const float scale = static_cast<float>(S::scale() * 1.4426950408889634);
-  size_t line[HB];
-  int32_t pos[HB];
-  bool on[HB];
-  float lse[HB], mass[HB];
-  Parts qf[HB][SLICES], df[HB][SLICES];
-  f4 acc[HB][G];
+  const size_t line = ((size_t)b * S::T + own / R) * S::H + hk * R + own % R;
+  const int32_t pos = w.first + static_cast<int32_t>(own / R);
+  const bool on = row < ROWS && w.stands(pos);
+  Parts qf[SLICES], df[SLICES];
+  window_line<S>(qf, a.q + line * S::DH, on, scale, minus);
+  window_line<S>(df, a.dy + line * S::DH, on, 1.f, minus);
+  const float lse = on ? a.lse[line] * LOG2E : 0.f, mass = window_row_mass<S>(a.o + line * S::DH, a.dy + line * S::DH, on);
+  f4 acc[1][G];
 #pragma unroll
-  for (int h = 0; h < HB; ++h) {
-    const uint32_t row = mine + 16u * h + t, at = min(row, ROWS - 1u);
-    line[h] = ((size_t)b * S::T + at / R) * S::H + hk * R + at % R;
-    pos[h] = w.first + static_cast<int32_t>(at / R);
-    on[h] = row < ROWS && w.stands(pos[h]);
-    window_line<S>(qf[h], a.q + line[h] * S::DH, on[h], scale, minus);
-    window_line<S>(df[h], a.dy + line[h] * S::DH, on[h], 1.f, minus);
-    lse[h] = on[h] ? a.lse[line[h]] * LOG2E : 0.f;
-    mass[h] = window_row_mass<S>(a.o + line[h] * S::DH, a.dy + line[h] * S::DH, on[h]);
-#pragma unroll
-    for (int g = 0; g < G; ++g) acc[h][g] = f4{0.f, 0.f, 0.f, 0.f};
-  }
-  const bool full = mine + 16u * HB <= ROWS && w.stands(w.first + static_cast<int32_t>(mine / R)) && w.stands(w.first + static_cast<int32_t>((mine + 16u * HB - 1u) / R));
-  const int32_t p0 = w.first + static_cast<int32_t>(min(mine, ROWS - 1u) / R), p1 = w.first + static_cast<int32_t>(min(mine + 16u * HB - 1u, ROWS - 1u) / R);
+  for (int g = 0; g < G; ++g) acc[0][g] = f4{0.f, 0.f, 0.f, 0.f};
+  const bool full = mine + 16u <= ROWS && w.stands(w.first + static_cast<int32_t>(mine / R)) && w.stands(w.first + static_cast<int32_t>((mine + 15u) / R));
+  const int32_t p0 = w.first + static_cast<int32_t>(min(mine, ROWS - 1u) / R), p1 = w.first + static_cast<int32_t>(min(mine + 15u, ROWS - 1u) / R);
   const size_t step = (size_t)S::HK * S::DH, base = ((size_t)b * S::KEYS * S::HK + hk) * S::DH;
   T kt, vt;
   char *klds = lds, *vlds = lds + T::BYTES;
@@ -553,32 +499,26 @@ __device__ __forceinline__ void window_wide_dq(const WindowGradArgs a, float* __
     if (i + 1 < end) load(i + 1);
     if (j0 > p1 || (j0 + NB <= w.from(p0) && j0 >= static_cast<int32_t>(S::SINKS))) continue;
     const bool whole = full && j0 + NB - 1 <= p0 && (j0 >= w.from(p1) || j0 + NB <= static_cast<int32_t>(S::SINKS));
-    f4 s[HB][BLOCKS], dp[HB][BLOCKS];
+    f4 s[2], dp[2];
     window_dots<T>(s, klds, qf);
     window_dots<T>(dp, vlds, df);
-    Parts ds[HB][1];
 #pragma unroll
-    for (int h = 0; h < HB; ++h) {
+    for (int k = 0; k < 2; ++k) {
 #pragma unroll
-      for (int k = 0; k < BLOCKS; ++k) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float d = __builtin_amdgcn_exp2f(s[h][k][r] - lse[h]) * (dp[h][k][r] - mass[h]);
-          s[h][k][r] = whole || (on[h] && w.sees(pos[h], j0 + 16 * k + 4 * q + r)) ? d : 0.f;
-        }
+      for (int r = 0; r < 4; ++r) {
+        const float d = __builtin_amdgcn_exp2f(s[k][r] - lse) * (dp[k][r] - mass);
+        s[k][r] = whole || (on && w.sees(pos, j0 + 16 * k + 4 * q + r)) ? d : 0.f;
       }
-      window_parts(s[h][0], s[h][1], minus, ds[h][0]);
     }
+    Parts ds[1][1];
+    window_parts(s[0], s[1], minus, ds[0][0]);
     window_sums<T>(acc, klds, ds);
   }
+  if (row >= ROWS) return;
+  float* to = S::SPLITS > 1u ? parts + ((size_t)split * S::B * S::T * S::H + line) * S::DH : dq + line * S::DH;
+  const float by = S::SPLITS > 1u ? 1.f : static_cast<float>(S::scale());
 #pragma unroll
-  for (int h = 0; h < HB; ++h) {
-    if (mine + 16u * h + t >= ROWS) continue;
-    float* to = S::SPLITS > 1u ? parts + ((size_t)split * S::B * S::T * S::H + line[h]) * S::DH : dq + line[h] * S::DH;
-    const float by = S::SPLITS > 1u ? 1.f : static_cast<float>(S::scale());
-#pragma unroll
-    for (int g = 0; g < G; ++g) window_store<S>(to, 16 * g + 4 * q, acc[h][g] * by);
-  }
+  for (int g = 0; g < G; ++g) window_store<S>(to, 16 * g + 4 * q, acc[0][g] * by);
 }
 
 // The positions that see one of `keys` keys from `first` on: from the first key on, up to the last one's window or the sequence's
@@ -643,33 +583,27 @@ __device__ __forceinline__ void window_wide_dkv(const WindowGradArgs a, float* _
   using T = typename W::T;
   using Span = WindowSpan<S>;
   constexpr int32_t R = Span::R, ROWS = Span::ROWS;
-  constexpr int NB = W::NB, HB = W::HB, BLOCKS = W::BLOCKS, SLICES = W::SLICES, G = W::G;
+  constexpr int NB = W::NB, SLICES = W::SLICES, G = W::G;
   const uint32_t b = head / S::HK, hk = head % S::HK;
   const int lane = threadIdx.x & 63, t = lane & 15, q = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Span w(a.lengths, b);
   const Minus minus;
-  const int32_t j0 = tile * W::ROWS, mine = j0 + 16 * HB * wave;
+  const int32_t j0 = tile * W::ROWS, mine = j0 + 16 * wave, key = mine + t;
   const float scale = static_cast<float>(S::scale() * 1.4426950408889634);
-  int32_t key[HB];
-  size_t line[HB];
-  Parts kf[HB][SLICES], vf[HB][SLICES];
-  f4 dka[HB][G], dva[HB][G];
-  const WindowSeen<S> all(w, j0, W::ROWS), own(w, mine, 16 * HB);
+  Parts kf[SLICES], vf[SLICES];
+  f4 dka[1][G], dva[1][G];
+  const WindowSeen<S> all(w, j0, W::ROWS), own(w, mine, 16);
   if (chunk < all.start()) return;
   chunk -= all.start();
   if (chunk > 0u && chunk >= all.chunks()) return;
   const int32_t p0 = all.p0, p1 = all.p1, m0 = own.p0, m1 = own.p1;
   const int32_t begin = all.from(chunk), end = all.to(chunk);
+  const size_t line = ((size_t)b * S::KEYS + min(key, static_cast<int32_t>(S::KEYS) - 1)) * S::HK + hk;
+  const bool on = begin < end && key < w.length;
+  window_line<S>(kf, a.k + line * S::DH, on, scale, minus);
+  if constexpr (DK) window_line<S>(vf, a.v + line * S::DH, on, 1.f, minus);
 #pragma unroll
-  for (int h = 0; h < HB; ++h) {
-    key[h] = mine + 16 * h + t;
-    line[h] = ((size_t)b * S::KEYS + min(key[h], static_cast<int32_t>(S::KEYS) - 1)) * S::HK + hk;
-    const bool on = begin < end && key[h] < w.length;
-    window_line<S>(kf[h], a.k + line[h] * S::DH, on, scale, minus);
-    if constexpr (DK) window_line<S>(vf[h], a.v + line[h] * S::DH, on, 1.f, minus);
-#pragma unroll
-    for (int g = 0; g < G; ++g) dka[h][g] = dva[h][g] = f4{0.f, 0.f, 0.f, 0.f};
-  }
+  for (int g = 0; g < G; ++g) dka[0][g] = dva[0][g] = f4{0.f, 0.f, 0.f, 0.f};
   const size_t top = ((size_t)b * S::T) * S::H + hk * R;
   auto place = [&](int32_t r) { return top + (size_t)(r / R) * S::H + r % R; };
   T qt, dt, ot;
@@ -741,48 +675,41 @@ __device__ __forceinline__ void window_wide_dkv(const WindowGradArgs a, float* _
     if (i + 1 < end) load(i + 1);
     const int32_t r0 = i * NB, a0 = w.first + r0 / R, a1 = w.first + min(r0 + NB - 1, ROWS - 1) / R;
     if (m0 > m1 || a1 < m0 || a0 > m1) continue;
-    const bool whole = r0 + NB <= ROWS && a0 >= max(p0, mine + 16 * HB - 1) && a1 <= p1 && mine + 16 * HB <= w.length && (w.from(a1) <= mine || mine + 16 * HB <= static_cast<int32_t>(S::SINKS));
-    f4 s[HB][BLOCKS];
+    const bool whole = r0 + NB <= ROWS && a0 >= max(p0, mine + 15) && a1 <= p1 && mine + 16 <= w.length && (w.from(a1) <= mine || mine + 16 <= static_cast<int32_t>(S::SINKS));
+    f4 s[2];
     window_dots<T>(s, qlds, kf);
-    Parts f[HB][1];
+    Parts f[1][1];
 #pragma unroll
-    for (int k = 0; k < BLOCKS; ++k) {
+    for (int k = 0; k < 2; ++k) {
       // (NaN where the row's numbers are not finite.)
       f4 ls = *reinterpret_cast<const f4*>(row_lse + 16 * k + 4 * q);
       const f4 marks = mass(k);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) ls[r] = marks[r] == marks[r] ? ls[r] : marks[r];
       const int4 ps = *reinterpret_cast<const int4*>(row_pos + 16 * k + 4 * q);
       const int32_t pos[4] = {ps.x, ps.y, ps.z, ps.w};
 #pragma unroll
-      for (int h = 0; h < HB; ++h) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) s[h][k][r] = whole || (pos[r] >= 0 && w.sees(pos[r], key[h])) ? __builtin_amdgcn_exp2f(s[h][k][r] - ls[r]) : 0.f;
+      for (int r = 0; r < 4; ++r) {
+        ls[r] = marks[r] == marks[r] ? ls[r] : marks[r];
+        s[k][r] = whole || (pos[r] >= 0 && w.sees(pos[r], key)) ? __builtin_amdgcn_exp2f(s[k][r] - ls[r]) : 0.f;
       }
     }
     if constexpr (DV) {
-#pragma unroll
-      for (int h = 0; h < HB; ++h) window_parts(s[h][0], s[h][1], minus, f[h][0]);
+      window_parts(s[0], s[1], minus, f[0][0]);
       window_sums<T>(dva, dlds, f);
     }
     if constexpr (DK) {
-      f4 dp[HB][BLOCKS];
+      f4 dp[2];
       window_dots<T>(dp, dlds, vf);
 #pragma unroll
-      for (int k = 0; k < BLOCKS; ++k) {
+      for (int k = 0; k < 2; ++k) {
         const f4 ms = mass(k);
 #pragma unroll
-        for (int h = 0; h < HB; ++h) {
-#pragma unroll
-          for (int r = 0; r < 4; ++r) s[h][k][r] = whole || s[h][k][r] != 0.f ? s[h][k][r] * fmaf(ms[r], OWN ? -0x1p8f : -1.f, dp[h][k][r]) : 0.f;
-        }
+        for (int r = 0; r < 4; ++r) s[k][r] = whole || s[k][r] != 0.f ? s[k][r] * fmaf(ms[r], OWN ? -0x1p8f : -1.f, dp[k][r]) : 0.f;
       }
-#pragma unroll
-      for (int h = 0; h < HB; ++h) window_parts(s[h][0], s[h][1], minus, f[h][0]);
+      window_parts(s[0], s[1], minus, f[0][0]);
       window_sums<T>(dka, qlds, f);
     }
   }
-  window_key_sums<S, DK, DV>(dk, dv, ws, b, hk, chunk, key, dka, dva);
+  window_key_sums<S, DK, DV>(dk, dv, ws, b, hk, chunk, {key}, dka, dva);
 }
 
 // dq from its splits' sums: thread `at`, four floats.

@@ -20,7 +20,7 @@ function residualSizes(graph, node) {
   let lanes = 16;
   while (lanes * 16 < D) lanes *= 2;
   const threads = Math.max(256, lanes), units = ceil(D, lanes * 4);
-  return { z: { N, D, LANES: lanes, UNITS: units, THREADS: threads, LAYER: a.norm === 'layer', PRE: a.pre, POST: a.post, GATE: gated < 0 ? GATE.none : full ? GATE.full : GATE.vector },
+  return { z: { N, D, LANES: lanes, UNITS: units, THREADS: threads, LAYER: a.norm === 'layer', POST: a.post, GATE: gated < 0 ? GATE.none : full ? GATE.full : GATE.vector },
     names, grad };
 }
 

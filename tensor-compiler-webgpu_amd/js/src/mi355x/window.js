@@ -105,16 +105,15 @@ function keySplits(z, rows, NB, blocks) {
 
 function wideForward(s, parts, joined) {
   const { z } = s, e = entry(joined ? parts : null), heads = z.B * z.HK, R = z.H / z.HK;
-  const HB = blocksOf(packs(z), z.T * R, heads, ceil(z.WINDOW ? Math.min(z.KEYS, z.WINDOW) : z.KEYS, 64)), rows = 64 * HB, tiles = ceil(z.T * R, rows), SPLITS = keySplits(z, rows, z.DH <= 64 ? 64 : 32, tiles * heads);
-  const more = { TILES: ceil(z.T * R, 16), SPLITS, HB }, types = { HB: 'int' };
+  const packed = packs(z), HB = blocksOf(packed, z.T * R, heads, ceil(z.WINDOW ? Math.min(z.KEYS, z.WINDOW) : z.KEYS, 64)), rows = 64 * HB, tiles = ceil(z.T * R, rows), SPLITS = keySplits(z, rows, z.DH <= 64 ? 64 : 32, tiles * heads);
+  const more = { TILES: ceil(z.T * R, 16), SPLITS }, types = { HB: 'int', WAVES: 'int' };
   let at = 0;
   const place = (name, bytes) => { more[name] = at; types[name] = 'size_t'; at = align(at + bytes, 256); };
   place('OUT', SPLITS > 1 ? 4 * SPLITS * heads * more.TILES * 16 * z.DH : 0);
   place('STATS', SPLITS > 1 ? 8 * SPLITS * heads * more.TILES * 16 : 0);
-  const KP = align(z.KEYS, 64), packed = packs(z);
+  const KP = align(z.KEYS, 64);
   if (packed) {
-    more.WAVES = 4;
-    types.WAVES = 'int';
+    Object.assign(more, { WAVES: 4, HB });
     place('KSCALE', 4 * heads * KP);
     place('KDOTS', formBytes(z, KP, 2));
     place('VSUMS', formBytes(z, KP, 3));
@@ -187,21 +186,21 @@ function joinKernel(m, z, out, ws, more, heads) {
 function forwardKernels(s, parts, joined) {
   const { z } = s, e = entry(joined ? parts : null);
   if (z.T * (z.H / z.HK) > FEW_ROWS) return wideForward(s, parts, joined);
-  const R = z.H / z.HK, TILES = ceil(z.T * R, 16), heads = z.B * z.HK;
-  // The keys that one tile sees at most, in tiles of 16, dealt to as many workgroups as fill the chip four times, eight tiles each or more.
+  const R = z.H / z.HK, heads = z.B * z.HK;
+  // The keys that the rows see at most, in tiles of 16, dealt to as many workgroups as fill the chip four times, eight tiles each or more.
   // (32 tokens of 8 heads over 1028 keys: 16.8 us by nine tiles, 21.6 by five.)
   const most = ceil(z.WINDOW ? Math.min(z.KEYS, z.WINDOW + ceil(16, R) + 32 + z.SINKS) : z.KEYS, 16);
-  const SPLITS = Math.max(1, Math.min(256, Math.floor(most / 8), ceil(4 * CUS, TILES * heads)));
+  const SPLITS = Math.max(1, Math.min(256, Math.floor(most / 8), ceil(4 * CUS, heads)));
   const types = {};
   let at = 0;
-  const more = { TILES, SPLITS };
+  const more = { TILES: 1, SPLITS };
   const place = (name, bytes) => { more[name] = at; types[name] = 'size_t'; at = align(at + bytes, 256); };
-  place('OUT', SPLITS > 1 ? 4 * SPLITS * heads * TILES * 16 * z.DH : 0);
-  place('STATS', SPLITS > 1 ? 8 * SPLITS * heads * TILES * 16 : 0);
+  place('OUT', SPLITS > 1 ? 4 * SPLITS * heads * 16 * z.DH : 0);
+  place('STATS', SPLITS > 1 ? 8 * SPLITS * heads * 16 : 0);
   const m = maker(s, e, types);
   const out = (p) => (parts.includes(p) ? e.out(p) : 'nullptr');
   const L = s.lengths ? 'A.in[3]' : 'nullptr', ws = `reinterpret_cast<char*>(${e.ws})`;
-  const kernels = [m('win', grid(TILES * heads * SPLITS), 256, `float lds[tcmi::window_lds<${z.DH}>()]`,
+  const kernels = [m('win', grid(heads * SPLITS), 256, `float lds[tcmi::window_lds<${z.DH}>()]`,
     `window_rows<${S}>(A.in[0], A.in[1], A.in[2], ${L}, ${out('o')}, ${out('lse')}, ${ws}, lds, blockIdx.x)`, more)];
   if (SPLITS > 1) kernels.push(joinKernel(m, z, out, ws, more, heads));
   return { kernels, workspace: at };
@@ -214,7 +213,7 @@ function backwardKernels(s, parts, joined) {
   const L = s.lengths ? 'A.in[3]' : 'nullptr', first = s.lengths ? 4 : 3;
   const args = `{A.in[0], A.in[1], A.in[2], ${L}, A.in[${first}], A.in[${first + 1}], A.in[${first + 2}], ${e.ws}}`;
   const dq = parts.includes('dq'), dk = parts.includes('dk'), dv = parts.includes('dv');
-  const types = { HB: 'int' }, more = {};
+  const types = { HB: 'int', WAVES: 'int' }, more = {};
   // dy·o of every row, where the gradients of keys do not form it.
   const masses = z.DH > 128 && (dk || dv);
   let at = masses ? align(4 * z.B * z.T * z.H, 256) : 0;
@@ -224,7 +223,6 @@ function backwardKernels(s, parts, joined) {
   const add = (n) => ceil(z.DH % 4 ? n : n / 4, 256), KP = align(z.KEYS, 64), RP = align(z.T * R, 64), packed = packs(z), lanes = lanesOf(z.DH);
   const hold = z.DH <= 64;
   if (packed) {
-    types.WAVES = 'int';
     Object.assign(more, { WAVES: 4, HB: 1, SPLITS: 1 });
     place('KSCALE', 4 * heads * KP);
     place('VSCALE', 4 * heads * KP);
@@ -284,7 +282,7 @@ function backwardKernels(s, parts, joined) {
         : `window_wide_dq<${sizes}>(${args}, ${out('dq')}, ${sums(sizes)}, lds, ${where(block)})`) });
     if (SPLITS > 1) joins.push({ blocks: add(lines * z.DH), call: (sizes, block) => `window_wide_add<${sizes}>(${out('dq')}, ${sums(sizes)}, ${block} * 256u + threadIdx.x)` });
   }
-  for (const j of jobs.concat(joins)) j.more = Object.assign({}, more, { HB: j.HB || 1 });
+  for (const j of jobs.concat(joins)) j.more = Object.assign({}, more, packed ? { HB: j.HB || 1 } : {});
   kernels.push(m.jobs('winback', 64 * waves, jobs));
   if (joins.length) kernels.push(m.jobs('winadd', 256, joins));
   return { kernels, workspace: at };

@@ -31,3 +31,16 @@ def test_every_form_is_run(tool):
     found = set().union(*(kernels(tool, c) for c in cases))
     assert found >= {("window_rows", 1), ("window_wide", 1), ("window_wide_dq", 1), ("window_wide_dkv", 1), ("window_packed", 1), ("window_packed_dq", 1),
                      ("window_packed_dkv", 1)}
+
+
+def test_no_size_is_written_that_no_kernel_reads(tool):
+    """The constants of a launch's struct are read by its kernels; blocks of lines are a choice of split operands alone."""
+    import pathlib
+    headers = "".join(p.read_text() for p in (pathlib.Path(__file__).resolve().parents[1] / "tensor-compiler-webgpu_amd" / "csrc" / "kernels").glob("tcmi_*.h"))
+    cases = [g["case"] for g in tool("operator-graphs", {"context": True})]
+    unit = tool("kernel-unit", {"operators": cases}, timeout=120)["unit"]
+    structs = {m.group(1): m.group(2) for m in re.finditer(r"struct (\w+_s\d*) \{\n(.*?)\n\};", unit, re.S)}
+    names = {n for body in structs.values() for n in re.findall(r"constexpr \w+ (\w+) = ", body)}
+    assert not [n for n in names if not re.search(rf"::{n}\b", headers + unit)]
+    for entry, sizes in re.findall(r"tcmi::(window_(?:rows|wide(?:_dq|_dkv)?|packed(?:_dq|_dkv)?))<(\w+)", unit):
+        assert ("HB" in re.findall(r" (\w+) = ", structs[sizes])) == ("packed" in entry), (entry, sizes)
