@@ -521,5 +521,7 @@ class Program:
         return np.array(ins + [0] * (MAX_IN - len(ins)) + [self.buffers[member["node"]].at, ws], dtype=np.uint64).tobytes()
 
     def run(self):
+        """Issues the launches on the library's own stream, which torch's streams are not ordered with, and returns the buffers that they write:
+        their values are there after torch.cuda.synchronize() (or the library's sync), and inputs change after it too."""
         self.t.launch_dag(*self.call)
         return self.results
