@@ -127,7 +127,10 @@ struct ResidualLane {
 #pragma unroll
     for (int i = 0; i < F; ++i) s[0] = fmaf(v[i], v[i], s[0]);
     total(s);
-    const float r = __builtin_amdgcn_rsqf(s[0] * (1.f / S::D) + S::eps());
+    // (The instruction takes what is below the normal numbers as 0.)
+    const float square = s[0] * (1.f / S::D) + S::eps();
+    float r = __builtin_amdgcn_rsqf(square);
+    if (square < 0x1p-126f) r = __builtin_amdgcn_rsqf(square * 0x1p48f) * 0x1p24f;
 #pragma unroll
     for (int i = 0; i < F; ++i) v[i] *= r;
     return r;

@@ -293,6 +293,8 @@ const FORMS = [
   ].map(([name, q, k, options]) => window(`window-${name}${gradient ? '' : '-forward'}`, q, k, options, { gradient }))), []),
   embedding('embedding-order', [900], 40, 36, { scale: 3, gradient: true }),
   window('window-few-large', [2, 4, 6, 160], [2, 21, 2, 160], { window: 11, sinks: 2 }, { gradient: true }),
+  residual('residual-small-rms', [37, 64], ['gain'], { eps: 0 }, { gradient: true }),
+  residual('residual-small-layer', [37, 64], ['gain'], { eps: 0, norm: 'layer' }, { gradient: true }),
   // Two blocks of rows, and in the gradients of keys, a wavefront (window.js blocksOf): sizes that end inside their tiles, heads of whole tiles and not.
   window('window-blocks', [32, 151, 16, 20], [32, 151, 4, 20], { window: 130, sinks: 3 }, { lengths: true, gradient: true }),
   window('window-blocks-odd', [32, 69, 32, 37], [32, 139, 4, 37], {}, { lengths: true, gradient: true }),

@@ -1,5 +1,5 @@
 """windowAttention and its gradients on the GPU over float32's range, in every form (few rows, many, operands split once, one block of rows a
-wavefront and two): operands far from 1 whose results are not, and what counts as no number."""
+wavefront and two): operands far from 1 whose results are not, and what counts as no number; and residualNorm of rows whose squares are below the normal numbers."""
 import numpy as np
 import pytest
 
@@ -145,3 +145,33 @@ def test_numbers_below_the_largest(tool, tmp_path, form, operand):
             # The other values' sum is below half a step of the product.
             seen = x[w][:, dh // 2]
             assert np.isfinite(x).all() and (seen > 2.0 ** 90).all()
+
+
+@pytest.mark.parametrize("norm", ["rms", "layer"])
+def test_rows_of_small_numbers(tool, tmp_path, norm):
+    """Without an eps, rows of 2^-60 down to 2^-70, whose squares' mean is below the normal numbers from 2^-63 on: it is off by 2^-149 at most there (half a
+    step of each square, whose sum is exact, and of the mean), r by half of that relative to it."""
+    from oracle import operators
+    form = f"residual-small-{norm}"
+    D = tool("operator-graphs", {"forms": [form]})[0]["case"]["x"][-1]
+    rng = np.random.default_rng(11)
+    v = {k: rng.standard_normal((37, D) if k != "gain" else D).astype(np.float32) for k in ("x", "y", "gain", "d0", "d1")}
+    down = 2.0 ** -np.linspace(60, 70, 37).round()[:, None]
+    v["x"], v["y"] = (v["x"] * down).astype(np.float32), (v["y"] * down).astype(np.float32)
+    v["d0"] = np.ldexp(v["d0"], 60).astype(np.float32)
+    c, (got,) = run_form(tool, tmp_path, form, [v])
+    h = (v["x"] + v["y"]).astype(np.float64)
+    attrs = {"norm": norm, "eps": 0.0}
+    centred = h - h.mean(1, keepdims=True) if norm == "layer" else h
+    square = (centred ** 2).mean(1, keepdims=True)
+    assert (square < 2.0 ** -126).any() and (square > 2.0 ** -126).any()
+    off = 0.5 * 2.0 ** -149 / square + 2.0 ** -24 * (64 + 8)               # and float32's roundings: 64 terms, eight steps
+    r, hat = operators.normalised(attrs, h)
+    dn, g = v["d1"].astype(np.float64), v["d1"] * v["gain"].astype(np.float64)
+    m, gv = (g.mean(1, keepdims=True) if norm == "layer" else 0.0), (g * hat).mean(1, keepdims=True)
+    dx = r * (g - m - hat * gv) + v["d0"]
+    mass = r * (np.abs(g) + np.abs(g).mean(1, keepdims=True) + np.abs(hat) * np.abs(g * hat).mean(1, keepdims=True)) + np.abs(v["d0"])
+    np.testing.assert_array_equal(got["h"].reshape(h.shape), h.astype(np.float32))
+    for n, want, allowed in (("n", hat * v["gain"], 2 * off * (np.abs(hat) + (r * np.abs(h).max(1, keepdims=True) if norm == "layer" else 0)) * np.abs(v["gain"])),
+                             ("dx", dx, 8 * off * mass), ("dgain", (dn * hat).sum(0), 2 * (off * np.abs(dn) * (np.abs(hat) + 4)).sum(0))):
+        assert (np.abs(got[n].reshape(want.shape) - want) <= allowed).all(), (n, np.abs(got[n].reshape(want.shape) - want).max(), allowed.min())
