@@ -6,7 +6,8 @@
 //   dS_j = P_j·(dy·v_j - dy·o),  dq = scale·sum_j dS_j k_j,  dk_j = scale·sum dS_j q,  dv_j = sum P_j dy (over the queries that see j).
 // A query that sees nothing has o = 0, lse = -inf and no gradients. A key whose key or value holds a number that is not finite makes
 // NaN of o and lse of the queries that see it, and a query's row with one (dy's too) of the gradients of the keys it sees; what does not
-// see them, or is not seen, is as without them: 0 times them is taken as 0 (they are read as 0 where a sum runs over them).
+// see them, or is not seen, is as without them: 0 times them is taken as 0 (they are read as 0 where a sum runs over them). (What bf16 rounds to
+// infinity counts as that wherever operands are split into parts, tcmi_window_wide.h: everywhere but in the forward pass here.)
 //
 // Rows: the queries of the R = H/HK heads that share a key head, query t's heads side by side. Here up to 16 of them, single tokens over a cache,
 // on the fp32 matrix cores; more are tcmi_window_wide.h's, and all gradients. Keys 16 a

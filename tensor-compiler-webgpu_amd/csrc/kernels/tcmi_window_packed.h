@@ -18,8 +18,10 @@
 //
 // Bound: the matrix cores. A library's bf16 product of 8192 x 8192 x 8192 reaches 1310 TFLOP/s here, which is 291 of these forward products (three of halves and
 // six of bf16 for two), and 218 of the gradients' (30 for five, as scores and dy·v are formed for queries and for keys).
-//   two sequences of 16384 tokens, 16 heads of 128 by 4, a window of 1024    1090 us (253 TFLOP/s), 48 to split keys and values
-//   8192 tokens, 8 heads of 64 by 2: 310 us (221 TFLOP/s) and 9 to join two splits; its gradients 830 (207) and 28 to split, 21 to join
+//   two sequences of 16384 tokens, 16 heads of 128 by 4, a window of 1024    1085 us (254 TFLOP/s), 49 to split keys and values
+//   8192 tokens, 8 heads of 64 by 2: 267 us (257 TFLOP/s) and 9 to join two splits; its gradients 911 (189) and 27 to split, 21 to join
+// (Medians of 60 passes; the first ten or twenty after the card was idle take up to a third longer.) Plain heads of 128 without a window keep 10 registers in
+// memory, one operand of four of them read again a tile: 8 sequences of 1024 tokens, 8 heads 141 us (58 at the rate above).
 // Of the cycles the matrix cores are busy in 49 %: the rest are the softmax, the split of P and dS into parts and the barriers, which two wavefronts a
 // SIMD do not hide whole. Taking the next tile's scores beside this one's softmax needs their registers twice: 313 us of 320 at heads of 64, and spilled at 128.
 
@@ -413,7 +415,7 @@ __device__ __forceinline__ void window_packed(const float* __restrict__ qp, cons
     if (i + 1 < end) keys(i + 1);
     if (some) {
       if (!rows.whole(w, j0, NB) || qs.some()) {
-        // (The rows' positions are found again here: kept, they spill other registers.)
+        // (The rows' positions are found again here: kept, they spill more registers.)
         int own = lane;
         asm volatile("" : "+v"(own));
 #pragma unroll
@@ -456,7 +458,7 @@ __device__ __forceinline__ void window_packed(const float* __restrict__ qp, cons
 #pragma unroll
         for (int k = 0; k < BLOCKS; k += 2) window_parts(s[h][k], s[h][k + 1], minus, pf[h][k / 2]);
       }
-      // (The places of heads above 64 are found again for each tile: kept, they spill other registers, whose reloads wait for the copies.)
+      // (The places of heads above 64 are found again for each tile: kept, they spill more registers, whose reloads wait for the copies.)
       int own = lane;
       if constexpr (G > 4) asm volatile("" : "+v"(own));
       __builtin_amdgcn_s_setprio(1);

@@ -243,7 +243,7 @@ function backwardKernels(s, parts, joined) {
   if (packed) more.WAVES = waves;
   const keyBlocks = blocksOf(hold && packed, z.KEYS, heads, ceil(Math.min(z.T, z.WINDOW || z.T) * R, 32)), rowBlocks = blocksOf(hold && packed, z.T * R, heads, ceil(z.WINDOW ? Math.min(z.KEYS, z.WINDOW) : z.KEYS, 64));
   const keyRows = 16 * waves * keyBlocks, rows = 16 * waves * rowBlocks;
-  // (Of heads above 64 a workgroup a CU, by its registers.)
+  // (Of heads above 64 a workgroup a CU, by its registers, and where operands are split once by LDS too.)
   const { CHUNK, SPLITS } = deal(z, heads, (hold ? 2 : 1) * CUS, keyRows, rows);
   const place4 = (name, floats) => place(name, 4 * floats);
   if (dk || dv) {
