@@ -292,6 +292,7 @@ const FORMS = [
     ['packed', [1, 300, 4, 64], [1, 300, 2, 64], { window: 260, sinks: 5 }], ['packed-odd', [1, 280, 4, 40], [1, 280, 2, 40], {}],
   ].map(([name, q, k, options]) => window(`window-${name}${gradient ? '' : '-forward'}`, q, k, options, { gradient }))), []),
   embedding('embedding-order', [900], 40, 36, { scale: 3, gradient: true }),
+  window('window-few-splits', [2, 1, 4, 64], [2, 2000, 2, 64], { sinks: 2, window: 1900 }, { gradient: true }),
   window('window-few-large', [2, 4, 6, 160], [2, 21, 2, 160], { window: 11, sinks: 2 }, { gradient: true }),
   residual('residual-small-rms', [37, 64], ['gain'], { eps: 0 }, { gradient: true }),
   residual('residual-small-layer', [37, 64], ['gain'], { eps: 0, norm: 'layer' }, { gradient: true }),

@@ -64,7 +64,7 @@ def touched(c, v, keys, queries, cotangents):
     return {"o": row.transpose(0, 2, 1), "dq": back.transpose(0, 2, 1), "dk": at.transpose(0, 2, 1), "dv": at.transpose(0, 2, 1)}
 
 
-NUMBERS = ["few", "few-whole", "few-large", "more", "wide", "wide-large", "packed", "packed-odd", "exact-packed-blocks"]
+NUMBERS = ["few", "few-whole", "few-splits", "few-large", "more", "wide", "wide-large", "packed", "packed-odd", "exact-packed-blocks"]
 
 
 def check_touched(tool, directory, form, v, bad, keys=(), queries=(), cotangents=()):
